@@ -317,8 +317,8 @@ def _adamw(st):
     c = (c + _up(y, c2 * c2, d2 * d2, uv).float()).clamp_max(255)
     c = torch.where((y > 0) & (c < 1), torch.ones_like(c), c)
     st["v"].copy_(c.to(torch.uint8).view(-1))
-    st["m_scale"].copy_(torch.where(sm > least, sm, zero))
-    st["v_scale"].copy_(torch.where(sv > least, sv, zero))
+    st["m_scale"].copy_(torch.where(sm < least, zero, sm))
+    st["v_scale"].copy_(torch.where(sv < least, zero, sv))
     m, v = _values(st["m"], st["m_scale"], st["v"], st["v_scale"])
     return {"p": st["p"], "m": m, "v": v}
 
