@@ -122,6 +122,42 @@ void check_metric(int metric) {
                 FDB_ERR_INVALID_ARG, "unknown metric");
 }
 
+void check_aligned(const void* p, size_t a, const char* what) {
+    FDB_REQUIRE(reinterpret_cast<uintptr_t>(p) % a == 0, FDB_ERR_INVALID_ARG,
+                std::string(what) + " is not aligned");
+}
+// What forward and backward share: the operands and the filter.
+template <class A>
+static void check_softmax(const A& a) {
+    FDB_REQUIRE(a.dtype == FDB_DTYPE_F32 || a.dtype == FDB_DTYPE_F16 || a.dtype == FDB_DTYPE_BF16,
+                FDB_ERR_INVALID_ARG, "unknown dtype");
+    FDB_REQUIRE(a.n > 0, FDB_ERR_EMPTY_VECTOR_SET, "no rows");
+    FDB_REQUIRE(a.n < (1ull << 31) - 512 && a.nq < (1ull << 31) - 512, FDB_ERR_INVALID_ARG,
+                "too many queries or rows");
+    FDB_REQUIRE(a.dim >= 1 && a.dim <= FDB_MAX_SOFTMAX_DIM, FDB_ERR_INVALID_ARG,
+                "dim must be in [1, FDB_MAX_SOFTMAX_DIM]");
+    FDB_REQUIRE(a.scale > 0.0f && a.scale <= 3.0e38f, FDB_ERR_INVALID_ARG,
+                "scale must be positive and finite");
+    FDB_REQUIRE(a.ld_queries >= a.dim && a.ld_rows >= a.dim, FDB_ERR_DIM_MISMATCH,
+                "rows overlap: ld is below dim");
+    FDB_REQUIRE(a.ld_queries < (1ull << 31) && a.ld_rows < (1ull << 31), FDB_ERR_INVALID_ARG,
+                "ld is too large");
+    FDB_REQUIRE(!a.allowed || a.ld_allowed == 0 || a.ld_allowed >= (a.n + 31) / 32,
+                FDB_ERR_DIM_MISMATCH, "ld_allowed is below (n + 31) / 32 words");
+}
+template <class A>
+static void check_softmax_buffers(const A& a, size_t need) {
+    FDB_REQUIRE(a.queries && a.rows, FDB_ERR_INVALID_ARG, "NULL argument");
+    const size_t es = a.dtype == FDB_DTYPE_F32 ? 4 : 2;
+    check_aligned(a.queries, es, "queries");
+    check_aligned(a.rows, es, "rows");
+    check_aligned(a.targets, 8, "targets");
+    check_aligned(a.allowed, 4, "allowed");
+    FDB_REQUIRE(a.workspace && a.workspace_bytes >= need, FDB_ERR_INVALID_ARG,
+                "the workspace is too small: " + std::to_string(need) + " bytes are needed");
+    check_aligned(a.workspace, 256, "the workspace");
+}
+
 // Pinned-or-not host <-> device staging for the host-buffer entry points.
 struct Staged {
     DevBuf<uint64_t> ids;
@@ -1146,6 +1182,249 @@ int fdb_bf_remove(fdb_bf* h, uint64_t id, int* removed) {
         h->sharded = false;
         h->shard_world = 1;
         h->dirty = true;
+    });
+}
+
+// ---------------------------------------------------------------------------
+// softmax over rows
+// ---------------------------------------------------------------------------
+int fdb_logprobs_workspace(fdb_ctx* ctx, const fdb_logprob_args* args, size_t* bytes) {
+    return guarded([&] {
+        FDB_REQUIRE(ctx && args && bytes, FDB_ERR_INVALID_ARG, "NULL argument");
+        check_softmax(*args);
+        FDB_REQUIRE(args->k <= FDB_MAX_ALTERNATIVES, FDB_ERR_INVALID_ARG,
+                    "k must not exceed FDB_MAX_ALTERNATIVES");
+        *bytes = args->nq ? sr::forward_bytes(ctx->c, *args) : 0;
+    });
+}
+
+int fdb_logprobs(fdb_ctx* ctx, const fdb_logprob_args* args) {
+    return guarded([&] {
+        FDB_REQUIRE(ctx && args, FDB_ERR_INVALID_ARG, "NULL argument");
+        const fdb_logprob_args& a = *args;
+        check_softmax(a);
+        FDB_REQUIRE(a.k <= FDB_MAX_ALTERNATIVES, FDB_ERR_INVALID_ARG,
+                    "k must not exceed FDB_MAX_ALTERNATIVES");
+        if (a.nq == 0) return;
+        FDB_REQUIRE(a.k == 0 || (a.top_ids && a.top_logprobs), FDB_ERR_INVALID_ARG,
+                    "k > 0 needs top_ids and top_logprobs");
+        check_softmax_buffers(a, sr::forward_bytes(ctx->c, a));
+        for (const void* p : {(const void*)a.logprob, (const void*)a.lse, (const void*)a.entropy,
+                              (const void*)a.top_logprobs})
+            check_aligned(p, 4, "an output");
+        check_aligned(a.top_ids, 8, "top_ids");
+        DeviceGuard g(ctx->c.device);
+        sr::forward_run(ctx->c, a);
+    });
+}
+
+int fdb_logprobs_backward_workspace(fdb_ctx* ctx, const fdb_logprob_grad_args* args,
+                                    size_t* bytes) {
+    return guarded([&] {
+        FDB_REQUIRE(ctx && args && bytes, FDB_ERR_INVALID_ARG, "NULL argument");
+        check_softmax(*args);
+        *bytes = args->nq ? sr::backward_bytes(ctx->c, *args) : 256;
+    });
+}
+
+int fdb_logprobs_backward(fdb_ctx* ctx, const fdb_logprob_grad_args* args) {
+    return guarded([&] {
+        FDB_REQUIRE(ctx && args, FDB_ERR_INVALID_ARG, "NULL argument");
+        const fdb_logprob_grad_args& a = *args;
+        check_softmax(a);
+        const size_t es = a.dtype == FDB_DTYPE_F32 ? 4 : 2;
+        FDB_REQUIRE(!a.d_queries || a.ld_d_queries >= a.dim, FDB_ERR_DIM_MISMATCH,
+                    "d_queries rows overlap");
+        FDB_REQUIRE(!a.d_rows || a.ld_d_rows >= a.dim, FDB_ERR_DIM_MISMATCH,
+                    "d_rows rows overlap");
+        check_aligned(a.d_queries, es, "d_queries");
+        check_aligned(a.d_rows, es, "d_rows");
+        DeviceGuard g(ctx->c.device);
+        if (a.nq == 0) {  // no query: the rows' gradient is zero
+            if (a.d_rows)
+                FDB_CUDA(cudaMemset2DAsync(a.d_rows, a.ld_d_rows * es, 0, a.dim * es, a.n,
+                                           static_cast<cudaStream_t>(a.stream)));
+            return;
+        }
+        FDB_REQUIRE(a.lse, FDB_ERR_INVALID_ARG, "lse is NULL");
+        FDB_REQUIRE(!a.d_entropy || a.entropy, FDB_ERR_INVALID_ARG,
+                    "d_entropy needs the entropy");
+        for (const float* p : {a.lse, a.entropy, a.d_logprob, a.d_lse, a.d_entropy})
+            check_aligned(p, 4, "an input");
+        check_softmax_buffers(a, sr::backward_bytes(ctx->c, a));
+        if (!a.d_queries && !a.d_rows) return;
+        sr::backward_run(ctx->c, a);
+    });
+}
+
+int fdb_logprobs_status(fdb_ctx* ctx, const void* workspace, void* stream) {
+    return guarded([&] {
+        FDB_REQUIRE(ctx && workspace, FDB_ERR_INVALID_ARG, "NULL argument");
+        DeviceGuard g(ctx->c.device);
+        int err = 0;
+        const cudaStream_t s = static_cast<cudaStream_t>(stream);
+        FDB_CUDA(cudaMemcpyAsync(&err, workspace, 4, cudaMemcpyDeviceToHost, s));
+        FDB_CUDA(cudaStreamSynchronize(s));
+        FDB_REQUIRE(err == 0, FDB_ERR_TIMEOUT, "a wait inside the kernels ran out");
+    });
+}
+
+int fdb_bf_logprobs(fdb_bf* h, const float* queries, size_t nq, float temperature,
+                    const uint64_t* target_ids, size_t k, float* logprob, float* lse,
+                    float* entropy, uint64_t* top_ids, float* top_logprobs) {
+    return guarded([&] {
+        FDB_REQUIRE(h && (nq == 0 || queries), FDB_ERR_INVALID_ARG, "NULL argument");
+        FDB_REQUIRE(temperature > 0.0f && 1.0f / temperature <= 3.0e38f &&
+                        1.0f / temperature > 0.0f,
+                    FDB_ERR_INVALID_ARG, "the temperature must be positive and finite");
+        FDB_REQUIRE(k <= FDB_MAX_ALTERNATIVES, FDB_ERR_INVALID_ARG,
+                    "k must not exceed FDB_MAX_ALTERNATIVES");
+        FDB_REQUIRE(k == 0 || nq == 0 || (top_ids && top_logprobs), FDB_ERR_INVALID_ARG,
+                    "k > 0 needs top_ids and top_logprobs");
+        FDB_REQUIRE(h->metric == FDB_METRIC_DOT_PRODUCT, FDB_ERR_UNSUPPORTED,
+                    "log probabilities need the dot-product metric");
+        DeviceGuard g(h->ctx->c.device);
+        std::lock_guard<std::mutex> lk(h->mu);
+        FDB_REQUIRE(!h->sharded, FDB_ERR_UNSUPPORTED, "the index is sharded");
+        FDB_REQUIRE(!h->h_ids.empty(), FDB_ERR_EMPTY_VECTOR_SET, "the index is empty");
+        if (nq == 0) return;
+        Ctx& c = h->ctx->c;
+        const cudaStream_t s = c.stream;
+        bf_upload(h);
+        h->s_q.ensure(nq * h->dim);
+        FDB_CUDA(cudaMemcpyAsync(h->s_q.p, queries, nq * h->dim * 4, cudaMemcpyHostToDevice, s));
+        std::vector<int64_t> targets;
+        if (target_ids) {
+            std::vector<uint64_t> want(target_ids, target_ids + nq);
+            std::sort(want.begin(), want.end());
+            want.erase(std::unique(want.begin(), want.end()), want.end());
+            const size_t w = want.size();
+            h->s_lp_want.ensure(2 * w);
+            uint64_t* slot = h->s_lp_want.p + w;
+            FDB_CUDA(cudaMemcpyAsync(h->s_lp_want.p, want.data(), w * 8, cudaMemcpyHostToDevice, s));
+            FDB_CUDA(cudaMemsetAsync(slot, 0xff, w * 8, s));
+            sr::launch_find_rows(s, h->ids.p, h->n, h->s_lp_want.p, w,
+                                 reinterpret_cast<unsigned long long*>(slot));
+            std::vector<int64_t> rows(w);
+            FDB_CUDA(cudaMemcpyAsync(rows.data(), slot, w * 8, cudaMemcpyDeviceToHost, s));
+            FDB_CUDA(cudaStreamSynchronize(s));
+            targets.resize(nq);
+            for (size_t i = 0; i < nq; ++i)  // (not found: -1, no target)
+                targets[i] = rows[std::lower_bound(want.begin(), want.end(), target_ids[i]) -
+                                  want.begin()];
+            h->s_lp_targets.ensure(nq);
+            FDB_CUDA(cudaMemcpyAsync(h->s_lp_targets.p, targets.data(), nq * 8,
+                                     cudaMemcpyHostToDevice, s));
+        }
+        h->s_lp_out.ensure(nq * (3 + k));
+        if (k) h->s_lp_ids.ensure(nq * k);
+        fdb_logprob_args a{};
+        a.dtype = FDB_DTYPE_F32;
+        a.queries = h->s_q.p, a.nq = nq, a.ld_queries = h->dim;
+        a.rows = h->x.p, a.n = h->n, a.ld_rows = h->dim;
+        a.dim = h->dim;
+        a.scale = 1.0f / temperature;
+        a.targets = target_ids ? h->s_lp_targets.p : nullptr;
+        a.k = k;
+        a.logprob = h->s_lp_out.p, a.lse = a.logprob + nq, a.entropy = a.lse + nq;
+        a.top_logprobs = a.entropy + nq;
+        a.top_ids = h->s_lp_ids.p;
+        check_softmax(a);
+        const size_t need = sr::forward_bytes(c, a);
+        h->s_lp_ws.ensure(need);
+        a.workspace = h->s_lp_ws.p, a.workspace_bytes = need;
+        a.stream = s;
+        // (a small batch's kernels have no waits and leave the word alone)
+        FDB_CUDA(cudaMemsetAsync(a.workspace, 0, 4, s));
+        sr::forward_run(c, a);
+        int err = 0;
+        std::vector<int64_t> rows(nq * k);
+        FDB_CUDA(cudaMemcpyAsync(&err, a.workspace, 4, cudaMemcpyDeviceToHost, s));
+        auto out = [&](float* to, const float* from, size_t count) {
+            if (to) FDB_CUDA(cudaMemcpyAsync(to, from, count * 4, cudaMemcpyDeviceToHost, s));
+        };
+        out(logprob, a.logprob, nq);
+        out(lse, a.lse, nq);
+        out(entropy, a.entropy, nq);
+        if (k) {
+            out(top_logprobs, a.top_logprobs, nq * k);
+            FDB_CUDA(cudaMemcpyAsync(rows.data(), a.top_ids, nq * k * 8, cudaMemcpyDeviceToHost,
+                                     s));
+        }
+        FDB_CUDA(cudaStreamSynchronize(s));
+        FDB_REQUIRE(err == 0, FDB_ERR_TIMEOUT, "a wait inside the kernels ran out");
+        for (size_t i = 0; i < nq * k; ++i)
+            top_ids[i] = rows[i] < 0 ? UINT64_MAX : h->h_ids[(size_t)rows[i]];
+    });
+}
+
+// ---------------------------------------------------------------------------
+// AdamW
+// ---------------------------------------------------------------------------
+int fdb_adamw_step(fdb_ctx* ctx, const fdb_adamw_tensor* tensors, size_t count,
+                   const fdb_adamw_opts* opts) {
+    return guarded([&] {
+        FDB_REQUIRE(ctx && opts && (count == 0 || tensors), FDB_ERR_INVALID_ARG, "NULL argument");
+        const fdb_adamw_opts& o = *opts;
+        for (int t : {o.param_dtype, o.grad_dtype})
+            FDB_REQUIRE(t == FDB_DTYPE_F32 || t == FDB_DTYPE_F16 || t == FDB_DTYPE_BF16,
+                        FDB_ERR_INVALID_ARG, "unknown dtype");
+        FDB_REQUIRE(o.state_bits == 32 || o.state_bits == 8, FDB_ERR_INVALID_ARG,
+                    "state_bits must be 32 or 8");
+        FDB_REQUIRE(o.beta1 >= 0.0 && o.beta1 < 1.0 && o.beta2 >= 0.0 && o.beta2 < 1.0,
+                    FDB_ERR_INVALID_ARG, "beta1 and beta2 must be in [0, 1)");
+        FDB_REQUIRE(o.eps > 0.0 && (float)o.eps > 0.0f && o.eps <= 1e30, FDB_ERR_INVALID_ARG,
+                    "eps must be positive");
+        FDB_REQUIRE(o.d_step || o.step >= 1, FDB_ERR_INVALID_ARG, "step counts from 1");
+        FDB_REQUIRE(std::isfinite(o.lr) && std::isfinite(o.weight_decay) &&
+                        std::isfinite(o.grad_scale),
+                    FDB_ERR_INVALID_ARG, "lr, weight_decay and grad_scale must be finite");
+        FDB_REQUIRE(count < (1ull << 31), FDB_ERR_INVALID_ARG, "too many tensors");
+        check_aligned(o.d_lr, 4, "d_lr");
+        check_aligned(o.d_step, 8, "d_step");
+        check_aligned(o.d_grad_scale, 4, "d_grad_scale");
+        const size_t ps = o.param_dtype == FDB_DTYPE_F32 ? 4 : 2;
+        const size_t gs = o.grad_dtype == FDB_DTYPE_F32 ? 4 : 2;
+        const size_t ss = o.state_bits == 8 ? 1 : 4;
+        std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+        spans.reserve(count);
+        for (size_t i = 0; i < count; ++i) {
+            const fdb_adamw_tensor& t = tensors[i];
+            if (t.n == 0) continue;
+            FDB_REQUIRE(t.param && t.grad && t.m && t.v &&
+                            (o.state_bits == 32 || (t.m_scale && t.v_scale)),
+                        FDB_ERR_INVALID_ARG, "NULL tensor");
+            FDB_REQUIRE(t.n < (1ull << 43), FDB_ERR_INVALID_ARG, "a tensor is too large");
+            check_aligned(t.param, ps, "a param");
+            check_aligned(t.grad, gs, "a gradient");
+            check_aligned(t.m, ss, "m");
+            check_aligned(t.v, ss, "v");
+            check_aligned(t.m_scale, 4, "m_scale");
+            check_aligned(t.v_scale, 4, "v_scale");
+            const uintptr_t b = reinterpret_cast<uintptr_t>(t.param);
+            spans.emplace_back(b, b + t.n * ps);
+        }
+        std::sort(spans.begin(), spans.end());
+        for (size_t i = 1; i < spans.size(); ++i)
+            FDB_REQUIRE(spans[i - 1].second <= spans[i].first, FDB_ERR_INVALID_ARG,
+                        "two tensors' params overlap");
+        DeviceGuard g(ctx->c.device);
+        adamw::step(static_cast<cudaStream_t>(o.stream), tensors, count, o);
+    });
+}
+
+int fdb_adamw_state_values(fdb_ctx* ctx, const int8_t* m, const float* m_scale, const uint8_t* v,
+                           const float* v_scale, size_t n, float* m_out, float* v_out,
+                           void* stream) {
+    return guarded([&] {
+        FDB_REQUIRE(ctx && (n == 0 || (m && m_scale && v && v_scale && m_out && v_out)),
+                    FDB_ERR_INVALID_ARG, "NULL argument");
+        for (const void* p : {(const void*)m_scale, (const void*)v_scale, (const void*)m_out,
+                              (const void*)v_out})
+            check_aligned(p, 4, "an argument");
+        DeviceGuard g(ctx->c.device);
+        adamw::values(static_cast<cudaStream_t>(stream), ctx->c.sm_count, m, m_scale, v, v_scale,
+                      n, m_out, v_out);
     });
 }
 

@@ -496,6 +496,22 @@ struct ScanParams;
 void ivf_tc_rescan(fdb_ivfpq* h, const ScanParams& base, size_t nq, size_t k, int order,
                    uint64_t* out_keys);
 void bf_upload(fdb_bf* h);
+// softmax_rows.cu: log probabilities under a softmax over rows, their gradient
+namespace sr {
+size_t forward_bytes(const Ctx& c, const fdb_logprob_args& a);
+void forward_run(Ctx& c, const fdb_logprob_args& a);
+size_t backward_bytes(const Ctx& c, const fdb_logprob_grad_args& a);
+void backward_run(Ctx& c, const fdb_logprob_grad_args& a);
+// slot[i] (preset to -1): the first row whose id is sorted[i]
+void launch_find_rows(cudaStream_t s, const uint64_t* ids, size_t n, const uint64_t* sorted,
+                      size_t count, unsigned long long* slot);
+}  // namespace sr
+// adamw.cu
+namespace adamw {
+void step(cudaStream_t s, const fdb_adamw_tensor* ts, size_t count, const fdb_adamw_opts& o);
+void values(cudaStream_t s, int sms, const int8_t* m, const float* ms, const uint8_t* v,
+            const float* vs, size_t n, float* om, float* ov);
+}  // namespace adamw
 void bf_shard(fdb_bf* h, int rank, int world);
 void bf_search_dev(fdb_bf* h, const float* dQ, size_t nq, size_t k, uint64_t* d_ids,
                    float* d_dists, uint32_t* d_counts, fdb_stats* st);
@@ -655,6 +671,10 @@ struct fdb_bf {
     fdb::GemmScratch gemm;
     fdb::DevBuf<uint64_t> s_part, s_keys, s_ids, s_gather, s_merged, s_merged_ids, s_out_ids;
     fdb::DevBuf<float> s_dists;
+    fdb::DevBuf<uint8_t> s_lp_ws;       // fdb_bf_logprobs: workspace, outputs, wanted ids
+    fdb::DevBuf<float> s_lp_out;
+    fdb::DevBuf<int64_t> s_lp_ids, s_lp_targets;
+    fdb::DevBuf<uint64_t> s_lp_want;
     fdb::DevBuf<uint32_t> s_counts, s_flags;
     fdb::DevBuf<uint64_t> s_cal_ids;    // pass-1 quota calibration outputs
     fdb::DevBuf<float> s_cal_d;

@@ -1,0 +1,1943 @@
+// softmax_rows.cu -- log probabilities under a softmax over index rows, and
+// their gradient, without ever holding the nq x n scores.
+//
+//   s_ij = scale * q_i . x_j         over the rows j that query i may see
+//   lse_i = log sum_j exp(s_ij),  p_ij = exp(s_ij - lse_i)
+//   H_i = lse_i - sum_j p_ij s_ij,  logprob_i = s_i,t(i) - lse_i
+//
+// Forward: the scores are formed tile by tile on the tensor cores (or, for a
+// few f32 queries, on the FMA pipes) and every thread folds its columns into
+// a running (max m, sum l = sum 2^(t - m), a = sum 2^(t - m) (t - m)) of its
+// query row, t = s log2(e); the partial triples are joined by
+// finish_kernel:  lse = ln2 (M + log2 L),  H = ln2 (log2 L - A / L).
+// For the top alternatives each group of 32 rows leaves its largest score,
+// the pair of rows that holds it (in the low 4 bits) and its second largest;
+// the best k + 8 groups are picked per query, their marked rows are scored
+// again exactly (64-bit sums), and a group whose second largest could still
+// enter is scored in full, as are all groups if one that was not picked could.
+// Which ids are returned therefore does not depend on the order of a 32-bit
+// sum; equal scores go to the lower id.
+//
+// Types: 16-bit rows go to the MMA as they are.  f32 rows are split once into
+// two fp16 parts of the row scaled by a power of two, x 2^e = hi + lo
+// (22 bits, the row's largest element at 2^14), and a score is the sum of
+// three products lo.hi + hi.lo + hi.hi, the small ones first: the tensor
+// core's accumulation cuts bits off the running sum, so its size should be
+// small for as long as possible.  lo.lo (2^-22 of the score) is left out.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+
+#include "fdb_internal.h"
+#include "tc_ptx.cuh"
+
+namespace fdb {
+namespace sr {
+
+using namespace tc;
+
+constexpr int BM = 128;                     // rows of an output tile
+constexpr int OPER = BM * 128;              // bytes of 128 rows of a 64-wide K step
+// 16-bit operands: 256 columns an accumulator, four K steps of 48 KB in
+// flight.  Two parts (f32): 128 columns, three K steps of 64 KB (both parts of
+// both operands).
+__host__ __device__ constexpr int bn_of(bool two) { return two ? 128 : 256; }
+__host__ __device__ constexpr int stages_of(bool two) { return two ? 3 : 4; }
+__host__ __device__ constexpr int stage_bytes(bool two) { return two ? 4 * OPER : 3 * OPER; }
+__host__ __device__ constexpr int accs_of(bool two) { return two ? 4 : 2; }
+constexpr int MAX_STG = 4, MAX_ACC = 4;
+constexpr int MAX_BN = 256;
+constexpr int THREADS = 640;                // 2 issuing warps, 2 idle, 16 epilogue warps
+constexpr int EPI_WARP0 = 4, EPI_WARPS = 16;
+constexpr int GROUP = 32;                   // rows whose largest scores are kept together
+constexpr int PAD = 8;                      // groups picked beyond k
+constexpr int MAX_SEL = FDB_MAX_ALTERNATIVES + PAD;
+constexpr float NONE = -FLT_MAX;            // score of a row that may not be seen
+constexpr float NONE_BELOW = -3.0e38f;
+constexpr double LOG2E = 1.4426950408889634074, LN2 = 0.69314718055994530942;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float lo_of(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi_of(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ uint64_t packf(float a, float b) {
+    return pack2(__float_as_uint(a), __float_as_uint(b));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) {
+    return __bfloat162float(v);
+}
+
+// A running (max, sum, weighted sum) of one query's columns, in raw score
+// units u (t = u * rf); rf > 0.
+struct Run {
+    float m, l, a;
+};
+__device__ __forceinline__ void run_raise(Run& r, float cm, float rf) {
+    if (cm > r.m) {
+        if (r.l != 0.0f) {  // (also NaN: it stays)
+            const float d = (r.m - cm) * rf;
+            const float f = ex2(d);
+            r.a = __fmaf_rn(d, r.l, r.a) * f;
+            r.l *= f;
+        }
+        r.m = cm;
+    }
+}
+// r joined with o (both in the same units)
+__device__ __forceinline__ void run_join(Run& r, Run o, float rf) {
+    if (o.m > r.m) {
+        const Run t = r;
+        r = o;
+        o = t;
+    }
+    if (!(o.l == 0.0f && o.a == 0.0f)) {
+        const float d = o.m == r.m ? 0.0f : (o.m - r.m) * rf;
+        const float f = ex2(d);
+        r.a += __fmaf_rn(d, o.l, o.a) * f;
+        r.l += o.l * f;
+    }
+}
+
+// The largest of 32 values with the number of its pair in the low 4 bits, and
+// the second largest (either may be moved by the marks: 2^-19 relative).
+__device__ __forceinline__ float2 top_pair(const float (&u)[32]) {
+    float h[16], lo = NONE;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+        const float l0 = fminf(u[2 * i], u[2 * i + 1]);
+        const float l1 = fminf(u[2 * i + 2], u[2 * i + 3]);
+        lo = max3(lo, l0, l1);
+        h[i] = __uint_as_float((__float_as_uint(fmaxf(u[2 * i], u[2 * i + 1])) & ~15u) | i);
+        h[i + 1] =
+            __uint_as_float((__float_as_uint(fmaxf(u[2 * i + 2], u[2 * i + 3])) & ~15u) | (i + 1));
+    }
+#pragma unroll
+    for (int w = 8; w >= 1; w >>= 1) {
+#pragma unroll
+        for (int i = 0; i < w; ++i) {
+            const float a = h[i], b = h[i + w];
+            lo = fmaxf(lo, fminf(a, b));
+            h[i] = fmaxf(a, b);
+        }
+    }
+    return make_float2(h[0], lo);
+}
+
+// ---------------------------------------------------------------------------
+// packing
+// ---------------------------------------------------------------------------
+// One warp per row: f32 (or 16-bit) values scaled by 2^e, |largest| in
+// [2^13, 2^14), as fp16 hi and, with two parts, lo = the rest; columns padded
+// with zeros to kp.  f[row] = 2^-e; 0 for a row of zeros, NaN for a row with
+// an infinity or NaN (its elements are then written as zeros: the NaN reaches
+// a score through f alone, so a query that may not see the row is not
+// touched).  `seen` (nullable): rows whose bit is clear are taken as zeros.
+// Bound by memory: reads d * size, writes 2 * parts * kp a row.
+template <typename T, int PARTS>
+__global__ void __launch_bounds__(256)
+    pack_kernel(const T* __restrict__ x, size_t ld, int n, int d, int kp,
+                const uint32_t* __restrict__ seen, __half* __restrict__ out,
+                float* __restrict__ f, unsigned* __restrict__ fmax_bits) {
+    const int lane = threadIdx.x & 31;
+    const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= n) return;
+    const T* src = x + (size_t)row * ld;
+    __half* dst = out + (size_t)row * (size_t)(PARTS * kp);
+    const bool use = !seen || (seen[row >> 5] >> (row & 31) & 1u);
+    float mx = 0.0f;
+    bool bad = false;
+    if (use)
+        for (int c = lane; c < d; c += 32) {
+            const float v = fabsf(to_f32<T>(src[c]));
+            bad |= !(v <= FLT_MAX);
+            mx = fmaxf(mx, v);
+        }
+    bad = __any_sync(0xffffffffu, bad);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    // 2^e with mx 2^e in [2^13, 2^14); e within +-120 keeps 2^e and 2^-e normal
+    int e = 0;
+    if (!bad && mx > 0.0f) e = max(-120, min(120, 13 - ilogbf(mx)));
+    const float s = ldexpf(1.0f, e);
+    const bool zero = bad || !(mx > 0.0f);
+    for (int c = lane; c < kp; c += 32) {
+        const float v = (!zero && c < d) ? to_f32<T>(src[c]) * s : 0.0f;
+        const __half hi = __float2half_rn(v);
+        dst[c] = hi;
+        if (PARTS == 2) dst[kp + c] = __float2half_rn(v - __half2float(hi));
+    }
+    if (lane == 0) {
+        const float r = bad ? __int_as_float(0x7fc00000) : (mx > 0.0f ? ldexpf(1.0f, -e) : 0.0f);
+        f[row] = r;
+        if (fmax_bits && r > 0.0f) atomicMax(fmax_bits, __float_as_uint(r));
+    }
+}
+// 16-bit rows copied to an aligned, zero-padded layout (their own is not one
+// that a tensor map can describe).
+__global__ void __launch_bounds__(256)
+    align_kernel(const uint16_t* __restrict__ x, size_t ld, int n, int d, int kp,
+                 uint16_t* __restrict__ out) {
+    const int lane = threadIdx.x & 31;
+    const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= n) return;
+    for (int c = lane; c < kp; c += 32)
+        out[(size_t)row * kp + c] = c < d ? x[(size_t)row * ld + c] : (uint16_t)0;
+}
+
+// ---------------------------------------------------------------------------
+// the tensor-core pipeline
+// ---------------------------------------------------------------------------
+// STATS: running triples of 128 queries x one column tile of rows; GRAD: the
+// score gradients of such a tile; PROD_Q, PROD_X: the products of the score
+// gradients with the rows and (transposed) with the queries.
+constexpr int STATS = 0, GRAD = 1, PROD_Q = 2, PROD_X = 3;
+
+struct Mma {
+    // Units: STATS, GRAD: (row block, chunk of the column tiles), the row
+    // block fastest so that the blocks that run together share column tiles.
+    // PROD: (row block, column block, split of K).
+    int mt, nt, chunks;
+    int atoms;                   // 64-wide steps of K
+    int klast;                   // 16-wide MMA steps of the last of them
+    int a_part, b_part;          // distance of the second part from the first in its map
+    int b_row0;                  // PROD_Q: first row of the chunk
+    int ncols;                   // PROD: columns of the output
+    uint32_t idesc;              // but for N
+    int stall;                   // test hook: no loads, so that the waits run out
+    int* err;
+    unsigned long long wait;
+};
+struct StatsArgs {
+    int q0, nq;                 // queries [q0, q0 + nq) of the call
+    int n;
+    const float* qf;            // [nq] 2^-e of the packed queries (f32 rows), else null
+    const float* xf;            // [padded n] 2^-e of the packed rows, else null
+    float rf;                   // scale * log2(e)
+    const uint32_t* allowed;    // nullable
+    size_t ld_allowed;          // words a query (0: one filter for all)
+    float4* part;               // [chunks * 4][nq]: m, l, a
+    float2* top;                // [nq][groups] or null
+    size_t groups;              // 32-row groups, whole column tiles
+};
+// What the score gradients of one query need (see coef_kernel).
+struct Coef {
+    float rf_hi, rf_lo, l_hi, l_lo;  // t - lse in log2 units = u rf - l, in two parts each
+    float c, h, g;                   // G = p (c + h x) + g at the given row
+    int target;
+};
+struct GradArgs {
+    int nq, n, j0, cols;        // this chunk: rows [j0, j0 + cols)
+    const Coef* coef;           // [nq]
+    const float *qf, *xf;       // 2^-e of the packed queries and rows
+    const float* bounds;        // [0] max of B_i qf_i, [1] max of xf
+    const uint32_t* allowed;
+    size_t ld_allowed;
+    __half* out;                // [parts][nqp][ldg]
+    size_t ldg, plane;          // plane: nqp * ldg
+};
+struct ProdArgs {
+    int rows, cols;             // output
+    const float* f;             // 2^-e of the output's rows
+    const float* bounds;
+    float* partial;             // [splits][rows][cols], or null: `out` is written
+    int add;                    // added to `partial` instead of stored
+    void* out;
+    size_t ldo;
+    int dtype;
+};
+
+// C = 2^c, the common factor of the stored score gradients: the largest
+// |G| * 2^-ei * 2^-ej comes to [2^13, 2^15).
+__device__ __forceinline__ float grad_factor(const float* bounds) {
+    const float b = bounds[0], x = bounds[1];
+    if (!(b > 0.0f) || !(x > 0.0f)) return 1.0f;
+    return ldexpf(1.0f, max(-100, min(100, 13 - ilogbf(b) - ilogbf(x))));
+}
+
+__device__ __forceinline__ uint32_t allowed_word(const uint32_t* al, size_t ld, int q, size_t col,
+                                                 int n) {
+    if (col >= (size_t)n) return 0u;
+    const uint32_t w = al ? __ldg(al + (size_t)q * ld + (col >> 5)) : 0xffffffffu;
+    const size_t left = (size_t)n - col;
+    return left >= 32 ? w : w & ((1u << left) - 1u);
+}
+
+// One 32-column chunk of the accumulator, in f32.
+__device__ __forceinline__ void load_chunk(uint32_t tmem, float (&u)[32]) {
+    uint32_t v[32];
+    tmem_ld32_nowait(tmem, v);
+    tmem_wait_regs(v);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) u[i] = __uint_as_float(v[i]);
+}
+__device__ __forceinline__ void scale_chunk(const float* f, float (&u)[32]) {
+    const float4* cf = reinterpret_cast<const float4*>(f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float4 c = __ldg(cf + i);
+        u[4 * i] *= c.x;
+        u[4 * i + 1] *= c.y;
+        u[4 * i + 2] *= c.z;
+        u[4 * i + 3] *= c.w;
+    }
+}
+
+// The epilogues: one object per thread and unit; `chunk` takes 32 columns of
+// the thread's row, from column `col` of the unit's matrix, in registers.
+template <bool TWO>
+struct StatsEpilogue {
+    typedef StatsArgs Args;
+    const StatsArgs& p;
+    int q;  // query of this pass, -1 past the end
+    float rf;
+    Run r;
+    bool live;
+    __device__ StatsEpilogue(const Mma&, const StatsArgs& a, int row, int row0, int, int) : p(a) {
+        q = row < a.nq ? row : -1;
+        live = row0 < a.nq;
+        rf = a.rf;
+        if (TWO && q >= 0) {
+            const float f = a.qf[q];
+            rf = f == 0.0f ? a.rf : f * a.rf;  // a query of zeros scores 0
+        }
+        r = Run{-INFINITY, 0.0f, 0.0f};
+    }
+    __device__ __forceinline__ void chunk(float (&u)[32], int icol) {
+        if (!live) return;
+        const size_t col = (size_t)icol;
+        const uint32_t w =
+            allowed_word(q < 0 ? nullptr : p.allowed, p.ld_allowed, p.q0 + q, col, p.n);
+        float2 best = make_float2(NONE, NONE);
+        if (__any_sync(0xffffffffu, w != 0u)) {
+            if (TWO) scale_chunk(p.xf + col, u);
+            const bool full = __all_sync(0xffffffffu, w == 0xffffffffu);
+            if (!full) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (!(w >> i & 1u)) u[i] = NONE;
+            }
+            if (p.top) best = top_pair(u);
+            float cm = max3(u[0], u[1], u[2]);
+#pragma unroll
+            for (int i = 3; i < 31; i += 2) cm = max3(cm, u[i], u[i + 1]);
+            cm = fmaxf(cm, u[31]);
+            if (cm > NONE_BELOW) run_raise(r, cm, rf);
+            const float m = r.m == -INFINITY ? 0.0f : r.m;
+            const uint64_t m2 = packf(-m, -m), rf2 = packf(rf, rf);
+            uint64_t l2[2] = {0, 0}, a2[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                // (the difference first: it is exact near the largest score)
+                uint64_t d = mul2(add2(packf(u[2 * i], u[2 * i + 1]), m2), rf2);
+                if (!full)
+                    d = packf((w >> (2 * i) & 1u) ? lo_of(d) : -200.0f,
+                              (w >> (2 * i + 1) & 1u) ? hi_of(d) : -200.0f);
+                const uint64_t e = packf(ex2(lo_of(d)), ex2(hi_of(d)));
+                l2[i & 1] = add2(l2[i & 1], e);
+                a2[i & 1] = fma2(e, d, a2[i & 1]);
+            }
+            l2[0] = add2(l2[0], l2[1]);
+            a2[0] = add2(a2[0], a2[1]);
+            r.l += lo_of(l2[0]) + hi_of(l2[0]);
+            r.a += lo_of(a2[0]) + hi_of(a2[0]);
+        }
+        if (p.top && q >= 0) p.top[(size_t)q * p.groups + (col >> 5)] = best;
+    }
+    __device__ __forceinline__ void finish(int chunk, int part) {
+        if (q >= 0)
+            p.part[(size_t)(chunk * 4 + part) * p.nq + q] = make_float4(r.m, r.l, r.a, 0.0f);
+    }
+};
+
+// Score gradients, stored as fp16 (two parts for f32 inputs) scaled by
+// 2^-ei 2^-ej C so that both products read them as they are.
+template <bool TWO>
+struct GradEpilogue {
+    typedef GradArgs Args;
+    const GradArgs& p;
+    int q, row;
+    Coef k;
+    float wi;
+    __device__ GradEpilogue(const Mma&, const GradArgs& a, int r, int, int, int) : p(a) {
+        row = r;
+        q = r < a.nq ? r : -1;
+        k = a.coef[q < 0 ? 0 : q];
+        const float f = q < 0 ? 0.0f : a.qf[q];
+        wi = f * grad_factor(a.bounds);
+    }
+    __device__ __forceinline__ void chunk(float (&u)[32], int icol) {  // icol: of the chunk
+        const size_t col = (size_t)icol, gcol = (size_t)p.j0 + col;
+        if (col >= p.ldg) return;
+        uint32_t w = allowed_word(q < 0 ? nullptr : p.allowed, p.ld_allowed, max(q, 0), gcol,
+                                  p.j0 + p.cols);
+        if (q < 0) w = 0u;
+        const bool any = __any_sync(0xffffffffu, w != 0u);
+        const bool full = __all_sync(0xffffffffu, w == 0xffffffffu);
+        const int at = k.target - (int)gcol;  // of the given row, if it is in this chunk
+        const float* xf = p.xf + gcol;
+        uint4* oh = reinterpret_cast<uint4*>(p.out + (size_t)row * p.ldg + col);
+        uint4* ol = reinterpret_cast<uint4*>(p.out + p.plane + (size_t)row * p.ldg + col);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            uint32_t h4[4], l4[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c0 = 8 * b + 2 * i;
+                h4[i] = l4[i] = 0u;
+                if (!any) continue;
+                const float2 cf = __ldg(reinterpret_cast<const float2*>(xf + c0));
+                float g2[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float c = j ? cf.y : cf.x;
+                    const float uu = u[c0 + j] * c;
+                    float x = __fmaf_rn(uu, k.rf_hi, -k.l_hi) + __fmaf_rn(uu, k.rf_lo, -k.l_lo);
+                    x = fmaxf(x, -160.0f);
+                    float g = ex2(x) * __fmaf_rn(x, k.h, k.c);
+                    if (at == c0 + j) g += k.g;
+                    g *= c * wi;
+                    if (!full && !(w >> (c0 + j) & 1u)) g = 0.0f;
+                    g2[j] = g;
+                }
+                const __half2 hh = __floats2half2_rn(g2[0], g2[1]);
+                h4[i] = *reinterpret_cast<const uint32_t*>(&hh);
+                if (TWO) {
+                    const float2 back = __half22float2(hh);
+                    const __half2 ll = __floats2half2_rn(g2[0] - back.x, g2[1] - back.y);
+                    l4[i] = *reinterpret_cast<const uint32_t*>(&ll);
+                }
+            }
+            oh[b] = make_uint4(h4[0], h4[1], h4[2], h4[3]);
+            if (TWO) ol[b] = make_uint4(l4[0], l4[1], l4[2], l4[3]);
+        }
+    }
+    __device__ __forceinline__ void finish(int, int) {}
+};
+
+// `count` values of one output row from column c, rounded to the output's type.
+__device__ __forceinline__ void store_row(void* out, size_t ldo, int dtype, int row, int c,
+                                          int count, const float (&v)[32]) {
+    const size_t es = dtype == FDB_DTYPE_F32 ? 4 : 2;
+    unsigned char* o = static_cast<unsigned char*>(out) + ((size_t)row * ldo + (size_t)c) * es;
+    const bool wide = (reinterpret_cast<uintptr_t>(o) & 15) == 0;
+    if (dtype == FDB_DTYPE_F32) {
+        float* f = reinterpret_cast<float*>(o);
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+            if (wide && i + 4 <= count)
+                *reinterpret_cast<float4*>(f + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (i + j < count) f[i + j] = v[i + j];
+            }
+        }
+        return;
+    }
+    uint16_t* h = reinterpret_cast<uint16_t*>(o);
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (dtype == FDB_DTYPE_BF16) {
+                const __nv_bfloat162 b = __floats2bfloat162_rn(v[i + 2 * j], v[i + 2 * j + 1]);
+                w[j] = *reinterpret_cast<const uint32_t*>(&b);
+            } else {
+                const __half2 b = __floats2half2_rn(v[i + 2 * j], v[i + 2 * j + 1]);
+                w[j] = *reinterpret_cast<const uint32_t*>(&b);
+            }
+        }
+        if (wide && i + 8 <= count)
+            *reinterpret_cast<uint4*>(h + i) = make_uint4(w[0], w[1], w[2], w[3]);
+        else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (i + j < count) h[i + j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+        }
+    }
+}
+
+struct ProdEpilogue {
+    typedef ProdArgs Args;
+    const ProdArgs& p;
+    int row, split;
+    float s;
+    __device__ ProdEpilogue(const Mma&, const ProdArgs& a, int r, int, int, int sp) : p(a) {
+        row = r;
+        split = sp;
+        s = !a.partial && row < a.rows ? 1.0f / (a.f[row] * grad_factor(a.bounds)) : 0.0f;
+    }
+    __device__ __forceinline__ void chunk(float (&u)[32], int c) {
+        if (c >= p.cols || row >= p.rows) return;
+        const int count = min(32, p.cols - c);
+        if (!p.partial) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) u[i] *= s;
+            store_row(p.out, p.ldo, p.dtype, row, c, count, u);
+            return;
+        }
+        float* o = p.partial + ((size_t)split * p.rows + row) * (size_t)p.cols + c;
+        if ((p.cols & 3) == 0 && count == 32) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float4 v = make_float4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
+                float4* o4 = reinterpret_cast<float4*>(o) + i;
+                if (p.add) {
+                    const float4 w = *o4;
+                    v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+                }
+                *o4 = v;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (i < count) o[i] = p.add ? o[i] + u[i] : u[i];
+        }
+    }
+    __device__ __forceinline__ void finish(int, int) {}
+};
+template <int MODE, bool TWO>
+struct EpilogueOf;
+template <bool TWO>
+struct EpilogueOf<STATS, TWO> {
+    typedef StatsEpilogue<TWO> Type;
+};
+template <bool TWO>
+struct EpilogueOf<GRAD, TWO> {
+    typedef GradEpilogue<TWO> Type;
+};
+template <bool TWO>
+struct EpilogueOf<PROD_Q, TWO> {
+    typedef ProdEpilogue Type;
+};
+template <bool TWO>
+struct EpilogueOf<PROD_X, TWO> {
+    typedef ProdEpilogue Type;
+};
+
+// MN-major operand tile (64 elements of M or N along a 128-byte row, one row
+// a k, 128-byte swizzle): 8-k groups 1024 B apart (SBO), 64-element groups
+// 64 k = 8192 B apart (LBO).
+__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)512 << 16) | ((uint64_t)64 << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// What a unit covers.
+struct Unit {
+    int mt, sp;      // sp: chunk (STATS, GRAD) or split of K (PROD)
+    int t0, t1;      // column tiles
+    int a0, a1;      // 64-wide steps of K
+};
+template <int MODE>
+__device__ __forceinline__ Unit unit_of(const Mma& g, int u) {
+    Unit x;
+    x.mt = u % g.mt;
+    if (MODE == PROD_Q || MODE == PROD_X) {
+        x.t0 = u / g.mt % g.nt;
+        x.t1 = x.t0 + 1;
+        x.sp = u / g.mt / g.nt;
+        x.a0 = (int)((long long)x.sp * g.atoms / g.chunks);
+        x.a1 = (int)((long long)(x.sp + 1) * g.atoms / g.chunks);
+    } else {
+        x.sp = u / g.mt;
+        x.t0 = (int)((long long)x.sp * g.nt / g.chunks);
+        x.t1 = (int)((long long)(x.sp + 1) * g.nt / g.chunks);
+        x.a0 = 0;
+        x.a1 = g.atoms;
+    }
+    return x;
+}
+
+// Warp 0 loads the K steps of both operands with TMA, warp 1 issues the MMAs
+// into the TMEM accumulators, sixteen epilogue warps (four per lane quadrant,
+// a quarter of the columns each) work on a finished one meanwhile.
+// Persistent: a block takes units blockIdx.x, + gridDim.x, ...
+//
+// One part: an accumulator is a whole tile (all of K).  TWO parts: it is ONE
+// K step, the products lo.hi, hi.lo, hi.hi in this order, and the epilogue
+// adds the steps up in registers: the tensor core's own additions cut the sum
+// towards zero (measured: 8e-7 of a score at dim 512, against 1.5e-7 when a
+// step of 64 is the longest such sum).
+template <int MODE, bool TWO>
+__global__ void __launch_bounds__(THREADS, 1)
+    rows_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
+                const Mma g, const typename EpilogueOf<MODE, TWO>::Type::Args p) {
+    constexpr bool PROD = MODE == PROD_Q || MODE == PROD_X;
+    constexpr bool A_MN = MODE == PROD_X, B_MN = PROD;
+    constexpr int BN = bn_of(TWO), NST = stages_of(TWO), NACC = accs_of(TWO);
+    constexpr int STAGE = stage_bytes(TWO), PARTS = TWO ? 2 : 1;
+    constexpr int B0 = PARTS * OPER;               // operand B in a stage
+    constexpr int B_PART = BN * 128;               // bytes of one part of it
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    const uint32_t base = smem_u32(smem_raw);
+    unsigned char* smem = smem_raw + ((1024 - (base & 1023)) & 1023);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + NST * STAGE);
+    uint64_t* empty = full + NST;
+    uint64_t* t_full = empty + NST;
+    uint64_t* t_empty = t_full + NACC;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(t_empty + NACC);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < NST; ++i) {
+            mbar_init(full + i, 1);
+            mbar_init(empty + i, 1);
+        }
+        for (int i = 0; i < NACC; ++i) {
+            mbar_init(t_full + i, 1);
+            mbar_init(t_empty + i, EPI_WARPS);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(tmem_slot)),
+                     "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int units = PROD ? g.mt * g.nt * g.chunks : g.mt * g.chunks;
+    int last_use[NST];  // producer: last use issued of each stage
+    for (int i = 0; i < NST; ++i) last_use[i] = -1;
+    int last_stage = -1, last_phase = 0;  // MMA issuer: last stage committed
+
+    if (warp == 0) {
+        if (lane == 0 && !g.stall) {
+            int it = 0;
+            bool ok = true;
+            for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+                const Unit x = unit_of<MODE>(g, u);
+                for (int t = x.t0; ok && t < x.t1; ++t) {
+                    const int boxes = B_MN ? (min(BN, g.ncols - t * BN) + 63) / 64 : 0;
+                    const uint32_t bytes =
+                        PARTS * (OPER + (uint32_t)(B_MN ? boxes * 8192 : B_PART));
+                    for (int a = x.a0; a < x.a1; ++a, ++it) {
+                        const int s = it % NST, use = it / NST;
+                        if (use > 0 && !mbar_wait(empty + s, (use - 1) & 1, g.err, g.wait)) {
+                            ok = false;
+                            break;
+                        }
+                        mbar_expect_tx(full + s, bytes);
+#pragma unroll
+                        for (int h = 0; h < PARTS; ++h) {
+                            unsigned char* da = smem + s * STAGE + h * OPER;
+                            unsigned char* db = smem + s * STAGE + B0 + h * B_PART;
+                            const int pa = h * g.a_part, pb = h * g.b_part;
+                            if (A_MN) {
+                                tma_load_2d(da, &amap, full + s, x.mt * BM, pa + a * KATOM);
+                                tma_load_2d(da + 8192, &amap, full + s, x.mt * BM + 64,
+                                            pa + a * KATOM);
+                            } else if (PROD) {
+                                tma_load_2d(da, &amap, full + s, a * KATOM, pa + x.mt * BM);
+                            } else {
+                                tma_load_2d(da, &amap, full + s, pa + a * KATOM, x.mt * BM);
+                            }
+                            if (B_MN) {
+                                for (int b = 0; b < boxes; ++b)
+                                    tma_load_2d(db + b * 8192, &bmap, full + s,
+                                                pb + t * BN + 64 * b, g.b_row0 + a * KATOM);
+                            } else {
+#pragma unroll
+                                for (int b = 0; b < BN / 128; ++b)
+                                    tma_load_2d(db + b * OPER, &bmap, full + s, pb + a * KATOM,
+                                                g.b_row0 + t * BN + 128 * b);
+                            }
+                        }
+                        last_use[s] = use;
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            int it = 0, ti = 0;  // K steps, accumulators
+            bool ok = true;
+            for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+                const Unit x = unit_of<MODE>(g, u);
+                for (int t = x.t0; ok && t < x.t1; ++t) {
+                    const int bn = PROD ? (min(BN, g.ncols - t * BN) + 15) & ~15 : BN;
+                    const uint32_t idesc = g.idesc | ((uint32_t)(bn >> 3) << 17);
+                    uint32_t acc = 0;
+                    for (int a = x.a0; a < x.a1; ++a, ++it) {
+                        const int b = ti % NACC;
+                        const uint32_t d = tmem + (uint32_t)(b * BN);
+                        if (TWO || a == x.a0) {  // a new accumulator
+                            if (ti >= NACC &&
+                                !mbar_wait(t_empty + b, (ti / NACC - 1) & 1, g.err, g.wait)) {
+                                ok = false;
+                                break;
+                            }
+                            acc = 0;
+                        }
+                        const int s = it % NST, use = it / NST;
+                        if (!mbar_wait(full + s, use & 1, g.err, g.wait)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t ab = smem_u32(smem + s * STAGE), bb = ab + B0;
+                        const int kk1 = a == g.atoms - 1 ? g.klast : 4;
+#pragma unroll
+                        for (int pr = 0; pr < (TWO ? 3 : 1); ++pr) {
+                            const uint32_t ap = ab + (TWO && pr == 0 ? OPER : 0);
+                            const uint32_t bp = bb + (TWO && pr == 1 ? B_PART : 0);
+                            for (int kk = 0; kk < kk1; ++kk) {
+                                umma_f16_n(d,
+                                           A_MN ? smem_desc_mn(ap + kk * 2048)
+                                                : smem_desc_sw128(ap + kk * 32),
+                                           B_MN ? smem_desc_mn(bp + kk * 2048)
+                                                : smem_desc_sw128(bp + kk * 32),
+                                           idesc, acc);
+                                acc = 1;
+                            }
+                        }
+                        umma_commit(empty + s);
+                        last_stage = s;
+                        last_phase = use & 1;
+                        if (TWO || a + 1 == x.a1) {
+                            umma_commit(t_full + b);
+                            ++ti;
+                        }
+                    }
+                }
+            }
+        }
+    } else if (warp >= EPI_WARP0) {
+        const int w = warp - EPI_WARP0, quad = w & 3, part = w >> 2;
+        const uint32_t mine = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(part * (BN / 4));
+        int ti = 0;
+        bool ok = true;
+        // the next accumulator, or false when the kernel is aborting
+        auto next = [&]() -> bool {
+            int got = 0;
+            if (lane == 0) got = mbar_wait(t_full + ti % NACC, (ti / NACC) & 1, g.err, g.wait);
+            got = __shfl_sync(0xffffffffu, got, 0);
+            tc_fence_after();
+            return got != 0;
+        };
+        auto release = [&] {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(t_empty + ti % NACC);
+            ++ti;
+        };
+        for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+            const Unit x = unit_of<MODE>(g, u);
+            const int row0 = x.mt * BM + quad * 32;
+            typename EpilogueOf<MODE, TWO>::Type epi(g, p, row0 + lane, row0, x.t0, x.sp);
+            for (int t = x.t0; ok && t < x.t1; ++t) {
+                const int col = t * BN + part * (BN / 4);
+                float v[32];
+                if (TWO) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+                    for (int a = x.a0; a < x.a1; ++a) {
+                        if (!next()) {
+                            ok = false;
+                            break;
+                        }
+                        float y[32];
+                        load_chunk(mine + (uint32_t)(ti % NACC * BN), y);
+                        release();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] += y[i];
+                    }
+                    if (ok) epi.chunk(v, col);
+                    __syncwarp();
+                } else {
+                    if (!next()) {
+                        ok = false;
+                        break;
+                    }
+#pragma unroll 1
+                    for (int h = 0; h < 2; ++h) {
+                        load_chunk(mine + (uint32_t)(ti % NACC * BN + h * 32), v);
+                        epi.chunk(v, col + h * 32);
+                        __syncwarp();
+                    }
+                    release();
+                }
+            }
+            if (ok) epi.finish(x.sp, part);
+        }
+    }
+    // One verdict for the whole block; an aborting block lets the copies and
+    // MMAs it issued land (bounded) before it frees TMEM and exits.
+    if (__syncthreads_or(*(volatile int*)g.err != 0)) {
+        if (warp == 0 && lane == 0)
+            for (int s = 0; s < NST; ++s)
+                if (last_use[s] >= 0) {
+                    const unsigned long long c0 = clock64();
+                    while (!mbar_try(full + s, last_use[s] & 1) && clock64() - c0 < WAIT_CYCLES) {
+                    }
+                }
+        if (warp == 1 && lane == 0 && last_stage >= 0) {
+            const unsigned long long c0 = clock64();
+            while (!mbar_try(empty + last_stage, last_phase) && clock64() - c0 < WAIT_CYCLES) {
+            }
+        }
+        __syncthreads();
+    }
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                     "r"(512));
+    }
+}
+
+// ---------------------------------------------------------------------------
+// a few f32 queries: one pass over the rows on the FMA pipes
+// ---------------------------------------------------------------------------
+// A warp takes groups of 32 rows, 8 at a time: each lane multiplies its
+// columns of 8 rows with its columns of NQ queries (from shared memory), and
+// a transposing reduction leaves each row's sums in four lanes, of which one
+// keeps them, so that after four batches every lane holds one row of the
+// group.  Bound by memory (each row read once) up to about 8 queries.
+template <int NQ, bool VEC>
+__global__ void __launch_bounds__(64)
+    few_kernel(const float* __restrict__ x, size_t ld, int n, int d, const float* __restrict__ q,
+               size_t ldq, int q0, int nq, float rf, const uint32_t* __restrict__ allowed,
+               size_t ld_allowed, float4* __restrict__ part, float2* __restrict__ top,
+               size_t groups) {
+    extern __shared__ float4 qs4[];
+    float* qs = reinterpret_cast<float*>(qs4);  // [NQ][dp]
+    const int dp = (d + 127) & ~127;
+    for (int i = threadIdx.x; i < NQ * dp; i += 64) {
+        const int j = i / dp, c = i - j * dp;
+        qs[i] = j < nq && c < d ? q[(size_t)(q0 + j) * ldq + c] : 0.0f;
+    }
+    __syncthreads();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int row_of_lane = ((lane >> 4 & 1) << 2 | (lane >> 3 & 1) << 1 | (lane >> 2 & 1)) +
+                            8 * (lane & 3);
+    Run r[NQ];
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) r[j] = Run{-INFINITY, 0.0f, 0.0f};
+    const int ng = (n + GROUP - 1) / GROUP;
+    for (int grp = blockIdx.x * 2 + warp; grp < ng; grp += gridDim.x * 2) {
+        float sc[NQ];
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) sc[j] = 0.0f;
+#pragma unroll 1
+        for (int b = 0; b < 4; ++b) {
+            const int r0 = grp * GROUP + b * 8;
+            float acc[NQ][8];
+#pragma unroll
+            for (int j = 0; j < NQ; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc[j][i] = 0.0f;
+            const float* row[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) row[i] = x + (size_t)min(r0 + i, n - 1) * ld;
+            if (VEC) {
+                for (int c = lane * 4; c < d; c += 128) {
+                    float4 xv[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        xv[i] = __ldg(reinterpret_cast<const float4*>(row[i] + c));
+#pragma unroll
+                    for (int j = 0; j < NQ; ++j) {
+                        const float4 qv = *reinterpret_cast<const float4*>(qs + j * dp + c);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            acc[j][i] = __fmaf_rn(xv[i].x, qv.x, acc[j][i]);
+                            acc[j][i] = __fmaf_rn(xv[i].y, qv.y, acc[j][i]);
+                            acc[j][i] = __fmaf_rn(xv[i].z, qv.z, acc[j][i]);
+                            acc[j][i] = __fmaf_rn(xv[i].w, qv.w, acc[j][i]);
+                        }
+                    }
+                }
+            } else {
+                for (int c = lane; c < d; c += 32) {
+                    float xv[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) xv[i] = __ldg(row[i] + c);
+#pragma unroll
+                    for (int j = 0; j < NQ; ++j) {
+                        const float qv = qs[j * dp + c];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) acc[j][i] = __fmaf_rn(xv[i], qv, acc[j][i]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < NQ; ++j) {
+                float t4[4], t2[2], t1;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float keep = lane & 16 ? acc[j][i + 4] : acc[j][i];
+                    const float give = lane & 16 ? acc[j][i] : acc[j][i + 4];
+                    t4[i] = keep + __shfl_xor_sync(0xffffffffu, give, 16);
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float keep = lane & 8 ? t4[i + 2] : t4[i];
+                    const float give = lane & 8 ? t4[i] : t4[i + 2];
+                    t2[i] = keep + __shfl_xor_sync(0xffffffffu, give, 8);
+                }
+                const float keep = lane & 4 ? t2[1] : t2[0];
+                const float give = lane & 4 ? t2[0] : t2[1];
+                t1 = keep + __shfl_xor_sync(0xffffffffu, give, 4);
+                t1 += __shfl_xor_sync(0xffffffffu, t1, 2);
+                t1 += __shfl_xor_sync(0xffffffffu, t1, 1);
+                if ((lane & 3) == b) sc[j] = t1;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+            if (j >= nq) break;
+            const uint32_t w =
+                allowed_word(allowed, ld_allowed, q0 + j, (size_t)grp * GROUP, n);
+            const bool ok = w >> row_of_lane & 1u;
+            if (ok) {
+                run_raise(r[j], sc[j], rf);
+                const float m = r[j].m == -INFINITY ? 0.0f : r[j].m;
+                const float dd = (sc[j] - m) * rf, e = ex2(dd);
+                r[j].l += e;
+                r[j].a = __fmaf_rn(e, dd, r[j].a);
+            }
+            if (top) {
+                float a = ok ? sc[j] : NONE, b2 = NONE;
+                a = __uint_as_float((__float_as_uint(a) & ~15u) | (unsigned)(row_of_lane >> 1));
+#pragma unroll
+                for (int o = 16; o; o >>= 1) {
+                    const float oa = __shfl_xor_sync(0xffffffffu, a, o);
+                    const float ob = __shfl_xor_sync(0xffffffffu, b2, o);
+                    b2 = max3(b2, ob, fminf(a, oa));
+                    a = fmaxf(a, oa);
+                }
+                if (lane == 0) top[(size_t)j * groups + grp] = make_float2(a, b2);
+            }
+        }
+    }
+    // the lanes' triples joined, then the two warps'
+    __shared__ Run other[NQ];
+#pragma unroll
+    for (int j = 0; j < NQ; ++j)
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            Run t;
+            t.m = __shfl_xor_sync(0xffffffffu, r[j].m, o);
+            t.l = __shfl_xor_sync(0xffffffffu, r[j].l, o);
+            t.a = __shfl_xor_sync(0xffffffffu, r[j].a, o);
+            run_join(r[j], t, rf);
+        }
+    if (warp == 1 && lane == 0)
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) other[j] = r[j];
+    __syncthreads();
+    if (warp == 0 && lane == 0)
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+            if (j < nq) {
+                run_join(r[j], other[j], rf);
+                part[(size_t)blockIdx.x * nq + j] = make_float4(r[j].m, r[j].l, r[j].a, 0.0f);
+            }
+}
+
+// ---------------------------------------------------------------------------
+// joining the parts, the given row, the top alternatives
+// ---------------------------------------------------------------------------
+struct FinishArgs {
+    const void *q, *x;
+    size_t ldq, ldx;
+    int q0, nq, n, d, k;
+    float scale;
+    const int64_t* targets;
+    const uint32_t* allowed;
+    size_t ld_allowed;
+    const float4* part;
+    int parts;
+    const float* qf;
+    const float2* top;
+    size_t groups;
+    float *logprob, *lse, *entropy, *top_logprob;
+    int64_t* top_ids;
+    const int* err;
+};
+
+// Order-preserving 32-bit image of a float.
+__device__ __forceinline__ uint32_t ordered(float f) {
+    const uint32_t u = __float_as_uint(f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+__device__ __forceinline__ float unordered(uint32_t u) {
+    return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+
+// 128 keys of a warp (4 a lane, key i of lane l at l + 32 i) sorted, largest first.
+__device__ __forceinline__ void warp_sort128(uint64_t (&v)[4], int lane) {
+#pragma unroll
+    for (int size = 2; size <= 128; size <<= 1) {
+#pragma unroll
+        for (int stride = size >> 1; stride > 0; stride >>= 1) {
+            if (stride >= 32) {
+                const int si = stride >> 5;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (!(i & si)) {
+                        const int e = lane + 32 * i;
+                        const bool desc = !(e & size);
+                        const uint64_t a = v[i], b = v[i | si];
+                        if ((a < b) == desc) {
+                            v[i] = b;
+                            v[i | si] = a;
+                        }
+                    }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int e = lane + 32 * i;
+                    const bool desc = !(e & size), lower = !(lane & stride);
+                    const uint64_t o = __shfl_xor_sync(0xffffffffu, v[i], stride);
+                    const bool keep_max = lower == desc;
+                    v[i] = keep_max ? (v[i] > o ? v[i] : o) : (v[i] < o ? v[i] : o);
+                }
+            }
+        }
+    }
+}
+
+// The `want` (<= 72) largest keys a warp has been offered: appended to a
+// buffer of 128 in shared memory when above the threshold, sorted when full.
+struct WarpTop {
+    uint64_t* buf;
+    int want, cnt, lane;
+    uint64_t thr;
+    __device__ WarpTop(uint64_t* b, int w, int l) : buf(b), want(w), cnt(0), lane(l), thr(0) {}
+    __device__ void shrink() {
+        uint64_t v[4];
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = lane + 32 * i < cnt ? buf[lane + 32 * i] : 0ull;
+        warp_sort128(v, lane);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) buf[lane + 32 * i] = v[i];
+        __syncwarp();
+        cnt = min(cnt, want);
+        if (cnt == want) thr = buf[want - 1];
+    }
+    __device__ void offer(uint64_t key) {  // key 0: none
+        const unsigned vote = __ballot_sync(0xffffffffu, key > thr);
+        if (!vote) return;
+        if (key > thr) buf[cnt + __popc(vote & ((1u << lane) - 1u))] = key;
+        cnt += __popc(vote);
+        if (cnt > 96) shrink();
+    }
+};
+
+constexpr int CAND = MAX_SEL * GROUP;  // the marked pairs, then the rest of their groups
+
+// q . x in 64 bits: 8 lanes a row, products of the inputs exact.
+template <typename T>
+__device__ __forceinline__ double dot8(const T* __restrict__ a, const T* __restrict__ b, int d,
+                                       int sub) {
+    double s0 = 0.0, s1 = 0.0;
+    int c = sub;
+    for (; c + 8 < d; c += 16) {
+        s0 = fma((double)to_f32<T>(a[c]), (double)to_f32<T>(b[c]), s0);
+        s1 = fma((double)to_f32<T>(a[c + 8]), (double)to_f32<T>(b[c + 8]), s1);
+    }
+    if (c < d) s0 = fma((double)to_f32<T>(a[c]), (double)to_f32<T>(b[c]), s0);
+    s0 += s1;
+#pragma unroll
+    for (int o = 4; o; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+    return s0;
+}
+
+// One block per query.
+template <typename T, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) finish_kernel(const FinishArgs p) {
+    __shared__ double red[WARPS][3];
+    __shared__ double s_lse;
+    __shared__ int s_bad;
+    __shared__ uint64_t buf[WARPS][128];
+    __shared__ int sel[MAX_SEL];
+    __shared__ float sel2[MAX_SEL];
+    __shared__ double cs[CAND + 1];
+    __shared__ uint32_t ci[CAND + 1];
+    __shared__ int s_cnt;
+    __shared__ double s_kth;
+    __shared__ double kept[FDB_MAX_ALTERNATIVES];
+    __shared__ uint32_t kept_id[FDB_MAX_ALTERNATIVES];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int ql = blockIdx.x, q = p.q0 + ql;
+    const T* qp = static_cast<const T*>(p.q) + (size_t)q * p.ldq;
+    const T* xp = static_cast<const T*>(p.x);
+    const uint32_t* al = p.allowed ? p.allowed + (size_t)q * p.ld_allowed : nullptr;
+    double f = 1.0;
+    if (p.qf) f = p.qf[ql] == 0.0f ? 1.0 : (double)p.qf[ql];
+    const double rf = f * (double)p.scale * LOG2E;
+
+    // ---- the running triples joined in 64 bits (m in units of t) ----
+    double M = -INFINITY, L = 0.0, A = 0.0;
+    auto join = [&](double m, double l, double a) {
+        if (m > M) {
+            const double t0 = M, t1 = L, t2 = A;
+            M = m, L = l, A = a;
+            m = t0, l = t1, a = t2;
+        }
+        if (!(l == 0.0 && a == 0.0)) {
+            const double d = m == M ? 0.0 : m - M, e = exp2(d);
+            A += (a + d * l) * e;
+            L += l * e;
+        }
+    };
+    for (int i = threadIdx.x; i < p.parts; i += WARPS * 32) {
+        const float4 t = p.part[(size_t)i * p.nq + ql];
+        join((double)t.x * rf, (double)t.y, (double)t.z);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        const double m = __shfl_xor_sync(0xffffffffu, M, o);
+        const double l = __shfl_xor_sync(0xffffffffu, L, o);
+        const double a = __shfl_xor_sync(0xffffffffu, A, o);
+        join(m, l, a);
+    }
+    if (lane == 0) red[warp][0] = M, red[warp][1] = L, red[warp][2] = A;
+    // the row whose log probability is asked for is the last candidate
+    const int64_t target = p.targets ? p.targets[q] : -1;
+    const bool given = target >= 0 && target < p.n;
+    if (threadIdx.x == 0) s_cnt = 0;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < WARPS; ++w) join(red[w][0], red[w][1], red[w][2]);
+        const bool empty = L == 0.0;
+        const bool bad = !(A == A) || !(L == L) || (p.err && *p.err != 0);
+        const double lg = empty ? 0.0 : log2(L);
+        const double lse = bad ? NAN : empty ? -INFINITY : LN2 * (M + lg);
+        if (p.lse) p.lse[q] = (float)lse;
+        if (p.entropy) p.entropy[q] = (float)(bad ? NAN : empty ? 0.0 : LN2 * (lg - A / L));
+        s_lse = lse;
+        s_bad = bad ? 2 : empty ? 1 : 0;
+    }
+
+    const int sub = lane & 7, per = WARPS * 4;  // rows scored at a time
+    const int slot = warp * 4 + (lane >> 3);
+    auto score = [&](int from, int to) {
+        for (int i = from; i < to; i += per) {
+            const int j = i + slot;
+            const double s = dot8<T>(qp, xp + (size_t)(j < to ? ci[j] : 0) * p.ldx, p.d, sub);
+            if (sub == 0 && j < to) cs[j] = s;
+        }
+    };
+    if (p.k > 0) {
+        // ---- the best k + 8 groups ----
+        const int want = (int)min((size_t)(p.k + PAD), p.groups);
+        const float2* top = p.top + (size_t)ql * p.groups;
+        WarpTop wt(buf[warp], want, lane);
+        for (size_t g0 = (size_t)warp * 32; g0 < p.groups; g0 += WARPS * 128) {
+            float2 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const size_t gi = g0 + (size_t)i * WARPS * 32 + lane;
+                v[i] = gi < p.groups ? top[gi] : make_float2(NONE, NONE);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const size_t gi = g0 + (size_t)i * WARPS * 32 + lane;
+                uint64_t key = 0;
+                if (v[i].x > NONE_BELOW)
+                    // (without the mark: equal scores by group number)
+                    key = (uint64_t)ordered(__uint_as_float(__float_as_uint(v[i].x) & ~15u)) << 32 |
+                          (uint32_t)~(uint32_t)gi;
+                wt.offer(key);
+            }
+        }
+        wt.shrink();
+        if (lane == 0) red[warp][0] = (double)wt.cnt;
+        __syncthreads();
+        if (warp == 0) {
+            for (int w = 1; w < WARPS; ++w) {
+                const int c = (int)red[w][0];
+                for (int i = 0; i < c; i += 32) wt.offer(i + lane < c ? buf[w][i + lane] : 0ull);
+            }
+            wt.shrink();
+            for (int i = lane; i < wt.cnt; i += 32) {
+                const uint32_t gi = ~(uint32_t)buf[0][i];
+                const float2 v = top[gi];
+                sel[i] = (int)gi;
+                sel2[i] = v.y;
+                const uint32_t pair = __float_as_uint(v.x) & 15u;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t id = gi * GROUP + pair * 2 + h;
+                    const bool ok = id < (uint32_t)p.n && (!al || (al[id >> 5] >> (id & 31) & 1u));
+                    if (ok) ci[atomicAdd(&s_cnt, 1)] = id;
+                }
+            }
+            if (lane == 0) {
+                red[0][1] = (double)wt.cnt;
+                // the largest a group that was not picked can hold
+                red[0][2] = wt.cnt == want && (size_t)want < p.groups
+                                ? (double)unordered((uint32_t)(buf[0][want - 1] >> 32))
+                                : -INFINITY;
+            }
+        }
+        __syncthreads();
+    }
+    int cnt = s_cnt;
+    const int nsel = p.k > 0 ? (int)red[0][1] : 0;
+    const double left_out = p.k > 0 ? red[0][2] : -INFINITY;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        ci[cnt] = given ? (uint32_t)target : 0u;
+        s_kth = -INFINITY;
+    }
+    __syncthreads();
+    score(0, cnt + 1);
+    __syncthreads();
+    // ---- the given row ----
+    const double lse = s_lse;
+    const int bad = s_bad;
+    if (threadIdx.x == 0 && p.logprob) {
+        float v = 0.0f;
+        if (given) {
+            const bool seen = !al || (al[target >> 5] >> (target & 31) & 1u);
+            v = bad == 2 ? NAN
+                : (bad == 1 || !seen) ? -INFINITY
+                                      : (float)(cs[cnt] * (double)p.scale - lse);
+        } else if (bad == 2) {
+            v = NAN;
+        }
+        p.logprob[q] = v;
+    }
+    if (p.k == 0) return;
+    // candidate i before candidate j
+    auto before = [&](int i, int j) { return cs[i] > cs[j] || (cs[i] == cs[j] && ci[i] < ci[j]); };
+    // Whether a score of at most `m` (as a group left it) may be among the best
+    // k, whose last exact score so far is s_kth: marks and 32-bit sums move it
+    // by far less than 2^-15 of the larger of the two.
+    auto may_enter = [&](double m) {
+        const double v = m * f, kth = s_kth;
+        return v >= kth - ldexp(fabs(v) + fabs(kth), -15);
+    };
+    // ---- groups whose second largest score may still enter ----
+    for (int i = threadIdx.x; i < cnt; i += WARPS * 32) {
+        int rank = 0;
+        for (int j = 0; j < cnt; ++j) rank += before(j, i);
+        if (rank == p.k - 1) s_kth = cs[i];
+    }
+    __syncthreads();
+    if (left_out > (double)NONE_BELOW && may_enter(left_out)) {
+        // ---- more groups are as good (many equal or nearly equal scores):
+        // every row of every group that may enter is scored, the best k kept ----
+        __syncthreads();
+        if (threadIdx.x == 0) s_cnt = 0;
+        const float2* top = p.top + (size_t)ql * p.groups;
+        for (size_t g0 = 0; g0 < p.groups; g0 += WARPS) {
+            __syncthreads();
+            const size_t gi = g0 + warp;
+            const float m1 = gi < p.groups ? top[gi].x : NONE;
+            if (m1 > NONE_BELOW && may_enter(m1)) {
+                const uint32_t w = allowed_word(al, 0, 0, gi * GROUP, p.n);
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t r = (uint32_t)(i * 4 + (lane >> 3));
+                    const bool in = w >> r & 1u;
+                    const uint32_t id = (uint32_t)gi * GROUP + r;
+                    const double v = dot8<T>(qp, xp + (size_t)(in ? id : 0) * p.ldx, p.d, sub);
+                    if (sub == 0 && in && !(v < s_kth)) {
+                        const int at = atomicAdd(&s_cnt, 1);
+                        cs[at] = v;
+                        ci[at] = id;
+                    }
+                }
+            }
+            __syncthreads();
+            const int have = s_cnt;
+            if (have + WARPS * GROUP > CAND || g0 + WARPS >= p.groups) {
+                for (int i = threadIdx.x; i < have; i += WARPS * 32) {
+                    int rank = 0;
+                    for (int j = 0; j < have; ++j) rank += before(j, i);
+                    if (rank < p.k) kept[rank] = cs[i], kept_id[rank] = ci[i];
+                }
+                __syncthreads();
+                const int keep = min(have, p.k);
+                for (int i = threadIdx.x; i < keep; i += WARPS * 32)
+                    cs[i] = kept[i], ci[i] = kept_id[i];
+                if (threadIdx.x == 0) {
+                    s_cnt = keep;
+                    if (keep == p.k) s_kth = kept[p.k - 1];
+                }
+            }
+        }
+        __syncthreads();
+        cnt = s_cnt;
+    } else if (threadIdx.x < nsel) {
+        const int gi = sel[threadIdx.x];
+        const float m2 = sel2[threadIdx.x];
+        if (m2 > NONE_BELOW && may_enter(m2)) {
+            const uint32_t pair = __float_as_uint(p.top[(size_t)ql * p.groups + gi].x) & 15u;
+            const uint32_t g0 = (uint32_t)gi * GROUP;
+            const uint32_t w = allowed_word(al, 0, 0, g0, p.n);
+            uint32_t rest = w & ~(3u << (2 * pair));
+            int at = atomicAdd(&s_cnt, __popc(rest));
+            while (rest) {
+                ci[at++] = g0 + (uint32_t)(__ffs(rest) - 1);
+                rest &= rest - 1;
+            }
+        }
+    }
+    __syncthreads();
+    const int all = s_cnt;
+    score(cnt, all);
+    __syncthreads();
+    // ---- written in order ----
+    for (int i = threadIdx.x; i < all; i += WARPS * 32) {
+        int rank = 0;
+        for (int j = 0; j < all; ++j) rank += before(j, i);
+        if (rank < p.k && bad == 0) {
+            p.top_ids[(size_t)q * p.k + rank] = (int64_t)ci[i];
+            p.top_logprob[(size_t)q * p.k + rank] = (float)(cs[i] * (double)p.scale - lse);
+        }
+    }
+    for (int i = (bad ? 0 : all) + (int)threadIdx.x; i < p.k; i += WARPS * 32) {
+        p.top_ids[(size_t)q * p.k + i] = -1;
+        p.top_logprob[(size_t)q * p.k + i] = bad == 2 ? NAN : -INFINITY;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// backward: what the products need
+// ---------------------------------------------------------------------------
+// Rows some query may see: the OR of the filters.
+__global__ void any_kernel(const uint32_t* __restrict__ allowed, size_t ld, int nq, size_t words,
+                           uint32_t* __restrict__ out) {
+    const size_t w = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (w >= words) return;
+    uint32_t r = 0;
+    for (int q = blockIdx.y; q < nq; q += gridDim.y) r |= allowed[(size_t)q * ld + w];
+    if (r) atomicOr(out + w, r);
+}
+// Queries that see anything, as bits (an empty one is taken as zeros, so that
+// what it holds cannot set the scale of the others).
+__global__ void alive_kernel(const float* __restrict__ lse, int nq, uint32_t* __restrict__ out) {
+    const int q = blockIdx.x * blockDim.x + threadIdx.x;
+    const bool on = q < nq && !(lse[q] == -INFINITY);
+    const unsigned b = __ballot_sync(0xffffffffu, on);
+    if ((threadIdx.x & 31) == 0 && q < nq) out[q >> 5] = b;
+}
+// The products sum over rows (or queries) whose scales 2^-e differ; the stored
+// score gradients carry the factor, so a row far below the largest would leave
+// too few bits there.  Such a row (below 2^-4 of the largest scale; also one
+// of zeros or with a NaN, whose elements are zeros) takes a larger scale and
+// is shifted down instead.  One warp per row, almost none has work.
+__global__ void __launch_bounds__(256)
+    fix_kernel(__half* __restrict__ x, float* __restrict__ f, int n, int width,
+               const float* __restrict__ largest) {
+    const int lane = threadIdx.x & 31;
+    const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= n) return;
+    const float mx = *largest, v = f[row];
+    if (!(mx > 0.0f)) {
+        if (lane == 0) f[row] = 1.0f;
+        return;
+    }
+    const float least = mx * 0x1p-4f;
+    if (v >= least) return;
+    if (v > 0.0f) {
+        const float s = v / least;
+        __half* h = x + (size_t)row * width;
+        for (int c = lane; c < width; c += 32) h[c] = __float2half_rn(__half2float(h[c]) * s);
+    }
+    __syncwarp();
+    if (lane == 0) f[row] = v > 0.0f ? least : mx;
+}
+struct CoefArgs {
+    int nq, n;
+    double scale;
+    const float *lse, *entropy, *d_logprob, *d_lse, *d_entropy;
+    const int64_t* targets;
+    const uint32_t* allowed;
+    size_t ld_allowed;
+    const float* qf;
+    Coef* out;
+    float* bounds;  // [0]
+};
+// G_ij = scale [ p_ij (dl - g - h (lp_ij + H)) + g 1{j = t} ] with lp = ln2 x:
+// = p (c + h' x) + g', and a bound of its size for the common scale
+// (p |lp| <= 1/e).
+__global__ void coef_kernel(const CoefArgs a) {
+    const int i = blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= a.nq) return;
+    const float lse = a.lse[i];
+    const bool empty = lse == -INFINITY;
+    const float f = a.qf[i];
+    const double rf = (double)f * a.scale * LOG2E, l = (double)lse * LOG2E;
+    const int64_t t = a.targets ? a.targets[i] : -1;
+    const bool given = !empty && t >= 0 && t < a.n &&
+                       (!a.allowed ||
+                        (a.allowed[(size_t)i * a.ld_allowed + (size_t)(t >> 5)] >> (t & 31) & 1u));
+    const double g = given && a.d_logprob ? a.d_logprob[i] : 0.0;
+    const double dl = !empty && a.d_lse ? a.d_lse[i] : 0.0;
+    const double dh = !empty && a.d_entropy ? a.d_entropy[i] : 0.0;
+    const double H = dh != 0.0 ? (double)a.entropy[i] : 0.0;
+    Coef k;
+    k.rf_hi = (float)rf;
+    k.rf_lo = (float)(rf - (double)k.rf_hi);
+    k.l_hi = empty ? INFINITY : (float)l;
+    k.l_lo = empty ? 0.0f : (float)(l - (double)k.l_hi);
+    k.c = lse == lse ? (float)(a.scale * (dl - g - dh * H)) : NAN;
+    k.h = (float)(-a.scale * dh * LN2);
+    k.g = (float)(a.scale * g);
+    k.target = given ? (int)t : -1;
+    a.out[i] = k;
+    const float b = (float)(a.scale * (fabs(dl) + 2.0 * fabs(g) + fabs(dh) * (fabs(H) + 1.0)) *
+                            (double)f);
+    if (b > 0.0f && b <= FLT_MAX)
+        atomicMax(reinterpret_cast<unsigned*>(a.bounds), __float_as_uint(b));
+}
+// Sum of the splits, scaled, in the output's type.
+__global__ void __launch_bounds__(256)
+    join_kernel(const float* __restrict__ partial, int splits, int rows, int cols,
+                const float* __restrict__ f, const float* __restrict__ bounds, void* out,
+                size_t ldo, int dtype) {
+    const size_t per = (size_t)rows * cols;
+    const float c = grad_factor(bounds);
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < per; i += (size_t)gridDim.x * 256) {
+        const size_t r = i / cols, k = i - r * cols;
+        float s = 0.0f;
+        for (int j = 0; j < splits; ++j) s += partial[(size_t)j * per + i];
+        s *= 1.0f / (f[r] * c);
+        const size_t o = r * ldo + k;
+        if (dtype == FDB_DTYPE_F32) static_cast<float*>(out)[o] = s;
+        else if (dtype == FDB_DTYPE_BF16)
+            static_cast<__nv_bfloat16*>(out)[o] = __float2bfloat16_rn(s);
+        else static_cast<__half*>(out)[o] = __float2half_rn(s);
+    }
+}
+// A call whose waits ran out has no gradient: NaN.
+__global__ void void_kernel(const int* err, void* out, size_t ldo, int rows, int cols, int dtype) {
+    if (*err == 0) return;
+    const size_t per = (size_t)rows * cols;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < per; i += (size_t)gridDim.x * 256) {
+        const size_t o = i / cols * ldo + i % cols;
+        if (dtype == FDB_DTYPE_F32) static_cast<float*>(out)[o] = NAN;
+        else static_cast<uint16_t*>(out)[o] = 0x7fff;  // NaN in both 16-bit types
+    }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+constexpr size_t HEAD = 256;                    // error word, bounds
+constexpr size_t CHUNK_BYTES = (size_t)512 << 20;  // of group maxima, of score gradients
+constexpr int FEW = 8;                          // f32 queries a pass of few_kernel takes
+constexpr int FEW_QUERIES = 16, FEW_DIM = 2048;
+static size_t smem_of(bool two) {
+    return 1024 + (size_t)stages_of(two) * stage_bytes(two) + (2 * MAX_STG + 2 * MAX_ACC) * 8 + 16;
+}
+
+static size_t up(size_t v, size_t m) { return (v + m - 1) / m * m; }
+static size_t elem(int dtype) { return dtype == FDB_DTYPE_F32 ? 4 : 2; }
+
+static CUtensorMap map2d(int dtype, const void* base, size_t inner, size_t rows, size_t ld_elems,
+                         int box_rows) {
+    CUtensorMap m;
+    cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld_elems * 2};
+    cuuint32_t box[2] = {(cuuint32_t)KATOM, (cuuint32_t)box_rows};
+    cuuint32_t one[2] = {1, 1};
+    const CUresult r = encode_fn()(
+        &m,
+        dtype == FDB_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+        2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    FDB_REQUIRE(r == CUDA_SUCCESS, FDB_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+    return m;
+}
+// D f32; A and B both f16 or both bf16; transposed operands; M = 128 (N is added
+// in the kernel).
+static uint32_t idesc_of(int dtype, bool a_mn, bool b_mn) {
+    const uint32_t t = dtype == FDB_DTYPE_BF16 ? 1u : 0u;
+    return (1u << 4) | (t << 7) | (t << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
+           ((uint32_t)(BM >> 4) << 24);
+}
+// Chunks of the column tiles: the count that leaves the busiest block the
+// fewest tiles, and of those the smallest.
+static int pick_chunks(int mt, int nt, int sms) {
+    sms = std::max(sms, 1);
+    int best = 1;
+    long long cost = -1;
+    for (int c = 1; c <= nt && c <= 4 * sms; ++c) {
+        const long long waves = ((long long)mt * c + sms - 1) / sms;
+        const long long t = waves * ((nt + c - 1) / c);
+        if (cost < 0 || t < cost) cost = t, best = c;
+    }
+    return best;
+}
+// Splits of K of a product with `tiles` output tiles: each costs a pass over
+// the partial sums, taken as 2% of the product.
+static int pick_splits(int tiles, int atoms, int sms) {
+    sms = std::max(sms, 1);
+    int best = 1;
+    double cost = -1.0;
+    for (int s = 1; s <= atoms && s <= 64; ++s) {
+        const long long waves = ((long long)tiles * s + sms - 1) / sms;
+        const double t = (double)waves * ((atoms + s - 1) / s) * (1.0 + 0.02 * (s - 1));
+        if (cost < 0.0 || t < cost) cost = t, best = s;
+    }
+    return best;
+}
+template <int MODE, bool TWO>
+static void launch_rows(cudaStream_t s, int sms, const CUtensorMap& a, const CUtensorMap& b,
+                        const Mma& g, const typename EpilogueOf<MODE, TWO>::Type::Args& p) {
+    const long long units = MODE == PROD_Q || MODE == PROD_X
+                                ? (long long)g.mt * g.nt * g.chunks
+                                : (long long)g.mt * g.chunks;
+    const size_t smem = smem_of(TWO);
+    FDB_CUDA(cudaFuncSetAttribute(rows_kernel<MODE, TWO>,
+                                  cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    rows_kernel<MODE, TWO>
+        <<<(unsigned)std::min<long long>(units, sms), THREADS, smem, s>>>(a, b, g, p);
+    FDB_LAUNCH_CHECK();
+}
+template <int MODE>
+static void launch_rows(bool two, cudaStream_t s, int sms, const CUtensorMap& a,
+                        const CUtensorMap& b, const Mma& g,
+                        const typename EpilogueOf<MODE, false>::Type::Args& p) {
+    if (two) launch_rows<MODE, true>(s, sms, a, b, g, p);
+    else launch_rows<MODE, false>(s, sms, a, b, g, p);
+}
+
+// Hands out 256-byte aligned parts of the caller's workspace.
+struct Carve {
+    unsigned char* base;
+    size_t at = 0;
+    explicit Carve(void* b) : base(static_cast<unsigned char*>(b)) {}
+    template <typename T>
+    T* take(size_t count) {
+        T* p = base ? reinterpret_cast<T*>(base + at) : nullptr;
+        at += up(count * sizeof(T), 256);
+        return p;
+    }
+};
+
+template <typename T, int PARTS>
+static void launch_pack(cudaStream_t s, const void* x, size_t ld, size_t n, size_t d, size_t kp,
+                        const uint32_t* seen, __half* out, float* f, unsigned* largest) {
+    pack_kernel<T, PARTS><<<(unsigned)((n + 7) / 8), 256, 0, s>>>(
+        static_cast<const T*>(x), ld, (int)n, (int)d, (int)kp, seen, out, f, largest);
+    FDB_LAUNCH_CHECK();
+}
+
+// The forward pass's workspace and launch shape.
+struct Forward {
+    bool few, packed, copy_q, copy_x;
+    size_t kp, qb, groups, parts_cap;
+    int bn, nt;
+    size_t bytes;
+    int* err;
+    void *qp, *xp;
+    float *qf, *xf;
+    float4* part;
+    float2* top;
+};
+static bool mappable(const void* p, size_t ld) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * 2 & 15) == 0;
+}
+static Forward plan_forward(const Ctx& c, const fdb_logprob_args& a) {
+    Forward w{};
+    Carve ws(a.workspace);
+    w.err = ws.take<int>(HEAD / 4);
+    w.few = a.dtype == FDB_DTYPE_F32 && a.nq <= FEW_QUERIES && a.dim <= FEW_DIM;
+    w.packed = a.dtype == FDB_DTYPE_F32 && !w.few;
+    w.kp = up(a.dim, 64);
+    w.bn = bn_of(w.packed);
+    w.nt = (int)((a.n + w.bn - 1) / w.bn);
+    w.groups = w.few ? (a.n + GROUP - 1) / GROUP : (size_t)w.nt * (w.bn / GROUP);
+    const size_t per = a.k ? w.groups * sizeof(float2) : 0;
+    w.qb = std::min<size_t>(a.nq, w.few ? (size_t)FEW
+                                  : per ? std::max<size_t>(BM, CHUNK_BYTES / per / BM * BM)
+                                        : (size_t)1 << 20);
+    if (w.packed) {
+        w.qp = ws.take<__half>(a.nq * 2 * w.kp);
+        w.xp = ws.take<__half>(a.n * 2 * w.kp);
+        w.qf = ws.take<float>(a.nq);
+        w.xf = ws.take<float>((size_t)w.nt * w.bn);
+    } else if (!w.few) {
+        w.copy_q = !mappable(a.queries, a.ld_queries);
+        w.copy_x = !mappable(a.rows, a.ld_rows);
+        if (w.copy_q) w.qp = ws.take<__half>(a.nq * w.kp);
+        if (w.copy_x) w.xp = ws.take<__half>(a.n * w.kp);
+    }
+    if (w.few) {
+        w.parts_cap = std::min<size_t>((w.groups + 1) / 2, (size_t)c.sm_count * 12);
+    } else {
+        // (the last pass has fewer row blocks and may take more chunks)
+        const int full = (int)((w.qb + BM - 1) / BM);
+        w.parts_cap = 0;
+        for (int mt = 1; mt <= full; ++mt)
+            if (mt == full || mt == (int)((a.nq % w.qb + BM - 1) / BM))
+                w.parts_cap = std::max<size_t>(w.parts_cap,
+                                               4 * (size_t)pick_chunks(mt, w.nt, c.sm_count));
+    }
+    w.part = ws.take<float4>(w.parts_cap * w.qb);
+    if (a.k) w.top = ws.take<float2>(w.qb * w.groups);
+    w.bytes = ws.at;
+    return w;
+}
+size_t forward_bytes(const Ctx& c, const fdb_logprob_args& a) {
+    fdb_logprob_args b = a;
+    b.workspace = nullptr;
+    return plan_forward(c, b).bytes;
+}
+
+template <typename T>
+static void launch_finish(cudaStream_t s, const FinishArgs& f) {
+    // A block a query.  Few queries: sixteen warps share the groups of one.
+    if (f.nq <= 64)
+        finish_kernel<T, 16><<<f.nq, 512, 0, s>>>(f);
+    else
+        finish_kernel<T, 4><<<f.nq, 128, 0, s>>>(f);
+    FDB_LAUNCH_CHECK();
+}
+
+void forward_run(Ctx& c, const fdb_logprob_args& a) {
+    const cudaStream_t s = static_cast<cudaStream_t>(a.stream);
+    const Forward w = plan_forward(c, a);
+    const int n = (int)a.n, d = (int)a.dim;
+    const float rf = (float)((double)a.scale * LOG2E);
+    const size_t ld_allowed = a.allowed ? a.ld_allowed : 0;
+    Mma g{};
+    CUtensorMap amap, bmap;
+    if (!w.few) {
+        FDB_CUDA(cudaMemsetAsync(w.err, 0, HEAD, s));
+        const void *qb = a.queries, *xb = a.rows;
+        size_t ldq = a.ld_queries, ldx = a.ld_rows, inner = a.dim;
+        if (w.packed) {
+            launch_pack<float, 2>(s, a.queries, a.ld_queries, a.nq, a.dim, w.kp, nullptr,
+                                  static_cast<__half*>(w.qp), w.qf, nullptr);
+            launch_pack<float, 2>(s, a.rows, a.ld_rows, a.n, a.dim, w.kp, nullptr,
+                                  static_cast<__half*>(w.xp), w.xf, nullptr);
+            qb = w.qp, xb = w.xp;
+            ldq = ldx = inner = 2 * w.kp;
+        }
+        if (w.copy_q) {
+            align_kernel<<<(unsigned)((a.nq + 7) / 8), 256, 0, s>>>(
+                static_cast<const uint16_t*>(a.queries), a.ld_queries, (int)a.nq, d, (int)w.kp,
+                static_cast<uint16_t*>(w.qp));
+            FDB_LAUNCH_CHECK();
+            qb = w.qp, ldq = w.kp;
+        }
+        if (w.copy_x) {
+            align_kernel<<<(unsigned)((a.n + 7) / 8), 256, 0, s>>>(
+                static_cast<const uint16_t*>(a.rows), a.ld_rows, n, d, (int)w.kp,
+                static_cast<uint16_t*>(w.xp));
+            FDB_LAUNCH_CHECK();
+            xb = w.xp, ldx = w.kp;
+        }
+        bmap = map2d(a.dtype, xb, inner, a.n, ldx, 128);
+        g.nt = w.nt;
+        g.atoms = (int)(w.kp / 64);
+        g.klast = (int)((a.dim - 64 * (w.kp / 64 - 1) + 15) / 16);
+        g.a_part = g.b_part = (int)w.kp;
+        g.idesc = idesc_of(w.packed ? FDB_DTYPE_F16 : a.dtype, false, false);
+        g.err = w.err;
+        g.wait = wait_limit_cycles(c);
+        g.stall = take_test_stall(c);
+        for (size_t q0 = 0; q0 < a.nq; q0 += w.qb) {
+            const size_t nq = std::min(w.qb, a.nq - q0);
+            g.mt = (int)((nq + BM - 1) / BM);
+            g.chunks = pick_chunks(g.mt, w.nt, c.sm_count);
+            amap = map2d(a.dtype,
+                         static_cast<const unsigned char*>(qb) + q0 * ldq * 2, inner, nq, ldq, BM);
+            StatsArgs p{};
+            p.q0 = (int)q0;
+            p.nq = (int)nq;
+            p.n = n;
+            p.qf = w.packed ? w.qf + q0 : nullptr;
+            p.xf = w.xf;
+            p.rf = rf;
+            p.allowed = a.allowed;
+            p.ld_allowed = ld_allowed;
+            p.part = w.part;
+            p.top = w.top;
+            p.groups = w.groups;
+            launch_rows<STATS>(w.packed, s, c.sm_count, amap, bmap, g, p);
+            FinishArgs f{};
+            f.q = a.queries, f.x = a.rows;
+            f.ldq = a.ld_queries, f.ldx = a.ld_rows;
+            f.q0 = (int)q0, f.nq = (int)nq, f.n = n, f.d = d, f.k = (int)a.k;
+            f.scale = a.scale;
+            f.targets = a.targets;
+            f.allowed = a.allowed, f.ld_allowed = ld_allowed;
+            f.part = w.part, f.parts = g.chunks * 4;
+            f.qf = p.qf;
+            f.top = w.top, f.groups = w.groups;
+            f.logprob = a.logprob, f.lse = a.lse, f.entropy = a.entropy;
+            f.top_logprob = a.top_logprobs, f.top_ids = a.top_ids;
+            f.err = w.err;
+            if (a.dtype == FDB_DTYPE_F32) launch_finish<float>(s, f);
+            else if (a.dtype == FDB_DTYPE_F16) launch_finish<__half>(s, f);
+            else launch_finish<__nv_bfloat16>(s, f);
+        }
+        return;
+    }
+    const bool vec = (reinterpret_cast<uintptr_t>(a.rows) & 15) == 0 && a.ld_rows % 4 == 0 &&
+                     a.dim % 4 == 0;
+    const size_t dp = up(a.dim, 128);
+    for (size_t q0 = 0; q0 < a.nq; q0 += w.qb) {
+        const int nq = (int)std::min(w.qb, a.nq - q0);
+        const unsigned blocks = (unsigned)w.parts_cap;
+        auto go = [&](auto kernel, int NQ) {
+            const size_t sm = NQ * dp * 4;
+            FDB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          (int)sm));
+            kernel<<<blocks, 64, sm, s>>>(static_cast<const float*>(a.rows), a.ld_rows, n, d,
+                                          static_cast<const float*>(a.queries), a.ld_queries,
+                                          (int)q0, nq, rf, a.allowed, ld_allowed, w.part, w.top,
+                                          w.groups);
+            FDB_LAUNCH_CHECK();
+        };
+        if (nq == 1) vec ? go(few_kernel<1, true>, 1) : go(few_kernel<1, false>, 1);
+        else if (nq == 2) vec ? go(few_kernel<2, true>, 2) : go(few_kernel<2, false>, 2);
+        else if (nq <= 4) vec ? go(few_kernel<4, true>, 4) : go(few_kernel<4, false>, 4);
+        else vec ? go(few_kernel<8, true>, 8) : go(few_kernel<8, false>, 8);
+        FinishArgs f{};
+        f.q = a.queries, f.x = a.rows;
+        f.ldq = a.ld_queries, f.ldx = a.ld_rows;
+        f.q0 = (int)q0, f.nq = nq, f.n = n, f.d = d, f.k = (int)a.k;
+        f.scale = a.scale;
+        f.targets = a.targets;
+        f.allowed = a.allowed, f.ld_allowed = ld_allowed;
+        f.part = w.part, f.parts = (int)blocks;
+        f.top = w.top, f.groups = w.groups;
+        f.logprob = a.logprob, f.lse = a.lse, f.entropy = a.entropy;
+        f.top_logprob = a.top_logprobs, f.top_ids = a.top_ids;
+        launch_finish<float>(s, f);
+    }
+}
+
+// ---- backward ----
+struct Backward {
+    int parts;
+    size_t kp, nqp, cols, ldg;  // cols: rows of a chunk
+    int bn, q_splits, x_splits;
+    size_t bytes;
+    int* err;
+    float* bounds;
+    __half *qp, *xp, *gr;
+    float *qf, *xf, *dq, *dx;
+    Coef* coef;
+    uint32_t *seen, *alive;
+};
+static Backward plan_backward(const Ctx& c, const fdb_logprob_grad_args& a) {
+    Backward w{};
+    Carve ws(a.workspace);
+    w.parts = a.dtype == FDB_DTYPE_F32 ? 2 : 1;
+    w.kp = up(a.dim, 64);
+    w.nqp = up(a.nq, BM);
+    w.bn = bn_of(w.parts == 2);
+    const size_t row_bytes = w.nqp * 2 * w.parts;
+    w.cols = std::min<size_t>(std::max<size_t>(MAX_BN, CHUNK_BYTES / row_bytes / MAX_BN * MAX_BN),
+                              a.n);
+    w.ldg = up(w.cols, 64);
+    const int ntd = (int)((a.dim + w.bn - 1) / w.bn);
+    w.q_splits = pick_splits((int)(w.nqp / BM) * ntd, (int)((w.cols + 63) / 64), c.sm_count);
+    w.x_splits = pick_splits((int)((w.cols + BM - 1) / BM) * ntd, (int)((a.nq + 63) / 64),
+                             c.sm_count);
+    unsigned char* head = ws.take<unsigned char>(HEAD);
+    w.err = reinterpret_cast<int*>(head);
+    w.bounds = reinterpret_cast<float*>(head ? head + 64 : nullptr);
+    w.qp = ws.take<__half>(a.nq * w.parts * w.kp);
+    w.xp = ws.take<__half>(a.n * w.parts * w.kp);
+    w.qf = ws.take<float>(a.nq);
+    w.xf = ws.take<float>(up(a.n, MAX_BN) + MAX_BN);
+    w.coef = ws.take<Coef>(a.nq);
+    w.gr = ws.take<__half>((size_t)w.parts * w.nqp * w.ldg);
+    w.dq = ws.take<float>((size_t)w.q_splits * a.nq * a.dim);
+    if (w.x_splits > 1) w.dx = ws.take<float>((size_t)w.x_splits * w.cols * a.dim);
+    w.alive = ws.take<uint32_t>((a.nq + 31) / 32);
+    if (a.allowed && a.ld_allowed) w.seen = ws.take<uint32_t>((a.n + 31) / 32);
+    w.bytes = ws.at;
+    return w;
+}
+size_t backward_bytes(const Ctx& c, const fdb_logprob_grad_args& a) {
+    fdb_logprob_grad_args b = a;
+    b.workspace = nullptr;
+    return plan_backward(c, b).bytes;
+}
+
+void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
+    const cudaStream_t s = static_cast<cudaStream_t>(a.stream);
+    const Backward w = plan_backward(c, a);
+    const int n = (int)a.n, d = (int)a.dim, nq = (int)a.nq;
+    const size_t ld_allowed = a.allowed ? a.ld_allowed : 0;
+    FDB_CUDA(cudaMemsetAsync(w.err, 0, HEAD, s));
+    const uint32_t* seen = a.allowed;
+    if (w.seen) {
+        const size_t words = (a.n + 31) / 32;
+        FDB_CUDA(cudaMemsetAsync(w.seen, 0, words * 4, s));
+        const unsigned gx = (unsigned)((words + 255) / 256);
+        any_kernel<<<dim3(gx, (unsigned)std::min<size_t>(a.nq, std::max(1u, 1184 / gx))), 256, 0,
+                     s>>>(a.allowed, a.ld_allowed, nq, words, w.seen);
+        FDB_LAUNCH_CHECK();
+        seen = w.seen;
+    }
+    alive_kernel<<<(nq + 255) / 256, 256, 0, s>>>(a.lse, nq, w.alive);
+    FDB_LAUNCH_CHECK();
+    unsigned* qmax = reinterpret_cast<unsigned*>(w.bounds + 2);
+    unsigned* xmax = reinterpret_cast<unsigned*>(w.bounds + 1);
+    auto pack = [&](const void* x, size_t ld, size_t rows, const uint32_t* bits, __half* out,
+                    float* f, unsigned* mx) {
+        if (a.dtype == FDB_DTYPE_F32)
+            launch_pack<float, 2>(s, x, ld, rows, a.dim, w.kp, bits, out, f, mx);
+        else if (a.dtype == FDB_DTYPE_F16)
+            launch_pack<__half, 1>(s, x, ld, rows, a.dim, w.kp, bits, out, f, mx);
+        else
+            launch_pack<__nv_bfloat16, 1>(s, x, ld, rows, a.dim, w.kp, bits, out, f, mx);
+        fix_kernel<<<(unsigned)((rows + 7) / 8), 256, 0, s>>>(out, f, (int)rows,
+                                                              w.parts * (int)w.kp,
+                                                              reinterpret_cast<float*>(mx));
+        FDB_LAUNCH_CHECK();
+    };
+    pack(a.queries, a.ld_queries, a.nq, w.alive, w.qp, w.qf, qmax);
+    pack(a.rows, a.ld_rows, a.n, seen, w.xp, w.xf, xmax);
+    CoefArgs k{};
+    k.nq = nq, k.n = n, k.scale = a.scale;
+    k.lse = a.lse, k.entropy = a.entropy;
+    k.d_logprob = a.d_logprob, k.d_lse = a.d_lse, k.d_entropy = a.d_entropy;
+    k.targets = a.targets, k.allowed = a.allowed, k.ld_allowed = ld_allowed;
+    k.qf = w.qf, k.out = w.coef, k.bounds = w.bounds;
+    coef_kernel<<<(nq + 255) / 256, 256, 0, s>>>(k);
+    FDB_LAUNCH_CHECK();
+
+    const size_t width = w.parts * w.kp;
+    const bool two = w.parts == 2;
+    const int mtq = (int)(w.nqp / BM), ntd = (d + w.bn - 1) / w.bn;
+    const CUtensorMap qk = map2d(FDB_DTYPE_F16, w.qp, width, a.nq, width, BM);
+    const CUtensorMap xk = map2d(FDB_DTYPE_F16, w.xp, width, a.n, width, 128);
+    const CUtensorMap qm = map2d(FDB_DTYPE_F16, w.qp, width, a.nq, width, 64);
+    const CUtensorMap xm = map2d(FDB_DTYPE_F16, w.xp, width, a.n, width, 64);
+    const size_t g_rows = w.parts * w.nqp;
+    const CUtensorMap gk = map2d(FDB_DTYPE_F16, w.gr, w.ldg, g_rows, w.ldg, BM);
+    const CUtensorMap gm = map2d(FDB_DTYPE_F16, w.gr, w.ldg, g_rows, w.ldg, 64);
+    Mma base{};
+    base.err = w.err;
+    base.wait = wait_limit_cycles(c);
+    base.stall = take_test_stall(c);
+    for (size_t j0 = 0; j0 < a.n; j0 += w.cols) {
+        const int cols = (int)std::min(w.cols, a.n - j0);
+        {
+            Mma g = base;
+            g.mt = mtq;
+            g.nt = (cols + w.bn - 1) / w.bn;
+            g.chunks = pick_chunks(g.mt, g.nt, c.sm_count);
+            g.atoms = (int)(w.kp / 64);
+            g.klast = (int)((a.dim - 64 * (w.kp / 64 - 1) + 15) / 16);
+            g.a_part = g.b_part = (int)w.kp;
+            g.b_row0 = (int)j0;
+            g.idesc = idesc_of(FDB_DTYPE_F16, false, false);
+            GradArgs p{};
+            p.nq = nq, p.n = n, p.j0 = (int)j0, p.cols = cols;
+            p.coef = w.coef, p.qf = w.qf, p.xf = w.xf, p.bounds = w.bounds;
+            p.allowed = a.allowed, p.ld_allowed = ld_allowed;
+            p.out = w.gr, p.ldg = w.ldg, p.plane = w.nqp * w.ldg;
+            launch_rows<GRAD>(two, s, c.sm_count, qk, xk, g, p);
+        }
+        if (a.d_queries) {
+            Mma g = base;
+            g.mt = mtq, g.nt = ntd;
+            g.atoms = (cols + 63) / 64;
+            g.klast = 4;
+            g.chunks = std::min(w.q_splits, g.atoms);
+            g.a_part = (int)w.nqp, g.b_part = (int)w.kp;
+            g.b_row0 = (int)j0;
+            g.ncols = d;
+            g.idesc = idesc_of(FDB_DTYPE_F16, false, true);
+            ProdArgs p{};
+            p.rows = nq, p.cols = d, p.f = w.qf, p.bounds = w.bounds;
+            p.partial = w.dq, p.add = j0 > 0;
+            launch_rows<PROD_Q>(two, s, c.sm_count, gk, xm, g, p);
+        }
+        if (a.d_rows) {
+            Mma g = base;
+            g.mt = (cols + BM - 1) / BM, g.nt = ntd, g.chunks = w.x_splits;
+            g.atoms = (nq + 63) / 64;
+            g.klast = 4;
+            g.a_part = (int)w.nqp, g.b_part = (int)w.kp;
+            g.ncols = d;
+            g.idesc = idesc_of(FDB_DTYPE_F16, true, true);
+            unsigned char* out =
+                static_cast<unsigned char*>(a.d_rows) + j0 * a.ld_d_rows * elem(a.dtype);
+            ProdArgs p{};
+            p.rows = cols, p.cols = d, p.f = w.xf + j0, p.bounds = w.bounds;
+            p.partial = w.dx;
+            p.out = out, p.ldo = a.ld_d_rows, p.dtype = a.dtype;
+            launch_rows<PROD_X>(two, s, c.sm_count, gm, qm, g, p);
+            if (w.dx) {
+                join_kernel<<<c.sm_count * 8, 256, 0, s>>>(w.dx, w.x_splits, cols, d, w.xf + j0,
+                                                           w.bounds, out, a.ld_d_rows, a.dtype);
+                FDB_LAUNCH_CHECK();
+            }
+        }
+    }
+    if (a.d_queries) {
+        join_kernel<<<c.sm_count * 8, 256, 0, s>>>(w.dq, w.q_splits, nq, d, w.qf, w.bounds,
+                                                   a.d_queries, a.ld_d_queries, a.dtype);
+        FDB_LAUNCH_CHECK();
+        void_kernel<<<c.sm_count, 256, 0, s>>>(w.err, a.d_queries, a.ld_d_queries, nq, d, a.dtype);
+        FDB_LAUNCH_CHECK();
+    }
+    if (a.d_rows) {
+        void_kernel<<<c.sm_count, 256, 0, s>>>(w.err, a.d_rows, a.ld_d_rows, n, d, a.dtype);
+        FDB_LAUNCH_CHECK();
+    }
+}
+
+// One thread per row: its id among the sorted wanted ones, the lowest row kept.
+__global__ void find_rows_kernel(const uint64_t* __restrict__ ids, size_t n,
+                                 const uint64_t* __restrict__ sorted, size_t count,
+                                 unsigned long long* __restrict__ slot) {
+    const size_t j = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (j >= n) return;
+    const uint64_t id = ids[j];
+    size_t lo = 0, hi = count;
+    while (lo < hi) {
+        const size_t mid = (lo + hi) >> 1;
+        if (sorted[mid] < id) lo = mid + 1;
+        else hi = mid;
+    }
+    if (lo < count && sorted[lo] == id) atomicMin(slot + lo, (unsigned long long)j);
+}
+void launch_find_rows(cudaStream_t s, const uint64_t* ids, size_t n, const uint64_t* sorted,
+                      size_t count, unsigned long long* slot) {
+    find_rows_kernel<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(ids, n, sorted, count, slot);
+    FDB_LAUNCH_CHECK();
+}
+
+}  // namespace sr
+}  // namespace fdb

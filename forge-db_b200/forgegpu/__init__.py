@@ -14,6 +14,7 @@ if the library is missing or no B200 is visible, calls raise ForgeGpuError.
 """
 from __future__ import annotations
 
+import collections
 import ctypes as C
 import os
 import threading
@@ -89,9 +90,55 @@ class TrainOpts(C.Structure):
                 ("pq_init_idx", C.c_void_p), ("seed", C.c_uint64)]
 
 
+class LogprobArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("queries", C.c_void_p), ("nq", C.c_size_t),
+                ("ld_queries", C.c_size_t), ("rows", C.c_void_p), ("n", C.c_size_t),
+                ("ld_rows", C.c_size_t), ("dim", C.c_size_t), ("scale", C.c_float),
+                ("targets", C.c_void_p), ("allowed", C.c_void_p), ("ld_allowed", C.c_size_t),
+                ("k", C.c_size_t), ("logprob", C.c_void_p), ("lse", C.c_void_p),
+                ("entropy", C.c_void_p), ("top_ids", C.c_void_p), ("top_logprobs", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+                ("stream", C.c_void_p)]
+
+
+class LogprobGradArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("queries", C.c_void_p), ("nq", C.c_size_t),
+                ("ld_queries", C.c_size_t), ("rows", C.c_void_p), ("n", C.c_size_t),
+                ("ld_rows", C.c_size_t), ("dim", C.c_size_t), ("scale", C.c_float),
+                ("targets", C.c_void_p), ("allowed", C.c_void_p), ("ld_allowed", C.c_size_t),
+                ("lse", C.c_void_p), ("entropy", C.c_void_p), ("d_logprob", C.c_void_p),
+                ("d_lse", C.c_void_p), ("d_entropy", C.c_void_p), ("d_queries", C.c_void_p),
+                ("ld_d_queries", C.c_size_t), ("d_rows", C.c_void_p), ("ld_d_rows", C.c_size_t),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+                ("stream", C.c_void_p)]
+
+
+class AdamwTensor(C.Structure):
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("m", C.c_void_p),
+                ("v", C.c_void_p), ("m_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("n", C.c_size_t)]
+
+
+class AdamwOpts(C.Structure):
+    _fields_ = [("param_dtype", C.c_int), ("grad_dtype", C.c_int), ("state_bits", C.c_int),
+                ("seed", C.c_uint32), ("lr", C.c_double), ("beta1", C.c_double),
+                ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double),
+                ("grad_scale", C.c_double), ("step", C.c_int64), ("d_lr", C.c_void_p),
+                ("d_step", C.c_void_p), ("d_grad_scale", C.c_void_p), ("stream", C.c_void_p)]
+
+
 _vp = C.c_void_p
 _sz = C.c_size_t
 _SIGS = {
+    "fdb_logprobs_workspace": (C.c_int, [_vp, C.POINTER(LogprobArgs), C.POINTER(_sz)]),
+    "fdb_logprobs": (C.c_int, [_vp, C.POINTER(LogprobArgs)]),
+    "fdb_logprobs_backward_workspace": (C.c_int, [_vp, C.POINTER(LogprobGradArgs),
+                                                  C.POINTER(_sz)]),
+    "fdb_logprobs_backward": (C.c_int, [_vp, C.POINTER(LogprobGradArgs)]),
+    "fdb_logprobs_status": (C.c_int, [_vp, _vp, _vp]),
+    "fdb_bf_logprobs": (C.c_int, [_vp, _vp, _sz, C.c_float, _vp, _sz, _vp, _vp, _vp, _vp, _vp]),
+    "fdb_adamw_step": (C.c_int, [_vp, _vp, _sz, C.POINTER(AdamwOpts)]),
+    "fdb_adamw_state_values": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp, _vp]),
     "fdb_last_error": (C.c_char_p, []),
     "fdb_version": (C.c_int, []),
     "fdb_ctx_create": (C.c_int, [C.c_int, C.POINTER(_vp)]),
@@ -810,6 +857,25 @@ class BruteForceIndex:
         ids, d, cnt = self.batch_search_arrays(queries, k)
         return _results(ids, d, cnt)
 
+    def log_probs(self, queries, target_ids=None, temperature: float = 1.0, k: int = 0):
+        """What the dot products are as probabilities over all vectors,
+        p(x | q) proportional to exp(q . x / temperature): a LogProbs of
+        arrays, with the log probability of target_ids[i] under query i (0
+        for an id the index does not hold), and the k most probable ids."""
+        Q = _f32(queries)
+        nq = Q.shape[0]
+        if Q.ndim != 2 or (self.len() and Q.shape[1] != self.dimension()):
+            raise ForgeGpuError(-2, f"queries of shape {Q.shape} on an index of dimension "
+                                    f"{self.dimension()}")
+        t = None if target_ids is None else np.ascontiguousarray(target_ids, np.uint64)
+        if t is not None and t.shape != (nq,):
+            raise ForgeGpuError(-2, f"{t.shape} target ids for {nq} queries")
+        lp, lse, ent = (np.empty(nq, np.float32) for _ in range(3))
+        ids, tlp = np.empty((nq, k), np.uint64), np.empty((nq, k), np.float32)
+        _check(lib().fdb_bf_logprobs(self.h, _p(Q), nq, float(temperature), _p(t), k, _p(lp),
+                                     _p(lse), _p(ent), _p(ids), _p(tlp)))
+        return LogProbs(lp, lse, ent, ids, tlp)
+
     def remove(self, id_: int) -> bool:
         out = C.c_int(0)
         _check(lib().fdb_bf_remove(self.h, int(id_), C.byref(out)))
@@ -842,3 +908,222 @@ class BruteForceIndex:
             self.close()
         except Exception:
             pass
+
+
+# ---------------------------------------------------------------------------
+# device operators on torch tensors: softmax over rows, AdamW
+# ---------------------------------------------------------------------------
+LogProbs = collections.namedtuple("LogProbs", "logprob lse entropy top_ids top_logprobs")
+_device_ctx: dict = {}
+_DTYPE: dict = {}
+
+
+def _torch():
+    import torch
+    if not _DTYPE:
+        _DTYPE.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+    return torch
+
+
+def _ctx_of(device) -> Context:
+    """The context of a tensor's device (made once per device)."""
+    i = device.index
+    with _lock:
+        c = _device_ctx.get(i)
+    if c is None:
+        c = default_context() if i == 0 else Context(i)
+        with _lock:
+            c = _device_ctx.setdefault(i, c)
+    return c
+
+
+def _refuse(msg: str):
+    raise ForgeGpuError(-1, msg)
+
+
+def _matrix(t, what: str, like=None):
+    """(pointer, rows, row distance) of a 2-d tensor whose rows are contiguous."""
+    if t.dim() != 2 or t.device.type != "cuda" or t.dtype not in _DTYPE:
+        _refuse(f"{what} must be a 2-d float32, float16 or bfloat16 tensor on a GPU")
+    n, d = t.shape
+    s0, s1 = t.stride()
+    if (s1 != 1 and d > 1) or (n > 1 and s0 < d):
+        _refuse(f"{what} must have contiguous rows")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        _refuse(f"{what} must have the queries' type and device")
+    return t.data_ptr(), n, s0 if n > 1 else max(s0, d)
+
+
+def _vector(t, n: int, dtype, like, what: str):
+    if t is None:
+        return None
+    if t.dtype != dtype or t.device != like.device or t.shape != (n,) or not t.is_contiguous():
+        _refuse(f"{what} must be a contiguous {dtype} tensor of {n} values on the queries' device")
+    return t.data_ptr()
+
+
+def _softmax_args(a, q, x, targets, scale, allowed):
+    torch = _torch()
+    a.queries, a.nq, a.ld_queries = _matrix(q, "queries")
+    a.rows, a.n, a.ld_rows = _matrix(x, "rows", q)
+    a.dtype = _DTYPE[q.dtype]
+    a.dim = q.shape[1]
+    if x.shape[1] != a.dim:
+        raise ForgeGpuError(-2, f"queries of {a.dim} and rows of {x.shape[1]} dimensions")
+    a.scale = scale
+    a.targets = _vector(targets, a.nq, torch.int64, q, "targets")
+    if allowed is not None:
+        words = (a.n + 31) // 32
+        if allowed.dtype != torch.int32 or allowed.device != q.device or allowed.dim() not in (1, 2) \
+                or allowed.shape[-1] != words or (words > 1 and allowed.stride(-1) != 1):
+            _refuse(f"allowed must be int32 words [{words}] or [1 or nq, {words}] on the "
+                    "queries' device")
+        rows = 1 if allowed.dim() == 1 else allowed.shape[0]
+        if rows not in (1, a.nq):
+            _refuse(f"allowed has {rows} filters for {a.nq} queries")
+        a.allowed = allowed.data_ptr()
+        if rows > 1:
+            if allowed.stride(0) < words:
+                _refuse("allowed must have contiguous rows")
+            a.ld_allowed = allowed.stride(0)
+    a.stream = torch.cuda.current_stream(q.device).cuda_stream
+    return torch
+
+
+def logprobs(queries, rows, targets=None, *, scale: float = 1.0, allowed=None, k: int = 0,
+             workspace=None) -> LogProbs:
+    """Log probabilities under softmax(scale * queries @ rows.T), on the current
+    stream, without the [nq, n] scores (fdb_logprobs in forgegpu.h).
+
+    targets: int64 [nq], the row whose log probability is wanted (none where
+    negative).  allowed: int32 words of a bit per row, one filter or one per
+    query.  k: number of alternatives.  workspace: a uint8 tensor to use
+    instead of a new one (fdb_logprobs_status reads a timeout from it)."""
+    a = LogprobArgs()
+    torch = _softmax_args(a, queries, rows, targets, scale, allowed)
+    ctx = _ctx_of(queries.device)
+    L = lib()
+    a.k = k
+    need = _sz()
+    _check(L.fdb_logprobs_workspace(ctx.h, C.byref(a), C.byref(need)))
+    dev, nq = queries.device, a.nq
+    out = torch.empty((3, nq), dtype=torch.float32, device=dev)
+    ids = torch.empty((nq, k), dtype=torch.int64, device=dev)
+    top = torch.empty((nq, k), dtype=torch.float32, device=dev)
+    ws = workspace if workspace is not None else torch.empty(need.value, dtype=torch.uint8,
+                                                             device=dev)
+    base = out.data_ptr()
+    a.logprob, a.lse, a.entropy = base, base + 4 * nq, base + 8 * nq
+    a.top_ids, a.top_logprobs = ids.data_ptr(), top.data_ptr()
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    _check(L.fdb_logprobs(ctx.h, C.byref(a)))
+    return LogProbs(out[0], out[1], out[2], ids, top)
+
+
+def logprobs_backward(queries, rows, targets, lse, entropy=None, *, d_logprob=None, d_lse=None,
+                      d_entropy=None, scale: float = 1.0, allowed=None,
+                      need_queries: bool = True, need_rows: bool = True, workspace=None):
+    """(d_queries, d_rows) of a loss from its gradients with respect to what
+    logprobs returned; lse and entropy are that call's (fdb_logprobs_backward
+    in forgegpu.h).  A gradient that is not needed is None."""
+    a = LogprobGradArgs()
+    torch = _softmax_args(a, queries, rows, targets, scale, allowed)
+    f32 = torch.float32
+    a.lse = _vector(lse, a.nq, f32, queries, "lse")
+    a.entropy = _vector(entropy, a.nq, f32, queries, "entropy")
+    a.d_logprob = _vector(d_logprob, a.nq, f32, queries, "d_logprob")
+    a.d_lse = _vector(d_lse, a.nq, f32, queries, "d_lse")
+    a.d_entropy = _vector(d_entropy, a.nq, f32, queries, "d_entropy")
+    ctx = _ctx_of(queries.device)
+    L = lib()
+    need = _sz()
+    _check(L.fdb_logprobs_backward_workspace(ctx.h, C.byref(a), C.byref(need)))
+    dev = queries.device
+    dq = torch.empty((a.nq, a.dim), dtype=queries.dtype, device=dev) if need_queries else None
+    dx = torch.empty((a.n, a.dim), dtype=queries.dtype, device=dev) if need_rows else None
+    ws = workspace if workspace is not None else torch.empty(need.value, dtype=torch.uint8,
+                                                             device=dev)
+    if dq is not None:
+        a.d_queries, a.ld_d_queries = dq.data_ptr(), a.dim
+    if dx is not None:
+        a.d_rows, a.ld_d_rows = dx.data_ptr(), a.dim
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    _check(L.fdb_logprobs_backward(ctx.h, C.byref(a)))
+    return dq, dx
+
+
+def logprobs_status(workspace):
+    """Raises Timeout if a kernel wait of the last call with this workspace
+    ran out (waits for the current stream)."""
+    torch = _torch()
+    ctx = _ctx_of(workspace.device)
+    _check(lib().fdb_logprobs_status(ctx.h, workspace.data_ptr(),
+                                     torch.cuda.current_stream(workspace.device).cuda_stream))
+
+
+def _scalar(t, dtype, like, what: str):
+    if t is None:
+        return None
+    if t.dtype != dtype or t.device != like.device or t.numel() != 1:
+        _refuse(f"{what} must be one {dtype} value on the params' device")
+    return t.data_ptr()
+
+
+def adamw_step(params, grads, m, v, *, lr: float, step: int = 1, betas=(0.9, 0.999),
+               eps: float = 1e-8, weight_decay: float = 0.01, grad_scale: float = 1.0,
+               m_scales=None, v_scales=None, seed: int = 0, d_lr=None, d_step=None,
+               d_grad_scale=None):
+    """One AdamW step in place over lists of tensors, on the current stream
+    (fdb_adamw_step in forgegpu.h).  With m_scales and v_scales the moments
+    are 8-bit: m int8, v uint8, a float32 scale per 256 elements each."""
+    torch = _torch()
+    count = len(params)
+    eight = m_scales is not None or v_scales is not None
+    lists = [params, grads, m, v] + ([m_scales, v_scales] if eight else [])
+    if any(x is None or len(x) != count for x in lists):
+        _refuse("params, grads and states must be lists of one length")
+    if count == 0:
+        return
+    p0, g0 = params[0], grads[0]
+    dev = p0.device
+    if dev.type != "cuda" or p0.dtype not in _DTYPE or g0.dtype not in _DTYPE:
+        _refuse("params and grads must be float32, float16 or bfloat16 tensors on a GPU")
+    types = [p0.dtype, g0.dtype] + ([torch.int8, torch.uint8, torch.float32, torch.float32]
+                                    if eight else [torch.float32, torch.float32])
+    sizes = [t.numel() for t in params]
+    blocks = [(n + 255) // 256 for n in sizes] if eight else None
+    for what, (ts, dtype) in enumerate(zip(lists, types)):
+        for t, n in zip(ts, sizes if what < 4 else blocks):
+            if t.dtype != dtype or t.device != dev or t.numel() != n or not t.is_contiguous():
+                _refuse("params, grads and states must be contiguous, of one type each, of the "
+                        "params' sizes (scales: one per 256 elements) and device")
+    table = np.zeros((count, 7), np.uint64)
+    for col, ts in enumerate(lists):
+        table[:, col] = [t.data_ptr() for t in ts]
+    table[:, 6] = sizes
+    o = AdamwOpts(_DTYPE[p0.dtype], _DTYPE[g0.dtype], 8 if eight else 32, seed & 0xFFFFFFFF, lr,
+                  betas[0], betas[1], eps, weight_decay, grad_scale, step,
+                  _scalar(d_lr, torch.float32, p0, "d_lr"),
+                  _scalar(d_step, torch.int64, p0, "d_step"),
+                  _scalar(d_grad_scale, torch.float32, p0, "d_grad_scale"),
+                  torch.cuda.current_stream(dev).cuda_stream)
+    _check(lib().fdb_adamw_step(_ctx_of(dev).h, table.ctypes.data, count, C.byref(o)))
+
+
+def adamw_state_values(m, m_scale, v, v_scale):
+    """The float32 values (m, v) that 8-bit moments stand for."""
+    torch = _torch()
+    n = m.numel()
+    for t, dtype, size in ((m, torch.int8, n), (v, torch.uint8, n),
+                           (m_scale, torch.float32, (n + 255) // 256),
+                           (v_scale, torch.float32, (n + 255) // 256)):
+        if t.dtype != dtype or t.device != m.device or t.numel() != size or \
+                not t.is_contiguous() or t.device.type != "cuda":
+            _refuse("8-bit moments are int8 m and uint8 v of one size with a float32 scale per "
+                    "256 elements, contiguous, on one GPU")
+    om = torch.empty(m.shape, dtype=torch.float32, device=m.device)
+    ov = torch.empty(m.shape, dtype=torch.float32, device=m.device)
+    _check(lib().fdb_adamw_state_values(
+        _ctx_of(m.device).h, m.data_ptr(), m_scale.data_ptr(), v.data_ptr(), v_scale.data_ptr(), n,
+        om.data_ptr(), ov.data_ptr(), torch.cuda.current_stream(m.device).cuda_stream))
+    return om, ov

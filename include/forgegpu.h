@@ -155,10 +155,11 @@ int fdb_ctx_init_comm_timeout(fdb_ctx* ctx, int rank, int world, const void* ncc
  * search_with_timeout (ivf_pq.rs:1369-1455). */
 int fdb_ctx_set_wait_limit(fdb_ctx* ctx, double seconds);
 /* Test hook for the timeout path: the next `count` list-scan launches of the
- * tensor path on this context issue no work, so the waits inside them find a
- * flag that nothing sets and run out after the wait limit (no fault, no hang:
- * nothing is in flight).  The call that contains them returns
- * FDB_ERR_TIMEOUT. */
+ * tensor path (or fdb_logprobs / fdb_logprobs_backward calls that use it) on
+ * this context issue no work, so the waits inside them find a flag that
+ * nothing sets and run out after the wait limit (no fault, no hang: nothing
+ * is in flight).  The call that contains them returns FDB_ERR_TIMEOUT
+ * (fdb_logprobs_status does). */
 int fdb_ctx_test_stall_scans(fdb_ctx* ctx, int count);
 /* Host memory the device can copy from at full speed (cudaHostAlloc). */
 int fdb_host_alloc(size_t bytes, void** out);
@@ -438,6 +439,156 @@ int fdb_bf_free(fdb_bf* h);
 /* MutableVectorIndex::remove (brute_force.rs:267-274): swap-remove the first
  * row with this id; *removed = 1 if one was found. */
 int fdb_bf_remove(fdb_bf* h, uint64_t id, int* removed);
+
+/* ---- softmax over rows: log probabilities and their gradient ------------- */
+/* No reference counterpart: a search returns the k best scores of a query;
+ * these return what the scores are as probabilities over ALL rows,
+ *     s_ij = scale * q_i . x_j,   p_ij = exp(s_ij) / sum_j exp(s_ij),
+ * without storing the nq x n scores.
+ *
+ * Every buffer is device memory of the context's device.  The calls only
+ * enqueue work on `stream` (a cudaStream_t of that device, used as given: NULL
+ * is the legacy default stream; fdb_ctx_stream gives the context's own) and
+ * return without waiting; inputs, outputs and the workspace have to stay valid
+ * until that work is done.  They allocate nothing and hold no state, so they
+ * can be captured into a CUDA graph, and calls on different streams may
+ * overlap as long as each has a workspace of its own. */
+#define FDB_DTYPE_F32 0
+#define FDB_DTYPE_F16 1
+#define FDB_DTYPE_BF16 2
+#define FDB_MAX_ALTERNATIVES 64   /* largest k of fdb_logprobs */
+#define FDB_MAX_SOFTMAX_DIM 16384 /* largest dim of fdb_logprobs */
+
+/* queries [nq][dim] and rows [n][dim] of one type, rows ld_* elements apart
+ * (ld >= dim).  targets[nq] (nullable): the row whose log probability is
+ * wanted; a value outside [0, n) means none.  allowed (nullable): a bit per
+ * row, bit j % 32 of word j / 32, (n + 31) / 32 words; ld_allowed words apart
+ * per query, or one filter for all queries with ld_allowed = 0.  A row whose
+ * bit is clear takes no part, whatever it holds.  1 <= n < 2^31 - 512,
+ * nq < 2^31 - 512, scale > 0 and finite.
+ *
+ * Outputs, each nullable: logprob[nq] = s_i,target - lse (0 without a target,
+ * -inf for a target that is not allowed), lse[nq], entropy[nq] in nats; with
+ * k > 0 top_ids[nq][k] and top_logprobs[nq][k] (both required), the k most
+ * probable rows in order, equal scores by row number, -1 and -inf past the
+ * allowed rows.  A query that may see no row has lse -inf, entropy 0.  If a
+ * query, or a row it may see, holds an infinity or NaN, the query's outputs
+ * are NaN (top_ids -1). */
+typedef struct fdb_logprob_args {
+    int dtype; /* FDB_DTYPE_* of queries and rows */
+    const void* queries;
+    size_t nq, ld_queries;
+    const void* rows;
+    size_t n, ld_rows;
+    size_t dim;
+    float scale;
+    const int64_t* targets;
+    const uint32_t* allowed;
+    size_t ld_allowed;
+    size_t k;
+    float *logprob, *lse, *entropy;
+    int64_t* top_ids;
+    float* top_logprobs;
+    void* workspace; /* 256-byte aligned, fdb_logprobs_workspace(...) bytes */
+    size_t workspace_bytes;
+    void* stream;
+} fdb_logprob_args;
+/* Bytes of workspace the call with these arguments needs (outputs, workspace
+ * and stream are not looked at).  Needs the context's device size only. */
+int fdb_logprobs_workspace(fdb_ctx* ctx, const fdb_logprob_args* args, size_t* bytes);
+int fdb_logprobs(fdb_ctx* ctx, const fdb_logprob_args* args);
+
+/* Gradient of a loss with respect to queries and rows, given its gradients
+ * d_logprob, d_lse, d_entropy ([nq], each nullable = 0) with respect to the
+ * outputs of fdb_logprobs, and the lse and entropy that call returned:
+ *     G_ij = scale * [ p_ij (d_lse - d_logprob - d_entropy (s_ij - lse + H))
+ *                      + d_logprob 1{j = target} ]
+ *     d_queries = G X,  d_rows = G^T Q
+ * in the type of the inputs, rows ld_d_* elements apart, overwritten; either
+ * may be NULL.  entropy may be NULL without d_entropy.  A target that is not
+ * allowed has no gradient.  Sums are taken in a fixed order: the same call
+ * gives the same bits. */
+typedef struct fdb_logprob_grad_args {
+    int dtype;
+    const void* queries;
+    size_t nq, ld_queries;
+    const void* rows;
+    size_t n, ld_rows;
+    size_t dim;
+    float scale;
+    const int64_t* targets;
+    const uint32_t* allowed;
+    size_t ld_allowed;
+    const float *lse, *entropy;
+    const float *d_logprob, *d_lse, *d_entropy;
+    void* d_queries;
+    size_t ld_d_queries;
+    void* d_rows;
+    size_t ld_d_rows;
+    void* workspace;
+    size_t workspace_bytes;
+    void* stream;
+} fdb_logprob_grad_args;
+int fdb_logprobs_backward_workspace(fdb_ctx* ctx, const fdb_logprob_grad_args* args,
+                                    size_t* bytes);
+int fdb_logprobs_backward(fdb_ctx* ctx, const fdb_logprob_grad_args* args);
+/* Whether a wait inside the kernels of the last of the two calls above that
+ * used this workspace ran out (see fdb_ctx_set_wait_limit): waits for the
+ * stream, then FDB_OK or FDB_ERR_TIMEOUT.  Such a call's outputs are NaN. */
+int fdb_logprobs_status(fdb_ctx* ctx, const void* workspace, void* stream);
+
+/* The same over the rows of a brute-force index with the dot-product metric
+ * (host buffers, like fdb_bf_batch_search): p(row | query) with
+ * scale = 1 / temperature.  target_ids[nq] (nullable): vector ids; an id that
+ * the index does not hold gives a logprob of 0, a repeated id its first row.
+ * top_ids / top_logprobs [nq][k], ids UINT64_MAX past the last row.  A
+ * sharded index is FDB_ERR_UNSUPPORTED, an empty one FDB_ERR_EMPTY_VECTOR_SET. */
+int fdb_bf_logprobs(fdb_bf* h, const float* queries, size_t nq, float temperature,
+                    const uint64_t* target_ids, size_t k, float* logprob, float* lse,
+                    float* entropy, uint64_t* top_ids, float* top_logprobs);
+
+/* ---- AdamW --------------------------------------------------------------- */
+/* No reference counterpart (it trains by k-means only).  One step over `count`
+ * tensors, enqueued on `stream` like the calls above:
+ *     m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
+ *     p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * each operation rounded in f32; p is then rounded to its type.  state_bits
+ * 32: m and v are float[n].  state_bits 8: m is int8_t[n], v uint8_t[n], with
+ * m_scale and v_scale float[(n + 255) / 256], one per FDB_ADAMW_BLOCK
+ * elements: m = m_scale c |c| / 127^2, v = v_scale c^4 / 255^4; a value
+ * between two codes is rounded up or down at random (a hash of seed, step,
+ * the tensor's number in the call and the element) so that its mean is kept,
+ * and v > 0 keeps a code of at least 1.  All zeros is the initial state.  A
+ * gradient with a NaN or infinity makes its element of p, m and v NaN or
+ * infinite, with 8-bit states the whole block's m and v.
+ * step counts from 1.  d_lr, d_step, d_grad_scale (device, nullable) replace
+ * lr and step and multiply grad_scale when the kernels run, so that a captured
+ * step can be replayed with other values.  No two tensors' params may overlap. */
+#define FDB_ADAMW_BLOCK 256
+typedef struct fdb_adamw_tensor {
+    void* param;
+    const void* grad;
+    void *m, *v;
+    float *m_scale, *v_scale; /* state_bits 8 */
+    size_t n;
+} fdb_adamw_tensor;
+typedef struct fdb_adamw_opts {
+    int param_dtype, grad_dtype; /* FDB_DTYPE_* */
+    int state_bits;              /* 32 or 8 */
+    uint32_t seed;
+    double lr, beta1, beta2, eps, weight_decay, grad_scale;
+    int64_t step;
+    const float* d_lr;
+    const int64_t* d_step;
+    const float* d_grad_scale;
+    void* stream;
+} fdb_adamw_opts;
+int fdb_adamw_step(fdb_ctx* ctx, const fdb_adamw_tensor* tensors, size_t count,
+                   const fdb_adamw_opts* opts);
+/* The values of n 8-bit moments (to save or to convert a state). */
+int fdb_adamw_state_values(fdb_ctx* ctx, const int8_t* m, const float* m_scale, const uint8_t* v,
+                           const float* v_scale, size_t n, float* m_out, float* v_out,
+                           void* stream);
 
 /* ---- .fdb files (src/persistence/mod.rs, format.rs) --------------------- */
 /* A 24-byte header (magic "FORGEDB\0", version u32 = 1, index type u32,
