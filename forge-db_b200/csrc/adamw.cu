@@ -31,6 +31,7 @@ namespace adamw {
 constexpr int TENSORS = 96;      // tensors a launch takes (their table is a kernel argument)
 constexpr int THREADS = 256;
 constexpr int CHUNK = 8192;      // elements a block works through
+constexpr int SMALL_CHUNK = 2048;  // ... when there are too few for every multiprocessor
 constexpr int BLOCK8 = FDB_ADAMW_BLOCK;
 constexpr float LEAST = 0x1p-90f;  // a block whose largest value is below this holds zeros
 constexpr float M_CODES = 16129.0f, V_CODES = 4228250625.0f;  // 127^2, 255^4
@@ -56,15 +57,14 @@ struct Hyper {
     uint32_t seed;
     const float *d_lr, *d_grad_scale;
     const int64_t* d_step;
+    int on_device;  // some of them are read when the kernel runs
 };
 // The constants of a step, each rounded once from 64 bits.
 struct Consts {
     float b1, c1, b2, c2, keep, rate, root, eps, gs;
     uint32_t salt;
 };
-__device__ Consts consts_of(const Hyper& h) {
-    const double lr = h.d_lr ? (double)*h.d_lr : h.lr;
-    const int64_t t = h.d_step ? *h.d_step : h.step;
+__host__ __device__ inline Consts consts_of(const Hyper& h, double lr, int64_t t, float gs) {
     Consts c;
     c.b1 = (float)h.b1, c.c1 = (float)(1.0 - h.b1);
     c.b2 = (float)h.b2, c.c2 = (float)(1.0 - h.b2);
@@ -72,9 +72,19 @@ __device__ Consts consts_of(const Hyper& h) {
     c.rate = (float)(lr / (1.0 - pow(h.b1, (double)t)));
     c.root = (float)(1.0 / sqrt(1.0 - pow(h.b2, (double)t)));
     c.eps = h.eps;
-    c.gs = h.d_grad_scale ? h.grad_scale * *h.d_grad_scale : h.grad_scale;
+    c.gs = gs;
     c.salt = h.seed + ((uint32_t)t << 16);
     return c;
+}
+// The constants of the step in a block: the host's, or from the device values.
+__device__ __forceinline__ Consts step_consts(const Hyper& h, const Consts& given, Consts* shared) {
+    if (!h.on_device) return given;
+    if (threadIdx.x == 0)
+        *shared = consts_of(h, h.d_lr ? (double)*h.d_lr : h.lr, h.d_step ? *h.d_step : h.step,
+                            h.d_grad_scale ? __fmul_rn(h.grad_scale, *h.d_grad_scale)
+                                           : h.grad_scale);
+    __syncthreads();
+    return *shared;
 }
 
 template <typename T>
@@ -118,6 +128,33 @@ __device__ __forceinline__ uint32_t mix(uint32_t h) {
 }
 __device__ __forceinline__ float unit(uint32_t h) { return (float)(h >> 8) * 0x1p-24f; }
 
+// floor(sqrt(y)) and floor(y^(1/4)) as the correctly rounded roots give them,
+// y in [0, 256^2) or [0, 256^4): from the approximate root (a relative error
+// of about 2^-22, so its floor is right but next to a whole number), which is
+// replaced by the exact one there.
+__device__ __forceinline__ float fast_sqrt(float y) {
+    float r;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(y));
+    return r;
+}
+__device__ __forceinline__ float root2(float y) {
+    const float r = fast_sqrt(y), n = rintf(r);
+    if (fabsf(r - n) < 0x1p-12f) return floorf(__fsqrt_rn(y));
+    return floorf(r);
+}
+__device__ __forceinline__ float root4(float y) {
+    const float r = fast_sqrt(fast_sqrt(y)), n = rintf(r);
+    if (fabsf(r - n) < 0x1p-12f) return floorf(__fsqrt_rn(__fsqrt_rn(y)));
+    return floorf(r);
+}
+// u < (y - lo) / (hi - lo), the quotient correctly rounded: decided by the
+// product unless the two sides are within the roundings of each other.
+__device__ __forceinline__ bool goes_up(float u, float y, float lo, float hi) {
+    const float a = __fsub_rn(y, lo), w = __fsub_rn(hi, lo), t = __fmaf_rn(u, w, -a);
+    if (fabsf(t) <= w * 0x1p-21f) return u < __fdiv_rn(a, w);
+    return t < 0.0f;
+}
+
 __device__ __forceinline__ const Entry& entry_of(const Table& t, unsigned block) {
     int lo = 0, hi = t.count - 1;
     while (lo < hi) {
@@ -130,21 +167,20 @@ __device__ __forceinline__ const Entry& entry_of(const Table& t, unsigned block)
 
 template <typename P, typename G>
 __global__ void __launch_bounds__(THREADS)
-    step32_kernel(const __grid_constant__ Table t, const __grid_constant__ Hyper h) {
+    step32_kernel(const __grid_constant__ Table t, const __grid_constant__ Hyper h,
+                  const __grid_constant__ Consts given, int chunk) {
     __shared__ Consts sc;
-    if (threadIdx.x == 0) sc = consts_of(h);
-    __syncthreads();
-    const Consts c = sc;
+    const Consts c = step_consts(h, given, &sc);
     const Entry& e = entry_of(t, blockIdx.x);
     P* p = static_cast<P*>(e.p);
     const G* g = static_cast<const G*>(e.g);
     float *m = static_cast<float*>(e.m), *v = static_cast<float*>(e.v);
-    const size_t n = e.n, i0 = (size_t)(blockIdx.x - e.first) * CHUNK;
-    const size_t i1 = min(n, i0 + CHUNK);
-    if (e.wide && i1 - i0 == CHUNK) {
-        constexpr int N = 4, U = 2;
+    const size_t n = e.n, i0 = (size_t)(blockIdx.x - e.first) * chunk;
+    const size_t i1 = min(n, i0 + chunk);
+    constexpr int N = 4, U = 2;
+    if (e.wide && (i1 - i0) % (THREADS * N * U) == 0) {
 #pragma unroll 1
-        for (int r = 0; r < CHUNK / (THREADS * N * U); ++r) {
+        for (int r = 0; r < (int)(i1 - i0) / (THREADS * N * U); ++r) {
             Vec<P, N> pv[U];
             Vec<G, N> gv[U];
             Vec<float, N> mv[U], vv[U];
@@ -185,18 +221,17 @@ __global__ void __launch_bounds__(THREADS)
 // One warp per block of 256 elements, 8 consecutive ones a lane.
 template <typename P, typename G>
 __global__ void __launch_bounds__(THREADS)
-    step8_kernel(const __grid_constant__ Table t, const __grid_constant__ Hyper h) {
+    step8_kernel(const __grid_constant__ Table t, const __grid_constant__ Hyper h,
+                  const __grid_constant__ Consts given, int chunk) {
     __shared__ Consts sc;
-    if (threadIdx.x == 0) sc = consts_of(h);
-    __syncthreads();
-    const Consts c = sc;
+    const Consts c = step_consts(h, given, &sc);
     const Entry& e = entry_of(t, blockIdx.x);
     P* p = static_cast<P*>(e.p);
     const G* g = static_cast<const G*>(e.g);
     int8_t* m8 = static_cast<int8_t*>(e.m);
     uint8_t* v8 = static_cast<uint8_t*>(e.v);
-    const size_t n = e.n, i0 = (size_t)(blockIdx.x - e.first) * CHUNK;
-    const size_t i1 = min(n, i0 + CHUNK);
+    const size_t n = e.n, i0 = (size_t)(blockIdx.x - e.first) * chunk;
+    const size_t i1 = min(n, i0 + chunk);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t salt = mix(c.salt + e.ordinal);
     constexpr float KM = (float)(1.0 / 16129.0), KV = (float)(1.0 / 4228250625.0);
@@ -255,20 +290,19 @@ __global__ void __launch_bounds__(THREADS)
             const size_t at = i + j;
             const uint32_t hh =
                 mix((uint32_t)at ^ salt ^ ((uint32_t)((uint64_t)at >> 32) * 0x9E3779B1u));
-            float y = __fmul_rn(fabsf(m[j]), km);
-            float k = floorf(__fsqrt_rn(y));
-            float lo = __fmul_rn(k, k), k1 = __fadd_rn(k, 1.0f), hi = __fmul_rn(k1, k1);
-            if (unit(hh) < __fdiv_rn(__fsub_rn(y, lo), __fsub_rn(hi, lo))) k = k1;
-            k = fminf(k, 127.0f);
-            mc.e[j] = y > 0.0f ? (int8_t)(m[j] < 0.0f ? -k : k) : (int8_t)0;
-            y = __fmul_rn(v[j], kw);
-            k = floorf(__fsqrt_rn(__fsqrt_rn(y)));
+            const float y = __fmul_rn(fabsf(m[j]), km);
+            float k = root2(y);
+            float k1 = __fadd_rn(k, 1.0f);
+            if (goes_up(unit(hh), y, __fmul_rn(k, k), __fmul_rn(k1, k1))) k = k1;
+            k = y > 0.0f ? fminf(k, 127.0f) : 0.0f;  // (also for a NaN)
+            mc.e[j] = (int8_t)(m[j] < 0.0f ? -k : k);
+            const float z = __fmul_rn(v[j], kw);
+            k = root4(z);
             k1 = __fadd_rn(k, 1.0f);
-            lo = __fmul_rn(k, k), hi = __fmul_rn(k1, k1);
-            lo = __fmul_rn(lo, lo), hi = __fmul_rn(hi, hi);
-            if (unit(mix(hh ^ 0x5BD1E995u)) < __fdiv_rn(__fsub_rn(y, lo), __fsub_rn(hi, lo)))
+            const float lo = __fmul_rn(k, k), hi = __fmul_rn(k1, k1);
+            if (goes_up(unit(mix(hh ^ 0x5BD1E995u)), z, __fmul_rn(lo, lo), __fmul_rn(hi, hi)))
                 k = k1;
-            vc.e[j] = y > 0.0f ? (uint8_t)fmaxf(fminf(k, 255.0f), 1.0f) : (uint8_t)0;
+            vc.e[j] = z > 0.0f ? (uint8_t)fmaxf(fminf(k, 255.0f), 1.0f) : (uint8_t)0;
         }
         if (wide) {
             *reinterpret_cast<Vec<P, 8>*>(p + i) = pv;
@@ -336,25 +370,32 @@ __global__ void __launch_bounds__(THREADS)
 static bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
 template <typename P, typename G>
-static void launch(cudaStream_t s, int bits, const Table& t, const Hyper& h, unsigned blocks) {
-    if (bits == 8) step8_kernel<P, G><<<blocks, THREADS, 0, s>>>(t, h);
-    else step32_kernel<P, G><<<blocks, THREADS, 0, s>>>(t, h);
+static void launch(cudaStream_t s, int bits, const Table& t, const Hyper& h, const Consts& c,
+                   int chunk, unsigned blocks) {
+    if (bits == 8) step8_kernel<P, G><<<blocks, THREADS, 0, s>>>(t, h, c, chunk);
+    else step32_kernel<P, G><<<blocks, THREADS, 0, s>>>(t, h, c, chunk);
     FDB_LAUNCH_CHECK();
 }
 template <typename P>
 static void launch_g(cudaStream_t s, int gtype, int bits, const Table& t, const Hyper& h,
-                     unsigned blocks) {
-    if (gtype == FDB_DTYPE_F32) launch<P, float>(s, bits, t, h, blocks);
-    else if (gtype == FDB_DTYPE_BF16) launch<P, __nv_bfloat16>(s, bits, t, h, blocks);
-    else launch<P, __half>(s, bits, t, h, blocks);
+                     const Consts& c, int chunk, unsigned blocks) {
+    if (gtype == FDB_DTYPE_F32) launch<P, float>(s, bits, t, h, c, chunk, blocks);
+    else if (gtype == FDB_DTYPE_BF16) launch<P, __nv_bfloat16>(s, bits, t, h, c, chunk, blocks);
+    else launch<P, __half>(s, bits, t, h, c, chunk, blocks);
 }
 
-void step(cudaStream_t s, const fdb_adamw_tensor* ts, size_t count, const fdb_adamw_opts& o) {
+void step(cudaStream_t s, int sms, const fdb_adamw_tensor* ts, size_t count,
+          const fdb_adamw_opts& o) {
     Hyper h{};
     h.lr = o.lr, h.b1 = o.beta1, h.b2 = o.beta2, h.wd = o.weight_decay;
     h.eps = (float)o.eps, h.grad_scale = (float)o.grad_scale;
     h.step = o.step, h.seed = o.seed;
     h.d_lr = o.d_lr, h.d_grad_scale = o.d_grad_scale, h.d_step = o.d_step;
+    h.on_device = o.d_lr || o.d_step || o.d_grad_scale;
+    const Consts c = consts_of(h, h.lr, std::max<int64_t>(h.step, 1), h.grad_scale);
+    size_t total = 0;
+    for (size_t i = 0; i < count; ++i) total += ts[i].n;
+    const int chunk = total < (size_t)CHUNK * 4 * sms ? SMALL_CHUNK : CHUNK;
     // vectors of 4 (f32 moments) or 8 (8-bit) elements, 16 bytes at most
     const size_t per = o.state_bits == 8 ? 8 : 4;
     auto vec = [&](int dtype) {
@@ -365,17 +406,17 @@ void step(cudaStream_t s, const fdb_adamw_tensor* ts, size_t count, const fdb_ad
     unsigned blocks = 0;
     auto flush = [&] {
         if (t.count == 0) return;
-        if (o.param_dtype == FDB_DTYPE_F32) launch_g<float>(s, o.grad_dtype, o.state_bits, t, h, blocks);
+        if (o.param_dtype == FDB_DTYPE_F32) launch_g<float>(s, o.grad_dtype, o.state_bits, t, h, c, chunk, blocks);
         else if (o.param_dtype == FDB_DTYPE_BF16)
-            launch_g<__nv_bfloat16>(s, o.grad_dtype, o.state_bits, t, h, blocks);
-        else launch_g<__half>(s, o.grad_dtype, o.state_bits, t, h, blocks);
+            launch_g<__nv_bfloat16>(s, o.grad_dtype, o.state_bits, t, h, c, chunk, blocks);
+        else launch_g<__half>(s, o.grad_dtype, o.state_bits, t, h, c, chunk, blocks);
         t.count = 0;
         blocks = 0;
     };
     for (size_t i = 0; i < count; ++i) {
         const fdb_adamw_tensor& x = ts[i];
         if (x.n == 0) continue;
-        const size_t need = (x.n + CHUNK - 1) / CHUNK;
+        const size_t need = (x.n + chunk - 1) / chunk;
         if (t.count == TENSORS || need + blocks > 0x7fffffffu) flush();
         Entry& e = t.e[t.count++];
         e.p = x.param, e.g = x.grad, e.m = x.m, e.v = x.v, e.ms = x.m_scale, e.vs = x.v_scale;

@@ -1334,8 +1334,6 @@ int fdb_bf_logprobs(fdb_bf* h, const float* queries, size_t nq, float temperatur
         h->s_lp_ws.ensure(need);
         a.workspace = h->s_lp_ws.p, a.workspace_bytes = need;
         a.stream = s;
-        // (a small batch's kernels have no waits and leave the word alone)
-        FDB_CUDA(cudaMemsetAsync(a.workspace, 0, 4, s));
         sr::forward_run(c, a);
         int err = 0;
         std::vector<int64_t> rows(nq * k);
@@ -1409,7 +1407,7 @@ int fdb_adamw_step(fdb_ctx* ctx, const fdb_adamw_tensor* tensors, size_t count,
             FDB_REQUIRE(spans[i - 1].second <= spans[i].first, FDB_ERR_INVALID_ARG,
                         "two tensors' params overlap");
         DeviceGuard g(ctx->c.device);
-        adamw::step(static_cast<cudaStream_t>(o.stream), tensors, count, o);
+        adamw::step(static_cast<cudaStream_t>(o.stream), ctx->c.sm_count, tensors, count, o);
     });
 }
 

@@ -508,7 +508,8 @@ void launch_find_rows(cudaStream_t s, const uint64_t* ids, size_t n, const uint6
 }  // namespace sr
 // adamw.cu
 namespace adamw {
-void step(cudaStream_t s, const fdb_adamw_tensor* ts, size_t count, const fdb_adamw_opts& o);
+void step(cudaStream_t s, int sms, const fdb_adamw_tensor* ts, size_t count,
+          const fdb_adamw_opts& o);
 void values(cudaStream_t s, int sms, const int8_t* m, const float* ms, const uint8_t* v,
             const float* vs, size_t n, float* om, float* ov);
 }  // namespace adamw

@@ -49,7 +49,6 @@ __host__ __device__ constexpr int bn_of(bool two) { return two ? 128 : 256; }
 __host__ __device__ constexpr int stages_of(bool two) { return two ? 3 : 4; }
 __host__ __device__ constexpr int stage_bytes(bool two) { return two ? 4 * OPER : 3 * OPER; }
 __host__ __device__ constexpr int accs_of(bool two) { return two ? 4 : 2; }
-constexpr int MAX_STG = 4, MAX_ACC = 4;
 constexpr int MAX_BN = 256;
 constexpr int THREADS = 640;                // 2 issuing warps, 2 idle, 16 epilogue warps
 constexpr int EPI_WARP0 = 4, EPI_WARPS = 16;
@@ -157,26 +156,54 @@ __device__ __forceinline__ float2 top_pair(const float (&u)[32]) {
 // an infinity or NaN (its elements are then written as zeros: the NaN reaches
 // a score through f alone, so a query that may not see the row is not
 // touched).  `seen` (nullable): rows whose bit is clear are taken as zeros.
-// Bound by memory: reads d * size, writes 2 * parts * kp a row.
+// Bound by memory: reads d * size, writes 2 * parts * kp a row; rows of up to
+// 16 vectors a lane stay in registers between the two passes.
+struct PackSide {
+    const void* x;
+    size_t ld;
+    int n;
+    const uint32_t* seen;
+    __half* out;
+    float* f;
+    unsigned* largest;   // bits of the largest f, nullable
+    int blocks;          // 8 rows each
+    int wide;            // rows can be read in 16-byte vectors
+};
 template <typename T, int PARTS>
-__global__ void __launch_bounds__(256)
-    pack_kernel(const T* __restrict__ x, size_t ld, int n, int d, int kp,
-                const uint32_t* __restrict__ seen, __half* __restrict__ out,
-                float* __restrict__ f, unsigned* __restrict__ fmax_bits) {
+__device__ __forceinline__ void pack_row(const PackSide& p, int row, int d, int kp) {
+    constexpr int V = 16 / (int)sizeof(T), NV = 4;
     const int lane = threadIdx.x & 31;
-    const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (row >= n) return;
-    const T* src = x + (size_t)row * ld;
-    __half* dst = out + (size_t)row * (size_t)(PARTS * kp);
-    const bool use = !seen || (seen[row >> 5] >> (row & 31) & 1u);
+    const T* src = static_cast<const T*>(p.x) + (size_t)row * p.ld;
+    __half* dst = p.out + (size_t)row * (size_t)(PARTS * kp);
+    const bool use = !p.seen || (p.seen[row >> 5] >> (row & 31) & 1u);
+    const bool held = p.wide && d <= 32 * V * NV;
+    uint4 raw[NV];
     float mx = 0.0f;
     bool bad = false;
-    if (use)
+    if (use && held) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * 32 + lane) * V;
+            raw[i] = make_uint4(0, 0, 0, 0);
+            if (c < d) raw[i] = __ldg(reinterpret_cast<const uint4*>(src + c));
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const T* e = reinterpret_cast<const T*>(&raw[i]);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float v = fabsf(to_f32<T>(e[j]));
+                bad |= !(v <= FLT_MAX);
+                mx = fmaxf(mx, v);
+            }
+        }
+    } else if (use) {
         for (int c = lane; c < d; c += 32) {
             const float v = fabsf(to_f32<T>(src[c]));
             bad |= !(v <= FLT_MAX);
             mx = fmaxf(mx, v);
         }
+    }
     bad = __any_sync(0xffffffffu, bad);
 #pragma unroll
     for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -185,16 +212,54 @@ __global__ void __launch_bounds__(256)
     if (!bad && mx > 0.0f) e = max(-120, min(120, 13 - ilogbf(mx)));
     const float s = ldexpf(1.0f, e);
     const bool zero = bad || !(mx > 0.0f);
-    for (int c = lane; c < kp; c += 32) {
-        const float v = (!zero && c < d) ? to_f32<T>(src[c]) * s : 0.0f;
-        const __half hi = __float2half_rn(v);
-        dst[c] = hi;
-        if (PARTS == 2) dst[kp + c] = __float2half_rn(v - __half2float(hi));
+    if (held) {  // (d is a multiple of V, kp of 16: whole vectors, zeros past d)
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * 32 + lane) * V;
+            if (c >= kp) break;
+            const T* x = reinterpret_cast<const T*>(&raw[i]);
+            __align__(16) __half hi[V], lo[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float v = !zero && c < d ? to_f32<T>(x[j]) * s : 0.0f;
+                hi[j] = __float2half_rn(v);
+                lo[j] = __float2half_rn(v - __half2float(hi[j]));
+            }
+            if (V == 8) {
+                *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(hi);
+            } else {
+                *reinterpret_cast<uint2*>(dst + c) = *reinterpret_cast<const uint2*>(hi);
+                if (PARTS == 2)
+                    *reinterpret_cast<uint2*>(dst + kp + c) = *reinterpret_cast<const uint2*>(lo);
+            }
+        }
+    } else {
+        for (int c = lane; c < kp; c += 32) {
+            const float v = (!zero && c < d) ? to_f32<T>(src[c]) * s : 0.0f;
+            const __half hi = __float2half_rn(v);
+            dst[c] = hi;
+            if (PARTS == 2) dst[kp + c] = __float2half_rn(v - __half2float(hi));
+        }
     }
     if (lane == 0) {
         const float r = bad ? __int_as_float(0x7fc00000) : (mx > 0.0f ? ldexpf(1.0f, -e) : 0.0f);
-        f[row] = r;
-        if (fmax_bits && r > 0.0f) atomicMax(fmax_bits, __float_as_uint(r));
+        p.f[row] = r;
+        // (most rows find their own power of two there already)
+        if (p.largest && r > 0.0f && __float_as_uint(r) > *(volatile unsigned*)p.largest)
+            atomicMax(p.largest, __float_as_uint(r));
+    }
+}
+// Both operands in one launch; the first block clears the error word.
+template <typename T, int PARTS>
+__global__ void __launch_bounds__(256)
+    pack_kernel(const PackSide a, const PackSide b, int d, int kp, int* err) {
+    if (err && blockIdx.x == 0 && threadIdx.x == 0) *err = 0;
+    const bool first = (int)blockIdx.x < a.blocks;
+    const int row = ((int)blockIdx.x - (first ? 0 : a.blocks)) * 8 + (threadIdx.x >> 5);
+    if (first) {
+        if (row < a.n) pack_row<T, PARTS>(a, row, d, kp);
+    } else if (row < b.n) {
+        pack_row<T, PARTS>(b, row, d, kp);
     }
 }
 // 16-bit rows copied to an aligned, zero-padded layout (their own is not one
@@ -295,11 +360,12 @@ __device__ __forceinline__ void load_chunk(uint32_t tmem, float (&u)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) u[i] = __uint_as_float(v[i]);
 }
+// `f`: 32 factors in shared memory.
 __device__ __forceinline__ void scale_chunk(const float* f, float (&u)[32]) {
     const float4* cf = reinterpret_cast<const float4*>(f);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float4 c = __ldg(cf + i);
+        const float4 c = cf[i];
         u[4 * i] *= c.x;
         u[4 * i + 1] *= c.y;
         u[4 * i + 2] *= c.z;
@@ -307,8 +373,37 @@ __device__ __forceinline__ void scale_chunk(const float* f, float (&u)[32]) {
     }
 }
 
+// What a chunk of 32 columns needs besides its scores: the filter's word of
+// the thread's row, and (scaled rows) the columns' factors, in the warp's own
+// shared memory.  `load` starts the reads of a tile's chunks while the tile
+// before it is worked on, `ready` hands them over.
+template <bool FACTORS, int CHUNKS>
+struct Columns {
+    uint32_t next[CHUNKS], word[CHUNKS];
+    float nf[CHUNKS];
+    float* fac;  // [CHUNKS][32]
+    __device__ __forceinline__ void load(const uint32_t* al, const float* f, size_t col, int n) {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int h = 0; h < CHUNKS; ++h) {
+            next[h] = allowed_word(al, 0, 0, col + 32 * h, n);
+            if (FACTORS) nf[h] = __ldg(f + col + 32 * h + lane);
+        }
+    }
+    __device__ __forceinline__ void ready() {
+        if (FACTORS) __syncwarp();
+#pragma unroll
+        for (int h = 0; h < CHUNKS; ++h) {
+            word[h] = next[h];
+            if (FACTORS) fac[32 * h + (threadIdx.x & 31)] = nf[h];
+        }
+        if (FACTORS) __syncwarp();
+    }
+};
+
 // The epilogues: one object per thread and unit; `chunk` takes 32 columns of
-// the thread's row, from column `col` of the unit's matrix, in registers.
+// the thread's row, from column `col` of the unit's matrix (chunk h of the
+// thread's columns of the tile), in registers.
 template <bool TWO>
 struct StatsEpilogue {
     typedef StatsArgs Args;
@@ -317,8 +412,14 @@ struct StatsEpilogue {
     float rf;
     Run r;
     bool live;
-    __device__ StatsEpilogue(const Mma&, const StatsArgs& a, int row, int row0, int, int) : p(a) {
+    Columns<TWO, TWO ? 1 : 2> c;
+    const uint32_t* al;
+    __device__ StatsEpilogue(const Mma&, const StatsArgs& a, int row, int row0, int, int,
+                             float* fac)
+        : p(a) {
+        c.fac = fac;
         q = row < a.nq ? row : -1;
+        al = q < 0 || !a.allowed ? nullptr : a.allowed + (size_t)(a.q0 + q) * a.ld_allowed;
         live = row0 < a.nq;
         rf = a.rf;
         if (TWO && q >= 0) {
@@ -327,14 +428,14 @@ struct StatsEpilogue {
         }
         r = Run{-INFINITY, 0.0f, 0.0f};
     }
-    __device__ __forceinline__ void chunk(float (&u)[32], int icol) {
+    __device__ __forceinline__ void load(int col) { c.load(al, p.xf, (size_t)col, p.n); }
+    __device__ __forceinline__ void chunk(float (&u)[32], int icol, int h) {
         if (!live) return;
         const size_t col = (size_t)icol;
-        const uint32_t w =
-            allowed_word(q < 0 ? nullptr : p.allowed, p.ld_allowed, p.q0 + q, col, p.n);
+        const uint32_t w = h ? c.word[sizeof(c.word) / 4 - 1] : c.word[0];
         float2 best = make_float2(NONE, NONE);
         if (__any_sync(0xffffffffu, w != 0u)) {
-            if (TWO) scale_chunk(p.xf + col, u);
+            if (TWO) scale_chunk(c.fac, u);
             const bool full = __all_sync(0xffffffffu, w == 0xffffffffu);
             if (!full) {
 #pragma unroll
@@ -383,23 +484,29 @@ struct GradEpilogue {
     int q, row;
     Coef k;
     float wi;
-    __device__ GradEpilogue(const Mma&, const GradArgs& a, int r, int, int, int) : p(a) {
+    Columns<true, TWO ? 1 : 2> c;
+    const uint32_t* al;
+    __device__ GradEpilogue(const Mma&, const GradArgs& a, int r, int, int, int, float* fac)
+        : p(a) {
+        c.fac = fac;
         row = r;
+        al = r >= a.nq || !a.allowed ? nullptr : a.allowed + (size_t)r * a.ld_allowed;
         q = r < a.nq ? r : -1;
         k = a.coef[q < 0 ? 0 : q];
         const float f = q < 0 ? 0.0f : a.qf[q];
         wi = f * grad_factor(a.bounds);
     }
-    __device__ __forceinline__ void chunk(float (&u)[32], int icol) {  // icol: of the chunk
+    __device__ __forceinline__ void load(int col) {
+        c.load(al, p.xf, (size_t)p.j0 + col, p.j0 + p.cols);
+    }
+    __device__ __forceinline__ void chunk(float (&u)[32], int icol, int h) {
         const size_t col = (size_t)icol, gcol = (size_t)p.j0 + col;
         if (col >= p.ldg) return;
-        uint32_t w = allowed_word(q < 0 ? nullptr : p.allowed, p.ld_allowed, max(q, 0), gcol,
-                                  p.j0 + p.cols);
-        if (q < 0) w = 0u;
+        const uint32_t w = q < 0 ? 0u : h ? c.word[sizeof(c.word) / 4 - 1] : c.word[0];
         const bool any = __any_sync(0xffffffffu, w != 0u);
         const bool full = __all_sync(0xffffffffu, w == 0xffffffffu);
         const int at = k.target - (int)gcol;  // of the given row, if it is in this chunk
-        const float* xf = p.xf + gcol;
+        const float* xf = c.fac + 32 * h;
         uint4* oh = reinterpret_cast<uint4*>(p.out + (size_t)row * p.ldg + col);
         uint4* ol = reinterpret_cast<uint4*>(p.out + p.plane + (size_t)row * p.ldg + col);
 #pragma unroll
@@ -410,17 +517,17 @@ struct GradEpilogue {
                 const int c0 = 8 * b + 2 * i;
                 h4[i] = l4[i] = 0u;
                 if (!any) continue;
-                const float2 cf = __ldg(reinterpret_cast<const float2*>(xf + c0));
+                const float2 cf = *reinterpret_cast<const float2*>(xf + c0);
                 float g2[2];
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const float c = j ? cf.y : cf.x;
-                    const float uu = u[c0 + j] * c;
+                    const float cj = j ? cf.y : cf.x;
+                    const float uu = u[c0 + j] * cj;
                     float x = __fmaf_rn(uu, k.rf_hi, -k.l_hi) + __fmaf_rn(uu, k.rf_lo, -k.l_lo);
                     x = fmaxf(x, -160.0f);
                     float g = ex2(x) * __fmaf_rn(x, k.h, k.c);
                     if (at == c0 + j) g += k.g;
-                    g *= c * wi;
+                    g *= cj * wi;
                     if (!full && !(w >> (c0 + j) & 1u)) g = 0.0f;
                     g2[j] = g;
                 }
@@ -488,12 +595,17 @@ struct ProdEpilogue {
     const ProdArgs& p;
     int row, split;
     float s;
-    __device__ ProdEpilogue(const Mma&, const ProdArgs& a, int r, int, int, int sp) : p(a) {
+    Columns<false, 1> c;
+    __device__ ProdEpilogue(const Mma&, const ProdArgs& a, int r, int, int, int sp, float*)
+        : p(a) {
         row = r;
         split = sp;
         s = !a.partial && row < a.rows ? 1.0f / (a.f[row] * grad_factor(a.bounds)) : 0.0f;
     }
-    __device__ __forceinline__ void chunk(float (&u)[32], int c) {
+    __device__ __forceinline__ void load(int) {
+        c.next[0] = 0;
+    }
+    __device__ __forceinline__ void chunk(float (&u)[32], int c, int) {
         if (c >= p.cols || row >= p.rows) return;
         const int count = min(32, p.cols - c);
         if (!p.partial) {
@@ -603,6 +715,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint64_t* t_full = empty + NST;
     uint64_t* t_empty = t_full + NACC;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(t_empty + NACC);
+    float* factors = reinterpret_cast<float*>(smem + NST * STAGE + 256);  // [16 warps][64]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < NST; ++i) {
@@ -753,9 +866,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
             const Unit x = unit_of<MODE>(g, u);
             const int row0 = x.mt * BM + quad * 32;
-            typename EpilogueOf<MODE, TWO>::Type epi(g, p, row0 + lane, row0, x.t0, x.sp);
+            typename EpilogueOf<MODE, TWO>::Type epi(g, p, row0 + lane, row0, x.t0, x.sp,
+                                                      factors + w * 64);
+            epi.load(x.t0 * BN + part * (BN / 4));
             for (int t = x.t0; ok && t < x.t1; ++t) {
                 const int col = t * BN + part * (BN / 4);
+                epi.c.ready();
+                if (t + 1 < x.t1) epi.load(col + BN);
                 float v[32];
                 if (TWO) {
 #pragma unroll
@@ -771,7 +888,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
                         for (int i = 0; i < 32; ++i) v[i] += y[i];
                     }
-                    if (ok) epi.chunk(v, col);
+                    if (ok) epi.chunk(v, col, 0);
                     __syncwarp();
                 } else {
                     if (!next()) {
@@ -781,7 +898,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll 1
                     for (int h = 0; h < 2; ++h) {
                         load_chunk(mine + (uint32_t)(ti % NACC * BN + h * 32), v);
-                        epi.chunk(v, col + h * 32);
+                        epi.chunk(v, col + h * 32, h);
                         __syncwarp();
                     }
                     release();
@@ -827,7 +944,8 @@ __global__ void __launch_bounds__(64)
     few_kernel(const float* __restrict__ x, size_t ld, int n, int d, const float* __restrict__ q,
                size_t ldq, int q0, int nq, float rf, const uint32_t* __restrict__ allowed,
                size_t ld_allowed, float4* __restrict__ part, float2* __restrict__ top,
-               size_t groups) {
+               size_t groups, int* __restrict__ err) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) *err = 0;  // (this path has no waits)
     extern __shared__ float4 qs4[];
     float* qs = reinterpret_cast<float*>(qs4);  // [NQ][dp]
     const int dp = (d + 127) & ~127;
@@ -990,283 +1108,255 @@ __device__ __forceinline__ uint32_t ordered(float f) {
     const uint32_t u = __float_as_uint(f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-
-__device__ __forceinline__ float unordered(uint32_t u) {
-    return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+// A group's largest score without the mark of its pair.
+__device__ __forceinline__ float unmarked(float f) {
+    return __uint_as_float(__float_as_uint(f) & ~15u);
 }
 
-// 128 keys of a warp (4 a lane, key i of lane l at l + 32 i) sorted, largest first.
-__device__ __forceinline__ void warp_sort128(uint64_t (&v)[4], int lane) {
+constexpr int PICKED = 256;              // groups picked for exact scoring at most
+constexpr int CAND = MAX_SEL * GROUP;    // rows scored exactly and ranked at once
+
+// x . q in 64 bits over LANES lanes (a power of two): each product exact (f32)
+// or exact in f32 (16-bit types), added in 64 bits.
+__device__ __forceinline__ double add_product(float x, float q, double s) {
+    return fma((double)x, (double)q, s);
+}
+template <typename T>
+__device__ __forceinline__ double dot_lanes(const T* __restrict__ x, const float* q, int d, int sub,
+                                            int lanes, bool wide) {
+    constexpr int V = 16 / (int)sizeof(T);
+    double s0 = 0.0, s1 = 0.0;
+    if (wide) {
+        for (int c = sub * V; c < d; c += lanes * V) {
+            if (c + V <= d) {
+                const uint4 raw = __ldg(reinterpret_cast<const uint4*>(x + c));
+                const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-    for (int size = 2; size <= 128; size <<= 1) {
-#pragma unroll
-        for (int stride = size >> 1; stride > 0; stride >>= 1) {
-            if (stride >= 32) {
-                const int si = stride >> 5;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (!(i & si)) {
-                        const int e = lane + 32 * i;
-                        const bool desc = !(e & size);
-                        const uint64_t a = v[i], b = v[i | si];
-                        if ((a < b) == desc) {
-                            v[i] = b;
-                            v[i | si] = a;
-                        }
+                for (int i = 0; i < V; i += 2) {
+                    if (sizeof(T) == 4) {
+                        s0 = add_product(to_f32<T>(e[i]), q[c + i], s0);
+                        s1 = add_product(to_f32<T>(e[i + 1]), q[c + i + 1], s1);
+                    } else {
+                        s0 += (double)__fmul_rn(to_f32<T>(e[i]), q[c + i]);
+                        s1 += (double)__fmul_rn(to_f32<T>(e[i + 1]), q[c + i + 1]);
                     }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int e = lane + 32 * i;
-                    const bool desc = !(e & size), lower = !(lane & stride);
-                    const uint64_t o = __shfl_xor_sync(0xffffffffu, v[i], stride);
-                    const bool keep_max = lower == desc;
-                    v[i] = keep_max ? (v[i] > o ? v[i] : o) : (v[i] < o ? v[i] : o);
                 }
+            } else {
+                for (int i = c; i < d; ++i) s0 = add_product(to_f32<T>(x[i]), q[i], s0);
             }
         }
+    } else {
+        for (int c = sub; c < d; c += lanes) s0 = add_product(to_f32<T>(x[c]), q[c], s0);
     }
-}
-
-// The `want` (<= 72) largest keys a warp has been offered: appended to a
-// buffer of 128 in shared memory when above the threshold, sorted when full.
-struct WarpTop {
-    uint64_t* buf;
-    int want, cnt, lane;
-    uint64_t thr;
-    __device__ WarpTop(uint64_t* b, int w, int l) : buf(b), want(w), cnt(0), lane(l), thr(0) {}
-    __device__ void shrink() {
-        uint64_t v[4];
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = lane + 32 * i < cnt ? buf[lane + 32 * i] : 0ull;
-        warp_sort128(v, lane);
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) buf[lane + 32 * i] = v[i];
-        __syncwarp();
-        cnt = min(cnt, want);
-        if (cnt == want) thr = buf[want - 1];
-    }
-    __device__ void offer(uint64_t key) {  // key 0: none
-        const unsigned vote = __ballot_sync(0xffffffffu, key > thr);
-        if (!vote) return;
-        if (key > thr) buf[cnt + __popc(vote & ((1u << lane) - 1u))] = key;
-        cnt += __popc(vote);
-        if (cnt > 96) shrink();
-    }
-};
-
-constexpr int CAND = MAX_SEL * GROUP;  // the marked pairs, then the rest of their groups
-
-// q . x in 64 bits: 8 lanes a row, products of the inputs exact.
-template <typename T>
-__device__ __forceinline__ double dot8(const T* __restrict__ a, const T* __restrict__ b, int d,
-                                       int sub) {
-    double s0 = 0.0, s1 = 0.0;
-    int c = sub;
-    for (; c + 8 < d; c += 16) {
-        s0 = fma((double)to_f32<T>(a[c]), (double)to_f32<T>(b[c]), s0);
-        s1 = fma((double)to_f32<T>(a[c + 8]), (double)to_f32<T>(b[c + 8]), s1);
-    }
-    if (c < d) s0 = fma((double)to_f32<T>(a[c]), (double)to_f32<T>(b[c]), s0);
     s0 += s1;
-#pragma unroll
-    for (int o = 4; o; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+    for (int o = lanes >> 1; o; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
     return s0;
 }
 
-// One block per query.
-template <typename T, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32) finish_kernel(const FinishArgs p) {
-    __shared__ double red[WARPS][3];
-    __shared__ double s_lse;
-    __shared__ int s_bad;
-    __shared__ uint64_t buf[WARPS][128];
-    __shared__ int sel[MAX_SEL];
-    __shared__ float sel2[MAX_SEL];
+// One block per query: the partial triples joined, the groups that may hold
+// one of the best k picked, their rows scored exactly and ranked.
+//
+// Picking needs no sort: the (k + 8)th largest of 128 maxima over interleaved
+// parts of the groups is a bound that at least k + 8 groups reach, and for
+// scores in no particular order hardly more do.
+template <typename T, int THREADS_>
+__global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
+    constexpr int W = THREADS_ / 32;
+    extern __shared__ float qs[];  // [dim]
+    __shared__ float part_max[128];
+    __shared__ double red[W][2];
+    __shared__ float redf[W];
+    __shared__ float s_bound;
+    __shared__ int s_picked, s_cnt;
+    __shared__ int sel[PICKED];
+    __shared__ float2 sel_m[PICKED];
     __shared__ double cs[CAND + 1];
     __shared__ uint32_t ci[CAND + 1];
-    __shared__ int s_cnt;
     __shared__ double s_kth;
     __shared__ double kept[FDB_MAX_ALTERNATIVES];
     __shared__ uint32_t kept_id[FDB_MAX_ALTERNATIVES];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int ql = blockIdx.x, q = p.q0 + ql;
     const T* qp = static_cast<const T*>(p.q) + (size_t)q * p.ldq;
     const T* xp = static_cast<const T*>(p.x);
     const uint32_t* al = p.allowed ? p.allowed + (size_t)q * p.ld_allowed : nullptr;
-    double f = 1.0;
-    if (p.qf) f = p.qf[ql] == 0.0f ? 1.0 : (double)p.qf[ql];
-    const double rf = f * (double)p.scale * LOG2E;
+    const float2* top = p.k > 0 ? p.top + (size_t)ql * p.groups : nullptr;
+    const int groups = p.k > 0 ? (int)p.groups : 0;
+    float f = 1.0f;
+    if (p.qf) f = p.qf[ql] == 0.0f ? 1.0f : p.qf[ql];
+    const float rf = f * (float)((double)p.scale * LOG2E);
+    const double rf64 = (double)f * (double)p.scale * LOG2E;
+    const int64_t target = p.targets ? p.targets[q] : -1;
+    const bool given = target >= 0 && target < p.n;
+    if (tid == 0) s_picked = s_cnt = 0, s_kth = -INFINITY;
+    for (int c = tid; c < p.d; c += THREADS_) qs[c] = to_f32<T>(qp[c]);
 
-    // ---- the running triples joined in 64 bits (m in units of t) ----
-    double M = -INFINITY, L = 0.0, A = 0.0;
-    auto join = [&](double m, double l, double a) {
-        if (m > M) {
-            const double t0 = M, t1 = L, t2 = A;
-            M = m, L = l, A = a;
-            m = t0, l = t1, a = t2;
-        }
-        if (!(l == 0.0 && a == 0.0)) {
-            const double d = m == M ? 0.0 : m - M, e = exp2(d);
-            A += (a + d * l) * e;
-            L += l * e;
-        }
-    };
-    for (int i = threadIdx.x; i < p.parts; i += WARPS * 32) {
+    // ---- largest scores: of the parts, and of 128 interleaved parts of the groups ----
+    float M = -INFINITY;
+    for (int i = tid; i < p.parts; i += THREADS_)
+        M = fmaxf(M, p.part[(size_t)i * p.nq + ql].x);
+    float gm = NONE;
+#pragma unroll 4
+    for (int i = tid; i < groups; i += THREADS_) gm = fmaxf(gm, unmarked(top[i].x));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+#pragma unroll
+    for (int o = THREADS_ / 256; o; o >>= 1) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, o));
+    if (lane == 0) redf[warp] = M;
+    if (tid % (THREADS_ / 128) == 0) part_max[tid / (THREADS_ / 128)] = gm;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < W; ++i) M = fmaxf(M, redf[i]);
+    // ---- the sums over the parts, in units of 2^(M rf) ----
+    double L = 0.0, A = 0.0;
+    for (int i = tid; i < p.parts; i += THREADS_) {
         const float4 t = p.part[(size_t)i * p.nq + ql];
-        join((double)t.x * rf, (double)t.y, (double)t.z);
+        if (t.y == 0.0f && t.z == 0.0f) continue;
+        const float d = t.x == M ? 0.0f : (t.x - M) * rf, e = ex2(d);
+        L += (double)(t.y * e);
+        A += (double)(__fmaf_rn(d, t.y, t.z) * e);
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
-        const double m = __shfl_xor_sync(0xffffffffu, M, o);
-        const double l = __shfl_xor_sync(0xffffffffu, L, o);
-        const double a = __shfl_xor_sync(0xffffffffu, A, o);
-        join(m, l, a);
+        L += __shfl_xor_sync(0xffffffffu, L, o);
+        A += __shfl_xor_sync(0xffffffffu, A, o);
     }
-    if (lane == 0) red[warp][0] = M, red[warp][1] = L, red[warp][2] = A;
-    // the row whose log probability is asked for is the last candidate
-    const int64_t target = p.targets ? p.targets[q] : -1;
-    const bool given = target >= 0 && target < p.n;
-    if (threadIdx.x == 0) s_cnt = 0;
+    if (lane == 0) red[warp][0] = L, red[warp][1] = A;
+    if (p.k > 0 && tid < 128) {
+        int rank = 0;
+        const float mine = part_max[tid];
+#pragma unroll 8
+        for (int i = 0; i < 128; ++i)
+            rank += part_max[i] > mine || (part_max[i] == mine && i < tid);
+        if (rank == p.k + PAD - 1) s_bound = mine;
+    }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < WARPS; ++w) join(red[w][0], red[w][1], red[w][2]);
-        const bool empty = L == 0.0;
-        const bool bad = !(A == A) || !(L == L) || (p.err && *p.err != 0);
-        const double lg = empty ? 0.0 : log2(L);
-        const double lse = bad ? NAN : empty ? -INFINITY : LN2 * (M + lg);
+    L = A = 0.0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) L += red[i][0], A += red[i][1];
+    const bool none = L == 0.0;  // no row may be seen
+    const bool bad = !(A == A) || !(L == L) || (p.err && *p.err != 0);
+    const double lg = none || bad ? 0.0 : log2(L);
+    const double lse = bad ? NAN : none ? -INFINITY : LN2 * ((double)M * rf64 + lg);
+    if (tid == 0) {
         if (p.lse) p.lse[q] = (float)lse;
-        if (p.entropy) p.entropy[q] = (float)(bad ? NAN : empty ? 0.0 : LN2 * (lg - A / L));
-        s_lse = lse;
-        s_bad = bad ? 2 : empty ? 1 : 0;
+        if (p.entropy) p.entropy[q] = (float)(bad ? NAN : none ? 0.0 : LN2 * (lg - A / L));
     }
 
-    const int sub = lane & 7, per = WARPS * 4;  // rows scored at a time
-    const int slot = warp * 4 + (lane >> 3);
+    // rows ci[from, to) scored exactly
+    const bool wide = ((reinterpret_cast<uintptr_t>(xp) | (p.ldx * sizeof(T))) & 15) == 0;
+    const int lanes = p.d * (int)sizeof(T) <= 512 ? 8 : 32;
+    const int sub = lane & (lanes - 1);
     auto score = [&](int from, int to) {
+        const int per = THREADS_ / lanes;
         for (int i = from; i < to; i += per) {
-            const int j = i + slot;
-            const double s = dot8<T>(qp, xp + (size_t)(j < to ? ci[j] : 0) * p.ldx, p.d, sub);
-            if (sub == 0 && j < to) cs[j] = s;
+            const int j = i + tid / lanes;
+            const double v = dot_lanes<T>(xp + (size_t)(j < to ? ci[j] : 0) * p.ldx, qs, p.d, sub,
+                                          lanes, wide);
+            if (sub == 0 && j < to) cs[j] = v;
         }
     };
-    if (p.k > 0) {
-        // ---- the best k + 8 groups ----
-        const int want = (int)min((size_t)(p.k + PAD), p.groups);
-        const float2* top = p.top + (size_t)ql * p.groups;
-        WarpTop wt(buf[warp], want, lane);
-        for (size_t g0 = (size_t)warp * 32; g0 < p.groups; g0 += WARPS * 128) {
-            float2 v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const size_t gi = g0 + (size_t)i * WARPS * 32 + lane;
-                v[i] = gi < p.groups ? top[gi] : make_float2(NONE, NONE);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const size_t gi = g0 + (size_t)i * WARPS * 32 + lane;
-                uint64_t key = 0;
-                if (v[i].x > NONE_BELOW)
-                    // (without the mark: equal scores by group number)
-                    key = (uint64_t)ordered(__uint_as_float(__float_as_uint(v[i].x) & ~15u)) << 32 |
-                          (uint32_t)~(uint32_t)gi;
-                wt.offer(key);
-            }
+    auto seen = [&](uint32_t id) {
+        return id < (uint32_t)p.n && (!al || (al[id >> 5] >> (id & 31) & 1u));
+    };
+
+    // ---- groups that reach the bound, the marked pair of each a candidate ----
+    const float bound = p.k > 0 && !bad ? s_bound : INFINITY;
+#pragma unroll 4
+    for (int i = tid; i < groups; i += THREADS_) {
+        const float2 m = top[i];
+        if (m.x > NONE_BELOW && unmarked(m.x) >= bound) {
+            const int at = atomicAdd(&s_picked, 1);
+            if (at < PICKED) sel[at] = i, sel_m[at] = m;
         }
-        wt.shrink();
-        if (lane == 0) red[warp][0] = (double)wt.cnt;
-        __syncthreads();
-        if (warp == 0) {
-            for (int w = 1; w < WARPS; ++w) {
-                const int c = (int)red[w][0];
-                for (int i = 0; i < c; i += 32) wt.offer(i + lane < c ? buf[w][i + lane] : 0ull);
-            }
-            wt.shrink();
-            for (int i = lane; i < wt.cnt; i += 32) {
-                const uint32_t gi = ~(uint32_t)buf[0][i];
-                const float2 v = top[gi];
-                sel[i] = (int)gi;
-                sel2[i] = v.y;
-                const uint32_t pair = __float_as_uint(v.x) & 15u;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t id = gi * GROUP + pair * 2 + h;
-                    const bool ok = id < (uint32_t)p.n && (!al || (al[id >> 5] >> (id & 31) & 1u));
-                    if (ok) ci[atomicAdd(&s_cnt, 1)] = id;
-                }
-            }
-            if (lane == 0) {
-                red[0][1] = (double)wt.cnt;
-                // the largest a group that was not picked can hold
-                red[0][2] = wt.cnt == want && (size_t)want < p.groups
-                                ? (double)unordered((uint32_t)(buf[0][want - 1] >> 32))
-                                : -INFINITY;
-            }
-        }
-        __syncthreads();
     }
+    __syncthreads();
+    const int picked = s_picked;
+    bool all_groups = picked > PICKED;  // (many equal scores)
+    if (!all_groups && tid < picked) {
+        const uint32_t pair = __float_as_uint(sel_m[tid].x) & 15u;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t id = (uint32_t)sel[tid] * GROUP + pair * 2 + h;
+            if (seen(id)) ci[atomicAdd(&s_cnt, 1)] = id;
+        }
+    }
+    if (THREADS_ < PICKED && !all_groups && tid + THREADS_ < picked) {
+        const uint32_t pair = __float_as_uint(sel_m[tid + THREADS_].x) & 15u;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t id = (uint32_t)sel[tid + THREADS_] * GROUP + pair * 2 + h;
+            if (seen(id)) ci[atomicAdd(&s_cnt, 1)] = id;
+        }
+    }
+    __syncthreads();
+    // the row whose log probability is asked for comes last
     int cnt = s_cnt;
-    const int nsel = p.k > 0 ? (int)red[0][1] : 0;
-    const double left_out = p.k > 0 ? red[0][2] : -INFINITY;
+    if (tid == 0) ci[cnt] = given ? (uint32_t)target : 0u;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        ci[cnt] = given ? (uint32_t)target : 0u;
-        s_kth = -INFINITY;
-    }
+    if (given || cnt > 0) score(0, cnt + 1);
     __syncthreads();
-    score(0, cnt + 1);
-    __syncthreads();
-    // ---- the given row ----
-    const double lse = s_lse;
-    const int bad = s_bad;
-    if (threadIdx.x == 0 && p.logprob) {
-        float v = 0.0f;
-        if (given) {
-            const bool seen = !al || (al[target >> 5] >> (target & 31) & 1u);
-            v = bad == 2 ? NAN
-                : (bad == 1 || !seen) ? -INFINITY
-                                      : (float)(cs[cnt] * (double)p.scale - lse);
-        } else if (bad == 2) {
-            v = NAN;
-        }
+    if (tid == 0 && p.logprob) {
+        float v = bad ? NAN : 0.0f;
+        if (given && !bad)
+            v = none || !seen((uint32_t)target) ? -INFINITY
+                                                : (float)(cs[cnt] * (double)p.scale - lse);
         p.logprob[q] = v;
     }
     if (p.k == 0) return;
+
     // candidate i before candidate j
     auto before = [&](int i, int j) { return cs[i] > cs[j] || (cs[i] == cs[j] && ci[i] < ci[j]); };
     // Whether a score of at most `m` (as a group left it) may be among the best
     // k, whose last exact score so far is s_kth: marks and 32-bit sums move it
     // by far less than 2^-15 of the larger of the two.
     auto may_enter = [&](double m) {
-        const double v = m * f, kth = s_kth;
+        const double v = m * (double)f, kth = s_kth;
         return v >= kth - ldexp(fabs(v) + fabs(kth), -15);
     };
-    // ---- groups whose second largest score may still enter ----
-    for (int i = threadIdx.x; i < cnt; i += WARPS * 32) {
+    for (int i = tid; i < cnt; i += THREADS_) {
         int rank = 0;
         for (int j = 0; j < cnt; ++j) rank += before(j, i);
         if (rank == p.k - 1) s_kth = cs[i];
     }
     __syncthreads();
-    if (left_out > (double)NONE_BELOW && may_enter(left_out)) {
-        // ---- more groups are as good (many equal or nearly equal scores):
-        // every row of every group that may enter is scored, the best k kept ----
+    // ---- groups whose second largest score may still enter: their other rows ----
+    const bool more = bound > NONE_BELOW && may_enter(bound);  // groups below the bound may
+    if (!all_groups && !more && !bad) {
+        for (int i = tid; i < picked; i += THREADS_) {
+            const float2 m = sel_m[i];
+            if (!(m.y > NONE_BELOW) || !may_enter(m.y)) continue;
+            const uint32_t pair = __float_as_uint(m.x) & 15u, g0 = (uint32_t)sel[i] * GROUP;
+            uint32_t rest = allowed_word(al, 0, 0, g0, p.n) & ~(3u << (2 * pair));
+            int at = atomicAdd(&s_cnt, __popc(rest));
+            while (rest) {
+                if (at < CAND) ci[at] = g0 + (uint32_t)(__ffs(rest) - 1);
+                ++at;
+                rest &= rest - 1;
+            }
+        }
         __syncthreads();
-        if (threadIdx.x == 0) s_cnt = 0;
-        const float2* top = p.top + (size_t)ql * p.groups;
-        for (size_t g0 = 0; g0 < p.groups; g0 += WARPS) {
+        if (s_cnt <= CAND) score(cnt, s_cnt);
+    }
+    __syncthreads();
+    all_groups = !bad && (all_groups || more || s_cnt > CAND);
+    __syncthreads();
+    if (all_groups) {
+        // ---- too many groups are as good (many equal or nearly equal scores):
+        // every row of every group that may enter is scored, the best k kept ----
+        if (tid == 0) s_cnt = 0;
+        for (int g0 = 0; g0 < groups; g0 += W) {
             __syncthreads();
-            const size_t gi = g0 + warp;
-            const float m1 = gi < p.groups ? top[gi].x : NONE;
+            const int gi = g0 + warp;
+            const float m1 = gi < groups ? top[gi].x : NONE;
             if (m1 > NONE_BELOW && may_enter(m1)) {
-                const uint32_t w = allowed_word(al, 0, 0, gi * GROUP, p.n);
-                for (int i = 0; i < 8; ++i) {
-                    const uint32_t r = (uint32_t)(i * 4 + (lane >> 3));
+                const uint32_t w = allowed_word(al, 0, 0, (size_t)gi * GROUP, p.n);
+                for (int i = 0; i < GROUP; i += 32 / lanes) {
+                    const uint32_t r = (uint32_t)(i + lane / lanes);
                     const bool in = w >> r & 1u;
                     const uint32_t id = (uint32_t)gi * GROUP + r;
-                    const double v = dot8<T>(qp, xp + (size_t)(in ? id : 0) * p.ldx, p.d, sub);
+                    const double v = dot_lanes<T>(xp + (size_t)(in ? id : 0) * p.ldx, qs, p.d, sub,
+                                                  lanes, wide);
                     if (sub == 0 && in && !(v < s_kth)) {
                         const int at = atomicAdd(&s_cnt, 1);
                         cs[at] = v;
@@ -1276,103 +1366,98 @@ __global__ void __launch_bounds__(WARPS * 32) finish_kernel(const FinishArgs p) 
             }
             __syncthreads();
             const int have = s_cnt;
-            if (have + WARPS * GROUP > CAND || g0 + WARPS >= p.groups) {
-                for (int i = threadIdx.x; i < have; i += WARPS * 32) {
+            if (have + W * GROUP > CAND || g0 + W >= groups) {
+                for (int i = tid; i < have; i += THREADS_) {
                     int rank = 0;
                     for (int j = 0; j < have; ++j) rank += before(j, i);
                     if (rank < p.k) kept[rank] = cs[i], kept_id[rank] = ci[i];
                 }
                 __syncthreads();
                 const int keep = min(have, p.k);
-                for (int i = threadIdx.x; i < keep; i += WARPS * 32)
-                    cs[i] = kept[i], ci[i] = kept_id[i];
-                if (threadIdx.x == 0) {
+                for (int i = tid; i < keep; i += THREADS_) cs[i] = kept[i], ci[i] = kept_id[i];
+                if (tid == 0) {
                     s_cnt = keep;
                     if (keep == p.k) s_kth = kept[p.k - 1];
                 }
             }
         }
         __syncthreads();
-        cnt = s_cnt;
-    } else if (threadIdx.x < nsel) {
-        const int gi = sel[threadIdx.x];
-        const float m2 = sel2[threadIdx.x];
-        if (m2 > NONE_BELOW && may_enter(m2)) {
-            const uint32_t pair = __float_as_uint(p.top[(size_t)ql * p.groups + gi].x) & 15u;
-            const uint32_t g0 = (uint32_t)gi * GROUP;
-            const uint32_t w = allowed_word(al, 0, 0, g0, p.n);
-            uint32_t rest = w & ~(3u << (2 * pair));
-            int at = atomicAdd(&s_cnt, __popc(rest));
-            while (rest) {
-                ci[at++] = g0 + (uint32_t)(__ffs(rest) - 1);
-                rest &= rest - 1;
-            }
-        }
     }
-    __syncthreads();
-    const int all = s_cnt;
-    score(cnt, all);
-    __syncthreads();
     // ---- written in order ----
-    for (int i = threadIdx.x; i < all; i += WARPS * 32) {
+    const int have = bad ? 0 : s_cnt;
+    for (int i = tid; i < have; i += THREADS_) {
         int rank = 0;
-        for (int j = 0; j < all; ++j) rank += before(j, i);
-        if (rank < p.k && bad == 0) {
+        for (int j = 0; j < have; ++j) rank += before(j, i);
+        if (rank < p.k) {
             p.top_ids[(size_t)q * p.k + rank] = (int64_t)ci[i];
             p.top_logprob[(size_t)q * p.k + rank] = (float)(cs[i] * (double)p.scale - lse);
         }
     }
-    for (int i = (bad ? 0 : all) + (int)threadIdx.x; i < p.k; i += WARPS * 32) {
+    for (int i = have + tid; i < p.k; i += THREADS_) {
         p.top_ids[(size_t)q * p.k + i] = -1;
-        p.top_logprob[(size_t)q * p.k + i] = bad == 2 ? NAN : -INFINITY;
+        p.top_logprob[(size_t)q * p.k + i] = bad ? NAN : -INFINITY;
     }
 }
 
 // ---------------------------------------------------------------------------
 // backward: what the products need
 // ---------------------------------------------------------------------------
-// Rows some query may see: the OR of the filters.
-__global__ void any_kernel(const uint32_t* __restrict__ allowed, size_t ld, int nq, size_t words,
-                           uint32_t* __restrict__ out) {
-    const size_t w = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (w >= words) return;
-    uint32_t r = 0;
-    for (int q = blockIdx.y; q < nq; q += gridDim.y) r |= allowed[(size_t)q * ld + w];
-    if (r) atomicOr(out + w, r);
-}
-// Queries that see anything, as bits (an empty one is taken as zeros, so that
-// what it holds cannot set the scale of the others).
-__global__ void alive_kernel(const float* __restrict__ lse, int nq, uint32_t* __restrict__ out) {
+// Clears the head of the workspace and marks the queries that see anything,
+// as bits (an empty one is taken as zeros, so that what it holds cannot set
+// the scale of the others).
+__global__ void head_kernel(const float* __restrict__ lse, int nq, uint32_t* __restrict__ alive,
+                            uint32_t* __restrict__ head, int head_words) {
     const int q = blockIdx.x * blockDim.x + threadIdx.x;
+    if (q < head_words) head[q] = 0u;
     const bool on = q < nq && !(lse[q] == -INFINITY);
     const unsigned b = __ballot_sync(0xffffffffu, on);
-    if ((threadIdx.x & 31) == 0 && q < nq) out[q >> 5] = b;
+    if ((threadIdx.x & 31) == 0 && q < nq) alive[q >> 5] = b;
+}
+// Rows some query may see: the OR of the filters, 32 words a block.
+__global__ void __launch_bounds__(256)
+    any_kernel(const uint32_t* __restrict__ allowed, size_t ld, int nq, size_t words,
+               uint32_t* __restrict__ out) {
+    __shared__ uint32_t part[8][32];
+    const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
+    const size_t w = (size_t)blockIdx.x * 32 + lane;
+    uint32_t r = 0;
+    if (w < words) {
+#pragma unroll 8
+        for (int q = row; q < nq; q += 8) r |= __ldg(allowed + (size_t)q * ld + w);
+    }
+    part[row][lane] = r;
+    __syncthreads();
+    if (row == 0 && w < words) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) r |= part[i][lane];
+        out[w] = r;
+    }
 }
 // The products sum over rows (or queries) whose scales 2^-e differ; the stored
 // score gradients carry the factor, so a row far below the largest would leave
 // too few bits there.  Such a row (below 2^-4 of the largest scale; also one
 // of zeros or with a NaN, whose elements are zeros) takes a larger scale and
-// is shifted down instead.  One warp per row, almost none has work.
-__global__ void __launch_bounds__(256)
-    fix_kernel(__half* __restrict__ x, float* __restrict__ f, int n, int width,
-               const float* __restrict__ largest) {
+// is shifted down instead.  Almost none has work.
+__device__ __forceinline__ float fix_row(__half* x, float* f, int row, int width, float mx) {
     const int lane = threadIdx.x & 31;
-    const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (row >= n) return;
-    const float mx = *largest, v = f[row];
+    const float v = f[row];
+    float now = v;
     if (!(mx > 0.0f)) {
-        if (lane == 0) f[row] = 1.0f;
-        return;
-    }
-    const float least = mx * 0x1p-4f;
-    if (v >= least) return;
-    if (v > 0.0f) {
-        const float s = v / least;
-        __half* h = x + (size_t)row * width;
-        for (int c = lane; c < width; c += 32) h[c] = __float2half_rn(__half2float(h[c]) * s);
+        now = 1.0f;
+    } else {
+        const float least = mx * 0x1p-4f;
+        if (v >= least) return v;
+        if (v > 0.0f) {
+            const float s = v / least;
+            __half* h = x + (size_t)row * width;
+            for (int c = lane; c < width; c += 32)
+                h[c] = __float2half_rn(__half2float(h[c]) * s);
+        }
+        now = v > 0.0f ? least : mx;
     }
     __syncwarp();
-    if (lane == 0) f[row] = v > 0.0f ? least : mx;
+    if (lane == 0) f[row] = now;
+    return now;
 }
 struct CoefArgs {
     int nq, n;
@@ -1381,19 +1466,15 @@ struct CoefArgs {
     const int64_t* targets;
     const uint32_t* allowed;
     size_t ld_allowed;
-    const float* qf;
     Coef* out;
     float* bounds;  // [0]
 };
 // G_ij = scale [ p_ij (dl - g - h (lp_ij + H)) + g 1{j = t} ] with lp = ln2 x:
 // = p (c + h' x) + g', and a bound of its size for the common scale
 // (p |lp| <= 1/e).
-__global__ void coef_kernel(const CoefArgs a) {
-    const int i = blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= a.nq) return;
+__device__ __forceinline__ void coef_of(const CoefArgs& a, int i, float f) {
     const float lse = a.lse[i];
     const bool empty = lse == -INFINITY;
-    const float f = a.qf[i];
     const double rf = (double)f * a.scale * LOG2E, l = (double)lse * LOG2E;
     const int64_t t = a.targets ? a.targets[i] : -1;
     const bool given = !empty && t >= 0 && t < a.n &&
@@ -1418,34 +1499,78 @@ __global__ void coef_kernel(const CoefArgs a) {
     if (b > 0.0f && b <= FLT_MAX)
         atomicMax(reinterpret_cast<unsigned*>(a.bounds), __float_as_uint(b));
 }
-// Sum of the splits, scaled, in the output's type.
+// One warp per row of either operand: its scale settled, and per query its
+// coefficients.  Queries come first.
+__global__ void __launch_bounds__(256)
+    settle_kernel(const CoefArgs a, __half* qp, float* qf, __half* xp, float* xf, int width,
+                  int qblocks) {
+    if ((int)blockIdx.x < qblocks) {
+        const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
+        if (row >= a.nq) return;
+        const float f = fix_row(qp, qf, row, width, a.bounds[2]);
+        if ((threadIdx.x & 31) == 0) coef_of(a, row, f);
+        return;
+    }
+    // rows: a lane looks at one, the warp mends those that need it
+    const int row0 = (((int)blockIdx.x - qblocks) * 8 + (threadIdx.x >> 5)) * 32;
+    const int row = row0 + (threadIdx.x & 31);
+    const float mx = a.bounds[1];
+    unsigned todo = __ballot_sync(
+        0xffffffffu, row < a.n && !(mx > 0.0f && xf[row < a.n ? row : 0] >= mx * 0x1p-4f));
+    while (todo) {
+        fix_row(xp, xf, row0 + __ffs(todo) - 1, width, mx);
+        todo &= todo - 1;
+    }
+}
+__device__ __forceinline__ void put(void* out, size_t o, int dtype, float v) {
+    if (dtype == FDB_DTYPE_F32) static_cast<float*>(out)[o] = v;
+    else if (dtype == FDB_DTYPE_BF16) static_cast<__nv_bfloat16*>(out)[o] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(out)[o] = __float2half_rn(v);
+}
+// Sum of the splits in order, scaled, in the output's type: four columns a
+// thread.
 __global__ void __launch_bounds__(256)
     join_kernel(const float* __restrict__ partial, int splits, int rows, int cols,
                 const float* __restrict__ f, const float* __restrict__ bounds, void* out,
                 size_t ldo, int dtype) {
-    const size_t per = (size_t)rows * cols;
+    const unsigned per4 = (unsigned)(cols + 3) / 4;
+    const size_t plane = (size_t)rows * cols, all = (size_t)rows * per4;
+    const bool wide = (cols & 3) == 0;
     const float c = grad_factor(bounds);
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < per; i += (size_t)gridDim.x * 256) {
-        const size_t r = i / cols, k = i - r * cols;
-        float s = 0.0f;
-        for (int j = 0; j < splits; ++j) s += partial[(size_t)j * per + i];
-        s *= 1.0f / (f[r] * c);
-        const size_t o = r * ldo + k;
-        if (dtype == FDB_DTYPE_F32) static_cast<float*>(out)[o] = s;
-        else if (dtype == FDB_DTYPE_BF16)
-            static_cast<__nv_bfloat16*>(out)[o] = __float2bfloat16_rn(s);
-        else static_cast<__half*>(out)[o] = __float2half_rn(s);
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (size_t)gridDim.x * 256) {
+        const size_t r = i / per4;
+        const int k = (int)(i - r * per4) * 4;
+        const float* src = partial + r * cols + k;
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (wide) {
+#pragma unroll 4
+            for (int j = 0; j < splits; ++j) {
+                const float4 t = __ldcs(reinterpret_cast<const float4*>(src + j * plane));
+                v[0] += t.x, v[1] += t.y, v[2] += t.z, v[3] += t.w;
+            }
+        } else {
+            for (int j = 0; j < splits; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (k + e < cols) v[e] += src[j * plane + e];
+        }
+        const float s = 1.0f / (f[r] * c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (k + e < cols) put(out, r * ldo + k + e, dtype, v[e] * s);
     }
 }
 // A call whose waits ran out has no gradient: NaN.
-__global__ void void_kernel(const int* err, void* out, size_t ldo, int rows, int cols, int dtype) {
+__global__ void void_kernel(const int* err, void* dq, size_t ldq, int nq, void* dx, size_t ldx,
+                            int n, int cols, int dtype) {
     if (*err == 0) return;
-    const size_t per = (size_t)rows * cols;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < per; i += (size_t)gridDim.x * 256) {
-        const size_t o = i / cols * ldo + i % cols;
-        if (dtype == FDB_DTYPE_F32) static_cast<float*>(out)[o] = NAN;
-        else static_cast<uint16_t*>(out)[o] = 0x7fff;  // NaN in both 16-bit types
-    }
+    const size_t step = (size_t)gridDim.x * 256, i0 = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (dq)
+        for (size_t i = i0; i < (size_t)nq * cols; i += step)
+            put(dq, i / cols * ldq + i % cols, dtype, NAN);
+    if (dx)
+        for (size_t i = i0; i < (size_t)n * cols; i += step)
+            put(dx, i / cols * ldx + i % cols, dtype, NAN);
 }
 
 // ---------------------------------------------------------------------------
@@ -1456,7 +1581,8 @@ constexpr size_t CHUNK_BYTES = (size_t)512 << 20;  // of group maxima, of score 
 constexpr int FEW = 8;                          // f32 queries a pass of few_kernel takes
 constexpr int FEW_QUERIES = 16, FEW_DIM = 2048;
 static size_t smem_of(bool two) {
-    return 1024 + (size_t)stages_of(two) * stage_bytes(two) + (2 * MAX_STG + 2 * MAX_ACC) * 8 + 16;
+    // alignment, stages, barriers, column factors
+    return 1024 + (size_t)stages_of(two) * stage_bytes(two) + 256 + EPI_WARPS * 64 * 4;
 }
 
 static size_t up(size_t v, size_t m) { return (v + m - 1) / m * m; }
@@ -1498,15 +1624,18 @@ static int pick_chunks(int mt, int nt, int sms) {
     }
     return best;
 }
-// Splits of K of a product with `tiles` output tiles: each costs a pass over
-// the partial sums, taken as 2% of the product.
-static int pick_splits(int tiles, int atoms, int sms) {
+// Splits of K of a rows x cols product.  A block runs the busiest share of the
+// (tile, split) pairs at about 0.3 us per 64 of K (f32: 0.5); more than one
+// split writes and reads `out_bytes` of partial sums each, at 4 MB/us, and
+// takes another launch (3 us).
+static int pick_splits(int tiles, int atoms, int sms, bool two, double out_bytes) {
     sms = std::max(sms, 1);
     int best = 1;
     double cost = -1.0;
     for (int s = 1; s <= atoms && s <= 64; ++s) {
         const long long waves = ((long long)tiles * s + sms - 1) / sms;
-        const double t = (double)waves * ((atoms + s - 1) / s) * (1.0 + 0.02 * (s - 1));
+        double t = (double)waves * ((atoms + s - 1) / s) * (two ? 0.5 : 0.3);
+        if (s > 1) t += 3.0 + s * out_bytes * 2.0 / 4e6;
         if (cost < 0.0 || t < cost) cost = t, best = s;
     }
     return best;
@@ -1545,11 +1674,23 @@ struct Carve {
     }
 };
 
-template <typename T, int PARTS>
-static void launch_pack(cudaStream_t s, const void* x, size_t ld, size_t n, size_t d, size_t kp,
-                        const uint32_t* seen, __half* out, float* f, unsigned* largest) {
-    pack_kernel<T, PARTS><<<(unsigned)((n + 7) / 8), 256, 0, s>>>(
-        static_cast<const T*>(x), ld, (int)n, (int)d, (int)kp, seen, out, f, largest);
+static PackSide pack_side(const void* x, size_t ld, size_t n, size_t dim, int dtype,
+                          const uint32_t* seen, __half* out, float* f, unsigned* largest) {
+    PackSide p;
+    p.x = x, p.ld = ld, p.n = (int)n, p.seen = seen, p.out = out, p.f = f, p.largest = largest;
+    p.blocks = (int)((n + 7) / 8);
+    const size_t es = elem(dtype);
+    p.wide = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ld * es & 15) == 0 &&
+             (dim * es & 15) == 0;
+    return p;
+}
+static void launch_pack(cudaStream_t s, int dtype, const PackSide& a, const PackSide& b, size_t d,
+                        size_t kp, int* err) {
+    const unsigned blocks = (unsigned)(a.blocks + b.blocks);
+    const int D = (int)d, K = (int)kp;
+    if (dtype == FDB_DTYPE_F32) pack_kernel<float, 2><<<blocks, 256, 0, s>>>(a, b, D, K, err);
+    else if (dtype == FDB_DTYPE_F16) pack_kernel<__half, 1><<<blocks, 256, 0, s>>>(a, b, D, K, err);
+    else pack_kernel<__nv_bfloat16, 1><<<blocks, 256, 0, s>>>(a, b, D, K, err);
     FDB_LAUNCH_CHECK();
 }
 
@@ -1574,7 +1715,7 @@ static Forward plan_forward(const Ctx& c, const fdb_logprob_args& a) {
     w.err = ws.take<int>(HEAD / 4);
     w.few = a.dtype == FDB_DTYPE_F32 && a.nq <= FEW_QUERIES && a.dim <= FEW_DIM;
     w.packed = a.dtype == FDB_DTYPE_F32 && !w.few;
-    w.kp = up(a.dim, 64);
+    w.kp = up(a.dim, 16);
     w.bn = bn_of(w.packed);
     w.nt = (int)((a.n + w.bn - 1) / w.bn);
     w.groups = w.few ? (a.n + GROUP - 1) / GROUP : (size_t)w.nt * (w.bn / GROUP);
@@ -1615,14 +1756,20 @@ size_t forward_bytes(const Ctx& c, const fdb_logprob_args& a) {
     return plan_forward(c, b).bytes;
 }
 
+template <typename T, int THREADS_>
+static void launch_finish_t(cudaStream_t s, const FinishArgs& f) {
+    const size_t smem = (size_t)f.d * 4;
+    if (smem > 8192)
+        FDB_CUDA(cudaFuncSetAttribute(finish_kernel<T, THREADS_>,
+                                      cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    finish_kernel<T, THREADS_><<<f.nq, THREADS_, smem, s>>>(f);
+    FDB_LAUNCH_CHECK();
+}
 template <typename T>
 static void launch_finish(cudaStream_t s, const FinishArgs& f) {
-    // A block a query.  Few queries: sixteen warps share the groups of one.
-    if (f.nq <= 64)
-        finish_kernel<T, 16><<<f.nq, 512, 0, s>>>(f);
-    else
-        finish_kernel<T, 4><<<f.nq, 128, 0, s>>>(f);
-    FDB_LAUNCH_CHECK();
+    // A block a query.  Few queries: more threads share the groups of one.
+    if (f.nq <= 296) launch_finish_t<T, 512>(s, f);
+    else launch_finish_t<T, 128>(s, f);
 }
 
 void forward_run(Ctx& c, const fdb_logprob_args& a) {
@@ -1634,14 +1781,16 @@ void forward_run(Ctx& c, const fdb_logprob_args& a) {
     Mma g{};
     CUtensorMap amap, bmap;
     if (!w.few) {
-        FDB_CUDA(cudaMemsetAsync(w.err, 0, HEAD, s));
+        if (!w.packed) FDB_CUDA(cudaMemsetAsync(w.err, 0, 4, s));
         const void *qb = a.queries, *xb = a.rows;
         size_t ldq = a.ld_queries, ldx = a.ld_rows, inner = a.dim;
         if (w.packed) {
-            launch_pack<float, 2>(s, a.queries, a.ld_queries, a.nq, a.dim, w.kp, nullptr,
-                                  static_cast<__half*>(w.qp), w.qf, nullptr);
-            launch_pack<float, 2>(s, a.rows, a.ld_rows, a.n, a.dim, w.kp, nullptr,
-                                  static_cast<__half*>(w.xp), w.xf, nullptr);
+            launch_pack(s, a.dtype,
+                        pack_side(a.queries, a.ld_queries, a.nq, a.dim, a.dtype, nullptr,
+                                  static_cast<__half*>(w.qp), w.qf, nullptr),
+                        pack_side(a.rows, a.ld_rows, a.n, a.dim, a.dtype, nullptr,
+                                  static_cast<__half*>(w.xp), w.xf, nullptr),
+                        a.dim, w.kp, w.err);
             qb = w.qp, xb = w.xp;
             ldq = ldx = inner = 2 * w.kp;
         }
@@ -1661,8 +1810,8 @@ void forward_run(Ctx& c, const fdb_logprob_args& a) {
         }
         bmap = map2d(a.dtype, xb, inner, a.n, ldx, 128);
         g.nt = w.nt;
-        g.atoms = (int)(w.kp / 64);
-        g.klast = (int)((a.dim - 64 * (w.kp / 64 - 1) + 15) / 16);
+        g.atoms = (int)((w.kp + 63) / 64);
+        g.klast = (int)((w.kp - 64 * (size_t)(g.atoms - 1)) / 16);
         g.a_part = g.b_part = (int)w.kp;
         g.idesc = idesc_of(w.packed ? FDB_DTYPE_F16 : a.dtype, false, false);
         g.err = w.err;
@@ -1719,7 +1868,7 @@ void forward_run(Ctx& c, const fdb_logprob_args& a) {
             kernel<<<blocks, 64, sm, s>>>(static_cast<const float*>(a.rows), a.ld_rows, n, d,
                                           static_cast<const float*>(a.queries), a.ld_queries,
                                           (int)q0, nq, rf, a.allowed, ld_allowed, w.part, w.top,
-                                          w.groups);
+                                          w.groups, w.err);
             FDB_LAUNCH_CHECK();
         };
         if (nq == 1) vec ? go(few_kernel<1, true>, 1) : go(few_kernel<1, false>, 1);
@@ -1758,7 +1907,7 @@ static Backward plan_backward(const Ctx& c, const fdb_logprob_grad_args& a) {
     Backward w{};
     Carve ws(a.workspace);
     w.parts = a.dtype == FDB_DTYPE_F32 ? 2 : 1;
-    w.kp = up(a.dim, 64);
+    w.kp = up(a.dim, 16);
     w.nqp = up(a.nq, BM);
     w.bn = bn_of(w.parts == 2);
     const size_t row_bytes = w.nqp * 2 * w.parts;
@@ -1766,9 +1915,10 @@ static Backward plan_backward(const Ctx& c, const fdb_logprob_grad_args& a) {
                               a.n);
     w.ldg = up(w.cols, 64);
     const int ntd = (int)((a.dim + w.bn - 1) / w.bn);
-    w.q_splits = pick_splits((int)(w.nqp / BM) * ntd, (int)((w.cols + 63) / 64), c.sm_count);
+    w.q_splits = pick_splits((int)(w.nqp / BM) * ntd, (int)((w.cols + 63) / 64), c.sm_count,
+                             w.parts == 2, (double)a.nq * a.dim * 4);
     w.x_splits = pick_splits((int)((w.cols + BM - 1) / BM) * ntd, (int)((a.nq + 63) / 64),
-                             c.sm_count);
+                             c.sm_count, w.parts == 2, (double)w.cols * a.dim * 4);
     unsigned char* head = ws.take<unsigned char>(HEAD);
     w.err = reinterpret_cast<int*>(head);
     w.bounds = reinterpret_cast<float*>(head ? head + 64 : nullptr);
@@ -1796,43 +1946,32 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
     const Backward w = plan_backward(c, a);
     const int n = (int)a.n, d = (int)a.dim, nq = (int)a.nq;
     const size_t ld_allowed = a.allowed ? a.ld_allowed : 0;
-    FDB_CUDA(cudaMemsetAsync(w.err, 0, HEAD, s));
+    head_kernel<<<(nq + 255) / 256, 256, 0, s>>>(a.lse, nq, w.alive,
+                                                 reinterpret_cast<uint32_t*>(w.err), HEAD / 4);
+    FDB_LAUNCH_CHECK();
     const uint32_t* seen = a.allowed;
     if (w.seen) {
         const size_t words = (a.n + 31) / 32;
-        FDB_CUDA(cudaMemsetAsync(w.seen, 0, words * 4, s));
-        const unsigned gx = (unsigned)((words + 255) / 256);
-        any_kernel<<<dim3(gx, (unsigned)std::min<size_t>(a.nq, std::max(1u, 1184 / gx))), 256, 0,
-                     s>>>(a.allowed, a.ld_allowed, nq, words, w.seen);
+        any_kernel<<<(unsigned)((words + 31) / 32), 256, 0, s>>>(a.allowed, a.ld_allowed, nq, words,
+                                                                 w.seen);
         FDB_LAUNCH_CHECK();
         seen = w.seen;
     }
-    alive_kernel<<<(nq + 255) / 256, 256, 0, s>>>(a.lse, nq, w.alive);
-    FDB_LAUNCH_CHECK();
-    unsigned* qmax = reinterpret_cast<unsigned*>(w.bounds + 2);
-    unsigned* xmax = reinterpret_cast<unsigned*>(w.bounds + 1);
-    auto pack = [&](const void* x, size_t ld, size_t rows, const uint32_t* bits, __half* out,
-                    float* f, unsigned* mx) {
-        if (a.dtype == FDB_DTYPE_F32)
-            launch_pack<float, 2>(s, x, ld, rows, a.dim, w.kp, bits, out, f, mx);
-        else if (a.dtype == FDB_DTYPE_F16)
-            launch_pack<__half, 1>(s, x, ld, rows, a.dim, w.kp, bits, out, f, mx);
-        else
-            launch_pack<__nv_bfloat16, 1>(s, x, ld, rows, a.dim, w.kp, bits, out, f, mx);
-        fix_kernel<<<(unsigned)((rows + 7) / 8), 256, 0, s>>>(out, f, (int)rows,
-                                                              w.parts * (int)w.kp,
-                                                              reinterpret_cast<float*>(mx));
-        FDB_LAUNCH_CHECK();
-    };
-    pack(a.queries, a.ld_queries, a.nq, w.alive, w.qp, w.qf, qmax);
-    pack(a.rows, a.ld_rows, a.n, seen, w.xp, w.xf, xmax);
+    launch_pack(s, a.dtype,
+                pack_side(a.queries, a.ld_queries, a.nq, a.dim, a.dtype, w.alive, w.qp, w.qf,
+                          reinterpret_cast<unsigned*>(w.bounds + 2)),
+                pack_side(a.rows, a.ld_rows, a.n, a.dim, a.dtype, seen, w.xp, w.xf,
+                          reinterpret_cast<unsigned*>(w.bounds + 1)),
+                a.dim, w.kp, nullptr);
     CoefArgs k{};
     k.nq = nq, k.n = n, k.scale = a.scale;
     k.lse = a.lse, k.entropy = a.entropy;
     k.d_logprob = a.d_logprob, k.d_lse = a.d_lse, k.d_entropy = a.d_entropy;
     k.targets = a.targets, k.allowed = a.allowed, k.ld_allowed = ld_allowed;
-    k.qf = w.qf, k.out = w.coef, k.bounds = w.bounds;
-    coef_kernel<<<(nq + 255) / 256, 256, 0, s>>>(k);
+    k.out = w.coef, k.bounds = w.bounds;
+    const int qblocks = (nq + 7) / 8;
+    settle_kernel<<<qblocks + (n + 255) / 256, 256, 0, s>>>(k, w.qp, w.qf, w.xp, w.xf,
+                                                            w.parts * (int)w.kp, qblocks);
     FDB_LAUNCH_CHECK();
 
     const size_t width = w.parts * w.kp;
@@ -1856,8 +1995,8 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
             g.mt = mtq;
             g.nt = (cols + w.bn - 1) / w.bn;
             g.chunks = pick_chunks(g.mt, g.nt, c.sm_count);
-            g.atoms = (int)(w.kp / 64);
-            g.klast = (int)((a.dim - 64 * (w.kp / 64 - 1) + 15) / 16);
+            g.atoms = (int)((w.kp + 63) / 64);
+            g.klast = (int)((w.kp - 64 * (size_t)(g.atoms - 1)) / 16);
             g.a_part = g.b_part = (int)w.kp;
             g.b_row0 = (int)j0;
             g.idesc = idesc_of(FDB_DTYPE_F16, false, false);
@@ -1909,13 +2048,10 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
         join_kernel<<<c.sm_count * 8, 256, 0, s>>>(w.dq, w.q_splits, nq, d, w.qf, w.bounds,
                                                    a.d_queries, a.ld_d_queries, a.dtype);
         FDB_LAUNCH_CHECK();
-        void_kernel<<<c.sm_count, 256, 0, s>>>(w.err, a.d_queries, a.ld_d_queries, nq, d, a.dtype);
-        FDB_LAUNCH_CHECK();
     }
-    if (a.d_rows) {
-        void_kernel<<<c.sm_count, 256, 0, s>>>(w.err, a.d_rows, a.ld_d_rows, n, d, a.dtype);
-        FDB_LAUNCH_CHECK();
-    }
+    void_kernel<<<c.sm_count, 256, 0, s>>>(w.err, a.d_queries, a.ld_d_queries, nq, a.d_rows,
+                                           a.ld_d_rows, n, d, a.dtype);
+    FDB_LAUNCH_CHECK();
 }
 
 // One thread per row: its id among the sorted wanted ones, the lowest row kept.
