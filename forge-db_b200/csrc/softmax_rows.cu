@@ -55,8 +55,9 @@ constexpr int EPI_WARP0 = 4, EPI_WARPS = 16;
 constexpr int GROUP = 32;                   // rows whose largest scores are kept together
 constexpr int PAD = 8;                      // groups picked beyond k
 constexpr int MAX_SEL = FDB_MAX_ALTERNATIVES + PAD;
-constexpr float NONE = -FLT_MAX;            // score of a row that may not be seen
-constexpr float NONE_BELOW = -3.0e38f;
+constexpr float NONE = -1e30f;              // score of a row that may not be seen
+constexpr float NONE_BELOW = -1e29f;
+constexpr float RAISE = 8.0f;               // see Run
 constexpr double LOG2E = 1.4426950408889634074, LN2 = 0.69314718055994530942;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -64,10 +65,20 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float lo_of(uint64_t v) { return __uint_as_float((uint32_t)v); }
-__device__ __forceinline__ float hi_of(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ float lo_of(uint64_t v) {
+    uint32_t a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
+    return __uint_as_float(a);
+}
+__device__ __forceinline__ float hi_of(uint64_t v) {
+    uint32_t a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
+    return __uint_as_float(b);
+}
 __device__ __forceinline__ uint64_t packf(float a, float b) {
-    return pack2(__float_as_uint(a), __float_as_uint(b));
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(__float_as_uint(a)), "r"(__float_as_uint(b)));
+    return d;
 }
 __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
     uint64_t d;
@@ -91,37 +102,51 @@ __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) {
     return __bfloat162float(v);
 }
 
-// A running (max, sum, weighted sum) of one query's columns, in raw score
-// units u (t = u * rf); rf > 0.
+// A running (reference m, sum l = sum 2^(t - m), a = sum 2^(t - m) (t - m)) of
+// one query's columns, t = score * log2(e).  m starts at the first columns'
+// largest t and is raised only when a t exceeds it by more than RAISE: the
+// sums then hold terms of at most 2^8 (f32's relative precision does not
+// care), and a new largest score seldom costs a rescaling.
 struct Run {
     float m, l, a;
+    float limit;  // -inf before the first columns, then RAISE
 };
-__device__ __forceinline__ void run_raise(Run& r, float cm, float rf) {
-    if (cm > r.m) {
-        if (r.l != 0.0f) {  // (also NaN: it stays)
-            const float d = (r.m - cm) * rf;
-            const float f = ex2(d);
-            r.a = __fmaf_rn(d, r.l, r.a) * f;
-            r.l *= f;
-        }
-        r.m = cm;
+__device__ __forceinline__ Run run_empty() { return Run{0.0f, 0.0f, 0.0f, -INFINITY}; }
+// For columns with largest t - m = cm: what t - m loses (0 mostly).
+__device__ __forceinline__ float run_raise(Run& r, float cm) {
+    if (!(cm > r.limit && cm > NONE_BELOW)) return 0.0f;
+    const float m = r.m + cm, d = m - r.m;  // (d: what m moved by after rounding)
+    r.m = m;
+    r.limit = RAISE;
+    if (!(r.l == 0.0f && r.a == 0.0f)) {
+        const float f = ex2(-d);
+        r.a = __fmaf_rn(-d, r.l, r.a) * f;
+        r.l *= f;
     }
+    return d;
 }
-// r joined with o (both in the same units)
-__device__ __forceinline__ void run_join(Run& r, Run o, float rf) {
-    if (o.m > r.m) {
+__device__ __forceinline__ void run_join(Run& r, Run o) {
+    if (o.limit == -INFINITY) return;
+    if (r.limit == -INFINITY || o.m > r.m) {
         const Run t = r;
         r = o;
         o = t;
     }
     if (!(o.l == 0.0f && o.a == 0.0f)) {
-        const float d = o.m == r.m ? 0.0f : (o.m - r.m) * rf;
-        const float f = ex2(d);
+        const float d = o.m - r.m, f = ex2(d);
         r.a += __fmaf_rn(d, o.l, o.a) * f;
         r.l += o.l * f;
     }
 }
+// As stored: m is -inf for a run without columns.
+__device__ __forceinline__ float4 run_stored(const Run& r) {
+    return make_float4(r.limit == -INFINITY ? -INFINITY : r.m, r.l, r.a, 0.0f);
+}
 
+// A group's largest score without the mark of its pair.
+__device__ __forceinline__ float unmarked(float f) {
+    return __uint_as_float(__float_as_uint(f) & ~15u);
+}
 // The largest of 32 values with the number of its pair in the low 4 bits, and
 // the second largest (either may be moved by the marks: 2^-19 relative).
 __device__ __forceinline__ float2 top_pair(const float (&u)[32]) {
@@ -305,8 +330,8 @@ struct StatsArgs {
     float rf;                   // scale * log2(e)
     const uint32_t* allowed;    // nullable
     size_t ld_allowed;          // words a query (0: one filter for all)
-    float4* part;               // [chunks * 4][nq]: m, l, a
-    float2* top;                // [nq][groups] or null
+    float4* part;               // [chunks * 4][nq]: m, l, a (see Run)
+    float2* top;                // [nq][groups] or null, in units of t
     size_t groups;              // 32-row groups, whole column tiles
 };
 // What the score gradients of one query need (see coef_kernel).
@@ -360,19 +385,6 @@ __device__ __forceinline__ void load_chunk(uint32_t tmem, float (&u)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) u[i] = __uint_as_float(v[i]);
 }
-// `f`: 32 factors in shared memory.
-__device__ __forceinline__ void scale_chunk(const float* f, float (&u)[32]) {
-    const float4* cf = reinterpret_cast<const float4*>(f);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float4 c = cf[i];
-        u[4 * i] *= c.x;
-        u[4 * i + 1] *= c.y;
-        u[4 * i + 2] *= c.z;
-        u[4 * i + 3] *= c.w;
-    }
-}
-
 // What a chunk of 32 columns needs besides its scores: the filter's word of
 // the thread's row, and (scaled rows) the columns' factors, in the warp's own
 // shared memory.  `load` starts the reads of a tile's chunks while the tile
@@ -426,52 +438,77 @@ struct StatsEpilogue {
             const float f = a.qf[q];
             rf = f == 0.0f ? a.rf : f * a.rf;  // a query of zeros scores 0
         }
-        r = Run{-INFINITY, 0.0f, 0.0f};
+        r = run_empty();
     }
     __device__ __forceinline__ void load(int col) { c.load(al, p.xf, (size_t)col, p.n); }
+    // MASKED: some bit of some row's word is clear (two copies of the code: the
+    // selects are not free).
+    template <bool MASKED>
+    __device__ __forceinline__ float2 fold(const float (&u)[32], uint32_t w) {
+        const uint64_t rf2 = packf(rf, rf), nm2 = packf(-r.m, -r.m);
+        float d[32];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            uint64_t t = packf(u[2 * i], u[2 * i + 1]);
+            if (TWO) {
+                const float2 f = reinterpret_cast<const float2*>(c.fac)[i];
+                t = mul2(t, packf(f.x, f.y));
+            }
+            t = fma2(t, rf2, nm2);
+            d[2 * i] = lo_of(t);
+            d[2 * i + 1] = hi_of(t);
+        }
+        if (MASKED) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (!(w >> i & 1u)) d[i] = NONE;
+        }
+        float2 best = make_float2(NONE, NONE);
+        float cm;
+        if (p.top) {
+            best = top_pair(d);
+            // (the mark may have moved it; by far less than RAISE)
+            cm = best.x;
+            if (best.x > NONE_BELOW)
+                best.x = __uint_as_float(
+                    (__float_as_uint(unmarked(best.x) + r.m) & ~15u) |
+                    (__float_as_uint(best.x) & 15u));
+            best.y += r.m;
+        } else {
+            cm = max3(d[0], d[1], d[2]);
+#pragma unroll
+            for (int i = 3; i < 31; i += 2) cm = max3(cm, d[i], d[i + 1]);
+            cm = fmaxf(cm, d[31]);
+        }
+        if (cm > r.limit) {
+            const float by = run_raise(r, cm);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) d[i] -= by;
+        }
+        uint64_t l2[2] = {0, 0}, a2[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const uint64_t e = packf(ex2(d[2 * i]), ex2(d[2 * i + 1]));
+            l2[i & 1] = add2(l2[i & 1], e);
+            a2[i & 1] = fma2(e, packf(d[2 * i], d[2 * i + 1]), a2[i & 1]);
+        }
+        l2[0] = add2(l2[0], l2[1]);
+        a2[0] = add2(a2[0], a2[1]);
+        r.l += lo_of(l2[0]) + hi_of(l2[0]);
+        r.a += lo_of(a2[0]) + hi_of(a2[0]);
+        return best;
+    }
     __device__ __forceinline__ void chunk(float (&u)[32], int icol, int h) {
         if (!live) return;
         const size_t col = (size_t)icol;
         const uint32_t w = h ? c.word[sizeof(c.word) / 4 - 1] : c.word[0];
         float2 best = make_float2(NONE, NONE);
-        if (__any_sync(0xffffffffu, w != 0u)) {
-            if (TWO) scale_chunk(c.fac, u);
-            const bool full = __all_sync(0xffffffffu, w == 0xffffffffu);
-            if (!full) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (!(w >> i & 1u)) u[i] = NONE;
-            }
-            if (p.top) best = top_pair(u);
-            float cm = max3(u[0], u[1], u[2]);
-#pragma unroll
-            for (int i = 3; i < 31; i += 2) cm = max3(cm, u[i], u[i + 1]);
-            cm = fmaxf(cm, u[31]);
-            if (cm > NONE_BELOW) run_raise(r, cm, rf);
-            const float m = r.m == -INFINITY ? 0.0f : r.m;
-            const uint64_t m2 = packf(-m, -m), rf2 = packf(rf, rf);
-            uint64_t l2[2] = {0, 0}, a2[2] = {0, 0};
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                // (the difference first: it is exact near the largest score)
-                uint64_t d = mul2(add2(packf(u[2 * i], u[2 * i + 1]), m2), rf2);
-                if (!full)
-                    d = packf((w >> (2 * i) & 1u) ? lo_of(d) : -200.0f,
-                              (w >> (2 * i + 1) & 1u) ? hi_of(d) : -200.0f);
-                const uint64_t e = packf(ex2(lo_of(d)), ex2(hi_of(d)));
-                l2[i & 1] = add2(l2[i & 1], e);
-                a2[i & 1] = fma2(e, d, a2[i & 1]);
-            }
-            l2[0] = add2(l2[0], l2[1]);
-            a2[0] = add2(a2[0], a2[1]);
-            r.l += lo_of(l2[0]) + hi_of(l2[0]);
-            r.a += lo_of(a2[0]) + hi_of(a2[0]);
-        }
+        if (__all_sync(0xffffffffu, w == 0xffffffffu)) best = fold<false>(u, w);
+        else if (__any_sync(0xffffffffu, w != 0u)) best = fold<true>(u, w);
         if (p.top && q >= 0) p.top[(size_t)q * p.groups + (col >> 5)] = best;
     }
     __device__ __forceinline__ void finish(int chunk, int part) {
-        if (q >= 0)
-            p.part[(size_t)(chunk * 4 + part) * p.nq + q] = make_float4(r.m, r.l, r.a, 0.0f);
+        if (q >= 0) p.part[(size_t)(chunk * 4 + part) * p.nq + q] = run_stored(r);
     }
 };
 
@@ -503,39 +540,56 @@ struct GradEpilogue {
         const size_t col = (size_t)icol, gcol = (size_t)p.j0 + col;
         if (col >= p.ldg) return;
         const uint32_t w = q < 0 ? 0u : h ? c.word[sizeof(c.word) / 4 - 1] : c.word[0];
-        const bool any = __any_sync(0xffffffffu, w != 0u);
-        const bool full = __all_sync(0xffffffffu, w == 0xffffffffu);
-        const int at = k.target - (int)gcol;  // of the given row, if it is in this chunk
-        const float* xf = c.fac + 32 * h;
         uint4* oh = reinterpret_cast<uint4*>(p.out + (size_t)row * p.ldg + col);
         uint4* ol = reinterpret_cast<uint4*>(p.out + p.plane + (size_t)row * p.ldg + col);
+        if (!__any_sync(0xffffffffu, w != 0u)) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                oh[b] = make_uint4(0, 0, 0, 0);
+                if (TWO) ol[b] = make_uint4(0, 0, 0, 0);
+            }
+            return;
+        }
+        const uint64_t rh2 = packf(k.rf_hi, k.rf_hi), rl2 = packf(k.rf_lo, k.rf_lo);
+        const uint64_t lh2 = packf(-k.l_hi, -k.l_hi), ll2 = packf(-k.l_lo, -k.l_lo);
+        const uint64_t h2 = packf(k.h, k.h), c2 = packf(k.c, k.c), w2 = packf(wi, wi);
+        const float2* xf = reinterpret_cast<const float2*>(c.fac + 32 * h);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float2 f = xf[i];
+            const uint64_t f2 = packf(f.x, f.y);
+            const uint64_t t = mul2(packf(u[2 * i], u[2 * i + 1]), f2);
+            const uint64_t y = add2(fma2(t, rh2, lh2), fma2(t, rl2, ll2));
+            const float x0 = fmaxf(lo_of(y), -160.0f), x1 = fmaxf(hi_of(y), -160.0f);
+            uint64_t g = mul2(packf(ex2(x0), ex2(x1)), fma2(packf(x0, x1), h2, c2));
+            g = mul2(g, mul2(f2, w2));
+            u[2 * i] = lo_of(g);
+            u[2 * i + 1] = hi_of(g);
+        }
+        const int at = k.target - (int)gcol;  // of the given row, if it is in this chunk
+        if ((unsigned)at < 32u) {
+            const float add = k.g * (c.fac[32 * h + at] * wi);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (i == at) u[i] += add;
+        }
+        __syncwarp();
+        if (!__all_sync(0xffffffffu, w == 0xffffffffu)) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (!(w >> i & 1u)) u[i] = 0.0f;
+        }
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
             uint32_t h4[4], l4[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int c0 = 8 * b + 2 * i;
-                h4[i] = l4[i] = 0u;
-                if (!any) continue;
-                const float2 cf = *reinterpret_cast<const float2*>(xf + c0);
-                float g2[2];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const float cj = j ? cf.y : cf.x;
-                    const float uu = u[c0 + j] * cj;
-                    float x = __fmaf_rn(uu, k.rf_hi, -k.l_hi) + __fmaf_rn(uu, k.rf_lo, -k.l_lo);
-                    x = fmaxf(x, -160.0f);
-                    float g = ex2(x) * __fmaf_rn(x, k.h, k.c);
-                    if (at == c0 + j) g += k.g;
-                    g *= cj * wi;
-                    if (!full && !(w >> (c0 + j) & 1u)) g = 0.0f;
-                    g2[j] = g;
-                }
-                const __half2 hh = __floats2half2_rn(g2[0], g2[1]);
+                const float g0 = u[8 * b + 2 * i], g1 = u[8 * b + 2 * i + 1];
+                const __half2 hh = __floats2half2_rn(g0, g1);
                 h4[i] = *reinterpret_cast<const uint32_t*>(&hh);
                 if (TWO) {
                     const float2 back = __half22float2(hh);
-                    const __half2 ll = __floats2half2_rn(g2[0] - back.x, g2[1] - back.y);
+                    const __half2 ll = __floats2half2_rn(g0 - back.x, g1 - back.y);
                     l4[i] = *reinterpret_cast<const uint32_t*>(&ll);
                 }
             }
@@ -959,7 +1013,7 @@ __global__ void __launch_bounds__(64)
                             8 * (lane & 3);
     Run r[NQ];
 #pragma unroll
-    for (int j = 0; j < NQ; ++j) r[j] = Run{-INFINITY, 0.0f, 0.0f};
+    for (int j = 0; j < NQ; ++j) r[j] = run_empty();
     const int ng = (n + GROUP - 1) / GROUP;
     for (int grp = blockIdx.x * 2 + warp; grp < ng; grp += gridDim.x * 2) {
         float sc[NQ];
@@ -1037,14 +1091,14 @@ __global__ void __launch_bounds__(64)
                 allowed_word(allowed, ld_allowed, q0 + j, (size_t)grp * GROUP, n);
             const bool ok = w >> row_of_lane & 1u;
             if (ok) {
-                run_raise(r[j], sc[j], rf);
-                const float m = r[j].m == -INFINITY ? 0.0f : r[j].m;
-                const float dd = (sc[j] - m) * rf, e = ex2(dd);
+                float dd = __fmaf_rn(sc[j], rf, -r[j].m);
+                dd -= run_raise(r[j], dd);
+                const float e = ex2(dd);
                 r[j].l += e;
                 r[j].a = __fmaf_rn(e, dd, r[j].a);
             }
             if (top) {
-                float a = ok ? sc[j] : NONE, b2 = NONE;
+                float a = ok ? sc[j] * rf : NONE, b2 = NONE;
                 a = __uint_as_float((__float_as_uint(a) & ~15u) | (unsigned)(row_of_lane >> 1));
 #pragma unroll
                 for (int o = 16; o; o >>= 1) {
@@ -1064,10 +1118,11 @@ __global__ void __launch_bounds__(64)
 #pragma unroll
         for (int o = 16; o; o >>= 1) {
             Run t;
+            t.limit = __shfl_xor_sync(0xffffffffu, r[j].limit, o);
             t.m = __shfl_xor_sync(0xffffffffu, r[j].m, o);
             t.l = __shfl_xor_sync(0xffffffffu, r[j].l, o);
             t.a = __shfl_xor_sync(0xffffffffu, r[j].a, o);
-            run_join(r[j], t, rf);
+            run_join(r[j], t);
         }
     if (warp == 1 && lane == 0)
 #pragma unroll
@@ -1077,8 +1132,8 @@ __global__ void __launch_bounds__(64)
 #pragma unroll
         for (int j = 0; j < NQ; ++j)
             if (j < nq) {
-                run_join(r[j], other[j], rf);
-                part[(size_t)blockIdx.x * nq + j] = make_float4(r[j].m, r[j].l, r[j].a, 0.0f);
+                run_join(r[j], other[j]);
+                part[(size_t)blockIdx.x * nq + j] = run_stored(r[j]);
             }
 }
 
@@ -1108,11 +1163,6 @@ __device__ __forceinline__ uint32_t ordered(float f) {
     const uint32_t u = __float_as_uint(f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-// A group's largest score without the mark of its pair.
-__device__ __forceinline__ float unmarked(float f) {
-    return __uint_as_float(__float_as_uint(f) & ~15u);
-}
-
 constexpr int PICKED = 256;              // groups picked for exact scoring at most
 constexpr int CAND = MAX_SEL * GROUP;    // rows scored exactly and ranked at once
 
@@ -1185,7 +1235,8 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
     float f = 1.0f;
     if (p.qf) f = p.qf[ql] == 0.0f ? 1.0f : p.qf[ql];
     const float rf = f * (float)((double)p.scale * LOG2E);
-    const double rf64 = (double)f * (double)p.scale * LOG2E;
+    // t was formed with rf, rounded to f32; M of it is set right here
+    const double unit = (double)p.scale * LOG2E, fix = (double)f * unit / (double)rf;
     const int64_t target = p.targets ? p.targets[q] : -1;
     const bool given = target >= 0 && target < p.n;
     if (tid == 0) s_picked = s_cnt = 0, s_kth = -INFINITY;
@@ -1207,12 +1258,12 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < W; ++i) M = fmaxf(M, redf[i]);
-    // ---- the sums over the parts, in units of 2^(M rf) ----
+    // ---- the sums over the parts, in units of 2^M ----
     double L = 0.0, A = 0.0;
     for (int i = tid; i < p.parts; i += THREADS_) {
         const float4 t = p.part[(size_t)i * p.nq + ql];
         if (t.y == 0.0f && t.z == 0.0f) continue;
-        const float d = t.x == M ? 0.0f : (t.x - M) * rf, e = ex2(d);
+        const float d = t.x == M ? 0.0f : t.x - M, e = ex2(d);
         L += (double)(t.y * e);
         A += (double)(__fmaf_rn(d, t.y, t.z) * e);
     }
@@ -1237,7 +1288,7 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
     const bool none = L == 0.0;  // no row may be seen
     const bool bad = !(A == A) || !(L == L) || (p.err && *p.err != 0);
     const double lg = none || bad ? 0.0 : log2(L);
-    const double lse = bad ? NAN : none ? -INFINITY : LN2 * ((double)M * rf64 + lg);
+    const double lse = bad ? NAN : none ? -INFINITY : LN2 * ((double)M * fix + lg);
     if (tid == 0) {
         if (p.lse) p.lse[q] = (float)lse;
         if (p.entropy) p.entropy[q] = (float)(bad ? NAN : none ? 0.0 : LN2 * (lg - A / L));
@@ -1311,7 +1362,7 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
     // k, whose last exact score so far is s_kth: marks and 32-bit sums move it
     // by far less than 2^-15 of the larger of the two.
     auto may_enter = [&](double m) {
-        const double v = m * (double)f, kth = s_kth;
+        const double v = m / unit, kth = s_kth;
         return v >= kth - ldexp(fabs(v) + fabs(kth), -15);
     };
     for (int i = tid; i < cnt; i += THREADS_) {
