@@ -40,16 +40,22 @@ namespace sr {
 
 using namespace tc;
 
-constexpr int BM = 128;                     // rows of an output tile
+constexpr int BM = 128;                     // rows of an output tile in one block
+constexpr int PM = 2 * BM;                  // ... of the pair of blocks that shares it
 constexpr int OPER = BM * 128;              // bytes of 128 rows of a 64-wide K step
-// 16-bit operands: 256 columns an accumulator, four K steps of 48 KB in
-// flight.  Two parts (f32): 128 columns, three K steps of 64 KB (both parts of
-// both operands).
+// Two blocks work on a tile as a pair (cta_group::2): each holds its 128 rows
+// of A and half of the columns' rows of B, so an operand byte is fetched and
+// read from shared memory half as often for B.  16-bit operands: 256 columns
+// an accumulator, six K steps of 32 KB a block in flight.  Two parts (f32):
+// 128 columns, four K steps of 48 KB (both parts of both operands).
 __host__ __device__ constexpr int bn_of(bool two) { return two ? 128 : 256; }
-__host__ __device__ constexpr int stages_of(bool two) { return two ? 3 : 4; }
-__host__ __device__ constexpr int stage_bytes(bool two) { return two ? 4 * OPER : 3 * OPER; }
+__host__ __device__ constexpr int stages_of(bool two) { return two ? 4 : 6; }
+__host__ __device__ constexpr int stage_bytes(bool two) {
+    return (two ? 2 : 1) * (OPER + bn_of(two) / 2 * 128);
+}
 __host__ __device__ constexpr int accs_of(bool two) { return two ? 4 : 2; }
 constexpr int MAX_BN = 256;
+constexpr unsigned long long DRAIN_CYCLES = 4000000ull;  // about 2 ms
 constexpr int THREADS = 640;                // 2 issuing warps, 2 idle, 16 epilogue warps
 constexpr int EPI_WARP0 = 4, EPI_WARPS = 16;
 constexpr int GROUP = 32;                   // rows whose largest scores are kept together
@@ -519,12 +525,14 @@ struct GradEpilogue {
     typedef GradArgs Args;
     const GradArgs& p;
     int q, row;
+    bool live;  // (rows up to a multiple of 128 are written)
     Coef k;
     float wi;
     Columns<true, TWO ? 1 : 2> c;
     const uint32_t* al;
-    __device__ GradEpilogue(const Mma&, const GradArgs& a, int r, int, int, int, float* fac)
+    __device__ GradEpilogue(const Mma&, const GradArgs& a, int r, int row0, int, int, float* fac)
         : p(a) {
+        live = row0 < (a.nq + BM - 1) / BM * BM;
         c.fac = fac;
         row = r;
         al = r >= a.nq || !a.allowed ? nullptr : a.allowed + (size_t)r * a.ld_allowed;
@@ -538,7 +546,7 @@ struct GradEpilogue {
     }
     __device__ __forceinline__ void chunk(float (&u)[32], int icol, int h) {
         const size_t col = (size_t)icol, gcol = (size_t)p.j0 + col;
-        if (col >= p.ldg) return;
+        if (col >= p.ldg || !live) return;
         const uint32_t w = q < 0 ? 0u : h ? c.word[sizeof(c.word) / 4 - 1] : c.word[0];
         uint4* oh = reinterpret_cast<uint4*>(p.out + (size_t)row * p.ldg + col);
         uint4* ol = reinterpret_cast<uint4*>(p.out + p.plane + (size_t)row * p.ldg + col);
@@ -715,6 +723,68 @@ __device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr) {
            ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
+// ---- pairs of blocks ----
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+// The address, in the cluster's window, of the first block's copy of `p`.
+__device__ __forceinline__ uint32_t leader_addr(const void* p) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Into this block's shared memory, counted on the first block's barrier.
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, uint32_t bar,
+                                              int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+}
+__device__ __forceinline__ void umma_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                          uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
+}
+// Arrives on the barrier of both blocks when the MMAs issued so far are done.
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;" ::"r"(smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+// One lane of a converged warp.  The issuing warps stay converged and only
+// this lane issues: the copies and MMAs take their operands from uniform
+// registers, which a branch on the lane number would have to fill lane by
+// lane (measured, 2048 x 131072 x 768 bf16: 424 us instead of 295).
+__device__ __forceinline__ bool elected() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
+// A bounded wait of a whole converged warp.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err,
+                                          unsigned long long limit) {
+    return __all_sync(0xffffffffu, mbar_wait_spin(bar, parity, err, limit));
+}
+__device__ __forceinline__ void arrive_leader(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
+                 : "memory");
+}
+
 // What a unit covers.
 struct Unit {
     int mt, sp;      // sp: chunk (STATS, GRAD) or split of K (PROD)
@@ -741,10 +811,11 @@ __device__ __forceinline__ Unit unit_of(const Mma& g, int u) {
     return x;
 }
 
-// Warp 0 loads the K steps of both operands with TMA, warp 1 issues the MMAs
-// into the TMEM accumulators, sixteen epilogue warps (four per lane quadrant,
-// a quarter of the columns each) work on a finished one meanwhile.
-// Persistent: a block takes units blockIdx.x, + gridDim.x, ...
+// A pair of blocks works on 256 rows x one column tile.  In each, warp 0 loads
+// its share of the K steps with TMA and sixteen epilogue warps (four per lane
+// quadrant, a quarter of the columns each) work on the block's 128 rows of a
+// finished accumulator; warp 1 of the first block issues the MMAs of both.
+// Persistent: a pair takes units blockIdx.x / 2, + gridDim.x / 2, ...
 //
 // One part: an accumulator is a whole tile (all of K).  TWO parts: it is ONE
 // K step, the products lo.hi, hi.lo, hi.hi in this order, and the epilogue
@@ -752,7 +823,7 @@ __device__ __forceinline__ Unit unit_of(const Mma& g, int u) {
 // towards zero (measured: 8e-7 of a score at dim 512, against 1.5e-7 when a
 // step of 64 is the longest such sum).
 template <int MODE, bool TWO>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     rows_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
                 const Mma g, const typename EpilogueOf<MODE, TWO>::Type::Args p) {
     constexpr bool PROD = MODE == PROD_Q || MODE == PROD_X;
@@ -760,17 +831,20 @@ __global__ void __launch_bounds__(THREADS, 1)
     constexpr int BN = bn_of(TWO), NST = stages_of(TWO), NACC = accs_of(TWO);
     constexpr int STAGE = stage_bytes(TWO), PARTS = TWO ? 2 : 1;
     constexpr int B0 = PARTS * OPER;               // operand B in a stage
-    constexpr int B_PART = BN * 128;               // bytes of one part of it
+    constexpr int B_PART = BN / 2 * 128;           // bytes of one part of this block's half
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     const uint32_t base = smem_u32(smem_raw);
     unsigned char* smem = smem_raw + ((1024 - (base & 1023)) & 1023);
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + NST * STAGE);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + NST * STAGE);  // the first block's count
     uint64_t* empty = full + NST;
     uint64_t* t_full = empty + NST;
-    uint64_t* t_empty = t_full + NACC;
+    uint64_t* t_empty = t_full + NACC;                                 // the first block's count
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(t_empty + NACC);
     float* factors = reinterpret_cast<float*>(smem + NST * STAGE + 256);  // [16 warps][64]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_rank();
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const uint32_t full0 = leader_addr(full);
     if (threadIdx.x == 0) {
         for (int i = 0; i < NST; ++i) {
             mbar_init(full + i, 1);
@@ -778,122 +852,123 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         for (int i = 0; i < NACC; ++i) {
             mbar_init(t_full + i, 1);
-            mbar_init(t_empty + i, EPI_WARPS);
+            mbar_init(t_empty + i, 2 * EPI_WARPS);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                          smem_u32(tmem_slot)),
                      "r"(512));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
         tc_fence_before();
     }
     __syncthreads();
+    cluster_sync();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const int units = PROD ? g.mt * g.nt * g.chunks : g.mt * g.chunks;
-    int last_use[NST];  // producer: last use issued of each stage
-    for (int i = 0; i < NST; ++i) last_use[i] = -1;
     int last_stage = -1, last_phase = 0;  // MMA issuer: last stage committed
 
     if (warp == 0) {
-        if (lane == 0 && !g.stall) {
-            int it = 0;
-            bool ok = true;
-            for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
-                const Unit x = unit_of<MODE>(g, u);
-                for (int t = x.t0; ok && t < x.t1; ++t) {
-                    const int boxes = B_MN ? (min(BN, g.ncols - t * BN) + 63) / 64 : 0;
-                    const uint32_t bytes =
-                        PARTS * (OPER + (uint32_t)(B_MN ? boxes * 8192 : B_PART));
-                    for (int a = x.a0; a < x.a1; ++a, ++it) {
-                        const int s = it % NST, use = it / NST;
-                        if (use > 0 && !mbar_wait(empty + s, (use - 1) & 1, g.err, g.wait)) {
-                            ok = false;
-                            break;
-                        }
-                        mbar_expect_tx(full + s, bytes);
+        int it = 0;
+        bool ok = !g.stall;
+        for (int u = pair; ok && u < units; u += pairs) {
+            const Unit x = unit_of<MODE>(g, u);
+            const int m0 = x.mt * PM + rank * BM;
+            for (int t = x.t0; ok && t < x.t1; ++t) {
+                // this block's half of the columns: [n0, n0 + half)
+                const int half = PROD ? ((min(BN, g.ncols - t * BN) + 31) & ~31) / 2 : BN / 2;
+                const int n0 = t * BN + rank * half;
+                const int boxes = B_MN ? (half + 63) / 64 : 0;
+                const uint32_t bytes = PARTS * (OPER + (uint32_t)(B_MN ? boxes * 8192 : B_PART));
+                for (int a = x.a0; a < x.a1; ++a, ++it) {
+                    const int s = it % NST, use = it / NST;
+                    if (use > 0 && !warp_wait(empty + s, (use - 1) & 1, g.err, g.wait)) {
+                        ok = false;
+                        break;
+                    }
+                    if (elected()) {
+                        if (rank == 0) mbar_expect_tx(full + s, 2 * bytes);
+                        const uint32_t bar = full0 + 8 * s;
 #pragma unroll
                         for (int h = 0; h < PARTS; ++h) {
                             unsigned char* da = smem + s * STAGE + h * OPER;
                             unsigned char* db = smem + s * STAGE + B0 + h * B_PART;
                             const int pa = h * g.a_part, pb = h * g.b_part;
                             if (A_MN) {
-                                tma_load_2d(da, &amap, full + s, x.mt * BM, pa + a * KATOM);
-                                tma_load_2d(da + 8192, &amap, full + s, x.mt * BM + 64,
-                                            pa + a * KATOM);
+                                tma_load_pair(da, &amap, bar, m0, pa + a * KATOM);
+                                tma_load_pair(da + 8192, &amap, bar, m0 + 64, pa + a * KATOM);
                             } else if (PROD) {
-                                tma_load_2d(da, &amap, full + s, a * KATOM, pa + x.mt * BM);
+                                tma_load_pair(da, &amap, bar, a * KATOM, pa + m0);
                             } else {
-                                tma_load_2d(da, &amap, full + s, pa + a * KATOM, x.mt * BM);
+                                tma_load_pair(da, &amap, bar, pa + a * KATOM, m0);
                             }
                             if (B_MN) {
-                                for (int b = 0; b < boxes; ++b)
-                                    tma_load_2d(db + b * 8192, &bmap, full + s,
-                                                pb + t * BN + 64 * b, g.b_row0 + a * KATOM);
+                                tma_load_pair(db, &bmap, bar, pb + n0, g.b_row0 + a * KATOM);
+                                if (boxes > 1)
+                                    tma_load_pair(db + 8192, &bmap, bar, pb + n0 + 64,
+                                                  g.b_row0 + a * KATOM);
                             } else {
-#pragma unroll
-                                for (int b = 0; b < BN / 128; ++b)
-                                    tma_load_2d(db + b * OPER, &bmap, full + s, pb + a * KATOM,
-                                                g.b_row0 + t * BN + 128 * b);
+                                tma_load_pair(db, &bmap, bar, pb + a * KATOM, g.b_row0 + n0);
                             }
                         }
-                        last_use[s] = use;
                     }
+                    __syncwarp();
                 }
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (rank == 0) {
             int it = 0, ti = 0;  // K steps, accumulators
             bool ok = true;
-            for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+            for (int u = pair; ok && u < units; u += pairs) {
                 const Unit x = unit_of<MODE>(g, u);
                 for (int t = x.t0; ok && t < x.t1; ++t) {
-                    const int bn = PROD ? (min(BN, g.ncols - t * BN) + 15) & ~15 : BN;
+                    const int bn = PROD ? (min(BN, g.ncols - t * BN) + 31) & ~31 : BN;
                     const uint32_t idesc = g.idesc | ((uint32_t)(bn >> 3) << 17);
-                    uint32_t acc = 0;
                     for (int a = x.a0; a < x.a1; ++a, ++it) {
                         const int b = ti % NACC;
-                        const uint32_t d = tmem + (uint32_t)(b * BN);
-                        if (TWO || a == x.a0) {  // a new accumulator
-                            if (ti >= NACC &&
-                                !mbar_wait(t_empty + b, (ti / NACC - 1) & 1, g.err, g.wait)) {
-                                ok = false;
-                                break;
-                            }
-                            acc = 0;
+                        const bool fresh = TWO || a == x.a0;  // a new accumulator
+                        if (fresh && ti >= NACC &&
+                            !warp_wait(t_empty + b, (ti / NACC - 1) & 1, g.err, g.wait)) {
+                            ok = false;
+                            break;
                         }
                         const int s = it % NST, use = it / NST;
-                        if (!mbar_wait(full + s, use & 1, g.err, g.wait)) {
+                        if (!warp_wait(full + s, use & 1, g.err, g.wait)) {
                             ok = false;
                             break;
                         }
                         tc_fence_after();
-                        const uint32_t ab = smem_u32(smem + s * STAGE), bb = ab + B0;
-                        const int kk1 = a == g.atoms - 1 ? g.klast : 4;
+                        const bool done = TWO || a + 1 == x.a1;
+                        if (elected()) {
+                            const uint32_t d = tmem + (uint32_t)(b * BN);
+                            const uint32_t ab = smem_u32(smem + s * STAGE), bb = ab + B0;
+                            // (past the operands' last column the steps hold zeros)
+                            const int kk1 = a == g.atoms - 1 ? g.klast : 4;
 #pragma unroll
-                        for (int pr = 0; pr < (TWO ? 3 : 1); ++pr) {
-                            const uint32_t ap = ab + (TWO && pr == 0 ? OPER : 0);
-                            const uint32_t bp = bb + (TWO && pr == 1 ? B_PART : 0);
-                            for (int kk = 0; kk < kk1; ++kk) {
-                                umma_f16_n(d,
-                                           A_MN ? smem_desc_mn(ap + kk * 2048)
-                                                : smem_desc_sw128(ap + kk * 32),
-                                           B_MN ? smem_desc_mn(bp + kk * 2048)
-                                                : smem_desc_sw128(bp + kk * 32),
-                                           idesc, acc);
-                                acc = 1;
+                            for (int pr = 0; pr < (TWO ? 3 : 1); ++pr) {
+                                const uint32_t ap = ab + (TWO && pr == 0 ? OPER : 0);
+                                const uint32_t bp = bb + (TWO && pr == 1 ? B_PART : 0);
+#pragma unroll
+                                for (int kk = 0; kk < 4; ++kk) {
+                                    if (kk < kk1)
+                                        umma_pair(d,
+                                                  A_MN ? smem_desc_mn(ap + kk * 2048)
+                                                       : smem_desc_sw128(ap + kk * 32),
+                                                  B_MN ? smem_desc_mn(bp + kk * 2048)
+                                                       : smem_desc_sw128(bp + kk * 32),
+                                                  idesc, !fresh || kk > 0 || pr > 0);
+                                }
                             }
+                            umma_commit_pair(empty + s);
+                            if (done) umma_commit_pair(t_full + b);
                         }
-                        umma_commit(empty + s);
+                        __syncwarp();
                         last_stage = s;
                         last_phase = use & 1;
-                        if (TWO || a + 1 == x.a1) {
-                            umma_commit(t_full + b);
-                            ++ti;
-                        }
+                        if (done) ++ti;
                     }
                 }
             }
@@ -901,6 +976,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     } else if (warp >= EPI_WARP0) {
         const int w = warp - EPI_WARP0, quad = w & 3, part = w >> 2;
         const uint32_t mine = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(part * (BN / 4));
+        const uint32_t release0 = leader_addr(t_empty);
         int ti = 0;
         bool ok = true;
         // the next accumulator, or false when the kernel is aborting
@@ -914,12 +990,12 @@ __global__ void __launch_bounds__(THREADS, 1)
         auto release = [&] {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(t_empty + ti % NACC);
+            if (lane == 0) arrive_leader(release0 + 8 * (ti % NACC));
             ++ti;
         };
-        for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+        for (int u = pair; ok && u < units; u += pairs) {
             const Unit x = unit_of<MODE>(g, u);
-            const int row0 = x.mt * BM + quad * 32;
+            const int row0 = x.mt * PM + rank * BM + quad * 32;
             typename EpilogueOf<MODE, TWO>::Type epi(g, p, row0 + lane, row0, x.t0, x.sp,
                                                       factors + w * 64);
             epi.load(x.t0 * BN + part * (BN / 4));
@@ -961,26 +1037,22 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (ok) epi.finish(x.sp, part);
         }
     }
-    // One verdict for the whole block; an aborting block lets the copies and
-    // MMAs it issued land (bounded) before it frees TMEM and exits.
+    // One verdict for the block.  An aborting block gives the copies that it
+    // issued (which the first block's barriers count, so they cannot be waited
+    // for here) time to land, and the MMAs; then the pair leaves together.
     if (__syncthreads_or(*(volatile int*)g.err != 0)) {
-        if (warp == 0 && lane == 0)
-            for (int s = 0; s < NST; ++s)
-                if (last_use[s] >= 0) {
-                    const unsigned long long c0 = clock64();
-                    while (!mbar_try(full + s, last_use[s] & 1) && clock64() - c0 < WAIT_CYCLES) {
-                    }
-                }
-        if (warp == 1 && lane == 0 && last_stage >= 0) {
-            const unsigned long long c0 = clock64();
-            while (!mbar_try(empty + last_stage, last_phase) && clock64() - c0 < WAIT_CYCLES) {
+        const unsigned long long c0 = clock64();
+        if (warp == 0)
+            while (clock64() - c0 < DRAIN_CYCLES) __nanosleep(1000);
+        if (warp == 1 && lane == 0 && last_stage >= 0)
+            while (!mbar_try(empty + last_stage, last_phase) && clock64() - c0 < DRAIN_CYCLES) {
             }
-        }
         __syncthreads();
     }
+    cluster_sync();
     if (warp == 1) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                      "r"(512));
     }
 }
@@ -1655,17 +1727,17 @@ static CUtensorMap map2d(int dtype, const void* base, size_t inner, size_t rows,
     FDB_REQUIRE(r == CUDA_SUCCESS, FDB_ERR_CUDA, "cuTensorMapEncodeTiled failed");
     return m;
 }
-// D f32; A and B both f16 or both bf16; transposed operands; M = 128 (N is added
+// D f32; A and B both f16 or both bf16; transposed operands; M = 256 (N is added
 // in the kernel).
 static uint32_t idesc_of(int dtype, bool a_mn, bool b_mn) {
     const uint32_t t = dtype == FDB_DTYPE_BF16 ? 1u : 0u;
     return (1u << 4) | (t << 7) | (t << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
-           ((uint32_t)(BM >> 4) << 24);
+           ((uint32_t)(PM >> 4) << 24);
 }
-// Chunks of the column tiles: the count that leaves the busiest block the
-// fewest tiles, and of those the smallest.
+// Chunks of the column tiles: the count that leaves the busiest pair of blocks
+// the fewest tiles, and of those the smallest.
 static int pick_chunks(int mt, int nt, int sms) {
-    sms = std::max(sms, 1);
+    sms = std::max(sms / 2, 1);
     int best = 1;
     long long cost = -1;
     for (int c = 1; c <= nt && c <= 4 * sms; ++c) {
@@ -1680,7 +1752,7 @@ static int pick_chunks(int mt, int nt, int sms) {
 // split writes and reads `out_bytes` of partial sums each, at 4 MB/us, and
 // takes another launch (3 us).
 static int pick_splits(int tiles, int atoms, int sms, bool two, double out_bytes) {
-    sms = std::max(sms, 1);
+    sms = std::max(sms / 2, 1);
     int best = 1;
     double cost = -1.0;
     for (int s = 1; s <= atoms && s <= 64; ++s) {
@@ -1701,7 +1773,7 @@ static void launch_rows(cudaStream_t s, int sms, const CUtensorMap& a, const CUt
     FDB_CUDA(cudaFuncSetAttribute(rows_kernel<MODE, TWO>,
                                   cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     rows_kernel<MODE, TWO>
-        <<<(unsigned)std::min<long long>(units, sms), THREADS, smem, s>>>(a, b, g, p);
+        <<<2 * (unsigned)std::min<long long>(units, sms / 2), THREADS, smem, s>>>(a, b, g, p);
     FDB_LAUNCH_CHECK();
 }
 template <int MODE>
@@ -1772,7 +1844,7 @@ static Forward plan_forward(const Ctx& c, const fdb_logprob_args& a) {
     w.groups = w.few ? (a.n + GROUP - 1) / GROUP : (size_t)w.nt * (w.bn / GROUP);
     const size_t per = a.k ? w.groups * sizeof(float2) : 0;
     w.qb = std::min<size_t>(a.nq, w.few ? (size_t)FEW
-                                  : per ? std::max<size_t>(BM, CHUNK_BYTES / per / BM * BM)
+                                  : per ? std::max<size_t>(PM, CHUNK_BYTES / per / PM * PM)
                                         : (size_t)1 << 20);
     if (w.packed) {
         w.qp = ws.take<__half>(a.nq * 2 * w.kp);
@@ -1789,10 +1861,10 @@ static Forward plan_forward(const Ctx& c, const fdb_logprob_args& a) {
         w.parts_cap = std::min<size_t>((w.groups + 1) / 2, (size_t)c.sm_count * 12);
     } else {
         // (the last pass has fewer row blocks and may take more chunks)
-        const int full = (int)((w.qb + BM - 1) / BM);
+        const int full = (int)((w.qb + PM - 1) / PM);
         w.parts_cap = 0;
         for (int mt = 1; mt <= full; ++mt)
-            if (mt == full || mt == (int)((a.nq % w.qb + BM - 1) / BM))
+            if (mt == full || mt == (int)((a.nq % w.qb + PM - 1) / PM))
                 w.parts_cap = std::max<size_t>(w.parts_cap,
                                                4 * (size_t)pick_chunks(mt, w.nt, c.sm_count));
     }
@@ -1859,7 +1931,7 @@ void forward_run(Ctx& c, const fdb_logprob_args& a) {
             FDB_LAUNCH_CHECK();
             xb = w.xp, ldx = w.kp;
         }
-        bmap = map2d(a.dtype, xb, inner, a.n, ldx, 128);
+        bmap = map2d(a.dtype, xb, inner, a.n, ldx, w.bn / 2);
         g.nt = w.nt;
         g.atoms = (int)((w.kp + 63) / 64);
         g.klast = (int)((w.kp - 64 * (size_t)(g.atoms - 1)) / 16);
@@ -1870,7 +1942,7 @@ void forward_run(Ctx& c, const fdb_logprob_args& a) {
         g.stall = take_test_stall(c);
         for (size_t q0 = 0; q0 < a.nq; q0 += w.qb) {
             const size_t nq = std::min(w.qb, a.nq - q0);
-            g.mt = (int)((nq + BM - 1) / BM);
+            g.mt = (int)((nq + PM - 1) / PM);
             g.chunks = pick_chunks(g.mt, w.nt, c.sm_count);
             amap = map2d(a.dtype,
                          static_cast<const unsigned char*>(qb) + q0 * ldq * 2, inner, nq, ldq, BM);
@@ -1966,9 +2038,9 @@ static Backward plan_backward(const Ctx& c, const fdb_logprob_grad_args& a) {
                               a.n);
     w.ldg = up(w.cols, 64);
     const int ntd = (int)((a.dim + w.bn - 1) / w.bn);
-    w.q_splits = pick_splits((int)(w.nqp / BM) * ntd, (int)((w.cols + 63) / 64), c.sm_count,
+    w.q_splits = pick_splits((int)((a.nq + PM - 1) / PM) * ntd, (int)((w.cols + 63) / 64), c.sm_count,
                              w.parts == 2, (double)a.nq * a.dim * 4);
-    w.x_splits = pick_splits((int)((w.cols + BM - 1) / BM) * ntd, (int)((a.nq + 63) / 64),
+    w.x_splits = pick_splits((int)((w.cols + PM - 1) / PM) * ntd, (int)((a.nq + 63) / 64),
                              c.sm_count, w.parts == 2, (double)w.cols * a.dim * 4);
     unsigned char* head = ws.take<unsigned char>(HEAD);
     w.err = reinterpret_cast<int*>(head);
@@ -2027,9 +2099,9 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
 
     const size_t width = w.parts * w.kp;
     const bool two = w.parts == 2;
-    const int mtq = (int)(w.nqp / BM), ntd = (d + w.bn - 1) / w.bn;
+    const int mtq = (int)((a.nq + PM - 1) / PM), ntd = (d + w.bn - 1) / w.bn;
     const CUtensorMap qk = map2d(FDB_DTYPE_F16, w.qp, width, a.nq, width, BM);
-    const CUtensorMap xk = map2d(FDB_DTYPE_F16, w.xp, width, a.n, width, 128);
+    const CUtensorMap xk = map2d(FDB_DTYPE_F16, w.xp, width, a.n, width, w.bn / 2);
     const CUtensorMap qm = map2d(FDB_DTYPE_F16, w.qp, width, a.nq, width, 64);
     const CUtensorMap xm = map2d(FDB_DTYPE_F16, w.xp, width, a.n, width, 64);
     const size_t g_rows = w.parts * w.nqp;
@@ -2075,7 +2147,7 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
         }
         if (a.d_rows) {
             Mma g = base;
-            g.mt = (cols + BM - 1) / BM, g.nt = ntd, g.chunks = w.x_splits;
+            g.mt = (cols + PM - 1) / PM, g.nt = ntd, g.chunks = w.x_splits;
             g.atoms = (nq + 63) / 64;
             g.klast = 4;
             g.a_part = (int)w.nqp, g.b_part = (int)w.kp;
