@@ -47,13 +47,21 @@ constexpr int OPER = BM * 128;              // bytes of 128 rows of a 64-wide K 
 // of A and half of the columns' rows of B, so an operand byte is fetched and
 // read from shared memory half as often for B.  16-bit operands: 256 columns
 // an accumulator, six K steps of 32 KB a block in flight.  Two parts (f32):
-// 128 columns, four K steps of 48 KB (both parts of both operands).
+// 128 columns, four K steps of 48 KB (both parts of both operands).  GRAD has
+// one stage less of either: its output is staged in shared memory too.
 __host__ __device__ constexpr int bn_of(bool two) { return two ? 128 : 256; }
-__host__ __device__ constexpr int stages_of(bool two) { return two ? 4 : 6; }
+__host__ __device__ constexpr int stages_of(bool two, bool grad) {
+    return (two ? 4 : 6) - (grad ? 1 : 0);
+}
+constexpr int STAGED = 32 * 64;             // one warp's 32 x 32 fp16 outputs
+__host__ __device__ constexpr int staged_of(bool two, bool grad) {
+    return grad ? 16 * (two ? 2 : 1) * STAGED : 0;
+}
 __host__ __device__ constexpr int stage_bytes(bool two) {
     return (two ? 2 : 1) * (OPER + bn_of(two) / 2 * 128);
 }
 __host__ __device__ constexpr int accs_of(bool two) { return two ? 4 : 2; }
+constexpr int KBLOCK = 2;                   // K steps of an accumulator (two parts)
 constexpr int MAX_BN = 256;
 constexpr unsigned long long DRAIN_CYCLES = 4000000ull;  // about 2 ms
 constexpr int THREADS = 640;                // 2 issuing warps, 2 idle, 16 epilogue warps
@@ -353,8 +361,8 @@ struct GradArgs {
     const float* bounds;        // [0] max of B_i qf_i, [1] max of xf
     const uint32_t* allowed;
     size_t ld_allowed;
-    __half* out;                // [parts][nqp][ldg]
-    size_t ldg, plane;          // plane: nqp * ldg
+    size_t ldg;                 // output [parts][nqp][ldg]
+    int nqp;
 };
 struct ProdArgs {
     int rows, cols;             // output
@@ -391,6 +399,75 @@ __device__ __forceinline__ void load_chunk(uint32_t tmem, float (&u)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) u[i] = __uint_as_float(v[i]);
 }
+// ---- pairs of blocks ----
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+// The address, in the cluster's window, of the first block's copy of `p`.
+__device__ __forceinline__ uint32_t leader_addr(const void* p) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Into this block's shared memory, counted on the first block's barrier.
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, uint32_t bar,
+                                              int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+}
+__device__ __forceinline__ void tma_store(const void* src, const CUtensorMap* map, int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+            reinterpret_cast<uint64_t>(map)),
+        "r"(smem_u32(src)), "r"(x), "r"(y)
+        : "memory");
+}
+__device__ __forceinline__ void umma_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                          uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
+}
+// Arrives on the barrier of both blocks when the MMAs issued so far are done.
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;" ::"r"(smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+// One lane of a converged warp.  The issuing warps stay converged and only
+// this lane issues: the copies and MMAs take their operands from uniform
+// registers, which a branch on the lane number would have to fill lane by
+// lane (measured, 2048 x 131072 x 768 bf16: 424 us instead of 295).
+__device__ __forceinline__ bool elected() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
+// A bounded wait of a whole converged warp.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err,
+                                          unsigned long long limit) {
+    return __all_sync(0xffffffffu, mbar_wait_spin(bar, parity, err, limit));
+}
+__device__ __forceinline__ void arrive_leader(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
+                 : "memory");
+}
+
 // What a chunk of 32 columns needs besides its scores: the filter's word of
 // the thread's row, and (scaled rows) the columns' factors, in the warp's own
 // shared memory.  `load` starts the reads of a tile's chunks while the tile
@@ -432,8 +509,8 @@ struct StatsEpilogue {
     bool live;
     Columns<TWO, TWO ? 1 : 2> c;
     const uint32_t* al;
-    __device__ StatsEpilogue(const Mma&, const StatsArgs& a, int row, int row0, int, int,
-                             float* fac)
+    __device__ StatsEpilogue(const StatsArgs& a, int row, int row0, int, float* fac,
+                             unsigned char*, const CUtensorMap*)
         : p(a) {
         c.fac = fac;
         q = row < a.nq ? row : -1;
@@ -530,8 +607,11 @@ struct GradEpilogue {
     float wi;
     Columns<true, TWO ? 1 : 2> c;
     const uint32_t* al;
-    __device__ GradEpilogue(const Mma&, const GradArgs& a, int r, int row0, int, int, float* fac)
-        : p(a) {
+    unsigned char* stage;      // the warp's staged outputs, part 1 STAGED bytes on
+    const CUtensorMap* omap;
+    __device__ GradEpilogue(const GradArgs& a, int r, int row0, int, float* fac,
+                            unsigned char* staged, const CUtensorMap* out)
+        : p(a), stage(staged), omap(out) {
         live = row0 < (a.nq + BM - 1) / BM * BM;
         c.fac = fac;
         row = r;
@@ -548,14 +628,10 @@ struct GradEpilogue {
         const size_t col = (size_t)icol, gcol = (size_t)p.j0 + col;
         if (col >= p.ldg || !live) return;
         const uint32_t w = q < 0 ? 0u : h ? c.word[sizeof(c.word) / 4 - 1] : c.word[0];
-        uint4* oh = reinterpret_cast<uint4*>(p.out + (size_t)row * p.ldg + col);
-        uint4* ol = reinterpret_cast<uint4*>(p.out + p.plane + (size_t)row * p.ldg + col);
         if (!__any_sync(0xffffffffu, w != 0u)) {
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                oh[b] = make_uint4(0, 0, 0, 0);
-                if (TWO) ol[b] = make_uint4(0, 0, 0, 0);
-            }
+            for (int i = 0; i < 32; ++i) u[i] = 0.0f;
+            store(u, col);
             return;
         }
         const uint64_t rh2 = packf(k.rf_hi, k.rf_hi), rl2 = packf(k.rf_lo, k.rf_lo);
@@ -587,6 +663,18 @@ struct GradEpilogue {
             for (int i = 0; i < 32; ++i)
                 if (!(w >> i & 1u)) u[i] = 0.0f;
         }
+        store(u, col);
+    }
+    // The warp's 32 x 32 values, staged in rows of 64 bytes (64-byte swizzle:
+    // 16-byte piece b of row r at b ^ (r / 2 % 4), so that eight lanes' pieces
+    // lie in different banks) and stored by TMA: straight from registers each
+    // 16-byte store of a warp would touch 32 lines (measured at 4096 x 65536:
+    // 120 us of 440).
+    __device__ __forceinline__ void store(const float (&u)[32], size_t col) {
+        const int lane = threadIdx.x & 31;
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        __syncwarp();
+        unsigned char* o = stage + lane * 64;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
             uint32_t h4[4], l4[4];
@@ -601,11 +689,23 @@ struct GradEpilogue {
                     l4[i] = *reinterpret_cast<const uint32_t*>(&ll);
                 }
             }
-            oh[b] = make_uint4(h4[0], h4[1], h4[2], h4[3]);
-            if (TWO) ol[b] = make_uint4(l4[0], l4[1], l4[2], l4[3]);
+            const int at = 16 * (b ^ (lane >> 1 & 3));
+            *reinterpret_cast<uint4*>(o + at) = make_uint4(h4[0], h4[1], h4[2], h4[3]);
+            if (TWO)
+                *reinterpret_cast<uint4*>(o + STAGED + at) = make_uint4(l4[0], l4[1], l4[2], l4[3]);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+            const int y = row;  // (lane 0: the warp's first row)
+            tma_store(stage, omap, (int)col, y);
+            if (TWO) tma_store(stage + STAGED, omap, (int)col, p.nqp + y);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
     }
-    __device__ __forceinline__ void finish(int, int) {}
+    __device__ __forceinline__ void finish(int, int) {
+        if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
 };
 
 // `count` values of one output row from column c, rounded to the output's type.
@@ -658,7 +758,8 @@ struct ProdEpilogue {
     int row, split;
     float s;
     Columns<false, 1> c;
-    __device__ ProdEpilogue(const Mma&, const ProdArgs& a, int r, int, int, int sp, float*)
+    __device__ ProdEpilogue(const ProdArgs& a, int r, int, int sp, float*, unsigned char*,
+                            const CUtensorMap*)
         : p(a) {
         row = r;
         split = sp;
@@ -723,68 +824,6 @@ __device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr) {
            ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
-// ---- pairs of blocks ----
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-// The address, in the cluster's window, of the first block's copy of `p`.
-__device__ __forceinline__ uint32_t leader_addr(const void* p) {
-    uint32_t r;
-    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// Into this block's shared memory, counted on the first block's barrier.
-__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, uint32_t bar,
-                                              int x, int y) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
-        : "memory");
-}
-__device__ __forceinline__ void umma_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
-                                          uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
-}
-// Arrives on the barrier of both blocks when the MMAs issued so far are done.
-__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
-    asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
-        "[%0], %1;" ::"r"(smem_u32(bar)),
-        "h"((uint16_t)3)
-        : "memory");
-}
-// One lane of a converged warp.  The issuing warps stay converged and only
-// this lane issues: the copies and MMAs take their operands from uniform
-// registers, which a branch on the lane number would have to fill lane by
-// lane (measured, 2048 x 131072 x 768 bf16: 424 us instead of 295).
-__device__ __forceinline__ bool elected() {
-    uint32_t p;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(p));
-    return p != 0;
-}
-// A bounded wait of a whole converged warp.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err,
-                                          unsigned long long limit) {
-    return __all_sync(0xffffffffu, mbar_wait_spin(bar, parity, err, limit));
-}
-__device__ __forceinline__ void arrive_leader(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
-                 : "memory");
-}
-
 // What a unit covers.
 struct Unit {
     int mt, sp;      // sp: chunk (STATS, GRAD) or split of K (PROD)
@@ -797,8 +836,12 @@ __device__ __forceinline__ Unit unit_of(const Mma& g, int u) {
     x.mt = u % g.mt;
     if (MODE == PROD_Q || MODE == PROD_X) {
         x.t0 = u / g.mt % g.nt;
+        if (MODE == PROD_X) {  // the large operand's rows once for all column tiles
+            x.t0 = u % g.nt;
+            x.mt = u / g.nt % g.mt;
+        }
         x.t1 = x.t0 + 1;
-        x.sp = u / g.mt / g.nt;
+        x.sp = u / (g.mt * g.nt);
         x.a0 = (int)((long long)x.sp * g.atoms / g.chunks);
         x.a1 = (int)((long long)(x.sp + 1) * g.atoms / g.chunks);
     } else {
@@ -817,30 +860,32 @@ __device__ __forceinline__ Unit unit_of(const Mma& g, int u) {
 // finished accumulator; warp 1 of the first block issues the MMAs of both.
 // Persistent: a pair takes units blockIdx.x / 2, + gridDim.x / 2, ...
 //
-// One part: an accumulator is a whole tile (all of K).  TWO parts: it is ONE
-// K step, the products lo.hi, hi.lo, hi.hi in this order, and the epilogue
-// adds the steps up in registers: the tensor core's own additions cut the sum
-// towards zero (measured: 8e-7 of a score at dim 512, against 1.5e-7 when a
-// step of 64 is the longest such sum).
+// One part: an accumulator is a whole tile (all of K).  TWO parts: it is 128
+// of K, first the products lo.hi and hi.lo, then hi.hi, and the epilogue adds
+// them up in registers: the tensor core's own additions cut the sum towards
+// zero, which at dim 512 cost 8e-7 of a score (all of K in one accumulator).
 template <int MODE, bool TWO>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     rows_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
-                const Mma g, const typename EpilogueOf<MODE, TWO>::Type::Args p) {
+                const __grid_constant__ CUtensorMap omap, const Mma g,
+                const typename EpilogueOf<MODE, TWO>::Type::Args p) {
     constexpr bool PROD = MODE == PROD_Q || MODE == PROD_X;
     constexpr bool A_MN = MODE == PROD_X, B_MN = PROD;
-    constexpr int BN = bn_of(TWO), NST = stages_of(TWO), NACC = accs_of(TWO);
+    constexpr int BN = bn_of(TWO), NST = stages_of(TWO, MODE == GRAD), NACC = accs_of(TWO);
     constexpr int STAGE = stage_bytes(TWO), PARTS = TWO ? 2 : 1;
     constexpr int B0 = PARTS * OPER;               // operand B in a stage
     constexpr int B_PART = BN / 2 * 128;           // bytes of one part of this block's half
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     const uint32_t base = smem_u32(smem_raw);
     unsigned char* smem = smem_raw + ((1024 - (base & 1023)) & 1023);
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + NST * STAGE);  // the first block's count
+    unsigned char* staged = smem + NST * STAGE;
+    unsigned char* after = staged + staged_of(TWO, MODE == GRAD);
+    uint64_t* full = reinterpret_cast<uint64_t*>(after);               // the first block's count
     uint64_t* empty = full + NST;
     uint64_t* t_full = empty + NST;
     uint64_t* t_empty = t_full + NACC;                                 // the first block's count
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(t_empty + NACC);
-    float* factors = reinterpret_cast<float*>(smem + NST * STAGE + 256);  // [16 warps][64]
+    float* factors = reinterpret_cast<float*>(after + 256);             // [16 warps][64]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank();
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -868,7 +913,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const int units = PROD ? g.mt * g.nt * g.chunks : g.mt * g.chunks;
-    int last_stage = -1, last_phase = 0;  // MMA issuer: last stage committed
+    int last_it = -1;  // MMA issuer: last K step committed
 
     if (warp == 0) {
         int it = 0;
@@ -927,48 +972,65 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 for (int t = x.t0; ok && t < x.t1; ++t) {
                     const int bn = PROD ? (min(BN, g.ncols - t * BN) + 31) & ~31 : BN;
                     const uint32_t idesc = g.idesc | ((uint32_t)(bn >> 3) << 17);
-                    for (int a = x.a0; a < x.a1; ++a, ++it) {
+                    for (int a = x.a0; ok && a < x.a1;) {
+                        // an accumulator: KBLOCK steps (two parts), or all
                         const int b = ti % NACC;
-                        const bool fresh = TWO || a == x.a0;  // a new accumulator
-                        if (fresh && ti >= NACC &&
+                        const int a1 = TWO ? min(x.a1, a + KBLOCK) : x.a1;
+                        const uint32_t d = tmem + (uint32_t)(b * BN);
+                        if (ti >= NACC &&
                             !warp_wait(t_empty + b, (ti / NACC - 1) & 1, g.err, g.wait)) {
                             ok = false;
                             break;
                         }
-                        const int s = it % NST, use = it / NST;
-                        if (!warp_wait(full + s, use & 1, g.err, g.wait)) {
-                            ok = false;
-                            break;
-                        }
                         tc_fence_after();
-                        const bool done = TWO || a + 1 == x.a1;
-                        if (elected()) {
-                            const uint32_t d = tmem + (uint32_t)(b * BN);
-                            const uint32_t ab = smem_u32(smem + s * STAGE), bb = ab + B0;
-                            // (past the operands' last column the steps hold zeros)
-                            const int kk1 = a == g.atoms - 1 ? g.klast : 4;
+                        // (past the operands' last column the steps hold zeros)
+                        auto issue = [&](int stage, int atom, int ao, int bo, bool first) {
+                            const uint32_t ap = smem_u32(smem + stage * STAGE) + ao;
+                            const uint32_t bp = smem_u32(smem + stage * STAGE) + B0 + bo;
+                            const int kk1 = atom == g.atoms - 1 ? g.klast : 4;
 #pragma unroll
-                            for (int pr = 0; pr < (TWO ? 3 : 1); ++pr) {
-                                const uint32_t ap = ab + (TWO && pr == 0 ? OPER : 0);
-                                const uint32_t bp = bb + (TWO && pr == 1 ? B_PART : 0);
-#pragma unroll
-                                for (int kk = 0; kk < 4; ++kk) {
-                                    if (kk < kk1)
-                                        umma_pair(d,
-                                                  A_MN ? smem_desc_mn(ap + kk * 2048)
-                                                       : smem_desc_sw128(ap + kk * 32),
-                                                  B_MN ? smem_desc_mn(bp + kk * 2048)
-                                                       : smem_desc_sw128(bp + kk * 32),
-                                                  idesc, !fresh || kk > 0 || pr > 0);
+                            for (int kk = 0; kk < 4; ++kk)
+                                if (kk < kk1)
+                                    umma_pair(d,
+                                              A_MN ? smem_desc_mn(ap + kk * 2048)
+                                                   : smem_desc_sw128(ap + kk * 32),
+                                              B_MN ? smem_desc_mn(bp + kk * 2048)
+                                                   : smem_desc_sw128(bp + kk * 32),
+                                              idesc, !first || kk > 0);
+                        };
+                        const int it0 = it, from = a;
+                        for (; a < a1; ++a, ++it) {
+                            const int s = it % NST;
+                            if (!warp_wait(full + s, (it / NST) & 1, g.err, g.wait)) {
+                                ok = false;
+                                break;
+                            }
+                            tc_fence_after();
+                            if (elected()) {
+                                if (TWO) {
+                                    issue(s, a, OPER, 0, a == from);
+                                    issue(s, a, 0, B_PART, false);
+                                } else {
+                                    issue(s, a, 0, 0, a == from);
+                                    umma_commit_pair(empty + s);
+                                    if (a + 1 == a1) umma_commit_pair(t_full + b);
                                 }
                             }
-                            umma_commit_pair(empty + s);
-                            if (done) umma_commit_pair(t_full + b);
+                            __syncwarp();
+                            if (!TWO) last_it = it;
                         }
-                        __syncwarp();
-                        last_stage = s;
-                        last_phase = use & 1;
-                        if (done) ++ti;
+                        if (TWO && ok) {
+                            if (elected()) {
+                                for (int i = it0; i < it; ++i) {
+                                    issue(i % NST, from + (i - it0), 0, 0, false);
+                                    umma_commit_pair(empty + i % NST);
+                                }
+                                umma_commit_pair(t_full + b);
+                            }
+                            __syncwarp();
+                            last_it = it - 1;
+                        }
+                        ++ti;
                     }
                 }
             }
@@ -982,7 +1044,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         // the next accumulator, or false when the kernel is aborting
         auto next = [&]() -> bool {
             int got = 0;
-            if (lane == 0) got = mbar_wait(t_full + ti % NACC, (ti / NACC) & 1, g.err, g.wait);
+            if (lane == 0) got = mbar_wait_spin(t_full + ti % NACC, (ti / NACC) & 1, g.err, g.wait);
             got = __shfl_sync(0xffffffffu, got, 0);
             tc_fence_after();
             return got != 0;
@@ -996,8 +1058,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         for (int u = pair; ok && u < units; u += pairs) {
             const Unit x = unit_of<MODE>(g, u);
             const int row0 = x.mt * PM + rank * BM + quad * 32;
-            typename EpilogueOf<MODE, TWO>::Type epi(g, p, row0 + lane, row0, x.t0, x.sp,
-                                                      factors + w * 64);
+            typename EpilogueOf<MODE, TWO>::Type epi(
+                p, row0 + lane, row0, x.sp, factors + w * 64,
+                staged + (MODE == GRAD ? w * PARTS * STAGED : 0), &omap);
             epi.load(x.t0 * BN + part * (BN / 4));
             for (int t = x.t0; ok && t < x.t1; ++t) {
                 const int col = t * BN + part * (BN / 4);
@@ -1007,7 +1070,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 if (TWO) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = 0.0f;
-                    for (int a = x.a0; a < x.a1; ++a) {
+                    for (int a = x.a0; a < x.a1; a += KBLOCK) {
                         if (!next()) {
                             ok = false;
                             break;
@@ -1044,9 +1107,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const unsigned long long c0 = clock64();
         if (warp == 0)
             while (clock64() - c0 < DRAIN_CYCLES) __nanosleep(1000);
-        if (warp == 1 && lane == 0 && last_stage >= 0)
-            while (!mbar_try(empty + last_stage, last_phase) && clock64() - c0 < DRAIN_CYCLES) {
+        if (warp == 1 && lane == 0 && last_it >= 0)
+            while (!mbar_try(empty + last_it % NST, (last_it / NST) & 1) &&
+                   clock64() - c0 < DRAIN_CYCLES) {
             }
+        if (MODE == GRAD && warp >= EPI_WARP0 && lane == 0)
+            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         __syncthreads();
     }
     cluster_sync();
@@ -1703,26 +1769,28 @@ constexpr size_t HEAD = 256;                    // error word, bounds
 constexpr size_t CHUNK_BYTES = (size_t)512 << 20;  // of group maxima, of score gradients
 constexpr int FEW = 8;                          // f32 queries a pass of few_kernel takes
 constexpr int FEW_QUERIES = 16, FEW_DIM = 2048;
-static size_t smem_of(bool two) {
-    // alignment, stages, barriers, column factors
-    return 1024 + (size_t)stages_of(two) * stage_bytes(two) + 256 + EPI_WARPS * 64 * 4;
+static size_t smem_of(bool two, bool grad) {
+    // alignment, stages, staged outputs, barriers, column factors
+    return 1024 + (size_t)stages_of(two, grad) * stage_bytes(two) + staged_of(two, grad) + 256 +
+           EPI_WARPS * 64 * 4;
 }
 
 static size_t up(size_t v, size_t m) { return (v + m - 1) / m * m; }
 static size_t elem(int dtype) { return dtype == FDB_DTYPE_F32 ? 4 : 2; }
 
 static CUtensorMap map2d(int dtype, const void* base, size_t inner, size_t rows, size_t ld_elems,
-                         int box_rows) {
+                         int box_rows, int box_cols = KATOM,
+                         CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
     CUtensorMap m;
     cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
     cuuint64_t strides[1] = {(cuuint64_t)ld_elems * 2};
-    cuuint32_t box[2] = {(cuuint32_t)KATOM, (cuuint32_t)box_rows};
+    cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
     cuuint32_t one[2] = {1, 1};
     const CUresult r = encode_fn()(
         &m,
         dtype == FDB_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
         2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+        swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     FDB_REQUIRE(r == CUDA_SUCCESS, FDB_ERR_CUDA, "cuTensorMapEncodeTiled failed");
     return m;
@@ -1765,23 +1833,25 @@ static int pick_splits(int tiles, int atoms, int sms, bool two, double out_bytes
 }
 template <int MODE, bool TWO>
 static void launch_rows(cudaStream_t s, int sms, const CUtensorMap& a, const CUtensorMap& b,
-                        const Mma& g, const typename EpilogueOf<MODE, TWO>::Type::Args& p) {
+                        const Mma& g, const typename EpilogueOf<MODE, TWO>::Type::Args& p,
+                        const CUtensorMap* out) {
     const long long units = MODE == PROD_Q || MODE == PROD_X
                                 ? (long long)g.mt * g.nt * g.chunks
                                 : (long long)g.mt * g.chunks;
-    const size_t smem = smem_of(TWO);
+    const size_t smem = smem_of(TWO, MODE == GRAD);
     FDB_CUDA(cudaFuncSetAttribute(rows_kernel<MODE, TWO>,
                                   cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     rows_kernel<MODE, TWO>
-        <<<2 * (unsigned)std::min<long long>(units, sms / 2), THREADS, smem, s>>>(a, b, g, p);
+        <<<2 * (unsigned)std::min<long long>(units, sms / 2), THREADS, smem, s>>>(a, b, out ? *out : a, g, p);
     FDB_LAUNCH_CHECK();
 }
 template <int MODE>
 static void launch_rows(bool two, cudaStream_t s, int sms, const CUtensorMap& a,
                         const CUtensorMap& b, const Mma& g,
-                        const typename EpilogueOf<MODE, false>::Type::Args& p) {
-    if (two) launch_rows<MODE, true>(s, sms, a, b, g, p);
-    else launch_rows<MODE, false>(s, sms, a, b, g, p);
+                        const typename EpilogueOf<MODE, false>::Type::Args& p,
+                        const CUtensorMap* out = nullptr) {
+    if (two) launch_rows<MODE, true>(s, sms, a, b, g, p, out);
+    else launch_rows<MODE, false>(s, sms, a, b, g, p, out);
 }
 
 // Hands out 256-byte aligned parts of the caller's workspace.
@@ -2107,6 +2177,8 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
     const size_t g_rows = w.parts * w.nqp;
     const CUtensorMap gk = map2d(FDB_DTYPE_F16, w.gr, w.ldg, g_rows, w.ldg, BM);
     const CUtensorMap gm = map2d(FDB_DTYPE_F16, w.gr, w.ldg, g_rows, w.ldg, 64);
+    const CUtensorMap go = map2d(FDB_DTYPE_F16, w.gr, w.ldg, g_rows, w.ldg, 32, 32,
+                                 CU_TENSOR_MAP_SWIZZLE_64B);
     Mma base{};
     base.err = w.err;
     base.wait = wait_limit_cycles(c);
@@ -2127,8 +2199,8 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
             p.nq = nq, p.n = n, p.j0 = (int)j0, p.cols = cols;
             p.coef = w.coef, p.qf = w.qf, p.xf = w.xf, p.bounds = w.bounds;
             p.allowed = a.allowed, p.ld_allowed = ld_allowed;
-            p.out = w.gr, p.ldg = w.ldg, p.plane = w.nqp * w.ldg;
-            launch_rows<GRAD>(two, s, c.sm_count, qk, xk, g, p);
+            p.ldg = w.ldg, p.nqp = (int)w.nqp;
+            launch_rows<GRAD>(two, s, c.sm_count, qk, xk, g, p, &go);
         }
         if (a.d_queries) {
             Mma g = base;
