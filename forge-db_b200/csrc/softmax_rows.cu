@@ -61,6 +61,7 @@ __host__ __device__ constexpr int stage_bytes(bool two) {
     return (two ? 2 : 1) * (OPER + bn_of(two) / 2 * 128);
 }
 __host__ __device__ constexpr int accs_of(bool two) { return two ? 4 : 2; }
+constexpr int MAX_STG = 8;
 constexpr int KBLOCK = 2;                   // K steps of an accumulator (two parts)
 constexpr int MAX_BN = 256;
 constexpr unsigned long long DRAIN_CYCLES = 4000000ull;  // about 2 ms
@@ -152,9 +153,10 @@ __device__ __forceinline__ void run_join(Run& r, Run o) {
         r.l += o.l * f;
     }
 }
-// As stored: m is -inf for a run without columns.
-__device__ __forceinline__ float4 run_stored(const Run& r) {
-    return make_float4(r.limit == -INFINITY ? -INFINITY : r.m, r.l, r.a, 0.0f);
+// As stored: m is -inf for a run without columns; top is the largest score of
+// its groups.
+__device__ __forceinline__ float4 run_stored(const Run& r, float top) {
+    return make_float4(r.limit == -INFINITY ? -INFINITY : r.m, r.l, r.a, top);
 }
 
 // A group's largest score without the mark of its pair.
@@ -328,6 +330,7 @@ struct Mma {
     int mt, nt, chunks;
     int atoms;                   // 64-wide steps of K
     int klast;                   // 16-wide MMA steps of the last of them
+    int resident;                // STATS, GRAD: A's K steps stay in shared memory for a unit
     int a_part, b_part;          // distance of the second part from the first in its map
     int b_row0;                  // PROD_Q: first row of the chunk
     int ncols;                   // PROD: columns of the output
@@ -471,12 +474,16 @@ __device__ __forceinline__ void arrive_leader(uint32_t bar) {
 // What a chunk of 32 columns needs besides its scores: the filter's word of
 // the thread's row, and (scaled rows) the columns' factors, in the warp's own
 // shared memory.  `load` starts the reads of a tile's chunks while the tile
-// before it is worked on, `ready` hands them over.
-template <bool FACTORS, int CHUNKS>
+// before it is worked on, `ready` hands them over.  BIAS, with a filter that all
+// queries share: what it adds to the columns (0 or NONE) lies there too, one
+// packed addition for two columns instead of a test and a select for each (the
+// factor of a column that nobody may see is 0, whatever its row holds).
+template <bool FACTORS, bool BIAS, int CHUNKS>
 struct Columns {
     uint32_t next[CHUNKS], word[CHUNKS];
     float nf[CHUNKS];
-    float* fac;  // [CHUNKS][32]
+    float* fac;  // [CHUNKS][32], then the biases
+    bool shared_filter;
     __device__ __forceinline__ void load(const uint32_t* al, const float* f, size_t col, int n) {
         const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -486,13 +493,16 @@ struct Columns {
         }
     }
     __device__ __forceinline__ void ready() {
-        if (FACTORS) __syncwarp();
+        if (FACTORS || BIAS) __syncwarp();
 #pragma unroll
         for (int h = 0; h < CHUNKS; ++h) {
             word[h] = next[h];
-            if (FACTORS) fac[32 * h + (threadIdx.x & 31)] = nf[h];
+            const int lane = threadIdx.x & 31;
+            const bool out = BIAS && shared_filter && !(next[h] >> lane & 1u);
+            if (FACTORS) fac[32 * h + lane] = out ? 0.0f : nf[h];
+            if (BIAS) fac[32 * (CHUNKS + h) + lane] = out ? NONE : 0.0f;
         }
-        if (FACTORS) __syncwarp();
+        if (FACTORS || BIAS) __syncwarp();
     }
 };
 
@@ -507,14 +517,19 @@ struct StatsEpilogue {
     float rf;
     Run r;
     bool live;
-    Columns<TWO, TWO ? 1 : 2> c;
+    Columns<TWO, TWO, TWO ? 1 : 2> c;
     const uint32_t* al;
+    float top_max;  // largest group's score of the unit (unmarked)
     __device__ StatsEpilogue(const StatsArgs& a, int row, int row0, int, float* fac,
                              unsigned char*, const CUtensorMap*)
         : p(a) {
         c.fac = fac;
+        c.shared_filter = a.ld_allowed == 0;
         q = row < a.nq ? row : -1;
-        al = q < 0 || !a.allowed ? nullptr : a.allowed + (size_t)(a.q0 + q) * a.ld_allowed;
+        // (with a filter of its own, rows past the end see everything: never stored)
+        al = !a.allowed || (q < 0 && a.ld_allowed)
+                 ? nullptr
+                 : a.allowed + (size_t)(a.q0 + max(q, 0)) * a.ld_allowed;
         live = row0 < a.nq;
         rf = a.rf;
         if (TWO && q >= 0) {
@@ -522,12 +537,16 @@ struct StatsEpilogue {
             rf = f == 0.0f ? a.rf : f * a.rf;  // a query of zeros scores 0
         }
         r = run_empty();
+        top_max = NONE;
     }
     __device__ __forceinline__ void load(int col) { c.load(al, p.xf, (size_t)col, p.n); }
-    // MASKED: some bit of some row's word is clear (two copies of the code: the
-    // selects are not free).
-    template <bool MASKED>
-    __device__ __forceinline__ float2 fold(const float (&u)[32], uint32_t w) {
+    // SEEN: 0: all rows see all columns; 1: each by its own word; 2: all rows
+    // see the same, by the columns' biases.  Copies of the code, as the selects
+    // are not free.
+    template <int SEEN>
+    __device__ __forceinline__ float2 fold(const float (&u)[32], uint32_t w, int h) {
+        constexpr int BIAS_AT = 32 * (TWO ? 1 : 2);
+        const float2* bias = reinterpret_cast<const float2*>(c.fac + BIAS_AT + 32 * h);
         const uint64_t rf2 = packf(rf, rf), nm2 = packf(-r.m, -r.m);
         float d[32];
 #pragma unroll
@@ -538,10 +557,14 @@ struct StatsEpilogue {
                 t = mul2(t, packf(f.x, f.y));
             }
             t = fma2(t, rf2, nm2);
+            if (SEEN == 2) {
+                const float2 f = bias[i];
+                t = add2(t, packf(f.x, f.y));
+            }
             d[2 * i] = lo_of(t);
             d[2 * i + 1] = hi_of(t);
         }
-        if (MASKED) {
+        if (SEEN == 1) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
                 if (!(w >> i & 1u)) d[i] = NONE;
@@ -552,10 +575,11 @@ struct StatsEpilogue {
             best = top_pair(d);
             // (the mark may have moved it; by far less than RAISE)
             cm = best.x;
-            if (best.x > NONE_BELOW)
-                best.x = __uint_as_float(
-                    (__float_as_uint(unmarked(best.x) + r.m) & ~15u) |
-                    (__float_as_uint(best.x) & 15u));
+            if (best.x > NONE_BELOW) {
+                const float v = unmarked(unmarked(best.x) + r.m);
+                best.x = __uint_as_float(__float_as_uint(v) | (__float_as_uint(best.x) & 15u));
+                top_max = fmaxf(top_max, v);
+            }
             best.y += r.m;
         } else {
             cm = max3(d[0], d[1], d[2]);
@@ -586,12 +610,13 @@ struct StatsEpilogue {
         const size_t col = (size_t)icol;
         const uint32_t w = h ? c.word[sizeof(c.word) / 4 - 1] : c.word[0];
         float2 best = make_float2(NONE, NONE);
-        if (__all_sync(0xffffffffu, w == 0xffffffffu)) best = fold<false>(u, w);
-        else if (__any_sync(0xffffffffu, w != 0u)) best = fold<true>(u, w);
+        if (__all_sync(0xffffffffu, w == 0xffffffffu)) best = fold<0>(u, w, h);
+        else if (__any_sync(0xffffffffu, w != 0u))
+            best = TWO && c.shared_filter ? fold<2>(u, w, h) : fold<1>(u, w, h);
         if (p.top && q >= 0) p.top[(size_t)q * p.groups + (col >> 5)] = best;
     }
     __device__ __forceinline__ void finish(int chunk, int part) {
-        if (q >= 0) p.part[(size_t)(chunk * 4 + part) * p.nq + q] = run_stored(r);
+        if (q >= 0) p.part[(size_t)(chunk * 4 + part) * p.nq + q] = run_stored(r, top_max);
     }
 };
 
@@ -605,7 +630,7 @@ struct GradEpilogue {
     bool live;  // (rows up to a multiple of 128 are written)
     Coef k;
     float wi;
-    Columns<true, TWO ? 1 : 2> c;
+    Columns<true, false, TWO ? 1 : 2> c;
     const uint32_t* al;
     unsigned char* stage;      // the warp's staged outputs, part 1 STAGED bytes on
     const CUtensorMap* omap;
@@ -757,7 +782,7 @@ struct ProdEpilogue {
     const ProdArgs& p;
     int row, split;
     float s;
-    Columns<false, 1> c;
+    Columns<false, false, 1> c;
     __device__ ProdEpilogue(const ProdArgs& a, int r, int, int sp, float*, unsigned char*,
                             const CUtensorMap*)
         : p(a) {
@@ -878,20 +903,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     const uint32_t base = smem_u32(smem_raw);
     unsigned char* smem = smem_raw + ((1024 - (base & 1023)) & 1023);
-    unsigned char* staged = smem + NST * STAGE;
+    constexpr int RING = NST * STAGE;
+    unsigned char* staged = smem + RING;
     unsigned char* after = staged + staged_of(TWO, MODE == GRAD);
+    // Few K steps: all of A at the ring's start, and stages of B alone.
+    const bool resident = !PROD && g.resident;
+    const int a_bytes = resident ? g.atoms * PARTS * OPER : 0;
+    const int stage = resident ? PARTS * B_PART : STAGE;
+    const int nst = resident ? min(MAX_STG, (RING - a_bytes) / stage) : NST;
+    const int b_at = resident ? 0 : B0;
+    unsigned char* ring = smem + a_bytes;
     uint64_t* full = reinterpret_cast<uint64_t*>(after);               // the first block's count
-    uint64_t* empty = full + NST;
-    uint64_t* t_full = empty + NST;
+    uint64_t* empty = full + MAX_STG;
+    uint64_t* t_full = empty + MAX_STG;
     uint64_t* t_empty = t_full + NACC;                                 // the first block's count
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(t_empty + NACC);
-    float* factors = reinterpret_cast<float*>(after + 256);             // [16 warps][64]
+    uint64_t* a_full = t_empty + NACC;                                 // the first block's counts
+    uint64_t* a_empty = a_full + 1;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(a_empty + 1);
+    float* factors = reinterpret_cast<float*>(after + 256);             // [16 warps][128]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank();
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const uint32_t full0 = leader_addr(full);
     if (threadIdx.x == 0) {
-        for (int i = 0; i < NST; ++i) {
+        for (int i = 0; i < MAX_STG; ++i) {
             mbar_init(full + i, 1);
             mbar_init(empty + i, 1);
         }
@@ -899,6 +934,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             mbar_init(t_full + i, 1);
             mbar_init(t_empty + i, 2 * EPI_WARPS);
         }
+        mbar_init(a_full, 1);
+        mbar_init(a_empty, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -913,22 +950,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const int units = PROD ? g.mt * g.nt * g.chunks : g.mt * g.chunks;
-    int last_it = -1;  // MMA issuer: last K step committed
+    int last_stage = -1;  // MMA issuer: last stage committed, and its phase
+    uint32_t last_phase = 0;
 
     if (warp == 0) {
-        int it = 0;
+        int s = 0, use = 0, ui = 0;  // stage, how often it was used before, units
         bool ok = !g.stall;
-        for (int u = pair; ok && u < units; u += pairs) {
+        for (int u = pair; ok && u < units; u += pairs, ++ui) {
             const Unit x = unit_of<MODE>(g, u);
             const int m0 = x.mt * PM + rank * BM;
+            if (resident) {
+                if (ui > 0 && !warp_wait(a_empty, (ui - 1) & 1, g.err, g.wait)) break;
+                if (elected()) {
+                    if (rank == 0) mbar_expect_tx(a_full, 2 * (uint32_t)a_bytes);
+                    const uint32_t bar = leader_addr(a_full);
+                    for (int a = 0; a < g.atoms; ++a)
+#pragma unroll
+                        for (int h = 0; h < PARTS; ++h)
+                            tma_load_pair(smem + (a * PARTS + h) * OPER, &amap, bar,
+                                          h * g.a_part + a * KATOM, m0);
+                }
+                __syncwarp();
+            }
             for (int t = x.t0; ok && t < x.t1; ++t) {
                 // this block's half of the columns: [n0, n0 + half)
                 const int half = PROD ? ((min(BN, g.ncols - t * BN) + 31) & ~31) / 2 : BN / 2;
                 const int n0 = t * BN + rank * half;
                 const int boxes = B_MN ? (half + 63) / 64 : 0;
-                const uint32_t bytes = PARTS * (OPER + (uint32_t)(B_MN ? boxes * 8192 : B_PART));
-                for (int a = x.a0; a < x.a1; ++a, ++it) {
-                    const int s = it % NST, use = it / NST;
+                const uint32_t bytes =
+                    PARTS * ((resident ? 0 : OPER) + (uint32_t)(B_MN ? boxes * 8192 : B_PART));
+                for (int a = x.a0; a < x.a1; ++a) {
                     if (use > 0 && !warp_wait(empty + s, (use - 1) & 1, g.err, g.wait)) {
                         ok = false;
                         break;
@@ -938,10 +989,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                         const uint32_t bar = full0 + 8 * s;
 #pragma unroll
                         for (int h = 0; h < PARTS; ++h) {
-                            unsigned char* da = smem + s * STAGE + h * OPER;
-                            unsigned char* db = smem + s * STAGE + B0 + h * B_PART;
+                            unsigned char* da = ring + s * stage + h * OPER;
+                            unsigned char* db = ring + s * stage + b_at + h * B_PART;
                             const int pa = h * g.a_part, pb = h * g.b_part;
-                            if (A_MN) {
+                            if (resident) {
+                            } else if (A_MN) {
                                 tma_load_pair(da, &amap, bar, m0, pa + a * KATOM);
                                 tma_load_pair(da + 8192, &amap, bar, m0 + 64, pa + a * KATOM);
                             } else if (PROD) {
@@ -960,15 +1012,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                         }
                     }
                     __syncwarp();
+                    if (++s == nst) s = 0, ++use;
                 }
             }
         }
     } else if (warp == 1) {
         if (rank == 0) {
-            int it = 0, ti = 0;  // K steps, accumulators
+            int s = 0, ti = 0, ui = 0;  // stage, accumulators, units
+            uint32_t phase = 0;         // of the stage
             bool ok = true;
-            for (int u = pair; ok && u < units; u += pairs) {
+            for (int u = pair; ok && u < units; u += pairs, ++ui) {
                 const Unit x = unit_of<MODE>(g, u);
+                if (resident && !warp_wait(a_full, ui & 1, g.err, g.wait)) break;
                 for (int t = x.t0; ok && t < x.t1; ++t) {
                     const int bn = PROD ? (min(BN, g.ncols - t * BN) + 31) & ~31 : BN;
                     const uint32_t idesc = g.idesc | ((uint32_t)(bn >> 3) << 17);
@@ -984,9 +1039,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                         }
                         tc_fence_after();
                         // (past the operands' last column the steps hold zeros)
-                        auto issue = [&](int stage, int atom, int ao, int bo, bool first) {
-                            const uint32_t ap = smem_u32(smem + stage * STAGE) + ao;
-                            const uint32_t bp = smem_u32(smem + stage * STAGE) + B0 + bo;
+                        auto issue = [&](int slot, int atom, int ao, int bo, bool first) {
+                            const uint32_t sp = smem_u32(ring + slot * stage);
+                            const uint32_t ap =
+                                (resident ? smem_u32(smem + atom * PARTS * OPER) : sp) + ao;
+                            const uint32_t bp = sp + b_at + bo;
                             const int kk1 = atom == g.atoms - 1 ? g.klast : 4;
 #pragma unroll
                             for (int kk = 0; kk < 4; ++kk)
@@ -998,10 +1055,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                                                    : smem_desc_sw128(bp + kk * 32),
                                               idesc, !first || kk > 0);
                         };
-                        const int it0 = it, from = a;
-                        for (; a < a1; ++a, ++it) {
-                            const int s = it % NST;
-                            if (!warp_wait(full + s, (it / NST) & 1, g.err, g.wait)) {
+                        const int s0 = s, from = a;
+                        uint32_t last = 0;
+                        for (; a < a1; ++a) {
+                            if (!warp_wait(full + s, phase, g.err, g.wait)) {
                                 ok = false;
                                 break;
                             }
@@ -1017,21 +1074,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                                 }
                             }
                             __syncwarp();
-                            if (!TWO) last_it = it;
+                            if (!TWO) last_stage = s, last_phase = phase;
+                            else last = phase;
+                            if (++s == nst) s = 0, phase ^= 1;
                         }
                         if (TWO && ok) {
-                            if (elected()) {
-                                for (int i = it0; i < it; ++i) {
-                                    issue(i % NST, from + (i - it0), 0, 0, false);
-                                    umma_commit_pair(empty + i % NST);
+                            int i = s0;
+                            for (int atom = from; atom < a1; ++atom) {
+                                if (elected()) {
+                                    issue(i, atom, 0, 0, false);
+                                    umma_commit_pair(empty + i);
+                                    if (atom + 1 == a1) umma_commit_pair(t_full + b);
                                 }
-                                umma_commit_pair(t_full + b);
+                                __syncwarp();
+                                last_stage = i;
+                                if (++i == nst) i = 0;
                             }
-                            __syncwarp();
-                            last_it = it - 1;
+                            last_phase = last;
                         }
                         ++ti;
                     }
+                }
+                if (resident && ok) {
+                    if (elected()) umma_commit_pair(a_empty);
+                    __syncwarp();
                 }
             }
         }
@@ -1059,7 +1125,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             const Unit x = unit_of<MODE>(g, u);
             const int row0 = x.mt * PM + rank * BM + quad * 32;
             typename EpilogueOf<MODE, TWO>::Type epi(
-                p, row0 + lane, row0, x.sp, factors + w * 64,
+                p, row0 + lane, row0, x.sp, factors + w * 128,
                 staged + (MODE == GRAD ? w * PARTS * STAGED : 0), &omap);
             epi.load(x.t0 * BN + part * (BN / 4));
             for (int t = x.t0; ok && t < x.t1; ++t) {
@@ -1068,9 +1134,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 if (t + 1 < x.t1) epi.load(col + BN);
                 float v[32];
                 if (TWO) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = 0.0f;
-                    for (int a = x.a0; a < x.a1; a += KBLOCK) {
+                    if (!next()) {
+                        ok = false;
+                        break;
+                    }
+                    load_chunk(mine + (uint32_t)(ti % NACC * BN), v);
+                    release();
+                    for (int a = x.a0 + KBLOCK; a < x.a1; a += KBLOCK) {
                         if (!next()) {
                             ok = false;
                             break;
@@ -1107,9 +1177,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const unsigned long long c0 = clock64();
         if (warp == 0)
             while (clock64() - c0 < DRAIN_CYCLES) __nanosleep(1000);
-        if (warp == 1 && lane == 0 && last_it >= 0)
-            while (!mbar_try(empty + last_it % NST, (last_it / NST) & 1) &&
-                   clock64() - c0 < DRAIN_CYCLES) {
+        if (warp == 1 && lane == 0 && last_stage >= 0)
+            while (!mbar_try(empty + last_stage, last_phase) && clock64() - c0 < DRAIN_CYCLES) {
             }
         if (MODE == GRAD && warp >= EPI_WARP0 && lane == 0)
             asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -1150,8 +1219,9 @@ __global__ void __launch_bounds__(64)
     const int row_of_lane = ((lane >> 4 & 1) << 2 | (lane >> 3 & 1) << 1 | (lane >> 2 & 1)) +
                             8 * (lane & 3);
     Run r[NQ];
+    float top_max[NQ];
 #pragma unroll
-    for (int j = 0; j < NQ; ++j) r[j] = run_empty();
+    for (int j = 0; j < NQ; ++j) r[j] = run_empty(), top_max[j] = NONE;
     const int ng = (n + GROUP - 1) / GROUP;
     for (int grp = blockIdx.x * 2 + warp; grp < ng; grp += gridDim.x * 2) {
         float sc[NQ];
@@ -1246,11 +1316,13 @@ __global__ void __launch_bounds__(64)
                     a = fmaxf(a, oa);
                 }
                 if (lane == 0) top[(size_t)j * groups + grp] = make_float2(a, b2);
+                if (a > NONE_BELOW) top_max[j] = fmaxf(top_max[j], unmarked(a));
             }
         }
     }
     // the lanes' triples joined, then the two warps'
     __shared__ Run other[NQ];
+    __shared__ float other_top[NQ];
 #pragma unroll
     for (int j = 0; j < NQ; ++j)
 #pragma unroll
@@ -1264,14 +1336,15 @@ __global__ void __launch_bounds__(64)
         }
     if (warp == 1 && lane == 0)
 #pragma unroll
-        for (int j = 0; j < NQ; ++j) other[j] = r[j];
+        for (int j = 0; j < NQ; ++j) other[j] = r[j], other_top[j] = top_max[j];
     __syncthreads();
     if (warp == 0 && lane == 0)
 #pragma unroll
         for (int j = 0; j < NQ; ++j)
             if (j < nq) {
                 run_join(r[j], other[j]);
-                part[(size_t)blockIdx.x * nq + j] = run_stored(r[j]);
+                part[(size_t)blockIdx.x * nq + j] =
+                    run_stored(r[j], fmaxf(top_max[j], other_top[j]));
             }
 }
 
@@ -1291,6 +1364,10 @@ struct FinishArgs {
     const float* qf;
     const float2* top;
     size_t groups;
+    // Which groups a part folded.  Tensor-core pass: part i is quarter i % 4 of
+    // the column tiles of chunk i / 4; few queries (nt = 0): part i is block i,
+    // whose two warps took every 2 * parts-th group.
+    int nt, chunks, per_tile, per_part;  // per_tile: groups of a tile, per_part: of its quarter
     float *logprob, *lse, *entropy, *top_logprob;
     int64_t* top_ids;
     const int* err;
@@ -1301,52 +1378,64 @@ __device__ __forceinline__ uint32_t ordered(float f) {
     const uint32_t u = __float_as_uint(f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+constexpr int PARTS_PICKED = 512;        // parts looked through at most
 constexpr int PICKED = 256;              // groups picked for exact scoring at most
-constexpr int CAND = MAX_SEL * GROUP;    // rows scored exactly and ranked at once
+constexpr int CAND = 1024;               // rows scored exactly and ranked at once
 
-// x . q in 64 bits over LANES lanes (a power of two): each product exact (f32)
-// or exact in f32 (16-bit types), added in 64 bits.
+// q . x of ROWS rows in 64 bits over `lanes` lanes (a power of two): each
+// product exact (f32) or exact in f32 (16-bit types), added in 64 bits.
 __device__ __forceinline__ double add_product(float x, float q, double s) {
     return fma((double)x, (double)q, s);
 }
-template <typename T>
-__device__ __forceinline__ double dot_lanes(const T* __restrict__ x, const float* q, int d, int sub,
-                                            int lanes, bool wide) {
+template <int ROWS, typename T>
+__device__ __forceinline__ void dot_lanes(const T* const (&x)[ROWS], const float* q, int d, int sub,
+                                          int lanes, bool wide, double (&s)[ROWS]) {
     constexpr int V = 16 / (int)sizeof(T);
-    double s0 = 0.0, s1 = 0.0;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) s[r] = 0.0;
     if (wide) {
-        for (int c = sub * V; c < d; c += lanes * V) {
-            if (c + V <= d) {
-                const uint4 raw = __ldg(reinterpret_cast<const uint4*>(x + c));
-                const T* e = reinterpret_cast<const T*>(&raw);
+        int c = sub * V;
+        for (; c + V <= d; c += lanes * V) {
+            uint4 raw[ROWS];
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) raw[r] = __ldg(reinterpret_cast<const uint4*>(x[r] + c));
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                const T* e = reinterpret_cast<const T*>(&raw[r]);
+                double a = 0.0, b = 0.0;
 #pragma unroll
                 for (int i = 0; i < V; i += 2) {
                     if (sizeof(T) == 4) {
-                        s0 = add_product(to_f32<T>(e[i]), q[c + i], s0);
-                        s1 = add_product(to_f32<T>(e[i + 1]), q[c + i + 1], s1);
+                        a = add_product(to_f32<T>(e[i]), q[c + i], a);
+                        b = add_product(to_f32<T>(e[i + 1]), q[c + i + 1], b);
                     } else {
-                        s0 += (double)__fmul_rn(to_f32<T>(e[i]), q[c + i]);
-                        s1 += (double)__fmul_rn(to_f32<T>(e[i + 1]), q[c + i + 1]);
+                        a += (double)__fmul_rn(to_f32<T>(e[i]), q[c + i]);
+                        b += (double)__fmul_rn(to_f32<T>(e[i + 1]), q[c + i + 1]);
                     }
                 }
-            } else {
-                for (int i = c; i < d; ++i) s0 = add_product(to_f32<T>(x[i]), q[i], s0);
+                s[r] += a + b;
             }
         }
+        for (; c < d; ++c) {  // (the row's last, partial vector: one lane's)
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) s[r] = add_product(to_f32<T>(x[r][c]), q[c], s[r]);
+        }
     } else {
-        for (int c = sub; c < d; c += lanes) s0 = add_product(to_f32<T>(x[c]), q[c], s0);
+        for (int c = sub; c < d; c += lanes)
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) s[r] = add_product(to_f32<T>(x[r][c]), q[c], s[r]);
     }
-    s0 += s1;
-    for (int o = lanes >> 1; o; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
-    return s0;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+        for (int o = lanes >> 1; o; o >>= 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], o);
 }
 
 // One block per query: the partial triples joined, the groups that may hold
 // one of the best k picked, their rows scored exactly and ranked.
 //
-// Picking needs no sort: the (k + 8)th largest of 128 maxima over interleaved
-// parts of the groups is a bound that at least k + 8 groups reach, and for
-// scores in no particular order hardly more do.
+// Picking needs no sort: the (k + 8)th largest of 128 maxima over the parts
+// is a bound that at least k + 8 groups reach, and for scores in no particular
+// order hardly more do; only the groups of the parts that reach it are read.
 template <typename T, int THREADS_>
 __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
     constexpr int W = THREADS_ / 32;
@@ -1355,7 +1444,8 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
     __shared__ double red[W][2];
     __shared__ float redf[W];
     __shared__ float s_bound;
-    __shared__ int s_picked, s_cnt;
+    __shared__ int s_picked, s_cnt, s_parts;
+    __shared__ int part_of[PARTS_PICKED];
     __shared__ int sel[PICKED];
     __shared__ float2 sel_m[PICKED];
     __shared__ double cs[CAND + 1];
@@ -1377,16 +1467,16 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
     const double unit = (double)p.scale * LOG2E, fix = (double)f * unit / (double)rf;
     const int64_t target = p.targets ? p.targets[q] : -1;
     const bool given = target >= 0 && target < p.n;
-    if (tid == 0) s_picked = s_cnt = 0, s_kth = -INFINITY;
+    if (tid == 0) s_picked = s_cnt = s_parts = 0, s_kth = -INFINITY;
     for (int c = tid; c < p.d; c += THREADS_) qs[c] = to_f32<T>(qp[c]);
 
-    // ---- largest scores: of the parts, and of 128 interleaved parts of the groups ----
-    float M = -INFINITY;
-    for (int i = tid; i < p.parts; i += THREADS_)
-        M = fmaxf(M, p.part[(size_t)i * p.nq + ql].x);
-    float gm = NONE;
-#pragma unroll 4
-    for (int i = tid; i < groups; i += THREADS_) gm = fmaxf(gm, unmarked(top[i].x));
+    // ---- the largest reference, and the largest scores of 128 sets of parts ----
+    float M = -INFINITY, gm = NONE;
+    for (int i = tid; i < p.parts; i += THREADS_) {
+        const float4 t = p.part[(size_t)i * p.nq + ql];
+        M = fmaxf(M, t.x);
+        gm = fmaxf(gm, t.w);
+    }
 #pragma unroll
     for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
 #pragma unroll
@@ -1437,12 +1527,22 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
     const int lanes = p.d * (int)sizeof(T) <= 512 ? 8 : 32;
     const int sub = lane & (lanes - 1);
     auto score = [&](int from, int to) {
+        constexpr int ROWS = 4;
         const int per = THREADS_ / lanes;
-        for (int i = from; i < to; i += per) {
-            const int j = i + tid / lanes;
-            const double v = dot_lanes<T>(xp + (size_t)(j < to ? ci[j] : 0) * p.ldx, qs, p.d, sub,
-                                          lanes, wide);
-            if (sub == 0 && j < to) cs[j] = v;
+        for (int i = from; i < to; i += ROWS * per) {
+            const T* x[ROWS];
+            double v[ROWS];
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                const int j = i + r * per + tid / lanes;
+                x[r] = xp + (size_t)ci[j < to ? j : from] * p.ldx;
+            }
+            dot_lanes<ROWS, T>(x, qs, p.d, sub, lanes, wide, v);
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                const int j = i + r * per + tid / lanes;
+                if (sub == 0 && j < to) cs[j] = v[r];
+            }
         }
     };
     auto seen = [&](uint32_t id) {
@@ -1451,17 +1551,41 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
 
     // ---- groups that reach the bound, the marked pair of each a candidate ----
     const float bound = p.k > 0 && !bad ? s_bound : INFINITY;
+    for (int i = tid; i < (groups ? p.parts : 0); i += THREADS_) {
+        const float t = p.part[(size_t)i * p.nq + ql].w;
+        if (t > NONE_BELOW && t >= bound) {
+            const int at = atomicAdd(&s_parts, 1);
+            if (at < PARTS_PICKED) part_of[at] = i;
+        }
+    }
+    __syncthreads();
+    const int nparts = min(s_parts, PARTS_PICKED);
+    // (the longest part's groups; chunks differ by one tile)
+    const int longest = p.nt ? (p.nt + p.chunks - 1) / p.chunks * p.per_part
+                             : 2 * ((groups + 2 * p.parts - 1) / max(1, 2 * p.parts));
 #pragma unroll 4
-    for (int i = tid; i < groups; i += THREADS_) {
-        const float2 m = top[i];
+    for (int i = tid; i < nparts * longest; i += THREADS_) {
+        const int part = part_of[i / longest], e = i % longest;
+        int gi;
+        if (p.nt) {
+            const int c = part >> 2;
+            const int t0 = (int)((long long)c * p.nt / p.chunks);
+            const int t = t0 + e / p.per_part;
+            gi = t < (int)((long long)(c + 1) * p.nt / p.chunks)
+                     ? t * p.per_tile + (part & 3) * p.per_part + e % p.per_part
+                     : groups;
+        } else {
+            gi = part * 2 + (e & 1) + (e >> 1) * 2 * p.parts;
+        }
+        const float2 m = gi < groups ? top[gi] : make_float2(NONE, NONE);
         if (m.x > NONE_BELOW && unmarked(m.x) >= bound) {
             const int at = atomicAdd(&s_picked, 1);
-            if (at < PICKED) sel[at] = i, sel_m[at] = m;
+            if (at < PICKED) sel[at] = gi, sel_m[at] = m;
         }
     }
     __syncthreads();
     const int picked = s_picked;
-    bool all_groups = picked > PICKED;  // (many equal scores)
+    bool all_groups = picked > PICKED || s_parts > PARTS_PICKED;  // (many equal scores)
     if (!all_groups && tid < picked) {
         const uint32_t pair = __float_as_uint(sel_m[tid].x) & 15u;
 #pragma unroll
@@ -1544,11 +1668,12 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
                     const uint32_t r = (uint32_t)(i + lane / lanes);
                     const bool in = w >> r & 1u;
                     const uint32_t id = (uint32_t)gi * GROUP + r;
-                    const double v = dot_lanes<T>(xp + (size_t)(in ? id : 0) * p.ldx, qs, p.d, sub,
-                                                  lanes, wide);
-                    if (sub == 0 && in && !(v < s_kth)) {
+                    const T* x[1] = {xp + (size_t)(in ? id : 0) * p.ldx};
+                    double v[1];
+                    dot_lanes<1, T>(x, qs, p.d, sub, lanes, wide, v);
+                    if (sub == 0 && in && !(v[0] < s_kth)) {
                         const int at = atomicAdd(&s_cnt, 1);
-                        cs[at] = v;
+                        cs[at] = v[0];
                         ci[at] = id;
                     }
                 }
@@ -1772,7 +1897,7 @@ constexpr int FEW_QUERIES = 16, FEW_DIM = 2048;
 static size_t smem_of(bool two, bool grad) {
     // alignment, stages, staged outputs, barriers, column factors
     return 1024 + (size_t)stages_of(two, grad) * stage_bytes(two) + staged_of(two, grad) + 256 +
-           EPI_WARPS * 64 * 4;
+           EPI_WARPS * 128 * 4;
 }
 
 static size_t up(size_t v, size_t m) { return (v + m - 1) / m * m; }
@@ -1844,6 +1969,11 @@ static void launch_rows(cudaStream_t s, int sms, const CUtensorMap& a, const CUt
     rows_kernel<MODE, TWO>
         <<<2 * (unsigned)std::min<long long>(units, sms / 2), THREADS, smem, s>>>(a, b, out ? *out : a, g, p);
     FDB_LAUNCH_CHECK();
+}
+// A's K steps stay in shared memory where they fill at most half of the ring
+// (4096 x 262144 x 96 f32: a tile's copies shrink to a third).
+static int stays(bool two, bool grad, int atoms) {
+    return atoms * (two ? 2 : 1) * OPER <= stages_of(two, grad) * stage_bytes(two) / 2;
 }
 template <int MODE>
 static void launch_rows(bool two, cudaStream_t s, int sms, const CUtensorMap& a,
@@ -2005,6 +2135,7 @@ void forward_run(Ctx& c, const fdb_logprob_args& a) {
         g.nt = w.nt;
         g.atoms = (int)((w.kp + 63) / 64);
         g.klast = (int)((w.kp - 64 * (size_t)(g.atoms - 1)) / 16);
+        g.resident = stays(w.packed, false, g.atoms);
         g.a_part = g.b_part = (int)w.kp;
         g.idesc = idesc_of(w.packed ? FDB_DTYPE_F16 : a.dtype, false, false);
         g.err = w.err;
@@ -2037,6 +2168,8 @@ void forward_run(Ctx& c, const fdb_logprob_args& a) {
             f.targets = a.targets;
             f.allowed = a.allowed, f.ld_allowed = ld_allowed;
             f.part = w.part, f.parts = g.chunks * 4;
+            f.nt = w.nt, f.chunks = g.chunks;
+            f.per_tile = w.bn / GROUP, f.per_part = w.bn / GROUP / 4;
             f.qf = p.qf;
             f.top = w.top, f.groups = w.groups;
             f.logprob = a.logprob, f.lse = a.lse, f.entropy = a.entropy;
@@ -2192,6 +2325,7 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
             g.chunks = pick_chunks(g.mt, g.nt, c.sm_count);
             g.atoms = (int)((w.kp + 63) / 64);
             g.klast = (int)((w.kp - 64 * (size_t)(g.atoms - 1)) / 16);
+            g.resident = stays(two, true, g.atoms);
             g.a_part = g.b_part = (int)w.kp;
             g.b_row0 = (int)j0;
             g.idesc = idesc_of(FDB_DTYPE_F16, false, false);

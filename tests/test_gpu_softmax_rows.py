@@ -224,6 +224,49 @@ def test_masked_rows_may_hold_anything(dtype, nq, bad):
 
 
 @pytest.mark.parametrize("dtype,nq", [("f32", 4), ("f32", 140), ("bf16", 140), ("f16", 20)])
+@pytest.mark.parametrize("bad", BADS)
+def test_one_filter_hides_what_its_rows_hold(dtype, nq, bad):
+    """The same with one filter for all queries."""
+    import forgegpu as fg
+    import torch
+    Q, X, T, _, *_ = make(dtype, nq, 700, 40, "none", seed=2)
+    keep = np.random.default_rng(1).random((1, 700)) < 0.6
+    keep[0, [0, 77, 350, 699]] = False
+    A = torch.from_numpy(so.words(keep)).cuda()
+    up = torch.rand(3, nq, device="cuda")
+
+    def go(X):
+        r = fg.logprobs(Q, X, T, scale=0.3, allowed=A, k=5)
+        return list(r) + list(fg.logprobs_backward(Q, X, T, r.lse, r.entropy, d_logprob=up[0],
+                                                   d_lse=up[1], d_entropy=up[2], scale=0.3,
+                                                   allowed=A))
+
+    X0, X1 = X.clone(), X.clone()
+    X0[[0, 77, 350, 699]] = 0
+    X1[[0, 77, 350, 699]] = bad
+    for a, b in zip(go(X0), go(X1)):
+        assert not torch.isnan(b).any()
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype,nq", [("f32", 3), ("f32", 40), ("bf16", 40)])
+def test_scores_that_lie_close_together(dtype, nq):
+    """A common part of 100 under differences of 1e-3 and less: more rows than
+    the picked groups hold are within the marks' reach of each other, and the
+    order is still that of 64-bit scores."""
+    import forgegpu as fg
+    import torch
+    rng = np.random.default_rng(7)
+    x = np.concatenate([np.full((4000, 1), 10.0), 2.0 ** -7 * rng.integers(0, 64, (4000, 7))], 1)
+    q = np.concatenate([np.full((nq, 1), 10.0), 2.0 ** -9 * rng.integers(1, 64, (nq, 7))], 1)
+    dt = _types()[dtype]
+    Q, X = torch.from_numpy(q).to(dt).cuda(), torch.from_numpy(x).to(dt).cuda()
+    r = fg.logprobs(Q, X, k=30)
+    f = so.forward(Q.double().cpu().numpy(), X.double().cpu().numpy(), None, 1.0, None, 30)
+    assert np.array_equal(r.top_ids.cpu().numpy(), f["top_ids"])
+
+
+@pytest.mark.parametrize("dtype,nq", [("f32", 4), ("f32", 140), ("bf16", 140), ("f16", 20)])
 @pytest.mark.parametrize("bad", BADS[:3])
 def test_what_is_not_finite_reaches_its_queries_only(dtype, nq, bad):
     import forgegpu as fg
