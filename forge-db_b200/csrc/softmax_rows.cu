@@ -1382,14 +1382,37 @@ constexpr int PARTS_PICKED = 512;        // parts looked through at most
 constexpr int PICKED = 256;              // groups picked for exact scoring at most
 constexpr int CAND = 1024;               // rows scored exactly and ranked at once
 
+// Order-preserving 64-bit image of a double, and back: integer comparisons are
+// what the ranking consists of.
+__device__ __forceinline__ uint64_t ordered64(double v) {
+    const uint64_t u = (uint64_t)__double_as_longlong(v);
+    return u >> 63 ? ~u : u | 0x8000000000000000ull;
+}
+__device__ __forceinline__ double unordered64(uint64_t u) {
+    return __longlong_as_double((long long)(u >> 63 ? u & 0x7fffffffffffffffull : ~u));
+}
+
 // q . x of ROWS rows in 64 bits over `lanes` lanes (a power of two): each
-// product exact (f32) or exact in f32 (16-bit types), added in 64 bits.
+// product exact (f32: of 64-bit copies of q) or exact in f32 (16-bit types),
+// added in 64 bits.
+template <typename T>
+struct Exact {
+    typedef float Q;
+};
+template <>
+struct Exact<float> {
+    typedef double Q;
+};
+__device__ __forceinline__ double add_product(float x, double q, double s) {
+    return fma((double)x, q, s);
+}
 __device__ __forceinline__ double add_product(float x, float q, double s) {
-    return fma((double)x, (double)q, s);
+    return s + (double)__fmul_rn(x, q);
 }
 template <int ROWS, typename T>
-__device__ __forceinline__ void dot_lanes(const T* const (&x)[ROWS], const float* q, int d, int sub,
-                                          int lanes, bool wide, double (&s)[ROWS]) {
+__device__ __forceinline__ void dot_lanes(const T* const (&x)[ROWS],
+                                          const typename Exact<T>::Q* q, int d, int sub, int lanes,
+                                          bool wide, double (&s)[ROWS]) {
     constexpr int V = 16 / (int)sizeof(T);
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) s[r] = 0.0;
@@ -1405,13 +1428,8 @@ __device__ __forceinline__ void dot_lanes(const T* const (&x)[ROWS], const float
                 double a = 0.0, b = 0.0;
 #pragma unroll
                 for (int i = 0; i < V; i += 2) {
-                    if (sizeof(T) == 4) {
-                        a = add_product(to_f32<T>(e[i]), q[c + i], a);
-                        b = add_product(to_f32<T>(e[i + 1]), q[c + i + 1], b);
-                    } else {
-                        a += (double)__fmul_rn(to_f32<T>(e[i]), q[c + i]);
-                        b += (double)__fmul_rn(to_f32<T>(e[i + 1]), q[c + i + 1]);
-                    }
+                    a = add_product(to_f32<T>(e[i]), q[c + i], a);
+                    b = add_product(to_f32<T>(e[i + 1]), q[c + i + 1], b);
                 }
                 s[r] += a + b;
             }
@@ -1439,19 +1457,20 @@ __device__ __forceinline__ void dot_lanes(const T* const (&x)[ROWS], const float
 template <typename T, int THREADS_>
 __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
     constexpr int W = THREADS_ / 32;
-    extern __shared__ float qs[];  // [dim]
-    __shared__ float part_max[128];
-    __shared__ double red[W][2];
+    extern __shared__ double qs_raw[];
+    typename Exact<T>::Q* qs = reinterpret_cast<typename Exact<T>::Q*>(qs_raw);  // [dim]
+    __shared__ __align__(16) float part_max[128];
+    __shared__ float2 red[W];
     __shared__ float redf[W];
     __shared__ float s_bound;
     __shared__ int s_picked, s_cnt, s_parts;
     __shared__ int part_of[PARTS_PICKED];
     __shared__ int sel[PICKED];
     __shared__ float2 sel_m[PICKED];
-    __shared__ double cs[CAND + 1];
+    __shared__ uint64_t cs[CAND + 1];  // exact scores, as ordered64
     __shared__ uint32_t ci[CAND + 1];
     __shared__ double s_kth;
-    __shared__ double kept[FDB_MAX_ALTERNATIVES];
+    __shared__ uint64_t kept[FDB_MAX_ALTERNATIVES];
     __shared__ uint32_t kept_id[FDB_MAX_ALTERNATIVES];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int ql = blockIdx.x, q = p.q0 + ql;
@@ -1487,39 +1506,50 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
 #pragma unroll
     for (int i = 0; i < W; ++i) M = fmaxf(M, redf[i]);
     // ---- the sums over the parts, in units of 2^M ----
-    double L = 0.0, A = 0.0;
+    float L = 0.0f, A = 0.0f;
     for (int i = tid; i < p.parts; i += THREADS_) {
         const float4 t = p.part[(size_t)i * p.nq + ql];
         if (t.y == 0.0f && t.z == 0.0f) continue;
         const float d = t.x == M ? 0.0f : t.x - M, e = ex2(d);
-        L += (double)(t.y * e);
-        A += (double)(__fmaf_rn(d, t.y, t.z) * e);
+        L = __fmaf_rn(t.y, e, L);
+        A = __fmaf_rn(__fmaf_rn(d, t.y, t.z), e, A);
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
         L += __shfl_xor_sync(0xffffffffu, L, o);
         A += __shfl_xor_sync(0xffffffffu, A, o);
     }
-    if (lane == 0) red[warp][0] = L, red[warp][1] = A;
+    if (lane == 0) red[warp] = make_float2(L, A);
     if (p.k > 0 && tid < 128) {
         int rank = 0;
         const float mine = part_max[tid];
+        const float4* all = reinterpret_cast<const float4*>(part_max);
 #pragma unroll 8
-        for (int i = 0; i < 128; ++i)
-            rank += part_max[i] > mine || (part_max[i] == mine && i < tid);
+        for (int i = 0; i < 32; ++i) {
+            const float4 v = all[i];
+            rank += v.x > mine || (v.x == mine && 4 * i < tid);
+            rank += v.y > mine || (v.y == mine && 4 * i + 1 < tid);
+            rank += v.z > mine || (v.z == mine && 4 * i + 2 < tid);
+            rank += v.w > mine || (v.w == mine && 4 * i + 3 < tid);
+        }
         if (rank == p.k + PAD - 1) s_bound = mine;
     }
     __syncthreads();
-    L = A = 0.0;
+    L = A = 0.0f;
 #pragma unroll
-    for (int i = 0; i < W; ++i) L += red[i][0], A += red[i][1];
-    const bool none = L == 0.0;  // no row may be seen
+    for (int i = 0; i < W; ++i) L += red[i].x, A += red[i].y;
+    const bool none = L == 0.0f;  // no row may be seen
     const bool bad = !(A == A) || !(L == L) || (p.err && *p.err != 0);
-    const double lg = none || bad ? 0.0 : log2(L);
+    // log2 of L by its exponent and its fraction: the large part is exact
+    double lg = 0.0;
+    if (!none && !bad) {
+        const int e = ilogbf(L);
+        lg = (double)e + (double)log2f(ldexpf(L, -e));
+    }
     const double lse = bad ? NAN : none ? -INFINITY : LN2 * ((double)M * fix + lg);
     if (tid == 0) {
         if (p.lse) p.lse[q] = (float)lse;
-        if (p.entropy) p.entropy[q] = (float)(bad ? NAN : none ? 0.0 : LN2 * (lg - A / L));
+        if (p.entropy) p.entropy[q] = (float)(bad ? NAN : none ? 0.0 : LN2 * (lg - (double)(A / L)));
     }
 
     // rows ci[from, to) scored exactly
@@ -1541,7 +1571,7 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
                 const int j = i + r * per + tid / lanes;
-                if (sub == 0 && j < to) cs[j] = v[r];
+                if (sub == 0 && j < to) cs[j] = ordered64(v[r]);
             }
         }
     };
@@ -1613,13 +1643,28 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
         float v = bad ? NAN : 0.0f;
         if (given && !bad)
             v = none || !seen((uint32_t)target) ? -INFINITY
-                                                : (float)(cs[cnt] * (double)p.scale - lse);
+                                                : (float)(unordered64(cs[cnt]) * (double)p.scale - lse);
         p.logprob[q] = v;
     }
     if (p.k == 0) return;
 
-    // candidate i before candidate j
-    auto before = [&](int i, int j) { return cs[i] > cs[j] || (cs[i] == cs[j] && ci[i] < ci[j]); };
+    // give(i, rank of candidate i among the first n), eight lanes a candidate
+    auto rank_all = [&](int n, auto&& give) {
+        for (int i0 = 0; i0 < n; i0 += THREADS_ / 8) {
+            const int i = i0 + tid / 8, at = min(i, n - 1);
+            const uint64_t v = cs[at];
+            const uint32_t id = ci[at];
+            int rank = 0;
+            for (int j = tid & 7; j < n; j += 8) {
+                const uint64_t o = cs[j];
+                rank += o > v || (o == v && ci[j] < id);
+            }
+            rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+            rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+            rank += __shfl_xor_sync(0xffffffffu, rank, 4);
+            if (i < n && (tid & 7) == 0) give(i, rank);
+        }
+    };
     // Whether a score of at most `m` (as a group left it) may be among the best
     // k, whose last exact score so far is s_kth: marks and 32-bit sums move it
     // by far less than 2^-15 of the larger of the two.
@@ -1627,11 +1672,9 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
         const double v = m / unit, kth = s_kth;
         return v >= kth - ldexp(fabs(v) + fabs(kth), -15);
     };
-    for (int i = tid; i < cnt; i += THREADS_) {
-        int rank = 0;
-        for (int j = 0; j < cnt; ++j) rank += before(j, i);
-        if (rank == p.k - 1) s_kth = cs[i];
-    }
+    rank_all(cnt, [&](int i, int rank) {
+        if (rank == p.k - 1) s_kth = unordered64(cs[i]);
+    });
     __syncthreads();
     // ---- groups whose second largest score may still enter: their other rows ----
     const bool more = bound > NONE_BELOW && may_enter(bound);  // groups below the bound may
@@ -1673,7 +1716,7 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
                     dot_lanes<1, T>(x, qs, p.d, sub, lanes, wide, v);
                     if (sub == 0 && in && !(v[0] < s_kth)) {
                         const int at = atomicAdd(&s_cnt, 1);
-                        cs[at] = v[0];
+                        cs[at] = ordered64(v[0]);
                         ci[at] = id;
                     }
                 }
@@ -1681,17 +1724,15 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
             __syncthreads();
             const int have = s_cnt;
             if (have + W * GROUP > CAND || g0 + W >= groups) {
-                for (int i = tid; i < have; i += THREADS_) {
-                    int rank = 0;
-                    for (int j = 0; j < have; ++j) rank += before(j, i);
+                rank_all(have, [&](int i, int rank) {
                     if (rank < p.k) kept[rank] = cs[i], kept_id[rank] = ci[i];
-                }
+                });
                 __syncthreads();
                 const int keep = min(have, p.k);
                 for (int i = tid; i < keep; i += THREADS_) cs[i] = kept[i], ci[i] = kept_id[i];
                 if (tid == 0) {
                     s_cnt = keep;
-                    if (keep == p.k) s_kth = kept[p.k - 1];
+                    if (keep == p.k) s_kth = unordered64(kept[p.k - 1]);
                 }
             }
         }
@@ -1699,14 +1740,13 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
     }
     // ---- written in order ----
     const int have = bad ? 0 : s_cnt;
-    for (int i = tid; i < have; i += THREADS_) {
-        int rank = 0;
-        for (int j = 0; j < have; ++j) rank += before(j, i);
+    rank_all(have, [&](int i, int rank) {
         if (rank < p.k) {
             p.top_ids[(size_t)q * p.k + rank] = (int64_t)ci[i];
-            p.top_logprob[(size_t)q * p.k + rank] = (float)(cs[i] * (double)p.scale - lse);
+            p.top_logprob[(size_t)q * p.k + rank] =
+                (float)(unordered64(cs[i]) * (double)p.scale - lse);
         }
-    }
+    });
     for (int i = have + tid; i < p.k; i += THREADS_) {
         p.top_ids[(size_t)q * p.k + i] = -1;
         p.top_logprob[(size_t)q * p.k + i] = bad ? NAN : -INFINITY;
@@ -2081,7 +2121,7 @@ size_t forward_bytes(const Ctx& c, const fdb_logprob_args& a) {
 
 template <typename T, int THREADS_>
 static void launch_finish_t(cudaStream_t s, const FinishArgs& f) {
-    const size_t smem = (size_t)f.d * 4;
+    const size_t smem = (size_t)f.d * sizeof(typename Exact<T>::Q);
     if (smem > 8192)
         FDB_CUDA(cudaFuncSetAttribute(finish_kernel<T, THREADS_>,
                                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
