@@ -132,20 +132,50 @@ __device__ __forceinline__ float unit(uint32_t h) { return (float)(h >> 8) * 0x1
 // y in [0, 256^2) or [0, 256^4): from the approximate root (a relative error
 // of about 2^-22, so its floor is right but next to a whole number), which is
 // replaced by the exact one there.
+// Conversions between small integers and floats go by adding 2^23, whose low
+// mantissa bits then are the integer: a quarter of the cycles of the conversion
+// instructions, of which a code would need ten.
 __device__ __forceinline__ float fast_sqrt(float y) {
     float r;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(y));
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
     return r;
 }
+__device__ __forceinline__ float nearest(float r) {  // 0 <= r < 2^22
+    return __fsub_rn(__fadd_rn(r, 8388608.0f), 8388608.0f);
+}
+__device__ __forceinline__ float below(float r, float n) { return r < n ? n - 1.0f : n; }
 __device__ __forceinline__ float root2(float y) {
-    const float r = fast_sqrt(y), n = rintf(r);
-    if (fabsf(r - n) < 0x1p-12f) return floorf(__fsqrt_rn(y));
-    return floorf(r);
+    const float r = fast_sqrt(y), n = nearest(r);
+    if (fabsf(r - n) < 0x1p-12f && y > 0.0f) {
+        const float e = __fsqrt_rn(y);
+        return below(e, nearest(e));
+    }
+    return below(r, n);
 }
 __device__ __forceinline__ float root4(float y) {
-    const float r = fast_sqrt(fast_sqrt(y)), n = rintf(r);
-    if (fabsf(r - n) < 0x1p-12f) return floorf(__fsqrt_rn(__fsqrt_rn(y)));
-    return floorf(r);
+    const float r = fast_sqrt(fast_sqrt(y)), n = nearest(r);
+    if (fabsf(r - n) < 0x1p-12f && y > 0.0f) {
+        const float e = __fsqrt_rn(__fsqrt_rn(y));
+        return below(e, nearest(e));
+    }
+    return below(r, n);
+}
+// Byte `i` of w as a float, less `off`.
+__device__ __forceinline__ float byte_float(uint32_t w, int i, float off) {
+    return __fsub_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7540 + i)), 8388608.0f + off);
+}
+// Whole numbers in [-128, 255] as the low bytes of four words, and these as one.
+__device__ __forceinline__ uint32_t low_byte(float k) {
+    return __float_as_uint(__fadd_rn(k, 12582912.0f));
+}
+__device__ __forceinline__ uint32_t pack_bytes(const uint32_t* w) {
+    return __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
+}
+// The larger of the two, NaN if one is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
 }
 // u < (y - lo) / (hi - lo), the quotient correctly rounded: decided by the
 // product unless the two sides are within the roundings of each other.
@@ -239,82 +269,82 @@ __global__ void __launch_bounds__(THREADS)
         const size_t i = b0 + (size_t)lane * 8, blk = b0 / BLOCK8;
         Vec<P, 8> pv;
         Vec<G, 8> gv;
-        Vec<int8_t, 8> mc;
-        Vec<uint8_t, 8> vc;
+        uint2 mc = make_uint2(0, 0), vc = make_uint2(0, 0);  // eight codes each
         const bool wide = e.wide && b0 + BLOCK8 <= i1;
         if (wide) {
             gv = *reinterpret_cast<const Vec<G, 8>*>(g + i);
             pv = *reinterpret_cast<const Vec<P, 8>*>(p + i);
-            mc = *reinterpret_cast<const Vec<int8_t, 8>*>(m8 + i);
-            vc = *reinterpret_cast<const Vec<uint8_t, 8>*>(v8 + i);
+            mc = *reinterpret_cast<const uint2*>(m8 + i);
+            vc = *reinterpret_cast<const uint2*>(v8 + i);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const bool in = i + j < i1;
                 gv.e[j] = in ? g[i + j] : put<G>(0.0f);
                 pv.e[j] = in ? p[i + j] : put<P>(0.0f);
-                mc.e[j] = in ? m8[i + j] : (int8_t)0;
-                vc.e[j] = in ? v8[i + j] : (uint8_t)0;
+                const uint32_t a = in ? (uint8_t)m8[i + j] : 0u, b = in ? v8[i + j] : 0u;
+                (j < 4 ? mc.x : mc.y) |= a << (8 * (j & 3));
+                (j < 4 ? vc.x : vc.y) |= b << (8 * (j & 3));
             }
         }
         const float ks = __fmul_rn(e.ms[blk], KM), kv = __fmul_rn(e.vs[blk], KV);
         float m[8], v[8], sm = 0.0f, sv = 0.0f;
-        bool nan_m = false, nan_v = false;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float a = (float)mc.e[j], r = (float)vc.e[j];
+            // (signed codes as c + 128)
+            const float a = byte_float((j < 4 ? mc.x : mc.y) ^ 0x80808080u, j & 3, 128.0f);
+            const float r = byte_float(j < 4 ? vc.x : vc.y, j & 3, 0.0f);
             m[j] = __fmul_rn(__fmul_rn(a, fabsf(a)), ks);
             const float r2 = __fmul_rn(r, r);
             v[j] = __fmul_rn(__fmul_rn(r2, r2), kv);
             moments(c, __fmul_rn(get<G>(gv.e[j]), c.gs), m[j], v[j]);
             pv.e[j] = put<P>(stepped(c, get<P>(pv.e[j]), m[j], v[j]));
-            if (i + j < i1) {
-                sm = fmaxf(sm, fabsf(m[j]));
-                sv = fmaxf(sv, v[j]);
-                nan_m |= m[j] != m[j];
-                nan_v |= v[j] != v[j];
-            }
+            // (past the tensor's end: zeros.  A NaN makes the block's scale NaN: the
+            // block reads as NaN from then on)
+            sm = max_nan(sm, fabsf(m[j]));
+            sv = max_nan(sv, v[j]);
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) {
-            sm = fmaxf(sm, __shfl_xor_sync(0xffffffffu, sm, o));
-            sv = fmaxf(sv, __shfl_xor_sync(0xffffffffu, sv, o));
+            sm = max_nan(sm, __shfl_xor_sync(0xffffffffu, sm, o));
+            sv = max_nan(sv, __shfl_xor_sync(0xffffffffu, sv, o));
         }
-        // (a NaN makes the block's scale NaN: the block reads as NaN from then on)
-        if (__any_sync(0xffffffffu, nan_m)) sm = NAN;
-        if (__any_sync(0xffffffffu, nan_v)) sv = NAN;
         const float km = sm > LEAST ? __fdiv_rn(M_CODES, sm) : 0.0f;
         const float kw = sv > LEAST ? __fdiv_rn(V_CODES, sv) : 0.0f;
+        // (i is a multiple of 8: the eight numbers differ in their last bits)
+        const uint32_t at =
+            (uint32_t)i ^ salt ^ ((uint32_t)((uint64_t)i >> 32) * 0x9E3779B1u);
+        uint32_t mb[8], vb[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const size_t at = i + j;
-            const uint32_t hh =
-                mix((uint32_t)at ^ salt ^ ((uint32_t)((uint64_t)at >> 32) * 0x9E3779B1u));
+            const uint32_t hh = mix(at ^ (uint32_t)j);
             const float y = __fmul_rn(fabsf(m[j]), km);
             float k = root2(y);
             float k1 = __fadd_rn(k, 1.0f);
             if (goes_up(unit(hh), y, __fmul_rn(k, k), __fmul_rn(k1, k1))) k = k1;
-            k = y > 0.0f ? fminf(k, 127.0f) : 0.0f;  // (also for a NaN)
-            mc.e[j] = (int8_t)(m[j] < 0.0f ? -k : k);
+            mb[j] = low_byte(copysignf(fminf(k, 127.0f), m[j]));
             const float z = __fmul_rn(v[j], kw);
             k = root4(z);
             k1 = __fadd_rn(k, 1.0f);
             const float lo = __fmul_rn(k, k), hi = __fmul_rn(k1, k1);
             if (goes_up(unit(mix(hh ^ 0x5BD1E995u)), z, __fmul_rn(lo, lo), __fmul_rn(hi, hi)))
                 k = k1;
-            vc.e[j] = z > 0.0f ? (uint8_t)fmaxf(fminf(k, 255.0f), 1.0f) : (uint8_t)0;
+            k = fmaxf(fminf(k, 255.0f), 1.0f);
+            vb[j] = low_byte(z > 0.0f ? k : 0.0f);
         }
+        mc = make_uint2(pack_bytes(mb), pack_bytes(mb + 4));
+        vc = make_uint2(pack_bytes(vb), pack_bytes(vb + 4));
         if (wide) {
             *reinterpret_cast<Vec<P, 8>*>(p + i) = pv;
-            *reinterpret_cast<Vec<int8_t, 8>*>(m8 + i) = mc;
-            *reinterpret_cast<Vec<uint8_t, 8>*>(v8 + i) = vc;
+            *reinterpret_cast<uint2*>(m8 + i) = mc;
+            *reinterpret_cast<uint2*>(v8 + i) = vc;
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (i + j < i1) {
                     p[i + j] = pv.e[j];
-                    m8[i + j] = mc.e[j];
-                    v8[i + j] = vc.e[j];
+                    m8[i + j] = (int8_t)((j < 4 ? mc.x : mc.y) >> (8 * (j & 3)));
+                    v8[i + j] = (uint8_t)((j < 4 ? vc.x : vc.y) >> (8 * (j & 3)));
                 }
         }
         if (lane == 0) {

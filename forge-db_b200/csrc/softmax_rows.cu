@@ -166,26 +166,31 @@ __device__ __forceinline__ float unmarked(float f) {
 // The largest of 32 values with the number of its pair in the low 4 bits, and
 // the second largest (either may be moved by the marks: 2^-19 relative).
 __device__ __forceinline__ float2 top_pair(const float (&u)[32]) {
-    float h[16], lo = NONE;
+    // four running (largest, second) pairs: an operation for the second, as
+    // there is a maximum of three
+    float m1[4], m2[4];
 #pragma unroll
-    for (int i = 0; i < 16; i += 2) {
-        const float l0 = fminf(u[2 * i], u[2 * i + 1]);
-        const float l1 = fminf(u[2 * i + 2], u[2 * i + 3]);
-        lo = max3(lo, l0, l1);
-        h[i] = __uint_as_float((__float_as_uint(fmaxf(u[2 * i], u[2 * i + 1])) & ~15u) | i);
-        h[i + 1] =
-            __uint_as_float((__float_as_uint(fmaxf(u[2 * i + 2], u[2 * i + 3])) & ~15u) | (i + 1));
-    }
-#pragma unroll
-    for (int w = 8; w >= 1; w >>= 1) {
-#pragma unroll
-        for (int i = 0; i < w; ++i) {
-            const float a = h[i], b = h[i + w];
-            lo = fmaxf(lo, fminf(a, b));
-            h[i] = fmaxf(a, b);
+    for (int i = 0; i < 16; ++i) {
+        const int c = i & 3;
+        const float hi = __uint_as_float(
+            (__float_as_uint(fmaxf(u[2 * i], u[2 * i + 1])) & ~15u) | (unsigned)i);
+        const float lo = fminf(u[2 * i], u[2 * i + 1]);
+        if (i < 4) {
+            m1[c] = hi;
+            m2[c] = lo;
+        } else {
+            m2[c] = max3(m2[c], lo, fminf(m1[c], hi));
+            m1[c] = fmaxf(m1[c], hi);
         }
     }
-    return make_float2(h[0], lo);
+#pragma unroll
+    for (int w = 2; w >= 1; w >>= 1)
+#pragma unroll
+        for (int c = 0; c < w; ++c) {
+            m2[c] = max3(m2[c], m2[c + w], fminf(m1[c], m1[c + w]));
+            m1[c] = fmaxf(m1[c], m1[c + w]);
+        }
+    return make_float2(m1[0], m2[0]);
 }
 
 // ---------------------------------------------------------------------------
@@ -211,7 +216,7 @@ struct PackSide {
     int wide;            // rows can be read in 16-byte vectors
 };
 template <typename T, int PARTS>
-__device__ __forceinline__ void pack_row(const PackSide& p, int row, int d, int kp) {
+__device__ __forceinline__ float pack_row(const PackSide& p, int row, int d, int kp) {
     constexpr int V = 16 / (int)sizeof(T), NV = 4;
     const int lane = threadIdx.x & 31;
     const T* src = static_cast<const T*>(p.x) + (size_t)row * p.ld;
@@ -282,13 +287,9 @@ __device__ __forceinline__ void pack_row(const PackSide& p, int row, int d, int 
             if (PARTS == 2) dst[kp + c] = __float2half_rn(v - __half2float(hi));
         }
     }
-    if (lane == 0) {
-        const float r = bad ? __int_as_float(0x7fc00000) : (mx > 0.0f ? ldexpf(1.0f, -e) : 0.0f);
-        p.f[row] = r;
-        // (most rows find their own power of two there already)
-        if (p.largest && r > 0.0f && __float_as_uint(r) > *(volatile unsigned*)p.largest)
-            atomicMax(p.largest, __float_as_uint(r));
-    }
+    const float r = bad ? __int_as_float(0x7fc00000) : (mx > 0.0f ? ldexpf(1.0f, -e) : 0.0f);
+    if (lane == 0) p.f[row] = r;
+    return r > 0.0f ? r : 0.0f;
 }
 // Both operands in one launch; the first block clears the error word.
 template <typename T, int PARTS>
@@ -297,10 +298,17 @@ __global__ void __launch_bounds__(256)
     if (err && blockIdx.x == 0 && threadIdx.x == 0) *err = 0;
     const bool first = (int)blockIdx.x < a.blocks;
     const int row = ((int)blockIdx.x - (first ? 0 : a.blocks)) * 8 + (threadIdx.x >> 5);
-    if (first) {
-        if (row < a.n) pack_row<T, PARTS>(a, row, d, kp);
-    } else if (row < b.n) {
-        pack_row<T, PARTS>(b, row, d, kp);
+    const PackSide& p = first ? a : b;
+    const float f = row < p.n ? pack_row<T, PARTS>(p, row, d, kp) : 0.0f;
+    if (!p.largest) return;
+    // the block's largest scale, unless it is there already
+    __shared__ unsigned most[8];
+    if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = __float_as_uint(f);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        unsigned m = 0;
+        for (int i = 0; i < 8; ++i) m = max(m, most[i]);
+        if (m > *(volatile unsigned*)p.largest) atomicMax(p.largest, m);
     }
 }
 // 16-bit rows copied to an aligned, zero-padded layout (their own is not one
@@ -546,23 +554,29 @@ struct StatsEpilogue {
     template <int SEEN>
     __device__ __forceinline__ float2 fold(const float (&u)[32], uint32_t w, int h) {
         constexpr int BIAS_AT = 32 * (TWO ? 1 : 2);
-        const float2* bias = reinterpret_cast<const float2*>(c.fac + BIAS_AT + 32 * h);
+        const float4* bias = reinterpret_cast<const float4*>(c.fac + BIAS_AT + 32 * h);
+        const float4* fac = reinterpret_cast<const float4*>(c.fac);
         const uint64_t rf2 = packf(rf, rf), nm2 = packf(-r.m, -r.m);
         float d[32];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            uint64_t t = packf(u[2 * i], u[2 * i + 1]);
+        for (int i = 0; i < 8; ++i) {
+            uint64_t t0 = packf(u[4 * i], u[4 * i + 1]), t1 = packf(u[4 * i + 2], u[4 * i + 3]);
             if (TWO) {
-                const float2 f = reinterpret_cast<const float2*>(c.fac)[i];
-                t = mul2(t, packf(f.x, f.y));
+                const float4 f = fac[i];
+                t0 = mul2(t0, packf(f.x, f.y));
+                t1 = mul2(t1, packf(f.z, f.w));
             }
-            t = fma2(t, rf2, nm2);
+            t0 = fma2(t0, rf2, nm2);
+            t1 = fma2(t1, rf2, nm2);
             if (SEEN == 2) {
-                const float2 f = bias[i];
-                t = add2(t, packf(f.x, f.y));
+                const float4 f = bias[i];
+                t0 = add2(t0, packf(f.x, f.y));
+                t1 = add2(t1, packf(f.z, f.w));
             }
-            d[2 * i] = lo_of(t);
-            d[2 * i + 1] = hi_of(t);
+            d[4 * i] = lo_of(t0);
+            d[4 * i + 1] = hi_of(t0);
+            d[4 * i + 2] = lo_of(t1);
+            d[4 * i + 3] = hi_of(t1);
         }
         if (SEEN == 1) {
 #pragma unroll
@@ -1881,38 +1895,73 @@ __device__ __forceinline__ void put(void* out, size_t o, int dtype, float v) {
     else if (dtype == FDB_DTYPE_BF16) static_cast<__nv_bfloat16*>(out)[o] = __float2bfloat16_rn(v);
     else static_cast<__half*>(out)[o] = __float2half_rn(v);
 }
-// Sum of the splits in order, scaled, in the output's type: four columns a
-// thread.
+// Sum of the splits, scaled, in the output's type: four columns of a row by one
+// thread, or by eight that take every eighth split and are added in order (16
+// splits and more: 64 of 100 x 128 took 10.9 us one after the other, now 3.7;
+// few splits of a large output are better off with more columns a block).
+template <int TURNS>
 __global__ void __launch_bounds__(256)
     join_kernel(const float* __restrict__ partial, int splits, int rows, int cols,
                 const float* __restrict__ f, const float* __restrict__ bounds, void* out,
                 size_t ldo, int dtype) {
+    constexpr int LANES = 256 / TURNS;
+    __shared__ float4 part[TURNS][LANES];
     const unsigned per4 = (unsigned)(cols + 3) / 4;
     const size_t plane = (size_t)rows * cols, all = (size_t)rows * per4;
     const bool wide = (cols & 3) == 0;
     const float c = grad_factor(bounds);
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (size_t)gridDim.x * 256) {
+    const int lane = threadIdx.x % LANES, turn = threadIdx.x / LANES;
+    for (size_t i0 = (size_t)blockIdx.x * LANES; i0 < all; i0 += (size_t)gridDim.x * LANES) {
+        const size_t i = i0 + lane;
         const size_t r = i / per4;
         const int k = (int)(i - r * per4) * 4;
         const float* src = partial + r * cols + k;
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (wide) {
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (i < all) {
+            if (wide) {
 #pragma unroll 4
-            for (int j = 0; j < splits; ++j) {
-                const float4 t = __ldcs(reinterpret_cast<const float4*>(src + j * plane));
-                v[0] += t.x, v[1] += t.y, v[2] += t.z, v[3] += t.w;
+                for (int j = turn; j < splits; j += TURNS) {
+                    const float4 t = __ldcs(reinterpret_cast<const float4*>(src + j * plane));
+                    v.x += t.x, v.y += t.y, v.z += t.z, v.w += t.w;
+                }
+            } else {
+                for (int j = turn; j < splits; j += TURNS) {
+                    const float* t = src + j * plane;
+                    v.x += t[0];
+                    if (k + 1 < cols) v.y += t[1];
+                    if (k + 2 < cols) v.z += t[2];
+                    if (k + 3 < cols) v.w += t[3];
+                }
             }
-        } else {
-            for (int j = 0; j < splits; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (k + e < cols) v[e] += src[j * plane + e];
         }
-        const float s = 1.0f / (f[r] * c);
+        if (TURNS > 1) {
+            part[turn][lane] = v;
+            __syncthreads();
+        }
+        if (turn == 0 && i < all) {
+            for (int j = 1; j < TURNS; ++j) {
+                const float4 t = part[j][lane];
+                v.x += t.x, v.y += t.y, v.z += t.z, v.w += t.w;
+            }
+            const float s = 1.0f / (f[r] * c);
+            const float o[4] = {v.x * s, v.y * s, v.z * s, v.w * s};
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (k + e < cols) put(out, r * ldo + k + e, dtype, v[e] * s);
+            for (int e = 0; e < 4; ++e)
+                if (k + e < cols) put(out, r * ldo + k + e, dtype, o[e]);
+        }
+        if (TURNS > 1) __syncthreads();
     }
+}
+static void launch_join(cudaStream_t s, int sms, const float* partial, int splits, int rows,
+                        int cols, const float* f, const float* bounds, void* out, size_t ldo,
+                        int dtype) {
+    if (splits >= 16)
+        join_kernel<8><<<sms * 8, 256, 0, s>>>(partial, splits, rows, cols, f, bounds, out, ldo,
+                                               dtype);
+    else
+        join_kernel<1><<<sms * 8, 256, 0, s>>>(partial, splits, rows, cols, f, bounds, out, ldo,
+                                               dtype);
+    FDB_LAUNCH_CHECK();
 }
 // A call whose waits ran out has no gradient: NaN.
 __global__ void void_kernel(const int* err, void* dq, size_t ldq, int nq, void* dx, size_t ldx,
@@ -2407,14 +2456,14 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
             p.out = out, p.ldo = a.ld_d_rows, p.dtype = a.dtype;
             launch_rows<PROD_X>(two, s, c.sm_count, gm, qm, g, p);
             if (w.dx) {
-                join_kernel<<<c.sm_count * 8, 256, 0, s>>>(w.dx, w.x_splits, cols, d, w.xf + j0,
+                launch_join(s, c.sm_count, w.dx, w.x_splits, cols, d, w.xf + j0,
                                                            w.bounds, out, a.ld_d_rows, a.dtype);
                 FDB_LAUNCH_CHECK();
             }
         }
     }
     if (a.d_queries) {
-        join_kernel<<<c.sm_count * 8, 256, 0, s>>>(w.dq, w.q_splits, nq, d, w.qf, w.bounds,
+        launch_join(s, c.sm_count, w.dq, w.q_splits, nq, d, w.qf, w.bounds,
                                                    a.d_queries, a.ld_d_queries, a.dtype);
         FDB_LAUNCH_CHECK();
     }
