@@ -203,7 +203,8 @@ __device__ __forceinline__ float2 top_pair(const float (&u)[32]) {
 // a score through f alone, so a query that may not see the row is not
 // touched).  `seen` (nullable): rows whose bit is clear are taken as zeros.
 // Bound by memory: reads d * size, writes 2 * parts * kp a row; rows of up to
-// 16 vectors a lane stay in registers between the two passes.
+// 4 vectors (or, unaligned, 14 pairs) a lane stay in registers between the two
+// passes.
 struct PackSide {
     const void* x;
     size_t ld;
@@ -217,13 +218,15 @@ struct PackSide {
 };
 template <typename T, int PARTS>
 __device__ __forceinline__ float pack_row(const PackSide& p, int row, int d, int kp) {
-    constexpr int V = 16 / (int)sizeof(T), NV = 4;
+    constexpr int V = 16 / (int)sizeof(T), NV = 4, NP = 14;
     const int lane = threadIdx.x & 31;
     const T* src = static_cast<const T*>(p.x) + (size_t)row * p.ld;
     __half* dst = p.out + (size_t)row * (size_t)(PARTS * kp);
     const bool use = !p.seen || (p.seen[row >> 5] >> (row & 31) & 1u);
     const bool held = p.wide && d <= 32 * V * NV;
+    const bool pairs = !held && d <= 64 * NP;  // two columns a lane and step
     uint4 raw[NV];
+    float two[2 * NP];
     float mx = 0.0f;
     bool bad = false;
     if (use && held) {
@@ -242,6 +245,19 @@ __device__ __forceinline__ float pack_row(const PackSide& p, int row, int d, int
                 bad |= !(v <= FLT_MAX);
                 mx = fmaxf(mx, v);
             }
+        }
+    } else if (use && pairs) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int c = i * 64 + 2 * lane;
+            two[2 * i] = c < d ? to_f32<T>(src[c]) : 0.0f;
+            two[2 * i + 1] = c + 1 < d ? to_f32<T>(src[c + 1]) : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * NP; ++i) {
+            const float v = fabsf(two[i]);
+            bad |= !(v <= FLT_MAX);
+            mx = fmaxf(mx, v);
         }
     } else if (use) {
         for (int c = lane; c < d; c += 32) {
@@ -277,6 +293,20 @@ __device__ __forceinline__ float pack_row(const PackSide& p, int row, int d, int
                 *reinterpret_cast<uint2*>(dst + c) = *reinterpret_cast<const uint2*>(hi);
                 if (PARTS == 2)
                     *reinterpret_cast<uint2*>(dst + kp + c) = *reinterpret_cast<const uint2*>(lo);
+            }
+        }
+    } else if (pairs) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int c = i * 64 + 2 * lane;
+            if (c >= kp) break;
+            const float a = zero ? 0.0f : two[2 * i] * s, b = zero ? 0.0f : two[2 * i + 1] * s;
+            const __half2 hi = __floats2half2_rn(a, b);
+            *reinterpret_cast<__half2*>(dst + c) = hi;
+            if (PARTS == 2) {
+                const float2 back = __half22float2(hi);
+                *reinterpret_cast<__half2*>(dst + kp + c) =
+                    __floats2half2_rn(a - back.x, b - back.y);
             }
         }
     } else {
@@ -374,6 +404,7 @@ struct GradArgs {
     size_t ld_allowed;
     size_t ldg;                 // output [parts][nqp][ldg]
     int nqp;
+    float* rest;                // one part: [nq] what fp16 leaves of the given row's G
 };
 struct ProdArgs {
     int rows, cols;             // output
@@ -692,9 +723,13 @@ struct GradEpilogue {
         const int at = k.target - (int)gcol;  // of the given row, if it is in this chunk
         if ((unsigned)at < 32u) {
             const float add = k.g * (c.fac[32 * h + at] * wi);
+            float all = 0.0f;
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-                if (i == at) u[i] += add;
+                if (i == at) all = u[i] += add;
+            // the largest G of most queries: what its rounding leaves is added to
+            // d_queries on its own (else it is most of the error of f16 results)
+            if (!TWO) p.rest[q] = all - __half2float(__float2half_rn(all));
         }
         __syncwarp();
         if (!__all_sync(0xffffffffu, w == 0xffffffffu)) {
@@ -747,60 +782,42 @@ struct GradEpilogue {
     }
 };
 
-// `count` values of one output row from column c, rounded to the output's type.
-__device__ __forceinline__ void store_row(void* out, size_t ldo, int dtype, int row, int c,
-                                          int count, const float (&v)[32]) {
-    const size_t es = dtype == FDB_DTYPE_F32 ? 4 : 2;
-    unsigned char* o = static_cast<unsigned char*>(out) + ((size_t)row * ldo + (size_t)c) * es;
-    const bool wide = (reinterpret_cast<uintptr_t>(o) & 15) == 0;
-    if (dtype == FDB_DTYPE_F32) {
-        float* f = reinterpret_cast<float*>(o);
+// Transposes a warp's 32 x 32 values: lane i's v[j] goes to lane j's v[i].
+__device__ __forceinline__ void transpose32(float (&v)[32]) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-            if (wide && i + 4 <= count)
-                *reinterpret_cast<float4*>(f + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-            else {
+    for (int s = 16; s; s >>= 1) {
+        const bool up = lane & s;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (i + j < count) f[i + j] = v[i + j];
-            }
-        }
-        return;
-    }
-    uint16_t* h = reinterpret_cast<uint16_t*>(o);
-#pragma unroll
-    for (int i = 0; i < 32; i += 8) {
-        uint32_t w[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (dtype == FDB_DTYPE_BF16) {
-                const __nv_bfloat162 b = __floats2bfloat162_rn(v[i + 2 * j], v[i + 2 * j + 1]);
-                w[j] = *reinterpret_cast<const uint32_t*>(&b);
-            } else {
-                const __half2 b = __floats2half2_rn(v[i + 2 * j], v[i + 2 * j + 1]);
-                w[j] = *reinterpret_cast<const uint32_t*>(&b);
-            }
-        }
-        if (wide && i + 8 <= count)
-            *reinterpret_cast<uint4*>(h + i) = make_uint4(w[0], w[1], w[2], w[3]);
-        else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (i + j < count) h[i + j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+        for (int i = 0; i < 32; ++i) {
+            if (i & s) continue;
+            const float give = up ? v[i] : v[i | s];
+            const float got = __shfl_xor_sync(0xffffffffu, give, s);
+            if (up) v[i] = got;
+            else v[i | s] = got;
         }
     }
 }
+__device__ __forceinline__ void put(void* out, size_t o, int dtype, float v) {
+    if (dtype == FDB_DTYPE_F32) static_cast<float*>(out)[o] = v;
+    else if (dtype == FDB_DTYPE_BF16) static_cast<__nv_bfloat16*>(out)[o] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(out)[o] = __float2half_rn(v);
+}
 
+// Stores go a row at a time, its 32 columns by the warp's lanes (whatever the
+// rows' alignment): a thread's own row in 16-byte pieces would touch 32 lines
+// an instruction.
 struct ProdEpilogue {
     typedef ProdArgs Args;
     const ProdArgs& p;
-    int row, split;
+    int row, row0, split;
     float s;
     Columns<false, false, 1> c;
-    __device__ ProdEpilogue(const ProdArgs& a, int r, int, int sp, float*, unsigned char*,
+    __device__ ProdEpilogue(const ProdArgs& a, int r, int r0, int sp, float*, unsigned char*,
                             const CUtensorMap*)
         : p(a) {
         row = r;
+        row0 = r0;
         split = sp;
         s = !a.partial && row < a.rows ? 1.0f / (a.f[row] * grad_factor(a.bounds)) : 0.0f;
     }
@@ -808,30 +825,28 @@ struct ProdEpilogue {
         c.next[0] = 0;
     }
     __device__ __forceinline__ void chunk(float (&u)[32], int c, int) {
-        if (c >= p.cols || row >= p.rows) return;
-        const int count = min(32, p.cols - c);
+        if (c >= p.cols || row0 >= p.rows) return;
+        const int lane = threadIdx.x & 31, rows = min(32, p.rows - row0);
         if (!p.partial) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) u[i] *= s;
-            store_row(p.out, p.ldo, p.dtype, row, c, count, u);
+        }
+        transpose32(u);
+        if (c + lane >= p.cols) return;
+        if (!p.partial) {
+            size_t o = (size_t)row0 * p.ldo + c + lane;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                if (i < rows) put(p.out, o, p.dtype, u[i]);
+                o += p.ldo;
+            }
             return;
         }
-        float* o = p.partial + ((size_t)split * p.rows + row) * (size_t)p.cols + c;
-        if ((p.cols & 3) == 0 && count == 32) {
+        float* o = p.partial + ((size_t)split * p.rows + row0) * (size_t)p.cols + c + lane;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float4 v = make_float4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
-                float4* o4 = reinterpret_cast<float4*>(o) + i;
-                if (p.add) {
-                    const float4 w = *o4;
-                    v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
-                }
-                *o4 = v;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-                if (i < count) o[i] = p.add ? o[i] + u[i] : u[i];
+        for (int i = 0; i < 32; ++i) {
+            if (i < rows) *o = p.add ? *o + u[i] : u[i];
+            o += p.cols;
         }
     }
     __device__ __forceinline__ void finish(int, int) {}
@@ -1505,17 +1520,22 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
 
     // ---- the largest reference, and the largest scores of 128 sets of parts ----
     float M = -INFINITY, gm = NONE;
-    for (int i = tid; i < p.parts; i += THREADS_) {
-        const float4 t = p.part[(size_t)i * p.nq + ql];
-        M = fmaxf(M, t.x);
-        gm = fmaxf(gm, t.w);
+    for (int i = tid; i < p.parts; i += THREADS_)
+        M = fmaxf(M, p.part[(size_t)i * p.nq + ql].x);
+    // (sets of parts where there are enough, else of groups)
+    const bool by_parts = p.parts >= 128;
+    if (tid < 128 && p.k > 0) {
+        if (by_parts)
+            for (int i = tid; i < p.parts; i += 128)
+                gm = fmaxf(gm, p.part[(size_t)i * p.nq + ql].w);
+        else
+#pragma unroll 4
+            for (int i = tid; i < groups; i += 128) gm = fmaxf(gm, unmarked(top[i].x));
+        part_max[tid] = gm;
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-#pragma unroll
-    for (int o = THREADS_ / 256; o; o >>= 1) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, o));
     if (lane == 0) redf[warp] = M;
-    if (tid % (THREADS_ / 128) == 0) part_max[tid / (THREADS_ / 128)] = gm;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < W; ++i) M = fmaxf(M, redf[i]);
@@ -1595,7 +1615,17 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
 
     // ---- groups that reach the bound, the marked pair of each a candidate ----
     const float bound = p.k > 0 && !bad ? s_bound : INFINITY;
-    for (int i = tid; i < (groups ? p.parts : 0); i += THREADS_) {
+    auto pick = [&](int gi, float2 m) {
+        if (m.x > NONE_BELOW && unmarked(m.x) >= bound) {
+            const int at = atomicAdd(&s_picked, 1);
+            if (at < PICKED) sel[at] = gi, sel_m[at] = m;
+        }
+    };
+    if (!by_parts) {
+#pragma unroll 4
+        for (int i = tid; i < groups; i += THREADS_) pick(i, top[i]);
+    }
+    for (int i = tid; i < (groups && by_parts ? p.parts : 0); i += THREADS_) {
         const float t = p.part[(size_t)i * p.nq + ql].w;
         if (t > NONE_BELOW && t >= bound) {
             const int at = atomicAdd(&s_parts, 1);
@@ -1621,11 +1651,7 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
         } else {
             gi = part * 2 + (e & 1) + (e >> 1) * 2 * p.parts;
         }
-        const float2 m = gi < groups ? top[gi] : make_float2(NONE, NONE);
-        if (m.x > NONE_BELOW && unmarked(m.x) >= bound) {
-            const int at = atomicAdd(&s_picked, 1);
-            if (at < PICKED) sel[at] = gi, sel_m[at] = m;
-        }
+        if (gi < groups) pick(gi, top[gi]);
     }
     __syncthreads();
     const int picked = s_picked;
@@ -1712,43 +1738,40 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
     all_groups = !bad && (all_groups || more || s_cnt > CAND);
     __syncthreads();
     if (all_groups) {
-        // ---- too many groups are as good (many equal or nearly equal scores):
-        // every row of every group that may enter is scored, the best k kept ----
+        // ---- too many groups are as good (many equal or nearly equal scores, or
+        // hardly more groups than k): every row of every group that may enter is
+        // scored, as many at a time as there is room for, the best k kept ----
         if (tid == 0) s_cnt = 0;
-        for (int g0 = 0; g0 < groups; g0 += W) {
+        __syncthreads();
+        const int step = (CAND - FDB_MAX_ALTERNATIVES) / GROUP;
+        for (int g0 = 0; g0 < groups; g0 += step) {
+            const int kept_now = s_cnt;
             __syncthreads();
-            const int gi = g0 + warp;
-            const float m1 = gi < groups ? top[gi].x : NONE;
-            if (m1 > NONE_BELOW && may_enter(m1)) {
+            for (int gi = g0 + warp; gi < min(groups, g0 + step); gi += W) {
+                const float m1 = top[gi].x;
+                if (!(m1 > NONE_BELOW) || !may_enter(m1)) continue;
                 const uint32_t w = allowed_word(al, 0, 0, (size_t)gi * GROUP, p.n);
-                for (int i = 0; i < GROUP; i += 32 / lanes) {
-                    const uint32_t r = (uint32_t)(i + lane / lanes);
-                    const bool in = w >> r & 1u;
-                    const uint32_t id = (uint32_t)gi * GROUP + r;
-                    const T* x[1] = {xp + (size_t)(in ? id : 0) * p.ldx};
-                    double v[1];
-                    dot_lanes<1, T>(x, qs, p.d, sub, lanes, wide, v);
-                    if (sub == 0 && in && !(v[0] < s_kth)) {
-                        const int at = atomicAdd(&s_cnt, 1);
-                        cs[at] = ordered64(v[0]);
-                        ci[at] = id;
-                    }
-                }
+                int at = 0;
+                if (lane == 0) at = atomicAdd(&s_cnt, __popc(w));
+                at = __shfl_sync(0xffffffffu, at, 0) + __popc(w & ((1u << lane) - 1u));
+                if (w >> lane & 1u) ci[at] = (uint32_t)gi * GROUP + (uint32_t)lane;
             }
             __syncthreads();
             const int have = s_cnt;
-            if (have + W * GROUP > CAND || g0 + W >= groups) {
-                rank_all(have, [&](int i, int rank) {
-                    if (rank < p.k) kept[rank] = cs[i], kept_id[rank] = ci[i];
-                });
-                __syncthreads();
-                const int keep = min(have, p.k);
-                for (int i = tid; i < keep; i += THREADS_) cs[i] = kept[i], ci[i] = kept_id[i];
-                if (tid == 0) {
-                    s_cnt = keep;
-                    if (keep == p.k) s_kth = unordered64(kept[p.k - 1]);
-                }
+            if (have == kept_now) continue;  // (the same for all threads)
+            score(kept_now, have);
+            __syncthreads();
+            rank_all(have, [&](int i, int rank) {
+                if (rank < p.k) kept[rank] = cs[i], kept_id[rank] = ci[i];
+            });
+            __syncthreads();
+            const int keep = min(have, p.k);
+            for (int i = tid; i < keep; i += THREADS_) cs[i] = kept[i], ci[i] = kept_id[i];
+            if (tid == 0) {
+                s_cnt = keep;
+                if (keep == p.k) s_kth = unordered64(kept[p.k - 1]);
             }
+            __syncthreads();
         }
         __syncthreads();
     }
@@ -1835,6 +1858,7 @@ struct CoefArgs {
     const uint32_t* allowed;
     size_t ld_allowed;
     Coef* out;
+    float* rest;    // nullable
     float* bounds;  // [0]
 };
 // G_ij = scale [ p_ij (dl - g - h (lp_ij + H)) + g 1{j = t} ] with lp = ln2 x:
@@ -1862,6 +1886,7 @@ __device__ __forceinline__ void coef_of(const CoefArgs& a, int i, float f) {
     k.g = (float)(a.scale * g);
     k.target = given ? (int)t : -1;
     a.out[i] = k;
+    if (a.rest) a.rest[i] = 0.0f;
     const float b = (float)(a.scale * (fabs(dl) + 2.0 * fabs(g) + fabs(dh) * (fabs(H) + 1.0)) *
                             (double)f);
     if (b > 0.0f && b <= FLT_MAX)
@@ -1890,11 +1915,13 @@ __global__ void __launch_bounds__(256)
         todo &= todo - 1;
     }
 }
-__device__ __forceinline__ void put(void* out, size_t o, int dtype, float v) {
-    if (dtype == FDB_DTYPE_F32) static_cast<float*>(out)[o] = v;
-    else if (dtype == FDB_DTYPE_BF16) static_cast<__nv_bfloat16*>(out)[o] = __float2bfloat16_rn(v);
-    else static_cast<__half*>(out)[o] = __float2half_rn(v);
-}
+// d_queries of 16-bit inputs: rest[r] times the given row is added (see GRAD).
+struct JoinRest {
+    const float* rest;  // null: nothing
+    const Coef* coef;
+    const __half* x;
+    int ldx;
+};
 // Sum of the splits, scaled, in the output's type: four columns of a row by one
 // thread, or by eight that take every eighth split and are added in order (16
 // splits and more: 64 of 100 x 128 took 10.9 us one after the other, now 3.7;
@@ -1903,7 +1930,7 @@ template <int TURNS>
 __global__ void __launch_bounds__(256)
     join_kernel(const float* __restrict__ partial, int splits, int rows, int cols,
                 const float* __restrict__ f, const float* __restrict__ bounds, void* out,
-                size_t ldo, int dtype) {
+                size_t ldo, int dtype, const JoinRest rest) {
     constexpr int LANES = 256 / TURNS;
     __shared__ float4 part[TURNS][LANES];
     const unsigned per4 = (unsigned)(cols + 3) / 4;
@@ -1943,6 +1970,16 @@ __global__ void __launch_bounds__(256)
                 const float4 t = part[j][lane];
                 v.x += t.x, v.y += t.y, v.z += t.z, v.w += t.w;
             }
+            if (rest.rest) {
+                const float g = rest.rest[r];
+                if (g != 0.0f) {
+                    const __half* x = rest.x + (size_t)rest.coef[r].target * rest.ldx + k;
+                    v.x = __fmaf_rn(g, __half2float(x[0]), v.x);
+                    if (k + 1 < cols) v.y = __fmaf_rn(g, __half2float(x[1]), v.y);
+                    if (k + 2 < cols) v.z = __fmaf_rn(g, __half2float(x[2]), v.z);
+                    if (k + 3 < cols) v.w = __fmaf_rn(g, __half2float(x[3]), v.w);
+                }
+            }
             const float s = 1.0f / (f[r] * c);
             const float o[4] = {v.x * s, v.y * s, v.z * s, v.w * s};
 #pragma unroll
@@ -1954,13 +1991,13 @@ __global__ void __launch_bounds__(256)
 }
 static void launch_join(cudaStream_t s, int sms, const float* partial, int splits, int rows,
                         int cols, const float* f, const float* bounds, void* out, size_t ldo,
-                        int dtype) {
+                        int dtype, const JoinRest& rest = JoinRest{}) {
     if (splits >= 16)
         join_kernel<8><<<sms * 8, 256, 0, s>>>(partial, splits, rows, cols, f, bounds, out, ldo,
-                                               dtype);
+                                               dtype, rest);
     else
         join_kernel<1><<<sms * 8, 256, 0, s>>>(partial, splits, rows, cols, f, bounds, out, ldo,
-                                               dtype);
+                                               dtype, rest);
     FDB_LAUNCH_CHECK();
 }
 // A call whose waits ran out has no gradient: NaN.
@@ -2316,6 +2353,7 @@ struct Backward {
     __half *qp, *xp, *gr;
     float *qf, *xf, *dq, *dx;
     Coef* coef;
+    float* rest;
     uint32_t *seen, *alive;
 };
 static Backward plan_backward(const Ctx& c, const fdb_logprob_grad_args& a) {
@@ -2342,6 +2380,7 @@ static Backward plan_backward(const Ctx& c, const fdb_logprob_grad_args& a) {
     w.qf = ws.take<float>(a.nq);
     w.xf = ws.take<float>(up(a.n, MAX_BN) + MAX_BN);
     w.coef = ws.take<Coef>(a.nq);
+    if (w.parts == 1) w.rest = ws.take<float>(a.nq);
     w.gr = ws.take<__half>((size_t)w.parts * w.nqp * w.ldg);
     w.dq = ws.take<float>((size_t)w.q_splits * a.nq * a.dim);
     if (w.x_splits > 1) w.dx = ws.take<float>((size_t)w.x_splits * w.cols * a.dim);
@@ -2383,7 +2422,7 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
     k.lse = a.lse, k.entropy = a.entropy;
     k.d_logprob = a.d_logprob, k.d_lse = a.d_lse, k.d_entropy = a.d_entropy;
     k.targets = a.targets, k.allowed = a.allowed, k.ld_allowed = ld_allowed;
-    k.out = w.coef, k.bounds = w.bounds;
+    k.out = w.coef, k.rest = w.rest, k.bounds = w.bounds;
     const int qblocks = (nq + 7) / 8;
     settle_kernel<<<qblocks + (n + 255) / 256, 256, 0, s>>>(k, w.qp, w.qf, w.xp, w.xf,
                                                             w.parts * (int)w.kp, qblocks);
@@ -2422,7 +2461,7 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
             p.nq = nq, p.n = n, p.j0 = (int)j0, p.cols = cols;
             p.coef = w.coef, p.qf = w.qf, p.xf = w.xf, p.bounds = w.bounds;
             p.allowed = a.allowed, p.ld_allowed = ld_allowed;
-            p.ldg = w.ldg, p.nqp = (int)w.nqp;
+            p.ldg = w.ldg, p.nqp = (int)w.nqp, p.rest = w.rest;
             launch_rows<GRAD>(two, s, c.sm_count, qk, xk, g, p, &go);
         }
         if (a.d_queries) {
@@ -2456,16 +2495,14 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
             p.out = out, p.ldo = a.ld_d_rows, p.dtype = a.dtype;
             launch_rows<PROD_X>(two, s, c.sm_count, gm, qm, g, p);
             if (w.dx) {
-                launch_join(s, c.sm_count, w.dx, w.x_splits, cols, d, w.xf + j0,
-                                                           w.bounds, out, a.ld_d_rows, a.dtype);
-                FDB_LAUNCH_CHECK();
+                launch_join(s, c.sm_count, w.dx, w.x_splits, cols, d, w.xf + j0, w.bounds, out,
+                            a.ld_d_rows, a.dtype);
             }
         }
     }
     if (a.d_queries) {
-        launch_join(s, c.sm_count, w.dq, w.q_splits, nq, d, w.qf, w.bounds,
-                                                   a.d_queries, a.ld_d_queries, a.dtype);
-        FDB_LAUNCH_CHECK();
+        launch_join(s, c.sm_count, w.dq, w.q_splits, nq, d, w.qf, w.bounds, a.d_queries,
+                    a.ld_d_queries, a.dtype, JoinRest{w.rest, w.coef, w.xp, (int)width});
     }
     void_kernel<<<c.sm_count, 256, 0, s>>>(w.err, a.d_queries, a.ld_d_queries, nq, a.d_rows,
                                            a.ld_d_rows, n, d, a.dtype);
