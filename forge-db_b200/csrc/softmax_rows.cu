@@ -1409,7 +1409,8 @@ __device__ __forceinline__ uint32_t ordered(float f) {
 }
 constexpr int PARTS_PICKED = 512;        // parts looked through at most
 constexpr int PICKED = 256;              // groups picked for exact scoring at most
-constexpr int CAND = 1024;               // rows scored exactly and ranked at once
+constexpr int CAND = 1024;               // rows scored exactly at once
+constexpr int KEPT = 256;                // ... and ranked, as a rule
 
 // Order-preserving 64-bit image of a double, and back: integer comparisons are
 // what the ranking consists of.
@@ -1499,8 +1500,10 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
     __shared__ uint64_t cs[CAND + 1];  // exact scores, as ordered64
     __shared__ uint32_t ci[CAND + 1];
     __shared__ double s_kth;
-    __shared__ uint64_t kept[FDB_MAX_ALTERNATIVES];
-    __shared__ uint32_t kept_id[FDB_MAX_ALTERNATIVES];
+    __shared__ uint64_t kept[KEPT];
+    __shared__ uint32_t kept_id[KEPT];
+    __shared__ uint64_t set_max[128];
+    __shared__ uint64_t s_least;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int ql = blockIdx.x, q = p.q0 + ql;
     const T* qp = static_cast<const T*>(p.q) + (size_t)q * p.ldq;
@@ -1705,6 +1708,45 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
             if (i < n && (tid & 7) == 0) give(i, rank);
         }
     };
+    // Of the first n candidates those of at least `least` (at least k), moved to
+    // the front if they are at most KEPT: ranking costs their number squared.
+    // Returns how many are left.
+    auto narrow = [&](int n, uint64_t least) -> int {
+        __syncthreads();
+        if (tid == 0) s_parts = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += THREADS_)
+            if (cs[i] >= least) {
+                const int at = atomicAdd(&s_parts, 1);
+                if (at < KEPT) kept[at] = cs[i], kept_id[at] = ci[i];
+            }
+        __syncthreads();
+        const int left = s_parts;
+        if (left > KEPT) return n;
+        for (int i = tid; i < left; i += THREADS_) cs[i] = kept[i], ci[i] = kept_id[i];
+        __syncthreads();
+        return left;
+    };
+    // The kth largest of 128 maxima over interleaved sets of n > 128 candidates:
+    // at least k reach it.
+    auto least_of = [&](int n) -> uint64_t {
+        if (tid < 128) {
+            uint64_t m = 0;
+            for (int i = tid; i < n; i += 128) m = max(m, cs[i]);
+            set_max[tid] = m;
+        }
+        __syncthreads();
+        if (tid < 128) {
+            const uint64_t m = set_max[tid];
+            int rank = 0;
+#pragma unroll 8
+            for (int i = 0; i < 128; ++i)
+                rank += set_max[i] > m || (set_max[i] == m && i < tid);
+            if (rank == p.k - 1) s_least = m;
+        }
+        __syncthreads();
+        return s_least;
+    };
     // Whether a score of at most `m` (as a group left it) may be among the best
     // k, whose last exact score so far is s_kth: marks and 32-bit sums move it
     // by far less than 2^-15 of the larger of the two.
@@ -1761,11 +1803,13 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
             if (have == kept_now) continue;  // (the same for all threads)
             score(kept_now, have);
             __syncthreads();
-            rank_all(have, [&](int i, int rank) {
+            int left = have;
+            if (have > KEPT) left = narrow(have, least_of(have));
+            rank_all(left, [&](int i, int rank) {
                 if (rank < p.k) kept[rank] = cs[i], kept_id[rank] = ci[i];
             });
             __syncthreads();
-            const int keep = min(have, p.k);
+            const int keep = min(left, p.k);
             for (int i = tid; i < keep; i += THREADS_) cs[i] = kept[i], ci[i] = kept_id[i];
             if (tid == 0) {
                 s_cnt = keep;
@@ -1776,7 +1820,8 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
         __syncthreads();
     }
     // ---- written in order ----
-    const int have = bad ? 0 : s_cnt;
+    int have = bad ? 0 : s_cnt;
+    if (have > 128 && s_kth > -INFINITY) have = narrow(have, ordered64(s_kth));
     rank_all(have, [&](int i, int rank) {
         if (rank < p.k) {
             p.top_ids[(size_t)q * p.k + rank] = (int64_t)ci[i];
@@ -2082,16 +2127,24 @@ static int pick_splits(int tiles, int atoms, int sms, bool two, double out_bytes
     }
     return best;
 }
+// Raises a kernel's shared-memory limit once per device.
+template <typename K>
+static void allow_smem(K* kernel, int device, size_t bytes, std::atomic<uint64_t>& done) {
+    if (device < 64 && done.load(std::memory_order_acquire) >> device & 1u) return;
+    FDB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    if (device < 64) done.fetch_or(1ull << device, std::memory_order_release);
+}
+
 template <int MODE, bool TWO>
-static void launch_rows(cudaStream_t s, int sms, const CUtensorMap& a, const CUtensorMap& b,
+static void launch_rows(cudaStream_t s, int device, int sms, const CUtensorMap& a, const CUtensorMap& b,
                         const Mma& g, const typename EpilogueOf<MODE, TWO>::Type::Args& p,
                         const CUtensorMap* out) {
     const long long units = MODE == PROD_Q || MODE == PROD_X
                                 ? (long long)g.mt * g.nt * g.chunks
                                 : (long long)g.mt * g.chunks;
     const size_t smem = smem_of(TWO, MODE == GRAD);
-    FDB_CUDA(cudaFuncSetAttribute(rows_kernel<MODE, TWO>,
-                                  cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    static std::atomic<uint64_t> done{0};
+    allow_smem(rows_kernel<MODE, TWO>, device, smem, done);
     rows_kernel<MODE, TWO>
         <<<2 * (unsigned)std::min<long long>(units, sms / 2), THREADS, smem, s>>>(a, b, out ? *out : a, g, p);
     FDB_LAUNCH_CHECK();
@@ -2102,12 +2155,12 @@ static int stays(bool two, bool grad, int atoms) {
     return atoms * (two ? 2 : 1) * OPER <= stages_of(two, grad) * stage_bytes(two) / 2;
 }
 template <int MODE>
-static void launch_rows(bool two, cudaStream_t s, int sms, const CUtensorMap& a,
+static void launch_rows(bool two, cudaStream_t s, int device, int sms, const CUtensorMap& a,
                         const CUtensorMap& b, const Mma& g,
                         const typename EpilogueOf<MODE, false>::Type::Args& p,
                         const CUtensorMap* out = nullptr) {
-    if (two) launch_rows<MODE, true>(s, sms, a, b, g, p, out);
-    else launch_rows<MODE, false>(s, sms, a, b, g, p, out);
+    if (two) launch_rows<MODE, true>(s, device, sms, a, b, g, p, out);
+    else launch_rows<MODE, false>(s, device, sms, a, b, g, p, out);
 }
 
 // Hands out 256-byte aligned parts of the caller's workspace.
@@ -2188,11 +2241,10 @@ static Forward plan_forward(const Ctx& c, const fdb_logprob_args& a) {
     } else {
         // (the last pass has fewer row blocks and may take more chunks)
         const int full = (int)((w.qb + PM - 1) / PM);
-        w.parts_cap = 0;
-        for (int mt = 1; mt <= full; ++mt)
-            if (mt == full || mt == (int)((a.nq % w.qb + PM - 1) / PM))
-                w.parts_cap = std::max<size_t>(w.parts_cap,
-                                               4 * (size_t)pick_chunks(mt, w.nt, c.sm_count));
+        const int last = (int)((a.nq % w.qb + PM - 1) / PM);
+        w.parts_cap = 4 * (size_t)pick_chunks(full, w.nt, c.sm_count);
+        if (last && last != full)
+            w.parts_cap = std::max(w.parts_cap, 4 * (size_t)pick_chunks(last, w.nt, c.sm_count));
     }
     w.part = ws.take<float4>(w.parts_cap * w.qb);
     if (a.k) w.top = ws.take<float2>(w.qb * w.groups);
@@ -2206,19 +2258,21 @@ size_t forward_bytes(const Ctx& c, const fdb_logprob_args& a) {
 }
 
 template <typename T, int THREADS_>
-static void launch_finish_t(cudaStream_t s, const FinishArgs& f) {
+static void launch_finish_t(cudaStream_t s, int device, const FinishArgs& f) {
     const size_t smem = (size_t)f.d * sizeof(typename Exact<T>::Q);
-    if (smem > 8192)
-        FDB_CUDA(cudaFuncSetAttribute(finish_kernel<T, THREADS_>,
-                                      cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (smem > 4096) {  // (with the static part, over what needs no permission)
+        static std::atomic<uint64_t> done{0};
+        allow_smem(finish_kernel<T, THREADS_>, device,
+                   FDB_MAX_SOFTMAX_DIM * sizeof(typename Exact<T>::Q), done);
+    }
     finish_kernel<T, THREADS_><<<f.nq, THREADS_, smem, s>>>(f);
     FDB_LAUNCH_CHECK();
 }
 template <typename T>
-static void launch_finish(cudaStream_t s, const FinishArgs& f) {
+static void launch_finish(cudaStream_t s, int device, const FinishArgs& f) {
     // A block a query.  Few queries: more threads share the groups of one.
-    if (f.nq <= 296) launch_finish_t<T, 512>(s, f);
-    else launch_finish_t<T, 128>(s, f);
+    if (f.nq <= 296) launch_finish_t<T, 512>(s, device, f);
+    else launch_finish_t<T, 128>(s, device, f);
 }
 
 void forward_run(Ctx& c, const fdb_logprob_args& a) {
@@ -2285,7 +2339,7 @@ void forward_run(Ctx& c, const fdb_logprob_args& a) {
             p.part = w.part;
             p.top = w.top;
             p.groups = w.groups;
-            launch_rows<STATS>(w.packed, s, c.sm_count, amap, bmap, g, p);
+            launch_rows<STATS>(w.packed, s, c.device, c.sm_count, amap, bmap, g, p);
             FinishArgs f{};
             f.q = a.queries, f.x = a.rows;
             f.ldq = a.ld_queries, f.ldx = a.ld_rows;
@@ -2301,9 +2355,9 @@ void forward_run(Ctx& c, const fdb_logprob_args& a) {
             f.logprob = a.logprob, f.lse = a.lse, f.entropy = a.entropy;
             f.top_logprob = a.top_logprobs, f.top_ids = a.top_ids;
             f.err = w.err;
-            if (a.dtype == FDB_DTYPE_F32) launch_finish<float>(s, f);
-            else if (a.dtype == FDB_DTYPE_F16) launch_finish<__half>(s, f);
-            else launch_finish<__nv_bfloat16>(s, f);
+            if (a.dtype == FDB_DTYPE_F32) launch_finish<float>(s, c.device, f);
+            else if (a.dtype == FDB_DTYPE_F16) launch_finish<__half>(s, c.device, f);
+            else launch_finish<__nv_bfloat16>(s, c.device, f);
         }
         return;
     }
@@ -2315,8 +2369,9 @@ void forward_run(Ctx& c, const fdb_logprob_args& a) {
         const unsigned blocks = (unsigned)w.parts_cap;
         auto go = [&](auto kernel, int NQ) {
             const size_t sm = NQ * dp * 4;
-            FDB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                          (int)sm));
+            if (sm > 40960)
+                FDB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                              (int)sm));
             kernel<<<blocks, 64, sm, s>>>(static_cast<const float*>(a.rows), a.ld_rows, n, d,
                                           static_cast<const float*>(a.queries), a.ld_queries,
                                           (int)q0, nq, rf, a.allowed, ld_allowed, w.part, w.top,
@@ -2338,7 +2393,7 @@ void forward_run(Ctx& c, const fdb_logprob_args& a) {
         f.top = w.top, f.groups = w.groups;
         f.logprob = a.logprob, f.lse = a.lse, f.entropy = a.entropy;
         f.top_logprob = a.top_logprobs, f.top_ids = a.top_ids;
-        launch_finish<float>(s, f);
+        launch_finish<float>(s, c.device, f);
     }
 }
 
@@ -2462,7 +2517,7 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
             p.coef = w.coef, p.qf = w.qf, p.xf = w.xf, p.bounds = w.bounds;
             p.allowed = a.allowed, p.ld_allowed = ld_allowed;
             p.ldg = w.ldg, p.nqp = (int)w.nqp, p.rest = w.rest;
-            launch_rows<GRAD>(two, s, c.sm_count, qk, xk, g, p, &go);
+            launch_rows<GRAD>(two, s, c.device, c.sm_count, qk, xk, g, p, &go);
         }
         if (a.d_queries) {
             Mma g = base;
@@ -2477,7 +2532,7 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
             ProdArgs p{};
             p.rows = nq, p.cols = d, p.f = w.qf, p.bounds = w.bounds;
             p.partial = w.dq, p.add = j0 > 0;
-            launch_rows<PROD_Q>(two, s, c.sm_count, gk, xm, g, p);
+            launch_rows<PROD_Q>(two, s, c.device, c.sm_count, gk, xm, g, p);
         }
         if (a.d_rows) {
             Mma g = base;
@@ -2493,7 +2548,7 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
             p.rows = cols, p.cols = d, p.f = w.xf + j0, p.bounds = w.bounds;
             p.partial = w.dx;
             p.out = out, p.ldo = a.ld_d_rows, p.dtype = a.dtype;
-            launch_rows<PROD_X>(two, s, c.sm_count, gm, qm, g, p);
+            launch_rows<PROD_X>(two, s, c.device, c.sm_count, gm, qm, g, p);
             if (w.dx) {
                 launch_join(s, c.sm_count, w.dx, w.x_splits, cols, d, w.xf + j0, w.bounds, out,
                             a.ld_d_rows, a.dtype);

@@ -928,8 +928,7 @@ def _torch():
 def _ctx_of(device) -> Context:
     """The context of a tensor's device (made once per device)."""
     i = device.index
-    with _lock:
-        c = _device_ctx.get(i)
+    c = _device_ctx.get(i)
     if c is None:
         c = default_context() if i == 0 else Context(i)
         with _lock:
@@ -943,51 +942,71 @@ def _refuse(msg: str):
 
 def _matrix(t, what: str, like=None):
     """(pointer, rows, row distance) of a 2-d tensor whose rows are contiguous."""
-    if t.dim() != 2 or t.device.type != "cuda" or t.dtype not in _DTYPE:
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or not t.is_cuda or t.dtype not in _DTYPE:
         _refuse(f"{what} must be a 2-d float32, float16 or bfloat16 tensor on a GPU")
-    n, d = t.shape
-    s0, s1 = t.stride()
+    n, d = shape
+    s0, s1 = stride
     if (s1 != 1 and d > 1) or (n > 1 and s0 < d):
         _refuse(f"{what} must have contiguous rows")
     if like is not None and (t.dtype != like.dtype or t.device != like.device):
         _refuse(f"{what} must have the queries' type and device")
-    return t.data_ptr(), n, s0 if n > 1 else max(s0, d)
+    return t.data_ptr(), n, s0 if n > 1 and s0 > d else d
 
 
-def _vector(t, n: int, dtype, like, what: str):
+def _vector(t, n: int, dtype, device, what: str):
     if t is None:
         return None
-    if t.dtype != dtype or t.device != like.device or t.shape != (n,) or not t.is_contiguous():
+    if t.dtype != dtype or t.device != device or t.shape != (n,) or not t.is_contiguous():
         _refuse(f"{what} must be a contiguous {dtype} tensor of {n} values on the queries' device")
     return t.data_ptr()
 
 
-def _softmax_args(a, q, x, targets, scale, allowed):
+def _softmax_args(q, x, targets, scale, allowed):
+    """The fields that both argument structures start with."""
     torch = _torch()
-    a.queries, a.nq, a.ld_queries = _matrix(q, "queries")
-    a.rows, a.n, a.ld_rows = _matrix(x, "rows", q)
-    a.dtype = _DTYPE[q.dtype]
-    a.dim = q.shape[1]
-    if x.shape[1] != a.dim:
-        raise ForgeGpuError(-2, f"queries of {a.dim} and rows of {x.shape[1]} dimensions")
-    a.scale = scale
-    a.targets = _vector(targets, a.nq, torch.int64, q, "targets")
+    qp, nq, ldq = _matrix(q, "queries")
+    xp, n, ldx = _matrix(x, "rows", q)
+    dim, dev = q.shape[1], q.device
+    if x.shape[1] != dim:
+        raise ForgeGpuError(-2, f"queries of {dim} and rows of {x.shape[1]} dimensions")
+    ap, lda = None, 0
     if allowed is not None:
-        words = (a.n + 31) // 32
-        if allowed.dtype != torch.int32 or allowed.device != q.device or allowed.dim() not in (1, 2) \
+        words = (n + 31) // 32
+        if allowed.dtype != torch.int32 or allowed.device != dev or allowed.dim() not in (1, 2) \
                 or allowed.shape[-1] != words or (words > 1 and allowed.stride(-1) != 1):
             _refuse(f"allowed must be int32 words [{words}] or [1 or nq, {words}] on the "
                     "queries' device")
         rows = 1 if allowed.dim() == 1 else allowed.shape[0]
-        if rows not in (1, a.nq):
-            _refuse(f"allowed has {rows} filters for {a.nq} queries")
-        a.allowed = allowed.data_ptr()
+        if rows not in (1, nq):
+            _refuse(f"allowed has {rows} filters for {nq} queries")
+        ap = allowed.data_ptr()
         if rows > 1:
-            if allowed.stride(0) < words:
+            lda = allowed.stride(0)
+            if lda < words:
                 _refuse("allowed must have contiguous rows")
-            a.ld_allowed = allowed.stride(0)
-    a.stream = torch.cuda.current_stream(q.device).cuda_stream
-    return torch
+    return (_DTYPE[q.dtype], qp, nq, ldq, xp, n, ldx, dim, scale,
+            _vector(targets, nq, torch.int64, dev, "targets"), ap, lda)
+
+
+_ws_bytes: dict = {}
+
+
+def _workspace(torch, ctx, fn, a, key, device, given):
+    """(tensor, its bytes): the caller's workspace, or a new one of the size that
+    the call needs (asked for once per shape)."""
+    if given is not None:
+        if given.dtype != torch.uint8 or given.device != device or not given.is_contiguous():
+            _refuse("the workspace must be a contiguous uint8 tensor on the queries' device")
+        return given, given.numel()
+    need = _ws_bytes.get(key)
+    if need is None:
+        size = _sz()
+        _check(fn(ctx.h, C.byref(a), C.byref(size)))
+        if len(_ws_bytes) > 1024:
+            _ws_bytes.clear()
+        need = _ws_bytes[key] = size.value
+    return torch.empty(need, dtype=torch.uint8, device=device), need
 
 
 def logprobs(queries, rows, targets=None, *, scale: float = 1.0, allowed=None, k: int = 0,
@@ -998,26 +1017,28 @@ def logprobs(queries, rows, targets=None, *, scale: float = 1.0, allowed=None, k
     targets: int64 [nq], the row whose log probability is wanted (none where
     negative).  allowed: int32 words of a bit per row, one filter or one per
     query.  k: number of alternatives.  workspace: a uint8 tensor to use
-    instead of a new one (fdb_logprobs_status reads a timeout from it)."""
-    a = LogprobArgs()
-    torch = _softmax_args(a, queries, rows, targets, scale, allowed)
-    ctx = _ctx_of(queries.device)
+    instead of a new one (logprobs_status reads a timeout from it)."""
+    torch = _torch()
+    head = _softmax_args(queries, rows, targets, scale, allowed)
+    dev, nq = queries.device, head[2]
+    ctx = _ctx_of(dev)
     L = lib()
-    a.k = k
-    need = _sz()
-    _check(L.fdb_logprobs_workspace(ctx.h, C.byref(a), C.byref(need)))
-    dev, nq = queries.device, a.nq
-    out = torch.empty((3, nq), dtype=torch.float32, device=dev)
-    ids = torch.empty((nq, k), dtype=torch.int64, device=dev)
-    top = torch.empty((nq, k), dtype=torch.float32, device=dev)
-    ws = workspace if workspace is not None else torch.empty(need.value, dtype=torch.uint8,
-                                                             device=dev)
-    base = out.data_ptr()
-    a.logprob, a.lse, a.entropy = base, base + 4 * nq, base + 8 * nq
-    a.top_ids, a.top_logprobs = ids.data_ptr(), top.data_ptr()
-    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-    _check(L.fdb_logprobs(ctx.h, C.byref(a)))
-    return LogProbs(out[0], out[1], out[2], ids, top)
+    empty, f32 = torch.empty, torch.float32
+    lp, lse, ent = (empty(nq, dtype=f32, device=dev), empty(nq, dtype=f32, device=dev),
+                    empty(nq, dtype=f32, device=dev))
+    ids = empty((nq, k), dtype=torch.int64, device=dev)
+    top = empty((nq, k), dtype=f32, device=dev)
+    a = LogprobArgs(*head, k, lp.data_ptr(), lse.data_ptr(), ent.data_ptr(), ids.data_ptr(),
+                    top.data_ptr())
+    # (whether the operands are copied depends on their alignment)
+    key = (dev.index, k, head[1] & 15, head[4] & 15) + head[0:1] + head[2:4] + head[5:8]
+    ws, a.workspace_bytes = _workspace(torch, ctx, L.fdb_logprobs_workspace, a, key, dev, workspace)
+    a.workspace = ws.data_ptr()
+    a.stream = torch._C._cuda_getCurrentRawStream(dev.index)
+    rc = L.fdb_logprobs(ctx.h, C.byref(a))
+    if rc:
+        _check(rc)
+    return LogProbs(lp, lse, ent, ids, top)
 
 
 def logprobs_backward(queries, rows, targets, lse, entropy=None, *, d_logprob=None, d_lse=None,
@@ -1026,29 +1047,29 @@ def logprobs_backward(queries, rows, targets, lse, entropy=None, *, d_logprob=No
     """(d_queries, d_rows) of a loss from its gradients with respect to what
     logprobs returned; lse and entropy are that call's (fdb_logprobs_backward
     in forgegpu.h).  A gradient that is not needed is None."""
-    a = LogprobGradArgs()
-    torch = _softmax_args(a, queries, rows, targets, scale, allowed)
-    f32 = torch.float32
-    a.lse = _vector(lse, a.nq, f32, queries, "lse")
-    a.entropy = _vector(entropy, a.nq, f32, queries, "entropy")
-    a.d_logprob = _vector(d_logprob, a.nq, f32, queries, "d_logprob")
-    a.d_lse = _vector(d_lse, a.nq, f32, queries, "d_lse")
-    a.d_entropy = _vector(d_entropy, a.nq, f32, queries, "d_entropy")
-    ctx = _ctx_of(queries.device)
+    torch = _torch()
+    head = _softmax_args(queries, rows, targets, scale, allowed)
+    dev, f32 = queries.device, torch.float32
+    nq, n, dim = head[2], head[5], head[7]
+    ctx = _ctx_of(dev)
     L = lib()
-    need = _sz()
-    _check(L.fdb_logprobs_backward_workspace(ctx.h, C.byref(a), C.byref(need)))
-    dev = queries.device
-    dq = torch.empty((a.nq, a.dim), dtype=queries.dtype, device=dev) if need_queries else None
-    dx = torch.empty((a.n, a.dim), dtype=queries.dtype, device=dev) if need_rows else None
-    ws = workspace if workspace is not None else torch.empty(need.value, dtype=torch.uint8,
-                                                             device=dev)
-    if dq is not None:
-        a.d_queries, a.ld_d_queries = dq.data_ptr(), a.dim
-    if dx is not None:
-        a.d_rows, a.ld_d_rows = dx.data_ptr(), a.dim
-    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-    _check(L.fdb_logprobs_backward(ctx.h, C.byref(a)))
+    dq = torch.empty((nq, dim), dtype=queries.dtype, device=dev) if need_queries else None
+    dx = torch.empty((n, dim), dtype=queries.dtype, device=dev) if need_rows else None
+    a = LogprobGradArgs(*head, _vector(lse, nq, f32, dev, "lse"),
+                        _vector(entropy, nq, f32, dev, "entropy"),
+                        _vector(d_logprob, nq, f32, dev, "d_logprob"),
+                        _vector(d_lse, nq, f32, dev, "d_lse"),
+                        _vector(d_entropy, nq, f32, dev, "d_entropy"),
+                        None if dq is None else dq.data_ptr(), dim,
+                        None if dx is None else dx.data_ptr(), dim)
+    key = (dev.index, allowed is not None and head[11]) + head[0:1] + head[2:4] + head[5:8]
+    ws, a.workspace_bytes = _workspace(torch, ctx, L.fdb_logprobs_backward_workspace, a, key, dev,
+                                       workspace)
+    a.workspace = ws.data_ptr()
+    a.stream = torch._C._cuda_getCurrentRawStream(dev.index)
+    rc = L.fdb_logprobs_backward(ctx.h, C.byref(a))
+    if rc:
+        _check(rc)
     return dq, dx
 
 
@@ -1057,8 +1078,9 @@ def logprobs_status(workspace):
     ran out (waits for the current stream)."""
     torch = _torch()
     ctx = _ctx_of(workspace.device)
-    _check(lib().fdb_logprobs_status(ctx.h, workspace.data_ptr(),
-                                     torch.cuda.current_stream(workspace.device).cuda_stream))
+    _check(lib().fdb_logprobs_status(
+        ctx.h, workspace.data_ptr(),
+        torch._C._cuda_getCurrentRawStream(workspace.device.index)))
 
 
 def _scalar(t, dtype, like, what: str):
@@ -1092,21 +1114,24 @@ def adamw_step(params, grads, m, v, *, lr: float, step: int = 1, betas=(0.9, 0.9
                                     if eight else [torch.float32, torch.float32])
     sizes = [t.numel() for t in params]
     blocks = [(n + 255) // 256 for n in sizes] if eight else None
+    cols = []
     for what, (ts, dtype) in enumerate(zip(lists, types)):
+        ptrs = []
         for t, n in zip(ts, sizes if what < 4 else blocks):
             if t.dtype != dtype or t.device != dev or t.numel() != n or not t.is_contiguous():
                 _refuse("params, grads and states must be contiguous, of one type each, of the "
                         "params' sizes (scales: one per 256 elements) and device")
-    table = np.zeros((count, 7), np.uint64)
-    for col, ts in enumerate(lists):
-        table[:, col] = [t.data_ptr() for t in ts]
-    table[:, 6] = sizes
+            ptrs.append(t.data_ptr())
+        cols.append(ptrs)
+    if not eight:
+        cols += [[0] * count] * 2
+    table = np.array(cols + [sizes], np.uint64).T.copy()
     o = AdamwOpts(_DTYPE[p0.dtype], _DTYPE[g0.dtype], 8 if eight else 32, seed & 0xFFFFFFFF, lr,
                   betas[0], betas[1], eps, weight_decay, grad_scale, step,
                   _scalar(d_lr, torch.float32, p0, "d_lr"),
                   _scalar(d_step, torch.int64, p0, "d_step"),
                   _scalar(d_grad_scale, torch.float32, p0, "d_grad_scale"),
-                  torch.cuda.current_stream(dev).cuda_stream)
+                  torch._C._cuda_getCurrentRawStream(dev.index))
     _check(lib().fdb_adamw_step(_ctx_of(dev).h, table.ctypes.data, count, C.byref(o)))
 
 
@@ -1125,5 +1150,5 @@ def adamw_state_values(m, m_scale, v, v_scale):
     ov = torch.empty(m.shape, dtype=torch.float32, device=m.device)
     _check(lib().fdb_adamw_state_values(
         _ctx_of(m.device).h, m.data_ptr(), m_scale.data_ptr(), v.data_ptr(), v_scale.data_ptr(), n,
-        om.data_ptr(), ov.data_ptr(), torch.cuda.current_stream(m.device).cuda_stream))
+        om.data_ptr(), ov.data_ptr(), torch._C._cuda_getCurrentRawStream(m.device.index)))
     return om, ov

@@ -89,7 +89,9 @@ def test_workspace_sizes_follow_the_work(call):
     assert 0 < small < large
     # a 16-bit operand that a tensor map can describe is not copied
     assert _bytes(fg, L, ctx, dtype=2, nq=64, n=100000)[1] < 8 << 20
-    assert _bytes(fg, L, ctx, dtype=2, nq=64, n=100000, ld_rows=9)[1] > 100000 * 64 * 2
+    plain = _bytes(fg, L, ctx, dtype=2, nq=64, n=100000)[1]
+    copied = _bytes(fg, L, ctx, dtype=2, nq=64, n=100000, ld_rows=9)[1]
+    assert copied >= plain + 100000 * 8 * 2
 
 
 OPTS = dict(param_dtype=0, grad_dtype=0, state_bits=32, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8,
