@@ -45,24 +45,26 @@ constexpr int PM = 2 * BM;                  // ... of the pair of blocks that sh
 constexpr int OPER = BM * 128;              // bytes of 128 rows of a 64-wide K step
 // Two blocks work on a tile as a pair (cta_group::2): each holds its 128 rows
 // of A and half of the columns' rows of B, so an operand byte is fetched and
-// read from shared memory half as often for B.  16-bit operands: 256 columns
-// an accumulator, six K steps of 32 KB a block in flight.  Two parts (f32):
-// 128 columns, four K steps of 48 KB (both parts of both operands).  GRAD has
-// one stage less of either: its output is staged in shared memory too.
-__host__ __device__ constexpr int bn_of(bool two) { return two ? 128 : 256; }
-__host__ __device__ constexpr int stages_of(bool two, bool grad) {
-    return (two ? 4 : 6) - (grad ? 1 : 0);
+// read from shared memory half as often for B.  Whole sums: 256 columns an
+// accumulator, six K steps of 32 KB a block in flight.  Sums in blocks (see
+// rows_kernel): 128 columns; two parts (f32) have four K steps of 48 KB (both
+// parts of both operands), one part eight of 24 KB.  GRAD has one stage less
+// of either: its output is staged in shared memory too.
+__host__ __device__ constexpr int bn_of(bool blk) { return blk ? 128 : 256; }
+__host__ __device__ constexpr int stages_of(bool two, bool blk, bool grad) {
+    return (two ? 4 : blk ? 8 : 6) - (grad ? 1 : 0);
 }
+__host__ __device__ constexpr int stage_bytes(bool two, bool blk) {
+    return (two ? 2 : 1) * (OPER + bn_of(blk) / 2 * 128);
+}
+__host__ __device__ constexpr int accs_of(bool blk) { return blk ? 4 : 2; }
 constexpr int STAGED = 32 * 64;             // one warp's 32 x 32 fp16 outputs
 __host__ __device__ constexpr int staged_of(bool two, bool grad) {
     return grad ? 16 * (two ? 2 : 1) * STAGED : 0;
 }
-__host__ __device__ constexpr int stage_bytes(bool two) {
-    return (two ? 2 : 1) * (OPER + bn_of(two) / 2 * 128);
-}
-__host__ __device__ constexpr int accs_of(bool two) { return two ? 4 : 2; }
 constexpr int MAX_STG = 8;
-constexpr int KBLOCK = 2;                   // K steps of an accumulator (two parts)
+// K steps of an accumulator, sums in blocks
+__host__ __device__ constexpr int kblock_of(bool two) { return two ? 2 : 4; }
 constexpr int MAX_BN = 256;
 constexpr unsigned long long DRAIN_CYCLES = 4000000ull;  // about 2 ms
 constexpr int THREADS = 640;                // 2 issuing warps, 2 idle, 16 epilogue warps
@@ -548,7 +550,7 @@ struct Columns {
 // The epilogues: one object per thread and unit; `chunk` takes 32 columns of
 // the thread's row, from column `col` of the unit's matrix (chunk h of the
 // thread's columns of the tile), in registers.
-template <bool TWO>
+template <bool TWO, bool BLK>
 struct StatsEpilogue {
     typedef StatsArgs Args;
     const StatsArgs& p;
@@ -556,7 +558,7 @@ struct StatsEpilogue {
     float rf;
     Run r;
     bool live;
-    Columns<TWO, TWO, TWO ? 1 : 2> c;
+    Columns<TWO, TWO, BLK ? 1 : 2> c;
     const uint32_t* al;
     float top_max;  // largest group's score of the unit (unmarked)
     __device__ StatsEpilogue(const StatsArgs& a, int row, int row0, int, float* fac,
@@ -584,7 +586,7 @@ struct StatsEpilogue {
     // are not free.
     template <int SEEN>
     __device__ __forceinline__ float2 fold(const float (&u)[32], uint32_t w, int h) {
-        constexpr int BIAS_AT = 32 * (TWO ? 1 : 2);
+        constexpr int BIAS_AT = 32 * (BLK ? 1 : 2);
         const float4* bias = reinterpret_cast<const float4*>(c.fac + BIAS_AT + 32 * h);
         const float4* fac = reinterpret_cast<const float4*>(c.fac);
         const uint64_t rf2 = packf(rf, rf), nm2 = packf(-r.m, -r.m);
@@ -851,22 +853,22 @@ struct ProdEpilogue {
     }
     __device__ __forceinline__ void finish(int, int) {}
 };
-template <int MODE, bool TWO>
+template <int MODE, bool TWO, bool BLK>
 struct EpilogueOf;
-template <bool TWO>
-struct EpilogueOf<STATS, TWO> {
-    typedef StatsEpilogue<TWO> Type;
+template <bool TWO, bool BLK>
+struct EpilogueOf<STATS, TWO, BLK> {
+    typedef StatsEpilogue<TWO, BLK> Type;
 };
 template <bool TWO>
-struct EpilogueOf<GRAD, TWO> {
+struct EpilogueOf<GRAD, TWO, TWO> {
     typedef GradEpilogue<TWO> Type;
 };
 template <bool TWO>
-struct EpilogueOf<PROD_Q, TWO> {
+struct EpilogueOf<PROD_Q, TWO, TWO> {
     typedef ProdEpilogue Type;
 };
 template <bool TWO>
-struct EpilogueOf<PROD_X, TWO> {
+struct EpilogueOf<PROD_X, TWO, TWO> {
     typedef ProdEpilogue Type;
 };
 
@@ -914,19 +916,23 @@ __device__ __forceinline__ Unit unit_of(const Mma& g, int u) {
 // finished accumulator; warp 1 of the first block issues the MMAs of both.
 // Persistent: a pair takes units blockIdx.x / 2, + gridDim.x / 2, ...
 //
-// One part: an accumulator is a whole tile (all of K).  TWO parts: it is 128
-// of K, first the products lo.hi and hi.lo, then hi.hi, and the epilogue adds
-// them up in registers: the tensor core's own additions cut the sum towards
-// zero, which at dim 512 cost 8e-7 of a score (all of K in one accumulator).
-template <int MODE, bool TWO>
+// The tensor core's own additions cut a sum towards zero, once for 16 of K:
+// measured on one row, a score comes out short by 4e-8 of itself for each 32
+// of K (bf16; f16, whose products have more bits to cut, up to 1.3e-7).  Where
+// that matters (f32, and long rows) sums are taken in blocks (BLK): an
+// accumulator holds 128 of K (TWO parts: first the products lo.hi and hi.lo,
+// then hi.hi) or 256, and the epilogue adds them up in registers.  Else an
+// accumulator is a whole tile.
+template <int MODE, bool TWO, bool BLK>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     rows_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
                 const __grid_constant__ CUtensorMap omap, const Mma g,
-                const typename EpilogueOf<MODE, TWO>::Type::Args p) {
+                const typename EpilogueOf<MODE, TWO, BLK>::Type::Args p) {
     constexpr bool PROD = MODE == PROD_Q || MODE == PROD_X;
     constexpr bool A_MN = MODE == PROD_X, B_MN = PROD;
-    constexpr int BN = bn_of(TWO), NST = stages_of(TWO, MODE == GRAD), NACC = accs_of(TWO);
-    constexpr int STAGE = stage_bytes(TWO), PARTS = TWO ? 2 : 1;
+    constexpr int BN = bn_of(BLK), NST = stages_of(TWO, BLK, MODE == GRAD), NACC = accs_of(BLK);
+    constexpr int STAGE = stage_bytes(TWO, BLK), PARTS = TWO ? 2 : 1;
+    constexpr int KBLOCK = kblock_of(TWO);
     constexpr int B0 = PARTS * OPER;               // operand B in a stage
     constexpr int B_PART = BN / 2 * 128;           // bytes of one part of this block's half
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -1057,9 +1063,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     const int bn = PROD ? (min(BN, g.ncols - t * BN) + 31) & ~31 : BN;
                     const uint32_t idesc = g.idesc | ((uint32_t)(bn >> 3) << 17);
                     for (int a = x.a0; ok && a < x.a1;) {
-                        // an accumulator: KBLOCK steps (two parts), or all
+                        // an accumulator: KBLOCK steps, or all
                         const int b = ti % NACC;
-                        const int a1 = TWO ? min(x.a1, a + KBLOCK) : x.a1;
+                        const int a1 = BLK ? min(x.a1, a + KBLOCK) : x.a1;
                         const uint32_t d = tmem + (uint32_t)(b * BN);
                         if (ti >= NACC &&
                             !warp_wait(t_empty + b, (ti / NACC - 1) & 1, g.err, g.wait)) {
@@ -1153,7 +1159,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         for (int u = pair; ok && u < units; u += pairs) {
             const Unit x = unit_of<MODE>(g, u);
             const int row0 = x.mt * PM + rank * BM + quad * 32;
-            typename EpilogueOf<MODE, TWO>::Type epi(
+            typename EpilogueOf<MODE, TWO, BLK>::Type epi(
                 p, row0 + lane, row0, x.sp, factors + w * 128,
                 staged + (MODE == GRAD ? w * PARTS * STAGED : 0), &omap);
             epi.load(x.t0 * BN + part * (BN / 4));
@@ -1162,7 +1168,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 epi.c.ready();
                 if (t + 1 < x.t1) epi.load(col + BN);
                 float v[32];
-                if (TWO) {
+                if (BLK) {
                     if (!next()) {
                         ok = false;
                         break;
@@ -1222,26 +1228,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 }
 
 // ---------------------------------------------------------------------------
-// a few f32 queries: one pass over the rows on the FMA pipes
+// a few queries: one pass over the rows on the FMA pipes
 // ---------------------------------------------------------------------------
-// A warp takes groups of 32 rows, 8 at a time: each lane multiplies its
-// columns of 8 rows with its columns of NQ queries (from shared memory), and
-// a transposing reduction leaves each row's sums in four lanes, of which one
-// keeps them, so that after four batches every lane holds one row of the
-// group.  Bound by memory (each row read once) up to about 8 queries.
-template <int NQ, bool VEC>
+// A warp takes groups of 32 rows, RB at a time: each lane multiplies its
+// columns of RB rows with its columns of NQ queries (from shared memory, two
+// products an instruction), and a transposing reduction leaves each row's sums
+// in 32 / RB lanes, of which one keeps them, so that after all batches every
+// lane holds one row of the group.  Bound by memory (each row read once) up to
+// about 8 queries; the tensor cores would work on 256 rows of queries.
+template <typename T, int NQ, bool VEC>
 __global__ void __launch_bounds__(64)
-    few_kernel(const float* __restrict__ x, size_t ld, int n, int d, const float* __restrict__ q,
+    few_kernel(const T* __restrict__ x, size_t ld, int n, int d, const T* __restrict__ q,
                size_t ldq, int q0, int nq, float rf, const uint32_t* __restrict__ allowed,
                size_t ld_allowed, float4* __restrict__ part, float2* __restrict__ top,
                size_t groups, int* __restrict__ err) {
     if (blockIdx.x == 0 && threadIdx.x == 0) *err = 0;  // (this path has no waits)
+    constexpr int V = 16 / (int)sizeof(T);
+    constexpr int RB = 8;
+    constexpr bool PAIRS = NQ < 8;  // (two sums for each would not fit the registers)
     extern __shared__ float4 qs4[];
     float* qs = reinterpret_cast<float*>(qs4);  // [NQ][dp]
     const int dp = (d + 127) & ~127;
     for (int i = threadIdx.x; i < NQ * dp; i += 64) {
         const int j = i / dp, c = i - j * dp;
-        qs[i] = j < nq && c < d ? q[(size_t)(q0 + j) * ldq + c] : 0.0f;
+        qs[i] = j < nq && c < d ? to_f32<T>(q[(size_t)(q0 + j) * ldq + c]) : 0.0f;
     }
     __syncthreads();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -1257,68 +1267,103 @@ __global__ void __launch_bounds__(64)
 #pragma unroll
         for (int j = 0; j < NQ; ++j) sc[j] = 0.0f;
 #pragma unroll 1
-        for (int b = 0; b < 4; ++b) {
-            const int r0 = grp * GROUP + b * 8;
-            float acc[NQ][8];
+        for (int b = 0; b < 32 / RB; ++b) {
+            const int r0 = grp * GROUP + b * RB;
+            uint64_t acc2[PAIRS ? NQ : 1][RB];  // sums of the even and of the odd columns
+            float acc[NQ][RB];
 #pragma unroll
             for (int j = 0; j < NQ; ++j)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) acc[j][i] = 0.0f;
-            const float* row[8];
+                for (int i = 0; i < RB; ++i) {
+                    acc[j][i] = 0.0f;
+                    if (PAIRS) acc2[j][i] = 0ull;
+                }
+            const T* row[RB];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) row[i] = x + (size_t)min(r0 + i, n - 1) * ld;
+            for (int i = 0; i < RB; ++i) row[i] = x + (size_t)min(r0 + i, n - 1) * ld;
             if (VEC) {
-                for (int c = lane * 4; c < d; c += 128) {
-                    float4 xv[8];
+                for (int c = lane * V; c < d; c += 32 * V) {
+                    uint4 xv[RB];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        xv[i] = __ldg(reinterpret_cast<const float4*>(row[i] + c));
+                    for (int i = 0; i < RB; ++i)
+                        xv[i] = __ldg(reinterpret_cast<const uint4*>(row[i] + c));
 #pragma unroll
-                    for (int j = 0; j < NQ; ++j) {
-                        const float4 qv = *reinterpret_cast<const float4*>(qs + j * dp + c);
+                    for (int h = 0; h < V; h += 4) {  // four columns at a time
+                        uint64_t x01[RB], x23[RB];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            acc[j][i] = __fmaf_rn(xv[i].x, qv.x, acc[j][i]);
-                            acc[j][i] = __fmaf_rn(xv[i].y, qv.y, acc[j][i]);
-                            acc[j][i] = __fmaf_rn(xv[i].z, qv.z, acc[j][i]);
-                            acc[j][i] = __fmaf_rn(xv[i].w, qv.w, acc[j][i]);
+                        for (int i = 0; i < RB; ++i) {
+                            const T* e = reinterpret_cast<const T*>(&xv[i]) + h;
+                            x01[i] = packf(to_f32<T>(e[0]), to_f32<T>(e[1]));
+                            x23[i] = packf(to_f32<T>(e[2]), to_f32<T>(e[3]));
+                        }
+#pragma unroll
+                        for (int j = 0; j < NQ; ++j) {
+                            const float4 qv =
+                                *reinterpret_cast<const float4*>(qs + j * dp + c + h);
+                            const uint64_t q01 = packf(qv.x, qv.y), q23 = packf(qv.z, qv.w);
+#pragma unroll
+                            for (int i = 0; i < RB; ++i) {
+                                if (PAIRS) {
+                                    acc2[j][i] = fma2(x01[i], q01, acc2[j][i]);
+                                    acc2[j][i] = fma2(x23[i], q23, acc2[j][i]);
+                                } else {
+                                    float a = acc[j][i];
+                                    a = __fmaf_rn(lo_of(x01[i]), qv.x, a);
+                                    a = __fmaf_rn(hi_of(x01[i]), qv.y, a);
+                                    a = __fmaf_rn(lo_of(x23[i]), qv.z, a);
+                                    acc[j][i] = __fmaf_rn(hi_of(x23[i]), qv.w, a);
+                                }
+                            }
                         }
                     }
                 }
             } else {
-                for (int c = lane; c < d; c += 32) {
-                    float xv[8];
+                for (int c = lane; c < d; c += 64) {  // columns c and c + 32
+                    const bool two = c + 32 < d;
+                    uint64_t xv[RB];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) xv[i] = __ldg(row[i] + c);
+                    for (int i = 0; i < RB; ++i)
+                        xv[i] = packf(to_f32<T>(row[i][c]), two ? to_f32<T>(row[i][c + 32]) : 0.0f);
 #pragma unroll
                     for (int j = 0; j < NQ; ++j) {
-                        const float qv = qs[j * dp + c];
+                        const float* qj = qs + j * dp + c;
+                        const float qa = qj[0], qb = two ? qj[32] : 0.0f;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) acc[j][i] = __fmaf_rn(xv[i], qv, acc[j][i]);
+                        for (int i = 0; i < RB; ++i) {
+                            if (PAIRS) acc2[j][i] = fma2(xv[i], packf(qa, qb), acc2[j][i]);
+                            else
+                                acc[j][i] = __fmaf_rn(hi_of(xv[i]), qb,
+                                                      __fmaf_rn(lo_of(xv[i]), qa, acc[j][i]));
+                        }
                     }
                 }
             }
+            if (PAIRS) {
+#pragma unroll
+                for (int j = 0; j < NQ; ++j)
+#pragma unroll
+                    for (int i = 0; i < RB; ++i) acc[j][i] = lo_of(acc2[j][i]) + hi_of(acc2[j][i]);
+            }
 #pragma unroll
             for (int j = 0; j < NQ; ++j) {
-                float t4[4], t2[2], t1;
+                // halves of the rows are exchanged while more than one is left
+                float t[RB];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float keep = lane & 16 ? acc[j][i + 4] : acc[j][i];
-                    const float give = lane & 16 ? acc[j][i] : acc[j][i + 4];
-                    t4[i] = keep + __shfl_xor_sync(0xffffffffu, give, 16);
-                }
+                for (int i = 0; i < RB; ++i) t[i] = acc[j][i];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float keep = lane & 8 ? t4[i + 2] : t4[i];
-                    const float give = lane & 8 ? t4[i] : t4[i + 2];
-                    t2[i] = keep + __shfl_xor_sync(0xffffffffu, give, 8);
+                for (int o = 16, m = RB / 2; o; o >>= 1, m >>= 1) {
+                    if (m > 0) {
+#pragma unroll
+                        for (int i = 0; i < m; ++i) {
+                            const float keep = lane & o ? t[i + m] : t[i];
+                            const float give = lane & o ? t[i] : t[i + m];
+                            t[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+                        }
+                    } else {
+                        t[0] += __shfl_xor_sync(0xffffffffu, t[0], o);
+                    }
                 }
-                const float keep = lane & 4 ? t2[1] : t2[0];
-                const float give = lane & 4 ? t2[0] : t2[1];
-                t1 = keep + __shfl_xor_sync(0xffffffffu, give, 4);
-                t1 += __shfl_xor_sync(0xffffffffu, t1, 2);
-                t1 += __shfl_xor_sync(0xffffffffu, t1, 1);
-                if ((lane & 3) == b) sc[j] = t1;
+                if ((lane & (32 / RB - 1)) == b) sc[j] = t[0];
             }
         }
 #pragma unroll
@@ -1422,30 +1467,29 @@ __device__ __forceinline__ double unordered64(uint64_t u) {
     return __longlong_as_double((long long)(u >> 63 ? u & 0x7fffffffffffffffull : ~u));
 }
 
-// q . x of ROWS rows in 64 bits over `lanes` lanes (a power of two): each
-// product exact (f32: of 64-bit copies of q) or exact in f32 (16-bit types),
-// added in 64 bits.
+// q . x of ROWS rows in 64 bits over `lanes` lanes (a power of two).  f32:
+// products and sums in 64 bits (of a 64-bit copy of q); 16-bit types: the
+// products are exact in f32, the sums in 64 bits.
 template <typename T>
 struct Exact {
     typedef float Q;
+    double s = 0.0;
+    __device__ __forceinline__ void add(float x, float q) { s += (double)__fmul_rn(x, q); }
+    __device__ __forceinline__ double sum() const { return s; }
 };
 template <>
 struct Exact<float> {
     typedef double Q;
+    double s = 0.0;
+    __device__ __forceinline__ void add(float x, double q) { s = fma((double)x, q, s); }
+    __device__ __forceinline__ double sum() const { return s; }
 };
-__device__ __forceinline__ double add_product(float x, double q, double s) {
-    return fma((double)x, q, s);
-}
-__device__ __forceinline__ double add_product(float x, float q, double s) {
-    return s + (double)__fmul_rn(x, q);
-}
 template <int ROWS, typename T>
 __device__ __forceinline__ void dot_lanes(const T* const (&x)[ROWS],
                                           const typename Exact<T>::Q* q, int d, int sub, int lanes,
                                           bool wide, double (&s)[ROWS]) {
     constexpr int V = 16 / (int)sizeof(T);
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r) s[r] = 0.0;
+    Exact<T> acc[ROWS][2];
     if (wide) {
         int c = sub * V;
         for (; c + V <= d; c += lanes * V) {
@@ -1455,27 +1499,25 @@ __device__ __forceinline__ void dot_lanes(const T* const (&x)[ROWS],
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
                 const T* e = reinterpret_cast<const T*>(&raw[r]);
-                double a = 0.0, b = 0.0;
 #pragma unroll
-                for (int i = 0; i < V; i += 2) {
-                    a = add_product(to_f32<T>(e[i]), q[c + i], a);
-                    b = add_product(to_f32<T>(e[i + 1]), q[c + i + 1], b);
-                }
-                s[r] += a + b;
+                for (int i = 0; i < V; ++i) acc[r][i & 1].add(to_f32<T>(e[i]), q[c + i]);
             }
         }
         for (; c < d; ++c) {  // (the row's last, partial vector: one lane's)
 #pragma unroll
-            for (int r = 0; r < ROWS; ++r) s[r] = add_product(to_f32<T>(x[r][c]), q[c], s[r]);
+            for (int r = 0; r < ROWS; ++r) acc[r][0].add(to_f32<T>(x[r][c]), q[c]);
         }
     } else {
+#pragma unroll 4
         for (int c = sub; c < d; c += lanes)
 #pragma unroll
-            for (int r = 0; r < ROWS; ++r) s[r] = add_product(to_f32<T>(x[r][c]), q[c], s[r]);
+            for (int r = 0; r < ROWS; ++r) acc[r][0].add(to_f32<T>(x[r][c]), q[c]);
     }
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r)
+    for (int r = 0; r < ROWS; ++r) {
+        s[r] = acc[r][0].sum() + acc[r][1].sum();
         for (int o = lanes >> 1; o; o >>= 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], o);
+    }
 }
 
 // One block per query: the partial triples joined, the groups that may hold
@@ -1485,7 +1527,7 @@ __device__ __forceinline__ void dot_lanes(const T* const (&x)[ROWS],
 // is a bound that at least k + 8 groups reach, and for scores in no particular
 // order hardly more do; only the groups of the parts that reach it are read.
 template <typename T, int THREADS_>
-__global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
+__global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kernel(const FinishArgs p) {
     constexpr int W = THREADS_ / 32;
     extern __shared__ double qs_raw[];
     typename Exact<T>::Q* qs = reinterpret_cast<typename Exact<T>::Q*>(qs_raw);  // [dim]
@@ -1821,7 +1863,7 @@ __global__ void __launch_bounds__(THREADS_) finish_kernel(const FinishArgs p) {
     }
     // ---- written in order ----
     int have = bad ? 0 : s_cnt;
-    if (have > 128 && s_kth > -INFINITY) have = narrow(have, ordered64(s_kth));
+    if (have > 128) have = narrow(have, least_of(have));
     rank_all(have, [&](int i, int rank) {
         if (rank < p.k) {
             p.top_ids[(size_t)q * p.k + rank] = (int64_t)ci[i];
@@ -2063,12 +2105,17 @@ __global__ void void_kernel(const int* err, void* dq, size_t ldq, int nq, void* 
 // ---------------------------------------------------------------------------
 constexpr size_t HEAD = 256;                    // error word, bounds
 constexpr size_t CHUNK_BYTES = (size_t)512 << 20;  // of group maxima, of score gradients
-constexpr int FEW = 8;                          // f32 queries a pass of few_kernel takes
-constexpr int FEW_QUERIES = 16, FEW_DIM = 2048;
-static size_t smem_of(bool two, bool grad) {
+// dims above which a score's sum is taken in blocks: 2048 x 131072 x 768 bf16
+// takes 284 us with whole sums, so they stay while the loss is below 1e-6
+constexpr size_t BLOCKS_F16 = 256, BLOCKS_BF16 = 768;
+constexpr int FEW = 8;                          // queries a pass of few_kernel takes
+// f32 rows would have to be split for the tensor cores first: two passes still
+// cost less; 16-bit rows are read by them as they are.
+constexpr int FEW_F32 = 16, FEW_16 = 2, FEW_DIM = 2048;
+static size_t smem_of(bool two, bool blk, bool grad) {
     // alignment, stages, staged outputs, barriers, column factors
-    return 1024 + (size_t)stages_of(two, grad) * stage_bytes(two) + staged_of(two, grad) + 256 +
-           EPI_WARPS * 128 * 4;
+    return 1024 + (size_t)stages_of(two, blk, grad) * stage_bytes(two, blk) +
+           staged_of(two, grad) + 256 + EPI_WARPS * 128 * 4;
 }
 
 static size_t up(size_t v, size_t m) { return (v + m - 1) / m * m; }
@@ -2135,32 +2182,34 @@ static void allow_smem(K* kernel, int device, size_t bytes, std::atomic<uint64_t
     if (device < 64) done.fetch_or(1ull << device, std::memory_order_release);
 }
 
-template <int MODE, bool TWO>
-static void launch_rows(cudaStream_t s, int device, int sms, const CUtensorMap& a, const CUtensorMap& b,
-                        const Mma& g, const typename EpilogueOf<MODE, TWO>::Type::Args& p,
-                        const CUtensorMap* out) {
+template <int MODE, bool TWO, bool BLK>
+static void launch_rows(cudaStream_t s, int device, int sms, const CUtensorMap& a,
+                        const CUtensorMap& b, const Mma& g,
+                        const typename EpilogueOf<MODE, TWO, BLK>::Type::Args& p,
+                        const CUtensorMap* out = nullptr) {
     const long long units = MODE == PROD_Q || MODE == PROD_X
                                 ? (long long)g.mt * g.nt * g.chunks
                                 : (long long)g.mt * g.chunks;
-    const size_t smem = smem_of(TWO, MODE == GRAD);
+    const size_t smem = smem_of(TWO, BLK, MODE == GRAD);
     static std::atomic<uint64_t> done{0};
-    allow_smem(rows_kernel<MODE, TWO>, device, smem, done);
-    rows_kernel<MODE, TWO>
-        <<<2 * (unsigned)std::min<long long>(units, sms / 2), THREADS, smem, s>>>(a, b, out ? *out : a, g, p);
+    allow_smem(rows_kernel<MODE, TWO, BLK>, device, smem, done);
+    rows_kernel<MODE, TWO, BLK>
+        <<<2 * (unsigned)std::min<long long>(units, sms / 2), THREADS, smem, s>>>(
+            a, b, out ? *out : a, g, p);
     FDB_LAUNCH_CHECK();
 }
 // A's K steps stay in shared memory where they fill at most half of the ring
 // (4096 x 262144 x 96 f32: a tile's copies shrink to a third).
-static int stays(bool two, bool grad, int atoms) {
-    return atoms * (two ? 2 : 1) * OPER <= stages_of(two, grad) * stage_bytes(two) / 2;
+static int stays(bool two, bool blk, bool grad, int atoms) {
+    return atoms * (two ? 2 : 1) * OPER <= stages_of(two, blk, grad) * stage_bytes(two, blk) / 2;
 }
 template <int MODE>
 static void launch_rows(bool two, cudaStream_t s, int device, int sms, const CUtensorMap& a,
                         const CUtensorMap& b, const Mma& g,
-                        const typename EpilogueOf<MODE, false>::Type::Args& p,
+                        const typename EpilogueOf<MODE, false, false>::Type::Args& p,
                         const CUtensorMap* out = nullptr) {
-    if (two) launch_rows<MODE, true>(s, device, sms, a, b, g, p, out);
-    else launch_rows<MODE, false>(s, device, sms, a, b, g, p, out);
+    if (two) launch_rows<MODE, true, true>(s, device, sms, a, b, g, p, out);
+    else launch_rows<MODE, false, false>(s, device, sms, a, b, g, p, out);
 }
 
 // Hands out 256-byte aligned parts of the caller's workspace.
@@ -2198,7 +2247,7 @@ static void launch_pack(cudaStream_t s, int dtype, const PackSide& a, const Pack
 
 // The forward pass's workspace and launch shape.
 struct Forward {
-    bool few, packed, copy_q, copy_x;
+    bool few, packed, blocks, copy_q, copy_x;
     size_t kp, qb, groups, parts_cap;
     int bn, nt;
     size_t bytes;
@@ -2215,10 +2264,12 @@ static Forward plan_forward(const Ctx& c, const fdb_logprob_args& a) {
     Forward w{};
     Carve ws(a.workspace);
     w.err = ws.take<int>(HEAD / 4);
-    w.few = a.dtype == FDB_DTYPE_F32 && a.nq <= FEW_QUERIES && a.dim <= FEW_DIM;
+    w.few = a.nq <= (a.dtype == FDB_DTYPE_F32 ? FEW_F32 : FEW_16) && a.dim <= FEW_DIM;
     w.packed = a.dtype == FDB_DTYPE_F32 && !w.few;
     w.kp = up(a.dim, 16);
-    w.bn = bn_of(w.packed);
+    // (16-bit rows: sums in blocks where whole ones would lose over 1e-6 of a score)
+    w.blocks = w.packed || a.dim > (a.dtype == FDB_DTYPE_F16 ? BLOCKS_F16 : BLOCKS_BF16);
+    w.bn = bn_of(w.blocks);
     w.nt = (int)((a.n + w.bn - 1) / w.bn);
     w.groups = w.few ? (a.n + GROUP - 1) / GROUP : (size_t)w.nt * (w.bn / GROUP);
     const size_t per = a.k ? w.groups * sizeof(float2) : 0;
@@ -2275,6 +2326,53 @@ static void launch_finish(cudaStream_t s, int device, const FinishArgs& f) {
     else launch_finish_t<T, 128>(s, device, f);
 }
 
+static FinishArgs finish_args(const fdb_logprob_args& a, const Forward& w, size_t q0, size_t nq) {
+    FinishArgs f{};
+    f.q = a.queries, f.x = a.rows;
+    f.ldq = a.ld_queries, f.ldx = a.ld_rows;
+    f.q0 = (int)q0, f.nq = (int)nq, f.n = (int)a.n, f.d = (int)a.dim, f.k = (int)a.k;
+    f.scale = a.scale;
+    f.targets = a.targets;
+    f.allowed = a.allowed, f.ld_allowed = a.allowed ? a.ld_allowed : 0;
+    f.part = w.part;
+    f.top = w.top, f.groups = w.groups;
+    f.logprob = a.logprob, f.lse = a.lse, f.entropy = a.entropy;
+    f.top_logprob = a.top_logprobs, f.top_ids = a.top_ids;
+    f.err = w.err;
+    return f;
+}
+
+template <typename T>
+static void few_run(const Ctx& c, const fdb_logprob_args& a, const Forward& w, float rf,
+                    size_t ld_allowed) {
+    const cudaStream_t s = static_cast<cudaStream_t>(a.stream);
+    const bool vec = (reinterpret_cast<uintptr_t>(a.rows) & 15) == 0 &&
+                     a.ld_rows * sizeof(T) % 16 == 0 && a.dim * sizeof(T) % 16 == 0;
+    const size_t dp = up(a.dim, 128);
+    for (size_t q0 = 0; q0 < a.nq; q0 += w.qb) {
+        const int nq = (int)std::min(w.qb, a.nq - q0);
+        const unsigned blocks = (unsigned)w.parts_cap;
+        auto go = [&](auto kernel, int NQ) {
+            const size_t sm = NQ * dp * 4;
+            if (sm > 40960)
+                FDB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                              (int)sm));
+            kernel<<<blocks, 64, sm, s>>>(static_cast<const T*>(a.rows), a.ld_rows, (int)a.n,
+                                          (int)a.dim, static_cast<const T*>(a.queries),
+                                          a.ld_queries, (int)q0, nq, rf, a.allowed, ld_allowed,
+                                          w.part, w.top, w.groups, w.err);
+            FDB_LAUNCH_CHECK();
+        };
+        if (nq == 1) vec ? go(few_kernel<T, 1, true>, 1) : go(few_kernel<T, 1, false>, 1);
+        else if (nq == 2) vec ? go(few_kernel<T, 2, true>, 2) : go(few_kernel<T, 2, false>, 2);
+        else if (nq <= 4) vec ? go(few_kernel<T, 4, true>, 4) : go(few_kernel<T, 4, false>, 4);
+        else vec ? go(few_kernel<T, 8, true>, 8) : go(few_kernel<T, 8, false>, 8);
+        FinishArgs f = finish_args(a, w, q0, nq);
+        f.parts = (int)blocks;
+        launch_finish<T>(s, c.device, f);
+    }
+}
+
 void forward_run(Ctx& c, const fdb_logprob_args& a) {
     const cudaStream_t s = static_cast<cudaStream_t>(a.stream);
     const Forward w = plan_forward(c, a);
@@ -2315,7 +2413,7 @@ void forward_run(Ctx& c, const fdb_logprob_args& a) {
         g.nt = w.nt;
         g.atoms = (int)((w.kp + 63) / 64);
         g.klast = (int)((w.kp - 64 * (size_t)(g.atoms - 1)) / 16);
-        g.resident = stays(w.packed, false, g.atoms);
+        g.resident = stays(w.packed, w.blocks, false, g.atoms);
         g.a_part = g.b_part = (int)w.kp;
         g.idesc = idesc_of(w.packed ? FDB_DTYPE_F16 : a.dtype, false, false);
         g.err = w.err;
@@ -2339,62 +2437,26 @@ void forward_run(Ctx& c, const fdb_logprob_args& a) {
             p.part = w.part;
             p.top = w.top;
             p.groups = w.groups;
-            launch_rows<STATS>(w.packed, s, c.device, c.sm_count, amap, bmap, g, p);
-            FinishArgs f{};
-            f.q = a.queries, f.x = a.rows;
-            f.ldq = a.ld_queries, f.ldx = a.ld_rows;
-            f.q0 = (int)q0, f.nq = (int)nq, f.n = n, f.d = d, f.k = (int)a.k;
-            f.scale = a.scale;
-            f.targets = a.targets;
-            f.allowed = a.allowed, f.ld_allowed = ld_allowed;
-            f.part = w.part, f.parts = g.chunks * 4;
+            if (w.packed)
+                launch_rows<STATS, true, true>(s, c.device, c.sm_count, amap, bmap, g, p);
+            else if (w.blocks)
+                launch_rows<STATS, false, true>(s, c.device, c.sm_count, amap, bmap, g, p);
+            else
+                launch_rows<STATS, false, false>(s, c.device, c.sm_count, amap, bmap, g, p);
+            FinishArgs f = finish_args(a, w, q0, nq);
+            f.parts = g.chunks * 4;
+            f.qf = p.qf;
             f.nt = w.nt, f.chunks = g.chunks;
             f.per_tile = w.bn / GROUP, f.per_part = w.bn / GROUP / 4;
-            f.qf = p.qf;
-            f.top = w.top, f.groups = w.groups;
-            f.logprob = a.logprob, f.lse = a.lse, f.entropy = a.entropy;
-            f.top_logprob = a.top_logprobs, f.top_ids = a.top_ids;
-            f.err = w.err;
             if (a.dtype == FDB_DTYPE_F32) launch_finish<float>(s, c.device, f);
             else if (a.dtype == FDB_DTYPE_F16) launch_finish<__half>(s, c.device, f);
             else launch_finish<__nv_bfloat16>(s, c.device, f);
         }
         return;
     }
-    const bool vec = (reinterpret_cast<uintptr_t>(a.rows) & 15) == 0 && a.ld_rows % 4 == 0 &&
-                     a.dim % 4 == 0;
-    const size_t dp = up(a.dim, 128);
-    for (size_t q0 = 0; q0 < a.nq; q0 += w.qb) {
-        const int nq = (int)std::min(w.qb, a.nq - q0);
-        const unsigned blocks = (unsigned)w.parts_cap;
-        auto go = [&](auto kernel, int NQ) {
-            const size_t sm = NQ * dp * 4;
-            if (sm > 40960)
-                FDB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                              (int)sm));
-            kernel<<<blocks, 64, sm, s>>>(static_cast<const float*>(a.rows), a.ld_rows, n, d,
-                                          static_cast<const float*>(a.queries), a.ld_queries,
-                                          (int)q0, nq, rf, a.allowed, ld_allowed, w.part, w.top,
-                                          w.groups, w.err);
-            FDB_LAUNCH_CHECK();
-        };
-        if (nq == 1) vec ? go(few_kernel<1, true>, 1) : go(few_kernel<1, false>, 1);
-        else if (nq == 2) vec ? go(few_kernel<2, true>, 2) : go(few_kernel<2, false>, 2);
-        else if (nq <= 4) vec ? go(few_kernel<4, true>, 4) : go(few_kernel<4, false>, 4);
-        else vec ? go(few_kernel<8, true>, 8) : go(few_kernel<8, false>, 8);
-        FinishArgs f{};
-        f.q = a.queries, f.x = a.rows;
-        f.ldq = a.ld_queries, f.ldx = a.ld_rows;
-        f.q0 = (int)q0, f.nq = nq, f.n = n, f.d = d, f.k = (int)a.k;
-        f.scale = a.scale;
-        f.targets = a.targets;
-        f.allowed = a.allowed, f.ld_allowed = ld_allowed;
-        f.part = w.part, f.parts = (int)blocks;
-        f.top = w.top, f.groups = w.groups;
-        f.logprob = a.logprob, f.lse = a.lse, f.entropy = a.entropy;
-        f.top_logprob = a.top_logprobs, f.top_ids = a.top_ids;
-        launch_finish<float>(s, c.device, f);
-    }
+    if (a.dtype == FDB_DTYPE_F32) few_run<float>(c, a, w, rf, ld_allowed);
+    else if (a.dtype == FDB_DTYPE_F16) few_run<__half>(c, a, w, rf, ld_allowed);
+    else few_run<__nv_bfloat16>(c, a, w, rf, ld_allowed);
 }
 
 // ---- backward ----
@@ -2508,7 +2570,7 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
             g.chunks = pick_chunks(g.mt, g.nt, c.sm_count);
             g.atoms = (int)((w.kp + 63) / 64);
             g.klast = (int)((w.kp - 64 * (size_t)(g.atoms - 1)) / 16);
-            g.resident = stays(two, true, g.atoms);
+            g.resident = stays(two, two, true, g.atoms);
             g.a_part = g.b_part = (int)w.kp;
             g.b_row0 = (int)j0;
             g.idesc = idesc_of(FDB_DTYPE_F16, false, false);
