@@ -6,15 +6,16 @@
 //   H_i = lse_i - sum_j p_ij s_ij,  logprob_i = s_i,t(i) - lse_i
 //
 // Forward: the scores are formed tile by tile on the tensor cores (or, for a
-// few f32 queries, on the FMA pipes) and every thread folds its columns into
+// few queries, on the FMA pipes) and every thread folds its columns into
 // a running (max m, sum l = sum 2^(t - m), a = sum 2^(t - m) (t - m)) of its
 // query row, t = s log2(e); the partial triples are joined by
 // finish_kernel:  lse = ln2 (M + log2 L),  H = ln2 (log2 L - A / L).
 // For the top alternatives each group of 32 rows leaves its largest score,
 // the pair of rows that holds it (in the low 4 bits) and its second largest;
-// the best k + 8 groups are picked per query, their marked rows are scored
-// again exactly (64-bit sums), and a group whose second largest could still
-// enter is scored in full, as are all groups if one that was not picked could.
+// a little more than the best k groups are picked per query, their marked rows
+// are scored again exactly (64-bit sums), and a group whose second largest
+// could still enter is scored in full, as are all groups if one that was not
+// picked could.
 // Which ids are returned therefore does not depend on the order of a 32-bit
 // sum; equal scores go to the lower id.
 //
@@ -1539,7 +1540,7 @@ __device__ __forceinline__ double unordered64(uint64_t u) {
 
 // q . x of ROWS rows in 64 bits over `lanes` lanes (a power of two).  f32:
 // products and sums in 64 bits (of a 64-bit copy of q); 16-bit types: the
-// products are exact in f32, the sums in 64 bits.
+// products are exact in f32, the sums in 64 bits.  z: the largest element.
 template <typename T>
 struct Exact {
     typedef float Q;
@@ -1554,10 +1555,39 @@ struct Exact<float> {
     __device__ __forceinline__ void add(float x, double q) { s = fma((double)x, q, s); }
     __device__ __forceinline__ double sum() const { return s; }
 };
+__device__ __forceinline__ __half2 pair_twice(__half x) { return __half2half2(x); }
+__device__ __forceinline__ __nv_bfloat162 pair_twice(__nv_bfloat16 x) {
+    return __bfloat162bfloat162(x);
+}
+// The largest size of the elements that a thread has read.
+template <typename T>
+struct Largest {
+    using Pair = decltype(pair_twice(T()));
+    Pair m = pair_twice(T(0.0f));
+    __device__ __forceinline__ void add(const uint4& raw) {
+        const Pair* e = reinterpret_cast<const Pair*>(&raw);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = __hmax2(m, __habs2(e[i]));
+    }
+    __device__ __forceinline__ void add(T x) { m = __hmax2(m, __habs2(pair_twice(x))); }
+    __device__ __forceinline__ float get() const {
+        return fmaxf(to_f32<T>(m.x), to_f32<T>(m.y));
+    }
+};
+template <>
+struct Largest<float> {
+    float m = 0.0f;
+    __device__ __forceinline__ void add(const uint4& raw) {
+        add(__uint_as_float(raw.x)), add(__uint_as_float(raw.y));
+        add(__uint_as_float(raw.z)), add(__uint_as_float(raw.w));
+    }
+    __device__ __forceinline__ void add(float x) { m = fmaxf(m, fabsf(x)); }
+    __device__ __forceinline__ float get() const { return m; }
+};
 template <int ROWS, typename T>
 __device__ __forceinline__ void dot_lanes(const T* const (&x)[ROWS],
                                           const typename Exact<T>::Q* q, int d, int sub, int lanes,
-                                          bool wide, double (&s)[ROWS]) {
+                                          bool wide, double (&s)[ROWS], Largest<T>& z) {
     constexpr int V = 16 / (int)sizeof(T);
     Exact<T> acc[ROWS][2];
     if (wide) {
@@ -1571,17 +1601,24 @@ __device__ __forceinline__ void dot_lanes(const T* const (&x)[ROWS],
                 const T* e = reinterpret_cast<const T*>(&raw[r]);
 #pragma unroll
                 for (int i = 0; i < V; ++i) acc[r][i & 1].add(to_f32<T>(e[i]), q[c + i]);
+                z.add(raw[r]);
             }
         }
         for (; c < d; ++c) {  // (the row's last, partial vector: one lane's)
 #pragma unroll
-            for (int r = 0; r < ROWS; ++r) acc[r][0].add(to_f32<T>(x[r][c]), q[c]);
+            for (int r = 0; r < ROWS; ++r) {
+                acc[r][0].add(to_f32<T>(x[r][c]), q[c]);
+                z.add(x[r][c]);
+            }
         }
     } else {
 #pragma unroll 4
         for (int c = sub; c < d; c += lanes)
 #pragma unroll
-            for (int r = 0; r < ROWS; ++r) acc[r][0].add(to_f32<T>(x[r][c]), q[c]);
+            for (int r = 0; r < ROWS; ++r) {
+                acc[r][0].add(to_f32<T>(x[r][c]), q[c]);
+                z.add(x[r][c]);
+            }
     }
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
@@ -1612,6 +1649,8 @@ __global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kern
     __shared__ uint64_t cs[CAND + 1];  // exact scores, as ordered64
     __shared__ uint32_t ci[CAND + 1];
     __shared__ double s_kth;
+    __shared__ int s_size;        // bits of the candidates' largest element
+    __shared__ float s_qsize[W];  // parts of |q|^2
     __shared__ uint64_t kept[KEPT];
     __shared__ uint32_t kept_id[KEPT];
     __shared__ uint64_t set_max[128];
@@ -1631,7 +1670,12 @@ __global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kern
     const int64_t target = p.targets ? p.targets[q] : -1;
     const bool given = target >= 0 && target < p.n;
     if (tid == 0) s_picked = s_cnt = s_parts = 0, s_kth = -INFINITY;
-    for (int c = tid; c < p.d; c += THREADS_) qs[c] = to_f32<T>(qp[c]);
+    float qq = 0.0f;
+    for (int c = tid; c < p.d; c += THREADS_) {
+        const float v = to_f32<T>(qp[c]);
+        qs[c] = v;
+        qq = __fmaf_rn(v, v, qq);
+    }
 
     // ---- the largest reference, and the largest scores of 128 sets of parts ----
     float M = -INFINITY, gm = NONE;
@@ -1650,7 +1694,10 @@ __global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kern
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    if (lane == 0) redf[warp] = M;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) qq += __shfl_xor_sync(0xffffffffu, qq, o);
+    if (lane == 0) redf[warp] = M, s_qsize[warp] = qq;
+    if (tid == 0) s_size = 0;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < W; ++i) M = fmaxf(M, redf[i]);
@@ -1707,6 +1754,7 @@ __global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kern
     const int sub = lane & (lanes - 1);
     auto score = [&](int from, int to) {
         constexpr int ROWS = 4;
+        Largest<T> largest;
         const int per = THREADS_ / lanes;
         for (int i = from; i < to; i += ROWS * per) {
             const T* x[ROWS];
@@ -1716,12 +1764,16 @@ __global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kern
                 const int j = i + r * per + tid / lanes;
                 x[r] = xp + (size_t)ci[j < to ? j : from] * p.ldx;
             }
-            dot_lanes<ROWS, T>(x, qs, p.d, sub, lanes, wide, v);
+            dot_lanes<ROWS, T>(x, qs, p.d, sub, lanes, wide, v, largest);
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
                 const int j = i + r * per + tid / lanes;
                 if (sub == 0 && j < to) cs[j] = ordered64(v[r]);
             }
+        }
+        if (p.k > 0) {
+            const int w = __reduce_max_sync(0xffffffffu, __float_as_int(largest.get()));
+            if (lane == 0) atomicMax(&s_size, w);
         }
     };
     auto seen = [&](uint32_t id) {
@@ -1860,11 +1912,15 @@ __global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kern
         return s_least;
     };
     // Whether a score of at most `m` (as a group left it) may be among the best
-    // k, whose last exact score so far is s_kth: marks and 32-bit sums move it
-    // by far less than 2^-15 of the larger of the two.
+    // k, whose last exact score so far is s_kth: a mark moves it by 2^-19 of
+    // itself, the 32-bit sums by less than 2^-18 of |q| sqrt(d) max |x_c|.
+    qq = 0.0f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) qq += s_qsize[i];
     auto may_enter = [&](double m) {
         const double v = m / unit, kth = s_kth;
-        return v >= kth - ldexp(fabs(v) + fabs(kth), -15);
+        const double size = (double)sqrtf(qq * (float)p.d) * (double)__int_as_float(s_size);
+        return !(v < kth - (fabs(v) + fabs(kth)) * 0x1p-16 - size * 0x1p-18);
     };
     rank_all(cnt, [&](int i, int rank) {
         if (rank == p.k - 1) s_kth = unordered64(cs[i]);
@@ -2436,8 +2492,10 @@ static void few_run(const Ctx& c, const fdb_logprob_args& a, const Forward& w, f
         };
         if (nq == 1) vec ? go(few_kernel<T, 1, true>, 1) : go(few_kernel<T, 1, false>, 1);
         else if (nq == 2) vec ? go(few_kernel<T, 2, true>, 2) : go(few_kernel<T, 2, false>, 2);
-        else if (nq <= 4) vec ? go(few_kernel<T, 4, true>, 4) : go(few_kernel<T, 4, false>, 4);
-        else vec ? go(few_kernel<T, 8, true>, 8) : go(few_kernel<T, 8, false>, 8);
+        else if constexpr (sizeof(T) == 4) {  // (of 16-bit queries at most FEW_16 come here)
+            if (nq <= 4) vec ? go(few_kernel<T, 4, true>, 4) : go(few_kernel<T, 4, false>, 4);
+            else vec ? go(few_kernel<T, 8, true>, 8) : go(few_kernel<T, 8, false>, 8);
+        }
         FinishArgs f = finish_args(a, w, q0, nq);
         f.parts = (int)blocks;
         launch_finish<T>(s, c.device, f);

@@ -266,6 +266,33 @@ def test_scores_that_lie_close_together(dtype, nq):
     assert np.array_equal(r.top_ids.cpu().numpy(), f["top_ids"])
 
 
+@pytest.mark.parametrize("nq", [3, 40, 140])
+@pytest.mark.parametrize("shift", [14, 17])
+def test_scores_that_are_small_beside_their_rows(nq, shift):
+    """Rows almost at right angles to their queries: what the 32-bit scores are
+    off by is of the size of their differences, the order is that of the 64-bit
+    ones."""
+    import forgegpu as fg
+    import torch
+    rng = np.random.default_rng(shift)
+    n, d = 3000, 64
+    q = np.concatenate([np.ones((nq, 1)), rng.standard_normal((nq, d - 1))], 1).astype(np.float32)
+    x = rng.standard_normal((n, d - 1)).astype(np.float32)
+    q[:, 33:] = q[:, 1:32]  # the second half of a row takes the first one's part away
+    q[:, 32] = 1
+    x = np.concatenate([np.zeros((n, 1)), x[:, :31], np.zeros((n, 1)), -x[:, :31]], 1)
+    x[:, 0] = rng.standard_normal(n)
+    x[:, 32] = -x[:, 0] + 2.0 ** -shift * rng.standard_normal(n)
+    Q, X = torch.from_numpy(q).cuda(), torch.from_numpy(x.astype(np.float32)).cuda()
+    r = fg.logprobs(Q, X, k=10)
+    # all but two products of a score take each other away, so it is the exact
+    # sum of those two, a multiple of 2^-24 or so: rows may share one
+    X = X.double().cpu().numpy()
+    s = X[:, 0] + X[:, 32]
+    best = np.sort(s)[::-1][:10]
+    assert (s[r.top_ids.cpu().numpy()] == best).all()
+
+
 @pytest.mark.parametrize("dtype,nq", [("f32", 4), ("f32", 140), ("bf16", 140), ("f16", 20)])
 @pytest.mark.parametrize("bad", BADS[:3])
 def test_what_is_not_finite_reaches_its_queries_only(dtype, nq, bad):
