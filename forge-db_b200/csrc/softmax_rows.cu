@@ -50,10 +50,12 @@ constexpr int OPER = BM * 128;              // bytes of 128 rows of a 64-wide K 
 // accumulator, six K steps of 32 KB a block in flight.  Sums in blocks (see
 // rows_kernel): 128 columns; two parts (f32) have four K steps of 48 KB (both
 // parts of both operands), one part eight of 24 KB.  GRAD has one stage less
-// of either: its output is staged in shared memory too.
+// of either: its output is staged in shared memory too.  Two parts of at most
+// 128 of K are one block anyway: whole sums of 256 columns, three K steps of
+// 64 KB.
 __host__ __device__ constexpr int bn_of(bool blk) { return blk ? 128 : 256; }
 __host__ __device__ constexpr int stages_of(bool two, bool blk, bool grad) {
-    return (two ? 4 : blk ? 8 : 6) - (grad ? 1 : 0);
+    return two && !blk ? 3 : (two ? 4 : blk ? 8 : 6) - (grad ? 1 : 0);
 }
 __host__ __device__ constexpr int stage_bytes(bool two, bool blk) {
     return (two ? 2 : 1) * (OPER + bn_of(blk) / 2 * 128);
@@ -664,7 +666,7 @@ struct StatsEpilogue {
     __device__ __forceinline__ float2 fold(const float (&u)[32], uint32_t w, int h) {
         constexpr int BIAS_AT = 32 * (BLK ? 1 : 2);
         const float4* bias = reinterpret_cast<const float4*>(c.fac + BIAS_AT + 32 * h);
-        const float4* fac = reinterpret_cast<const float4*>(c.fac);
+        const float4* fac = reinterpret_cast<const float4*>(c.fac + 32 * h);
         const uint64_t rf2 = packf(rf, rf), nm2 = packf(-r.m, -r.m);
         float d[32];
 #pragma unroll
@@ -2237,8 +2239,11 @@ __global__ void void_kernel(const int* err, void* dq, size_t ldq, int nq, void* 
 constexpr size_t HEAD = 256;                    // error word, bounds
 constexpr size_t CHUNK_BYTES = (size_t)512 << 20;  // of group maxima, of score gradients
 // dims above which a score's sum is taken in blocks: 2048 x 131072 x 768 bf16
-// takes 284 us with whole sums, so they stay while the loss is below 1e-6
-constexpr size_t BLOCKS_F16 = 256, BLOCKS_BF16 = 768;
+// takes 284 us with whole sums, so they stay while the loss is below 1e-6.
+// Two parts of 128 are one block: 4096 x 262144 x 96 f32 takes 811 us in tiles
+// of 128 columns, 694 in those of 256, whose waits and loads serve twice as
+// many
+constexpr size_t BLOCKS_F32 = 128, BLOCKS_F16 = 256, BLOCKS_BF16 = 768;
 constexpr int FEW = 8;                          // queries a pass of few_kernel takes
 // f32 rows would have to be split for the tensor cores first: two passes still
 // cost less; 16-bit rows are read by them as they are.
@@ -2399,8 +2404,8 @@ static Forward plan_forward(const Ctx& c, const fdb_logprob_args& a) {
     w.few = a.nq <= (a.dtype == FDB_DTYPE_F32 ? FEW_F32 : FEW_16) && a.dim <= FEW_DIM;
     w.packed = a.dtype == FDB_DTYPE_F32 && !w.few;
     w.kp = up(a.dim, 16);
-    // (16-bit rows: sums in blocks where whole ones would lose over 1e-6 of a score)
-    w.blocks = w.packed || a.dim > (a.dtype == FDB_DTYPE_F16 ? BLOCKS_F16 : BLOCKS_BF16);
+    // (sums in blocks where whole ones would lose over 1e-6 of a score)
+    w.blocks = a.dim > (w.packed ? BLOCKS_F32 : a.dtype == FDB_DTYPE_F16 ? BLOCKS_F16 : BLOCKS_BF16);
     w.bn = bn_of(w.blocks);
     w.nt = (int)((a.n + w.bn - 1) / w.bn);
     w.groups = w.few ? (a.n + GROUP - 1) / GROUP : (size_t)w.nt * (w.bn / GROUP);
@@ -2571,7 +2576,9 @@ void forward_run(Ctx& c, const fdb_logprob_args& a) {
             p.part = w.part;
             p.top = w.top;
             p.groups = w.groups;
-            if (w.packed)
+            if (w.packed && !w.blocks)
+                launch_rows<STATS, true, false>(s, c.device, c.sm_count, amap, bmap, g, p);
+            else if (w.packed)
                 launch_rows<STATS, true, true>(s, c.device, c.sm_count, amap, bmap, g, p);
             else if (w.blocks)
                 launch_rows<STATS, false, true>(s, c.device, c.sm_count, amap, bmap, g, p);
