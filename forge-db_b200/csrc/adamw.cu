@@ -14,8 +14,9 @@
 // a code of at least 1: a zero under a moment that is not zero would make the
 // update m / eps.
 //
-// Bound by memory: f32 p, g, m, v move 28 bytes an element, bf16 p, g with
-// 8-bit moments 10.
+// Bound by memory with f32 moments: f32 p, g, m, v move 28 bytes an element
+// (131072 x 768: 419 us, 6.7 TB/s).  bf16 p, g with 8-bit moments move 10, and
+// 147 instructions an element take longer than that (40 M elements: 198 us).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -128,10 +129,6 @@ __device__ __forceinline__ uint32_t mix(uint32_t h) {
 }
 __device__ __forceinline__ float unit(uint32_t h) { return (float)(h >> 8) * 0x1p-24f; }
 
-// floor(sqrt(y)) and floor(y^(1/4)) as the correctly rounded roots give them,
-// y in [0, 256^2) or [0, 256^4): from the approximate root (a relative error
-// of about 2^-22, so its floor is right but next to a whole number), which is
-// replaced by the exact one there.
 // Conversions between small integers and floats go by adding 2^23, whose low
 // mantissa bits then are the integer: a quarter of the cycles of the conversion
 // instructions, of which a code would need ten.
@@ -144,22 +141,6 @@ __device__ __forceinline__ float nearest(float r) {  // 0 <= r < 2^22
     return __fsub_rn(__fadd_rn(r, 8388608.0f), 8388608.0f);
 }
 __device__ __forceinline__ float below(float r, float n) { return r < n ? n - 1.0f : n; }
-__device__ __forceinline__ float root2(float y) {
-    const float r = fast_sqrt(y), n = nearest(r);
-    if (fabsf(r - n) < 0x1p-12f && y > 0.0f) {
-        const float e = __fsqrt_rn(y);
-        return below(e, nearest(e));
-    }
-    return below(r, n);
-}
-__device__ __forceinline__ float root4(float y) {
-    const float r = fast_sqrt(fast_sqrt(y)), n = nearest(r);
-    if (fabsf(r - n) < 0x1p-12f && y > 0.0f) {
-        const float e = __fsqrt_rn(__fsqrt_rn(y));
-        return below(e, nearest(e));
-    }
-    return below(r, n);
-}
 // Byte `i` of w as a float, less `off`.
 __device__ __forceinline__ float byte_float(uint32_t w, int i, float off) {
     return __fsub_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7540 + i)), 8388608.0f + off);
@@ -177,12 +158,44 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
     return d;
 }
-// u < (y - lo) / (hi - lo), the quotient correctly rounded: decided by the
-// product unless the two sides are within the roundings of each other.
-__device__ __forceinline__ bool goes_up(float u, float y, float lo, float hi) {
-    const float a = __fsub_rn(y, lo), w = __fsub_rn(hi, lo), t = __fmaf_rn(u, w, -a);
-    if (fabsf(t) <= w * 0x1p-21f) return u < __fdiv_rn(a, w);
-    return t < 0.0f;
+// The codes of y = |m| (127^2 / scale) and z = v (255^4 / scale): the root's
+// floor k, or k + 1 if u < (y - k^p) / ((k + 1)^p - k^p), p = 2 or 4.
+__device__ __forceinline__ float code_m_exact(float y, float u) {
+    const float r = __fsqrt_rn(y), k = below(r, nearest(r)), lo = __fmul_rn(k, k);
+    const float k1 = __fadd_rn(k, 1.0f), hi = __fmul_rn(k1, k1);
+    return u < __fdiv_rn(__fsub_rn(y, lo), __fsub_rn(hi, lo)) ? k1 : k;
+}
+__device__ __forceinline__ float code_v_exact(float z, float u) {
+    const float r = __fsqrt_rn(__fsqrt_rn(z)), k = below(r, nearest(r));
+    const float k1 = __fadd_rn(k, 1.0f), l = __fmul_rn(k, k), h = __fmul_rn(k1, k1);
+    const float lo = __fmul_rn(l, l), hi = __fmul_rn(h, h);
+    return u < __fdiv_rn(__fsub_rn(z, lo), __fsub_rn(hi, lo)) ? k1 : k;
+}
+// The same from approximate roots and without the division, and whether that
+// may differ (one branch then leads to the exact ones; a warp takes it for one
+// element in fifty).  u is compared with the quotient by the sign of u w - a,
+// certain where that is more than the roundings of both sides.  The roots are
+// off by less than 2^-22 of themselves, so a floor is wrong only if the root
+// is that close to a whole number n <= 255: the quotient is then within 2^-13
+// of 1 from n - 1 and of 0 from n, and both give n unless u is as close to
+// either.  (Testing the root instead would find every block's largest element.)
+__device__ __forceinline__ bool extreme(float u) {
+    return fabsf(__fsub_rn(u, 0.5f)) >= 0.5f - 0x1p-13f;
+}
+__device__ __forceinline__ float code_m(float y, float u, bool& unsure) {
+    const float r = fast_sqrt(y), k = below(r, nearest(r));
+    // (k^2 and 2 k + 1 are exact, so both are rounded as in the exact form)
+    const float a = __fmaf_rn(-k, k, y), w = __fmaf_rn(2.0f, k, 1.0f), t = __fmaf_rn(u, w, -a);
+    unsure = extreme(u) || fabsf(t) <= w * 0x1p-21f;
+    return t < 0.0f ? __fadd_rn(k, 1.0f) : k;
+}
+__device__ __forceinline__ float code_v(float z, float u, bool& unsure) {
+    const float r = fast_sqrt(fast_sqrt(z)), k = below(r, nearest(r));
+    const float k1 = __fadd_rn(k, 1.0f), l = __fmul_rn(k, k), h = __fmul_rn(k1, k1);
+    const float lo = __fmul_rn(l, l), w = __fsub_rn(__fmul_rn(h, h), lo);
+    const float t = __fmaf_rn(u, w, -__fsub_rn(z, lo));
+    unsure = extreme(u) || fabsf(t) <= w * 0x1p-21f;
+    return t < 0.0f ? k1 : k;
 }
 
 __device__ __forceinline__ const Entry& entry_of(const Table& t, unsigned block) {
@@ -318,19 +331,13 @@ __global__ void __launch_bounds__(THREADS)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const uint32_t hh = mix(at ^ (uint32_t)j);
-            const float y = __fmul_rn(fabsf(m[j]), km);
-            float k = root2(y);
-            float k1 = __fadd_rn(k, 1.0f);
-            if (goes_up(unit(hh), y, __fmul_rn(k, k), __fmul_rn(k1, k1))) k = k1;
+            const float um = unit(hh), uv = unit(mix(hh ^ 0x5BD1E995u));
+            const float y = __fmul_rn(fabsf(m[j]), km), z = __fmul_rn(v[j], kw);
+            bool unsure_m, unsure_v;
+            float k = code_m(y, um, unsure_m), l = code_v(z, uv, unsure_v);
+            if (unsure_m || unsure_v) k = code_m_exact(y, um), l = code_v_exact(z, uv);
             mb[j] = low_byte(copysignf(fminf(k, 127.0f), m[j]));
-            const float z = __fmul_rn(v[j], kw);
-            k = root4(z);
-            k1 = __fadd_rn(k, 1.0f);
-            const float lo = __fmul_rn(k, k), hi = __fmul_rn(k1, k1);
-            if (goes_up(unit(mix(hh ^ 0x5BD1E995u)), z, __fmul_rn(lo, lo), __fmul_rn(hi, hi)))
-                k = k1;
-            k = fmaxf(fminf(k, 255.0f), 1.0f);
-            vb[j] = low_byte(z > 0.0f ? k : 0.0f);
+            vb[j] = low_byte(z > 0.0f ? fmaxf(fminf(l, 255.0f), 1.0f) : 0.0f);
         }
         mc = make_uint2(pack_bytes(mb), pack_bytes(mb + 4));
         vc = make_uint2(pack_bytes(vb), pack_bytes(vb + 4));

