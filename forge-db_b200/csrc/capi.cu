@@ -158,6 +158,14 @@ static void check_softmax_buffers(const A& a, size_t need) {
     check_aligned(a.workspace, 256, "the workspace");
 }
 
+// A call without work has not timed out, whatever its workspace holds.
+template <class A>
+static void clear_status(int device, const A& a) {
+    if (!a.workspace || a.workspace_bytes < 4) return;
+    DeviceGuard g(device);
+    FDB_CUDA(cudaMemsetAsync(a.workspace, 0, 4, static_cast<cudaStream_t>(a.stream)));
+}
+
 // Pinned-or-not host <-> device staging for the host-buffer entry points.
 struct Staged {
     DevBuf<uint64_t> ids;
@@ -1205,7 +1213,7 @@ int fdb_logprobs(fdb_ctx* ctx, const fdb_logprob_args* args) {
         check_softmax(a);
         FDB_REQUIRE(a.k <= FDB_MAX_ALTERNATIVES, FDB_ERR_INVALID_ARG,
                     "k must not exceed FDB_MAX_ALTERNATIVES");
-        if (a.nq == 0) return;
+        if (a.nq == 0) return clear_status(ctx->c.device, a);
         FDB_REQUIRE(a.k == 0 || (a.top_ids && a.top_logprobs), FDB_ERR_INVALID_ARG,
                     "k > 0 needs top_ids and top_logprobs");
         check_softmax_buffers(a, sr::forward_bytes(ctx->c, a));
@@ -1244,7 +1252,7 @@ int fdb_logprobs_backward(fdb_ctx* ctx, const fdb_logprob_grad_args* args) {
             if (a.d_rows)
                 FDB_CUDA(cudaMemset2DAsync(a.d_rows, a.ld_d_rows * es, 0, a.dim * es, a.n,
                                            static_cast<cudaStream_t>(a.stream)));
-            return;
+            return clear_status(ctx->c.device, a);
         }
         FDB_REQUIRE(a.lse, FDB_ERR_INVALID_ARG, "lse is NULL");
         FDB_REQUIRE(!a.d_entropy || a.entropy, FDB_ERR_INVALID_ARG,
@@ -1252,7 +1260,7 @@ int fdb_logprobs_backward(fdb_ctx* ctx, const fdb_logprob_grad_args* args) {
         for (const float* p : {a.lse, a.entropy, a.d_logprob, a.d_lse, a.d_entropy})
             check_aligned(p, 4, "an input");
         check_softmax_buffers(a, sr::backward_bytes(ctx->c, a));
-        if (!a.d_queries && !a.d_rows) return;
+        if (!a.d_queries && !a.d_rows) return clear_status(ctx->c.device, a);
         sr::backward_run(ctx->c, a);
     });
 }

@@ -452,7 +452,8 @@ int fdb_bf_remove(fdb_bf* h, uint64_t id, int* removed);
  * return without waiting; inputs, outputs and the workspace have to stay valid
  * until that work is done.  They allocate nothing and hold no state, so they
  * can be captured into a CUDA graph, and calls on different streams may
- * overlap as long as each has a workspace of its own. */
+ * overlap as long as each has a workspace of its own.  No output may overlap
+ * an input, another output or the workspace. */
 #define FDB_DTYPE_F32 0
 #define FDB_DTYPE_F16 1
 #define FDB_DTYPE_BF16 2
@@ -471,7 +472,8 @@ int fdb_bf_remove(fdb_bf* h, uint64_t id, int* removed);
  * -inf for a target that is not allowed), lse[nq], entropy[nq] in nats; with
  * k > 0 top_ids[nq][k] and top_logprobs[nq][k] (both required), the k most
  * probable rows in order, equal scores by row number, -1 and -inf past the
- * allowed rows.  A query that may see no row has lse -inf, entropy 0.  If a
+ * allowed rows.  A query that may see no row has lse -inf, entropy 0.  Scores
+ * have to lie within +-1e28.  If a
  * query, or a row it may see, holds an infinity or NaN, the query's outputs
  * are NaN (top_ids -1). */
 typedef struct fdb_logprob_args {

@@ -629,3 +629,86 @@ def test_index_follows_its_changes_and_refuses():
     with pytest.raises(fg.ForgeGpuError) as e:
         eu.log_probs(q)
     assert e.value.kind == "NotSupported"
+
+
+@pytest.mark.parametrize("dtype,nq,n,dim,mask,pad,shift,k", [
+    # f32 rows of one block of K, tiles of 256 columns: both sides of its last dimension
+    ("f32", 300, 4099, 128, "each", 0, 0, 10), ("f32", 257, 2050, 113, "one", 3, 1, 64),
+    ("f32", 130, 2305, 129, "one", 0, 0, 5), ("f32", 520, 1, 16, "none", 0, 0, 3),
+    ("f32", 18, 767, 64, "none", 0, 0, 0),
+    # the largest dimension
+    ("f32", 2, 70, 16384, "none", 0, 0, 4), ("f32", 33, 400, 16384, "each", 0, 0, 4),
+    ("bf16", 5, 300, 16384, "one", 0, 0, 64), ("f16", 20, 90, 16383, "none", 1, 0, 2),
+])
+def test_forward_at_its_limits(dtype, nq, n, dim, mask, pad, shift, k):
+    test_forward(dtype, nq, n, dim, mask, pad, shift, k)
+
+
+@pytest.mark.parametrize("dtype,nq,n,dim,mask,pad,shift", [
+    ("f32", 1, 4000, 128, "none", 0, 0), ("f32", 9, 50, 16384, "each", 0, 0),
+    ("bf16", 9, 50, 16384, "none", 0, 0), ("f16", 3, 40, 16383, "one", 0, 1),
+    ("f32", 600, 1, 32, "each", 0, 0), ("bf16", 70, 2, 1, "each", 0, 0),
+    ("bf16", 1500, 700, 64, "each", 0, 0),
+])
+def test_backward_at_its_limits(dtype, nq, n, dim, mask, pad, shift):
+    test_backward(dtype, nq, n, dim, mask, pad, shift)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_one_target_for_all_queries(dtype):
+    """Every query's given row is the same: its gradient is the sum of all of
+    theirs, in a fixed order."""
+    import forgegpu as fg
+    import torch
+    nq, n = 400, 900
+    Q, X, _, _, q, x, _, _ = make(dtype, nq, n, 72, "none", seed=12)
+    t = np.full(nq, 77)
+    T = torch.from_numpy(t).cuda()
+    f = so.forward(q, x, t, 0.25, None, 0)
+    lse = f["lse"].astype(np.float32)
+    up = torch.full((nq,), -1.0 / nq, device="cuda")
+    run = lambda: fg.logprobs_backward(Q, X, T, torch.from_numpy(lse).cuda(), d_logprob=up,
+                                       scale=0.25)
+    got, again = run(), run()
+    u = up.double().cpu().numpy()
+    z = np.zeros(nq)
+    dq, dx, _, size = so.backward(q, x, t, lse.astype(np.float64), z, u, z, z, 0.25, None)
+    es = so.score_bound(q, x, 0.25, dtype)
+    bounds = so.gradient_bounds(q, x, es, size, f["keep"], dtype, dq, dx)
+    for g, h, w, b in zip(got, again, (dq, dx), bounds):
+        assert torch.equal(g, h)
+        assert (np.abs(g.double().cpu().numpy() - w) <= b + 1e-30).all()
+
+
+@pytest.mark.parametrize("dtype,nq", [("f32", 3), ("f32", 40), ("bf16", 2), ("bf16", 300)])
+@pytest.mark.parametrize("rows", [1, "nq"])
+def test_a_filter_that_leaves_nothing(dtype, nq, rows):
+    """No query sees a row: lse -inf, entropy 0, no alternatives, a given row
+    -inf, gradients of zero."""
+    import forgegpu as fg
+    import torch
+    Q, X, T, *_ = make(dtype, nq, 700, 24, "none", seed=13)
+    A = torch.zeros((nq if rows == "nq" else 1, 22), dtype=torch.int32, device="cuda")
+    r = fg.logprobs(Q, X, T, scale=0.5, allowed=A, k=4)
+    assert (r.lse == -float("inf")).all() and (r.entropy == 0).all()
+    assert torch.equal(r.logprob, torch.where(T >= 0, -float("inf"), 0.0))
+    assert (r.top_ids == -1).all() and (r.top_logprobs == -float("inf")).all()
+    up = torch.ones(nq, device="cuda")
+    for g in fg.logprobs_backward(Q, X, T, r.lse, r.entropy, d_logprob=up, d_lse=up,
+                                  d_entropy=up, scale=0.5, allowed=A):
+        assert (g == 0).all()
+
+
+def test_status_of_a_call_without_work():
+    import forgegpu as fg
+    import torch
+    Q, X, T, *_ = make("bf16", 4, 50, 16, "none", seed=14)
+    for call in (lambda ws: fg.logprobs(Q[:0], X, T[:0], k=2, workspace=ws),
+                 lambda ws: fg.logprobs_backward(Q[:0], X, T[:0], torch.zeros(0, device="cuda"),
+                                                 workspace=ws),
+                 lambda ws: fg.logprobs_backward(Q, X, T, torch.zeros(4, device="cuda"),
+                                                 need_queries=False, need_rows=False,
+                                                 workspace=ws)):
+        ws = torch.full((1 << 20,), 255, dtype=torch.uint8, device="cuda")
+        call(ws)
+        fg.logprobs_status(ws)
