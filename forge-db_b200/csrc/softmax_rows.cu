@@ -67,7 +67,7 @@ __host__ __device__ constexpr int staged_of(bool two, bool grad) {
 }
 constexpr int MAX_STG = 8;
 // K steps of an accumulator, sums in blocks
-__host__ __device__ constexpr int kblock_of(bool two) { return two ? 2 : 4; }
+__host__ __device__ constexpr int kblock_of(bool two, bool grad) { return grad ? 1 : two ? 2 : 4; }
 constexpr int MAX_BN = 256;
 constexpr unsigned long long DRAIN_CYCLES = 4000000ull;  // about 2 ms
 constexpr int THREADS = 640;                // 2 issuing warps, 2 idle, 16 epilogue warps
@@ -1000,7 +1000,10 @@ __device__ __forceinline__ Unit unit_of(const Mma& g, int u) {
 // that matters (f32, and long rows) sums are taken in blocks (BLK): an
 // accumulator holds 128 of K (TWO parts: first the products lo.hi and hi.lo,
 // then hi.hi) or 256, and the epilogue adds them up in registers.  Else an
-// accumulator is a whole tile.
+// accumulator is a whole tile.  GRAD takes 64 of K, whose sums it has the time
+// for: what a score is off by, its probability is off by of itself (d_rows of
+// 125 x 4405 x 74 f32: 1.3e-6 of its norm with 128, 4.6e-7 with 64 and the half
+// of cut_of; 60 us either way).
 template <int MODE, bool TWO, bool BLK>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     rows_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
@@ -1010,7 +1013,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     constexpr bool A_MN = MODE == PROD_X, B_MN = PROD;
     constexpr int BN = bn_of(BLK), NST = stages_of(TWO, BLK, MODE == GRAD), NACC = accs_of(BLK);
     constexpr int STAGE = stage_bytes(TWO, BLK), PARTS = TWO ? 2 : 1;
-    constexpr int KBLOCK = kblock_of(TWO);
+    constexpr int KBLOCK = kblock_of(TWO, MODE == GRAD);
     constexpr int B0 = PARTS * OPER;               // operand B in a stage
     constexpr int B_PART = BN / 2 * 128;           // bytes of one part of this block's half
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -1520,6 +1523,7 @@ struct FinishArgs {
     // the column tiles of chunk i / 4; few queries (nt = 0): part i is block i,
     // whose two warps took every 2 * parts-th group.
     int nt, chunks, per_tile, per_part;  // per_tile: groups of a tile, per_part: of its quarter
+    double whole;  // a score over what its tensor-core sum comes to (see cut_of)
     float *logprob, *lse, *entropy, *top_logprob;
     int64_t* top_ids;
     const int* err;
@@ -1672,8 +1676,10 @@ __global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kern
     float f = 1.0f;
     if (p.qf) f = p.qf[ql] == 0.0f ? 1.0f : p.qf[ql];
     const float rf = f * (float)((double)p.scale * LOG2E);
-    // t was formed with rf, rounded to f32; M of it is set right here
-    const double unit = (double)p.scale * LOG2E, fix = (double)f * unit / (double)rf;
+    // t was formed with rf, rounded to f32, from a sum that was cut; M of it is
+    // set right here (t - M is small where it counts)
+    const double unit = (double)p.scale * LOG2E;
+    const double fix = (double)f * unit / (double)rf * p.whole;
     const int64_t target = p.targets ? p.targets[q] : -1;
     const bool given = target >= 0 && target < p.n;
     if (tid == 0) s_picked = s_cnt = s_parts = 0, s_kth = -INFINITY;
@@ -2072,7 +2078,7 @@ __device__ __forceinline__ float fix_row(__half* x, float* f, int row, int width
 }
 struct CoefArgs {
     int nq, n;
-    double scale;
+    double scale, whole;  // (whole: see cut_of)
     const float *lse, *entropy, *d_logprob, *d_lse, *d_entropy;
     const int64_t* targets;
     const uint32_t* allowed;
@@ -2087,7 +2093,7 @@ struct CoefArgs {
 __device__ __forceinline__ void coef_of(const CoefArgs& a, int i, float f) {
     const float lse = a.lse[i];
     const bool empty = lse == -INFINITY;
-    const double rf = (double)f * a.scale * LOG2E, l = (double)lse * LOG2E;
+    const double rf = (double)f * a.scale * LOG2E * a.whole, l = (double)lse * LOG2E;
     const int64_t t = a.targets ? a.targets[i] : -1;
     const bool given = !empty && t >= 0 && t < a.n &&
                        (!a.allowed ||
@@ -2463,6 +2469,19 @@ static void launch_finish(cudaStream_t s, int device, const FinishArgs& f) {
     else launch_finish_t<T, 128>(s, device, f);
 }
 
+// The share of a score that the tensor core's additions cut off on average,
+// for sums over `block` 16-wide steps (0: all of them).  They cut towards zero:
+// terms of one sign fall short by a share of the score that grows with the steps
+// (measured over rows of 16 to 768 dimensions: 5.2e-8 a step less 2e-8 for fp16
+// products, 2.3e-8 a step for bf16, with a spread of 0.6 to 1.0e-7 between
+// scores), in sums of mixed signs nearly all of it cancels.  Half of the former
+// is added to every score, so that neither kind is off by more than half.
+static double cut_of(bool bf16, size_t dim, int block) {
+    const double steps = (double)((dim + 15) / 16), b = block ? block : steps;
+    auto cut = [&](double n) { return bf16 ? 2.3e-8 * n : 5.2e-8 * n - 2e-8; };
+    const double whole = floor(steps / b) * b, rest = steps - whole;
+    return 0.5 * (whole * cut(b) + (rest > 0.0 ? rest * cut(rest) : 0.0)) / steps;
+}
 static FinishArgs finish_args(const fdb_logprob_args& a, const Forward& w, size_t q0, size_t nq) {
     FinishArgs f{};
     f.q = a.queries, f.x = a.rows;
@@ -2476,6 +2495,9 @@ static FinishArgs finish_args(const fdb_logprob_args& a, const Forward& w, size_
     f.logprob = a.logprob, f.lse = a.lse, f.entropy = a.entropy;
     f.top_logprob = a.top_logprobs, f.top_ids = a.top_ids;
     f.err = w.err;
+    f.whole = w.few ? 1.0
+                    : 1.0 + cut_of(a.dtype == FDB_DTYPE_BF16, a.dim,
+                                   w.blocks ? 4 * kblock_of(w.packed, false) : 0);
     return f;
 }
 
@@ -2677,6 +2699,7 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
                 a.dim, w.kp, nullptr);
     CoefArgs k{};
     k.nq = nq, k.n = n, k.scale = a.scale;
+    k.whole = 1.0 + cut_of(false, a.dim, w.parts == 2 ? 4 * kblock_of(true, true) : 0);
     k.lse = a.lse, k.entropy = a.entropy;
     k.d_logprob = a.d_logprob, k.d_lse = a.d_lse, k.d_entropy = a.d_entropy;
     k.targets = a.targets, k.allowed = a.allowed, k.ld_allowed = ld_allowed;
