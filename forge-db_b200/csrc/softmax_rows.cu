@@ -122,6 +122,17 @@ __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) {
     return __bfloat162float(v);
 }
 
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+    return __float2bfloat16_rn(v);
+}
+
 // A running (reference m, sum l = sum 2^(t - m), a = sum 2^(t - m) (t - m)) of
 // one query's columns, t = score * log2(e).  m starts at the first columns'
 // largest t and is raised only when a t exceeds it by more than RAISE: the
@@ -2090,7 +2101,7 @@ struct CoefArgs {
 // G_ij = scale [ p_ij (dl - g - h (lp_ij + H)) + g 1{j = t} ] with lp = ln2 x:
 // = p (c + h' x) + g', and a bound of its size for the common scale
 // (p |lp| <= 1/e).
-__device__ __forceinline__ void coef_of(const CoefArgs& a, int i, float f) {
+__device__ __forceinline__ Coef coef_of(const CoefArgs& a, int i, float f, float& bound) {
     const float lse = a.lse[i];
     const bool empty = lse == -INFINITY;
     const double rf = (double)f * a.scale * LOG2E * a.whole, l = (double)lse * LOG2E;
@@ -2111,12 +2122,8 @@ __device__ __forceinline__ void coef_of(const CoefArgs& a, int i, float f) {
     k.h = (float)(-a.scale * dh * LN2);
     k.g = (float)(a.scale * g);
     k.target = given ? (int)t : -1;
-    a.out[i] = k;
-    if (a.rest) a.rest[i] = 0.0f;
-    const float b = (float)(a.scale * (fabs(dl) + 2.0 * fabs(g) + fabs(dh) * (fabs(H) + 1.0)) *
-                            (double)f);
-    if (b > 0.0f && b <= FLT_MAX)
-        atomicMax(reinterpret_cast<unsigned*>(a.bounds), __float_as_uint(b));
+    bound = (float)(a.scale * (fabs(dl) + 2.0 * fabs(g) + fabs(dh) * (fabs(H) + 1.0)) * (double)f);
+    return k;
 }
 // One warp per row of either operand: its scale settled, and per query its
 // coefficients.  Queries come first.
@@ -2127,7 +2134,13 @@ __global__ void __launch_bounds__(256)
         const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
         if (row >= a.nq) return;
         const float f = fix_row(qp, qf, row, width, a.bounds[2]);
-        if ((threadIdx.x & 31) == 0) coef_of(a, row, f);
+        if ((threadIdx.x & 31) == 0) {
+            float b;
+            a.out[row] = coef_of(a, row, f, b);
+            if (a.rest) a.rest[row] = 0.0f;
+            if (b > 0.0f && b <= FLT_MAX)
+                atomicMax(reinterpret_cast<unsigned*>(a.bounds), __float_as_uint(b));
+        }
         return;
     }
     // rows: a lane looks at one, the warp mends those that need it
@@ -2148,7 +2161,7 @@ struct JoinRest {
     const __half* x;
     int ldx;
 };
-// Sum of the splits, scaled, in the output's type: four columns of a row by one
+// Sum of the splits, scaled (f null: not), in the output's type: four columns of a row by one
 // thread, or by eight that take every eighth split and are added in order (16
 // splits and more: 64 of 100 x 128 took 10.9 us one after the other, now 3.7;
 // few splits of a large output are better off with more columns a block).
@@ -2162,7 +2175,7 @@ __global__ void __launch_bounds__(256)
     const unsigned per4 = (unsigned)(cols + 3) / 4;
     const size_t plane = (size_t)rows * cols, all = (size_t)rows * per4;
     const bool wide = (cols & 3) == 0;
-    const float c = grad_factor(bounds);
+    const float c = f ? grad_factor(bounds) : 1.0f;
     const int lane = threadIdx.x % LANES, turn = threadIdx.x / LANES;
     for (size_t i0 = (size_t)blockIdx.x * LANES; i0 < all; i0 += (size_t)gridDim.x * LANES) {
         const size_t i = i0 + lane;
@@ -2206,7 +2219,7 @@ __global__ void __launch_bounds__(256)
                     if (k + 3 < cols) v.w = __fmaf_rn(g, __half2float(x[3]), v.w);
                 }
             }
-            const float s = 1.0f / (f[r] * c);
+            const float s = f ? 1.0f / (f[r] * c) : 1.0f;
             const float o[4] = {v.x * s, v.y * s, v.z * s, v.w * s};
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -2225,6 +2238,215 @@ static void launch_join(cudaStream_t s, int sms, const float* partial, int split
         join_kernel<1><<<sms * 8, 256, 0, s>>>(partial, splits, rows, cols, f, bounds, out, ldo,
                                                dtype, rest);
     FDB_LAUNCH_CHECK();
+}
+// ---------------------------------------------------------------------------
+// the gradient for a few queries: one pass over the rows on the FMA pipes
+// ---------------------------------------------------------------------------
+// A block takes 16 rows at a time.  Each warp forms the scores of two of them
+// (its lanes share the columns) while it lays them into shared memory, and the
+// score gradients; then a thread owns four columns of the 16 rows (or of a share
+// of them, if the columns are few): d_rows = G^T Q is complete and stored, its
+// columns of d_queries = G X stay in registers until the block's last rows.
+// Every row is read and its gradient written once; what bounds it is the latency
+// of the two halves, which the blocks of a multiprocessor (registers: three of 1
+// or 2 queries, two of more) hide for each other: 100000 x 768 f32 takes 132 us
+// with 1 query and 249 with 8, where the bytes alone take 92.  The tensor-core
+// path, which copies the rows and pads the queries to 256, took 513 and 453 (bf16:
+// 113 and 248, was 257 and 240), and 2000 x 128 with 8 queries 34 us, here 11.
+template <typename T>
+struct FewGrad {
+    const T* x;
+    size_t ldx;
+    const T* q;
+    size_t ldq;
+    int n, d, nq;
+    CoefArgs coef;
+    T* dx;           // nullable
+    size_t ld_dx;
+    float* partial;  // [blocks][nq][d], nullable
+    int* err;
+};
+constexpr int FEW_ROWS = 16;
+constexpr int few_per_sm(int NQ) { return NQ <= 2 ? 3 : 2; }  // (blocks; registers)
+static size_t few_grad_smem(int NQ, size_t d, size_t elem) {
+    const size_t dp = (d + 63) / 64 * 64;
+    return NQ * dp * 4 + FEW_ROWS * NQ * 8 +
+           std::max<size_t>(FEW_ROWS * dp * elem, (size_t)NQ * 4096);
+}
+// Columns c and c + 32 of a query lie side by side, as the lanes multiply two
+// at a time.
+__device__ __forceinline__ int few_at(int c) {
+    return (c & ~63) + 2 * (c & 31) + (c >> 5 & 1);
+}
+template <typename T, int NQ>
+__global__ void __launch_bounds__(256, few_per_sm(NQ)) few_grad_kernel(const FewGrad<T> p) {
+    extern __shared__ float4 few_raw[];
+    const int d = p.d, ct_n = (d + 3) / 4, dp = (d + 63) & ~63;
+    float* qs = reinterpret_cast<float*>(few_raw);                  // [NQ][dp], see few_at
+    float2* gs = reinterpret_cast<float2*>(qs + NQ * dp);           // [rows][NQ], twice each
+    T* xs = reinterpret_cast<T*>(gs + FEW_ROWS * NQ);               // [rows][dp], at the end sums
+    __shared__ Coef co[NQ];
+    __shared__ int q_bad[NQ], x_bad[FEW_ROWS];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (blockIdx.x == 0 && tid == 0) *p.err = 0;  // (this path has no waits)
+    if (tid < NQ) q_bad[tid] = 0;
+    __syncthreads();
+    for (int i = tid; i < NQ * dp; i += 256) {
+        const int j = i / dp, c = i - j * dp;
+        const float v = j < p.nq && c < d ? to_f32<T>(p.q[(size_t)j * p.ldq + c]) : 0.0f;
+        if (!(fabsf(v) <= FLT_MAX)) q_bad[j] = 1;
+        qs[j * dp + few_at(c)] = v;
+    }
+    if (tid < p.nq) {
+        float bound;
+        co[tid] = coef_of(p.coef, tid, 1.0f, bound);
+    }
+    __syncthreads();
+    // what a query that sees nothing holds does not count, an infinity or NaN of
+    // another reaches the rows that it sees through G alone
+    for (int i = tid; i < NQ * dp; i += 256) {
+        const int j = i / dp;
+        if (j < p.nq && (q_bad[j] || p.coef.lse[j] == -INFINITY)) qs[i] = 0.0f;
+    }
+    __syncthreads();
+    const int groups = 256 / ct_n, rg = tid / ct_n, ct = tid - rg * ct_n;
+    uint64_t qr[NQ][2], acc[NQ][2];
+#pragma unroll
+    for (int j = 0; j < NQ; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int c = ct + 2 * h * ct_n;
+            const float* o = qs + j * dp;
+            qr[j][h] = packf(c < d ? o[few_at(c)] : 0.0f,
+                             c + ct_n < d ? o[few_at(c + ct_n)] : 0.0f);
+            acc[j][h] = 0ull;
+        }
+    // (unsigned: the last step may pass 2^31)
+    for (unsigned u0 = blockIdx.x * FEW_ROWS; u0 < (unsigned)p.n; u0 += gridDim.x * FEW_ROWS) {
+        const int r0 = (int)u0;
+        {  // the next rows on their way
+            const int lines = (d * (int)sizeof(T) + 127) / 128;
+            for (int i = tid; i < FEW_ROWS * lines; i += 256) {
+                const long long row = (long long)r0 + (long long)gridDim.x * FEW_ROWS + i / lines;
+                if (row < p.n)
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(
+                        p.x + (size_t)row * p.ldx + i % lines * (128 / (int)sizeof(T))));
+            }
+        }
+        const int w0 = 2 * warp;
+        if (lane < 2) x_bad[w0 + lane] = 0;
+        const T* xa = p.x + (size_t)min(r0 + w0, p.n - 1) * p.ldx;
+        const T* xb = p.x + (size_t)min(r0 + w0 + 1, p.n - 1) * p.ldx;
+        uint64_t sa[NQ], sb[NQ];
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) sa[j] = sb[j] = 0ull;
+#pragma unroll 4
+        for (int c = lane; c < d; c += 64) {
+            const bool two = c + 32 < d;
+            const T zero = from_f32<T>(0.0f);
+            const T a0 = xa[c], b0 = xb[c];
+            const T a1 = two ? xa[c + 32] : zero, b1 = two ? xb[c + 32] : zero;
+            T* o = xs + w0 * dp + c;
+            o[0] = a0, o[32] = a1, o[dp] = b0, o[dp + 32] = b1;
+            const uint64_t a = packf(to_f32<T>(a0), to_f32<T>(a1));
+            const uint64_t b = packf(to_f32<T>(b0), to_f32<T>(b1));
+#pragma unroll
+            for (int j = 0; j < NQ; ++j) {
+                const uint64_t v =
+                    *reinterpret_cast<const uint64_t*>(qs + j * dp + (c & ~63) + 2 * lane);
+                sa[j] = fma2(a, v, sa[j]);
+                sb[j] = fma2(b, v, sb[j]);
+            }
+        }
+        // halves of the sums are exchanged while more than one is left
+        float v[2 * NQ];
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+            v[2 * j] = lo_of(sa[j]) + hi_of(sa[j]);
+            v[2 * j + 1] = lo_of(sb[j]) + hi_of(sb[j]);
+        }
+#pragma unroll
+        for (int o = 16, m = NQ; o; o >>= 1, m >>= 1) {
+            if (m > 0) {
+#pragma unroll
+                for (int i = 0; i < m; ++i) {
+                    const float keep = lane & o ? v[i + m] : v[i];
+                    const float give = lane & o ? v[i] : v[i + m];
+                    v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+                }
+            } else {
+                v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+            }
+        }
+        __syncwarp();
+        if (lane % (16 / NQ) == 0) {
+            const int i = lane / (16 / NQ), j = i >> 1, r = w0 + (i & 1), row = r0 + r;
+            float g = 0.0f;
+            if (j < p.nq && row < p.n) {
+                const bool x_off = !(fabsf(v[0]) <= FLT_MAX);
+                if (x_off) x_bad[r] = 1;
+                const uint32_t w = allowed_word(p.coef.allowed, p.coef.ld_allowed, j,
+                                                (size_t)(row & ~31), p.n);
+                const Coef& k = co[j];
+                const float y = __fmaf_rn(v[0], k.rf_hi, -k.l_hi) + __fmaf_rn(v[0], k.rf_lo, -k.l_lo);
+                const float t = fmaxf(y, -160.0f);
+                g = ex2(t) * __fmaf_rn(t, k.h, k.c);
+                if (row == k.target) g += k.g;
+                if (x_off || q_bad[j]) g = NAN;
+                if (!(w >> (row & 31) & 1u)) g = 0.0f;
+            }
+            gs[r * NQ + j] = make_float2(g, g);
+        }
+        __syncthreads();
+        if (rg < groups) {
+#pragma unroll (NQ > 4 ? 1 : 2)
+            for (int r = rg; r < FEW_ROWS; r += groups) {
+                // (columns past the last: whatever lies there, for sums that nobody takes)
+                const T* x = xs + r * dp + ct;
+                float xv[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) xv[i] = to_f32<T>(x[i * ct_n]);
+                if (x_bad[r] || r0 + r >= p.n) xv[0] = xv[1] = xv[2] = xv[3] = 0.0f;
+                const uint64_t x2[2] = {packf(xv[0], xv[1]), packf(xv[2], xv[3])};
+                uint64_t o2[2] = {0ull, 0ull};
+#pragma unroll
+                for (int j = 0; j < NQ; ++j) {
+                    const uint64_t g2 = *reinterpret_cast<const uint64_t*>(gs + r * NQ + j);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        acc[j][h] = fma2(g2, x2[h], acc[j][h]);
+                        o2[h] = fma2(g2, qr[j][h], o2[h]);
+                    }
+                }
+                if (p.dx && r0 + r < p.n) {
+                    T* o = p.dx + (size_t)(r0 + r) * p.ld_dx + ct;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float y = i & 1 ? hi_of(o2[i >> 1]) : lo_of(o2[i >> 1]);
+                        if (ct + i * ct_n < d) o[i * ct_n] = from_f32<T>(y);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+    if (!p.partial) return;
+    float* sums = reinterpret_cast<float*>(xs);  // [groups][NQ][4 ct_n]
+    if (rg < groups) {
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                sums[(rg * NQ + j) * 4 * ct_n + ct + i * ct_n] =
+                    i & 1 ? hi_of(acc[j][i >> 1]) : lo_of(acc[j][i >> 1]);
+    }
+    __syncthreads();
+    for (int i = tid; i < p.nq * d; i += 256) {
+        const int j = i / d, c = i - j * d;
+        float t = 0.0f;
+        for (int k = 0; k < min(groups, FEW_ROWS); ++k) t += sums[(k * NQ + j) * 4 * ct_n + c];
+        p.partial[((size_t)blockIdx.x * p.nq + j) * d + c] = t;
+    }
 }
 // A call whose waits ran out has no gradient: NaN.
 __global__ void void_kernel(const int* err, void* dq, size_t ldq, int nq, void* dx, size_t ldx,
@@ -2254,6 +2476,7 @@ constexpr int FEW = 8;                          // queries a pass of few_kernel 
 // f32 rows would have to be split for the tensor cores first: two passes still
 // cost less; 16-bit rows are read by them as they are.
 constexpr int FEW_F32 = 16, FEW_16 = 2, FEW_DIM = 2048;
+constexpr int FEW_GRAD = 8, FEW_GRAD_DIM = 1024;  // few_grad_kernel: see there
 static size_t smem_of(bool two, bool blk, bool grad) {
     // alignment, stages, staged outputs, barriers, column factors
     return 1024 + (size_t)stages_of(two, blk, grad) * stage_bytes(two, blk) +
@@ -2624,7 +2847,8 @@ void forward_run(Ctx& c, const fdb_logprob_args& a) {
 
 // ---- backward ----
 struct Backward {
-    int parts;
+    bool few;
+    int parts, few_blocks;
     size_t kp, nqp, cols, ldg;  // cols: rows of a chunk
     int bn, q_splits, x_splits;
     size_t bytes;
@@ -2639,6 +2863,15 @@ struct Backward {
 static Backward plan_backward(const Ctx& c, const fdb_logprob_grad_args& a) {
     Backward w{};
     Carve ws(a.workspace);
+    w.few = a.nq <= FEW_GRAD && a.dim <= FEW_GRAD_DIM;
+    if (w.few) {
+        w.err = ws.take<int>(HEAD / 4);
+        w.few_blocks = (int)std::min<size_t>((a.n + FEW_ROWS - 1) / FEW_ROWS,
+                                             few_per_sm((int)a.nq) * c.sm_count);
+        w.dq = ws.take<float>((size_t)w.few_blocks * a.nq * a.dim);
+        w.bytes = ws.at;
+        return w;
+    }
     w.parts = a.dtype == FDB_DTYPE_F32 ? 2 : 1;
     w.kp = up(a.dim, 16);
     w.nqp = up(a.nq, BM);
@@ -2675,9 +2908,49 @@ size_t backward_bytes(const Ctx& c, const fdb_logprob_grad_args& a) {
     return plan_backward(c, b).bytes;
 }
 
+template <typename T>
+static void few_backward(const Ctx& c, const fdb_logprob_grad_args& a, const Backward& w,
+                         const CoefArgs& k) {
+    const cudaStream_t s = static_cast<cudaStream_t>(a.stream);
+    FewGrad<T> p{};
+    p.x = static_cast<const T*>(a.rows), p.ldx = a.ld_rows;
+    p.q = static_cast<const T*>(a.queries), p.ldq = a.ld_queries;
+    p.n = (int)a.n, p.d = (int)a.dim, p.nq = (int)a.nq;
+    p.coef = k;
+    p.dx = static_cast<T*>(a.d_rows), p.ld_dx = a.ld_d_rows;
+    p.partial = a.d_queries ? w.dq : nullptr;
+    p.err = w.err;
+    auto go = [&](auto kernel, int NQ) {
+        const size_t sm = few_grad_smem(NQ, a.dim, sizeof(T));
+        if (sm > 40960)
+            FDB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          (int)sm));
+        kernel<<<w.few_blocks, 256, sm, s>>>(p);
+        FDB_LAUNCH_CHECK();
+    };
+    if (a.nq == 1) go(few_grad_kernel<T, 1>, 1);
+    else if (a.nq == 2) go(few_grad_kernel<T, 2>, 2);
+    else if (a.nq <= 4) go(few_grad_kernel<T, 4>, 4);
+    else go(few_grad_kernel<T, 8>, 8);
+    if (a.d_queries)
+        launch_join(s, c.sm_count, w.dq, w.few_blocks, (int)a.nq, (int)a.dim, nullptr, nullptr,
+                    a.d_queries, a.ld_d_queries, a.dtype);
+}
+
 void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
     const cudaStream_t s = static_cast<cudaStream_t>(a.stream);
     const Backward w = plan_backward(c, a);
+    if (w.few) {
+        CoefArgs k{};
+        k.nq = (int)a.nq, k.n = (int)a.n, k.scale = a.scale, k.whole = 1.0;
+        k.lse = a.lse, k.entropy = a.entropy;
+        k.d_logprob = a.d_logprob, k.d_lse = a.d_lse, k.d_entropy = a.d_entropy;
+        k.targets = a.targets, k.allowed = a.allowed, k.ld_allowed = a.allowed ? a.ld_allowed : 0;
+        if (a.dtype == FDB_DTYPE_F32) few_backward<float>(c, a, w, k);
+        else if (a.dtype == FDB_DTYPE_F16) few_backward<__half>(c, a, w, k);
+        else few_backward<__nv_bfloat16>(c, a, w, k);
+        return;
+    }
     const int n = (int)a.n, d = (int)a.dim, nq = (int)a.nq;
     const size_t ld_allowed = a.allowed ? a.ld_allowed : 0;
     head_kernel<<<(nq + 255) / 256, 256, 0, s>>>(a.lse, nq, w.alive,

@@ -649,6 +649,12 @@ def test_forward_at_its_limits(dtype, nq, n, dim, mask, pad, shift, k):
     ("bf16", 9, 50, 16384, "none", 0, 0), ("f16", 3, 40, 16383, "one", 0, 1),
     ("f32", 600, 1, 32, "each", 0, 0), ("bf16", 70, 2, 1, "each", 0, 0),
     ("bf16", 1500, 700, 64, "each", 0, 0),
+    # few queries: several steps a block, the largest dimension, one past either
+    ("f32", 1, 16000, 100, "one", 0, 0), ("f32", 3, 9001, 61, "each", 1, 1),
+    ("f32", 8, 500, 1024, "each", 0, 0), ("f32", 8, 30, 1025, "none", 0, 0),
+    ("f32", 9, 700, 33, "each", 0, 0), ("bf16", 2, 12001, 200, "each", 3, 1),
+    ("bf16", 6, 300, 1023, "one", 0, 0), ("f16", 8, 5000, 5, "each", 0, 0),
+    ("f16", 4, 17, 96, "none", 0, 0),
 ])
 def test_backward_at_its_limits(dtype, nq, n, dim, mask, pad, shift):
     test_backward(dtype, nq, n, dim, mask, pad, shift)
