@@ -1665,7 +1665,7 @@ __global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kern
     __shared__ float redf[W];
     __shared__ float s_bound;
     __shared__ int s_picked, s_cnt, s_parts;
-    __shared__ int part_of[PARTS_PICKED];
+    __shared__ int2 part_of[PARTS_PICKED];  // first group, groups
     __shared__ int sel[PICKED];
     __shared__ float2 sel_m[PICKED];
     __shared__ uint64_t cs[CAND + 1];  // exact scores, as ordered64
@@ -1816,33 +1816,31 @@ __global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kern
 #pragma unroll 4
         for (int i = tid; i < groups; i += THREADS_) pick(i, top[i]);
     }
+    // a part's groups are `run` side by side, `step` from one run to the next
+    const int run = p.nt ? p.per_part : 2, step = p.nt ? p.per_tile : 2 * p.parts;
     for (int i = tid; i < (groups && by_parts ? p.parts : 0); i += THREADS_) {
         const float t = p.part[(size_t)i * p.nq + ql].w;
         if (t > NONE_BELOW && t >= bound) {
             const int at = atomicAdd(&s_parts, 1);
-            if (at < PARTS_PICKED) part_of[at] = i;
+            if (at >= PARTS_PICKED) continue;
+            if (p.nt) {
+                const long long c = i >> 2;
+                const int t0 = (int)(c * p.nt / p.chunks), t1 = (int)((c + 1) * p.nt / p.chunks);
+                part_of[at] = make_int2(t0 * step + (i & 3) * run, (t1 - t0) * run);
+            } else {
+                part_of[at] = make_int2(2 * i, 2 * ((groups + step - 1) / step));
+            }
         }
     }
     __syncthreads();
-    const int nparts = min(s_parts, PARTS_PICKED);
-    // (the longest part's groups; chunks differ by one tile)
-    const int longest = p.nt ? (p.nt + p.chunks - 1) / p.chunks * p.per_part
-                             : 2 * ((groups + 2 * p.parts - 1) / max(1, 2 * p.parts));
+    const int nparts = min(s_parts, PARTS_PICKED), few = run >> 1;  // (run: 1 or 2)
+    for (int i = tid >> 4; i < nparts; i += THREADS_ / 16) {
+        const int2 part = part_of[i];
 #pragma unroll 4
-    for (int i = tid; i < nparts * longest; i += THREADS_) {
-        const int part = part_of[i / longest], e = i % longest;
-        int gi;
-        if (p.nt) {
-            const int c = part >> 2;
-            const int t0 = (int)((long long)c * p.nt / p.chunks);
-            const int t = t0 + e / p.per_part;
-            gi = t < (int)((long long)(c + 1) * p.nt / p.chunks)
-                     ? t * p.per_tile + (part & 3) * p.per_part + e % p.per_part
-                     : groups;
-        } else {
-            gi = part * 2 + (e & 1) + (e >> 1) * 2 * p.parts;
+        for (int e = tid & 15; e < part.y; e += 16) {
+            const int gi = part.x + (e >> few) * step + (e & few);
+            if (gi < groups) pick(gi, __ldg(top + gi));
         }
-        if (gi < groups) pick(gi, top[gi]);
     }
     __syncthreads();
     const int picked = s_picked;

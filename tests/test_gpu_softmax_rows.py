@@ -718,3 +718,58 @@ def test_status_of_a_call_without_work():
         ws = torch.full((1 << 20,), 255, dtype=torch.uint8, device="cuda")
         call(ws)
         fg.logprobs_status(ws)
+
+
+@pytest.mark.parametrize("dtype,nq", [("f32", 3), ("f32", 40), ("bf16", 2), ("bf16", 300)])
+def test_gradients_into_parts_of_wider_buffers(dtype, nq):
+    """Rows ld_d_* elements apart: what lies between and behind them stays."""
+    import ctypes as C
+    import forgegpu as fg
+    import torch
+    n, d, gap = 333, 41, 3
+    Q, X, T, A, *_ = make(dtype, nq, n, d, "each", seed=15)
+    r = fg.logprobs(Q, X, T, scale=0.3, allowed=A)
+    up = torch.rand(nq, device="cuda")
+    want = fg.logprobs_backward(Q, X, T, r.lse, d_logprob=up, scale=0.3, allowed=A)
+    dq = torch.full((nq + 2, d + gap), 7.0, dtype=Q.dtype, device="cuda")
+    dx = torch.full((n + 2, d + gap), 7.0, dtype=Q.dtype, device="cuda")
+    ws = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")
+    a = fg.LogprobGradArgs(
+        dtype={"f32": 0, "bf16": 2}[dtype], queries=Q.data_ptr(), nq=nq, ld_queries=d,
+        rows=X.data_ptr(), n=n, ld_rows=d, dim=d, scale=0.3, targets=T.data_ptr(),
+        allowed=A.data_ptr(), ld_allowed=A.stride(0), lse=r.lse.data_ptr(),
+        d_logprob=up.data_ptr(), d_queries=dq.data_ptr(), ld_d_queries=d + gap,
+        d_rows=dx.data_ptr(), ld_d_rows=d + gap, workspace=ws.data_ptr(),
+        workspace_bytes=ws.numel(), stream=torch.cuda.current_stream().cuda_stream)
+    assert fg.lib().fdb_logprobs_backward(fg.default_context().h, C.byref(a)) == 0
+    for got, w in ((dq, want[0]), (dx, want[1])):
+        assert torch.equal(got[:-2, :d], w)
+        assert (got[:-2, d:] == 7).all() and (got[-2:] == 7).all()
+
+
+def test_two_eager_calls_at_once():
+    """Calls on two streams, each with a workspace of its own, over the same
+    inputs: the same bits as one after the other."""
+    import forgegpu as fg
+    import torch
+    Q, X, T, A, *_ = make("f32", 300, 20000, 96, "one", seed=16)
+    up = torch.rand(300, device="cuda")
+
+    def both(q, t, u):
+        r = fg.logprobs(q, X, t, scale=0.2, allowed=A, k=9)
+        return list(r) + list(fg.logprobs_backward(q, X, t, r.lse, d_logprob=u, scale=0.2,
+                                                   allowed=A))
+
+    parts = [(Q, T, up), (Q[:5], T[:5], up[:5])]
+    want = [both(*p) for p in parts]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in parts]
+    got = [[], []]
+    for _ in range(4):
+        for i, (s, p) in enumerate(zip(streams, parts)):
+            with torch.cuda.stream(s):
+                got[i].append(both(*p))
+    torch.cuda.synchronize()
+    for w, runs in zip(want, got):
+        for g in runs:
+            assert all(torch.equal(a, b) for a, b in zip(w, g))
