@@ -1741,18 +1741,17 @@ __global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kern
     }
     if (lane == 0) red[warp] = make_float2(L, A);
     if (p.k > 0 && tid < 128) {
-        int rank = 0;
+        // (equal ones all write the same)
+        int above = 0, from = 0;
         const float mine = part_max[tid];
         const float4* all = reinterpret_cast<const float4*>(part_max);
 #pragma unroll 8
         for (int i = 0; i < 32; ++i) {
             const float4 v = all[i];
-            rank += v.x > mine || (v.x == mine && 4 * i < tid);
-            rank += v.y > mine || (v.y == mine && 4 * i + 1 < tid);
-            rank += v.z > mine || (v.z == mine && 4 * i + 2 < tid);
-            rank += v.w > mine || (v.w == mine && 4 * i + 3 < tid);
+            above += (v.x > mine) + (v.y > mine) + (v.z > mine) + (v.w > mine);
+            from += (v.x >= mine) + (v.y >= mine) + (v.z >= mine) + (v.w >= mine);
         }
-        if (rank == p.k + PAD - 1) s_bound = mine;
+        if (above < p.k + PAD && p.k + PAD <= from) s_bound = mine;
     }
     __syncthreads();
     L = A = 0.0f;
