@@ -1943,9 +1943,13 @@ __global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kern
         const double size = (double)sqrtf(qq * (float)p.d) * (double)__int_as_float(s_size);
         return !(v < kth - (fabs(v) + fabs(kth)) * 0x1p-16 - size * 0x1p-18);
     };
-    rank_all(cnt, [&](int i, int rank) {
+    const int ranked = cnt > 128 ? narrow(cnt, least_of(cnt)) : cnt;
+    const int best = min(ranked, p.k);
+    rank_all(ranked, [&](int i, int rank) {
+        if (rank < p.k) kept[rank] = cs[i], kept_id[rank] = ci[i];
         if (rank == p.k - 1) s_kth = unordered64(cs[i]);
     });
+    if (tid == 0) s_parts = best;
     __syncthreads();
     // ---- groups whose second largest score may still enter: their other rows ----
     const bool more = bound > NONE_BELOW && may_enter(bound);  // groups below the bound may
@@ -1963,10 +1967,21 @@ __global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kern
             }
         }
         __syncthreads();
-        if (s_cnt <= CAND) score(cnt, s_cnt);
+        if (s_cnt <= CAND) {
+            score(cnt, s_cnt);
+            __syncthreads();
+            // those that do, behind the best so far
+            const uint64_t least = best == p.k ? kept[p.k - 1] : 0;
+            for (int i = cnt + tid; i < s_cnt; i += THREADS_) {
+                if (cs[i] < least) continue;
+                const int at = atomicAdd(&s_parts, 1);
+                if (at < KEPT) kept[at] = cs[i], kept_id[at] = ci[i];
+            }
+        }
     }
     __syncthreads();
-    all_groups = !bad && (all_groups || more || s_cnt > CAND);
+    const int total = s_parts;
+    all_groups = !bad && (all_groups || more || s_cnt > CAND || total > KEPT);
     __syncthreads();
     if (all_groups) {
         // ---- too many groups are as good (many equal or nearly equal scores, or
@@ -2009,15 +2024,22 @@ __global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kern
         __syncthreads();
     }
     // ---- written in order ----
-    int have = bad ? 0 : s_cnt;
-    if (have > 128) have = narrow(have, least_of(have));
-    rank_all(have, [&](int i, int rank) {
-        if (rank < p.k) {
-            p.top_ids[(size_t)q * p.k + rank] = (int64_t)ci[i];
-            p.top_logprob[(size_t)q * p.k + rank] =
-                (float)(unordered64(cs[i]) * (double)p.scale - lse);
-        }
-    });
+    const int have = bad ? 0 : all_groups ? s_cnt : total;
+    auto write = [&](int rank, uint64_t score, uint32_t id) {
+        if (rank >= p.k) return;
+        p.top_ids[(size_t)q * p.k + rank] = (int64_t)id;
+        p.top_logprob[(size_t)q * p.k + rank] =
+            (float)(unordered64(score) * (double)p.scale - lse);
+    };
+    if (all_groups) {  // (at most k, ranked in the last round)
+        for (int i = tid; i < have; i += THREADS_) write(i, cs[i], ci[i]);
+    } else if (total == best) {
+        for (int i = tid; i < have; i += THREADS_) write(i, kept[i], kept_id[i]);
+    } else {
+        for (int i = tid; i < have; i += THREADS_) cs[i] = kept[i], ci[i] = kept_id[i];
+        __syncthreads();
+        rank_all(have, [&](int i, int rank) { write(rank, cs[i], ci[i]); });
+    }
     for (int i = have + tid; i < p.k; i += THREADS_) {
         p.top_ids[(size_t)q * p.k + i] = -1;
         p.top_logprob[(size_t)q * p.k + i] = bad ? NAN : -INFINITY;
