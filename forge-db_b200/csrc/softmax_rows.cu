@@ -73,8 +73,12 @@ constexpr unsigned long long DRAIN_CYCLES = 4000000ull;  // about 2 ms
 constexpr int THREADS = 640;                // 2 issuing warps, 2 idle, 16 epilogue warps
 constexpr int EPI_WARP0 = 4, EPI_WARPS = 16;
 constexpr int GROUP = 32;                   // rows whose largest scores are kept together
-constexpr int PAD = 8;                      // groups picked beyond k
-constexpr int MAX_SEL = FDB_MAX_ALTERNATIVES + PAD;
+// Groups picked beyond k: what the bound then lies below the kth score by has to
+// exceed the errors of 32-bit scores, else all groups are looked at.  Of random
+// scores 4 places are some hundred times that (8: 2048 x 131072 x 768, k = 20
+// takes 108 us instead of 99).
+constexpr int PAD = 4;
+static_assert(FDB_MAX_ALTERNATIVES + PAD <= 128, "the bound is one of 128 maxima");
 constexpr float NONE = -1e30f;              // score of a row that may not be seen
 constexpr float NONE_BELOW = -1e29f;
 constexpr float RAISE = 8.0f;               // see Run
@@ -1652,9 +1656,15 @@ __device__ __forceinline__ void dot_lanes(const T* const (&x)[ROWS],
 // One block per query: the partial triples joined, the groups that may hold
 // one of the best k picked, their rows scored exactly and ranked.
 //
-// Picking needs no sort: the (k + 8)th largest of 128 maxima over the parts
-// is a bound that at least k + 8 groups reach, and for scores in no particular
+// Picking needs no sort: the (k + PAD)th largest of 128 maxima over the parts
+// is a bound that at least k + PAD groups reach, and for scores in no particular
 // order hardly more do; only the groups of the parts that reach it are read.
+//
+// Bound by its chain of short dependent steps, half of whose time instructions
+// are issued: 13 us for one query of 10000 x 128, 99 for 2048 of 131072 x 768
+// (k = 20: some 60 rows a query gathered, 190 MB), 129 for 4096 of 262144 x 96.
+// Seven blocks of 128 threads a multiprocessor (six: 126 and 145 us; eight spill:
+// 110 and 170), one of 512 where there are fewer queries than that holds.
 template <typename T, int THREADS_>
 __global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kernel(const FinishArgs p) {
     constexpr int W = THREADS_ / 32;
