@@ -2519,8 +2519,10 @@ constexpr size_t CHUNK_BYTES = (size_t)512 << 20;  // of group maxima, of score 
 constexpr size_t BLOCKS_F32 = 128, BLOCKS_F16 = 256, BLOCKS_BF16 = 768;
 constexpr int FEW = 8;                          // queries a pass of few_kernel takes
 // f32 rows would have to be split for the tensor cores first: two passes still
-// cost less; 16-bit rows are read by them as they are.
-constexpr int FEW_F32 = 16, FEW_16 = 2, FEW_DIM = 2048;
+// cost less; 16-bit rows are read by them as they are, if their alignment lets a
+// tensor map describe them (100000 x 376, 4 queries: 54 us here, 38 there), else
+// after a copy (100000 x 374: 58 and 70, with 8 queries 79 and 69).
+constexpr int FEW_F32 = 16, FEW_16 = 2, FEW_16_COPIED = 4, FEW_DIM = 2048;
 constexpr int FEW_GRAD = 8, FEW_GRAD_DIM = 1024;  // few_grad_kernel: see there
 static size_t smem_of(bool two, bool blk, bool grad) {
     // alignment, stages, staged outputs, barriers, column factors
@@ -2690,7 +2692,10 @@ static Forward plan_forward(const Ctx& c, const fdb_logprob_args& a) {
     Forward w{};
     Carve ws(a.workspace);
     w.err = ws.take<int>(HEAD / 4);
-    w.few = a.nq <= (a.dtype == FDB_DTYPE_F32 ? FEW_F32 : FEW_16) && a.dim <= FEW_DIM;
+    w.few = a.nq <= (a.dtype == FDB_DTYPE_F32         ? FEW_F32
+                     : mappable(a.rows, a.ld_rows) ? FEW_16
+                                                   : FEW_16_COPIED) &&
+            a.dim <= FEW_DIM;
     w.packed = a.dtype == FDB_DTYPE_F32 && !w.few;
     w.kp = up(a.dim, 16);
     // (sums in blocks where whole ones would lose over 1e-6 of a score)
@@ -2807,9 +2812,11 @@ static void few_run(const Ctx& c, const fdb_logprob_args& a, const Forward& w, f
         };
         if (nq == 1) vec ? go(few_kernel<T, 1, true>, 1) : go(few_kernel<T, 1, false>, 1);
         else if (nq == 2) vec ? go(few_kernel<T, 2, true>, 2) : go(few_kernel<T, 2, false>, 2);
-        else if constexpr (sizeof(T) == 4) {  // (of 16-bit queries at most FEW_16 come here)
+        else if constexpr (sizeof(T) == 4) {
             if (nq <= 4) vec ? go(few_kernel<T, 4, true>, 4) : go(few_kernel<T, 4, false>, 4);
             else vec ? go(few_kernel<T, 8, true>, 8) : go(few_kernel<T, 8, false>, 8);
+        } else {  // (more than FEW_16: rows that would be copied, so unaligned ones)
+            go(few_kernel<T, 4, false>, 4);
         }
         FinishArgs f = finish_args(a, w, q0, nq);
         f.parts = (int)blocks;

@@ -636,6 +636,9 @@ def test_index_follows_its_changes_and_refuses():
     ("f32", 300, 4099, 128, "each", 0, 0, 10), ("f32", 257, 2050, 113, "one", 3, 1, 64),
     ("f32", 130, 2305, 129, "one", 0, 0, 5), ("f32", 520, 1, 16, "none", 0, 0, 3),
     ("f32", 18, 767, 64, "none", 0, 0, 0),
+    # 16-bit rows whose alignment has them copied: to 4 queries, and more
+    ("bf16", 4, 3001, 75, "each", 0, 0, 10), ("f16", 3, 800, 129, "one", 0, 1, 64),
+    ("bf16", 5, 1500, 131, "each", 0, 0, 5), ("f16", 4, 40, 2049, "none", 0, 0, 3),
     # the largest dimension
     ("f32", 2, 70, 16384, "none", 0, 0, 4), ("f32", 33, 400, 16384, "each", 0, 0, 4),
     ("bf16", 5, 300, 16384, "one", 0, 0, 64), ("f16", 20, 90, 16383, "none", 1, 0, 2),
