@@ -14,8 +14,10 @@ if the library is missing or no B200 is visible, calls raise ForgeGpuError.
 """
 from __future__ import annotations
 
+import array
 import collections
 import ctypes as C
+import itertools
 import os
 import threading
 
@@ -1112,27 +1114,27 @@ def adamw_step(params, grads, m, v, *, lr: float, step: int = 1, betas=(0.9, 0.9
         _refuse("params and grads must be float32, float16 or bfloat16 tensors on a GPU")
     types = [p0.dtype, g0.dtype] + ([torch.int8, torch.uint8, torch.float32, torch.float32]
                                     if eight else [torch.float32, torch.float32])
-    sizes = [t.numel() for t in params]
+    T = torch.Tensor  # (its methods mapped: a model's tensors are many)
+    sizes = list(map(T.numel, params))
     blocks = [(n + 255) // 256 for n in sizes] if eight else None
     cols = []
     for what, (ts, dtype) in enumerate(zip(lists, types)):
-        ptrs = []
-        for t, n in zip(ts, sizes if what < 4 else blocks):
-            if t.dtype != dtype or t.device != dev or t.numel() != n or not t.is_contiguous():
-                _refuse("params, grads and states must be contiguous, of one type each, of the "
-                        "params' sizes (scales: one per 256 elements) and device")
-            ptrs.append(t.data_ptr())
-        cols.append(ptrs)
+        if {t.dtype for t in ts} != {dtype} or set(map(T.get_device, ts)) != {dev.index} \
+                or list(map(T.numel, ts)) != (sizes if what < 4 else blocks) \
+                or not all(map(T.is_contiguous, ts)):
+            _refuse("params, grads and states must be contiguous, of one type each, of the "
+                    "params' sizes (scales: one per 256 elements) and device")
+        cols.append(list(map(T.data_ptr, ts)))
     if not eight:
         cols += [[0] * count] * 2
-    table = np.array(cols + [sizes], np.uint64).T.copy()
+    table = array.array("Q", itertools.chain.from_iterable(zip(*cols, sizes)))
     o = AdamwOpts(_DTYPE[p0.dtype], _DTYPE[g0.dtype], 8 if eight else 32, seed & 0xFFFFFFFF, lr,
                   betas[0], betas[1], eps, weight_decay, grad_scale, step,
                   _scalar(d_lr, torch.float32, p0, "d_lr"),
                   _scalar(d_step, torch.int64, p0, "d_step"),
                   _scalar(d_grad_scale, torch.float32, p0, "d_grad_scale"),
                   torch._C._cuda_getCurrentRawStream(dev.index))
-    _check(lib().fdb_adamw_step(_ctx_of(dev).h, table.ctypes.data, count, C.byref(o)))
+    _check(lib().fdb_adamw_step(_ctx_of(dev).h, table.buffer_info()[0], count, C.byref(o)))
 
 
 def adamw_state_values(m, m_scale, v, v_scale):
