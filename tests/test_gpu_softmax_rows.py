@@ -776,3 +776,62 @@ def test_two_eager_calls_at_once():
     for w, runs in zip(want, got):
         for g in runs:
             assert all(torch.equal(a, b) for a, b in zip(w, g))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_few_queries_captured(dtype):
+    """The passes for a few queries, with more shared memory than a kernel has
+    by default, captured before their first eager call of that size."""
+    import forgegpu as fg
+    import torch
+    Q, X, T, *_ = make(dtype, 5, 900, 1001, "none", seed=17)
+    up = torch.rand(5, device="cuda")
+
+    def run():
+        r = fg.logprobs(Q, X, T, scale=0.05, k=3)
+        return list(r) + list(fg.logprobs_backward(Q, X, T, r.lse, d_logprob=up, scale=0.05))
+
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = run()
+    X.copy_(X.flip(0).clone())
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, run()))
+
+
+@pytest.mark.parametrize("dtype,nq", [("f32", 1), ("f32", 7), ("bf16", 4), ("f16", 8)])
+@pytest.mark.parametrize("bad", BADS)
+def test_gradients_of_a_few_queries_beside_what_is_not_finite(dtype, nq, bad):
+    """What a masked row, or a query that sees nothing, holds changes no bit; a
+    row that one query may see makes that query's gradient NaN, and the others'
+    stay."""
+    import forgegpu as fg
+    import torch
+    Q, X, T, _, q, x, t, _ = make(dtype, nq, 700, 45, "none", seed=18)
+    keep = np.random.default_rng(2).random((nq, 700)) < 0.6
+    keep[:, 123] = False
+    keep[:, 400] = False
+    keep[0, 400] = True  # the first query alone
+    if nq > 2:
+        keep[2] = False
+    A = torch.from_numpy(so.words(keep)).cuda()
+    r = fg.logprobs(Q, X, T, scale=0.3, allowed=A)
+    up = torch.rand(nq, device="cuda")
+    go = lambda Q, X: fg.logprobs_backward(Q, X, T, r.lse, d_logprob=up, d_lse=up, scale=0.3,
+                                           allowed=A)
+    want = go(Q, X)
+    X1, Q1 = X.clone(), Q.clone()
+    X1[123, 4] = bad
+    if nq > 2:
+        Q1[2, 7] = bad
+    for a, b in zip(want, go(Q1, X1)):
+        assert torch.equal(a, b)
+    if np.isfinite(bad):
+        return
+    X1[400, 9] = bad
+    dq, dx = go(Q1, X1)
+    assert torch.isnan(dq[0].float()).all() and torch.equal(dq[1:], want[0][1:])
+    other = torch.arange(700, device="cuda") != 400
+    assert torch.equal(dx[other], want[1][other]) and torch.isnan(dx[400].float()).all()
