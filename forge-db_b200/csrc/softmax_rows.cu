@@ -798,7 +798,11 @@ struct GradEpilogue {
         row = r;
         al = r >= a.nq || !a.allowed ? nullptr : a.allowed + (size_t)r * a.ld_allowed;
         q = r < a.nq ? r : -1;
-        k = a.coef[q < 0 ? 0 : q];
+        // (a row past the last query has no given row: it would leave the rest of
+        // its rounding in front of p.rest)
+        k = Coef{};
+        k.target = -1;
+        if (q >= 0) k = a.coef[q];
         const float f = q < 0 ? 0.0f : a.qf[q];
         wi = f * grad_factor(a.bounds);
     }
