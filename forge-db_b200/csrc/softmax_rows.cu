@@ -2793,37 +2793,46 @@ static FinishArgs finish_args(const fdb_logprob_args& a, const Forward& w, size_
     return f;
 }
 
+// A kernel's limit is the process's, not the call's: it is set to the largest
+// size that any call takes, as two threads may launch the same kernel at once.
+template <typename T, int NQ, bool VEC>
+static void launch_few(const Ctx& c, const fdb_logprob_args& a, const Forward& w, int q0, int nq,
+                       float rf, size_t ld_allowed) {
+    const size_t smem = NQ * up(a.dim, 128) * 4;
+    if (smem > 40960) {  // (with the static part, over what needs no permission)
+        static std::atomic<uint64_t> done{0};
+        allow_smem(few_kernel<T, NQ, VEC>, c.device, NQ * up(FEW_DIM, 128) * 4, done);
+    }
+    few_kernel<T, NQ, VEC><<<(unsigned)w.parts_cap, 64, smem, static_cast<cudaStream_t>(a.stream)>>>(
+        static_cast<const T*>(a.rows), a.ld_rows, (int)a.n, (int)a.dim,
+        static_cast<const T*>(a.queries), a.ld_queries, q0, nq, rf, a.allowed, ld_allowed, w.part,
+        w.top, w.groups, w.err);
+    FDB_LAUNCH_CHECK();
+}
+template <typename T, int NQ>
+static void launch_few(bool vec, const Ctx& c, const fdb_logprob_args& a, const Forward& w, int q0,
+                       int nq, float rf, size_t ld_allowed) {
+    if (vec) launch_few<T, NQ, true>(c, a, w, q0, nq, rf, ld_allowed);
+    else launch_few<T, NQ, false>(c, a, w, q0, nq, rf, ld_allowed);
+}
 template <typename T>
 static void few_run(const Ctx& c, const fdb_logprob_args& a, const Forward& w, float rf,
                     size_t ld_allowed) {
     const cudaStream_t s = static_cast<cudaStream_t>(a.stream);
     const bool vec = (reinterpret_cast<uintptr_t>(a.rows) & 15) == 0 &&
                      a.ld_rows * sizeof(T) % 16 == 0 && a.dim * sizeof(T) % 16 == 0;
-    const size_t dp = up(a.dim, 128);
-    for (size_t q0 = 0; q0 < a.nq; q0 += w.qb) {
-        const int nq = (int)std::min(w.qb, a.nq - q0);
-        const unsigned blocks = (unsigned)w.parts_cap;
-        auto go = [&](auto kernel, int NQ) {
-            const size_t sm = NQ * dp * 4;
-            if (sm > 40960)
-                FDB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                              (int)sm));
-            kernel<<<blocks, 64, sm, s>>>(static_cast<const T*>(a.rows), a.ld_rows, (int)a.n,
-                                          (int)a.dim, static_cast<const T*>(a.queries),
-                                          a.ld_queries, (int)q0, nq, rf, a.allowed, ld_allowed,
-                                          w.part, w.top, w.groups, w.err);
-            FDB_LAUNCH_CHECK();
-        };
-        if (nq == 1) vec ? go(few_kernel<T, 1, true>, 1) : go(few_kernel<T, 1, false>, 1);
-        else if (nq == 2) vec ? go(few_kernel<T, 2, true>, 2) : go(few_kernel<T, 2, false>, 2);
+    for (size_t q = 0; q < a.nq; q += w.qb) {
+        const int nq = (int)std::min(w.qb, a.nq - q), q0 = (int)q;
+        if (nq == 1) launch_few<T, 1>(vec, c, a, w, q0, nq, rf, ld_allowed);
+        else if (nq == 2) launch_few<T, 2>(vec, c, a, w, q0, nq, rf, ld_allowed);
         else if constexpr (sizeof(T) == 4) {
-            if (nq <= 4) vec ? go(few_kernel<T, 4, true>, 4) : go(few_kernel<T, 4, false>, 4);
-            else vec ? go(few_kernel<T, 8, true>, 8) : go(few_kernel<T, 8, false>, 8);
+            if (nq <= 4) launch_few<T, 4>(vec, c, a, w, q0, nq, rf, ld_allowed);
+            else launch_few<T, 8>(vec, c, a, w, q0, nq, rf, ld_allowed);
         } else {  // (more than FEW_16: rows that would be copied, so unaligned ones)
-            go(few_kernel<T, 4, false>, 4);
+            launch_few<T, 4, false>(c, a, w, q0, nq, rf, ld_allowed);
         }
-        FinishArgs f = finish_args(a, w, q0, nq);
-        f.parts = (int)blocks;
+        FinishArgs f = finish_args(a, w, q, nq);
+        f.parts = (int)w.parts_cap;
         launch_finish<T>(s, c.device, f);
     }
 }
@@ -2973,6 +2982,17 @@ size_t backward_bytes(const Ctx& c, const fdb_logprob_grad_args& a) {
     return plan_backward(c, b).bytes;
 }
 
+template <typename T, int NQ>
+static void launch_few_grad(const Ctx& c, const Backward& w, const FewGrad<T>& p, cudaStream_t s) {
+    const size_t smem = few_grad_smem(NQ, p.d, sizeof(T));
+    if (smem > 40960) {  // (see launch_few)
+        static std::atomic<uint64_t> done{0};
+        allow_smem(few_grad_kernel<T, NQ>, c.device, few_grad_smem(NQ, FEW_GRAD_DIM, sizeof(T)),
+                   done);
+    }
+    few_grad_kernel<T, NQ><<<w.few_blocks, 256, smem, s>>>(p);
+    FDB_LAUNCH_CHECK();
+}
 template <typename T>
 static void few_backward(const Ctx& c, const fdb_logprob_grad_args& a, const Backward& w,
                          const CoefArgs& k) {
@@ -2985,18 +3005,10 @@ static void few_backward(const Ctx& c, const fdb_logprob_grad_args& a, const Bac
     p.dx = static_cast<T*>(a.d_rows), p.ld_dx = a.ld_d_rows;
     p.partial = a.d_queries ? w.dq : nullptr;
     p.err = w.err;
-    auto go = [&](auto kernel, int NQ) {
-        const size_t sm = few_grad_smem(NQ, a.dim, sizeof(T));
-        if (sm > 40960)
-            FDB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                          (int)sm));
-        kernel<<<w.few_blocks, 256, sm, s>>>(p);
-        FDB_LAUNCH_CHECK();
-    };
-    if (a.nq == 1) go(few_grad_kernel<T, 1>, 1);
-    else if (a.nq == 2) go(few_grad_kernel<T, 2>, 2);
-    else if (a.nq <= 4) go(few_grad_kernel<T, 4>, 4);
-    else go(few_grad_kernel<T, 8>, 8);
+    if (a.nq == 1) launch_few_grad<T, 1>(c, w, p, s);
+    else if (a.nq == 2) launch_few_grad<T, 2>(c, w, p, s);
+    else if (a.nq <= 4) launch_few_grad<T, 4>(c, w, p, s);
+    else launch_few_grad<T, 8>(c, w, p, s);
     if (a.d_queries)
         launch_join(s, c.sm_count, w.dq, w.few_blocks, (int)a.nq, (int)a.dim, nullptr, nullptr,
                     a.d_queries, a.ld_d_queries, a.dtype);

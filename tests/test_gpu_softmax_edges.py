@@ -101,3 +101,70 @@ def test_the_last_query_keeps_its_given_row(dtype, nq, n, dim):
             floor * nq * Q.abs().max() + (2.0 ** -25 if dtype == "f16" else 0.0)
         off = (probe[1][j].double() - want).abs()
         assert (off <= b).all(), (j, (off / b).max())
+
+
+@pytest.mark.parametrize("dtype,nq,dims", [("f32", 8, (2048, 1400)), ("bf16", 2, (2048, 64)),
+                                           ("f32", 2, (16384, 9000))])
+@pytest.mark.parametrize("backward", [False, True])
+def test_host_threads_at_once(dtype, nq, dims, backward):
+    """The same kernels, launched by four threads with two amounts of shared
+    memory: the limit that one of them needs is not taken away by another
+    between its setting and the launch."""
+    import ctypes as C
+    import threading
+
+    import forgegpu as fg
+    import torch
+    if backward:
+        dims = tuple(max(8, d // 2) for d in dims)
+    L, ctx, n, reps = fg.lib(), fg.default_context().h, 64, 8000
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    code = {"f32": 0, "bf16": 2}[dtype]
+    keep, calls, want = [], [], []
+    for i in range(4):
+        d = dims[i % 2]
+        s = torch.cuda.Stream()
+        q = torch.randn(nq, d, device="cuda", generator=gen).to(_type(dtype))
+        x = torch.randn(n, d, device="cuda", generator=gen).to(_type(dtype))
+        t = torch.arange(nq, device="cuda")
+        up = torch.rand(nq, device="cuda", generator=gen)
+        ws = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
+        r = fg.logprobs(q, x, t, scale=0.02)
+        if backward:
+            out = [torch.empty_like(q), torch.empty_like(x)]
+            a = fg.LogprobGradArgs(
+                dtype=code, queries=q.data_ptr(), nq=nq, ld_queries=d, rows=x.data_ptr(), n=n,
+                ld_rows=d, dim=d, scale=0.02, targets=t.data_ptr(), lse=r.lse.data_ptr(),
+                d_logprob=up.data_ptr(), d_queries=out[0].data_ptr(), ld_d_queries=d,
+                d_rows=out[1].data_ptr(), ld_d_rows=d, workspace=ws.data_ptr(),
+                workspace_bytes=ws.numel(), stream=s.cuda_stream)
+            want.append(fg.logprobs_backward(q, x, t, r.lse, d_logprob=up, scale=0.02))
+        else:
+            out = [torch.empty(nq, device="cuda") for _ in range(2)]
+            a = fg.LogprobArgs(
+                dtype=code, queries=q.data_ptr(), nq=nq, ld_queries=d, rows=x.data_ptr(), n=n,
+                ld_rows=d, dim=d, scale=0.02, targets=t.data_ptr(), logprob=out[0].data_ptr(),
+                lse=out[1].data_ptr(), workspace=ws.data_ptr(), workspace_bytes=ws.numel(),
+                stream=s.cuda_stream)
+            want.append(r[:2])
+        keep.append((q, x, t, up, ws, r, s, out))
+        calls.append(a)
+    torch.cuda.synchronize()
+    f = L.fdb_logprobs_backward if backward else L.fdb_logprobs
+    failed = []
+
+    def run(a):
+        for _ in range(reps):
+            if f(ctx, C.byref(a)):
+                failed.append(L.fdb_last_error())
+                return
+
+    threads = [threading.Thread(target=run, args=(a,)) for a in calls]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    for w, k in zip(want, keep):
+        assert all(torch.equal(a, b) for a, b in zip(w, k[-1]))
