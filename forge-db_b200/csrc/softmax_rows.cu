@@ -232,13 +232,24 @@ struct PackSide {
     const uint32_t* seen;
     __half* out;
     float* f;
-    unsigned* largest;   // bits of the largest f, nullable
+    unsigned* largest;   // see most_of, nullable
+    const int* weight;   // nullable
     int blocks;          // of 8 warps
     int rows;            // a warp's: 4 short ones or 1
     int wide;            // rows can be read in 16-byte vectors
 };
+// What the largest is taken of: the scales' bits, or, with weights, the exponents
+// of scale times weight, counted from 1.
+constexpr int NO_WEIGHT = -10000;
+constexpr int WEIGHT_ZERO = 1024;
+__device__ __forceinline__ unsigned most_of(const PackSide& p, int row, float f) {
+    if (!p.largest || !(f > 0.0f)) return 0u;
+    if (!p.weight) return __float_as_uint(f);
+    const int w = p.weight[row];
+    return w == NO_WEIGHT ? 0u : (unsigned)(ilogbf(f) + w + WEIGHT_ZERO);
+}
 template <typename T, int PARTS>
-__device__ __forceinline__ float pack_row(const PackSide& p, int row, int d, int kp) {
+__device__ __forceinline__ unsigned pack_row(const PackSide& p, int row, int d, int kp) {
     constexpr int V = 16 / (int)sizeof(T), NV = 4, NP = 14;
     const int lane = threadIdx.x & 31;
     const T* src = static_cast<const T*>(p.x) + (size_t)row * p.ld;
@@ -340,13 +351,13 @@ __device__ __forceinline__ float pack_row(const PackSide& p, int row, int d, int
     }
     const float r = bad ? __int_as_float(0x7fc00000) : (mx > 0.0f ? ldexpf(1.0f, -e) : 0.0f);
     if (lane == 0) p.f[row] = r;
-    return r > 0.0f ? r : 0.0f;
+    return most_of(p, row, r);
 }
 // Rows of one vector a lane at most, four at a time: a warp that waits for one
 // such row after the other has too little in flight (262144 x 96 f32: 85 us,
-// four at a time 43).  Returns the largest scale.
+// four at a time 43).
 template <typename T, int PARTS>
-__device__ __forceinline__ float pack_short(const PackSide& p, int row0, int d, int kp) {
+__device__ __forceinline__ unsigned pack_short(const PackSide& p, int row0, int d, int kp) {
     constexpr int V = 16 / (int)sizeof(T), R = 4;
     const int lane = threadIdx.x & 31, c = lane * V;
     uint4 raw[R];
@@ -359,7 +370,8 @@ __device__ __forceinline__ float pack_short(const PackSide& p, int row0, int d, 
             raw[r] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) +
                                                           (size_t)row * p.ld + c));
     }
-    float mx[R], most = 0.0f;
+    float mx[R];
+    unsigned most = 0u;
     bool bad[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -405,7 +417,7 @@ __device__ __forceinline__ float pack_short(const PackSide& p, int row0, int d, 
         }
         const float f = bad[r] ? __int_as_float(0x7fc00000) : zero ? 0.0f : ldexpf(1.0f, -e);
         if (lane == 0) p.f[row] = f;
-        if (f > 0.0f) most = fmaxf(most, f);
+        most = max(most, most_of(p, row, f));
     }
     return most;
 }
@@ -417,13 +429,13 @@ __global__ void __launch_bounds__(256)
     const bool first = (int)blockIdx.x < a.blocks;
     const PackSide& p = first ? a : b;
     const int row = (((int)blockIdx.x - (first ? 0 : a.blocks)) * 8 + (threadIdx.x >> 5)) * p.rows;
-    const float f = row >= p.n      ? 0.0f
-                    : p.rows == 4 ? pack_short<T, PARTS>(p, row, d, kp)
-                                  : pack_row<T, PARTS>(p, row, d, kp);
+    const unsigned mine = row >= p.n      ? 0u
+                          : p.rows == 4 ? pack_short<T, PARTS>(p, row, d, kp)
+                                        : pack_row<T, PARTS>(p, row, d, kp);
     if (!p.largest) return;
-    // the block's largest scale, unless it is there already
+    // the block's largest, unless it is there already
     __shared__ unsigned most[8];
-    if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = __float_as_uint(f);
+    if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = mine;
     __syncthreads();
     if (threadIdx.x == 0) {
         unsigned m = 0;
@@ -495,17 +507,21 @@ struct StatsArgs {
     float2* top;                // [nq][groups] or null, in units of t
     size_t groups;              // 32-row groups, whole column tiles
 };
-// What the score gradients of one query need (see coef_kernel).
+// What the score gradients of one query need (see coef_of).
 struct Coef {
     float rf_hi, rf_lo, l_hi, l_lo;  // t - lse in log2 units = u rf - l, in two parts each
-    float c, h, g;                   // G = p (c + h x) + g at the given row
+    float c, h, g;                   // G W = p (c + h x) + g at the given row
     int target;
+};
+// The head of the gradient's workspace, cleared by head_kernel.
+struct GradHead {
+    unsigned q_most;            // WEIGHT_ZERO + the largest exponent of qf_i B_i
+    float x_most;               // the largest xf
 };
 struct GradArgs {
     int nq, n, j0, cols;        // this chunk: rows [j0, j0 + cols)
     const Coef* coef;           // [nq]
-    const float *qf, *xf;       // 2^-e of the packed queries and rows
-    const float* bounds;        // [0] max of B_i qf_i, [1] max of xf
+    const float* xf;            // 2^-e of the packed rows, over the largest
     const uint32_t* allowed;
     size_t ld_allowed;
     size_t ldg;                 // output [parts][nqp][ldg]
@@ -514,8 +530,8 @@ struct GradArgs {
 };
 struct ProdArgs {
     int rows, cols;             // output
-    const float* f;             // 2^-e of the output's rows
-    const float* bounds;
+    const float* f;             // see out_factor
+    const GradHead* head;
     float* partial;             // [splits][rows][cols], or null: `out` is written
     int add;                    // added to `partial` instead of stored
     void* out;
@@ -523,12 +539,11 @@ struct ProdArgs {
     int dtype;
 };
 
-// C = 2^c, the common factor of the stored score gradients: the largest
-// |G| * 2^-ei * 2^-ej comes to [2^13, 2^15).
-__device__ __forceinline__ float grad_factor(const float* bounds) {
-    const float b = bounds[0], x = bounds[1];
-    if (!(b > 0.0f) || !(x > 0.0f)) return 1.0f;
-    return ldexpf(1.0f, max(-100, min(100, 13 - ilogbf(b) - ilogbf(x))));
+// What an output row is multiplied with: of the queries (no head) its own factor
+// f, of the rows 2^(most - 13) / f.  (See settle_kernel.)
+__device__ __forceinline__ float out_factor(float f, const GradHead* head) {
+    if (!head) return f;
+    return ldexpf(1.0f / f, min((int)head->q_most - WEIGHT_ZERO - 13, 120));
 }
 
 __device__ __forceinline__ uint32_t allowed_word(const uint32_t* al, size_t ld, int q, size_t col,
@@ -776,8 +791,10 @@ struct StatsEpilogue {
     }
 };
 
-// Score gradients, stored as fp16 (two parts for f32 inputs) scaled by
-// 2^-ei 2^-ej C so that both products read them as they are.
+// Score gradients, stored as fp16 (two parts for f32 inputs) scaled by 2^-ej and
+// the query's W (see settle_kernel) so that both products read them as they are.
+// One part rounds G by up to 2^-11 of it, as a result in f16 is rounded and an
+// eighth of what a bf16 one is; a second part would cost a second product each.
 template <bool TWO>
 struct GradEpilogue {
     typedef GradArgs Args;
@@ -785,7 +802,6 @@ struct GradEpilogue {
     int q, row;
     bool live;  // (rows up to a multiple of 128 are written)
     Coef k;
-    float wi;
     Columns<true, false, TWO ? 1 : 2> c;
     const uint32_t* al;
     unsigned char* stage;      // the warp's staged outputs, part 1 STAGED bytes on
@@ -803,8 +819,6 @@ struct GradEpilogue {
         k = Coef{};
         k.target = -1;
         if (q >= 0) k = a.coef[q];
-        const float f = q < 0 ? 0.0f : a.qf[q];
-        wi = f * grad_factor(a.bounds);
     }
     __device__ __forceinline__ void load(int col) {
         c.load(al, p.xf, (size_t)p.j0 + col, p.j0 + p.cols);
@@ -821,7 +835,7 @@ struct GradEpilogue {
         }
         const uint64_t rh2 = packf(k.rf_hi, k.rf_hi), rl2 = packf(k.rf_lo, k.rf_lo);
         const uint64_t lh2 = packf(-k.l_hi, -k.l_hi), ll2 = packf(-k.l_lo, -k.l_lo);
-        const uint64_t h2 = packf(k.h, k.h), c2 = packf(k.c, k.c), w2 = packf(wi, wi);
+        const uint64_t h2 = packf(k.h, k.h), c2 = packf(k.c, k.c);
         const float2* xf = reinterpret_cast<const float2*>(c.fac + 32 * h);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -831,13 +845,13 @@ struct GradEpilogue {
             const uint64_t y = add2(fma2(t, rh2, lh2), fma2(t, rl2, ll2));
             const float x0 = fmaxf(lo_of(y), -160.0f), x1 = fmaxf(hi_of(y), -160.0f);
             uint64_t g = mul2(packf(ex2(x0), ex2(x1)), fma2(packf(x0, x1), h2, c2));
-            g = mul2(g, mul2(f2, w2));
+            g = mul2(g, f2);
             u[2 * i] = lo_of(g);
             u[2 * i + 1] = hi_of(g);
         }
         const int at = k.target - (int)gcol;  // of the given row, if it is in this chunk
         if ((unsigned)at < 32u) {
-            const float add = k.g * (c.fac[32 * h + at] * wi);
+            const float add = k.g * c.fac[32 * h + at];
             float all = 0.0f;
 #pragma unroll
             for (int i = 0; i < 32; ++i)
@@ -934,7 +948,7 @@ struct ProdEpilogue {
         row = r;
         row0 = r0;
         split = sp;
-        s = !a.partial && row < a.rows ? 1.0f / (a.f[row] * grad_factor(a.bounds)) : 0.0f;
+        s = !a.partial && row < a.rows ? out_factor(a.f[row], a.head) : 0.0f;
     }
     __device__ __forceinline__ void load(int) {
         c.next[0] = 0;
@@ -2079,17 +2093,6 @@ __global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kern
 // ---------------------------------------------------------------------------
 // backward: what the products need
 // ---------------------------------------------------------------------------
-// Clears the head of the workspace and marks the queries that see anything,
-// as bits (an empty one is taken as zeros, so that what it holds cannot set
-// the scale of the others).
-__global__ void head_kernel(const float* __restrict__ lse, int nq, uint32_t* __restrict__ alive,
-                            uint32_t* __restrict__ head, int head_words) {
-    const int q = blockIdx.x * blockDim.x + threadIdx.x;
-    if (q < head_words) head[q] = 0u;
-    const bool on = q < nq && !(lse[q] == -INFINITY);
-    const unsigned b = __ballot_sync(0xffffffffu, on);
-    if ((threadIdx.x & 31) == 0 && q < nq) alive[q >> 5] = b;
-}
 // Rows some query may see: the OR of the filters, 32 words a block, 32 queries
 // at a time (latency-bound: 777 filters of 20003 rows took 15.4 us eight at a
 // time, 4.6 now).
@@ -2110,32 +2113,6 @@ __global__ void __launch_bounds__(1024)
     const size_t o = (size_t)blockIdx.x * 32 + row;
     if (lane == 0 && o < words) out[o] = r;
 }
-// The products sum over rows (or queries) whose scales 2^-e differ; the stored
-// score gradients carry the factor, so a row far below the largest would leave
-// too few bits there.  Such a row (below 2^-4 of the largest scale; also one
-// of zeros or with a NaN, whose elements are zeros) takes a larger scale and
-// is shifted down instead.  Almost none has work.
-__device__ __forceinline__ float fix_row(__half* x, float* f, int row, int width, float mx) {
-    const int lane = threadIdx.x & 31;
-    const float v = f[row];
-    float now = v;
-    if (!(mx > 0.0f)) {
-        now = 1.0f;
-    } else {
-        const float least = mx * 0x1p-4f;
-        if (v >= least) return v;
-        if (v > 0.0f) {
-            const float s = v / least;
-            __half* h = x + (size_t)row * width;
-            for (int c = lane; c < width; c += 32)
-                h[c] = __float2half_rn(__half2float(h[c]) * s);
-        }
-        now = v > 0.0f ? least : mx;
-    }
-    __syncwarp();
-    if (lane == 0) f[row] = now;
-    return now;
-}
 struct CoefArgs {
     int nq, n;
     double scale, whole;  // (whole: see cut_of)
@@ -2144,64 +2121,137 @@ struct CoefArgs {
     const uint32_t* allowed;
     size_t ld_allowed;
     Coef* out;
-    float* rest;    // nullable
-    float* bounds;  // [0]
+    float* rest;  // nullable
 };
-// G_ij = scale [ p_ij (dl - g - h (lp_ij + H)) + g 1{j = t} ] with lp = ln2 x:
-// = p (c + h' x) + g', and a bound of its size for the common scale
-// (p |lp| <= 1/e).
-__device__ __forceinline__ Coef coef_of(const CoefArgs& a, int i, float f, float& bound) {
-    const float lse = a.lse[i];
-    const bool empty = lse == -INFINITY;
-    const double rf = (double)f * a.scale * LOG2E * a.whole, l = (double)lse * LOG2E;
+// What reaches a query's scores, and a bound B of its G's size (p |lp| <= 1/e).
+struct Upstream {
+    double dl, g, dh, H;
+    int target;
+    bool empty;
+    float bound;
+};
+__device__ __forceinline__ Upstream upstream_of(const CoefArgs& a, int i) {
+    Upstream u;
+    u.empty = a.lse[i] == -INFINITY;
     const int64_t t = a.targets ? a.targets[i] : -1;
-    const bool given = !empty && t >= 0 && t < a.n &&
+    const bool given = !u.empty && t >= 0 && t < a.n &&
                        (!a.allowed ||
                         (a.allowed[(size_t)i * a.ld_allowed + (size_t)(t >> 5)] >> (t & 31) & 1u));
-    const double g = given && a.d_logprob ? a.d_logprob[i] : 0.0;
-    const double dl = !empty && a.d_lse ? a.d_lse[i] : 0.0;
-    const double dh = !empty && a.d_entropy ? a.d_entropy[i] : 0.0;
-    const double H = dh != 0.0 ? (double)a.entropy[i] : 0.0;
+    u.g = given && a.d_logprob ? a.d_logprob[i] : 0.0;
+    u.dl = !u.empty && a.d_lse ? a.d_lse[i] : 0.0;
+    u.dh = !u.empty && a.d_entropy ? a.d_entropy[i] : 0.0;
+    u.H = u.dh != 0.0 ? (double)a.entropy[i] : 0.0;
+    u.target = given ? (int)t : -1;
+    u.bound = (float)(a.scale * (fabs(u.dl) + 2.0 * fabs(u.g) + fabs(u.dh) * (fabs(u.H) + 1.0)));
+    return u;
+}
+// G_ij = scale [ p_ij (dl - g - h (lp_ij + H)) + g 1{j = t} ] with lp = ln2 x:
+// = p (c + h' x) + g'; times w.  f: a score over its sum of packed products.
+__device__ __forceinline__ Coef coef_of(const CoefArgs& a, int i, double f, double w) {
+    const Upstream u = upstream_of(a, i);
+    const float lse = a.lse[i];
+    const double rf = f * a.scale * LOG2E * a.whole, l = (double)lse * LOG2E;
     Coef k;
     k.rf_hi = (float)rf;
     k.rf_lo = (float)(rf - (double)k.rf_hi);
-    k.l_hi = empty ? INFINITY : (float)l;
-    k.l_lo = empty ? 0.0f : (float)(l - (double)k.l_hi);
-    k.c = lse == lse ? (float)(a.scale * (dl - g - dh * H)) : NAN;
-    k.h = (float)(-a.scale * dh * LN2);
-    k.g = (float)(a.scale * g);
-    k.target = given ? (int)t : -1;
-    bound = (float)(a.scale * (fabs(dl) + 2.0 * fabs(g) + fabs(dh) * (fabs(H) + 1.0)) * (double)f);
+    k.l_hi = u.empty ? INFINITY : (float)l;
+    k.l_lo = u.empty ? 0.0f : (float)(l - (double)k.l_hi);
+    k.c = lse == lse ? (float)(a.scale * w * (u.dl - u.g - u.dh * u.H)) : NAN;
+    k.h = (float)(-a.scale * w * u.dh * LN2);
+    k.g = (float)(a.scale * w * u.g);
+    k.target = u.target;
     return k;
 }
-// One warp per row of either operand: its scale settled, and per query its
-// coefficients.  Queries come first.
+// Clears the head of the workspace, marks the queries that see anything, as bits
+// (an empty one is taken as zeros, so that what it holds cannot set the scale of
+// the others), and leaves the exponent of each query's B.
+__global__ void head_kernel(const CoefArgs a, uint32_t* __restrict__ alive,
+                            int* __restrict__ weight, uint32_t* __restrict__ head,
+                            int head_words) {
+    const int q = blockIdx.x * blockDim.x + threadIdx.x;
+    if (q < head_words) head[q] = 0u;
+    bool on = false;
+    if (q < a.nq) {
+        const Upstream u = upstream_of(a, q);
+        on = !u.empty;
+        weight[q] = u.bound > 0.0f && u.bound <= FLT_MAX ? max(-100, min(100, ilogbf(u.bound)))
+                                                         : NO_WEIGHT;
+    }
+    const unsigned b = __ballot_sync(0xffffffffu, on);
+    if ((threadIdx.x & 31) == 0 && q < a.nq) alive[q >> 5] = b;
+}
+// The scales of what is stored.  With rows x_j = 2^-ej xp_j and queries
+// q_i = 2^-ei qp_i (packed), X the largest 2^-ej and f_j = 2^-ej / X:
+//
+//   G'_ij = G_ij f_j W_i,   W_i = 2^13 / B_i to a power of two
+//   d_queries_i = X / W_i sum_j G'_ij xp_j
+//   d_rows_j = M 2^-13 / f_j sum_i G'_ij qs_i,   qs_i = qp_i 2^-ei B_i / M
+//
+// M the largest 2^-ei B_i.  Every query's largest |G'| comes to [2^13, 2^15)
+// whatever the others' upstream gradients are (with one factor for all, a query
+// with 1e-6 of the largest had its d_queries off by 4e-3 of themselves in f32);
+// d_rows' sums, over queries, hold the terms of each to fp16's least step in the
+// scale of the largest, 2^-37 of it.
+//
+// A row far below the largest would leave too few bits in G'.  Such a row (below
+// 2^-4 of the largest scale) takes a larger one and is shifted down instead;
+// rows of zeros or with a NaN, whose elements are zeros, take any.  Almost none
+// has work.  One warp per query: its copy qs, its coefficients; one per 32 rows.
 __global__ void __launch_bounds__(256)
-    settle_kernel(const CoefArgs a, __half* qp, float* qf, __half* xp, float* xf, int width,
-                  int qblocks) {
+    settle_kernel(const CoefArgs a, const __half* __restrict__ qp, const float* __restrict__ qf,
+                  const int* __restrict__ weight, __half* __restrict__ qs,
+                  float* __restrict__ out_f, __half* __restrict__ xp, float* __restrict__ xf,
+                  int kp, int parts, int qblocks, const GradHead* __restrict__ head) {
+    const int lane = threadIdx.x & 31;
+    const float mx = head->x_most;
+    const int lx = mx > 0.0f ? ilogbf(mx) : 0;
     if ((int)blockIdx.x < qblocks) {
         const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
         if (row >= a.nq) return;
-        const float f = fix_row(qp, qf, row, width, a.bounds[2]);
-        if ((threadIdx.x & 31) == 0) {
-            float b;
-            a.out[row] = coef_of(a, row, f, b);
+        const float f = qf[row];
+        const bool none = weight[row] == NO_WEIGHT;
+        const int e = none ? 13 : weight[row];
+        if (lane == 0) {
+            a.out[row] = coef_of(a, row, ldexp((double)f, lx), ldexp(1.0, 13 - e));
+            out_f[row] = ldexpf(1.0f, min(lx - 13 + e, 127));
             if (a.rest) a.rest[row] = 0.0f;
-            if (b > 0.0f && b <= FLT_MAX)
-                atomicMax(reinterpret_cast<unsigned*>(a.bounds), __float_as_uint(b));
+        }
+        const float s = none || !(f > 0.0f)
+                            ? 0.0f
+                            : ldexpf(1.0f, ilogbf(f) + e + WEIGHT_ZERO - (int)head->q_most);
+        const size_t at = (size_t)row * (size_t)(parts * kp);
+        for (int c = lane * 8; c < kp; c += 256) {
+            __align__(16) __half hi[8], lo[8];
+            *reinterpret_cast<uint4*>(hi) = *reinterpret_cast<const uint4*>(qp + at + c);
+            if (parts == 2)
+                *reinterpret_cast<uint4*>(lo) = *reinterpret_cast<const uint4*>(qp + at + kp + c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float v = __half2float(hi[i]) * s;
+                if (parts == 2) v = __fmaf_rn(__half2float(lo[i]), s, v);
+                hi[i] = __float2half_rn(v);
+                lo[i] = __float2half_rn(v - __half2float(hi[i]));
+            }
+            *reinterpret_cast<uint4*>(qs + at + c) = *reinterpret_cast<const uint4*>(hi);
+            if (parts == 2)
+                *reinterpret_cast<uint4*>(qs + at + kp + c) = *reinterpret_cast<const uint4*>(lo);
         }
         return;
     }
-    // rows: a lane looks at one, the warp mends those that need it
+    // rows: a lane looks at one, the warp shifts those that need it
     const int row0 = (((int)blockIdx.x - qblocks) * 8 + (threadIdx.x >> 5)) * 32;
-    const int row = row0 + (threadIdx.x & 31);
-    const float mx = a.bounds[1];
-    unsigned todo = __ballot_sync(
-        0xffffffffu, row < a.n && !(mx > 0.0f && xf[row < a.n ? row : 0] >= mx * 0x1p-4f));
+    const int row = row0 + lane;
+    const float least = mx * 0x1p-4f, v = row < a.n ? xf[row] : 0.0f;
+    const bool small = v > 0.0f && v < least;
+    unsigned todo = __ballot_sync(0xffffffffu, small);
     while (todo) {
-        fix_row(xp, xf, row0 + __ffs(todo) - 1, width, mx);
+        const int r = __ffs(todo) - 1, width = parts * kp;
+        const float s = __shfl_sync(0xffffffffu, v, r) / least;
+        __half* h = xp + (size_t)(row0 + r) * width;
+        for (int c = lane; c < width; c += 32) h[c] = __float2half_rn(__half2float(h[c]) * s);
         todo &= todo - 1;
     }
+    if (row < a.n) xf[row] = !(v > 0.0f) ? 1.0f : small ? 0x1p-4f : ldexpf(v, -lx);
 }
 // d_queries of 16-bit inputs: rest[r] times the given row is added (see GRAD).
 struct JoinRest {
@@ -2217,14 +2267,13 @@ struct JoinRest {
 template <int TURNS>
 __global__ void __launch_bounds__(256)
     join_kernel(const float* __restrict__ partial, int splits, int rows, int cols,
-                const float* __restrict__ f, const float* __restrict__ bounds, void* out,
+                const float* __restrict__ f, const GradHead* __restrict__ head, void* out,
                 size_t ldo, int dtype, const JoinRest rest) {
     constexpr int LANES = 256 / TURNS;
     __shared__ float4 part[TURNS][LANES];
     const unsigned per4 = (unsigned)(cols + 3) / 4;
     const size_t plane = (size_t)rows * cols, all = (size_t)rows * per4;
     const bool wide = (cols & 3) == 0;
-    const float c = f ? grad_factor(bounds) : 1.0f;
     const int lane = threadIdx.x % LANES, turn = threadIdx.x / LANES;
     for (size_t i0 = (size_t)blockIdx.x * LANES; i0 < all; i0 += (size_t)gridDim.x * LANES) {
         const size_t i = i0 + lane;
@@ -2268,7 +2317,7 @@ __global__ void __launch_bounds__(256)
                     if (k + 3 < cols) v.w = __fmaf_rn(g, __half2float(x[3]), v.w);
                 }
             }
-            const float s = f ? 1.0f / (f[r] * c) : 1.0f;
+            const float s = f ? out_factor(f[r], head) : 1.0f;
             const float o[4] = {v.x * s, v.y * s, v.z * s, v.w * s};
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -2278,13 +2327,13 @@ __global__ void __launch_bounds__(256)
     }
 }
 static void launch_join(cudaStream_t s, int sms, const float* partial, int splits, int rows,
-                        int cols, const float* f, const float* bounds, void* out, size_t ldo,
+                        int cols, const float* f, const GradHead* head, void* out, size_t ldo,
                         int dtype, const JoinRest& rest = JoinRest{}) {
     if (splits >= 16)
-        join_kernel<8><<<sms * 8, 256, 0, s>>>(partial, splits, rows, cols, f, bounds, out, ldo,
+        join_kernel<8><<<sms * 8, 256, 0, s>>>(partial, splits, rows, cols, f, head, out, ldo,
                                                dtype, rest);
     else
-        join_kernel<1><<<sms * 8, 256, 0, s>>>(partial, splits, rows, cols, f, bounds, out, ldo,
+        join_kernel<1><<<sms * 8, 256, 0, s>>>(partial, splits, rows, cols, f, head, out, ldo,
                                                dtype, rest);
     FDB_LAUNCH_CHECK();
 }
@@ -2347,8 +2396,7 @@ __global__ void __launch_bounds__(256, few_per_sm(NQ)) few_grad_kernel(const Few
         qs[j * dp + few_at(c)] = v;
     }
     if (tid < p.nq) {
-        float bound;
-        co[tid] = coef_of(p.coef, tid, 1.0f, bound);
+        co[tid] = coef_of(p.coef, tid, 1.0, 1.0);
     }
     __syncthreads();
     // what a query that sees nothing holds does not count, an infinity or NaN of
@@ -2513,7 +2561,7 @@ __global__ void void_kernel(const int* err, void* dq, size_t ldq, int nq, void* 
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-constexpr size_t HEAD = 256;                    // error word, bounds
+constexpr size_t HEAD = 256;                    // error word, GradHead
 constexpr size_t CHUNK_BYTES = (size_t)512 << 20;  // of group maxima, of score gradients
 // dims above which a score's sum is taken in blocks: 2048 x 131072 x 768 bf16
 // takes 284 us with whole sums, so they stay while the loss is below 1e-6.
@@ -2658,7 +2706,7 @@ struct Carve {
 
 static PackSide pack_side(const void* x, size_t ld, size_t n, size_t dim, int dtype,
                           const uint32_t* seen, __half* out, float* f, unsigned* largest) {
-    PackSide p;
+    PackSide p{};
     p.x = x, p.ld = ld, p.n = (int)n, p.seen = seen, p.out = out, p.f = f, p.largest = largest;
     const size_t es = elem(dtype);
     p.wide = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ld * es & 15) == 0 &&
@@ -2927,9 +2975,10 @@ struct Backward {
     int bn, q_splits, x_splits;
     size_t bytes;
     int* err;
-    float* bounds;
-    __half *qp, *xp, *gr;
-    float *qf, *xf, *dq, *dx;
+    GradHead* head;
+    __half *qp, *qs, *xp, *gr;
+    float *qf, *xf, *out_f, *dq, *dx;
+    int* weight;
     Coef* coef;
     float* rest;
     uint32_t *seen, *alive;
@@ -2961,11 +3010,14 @@ static Backward plan_backward(const Ctx& c, const fdb_logprob_grad_args& a) {
                              c.sm_count, w.parts == 2, (double)w.cols * a.dim * 4);
     unsigned char* head = ws.take<unsigned char>(HEAD);
     w.err = reinterpret_cast<int*>(head);
-    w.bounds = reinterpret_cast<float*>(head ? head + 64 : nullptr);
+    w.head = reinterpret_cast<GradHead*>(head ? head + 64 : nullptr);
     w.qp = ws.take<__half>(a.nq * w.parts * w.kp);
+    w.qs = ws.take<__half>(a.nq * w.parts * w.kp);
     w.xp = ws.take<__half>(a.n * w.parts * w.kp);
     w.qf = ws.take<float>(a.nq);
     w.xf = ws.take<float>(up(a.n, MAX_BN) + MAX_BN);
+    w.out_f = ws.take<float>(a.nq);
+    w.weight = ws.take<int>(a.nq);
     w.coef = ws.take<Coef>(a.nq);
     if (w.parts == 1) w.rest = ws.take<float>(a.nq);
     w.gr = ws.take<__half>((size_t)w.parts * w.nqp * w.ldg);
@@ -3030,7 +3082,14 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
     }
     const int n = (int)a.n, d = (int)a.dim, nq = (int)a.nq;
     const size_t ld_allowed = a.allowed ? a.ld_allowed : 0;
-    head_kernel<<<(nq + 255) / 256, 256, 0, s>>>(a.lse, nq, w.alive,
+    CoefArgs k{};
+    k.nq = nq, k.n = n, k.scale = a.scale;
+    k.whole = 1.0 + cut_of(false, a.dim, w.parts == 2 ? 4 * kblock_of(true, true) : 0);
+    k.lse = a.lse, k.entropy = a.entropy;
+    k.d_logprob = a.d_logprob, k.d_lse = a.d_lse, k.d_entropy = a.d_entropy;
+    k.targets = a.targets, k.allowed = a.allowed, k.ld_allowed = ld_allowed;
+    k.out = w.coef, k.rest = w.rest;
+    head_kernel<<<(nq + 255) / 256, 256, 0, s>>>(k, w.alive, w.weight,
                                                  reinterpret_cast<uint32_t*>(w.err), HEAD / 4);
     FDB_LAUNCH_CHECK();
     const uint32_t* seen = a.allowed;
@@ -3041,22 +3100,17 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
         FDB_LAUNCH_CHECK();
         seen = w.seen;
     }
-    launch_pack(s, a.dtype,
-                pack_side(a.queries, a.ld_queries, a.nq, a.dim, a.dtype, w.alive, w.qp, w.qf,
-                          reinterpret_cast<unsigned*>(w.bounds + 2)),
+    PackSide qside = pack_side(a.queries, a.ld_queries, a.nq, a.dim, a.dtype, w.alive, w.qp, w.qf,
+                               &w.head->q_most);
+    qside.weight = w.weight;
+    launch_pack(s, a.dtype, qside,
                 pack_side(a.rows, a.ld_rows, a.n, a.dim, a.dtype, seen, w.xp, w.xf,
-                          reinterpret_cast<unsigned*>(w.bounds + 1)),
+                          reinterpret_cast<unsigned*>(&w.head->x_most)),
                 a.dim, w.kp, nullptr);
-    CoefArgs k{};
-    k.nq = nq, k.n = n, k.scale = a.scale;
-    k.whole = 1.0 + cut_of(false, a.dim, w.parts == 2 ? 4 * kblock_of(true, true) : 0);
-    k.lse = a.lse, k.entropy = a.entropy;
-    k.d_logprob = a.d_logprob, k.d_lse = a.d_lse, k.d_entropy = a.d_entropy;
-    k.targets = a.targets, k.allowed = a.allowed, k.ld_allowed = ld_allowed;
-    k.out = w.coef, k.rest = w.rest, k.bounds = w.bounds;
     const int qblocks = (nq + 7) / 8;
-    settle_kernel<<<qblocks + (n + 255) / 256, 256, 0, s>>>(k, w.qp, w.qf, w.xp, w.xf,
-                                                            w.parts * (int)w.kp, qblocks);
+    settle_kernel<<<qblocks + (n + 255) / 256, 256, 0, s>>>(k, w.qp, w.qf, w.weight, w.qs, w.out_f,
+                                                            w.xp, w.xf, (int)w.kp, w.parts, qblocks,
+                                                            w.head);
     FDB_LAUNCH_CHECK();
 
     const size_t width = w.parts * w.kp;
@@ -3064,7 +3118,7 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
     const int mtq = (int)((a.nq + PM - 1) / PM), ntd = (d + w.bn - 1) / w.bn;
     const CUtensorMap qk = map2d(FDB_DTYPE_F16, w.qp, width, a.nq, width, BM);
     const CUtensorMap xk = map2d(FDB_DTYPE_F16, w.xp, width, a.n, width, w.bn / 2);
-    const CUtensorMap qm = map2d(FDB_DTYPE_F16, w.qp, width, a.nq, width, 64);
+    const CUtensorMap qm = map2d(FDB_DTYPE_F16, w.qs, width, a.nq, width, 64);
     const CUtensorMap xm = map2d(FDB_DTYPE_F16, w.xp, width, a.n, width, 64);
     const size_t g_rows = w.parts * w.nqp;
     const CUtensorMap gk = map2d(FDB_DTYPE_F16, w.gr, w.ldg, g_rows, w.ldg, BM);
@@ -3090,7 +3144,7 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
             g.idesc = idesc_of(FDB_DTYPE_F16, false, false);
             GradArgs p{};
             p.nq = nq, p.n = n, p.j0 = (int)j0, p.cols = cols;
-            p.coef = w.coef, p.qf = w.qf, p.xf = w.xf, p.bounds = w.bounds;
+            p.coef = w.coef, p.xf = w.xf;
             p.allowed = a.allowed, p.ld_allowed = ld_allowed;
             p.ldg = w.ldg, p.nqp = (int)w.nqp, p.rest = w.rest;
             launch_rows<GRAD>(two, s, c.device, c.sm_count, qk, xk, g, p, &go);
@@ -3106,7 +3160,7 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
             g.ncols = d;
             g.idesc = idesc_of(FDB_DTYPE_F16, false, true);
             ProdArgs p{};
-            p.rows = nq, p.cols = d, p.f = w.qf, p.bounds = w.bounds;
+            p.rows = nq, p.cols = d, p.f = w.out_f;
             p.partial = w.dq, p.add = j0 > 0;
             launch_rows<PROD_Q>(two, s, c.device, c.sm_count, gk, xm, g, p);
         }
@@ -3121,18 +3175,18 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
             unsigned char* out =
                 static_cast<unsigned char*>(a.d_rows) + j0 * a.ld_d_rows * elem(a.dtype);
             ProdArgs p{};
-            p.rows = cols, p.cols = d, p.f = w.xf + j0, p.bounds = w.bounds;
+            p.rows = cols, p.cols = d, p.f = w.xf + j0, p.head = w.head;
             p.partial = w.dx;
             p.out = out, p.ldo = a.ld_d_rows, p.dtype = a.dtype;
             launch_rows<PROD_X>(two, s, c.device, c.sm_count, gm, qm, g, p);
             if (w.dx) {
-                launch_join(s, c.sm_count, w.dx, w.x_splits, cols, d, w.xf + j0, w.bounds, out,
+                launch_join(s, c.sm_count, w.dx, w.x_splits, cols, d, w.xf + j0, w.head, out,
                             a.ld_d_rows, a.dtype);
             }
         }
     }
     if (a.d_queries) {
-        launch_join(s, c.sm_count, w.dq, w.q_splits, nq, d, w.qf, w.bounds, a.d_queries,
+        launch_join(s, c.sm_count, w.dq, w.q_splits, nq, d, w.out_f, nullptr, a.d_queries,
                     a.ld_d_queries, a.dtype, JoinRest{w.rest, w.coef, w.xp, (int)width});
     }
     void_kernel<<<c.sm_count, 256, 0, s>>>(w.err, a.d_queries, a.ld_d_queries, nq, a.d_rows,

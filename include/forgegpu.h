@@ -509,7 +509,10 @@ int fdb_logprobs(fdb_ctx* ctx, const fdb_logprob_args* args);
  * in the type of the inputs, rows ld_d_* elements apart, overwritten; either
  * may be NULL.  entropy may be NULL without d_entropy.  A target that is not
  * allowed has no gradient.  Sums are taken in a fixed order: the same call
- * gives the same bits. */
+ * gives the same bits.  d_queries of a query is held to its own size, whatever
+ * the other queries' upstream gradients are.  d_rows are sums over the queries,
+ * each held to the largest query's upstream gradient times its size: what a
+ * query adds is off by up to 2^-37 of that. */
 typedef struct fdb_logprob_grad_args {
     int dtype;
     const void* queries;

@@ -168,3 +168,95 @@ def test_host_threads_at_once(dtype, nq, dims, backward):
     assert not failed, failed
     for w, k in zip(want, keep):
         assert all(torch.equal(a, b) for a, b in zip(w, k[-1]))
+
+
+def _gradient(q, x, t, scale, keep, lse, ent, up):
+    """softmax_oracle.backward and the size of its terms on GPU tensors (f64)."""
+    import torch
+    s = q @ x.T * scale
+    if keep is not None:
+        s = s.masked_fill(~keep, -float("inf"))
+    some = lse > -float("inf")
+    lp = s - torch.where(some, lse, 0.0)[:, None]
+    p = torch.where(some[:, None], lp.exp(), 0.0)
+    lp = torch.where(p > 0, lp, 0.0)
+    i = torch.arange(len(t), device="cuda")
+    ok = (t >= 0) & some
+    ok &= s[i, t.clamp_min(0)] > -float("inf")
+    dlp, dl, dh = up
+    g = torch.where(ok, dlp, 0.0)
+    e = torch.where(some, ent, 0.0)
+    G = p * ((dl - g)[:, None] - dh[:, None] * (lp + e[:, None]))
+    size = p * ((dl.abs() + g.abs())[:, None] + dh.abs()[:, None] * (lp.abs() + e.abs()[:, None] + 1))
+    G[i[ok], t[ok]] += g[ok]
+    size[i[ok], t[ok]] += g[ok].abs()
+    return G * scale, size * scale
+
+
+@pytest.mark.parametrize("dtype,nq,n,dim,mask", [
+    ("f32", 64, 20000, 64, False), ("f32", 300, 3001, 33, True), ("f32", 17, 500, 200, False),
+    ("bf16", 64, 20000, 64, False), ("bf16", 130, 1500, 129, True),
+])
+@pytest.mark.parametrize("which", ["d_logprob", "d_lse", "all"])
+def test_upstream_gradients_of_many_sizes(dtype, nq, n, dim, mask, which):
+    """Upstream gradients from 1e-8 to 1 of the largest: each query's d_queries
+    within the bound that its own upstream gradient gives.  G is held down to
+    2^-25 with its bound at 2^13 or above, rows down to 2^-4 of the largest
+    scale enlarge that: 2^-33 of the query's own largest for each row."""
+    import forgegpu as fg
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(nq)
+    q = torch.randn(nq, dim, device="cuda", generator=gen).to(_type(dtype))
+    x = torch.randn(n, dim, device="cuda", generator=gen).to(_type(dtype))
+    t = torch.randint(-1, n, (nq,), device="cuda", generator=gen)
+    keep = words = None
+    if mask:
+        keep = torch.rand(nq, n, device="cuda", generator=gen) < 0.4
+        keep[3] = False
+        words = torch.from_numpy(so.words(keep.cpu().numpy())).cuda()
+    scale = float(np.float32(1.5 / np.sqrt(dim)))
+    r = fg.logprobs(q, x, t, scale=scale, allowed=words)
+    w = 10.0 ** -(torch.arange(nq, device="cuda") % 9).float()
+    up = torch.randn(3, nq, device="cuda", generator=gen) * w
+    if which != "all":
+        up[[i for i, k in enumerate(("d_logprob", "d_lse", "d_entropy")) if k != which]] = 0.0
+    dq, dx = fg.logprobs_backward(q, x, t, r.lse, r.entropy, d_logprob=up[0], d_lse=up[1],
+                                  d_entropy=up[2], scale=scale, allowed=words)
+    Q, X = q.double(), x.double()
+    G, size = _gradient(Q, X, t, scale, keep, r.lse.double(), r.entropy.double(), up.double())
+    e = size * (_score_off(Q, X, scale, dtype) + 2.0 ** -19 + _held(dtype))
+    own = size.amax(1)
+    want = G @ X
+    b = e @ X.abs() + size @ X.abs() * _cut(dtype, n) + HALF[dtype] * want.abs() + \
+        own[:, None] * 2.0 ** -33 * n * X.abs().max()
+    off = (dq.double() - want).abs()
+    assert (off <= b + 1e-35).all(), (off / (b + 1e-35)).max()
+    want = G.T @ Q
+    b = e.T @ Q.abs() + size.T @ Q.abs() * _cut(dtype, nq) + HALF[dtype] * want.abs() + \
+        own.max() * 2.0 ** -33 * nq * Q.abs().max()
+    off = (dx.double() - want).abs()
+    assert (off <= b + 1e-35).all(), (off / (b + 1e-35)).max()
+    # what another query's upstream gradient is does not change a bit
+    up2 = up.clone()
+    up2[:, 0] *= 2.0 ** 20
+    dq2, _ = fg.logprobs_backward(q, x, t, r.lse, r.entropy, d_logprob=up2[0], d_lse=up2[1],
+                                  d_entropy=up2[2], scale=scale, allowed=words)
+    assert torch.equal(dq[1:], dq2[1:])
+
+
+@pytest.mark.parametrize("dtype,shift", [("f32", 100), ("f32", -100), ("bf16", 90), ("bf16", -90)])
+def test_gradients_of_very_large_and_small_operands(dtype, shift):
+    """Rows of size 2^shift and queries of 2^-shift: the scores are those of
+    both at 1, the gradients are scaled by the powers of two."""
+    import forgegpu as fg
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.randn(40, 48, device="cuda", generator=gen).to(_type(dtype))
+    x = torch.randn(700, 48, device="cuda", generator=gen).to(_type(dtype))
+    t = torch.randint(-1, 700, (40,), device="cuda", generator=gen)
+    r = fg.logprobs(q, x, t, scale=0.2)
+    up = torch.randn(40, device="cuda", generator=gen)
+    dq, dx = fg.logprobs_backward(q, x, t, r.lse, d_logprob=up, scale=0.2)
+    two = 2.0 ** shift
+    eq, ex = fg.logprobs_backward(q / two, x * two, t, r.lse, d_logprob=up, scale=0.2)
+    assert torch.equal(eq, dq * two) and torch.equal(ex, dx / two)
