@@ -1905,17 +1905,18 @@ __global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kern
         }
     }
     __syncthreads();
-    // the row whose log probability is asked for comes last
-    int cnt = s_cnt;
-    if (tid == 0) ci[cnt] = given ? (uint32_t)target : 0u;
+    // the row whose log probability is asked for comes last (a row that the query
+    // may not see is not looked at: what it holds would count as a candidate's size)
+    const int cnt = s_cnt;
+    const bool last = given && seen((uint32_t)target);
+    if (tid == 0 && last) ci[cnt] = (uint32_t)target;
     __syncthreads();
-    if (given || cnt > 0) score(0, cnt + 1);
+    if (cnt + last > 0) score(0, cnt + last);
     __syncthreads();
     if (tid == 0 && p.logprob) {
         float v = bad ? NAN : 0.0f;
         if (given && !bad)
-            v = none || !seen((uint32_t)target) ? -INFINITY
-                                                : (float)(unordered64(cs[cnt]) * (double)p.scale - lse);
+            v = last ? (float)(unordered64(cs[cnt]) * (double)p.scale - lse) : -INFINITY;
         p.logprob[q] = v;
     }
     if (p.k == 0) return;

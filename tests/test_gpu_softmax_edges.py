@@ -260,3 +260,39 @@ def test_gradients_of_very_large_and_small_operands(dtype, shift):
     two = 2.0 ** shift
     eq, ex = fg.logprobs_backward(q / two, x * two, t, r.lse, d_logprob=up, scale=0.2)
     assert torch.equal(eq, dq * two) and torch.equal(ex, dx / two)
+
+
+@pytest.mark.parametrize("dtype,nq,dim", [("f32", 1, 768), ("f32", 300, 96), ("bf16", 300, 128),
+                                          ("f16", 2, 256)])
+@pytest.mark.parametrize("bad", [float("inf"), 6e4])
+@pytest.mark.parametrize("targets", [False, True])
+def test_a_row_that_is_not_seen_takes_no_part(dtype, nq, dim, bad, targets):
+    """A masked row, the first one or the given one, that holds an infinity or
+    something large: the same bits, and no more work, than beside zeros (the
+    alternatives of every query would be looked for in all rows if it counted
+    for the size of the scores' errors: some hundred times the work)."""
+    import forgegpu as fg
+    import torch
+    n = 200000
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    q = torch.randn(nq, dim, device="cuda", generator=gen).to(_type(dtype))
+    x = torch.randn(n, dim, device="cuda", generator=gen).to(_type(dtype))
+    keep = torch.ones(1, n, dtype=torch.bool)
+    keep[0, :2] = False
+    words = torch.from_numpy(so.words(keep.numpy())).cuda()
+    t = torch.ones(nq, dtype=torch.int64, device="cuda") if targets else None
+    out, times = [], []
+    for value in (0.0, bad):
+        x[:2] = value
+        ev = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+        for _ in range(3):
+            r = fg.logprobs(q, x, t, scale=0.1, allowed=words, k=10)
+        ev[0].record()
+        for _ in range(5):
+            r = fg.logprobs(q, x, t, scale=0.1, allowed=words, k=10)
+        ev[1].record()
+        torch.cuda.synchronize()
+        out.append(r)
+        times.append(ev[0].elapsed_time(ev[1]))
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+    assert times[1] < 3 * times[0], times
