@@ -17,7 +17,7 @@
 // could still enter is scored in full, as are all groups if one that was not
 // picked could.
 // Which ids are returned therefore does not depend on the order of a 32-bit
-// sum; equal scores go to the lower id.
+// sum (but see may_enter); equal scores go to the lower id.
 //
 // Types: 16-bit rows go to the MMA as they are.  f32 rows are split once into
 // two fp16 parts of the row scaled by a power of two, x 2^e = hi + lo
@@ -506,6 +506,7 @@ struct StatsArgs {
     float4* part;               // [chunks * 4][nq]: m, l, a (see Run)
     float2* top;                // [nq][groups] or null, in units of t
     size_t groups;              // 32-row groups, whole column tiles
+    float* size;                // [blocks] largest xf, with f32 rows and top
 };
 // What the score gradients of one query need (see coef_of).
 struct Coef {
@@ -1266,6 +1267,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 }
             }
         }
+    } else if (warp == 2) {
+        // (else idle) the largest factor of the rows that a shared filter lets see,
+        // all rows with filters of their own
+        if constexpr (MODE == STATS && TWO) {
+            if (p.size) {
+                const uint32_t* al = p.ld_allowed ? nullptr : p.allowed;
+                float m = 0.0f;
+                for (int j = blockIdx.x * 32 + lane; j < p.n; j += gridDim.x * 32)
+                    if (!al || (__ldg(al + (j >> 5)) >> lane & 1u)) m = fmaxf(m, p.xf[j]);
+                const int most = __reduce_max_sync(0xffffffffu, __float_as_int(m));
+                if (lane == 0) p.size[blockIdx.x] = __int_as_float(most);
+            }
+        }
     } else if (warp >= EPI_WARP0) {
         const int w = warp - EPI_WARP0, quad = w & 3, part = w >> 2;
         const uint32_t mine = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(part * (BN / 4));
@@ -1357,6 +1371,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
 }
 
+__device__ __forceinline__ __half2 pair_twice(__half x) { return __half2half2(x); }
+__device__ __forceinline__ __nv_bfloat162 pair_twice(__nv_bfloat16 x) {
+    return __bfloat162bfloat162(x);
+}
+// The largest size of the elements that a thread has read.
+template <typename T>
+struct Largest {
+    using Pair = decltype(pair_twice(T()));
+    Pair m = pair_twice(T(0.0f));
+    __device__ __forceinline__ void add(const uint4& raw) {
+        const Pair* e = reinterpret_cast<const Pair*>(&raw);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = __hmax2(m, __habs2(e[i]));
+    }
+    __device__ __forceinline__ void add(T x) { m = __hmax2(m, __habs2(pair_twice(x))); }
+    __device__ __forceinline__ float get() const {
+        return fmaxf(to_f32<T>(m.x), to_f32<T>(m.y));
+    }
+};
+template <>
+struct Largest<float> {
+    float m = 0.0f;
+    __device__ __forceinline__ void add(const uint4& raw) {
+        m = max3(m, fabsf(__uint_as_float(raw.x)), fabsf(__uint_as_float(raw.y)));
+        m = max3(m, fabsf(__uint_as_float(raw.z)), fabsf(__uint_as_float(raw.w)));
+    }
+    __device__ __forceinline__ void add(float x) { m = fmaxf(m, fabsf(x)); }
+    __device__ __forceinline__ float get() const { return m; }
+};
 // ---------------------------------------------------------------------------
 // a few queries: one pass over the rows on the FMA pipes
 // ---------------------------------------------------------------------------
@@ -1366,12 +1409,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 // in 32 / RB lanes, of which one keeps them, so that after all batches every
 // lane holds one row of the group.  Bound by memory (each row read once) up to
 // about 8 queries; the tensor cores would work on 256 rows of queries.
-template <typename T, int NQ, bool VEC>
+// TOP, with alternatives: finds the largest element of the rows that some query
+// sees, too (up to 7 % of the time: 100000 x 768 f32, 4 queries, 113 -> 120 us).
+// The loops over the columns are unrolled as measured: aligned rows twice for 1 and
+// 8 queries (100000 x 768 bf16, 1 query: 70 -> 60 us; not 300000 x 96 f32, 4
+// queries: 58 would be 67, nor 100000 x 768 f32, 1 query without TOP: 85 and 99),
+// unaligned ones four times in 16 bits (200000 x 75, 1
+// query: 38 -> 28; f32 with 8 queries would go from 66 to 85).
+template <typename T, int NQ, bool VEC, bool TOP>
 __global__ void __launch_bounds__(64)
     few_kernel(const T* __restrict__ x, size_t ld, int n, int d, const T* __restrict__ q,
                size_t ldq, int q0, int nq, float rf, const uint32_t* __restrict__ allowed,
                size_t ld_allowed, float4* __restrict__ part, float2* __restrict__ top,
-               size_t groups, int* __restrict__ err) {
+               size_t groups, float* __restrict__ size, int* __restrict__ err) {
     if (blockIdx.x == 0 && threadIdx.x == 0) *err = 0;  // (this path has no waits)
     constexpr int V = 16 / (int)sizeof(T);
     constexpr int RB = 8;
@@ -1389,6 +1439,8 @@ __global__ void __launch_bounds__(64)
                             8 * (lane & 3);
     Run r[NQ];
     float top_max[NQ];
+    Largest<T> largest;  // of the rows that some query sees
+    float most = 0.0f;
 #pragma unroll
     for (int j = 0; j < NQ; ++j) r[j] = run_empty(), top_max[j] = NONE;
     const int ng = (n + GROUP - 1) / GROUP;
@@ -1396,8 +1448,15 @@ __global__ void __launch_bounds__(64)
         float sc[NQ];
 #pragma unroll
         for (int j = 0; j < NQ; ++j) sc[j] = 0.0f;
+        uint32_t seen = 0xffffffffu;
+        if (TOP) {
+            seen = 0u;
+            for (int j = 0; j < (allowed && ld_allowed ? nq : 1); ++j)
+                seen |= allowed_word(allowed, ld_allowed, q0 + j, (size_t)grp * GROUP, n);
+        }
+        const int first = TOP ? __ffs(seen) - 1 : 0;
 #pragma unroll 1
-        for (int b = 0; b < 32 / RB; ++b) {
+        for (int b = 0; b < (seen ? 32 / RB : 0); ++b) {
             const int r0 = grp * GROUP + b * RB;
             uint64_t acc2[PAIRS ? NQ : 1][RB];  // sums of the even and of the odd columns
             float acc[NQ][RB];
@@ -1410,13 +1469,23 @@ __global__ void __launch_bounds__(64)
                 }
             const T* row[RB];
 #pragma unroll
-            for (int i = 0; i < RB; ++i) row[i] = x + (size_t)min(r0 + i, n - 1) * ld;
+            for (int i = 0; i < RB; ++i) {
+                // (TOP: a row that no query sees is one that is seen, read again)
+                const int at = TOP ? grp * GROUP + (seen >> (b * RB + i) & 1u ? b * RB + i : first)
+                                   : min(r0 + i, n - 1);
+                row[i] = x + (size_t)at * ld;
+            }
             if (VEC) {
+#pragma unroll ((NQ == 1 && (TOP || sizeof(T) == 2)) || NQ == 8 ? 2 : 1)
                 for (int c = lane * V; c < d; c += 32 * V) {
                     uint4 xv[RB];
 #pragma unroll
                     for (int i = 0; i < RB; ++i)
                         xv[i] = __ldg(reinterpret_cast<const uint4*>(row[i] + c));
+                    if (TOP) {
+#pragma unroll
+                        for (int i = 0; i < RB; ++i) largest.add(xv[i]);
+                    }
 #pragma unroll
                     for (int h = 0; h < V; h += 4) {  // four columns at a time
                         uint64_t x01[RB], x23[RB];
@@ -1448,12 +1517,17 @@ __global__ void __launch_bounds__(64)
                     }
                 }
             } else {
+#pragma unroll (sizeof(T) == 2 ? 4 : 1)
                 for (int c = lane; c < d; c += 64) {  // columns c and c + 32
                     const bool two = c + 32 < d;
                     uint64_t xv[RB];
 #pragma unroll
-                    for (int i = 0; i < RB; ++i)
-                        xv[i] = packf(to_f32<T>(row[i][c]), two ? to_f32<T>(row[i][c + 32]) : 0.0f);
+                    for (int i = 0; i < RB; ++i) {
+                        const float x0 = to_f32<T>(row[i][c]);
+                        const float x1 = two ? to_f32<T>(row[i][c + 32]) : 0.0f;
+                        xv[i] = packf(x0, x1);
+                        if (TOP) most = max3(most, fabsf(x0), fabsf(x1));
+                    }
 #pragma unroll
                     for (int j = 0; j < NQ; ++j) {
                         const float* qj = qs + j * dp + c;
@@ -1509,7 +1583,7 @@ __global__ void __launch_bounds__(64)
                 r[j].l += e;
                 r[j].a = __fmaf_rn(e, dd, r[j].a);
             }
-            if (top) {
+            if (TOP) {
                 float a = ok ? sc[j] * rf : NONE, b2 = NONE;
                 a = __uint_as_float((__float_as_uint(a) & ~15u) | (unsigned)(row_of_lane >> 1));
 #pragma unroll
@@ -1527,6 +1601,10 @@ __global__ void __launch_bounds__(64)
     // the lanes' triples joined, then the two warps'
     __shared__ Run other[NQ];
     __shared__ float other_top[NQ];
+    __shared__ int other_size;
+    const int size_all =
+        __reduce_max_sync(0xffffffffu, __float_as_int(fmaxf(most, largest.get())));
+    if (warp == 1 && lane == 0) other_size = size_all;
 #pragma unroll
     for (int j = 0; j < NQ; ++j)
 #pragma unroll
@@ -1550,6 +1628,7 @@ __global__ void __launch_bounds__(64)
                 part[(size_t)blockIdx.x * nq + j] =
                     run_stored(r[j], fmaxf(top_max[j], other_top[j]));
             }
+    if (TOP && threadIdx.x == 0) size[blockIdx.x] = __int_as_float(max(size_all, other_size));
 }
 
 // ---------------------------------------------------------------------------
@@ -1568,6 +1647,12 @@ struct FinishArgs {
     const float* qf;
     const float2* top;
     size_t groups;
+    // [sizes] whose largest bounds the elements of the rows that a query sees, null:
+    // unknown.  Few queries: of the rows that one of them sees.  f32 rows on the
+    // tensor cores: the rows' factors xf; with filters of their own those of all
+    // rows, and a query that this sends to all groups takes its own.
+    const float *size, *xf;
+    int sizes;
     // Which groups a part folded.  Tensor-core pass: part i is quarter i % 4 of
     // the column tiles of chunk i / 4; few queries (nt = 0): part i is block i,
     // whose two warps took every 2 * parts-th group.
@@ -1614,35 +1699,6 @@ struct Exact<float> {
     double s = 0.0;
     __device__ __forceinline__ void add(float x, double q) { s = fma((double)x, q, s); }
     __device__ __forceinline__ double sum() const { return s; }
-};
-__device__ __forceinline__ __half2 pair_twice(__half x) { return __half2half2(x); }
-__device__ __forceinline__ __nv_bfloat162 pair_twice(__nv_bfloat16 x) {
-    return __bfloat162bfloat162(x);
-}
-// The largest size of the elements that a thread has read.
-template <typename T>
-struct Largest {
-    using Pair = decltype(pair_twice(T()));
-    Pair m = pair_twice(T(0.0f));
-    __device__ __forceinline__ void add(const uint4& raw) {
-        const Pair* e = reinterpret_cast<const Pair*>(&raw);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) m = __hmax2(m, __habs2(e[i]));
-    }
-    __device__ __forceinline__ void add(T x) { m = __hmax2(m, __habs2(pair_twice(x))); }
-    __device__ __forceinline__ float get() const {
-        return fmaxf(to_f32<T>(m.x), to_f32<T>(m.y));
-    }
-};
-template <>
-struct Largest<float> {
-    float m = 0.0f;
-    __device__ __forceinline__ void add(const uint4& raw) {
-        add(__uint_as_float(raw.x)), add(__uint_as_float(raw.y));
-        add(__uint_as_float(raw.z)), add(__uint_as_float(raw.w));
-    }
-    __device__ __forceinline__ void add(float x) { m = fmaxf(m, fabsf(x)); }
-    __device__ __forceinline__ float get() const { return m; }
 };
 template <int ROWS, typename T>
 __device__ __forceinline__ void dot_lanes(const T* const (&x)[ROWS],
@@ -1771,6 +1827,12 @@ __global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kern
     for (int i = 0; i < W; ++i) M = fmaxf(M, redf[i]);
     // ---- the sums over the parts, in units of 2^M ----
     float L = 0.0f, A = 0.0f;
+    if (p.size) {
+        float z = 0.0f;
+        for (int i = tid; i < p.sizes; i += THREADS_) z = fmaxf(z, p.size[i]);
+        const int w = __reduce_max_sync(0xffffffffu, __float_as_int(z));
+        if (lane == 0) atomicMax(&s_size, w);
+    }
     for (int i = tid; i < p.parts; i += THREADS_) {
         const float4 t = p.part[(size_t)i * p.nq + ql];
         if (t.y == 0.0f && t.z == 0.0f) continue;
@@ -1838,7 +1900,7 @@ __global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kern
                 if (sub == 0 && j < to) cs[j] = ordered64(v[r]);
             }
         }
-        if (p.k > 0) {
+        if (p.k > 0 && !p.size) {
             const int w = __reduce_max_sync(0xffffffffu, __float_as_int(largest.get()));
             if (lane == 0) atomicMax(&s_size, w);
         }
@@ -1979,13 +2041,19 @@ __global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kern
     };
     // Whether a score of at most `m` (as a group left it) may be among the best
     // k, whose last exact score so far is s_kth: a mark moves it by 2^-19 of
-    // itself, the 32-bit sums by less than 2^-18 of |q| sqrt(d) max |x_c|.
+    // itself, the 32-bit sums by less than 2^-18 of |q| sqrt(d) max |x_c|, x the
+    // rows that the query sees.  The tensor cores read 16-bit rows as they are,
+    // so nothing has looked at their sizes: x then are those scored so far, and a
+    // row whose elements are many times theirs may be passed over if its score is
+    // above the kth by less than its own error.  (A pass for the sizes alone
+    // would read the rows again: 100003 x 768 with 8 queries 55 us and 24 more.)
     qq = 0.0f;
 #pragma unroll
     for (int i = 0; i < W; ++i) qq += s_qsize[i];
     auto may_enter = [&](double m) {
         const double v = m / unit, kth = s_kth;
-        const double size = (double)sqrtf(qq * (float)p.d) * (double)__int_as_float(s_size);
+        const double size = (double)sqrtf(qq * (float)p.d) * (double)__int_as_float(s_size) *
+                            (p.xf ? 16384.0 : 1.0);  // (packed: below 2^14 of the factor)
         return !(v < kth - (fabs(v) + fabs(kth)) * 0x1p-16 - size * 0x1p-18);
     };
     const int ranked = cnt > 128 ? narrow(cnt, least_of(cnt)) : cnt;
@@ -1997,7 +2065,19 @@ __global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kern
     if (tid == 0) s_parts = best;
     __syncthreads();
     // ---- groups whose second largest score may still enter: their other rows ----
-    const bool more = bound > NONE_BELOW && may_enter(bound);  // groups below the bound may
+    bool more = bound > NONE_BELOW && may_enter(bound);  // groups below the bound may
+    if ((more || all_groups) && !bad && p.xf && p.ld_allowed) {
+        __syncthreads();
+        if (tid == 0) s_size = 0;
+        __syncthreads();
+        float z = 0.0f;
+        for (int j = tid; j < p.n; j += THREADS_)
+            if (al[j >> 5] >> (j & 31) & 1u) z = fmaxf(z, p.xf[j]);
+        const int w = __reduce_max_sync(0xffffffffu, __float_as_int(z));
+        if (lane == 0) atomicMax(&s_size, w);
+        __syncthreads();
+        more = bound > NONE_BELOW && may_enter(bound);
+    }
     if (!all_groups && !more && !bad) {
         for (int i = tid; i < picked; i += THREADS_) {
             const float2 m = sel_m[i];
@@ -2662,6 +2742,9 @@ static void allow_smem(K* kernel, int device, size_t bytes, std::atomic<uint64_t
     if (device < 64) done.fetch_or(1ull << device, std::memory_order_release);
 }
 
+static unsigned blocks_of(int sms, long long units) {
+    return 2 * (unsigned)std::min<long long>(units, sms / 2);
+}
 template <int MODE, bool TWO, bool BLK>
 static void launch_rows(cudaStream_t s, int device, int sms, const CUtensorMap& a,
                         const CUtensorMap& b, const Mma& g,
@@ -2673,9 +2756,8 @@ static void launch_rows(cudaStream_t s, int device, int sms, const CUtensorMap& 
     const size_t smem = smem_of(TWO, BLK, MODE == GRAD);
     static std::atomic<uint64_t> done{0};
     allow_smem(rows_kernel<MODE, TWO, BLK>, device, smem, done);
-    rows_kernel<MODE, TWO, BLK>
-        <<<2 * (unsigned)std::min<long long>(units, sms / 2), THREADS, smem, s>>>(
-            a, b, out ? *out : a, g, p);
+    rows_kernel<MODE, TWO, BLK><<<blocks_of(sms, units), THREADS, smem, s>>>(a, b, out ? *out : a,
+                                                                             g, p);
     FDB_LAUNCH_CHECK();
 }
 // A's K steps stay in shared memory where they fill at most half of the ring
@@ -2737,6 +2819,7 @@ struct Forward {
     float *qf, *xf;
     float4* part;
     float2* top;
+    float* size;  // see FinishArgs
 };
 static bool mappable(const void* p, size_t ld) {
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * 2 & 15) == 0;
@@ -2783,6 +2866,8 @@ static Forward plan_forward(const Ctx& c, const fdb_logprob_args& a) {
     }
     w.part = ws.take<float4>(w.parts_cap * w.qb);
     if (a.k) w.top = ws.take<float2>(w.qb * w.groups);
+    if (a.k && (w.few || w.packed))
+        w.size = ws.take<float>(std::max<size_t>(w.parts_cap, c.sm_count));
     w.bytes = ws.at;
     return w;
 }
@@ -2833,6 +2918,7 @@ static FinishArgs finish_args(const fdb_logprob_args& a, const Forward& w, size_
     f.allowed = a.allowed, f.ld_allowed = a.allowed ? a.ld_allowed : 0;
     f.part = w.part;
     f.top = w.top, f.groups = w.groups;
+    f.size = w.size, f.xf = w.xf;
     f.logprob = a.logprob, f.lse = a.lse, f.entropy = a.entropy;
     f.top_logprob = a.top_logprobs, f.top_ids = a.top_ids;
     f.err = w.err;
@@ -2844,19 +2930,25 @@ static FinishArgs finish_args(const fdb_logprob_args& a, const Forward& w, size_
 
 // A kernel's limit is the process's, not the call's: it is set to the largest
 // size that any call takes, as two threads may launch the same kernel at once.
-template <typename T, int NQ, bool VEC>
+template <typename T, int NQ, bool VEC, bool TOP>
 static void launch_few(const Ctx& c, const fdb_logprob_args& a, const Forward& w, int q0, int nq,
                        float rf, size_t ld_allowed) {
     const size_t smem = NQ * up(a.dim, 128) * 4;
     if (smem > 40960) {  // (with the static part, over what needs no permission)
         static std::atomic<uint64_t> done{0};
-        allow_smem(few_kernel<T, NQ, VEC>, c.device, NQ * up(FEW_DIM, 128) * 4, done);
+        allow_smem(few_kernel<T, NQ, VEC, TOP>, c.device, NQ * up(FEW_DIM, 128) * 4, done);
     }
-    few_kernel<T, NQ, VEC><<<(unsigned)w.parts_cap, 64, smem, static_cast<cudaStream_t>(a.stream)>>>(
+    few_kernel<T, NQ, VEC, TOP><<<(unsigned)w.parts_cap, 64, smem, static_cast<cudaStream_t>(a.stream)>>>(
         static_cast<const T*>(a.rows), a.ld_rows, (int)a.n, (int)a.dim,
         static_cast<const T*>(a.queries), a.ld_queries, q0, nq, rf, a.allowed, ld_allowed, w.part,
-        w.top, w.groups, w.err);
+        w.top, w.groups, w.size, w.err);
     FDB_LAUNCH_CHECK();
+}
+template <typename T, int NQ, bool VEC>
+static void launch_few(const Ctx& c, const fdb_logprob_args& a, const Forward& w, int q0, int nq,
+                       float rf, size_t ld_allowed) {
+    if (w.top) launch_few<T, NQ, VEC, true>(c, a, w, q0, nq, rf, ld_allowed);
+    else launch_few<T, NQ, VEC, false>(c, a, w, q0, nq, rf, ld_allowed);
 }
 template <typename T, int NQ>
 static void launch_few(bool vec, const Ctx& c, const fdb_logprob_args& a, const Forward& w, int q0,
@@ -2881,7 +2973,7 @@ static void few_run(const Ctx& c, const fdb_logprob_args& a, const Forward& w, f
             launch_few<T, 4, false>(c, a, w, q0, nq, rf, ld_allowed);
         }
         FinishArgs f = finish_args(a, w, q, nq);
-        f.parts = (int)w.parts_cap;
+        f.parts = f.sizes = (int)w.parts_cap;
         launch_finish<T>(s, c.device, f);
     }
 }
@@ -2944,6 +3036,7 @@ void forward_run(Ctx& c, const fdb_logprob_args& a) {
             p.part = w.part;
             p.top = w.top;
             p.groups = w.groups;
+            p.size = w.size;
             if (w.packed && !w.blocks)
                 launch_rows<STATS, true, false>(s, c.device, c.sm_count, amap, bmap, g, p);
             else if (w.packed)
@@ -2955,6 +3048,7 @@ void forward_run(Ctx& c, const fdb_logprob_args& a) {
             FinishArgs f = finish_args(a, w, q0, nq);
             f.parts = g.chunks * 4;
             f.qf = p.qf;
+            f.sizes = (int)blocks_of(c.sm_count, (long long)g.mt * g.chunks);
             f.nt = w.nt, f.chunks = g.chunks;
             f.per_tile = w.bn / GROUP, f.per_part = w.bn / GROUP / 4;
             if (a.dtype == FDB_DTYPE_F32) launch_finish<float>(s, c.device, f);

@@ -266,7 +266,8 @@ def test_gradients_of_very_large_and_small_operands(dtype, shift):
                                           ("f16", 2, 256)])
 @pytest.mark.parametrize("bad", [float("inf"), 6e4])
 @pytest.mark.parametrize("targets", [False, True])
-def test_a_row_that_is_not_seen_takes_no_part(dtype, nq, dim, bad, targets):
+@pytest.mark.parametrize("filters", ["one", "each"])
+def test_a_row_that_is_not_seen_takes_no_part(dtype, nq, dim, bad, targets, filters):
     """A masked row, the first one or the given one, that holds an infinity or
     something large: the same bits, and no more work, than beside zeros (the
     alternatives of every query would be looked for in all rows if it counted
@@ -280,6 +281,8 @@ def test_a_row_that_is_not_seen_takes_no_part(dtype, nq, dim, bad, targets):
     keep = torch.ones(1, n, dtype=torch.bool)
     keep[0, :2] = False
     words = torch.from_numpy(so.words(keep.numpy())).cuda()
+    if filters == "each":
+        words = words.repeat(nq, 1)
     t = torch.ones(nq, dtype=torch.int64, device="cuda") if targets else None
     out, times = [], []
     for value in (0.0, bad):
@@ -296,3 +299,37 @@ def test_a_row_that_is_not_seen_takes_no_part(dtype, nq, dim, bad, targets):
         times.append(ev[0].elapsed_time(ev[1]))
     assert all(torch.equal(a, b) for a, b in zip(*out))
     assert times[1] < 3 * times[0], times
+
+
+@pytest.mark.parametrize("nq,seed", [(1, 0), (1, 1), (1, 2), (1, 3), (8, 0), (16, 0), (40, 0),
+                                     (300, 0)])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_a_large_row_nearly_at_right_angles(nq, seed, dim):
+    """Each query sees one row a million times the others', whose true score is
+    just above their best; its 32-bit score may be far below all of them."""
+    import forgegpu as fg
+    import torch
+    rng = np.random.default_rng(100 * nq + seed)
+    n = 20000
+    q = rng.standard_normal((nq, dim)).astype(np.float32)
+    q[:, 0] = np.abs(q[:, 0]) + 1
+    x = (rng.standard_normal((n + nq, dim)) / np.sqrt(dim)).astype(np.float32)
+    q64 = q.astype(np.float64)
+    best = (q64 @ x[:n].astype(np.float64).T).max(1)
+    for i in range(nq):
+        g = (1e6 * rng.standard_normal(dim)).astype(np.float32)
+        g[0] = 0
+        c = 1 + np.argmax(np.abs(q[i, 1:]))  # two corrections: most of it, then the rest
+        g[c] -= np.float32((q64[i] @ g.astype(np.float64)) / q64[i, c])
+        g[0] = np.float32((best[i] + 0.01 - q64[i] @ g.astype(np.float64)) / q64[i, 0])
+        x[n + i] = g
+    keep = np.ones((nq, n + nq), bool)
+    keep[:, n:] = np.eye(nq, dtype=bool)
+    s = np.where(keep, q64 @ x.astype(np.float64).T, -np.inf)
+    s[np.arange(nq), n + np.arange(nq)] = [q64[i] @ x[n + i].astype(np.float64) for i in range(nq)]
+    assert (np.abs(s[np.arange(nq), n + np.arange(nq)] - best - 0.01) < 1e-3).all()
+    want = np.argsort(-s, 1)[:, :5]
+    Q, X = torch.from_numpy(q).cuda(), torch.from_numpy(x).cuda()
+    A = torch.from_numpy(so.words(keep)).cuda()
+    r = fg.logprobs(Q, X, scale=1.0, allowed=A, k=5)
+    assert np.array_equal(r.top_ids.cpu().numpy(), want)
