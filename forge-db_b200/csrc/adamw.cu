@@ -12,7 +12,9 @@
 // a thousandth, far less than a code, and rounding to nearest would never
 // move it.  The draw is a hash of (seed, step, tensor, element).  v > 0 keeps
 // a code of at least 1: a zero under a moment that is not zero would make the
-// update m / eps.
+// update m / eps.  v is a square, so a block whose largest v is small (gradients
+// below about 1e-12) is held and read 2^64 larger, down to 2^-112; below that
+// (gradients below about 1e-15) its v is held as zeros, and its m with it.
 //
 // Bound by memory with f32 moments: f32 p, g, m, v move 28 bytes an element
 // (131072 x 768: 419 us, 6.7 TB/s).  bf16 p, g with 8-bit moments move 10, and
@@ -34,7 +36,10 @@ constexpr int THREADS = 256;
 constexpr int CHUNK = 8192;      // elements a block works through
 constexpr int SMALL_CHUNK = 2048;  // ... when there are too few for every multiprocessor
 constexpr int BLOCK8 = FDB_ADAMW_BLOCK;
-constexpr float LEAST = 0x1p-90f;  // a block whose largest value is below this holds zeros
+// A block whose largest |m| is below LEAST, or largest v below LEAST_V, holds zeros;
+// one whose largest v is below LEAST is worked on UP times larger (255^4 / v has to
+// stay in range, and v / 255^4 out of f32's subnormal numbers).
+constexpr float LEAST = 0x1p-90f, LEAST_V = 0x1p-112f, UP = 0x1p64f;
 constexpr float M_CODES = 16129.0f, V_CODES = 4228250625.0f;  // 127^2, 255^4
 
 struct Entry {
@@ -113,15 +118,16 @@ struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Vec {
     T e[N];
 };
 
-__device__ __forceinline__ void moments(const Consts& c, float g, float& m, float& v) {
+__device__ __forceinline__ void moments(const Consts& c, float b2, float g, float& m, float& v) {
     m = __fadd_rn(__fmul_rn(m, c.b1), __fmul_rn(g, c.c1));
-    v = __fadd_rn(__fmul_rn(v, c.b2), __fmul_rn(__fmul_rn(g, g), c.c2));
+    v = __fadd_rn(__fmul_rn(v, b2), __fmul_rn(__fmul_rn(g, g), c.c2));
 }
 __device__ __forceinline__ float stepped(const Consts& c, float p, float m, float v) {
     const float den = __fadd_rn(__fmul_rn(__fsqrt_rn(v), c.root), c.eps);
     return __fsub_rn(__fmul_rn(p, c.keep), __fmul_rn(__fdiv_rn(m, den), c.rate));
 }
 
+// The published 32-bit mixer lowbias32: its shifts and constants.
 __device__ __forceinline__ uint32_t mix(uint32_t h) {
     h = (h ^ (h >> 16)) * 0x7FEB352Du;
     h = (h ^ (h >> 15)) * 0x846CA68Bu;
@@ -241,7 +247,7 @@ __global__ void __launch_bounds__(THREADS)
                 const size_t i = b + (size_t)u * THREADS * N;
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
-                    moments(c, __fmul_rn(get<G>(gv[u].e[j]), c.gs), mv[u].e[j], vv[u].e[j]);
+                    moments(c, c.b2, __fmul_rn(get<G>(gv[u].e[j]), c.gs), mv[u].e[j], vv[u].e[j]);
                     pv[u].e[j] =
                         put<P>(stepped(c, get<P>(pv[u].e[j]), mv[u].e[j], vv[u].e[j]));
                 }
@@ -254,7 +260,7 @@ __global__ void __launch_bounds__(THREADS)
     }
     for (size_t i = i0 + threadIdx.x; i < i1; i += THREADS) {
         float mi = m[i], vi = v[i];
-        moments(c, __fmul_rn(get<G>(g[i]), c.gs), mi, vi);
+        moments(c, c.b2, __fmul_rn(get<G>(g[i]), c.gs), mi, vi);
         p[i] = put<P>(stepped(c, get<P>(p[i]), mi, vi));
         m[i] = mi;
         v[i] = vi;
@@ -300,7 +306,9 @@ __global__ void __launch_bounds__(THREADS)
                 (j < 4 ? vc.x : vc.y) |= b << (8 * (j & 3));
             }
         }
-        const float ks = __fmul_rn(e.ms[blk], KM), kv = __fmul_rn(e.vs[blk], KV);
+        const float ks = __fmul_rn(e.ms[blk], KM), s0 = e.vs[blk];
+        const float kv = __fmul_rn(s0 < LEAST ? __fmul_rn(s0, UP) : s0, KV);
+        const float b2 = s0 < LEAST ? __fmul_rn(c.b2, 1.0f / UP) : c.b2;  // (and back)
         float m[8], v[8], sm = 0.0f, sv = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -310,7 +318,7 @@ __global__ void __launch_bounds__(THREADS)
             m[j] = __fmul_rn(__fmul_rn(a, fabsf(a)), ks);
             const float r2 = __fmul_rn(r, r);
             v[j] = __fmul_rn(__fmul_rn(r2, r2), kv);
-            moments(c, __fmul_rn(get<G>(gv.e[j]), c.gs), m[j], v[j]);
+            moments(c, b2, __fmul_rn(get<G>(gv.e[j]), c.gs), m[j], v[j]);
             pv.e[j] = put<P>(stepped(c, get<P>(pv.e[j]), m[j], v[j]));
             // (past the tensor's end: zeros.  A NaN makes the block's scale NaN: the
             // block reads as NaN from then on)
@@ -322,8 +330,14 @@ __global__ void __launch_bounds__(THREADS)
             sm = max_nan(sm, __shfl_xor_sync(0xffffffffu, sm, o));
             sv = max_nan(sv, __shfl_xor_sync(0xffffffffu, sv, o));
         }
+        if (sv > 0.0f && sv < LEAST_V) sm = 0.0f;
         const float km = sm > LEAST ? __fdiv_rn(M_CODES, sm) : 0.0f;
-        const float kw = sv > LEAST ? __fdiv_rn(V_CODES, sv) : 0.0f;
+        float kw = sv > LEAST ? __fdiv_rn(V_CODES, sv) : 0.0f;
+        if (sv >= LEAST_V && sv <= LEAST) {
+            kw = __fdiv_rn(V_CODES, __fmul_rn(sv, UP));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(v[j], UP);
+        }
         // (i is a multiple of 8: the eight numbers differ in their last bits)
         const uint32_t at =
             (uint32_t)i ^ salt ^ ((uint32_t)((uint64_t)i >> 32) * 0x9E3779B1u);
@@ -356,7 +370,7 @@ __global__ void __launch_bounds__(THREADS)
         }
         if (lane == 0) {
             e.ms[blk] = sm < LEAST ? 0.0f : sm;
-            e.vs[blk] = sv < LEAST ? 0.0f : sv;
+            e.vs[blk] = sv < LEAST_V ? 0.0f : sv;
         }
     }
 }
@@ -369,7 +383,9 @@ __global__ void __launch_bounds__(THREADS)
     constexpr float KM = (float)(1.0 / 16129.0), KV = (float)(1.0 / 4228250625.0);
     const size_t step = (size_t)gridDim.x * THREADS * 4;
     for (size_t i = ((size_t)blockIdx.x * THREADS + threadIdx.x) * 4; i < n; i += step) {
-        const float ks = __fmul_rn(ms[i / BLOCK8], KM), kv = __fmul_rn(vs[i / BLOCK8], KV);
+        const float ks = __fmul_rn(ms[i / BLOCK8], KM), s0 = vs[i / BLOCK8];
+        const float kv = __fmul_rn(s0 < LEAST ? __fmul_rn(s0, UP) : s0, KV);
+        const float down = s0 < LEAST ? 1.0f / UP : 1.0f;
         const bool whole = wide && i + 4 <= n;
         Vec<int8_t, 4> mc;
         Vec<uint8_t, 4> vc;
@@ -388,7 +404,7 @@ __global__ void __launch_bounds__(THREADS)
         for (int j = 0; j < 4; ++j) {
             const float x = (float)mc.e[j], r = (float)vc.e[j], r2 = __fmul_rn(r, r);
             a.e[j] = __fmul_rn(__fmul_rn(x, fabsf(x)), ks);
-            b.e[j] = __fmul_rn(__fmul_rn(r2, r2), kv);
+            b.e[j] = __fmul_rn(__fmul_rn(__fmul_rn(r2, r2), kv), down);
         }
         if (whole) {
             *reinterpret_cast<Vec<float, 4>*>(om + i) = a;

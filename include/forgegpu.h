@@ -567,7 +567,9 @@ int fdb_bf_logprobs(fdb_bf* h, const float* queries, size_t nq, float temperatur
  * elements: m = m_scale c |c| / 127^2, v = v_scale c^4 / 255^4; a value
  * between two codes is rounded up or down at random (a hash of seed, step,
  * the tensor's number in the call and the element) so that its mean is kept,
- * and v > 0 keeps a code of at least 1.  All zeros is the initial state.  A
+ * and v > 0 keeps a code of at least 1.  A block whose largest |m| is below
+ * 2^-90, or whose largest v is not 0 and below 2^-112 (gradients below about
+ * 1e-15), is held as zeros.  All zeros is the initial state.  A
  * gradient with a NaN or infinity makes its element of p, m and v NaN or
  * infinite, with 8-bit states the whole block's m and v.
  * step counts from 1.  d_lr, d_step, d_grad_scale (device, nullable) replace
