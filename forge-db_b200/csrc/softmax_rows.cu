@@ -2584,7 +2584,14 @@ __global__ void __launch_bounds__(256, few_per_sm(NQ)) few_grad_kernel(const Few
                 float xv[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) xv[i] = to_f32<T>(x[i * ct_n]);
-                if (x_bad[r] || r0 + r >= p.n) xv[0] = xv[1] = xv[2] = xv[3] = 0.0f;
+                if (r0 + r >= p.n) xv[0] = xv[1] = xv[2] = xv[3] = 0.0f;
+                // (its elements, or only a product with a query that may not see it,
+                // are not finite: the former reach those that see it through G)
+                if (x_bad[r]) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (!(fabsf(xv[i]) <= FLT_MAX)) xv[i] = 0.0f;
+                }
                 const uint64_t x2[2] = {packf(xv[0], xv[1]), packf(xv[2], xv[3])};
                 uint64_t o2[2] = {0ull, 0ull};
 #pragma unroll

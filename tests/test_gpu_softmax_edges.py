@@ -333,3 +333,35 @@ def test_a_large_row_nearly_at_right_angles(nq, seed, dim):
     A = torch.from_numpy(so.words(keep)).cuda()
     r = fg.logprobs(Q, X, scale=1.0, allowed=A, k=5)
     assert np.array_equal(r.top_ids.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("dtype,nq", [("f32", 2), ("f32", 7), ("bf16", 3), ("f32", 40)])
+def test_a_product_out_of_range_that_is_masked(dtype, nq):
+    """A large row that the last query may not see, and whose product with it is
+    beyond f32: the others' gradients are those beside a query of zeros."""
+    import forgegpu as fg
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(nq)
+    q = torch.randn(nq, 40, device="cuda", generator=gen).to(_type(dtype))
+    x = torch.randn(90, 40, device="cuda", generator=gen).to(_type(dtype))
+    q[-1] *= 1e15
+    x[50] *= 1e25
+    scale = 1e-25
+    keep = torch.ones(nq, 90, dtype=torch.bool)
+    keep[-1, 50] = False
+    words = torch.from_numpy(so.words(keep.numpy())).cuda()
+    t = torch.full((nq,), 50, device="cuda")
+    t[-1] = 3
+    up = torch.rand(nq, device="cuda", generator=gen)
+    got = []
+    for last in (q[-1].clone(), torch.zeros_like(q[-1])):
+        q[-1] = last
+        r = fg.logprobs(q, x, t, scale=scale, allowed=words)
+        dq, dx = fg.logprobs_backward(q, x, t, r.lse, d_logprob=up, scale=scale, allowed=words)
+        got.append((r.lse[:-1], dq[:-1], dx[50]))
+    assert got[0][1].float().abs().max() > 1e-3
+    assert all(torch.isfinite(a.float()).all() for a in got[0])
+    if nq <= 8:
+        assert all(torch.equal(a, b) for a, b in zip(*got))
+    else:  # (d_rows' scale is that of the largest query: its terms are 1e-15 of it)
+        assert all(torch.equal(a, b) for a, b in zip(got[0][:2], got[1][:2]))
