@@ -64,6 +64,16 @@ static void release_comm(ncclComm_t comm) {
     else ncclCommAbort(comm);
 }
 
+void ctx_release(fdb_ctx* ctx) {
+    if (ctx->refs.fetch_sub(1, std::memory_order_acq_rel) > 1) return;
+    {
+        DeviceGuard g(ctx->c.device);
+        release_comm(ctx->c.comm);
+        if (ctx->c.stream) cudaStreamDestroy(ctx->c.stream);
+    }
+    delete ctx;
+}
+
 uint64_t splitmix64(uint64_t& state) {
     uint64_t z = (state += 0x9e3779b97f4a7c15ull);
     z = (z ^ (z >> 30)) * 0xbf58476d1ce4e5b9ull;
@@ -206,13 +216,7 @@ int fdb_ctx_create(int device, fdb_ctx** out) {
 
 int fdb_ctx_free(fdb_ctx* ctx) {
     return guarded([&] {
-        if (!ctx) return;
-        {
-            DeviceGuard g(ctx->c.device);
-            release_comm(ctx->c.comm);
-            if (ctx->c.stream) cudaStreamDestroy(ctx->c.stream);
-        }
-        delete ctx;
+        if (ctx) ctx_release(ctx);
     });
 }
 

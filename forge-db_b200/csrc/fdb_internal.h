@@ -521,12 +521,39 @@ void bf_search_dev(fdb_bf* h, const float* dQ, size_t nq, size_t k, uint64_t* d_
 // ---------------------------------------------------------------------------
 // the opaque handles
 // ---------------------------------------------------------------------------
+// Kept by its owner's handle and by every index on it: whichever is freed last
+// takes it along (a garbage collector frees them in any order).
 struct fdb_ctx {
     fdb::Ctx c;
+    std::atomic<int> refs{1};
 };
+namespace fdb {
+void ctx_release(fdb_ctx* ctx);
+class CtxRef {
+    fdb_ctx* p = nullptr;
+
+public:
+    CtxRef() = default;
+    CtxRef(const CtxRef&) = delete;
+    CtxRef& operator=(const CtxRef&) = delete;
+    ~CtxRef() {
+        if (!p) return;
+        try {
+            ctx_release(p);
+        } catch (const Error&) {  // (a destructor; the handle is gone either way)
+        }
+    }
+    void operator=(fdb_ctx* ctx) {  // once
+        p = ctx;
+        p->refs.fetch_add(1, std::memory_order_relaxed);
+    }
+    fdb_ctx* operator->() const { return p; }
+    operator fdb_ctx*() const { return p; }
+};
+}  // namespace fdb
 
 struct fdb_ivfpq {
-    fdb_ctx* ctx = nullptr;
+    fdb::CtxRef ctx;  // (first: the buffers below are gone before it)
     size_t dim = 0, nlist = 0, m = 0;
     int metric = 0;
     std::atomic<size_t> nprobe{1};
@@ -647,7 +674,7 @@ struct fdb_ivfpq {
 };
 
 struct fdb_bf {
-    fdb_ctx* ctx = nullptr;
+    fdb::CtxRef ctx;
     int metric = 0;
     size_t dim = 0;
     size_t n = 0;          // rows held on this device

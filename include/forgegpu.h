@@ -134,6 +134,7 @@ int fdb_version(void);            /* major*10000 + minor*100 + patch */
 
 /* ---- context: one device, one stream, optional NCCL communicator -------- */
 int fdb_ctx_create(int device, fdb_ctx** out);
+/* Indexes on the context may be freed after it: it is then gone with the last. */
 int fdb_ctx_free(fdb_ctx* ctx);
 /* The CUDA stream (cudaStream_t) every call of this context runs on. */
 int fdb_ctx_stream(fdb_ctx* ctx, void** stream_out);

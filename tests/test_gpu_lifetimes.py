@@ -1,0 +1,55 @@
+"""Contexts and indexes may be freed in any order, as a garbage collector does
+with objects that refer to one another."""
+import gc
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def _bf(fg, ctx, x):
+    return fg.BruteForceIndex(fg.DistanceMetric.DotProduct, ctx).add(x)
+
+
+def test_an_index_outlives_its_context():
+    import forgegpu as fg
+    rng = np.random.default_rng(0)
+    x = rng.standard_normal((3000, 32)).astype(np.float32)
+    q = rng.standard_normal((5, 32)).astype(np.float32)
+    ctx = fg.Context(0)
+    bf = _bf(fg, ctx, x)
+    iv = fg.IVFPQIndex.build(x, 8, 8, ctx=ctx, seed=1)
+    want = bf.batch_search_arrays(q, 3), iv.batch_search_arrays(q, 3)
+    ctx.close()
+    got = bf.batch_search_arrays(q, 3), iv.batch_search_arrays(q, 3)
+    for a, b in zip(want, got):
+        assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
+    p = bf.log_probs(q, k=3)
+    assert np.array_equal(p.top_ids, want[0][0])
+    iv.close()
+    assert np.array_equal(bf.log_probs(q, k=3).top_ids, p.top_ids)
+    bf.close()
+    other = _bf(fg, fg.Context(0), x)
+    assert np.array_equal(other.batch_search_arrays(q, 3)[0], want[0][0])
+
+
+def test_a_cycle_of_a_context_and_its_indexes_is_collected():
+    """Cycles with the context in front of and behind its indexes; the next
+    call finds no error that freeing them left."""
+    import forgegpu as fg
+    rng = np.random.default_rng(0)
+    x = rng.standard_normal((500, 16)).astype(np.float32)
+    keep = _bf(fg, fg.default_context(), x)
+    for first in (True, False):
+        for _ in range(4):
+            ctx = fg.Context(0)
+            parts = [_bf(fg, ctx, x) for _ in range(2)]
+            cycle = [ctx, *parts] if first else [*parts, ctx]
+            cycle.append(cycle)
+            for p in parts:
+                p.cycle = cycle
+            ctx.cycle = cycle
+            del ctx, parts, cycle, p
+            gc.collect()
+            assert keep.batch_search_arrays(x[:3], 1)[0].shape == (3, 1)
