@@ -37,9 +37,11 @@ void set_last_error(const std::string& msg);
 #define FDB_CUDA(x)                                                                           \
     do {                                                                                      \
         cudaError_t e__ = (x);                                                                \
-        if (e__ != cudaSuccess)                                                               \
+        if (e__ != cudaSuccess) {                                                             \
+            (void)cudaGetLastError(); /* reported here, not by the next launch */             \
             ::fdb::fail(e__ == cudaErrorMemoryAllocation ? FDB_ERR_OOM : FDB_ERR_CUDA,         \
                         std::string(#x) + ": " + cudaGetErrorString(e__));                    \
+        }                                                                                     \
     } while (0)
 
 #define FDB_LAUNCH_CHECK() FDB_CUDA(cudaGetLastError())

@@ -53,3 +53,24 @@ def test_a_cycle_of_a_context_and_its_indexes_is_collected():
             del ctx, parts, cycle, p
             gc.collect()
             assert keep.batch_search_arrays(x[:3], 1)[0].shape == (3, 1)
+
+
+def test_a_failed_call_does_not_fail_the_next():
+    """An allocation that cannot be had is reported once: the next call's
+    launches do not find its error."""
+    import ctypes as C
+
+    import forgegpu as fg
+    import torch
+    rng = np.random.default_rng(0)
+    x = rng.standard_normal((500, 16)).astype(np.float32)
+    ix = _bf(fg, fg.default_context(), x)
+    q = torch.randn(3, 16, device="cuda")
+    want = ix.batch_search_arrays(x[:3], 2), fg.logprobs(q, q)
+    out = C.c_void_p()
+    for again in (lambda: ix.batch_search_arrays(x[:3], 2)[0], lambda: fg.logprobs(q, q).lse):
+        assert fg.lib().fdb_host_alloc(1 << 60, C.byref(out)) != 0
+        assert b"cudaHostAlloc" in fg.lib().fdb_last_error()
+        got = again()
+    assert np.array_equal(ix.batch_search_arrays(x[:3], 2)[0], want[0][0])
+    assert torch.equal(got, want[1].lse)
