@@ -1019,7 +1019,9 @@ def logprobs(queries, rows, targets=None, *, scale: float = 1.0, allowed=None, k
     targets: int64 [nq], the row whose log probability is wanted (none where
     negative).  allowed: int32 words of a bit per row, one filter or one per
     query.  k: number of alternatives.  workspace: a uint8 tensor to use
-    instead of a new one (logprobs_status reads a timeout from it)."""
+    instead of a new one (logprobs_status reads a timeout from it).  The
+    results have no autograd history, whatever the inputs require: the gradient
+    is logprobs_backward's."""
     torch = _torch()
     head = _softmax_args(queries, rows, targets, scale, allowed)
     dev, nq = queries.device, head[2]
@@ -1099,7 +1101,8 @@ def adamw_step(params, grads, m, v, *, lr: float, step: int = 1, betas=(0.9, 0.9
                d_grad_scale=None):
     """One AdamW step in place over lists of tensors, on the current stream
     (fdb_adamw_step in forgegpu.h).  With m_scales and v_scales the moments
-    are 8-bit: m int8, v uint8, a float32 scale per 256 elements each."""
+    are 8-bit: m int8, v uint8, a float32 scale per 256 elements each.  To
+    autograd it is an in-place change of params and states."""
     torch = _torch()
     count = len(params)
     eight = m_scales is not None or v_scales is not None
@@ -1135,6 +1138,8 @@ def adamw_step(params, grads, m, v, *, lr: float, step: int = 1, betas=(0.9, 0.9
                   _scalar(d_grad_scale, torch.float32, p0, "d_grad_scale"),
                   torch._C._cuda_getCurrentRawStream(dev.index))
     _check(lib().fdb_adamw_step(_ctx_of(dev).h, table.buffer_info()[0], count, C.byref(o)))
+    # (written through pointers: a graph that saved one of them has to notice)
+    torch.autograd.graph.increment_version(list(itertools.chain(params, *lists[2:])))
 
 
 def adamw_state_values(m, m_scale, v, v_scale):

@@ -53,3 +53,38 @@ def test_a_block_without_v_has_no_m():
     assert torch.isfinite(p).all()
     # each step is then one from zeros: at most lr (1 - b1) / sqrt(1 - b2)
     assert (p - torch.linspace(-1, 1, 600, device="cuda")).abs()[:256].max() <= 4 * 1e-2 * 3.2
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_step_is_an_in_place_change_to_autograd(bits):
+    """A graph that saved a parameter or a state before the step refuses its
+    backward pass; results of logprobs have no history."""
+    import forgegpu as fg
+    import torch
+    w = torch.nn.Parameter(torch.randn(300, device="cuda"))
+    g = torch.randn(300, device="cuda")
+    if bits == 32:
+        m, v = [torch.zeros(300, device="cuda")], [torch.zeros(300, device="cuda")]
+        kw = {}
+    else:
+        m = [torch.zeros(300, dtype=torch.int8, device="cuda")]
+        v = [torch.zeros(300, dtype=torch.uint8, device="cuda")]
+        kw = {k: [torch.zeros(2, device="cuda")] for k in ("m_scales", "v_scales")}
+    loss = (w * w).sum()
+    written = [w, *m, *v, *(x for xs in kw.values() for x in xs)]
+    before = [x._version for x in written]
+    fg.adamw_step([w], [g], m, v, lr=1e-2, **kw)
+    assert all(x._version > b for x, b in zip(written, before))
+    with pytest.raises(RuntimeError):
+        loss.backward()
+    (w * w).sum().backward()
+    assert torch.equal(w.grad, 2 * w.detach())
+    q = torch.randn(3, 4, device="cuda", requires_grad=True)
+    x = torch.nn.Parameter(torch.randn(9, 4, device="cuda"))
+    r = fg.logprobs(q, x, k=1)
+    assert not any(t.requires_grad for t in r)
+    fg.adamw_step([w.detach()], [g], m, v, lr=1e-2, **kw)
+    with torch.inference_mode():
+        z = torch.zeros(5, device="cuda")
+        s = [torch.zeros(5, device="cuda") for _ in range(3)]
+        fg.adamw_step([z], s[:1], s[1:2], s[2:], lr=1e-2)
