@@ -1397,7 +1397,11 @@ int fdb_adamw_step(fdb_ctx* ctx, const fdb_adamw_tensor* tensors, size_t count,
         const size_t gs = o.grad_dtype == FDB_DTYPE_F32 ? 4 : 2;
         const size_t ss = o.state_bits == 8 ? 1 : 4;
         std::vector<std::pair<uintptr_t, uintptr_t>> spans;
-        spans.reserve(count);
+        spans.reserve(count * (o.state_bits == 8 ? 5 : 3));
+        auto written = [&](const void* p, size_t bytes) {
+            const uintptr_t b = reinterpret_cast<uintptr_t>(p);
+            spans.emplace_back(b, b + bytes);
+        };
         for (size_t i = 0; i < count; ++i) {
             const fdb_adamw_tensor& t = tensors[i];
             if (t.n == 0) continue;
@@ -1411,13 +1415,19 @@ int fdb_adamw_step(fdb_ctx* ctx, const fdb_adamw_tensor* tensors, size_t count,
             check_aligned(t.v, ss, "v");
             check_aligned(t.m_scale, 4, "m_scale");
             check_aligned(t.v_scale, 4, "v_scale");
-            const uintptr_t b = reinterpret_cast<uintptr_t>(t.param);
-            spans.emplace_back(b, b + t.n * ps);
+            written(t.param, t.n * ps);
+            written(t.m, t.n * ss);
+            written(t.v, t.n * ss);
+            if (o.state_bits == 8) {
+                const size_t blocks = (t.n + FDB_ADAMW_BLOCK - 1) / FDB_ADAMW_BLOCK;
+                written(t.m_scale, blocks * 4);
+                written(t.v_scale, blocks * 4);
+            }
         }
         std::sort(spans.begin(), spans.end());
         for (size_t i = 1; i < spans.size(); ++i)
             FDB_REQUIRE(spans[i - 1].second <= spans[i].first, FDB_ERR_INVALID_ARG,
-                        "two tensors' params overlap");
+                        "params or states overlap");
         DeviceGuard g(ctx->c.device);
         adamw::step(static_cast<cudaStream_t>(o.stream), ctx->c.sm_count, tensors, count, o);
     });

@@ -575,7 +575,7 @@ int fdb_bf_logprobs(fdb_bf* h, const float* queries, size_t nq, float temperatur
  * infinite, with 8-bit states the whole block's m and v.
  * step counts from 1.  d_lr, d_step, d_grad_scale (device, nullable) replace
  * lr and step and multiply grad_scale when the kernels run, so that a captured
- * step can be replayed with other values.  No two tensors' params may overlap. */
+ * step can be replayed with other values.  No params or states may overlap. */
 #define FDB_ADAMW_BLOCK 256
 typedef struct fdb_adamw_tensor {
     void* param;
