@@ -1411,15 +1411,15 @@ struct Largest<float> {
 // about 8 queries; the tensor cores would work on 256 rows of queries.
 // TOP, with alternatives: finds the largest element of the rows that some query
 // sees, too (up to 7 % of the time: 100000 x 768 f32, 4 queries, 113 -> 120 us).
-// The loops over the columns are unrolled as measured: aligned rows twice for 1 and
-// 8 queries (100000 x 768 bf16, 1 query: 70 -> 60 us; not 300000 x 96 f32, 4
-// queries: 58 would be 67, nor 100000 x 768 f32, 1 query without TOP: 85 and 99),
-// unaligned ones four times in 16 bits (200000 x 75, 1
+// The loops over the columns are unrolled as measured: aligned rows twice for 1, 4
+// (TOP) and 8 queries (100000 x 768 bf16, 1 query: 70 -> 60 us, f32, 4 queries, TOP:
+// 130 -> 120; not 300000 x 96 f32, 4 queries without TOP: 58 would be 67, nor
+// 100000 x 768 f32, 1 query without TOP: 85 and 99), unaligned ones four times in 16 bits (200000 x 75, 1
 // query: 38 -> 28; f32 with 8 queries would go from 66 to 85).
 template <typename T, int NQ, bool VEC, bool TOP>
 __global__ void __launch_bounds__(64)
     few_kernel(const T* __restrict__ x, size_t ld, int n, int d, const T* __restrict__ q,
-               size_t ldq, int q0, int nq, float rf, const uint32_t* __restrict__ allowed,
+               size_t ldq, int nq, float rf, const uint32_t* __restrict__ allowed,
                size_t ld_allowed, float4* __restrict__ part, float2* __restrict__ top,
                size_t groups, float* __restrict__ size, int* __restrict__ err) {
     if (blockIdx.x == 0 && threadIdx.x == 0) *err = 0;  // (this path has no waits)
@@ -1431,7 +1431,7 @@ __global__ void __launch_bounds__(64)
     const int dp = (d + 127) & ~127;
     for (int i = threadIdx.x; i < NQ * dp; i += 64) {
         const int j = i / dp, c = i - j * dp;
-        qs[i] = j < nq && c < d ? to_f32<T>(q[(size_t)(q0 + j) * ldq + c]) : 0.0f;
+        qs[i] = j < nq && c < d ? to_f32<T>(q[(size_t)j * ldq + c]) : 0.0f;
     }
     __syncthreads();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -1452,7 +1452,7 @@ __global__ void __launch_bounds__(64)
         if (TOP) {
             seen = 0u;
             for (int j = 0; j < (allowed && ld_allowed ? nq : 1); ++j)
-                seen |= allowed_word(allowed, ld_allowed, q0 + j, (size_t)grp * GROUP, n);
+                seen |= allowed_word(allowed, ld_allowed, j, (size_t)grp * GROUP, n);
         }
         const int first = TOP ? __ffs(seen) - 1 : 0;
 #pragma unroll 1
@@ -1476,7 +1476,7 @@ __global__ void __launch_bounds__(64)
                 row[i] = x + (size_t)at * ld;
             }
             if (VEC) {
-#pragma unroll ((NQ == 1 && (TOP || sizeof(T) == 2)) || NQ == 8 ? 2 : 1)
+#pragma unroll ((NQ == 1 && (TOP || sizeof(T) == 2)) || (NQ == 4 && TOP) || NQ == 8 ? 2 : 1)
                 for (int c = lane * V; c < d; c += 32 * V) {
                     uint4 xv[RB];
 #pragma unroll
@@ -1574,7 +1574,7 @@ __global__ void __launch_bounds__(64)
         for (int j = 0; j < NQ; ++j) {
             if (j >= nq) break;
             const uint32_t w =
-                allowed_word(allowed, ld_allowed, q0 + j, (size_t)grp * GROUP, n);
+                allowed_word(allowed, ld_allowed, j, (size_t)grp * GROUP, n);
             const bool ok = w >> row_of_lane & 1u;
             if (ok) {
                 float dd = __fmaf_rn(sc[j], rf, -r[j].m);
@@ -2429,9 +2429,8 @@ static void launch_join(cudaStream_t s, int sms, const float* partial, int split
 // Every row is read and its gradient written once; what bounds it is the latency
 // of the two halves, which the blocks of a multiprocessor (registers: three of 1
 // or 2 queries, two of more) hide for each other: 100000 x 768 f32 takes 132 us
-// with 1 query and 249 with 8, where the bytes alone take 92.  The tensor-core
-// path, which copies the rows and pads the queries to 256, took 513 and 453 (bf16:
-// 113 and 248, was 257 and 240), and 2000 x 128 with 8 queries 34 us, here 11.
+// with 1 query and 252 with 8, where the bytes alone take 92 (bf16: 113 and 250, 46).
+// The tensor-core path copies the rows and pads the queries to 256: see FEW_GRAD.
 template <typename T>
 struct FewGrad {
     const T* x;
@@ -2657,13 +2656,17 @@ constexpr size_t CHUNK_BYTES = (size_t)512 << 20;  // of group maxima, of score 
 // of 128 columns, 694 in those of 256, whose waits and loads serve twice as
 // many
 constexpr size_t BLOCKS_F32 = 128, BLOCKS_F16 = 256, BLOCKS_BF16 = 768;
-constexpr int FEW = 8;                          // queries a pass of few_kernel takes
-// f32 rows would have to be split for the tensor cores first: two passes still
-// cost less; 16-bit rows are read by them as they are, if their alignment lets a
-// tensor map describe them (100000 x 376, 4 queries: 54 us here, 38 there), else
-// after a copy (100000 x 374: 58 and 70, with 8 queries 79 and 69).
-constexpr int FEW_F32 = 16, FEW_16 = 2, FEW_16_COPIED = 4, FEW_DIM = 2048;
-constexpr int FEW_GRAD = 8, FEW_GRAD_DIM = 1024;  // few_grad_kernel: see there
+// Queries that few_kernel takes.  f32 rows would have to be split for the tensor
+// cores first: 8 queries take 148 us here and 249 there (100000 x 768), 28 and 27
+// (2000 x 128); 12, in two passes, 239 and 251, but 46 and 27.  16-bit rows are
+// read by the tensor cores as they are, if their alignment lets a tensor map
+// describe them (100000 x 376, 4 queries: 54 us here, 38 there), else after a copy
+// (100000 x 374: 58 and 70, with 8 queries 79 and 69).
+constexpr int FEW_F32 = 8, FEW_16 = 2, FEW_16_COPIED = 4, FEW_DIM = 2048;
+// Queries and dimensions that few_grad_kernel takes (a call of 8: 100000 x 768 f32
+// 261 us, by the tensor cores 486; bf16 259 and 265, 300000 x 96 171 and 239, 2000 x
+// 128 19 and 56).
+constexpr int FEW_GRAD = 8, FEW_GRAD_DIM = 1024;
 static size_t smem_of(bool two, bool blk, bool grad) {
     // alignment, stages, staged outputs, barriers, column factors
     return 1024 + (size_t)stages_of(two, blk, grad) * stage_bytes(two, blk) +
@@ -2847,9 +2850,8 @@ static Forward plan_forward(const Ctx& c, const fdb_logprob_args& a) {
     w.nt = (int)((a.n + w.bn - 1) / w.bn);
     w.groups = w.few ? (a.n + GROUP - 1) / GROUP : (size_t)w.nt * (w.bn / GROUP);
     const size_t per = a.k ? w.groups * sizeof(float2) : 0;
-    w.qb = std::min<size_t>(a.nq, w.few ? (size_t)FEW
-                                  : per ? std::max<size_t>(PM, CHUNK_BYTES / per / PM * PM)
-                                        : (size_t)1 << 20);
+    w.qb = std::min<size_t>(a.nq, per ? std::max<size_t>(PM, CHUNK_BYTES / per / PM * PM)
+                                      : (size_t)1 << 20);
     if (w.packed) {
         w.qp = ws.take<__half>(a.nq * 2 * w.kp);
         w.xp = ws.take<__half>(a.n * 2 * w.kp);
@@ -2938,8 +2940,8 @@ static FinishArgs finish_args(const fdb_logprob_args& a, const Forward& w, size_
 // A kernel's limit is the process's, not the call's: it is set to the largest
 // size that any call takes, as two threads may launch the same kernel at once.
 template <typename T, int NQ, bool VEC, bool TOP>
-static void launch_few(const Ctx& c, const fdb_logprob_args& a, const Forward& w, int q0, int nq,
-                       float rf, size_t ld_allowed) {
+static void launch_few(const Ctx& c, const fdb_logprob_args& a, const Forward& w, float rf,
+                       size_t ld_allowed) {
     const size_t smem = NQ * up(a.dim, 128) * 4;
     if (smem > 40960) {  // (with the static part, over what needs no permission)
         static std::atomic<uint64_t> done{0};
@@ -2947,21 +2949,21 @@ static void launch_few(const Ctx& c, const fdb_logprob_args& a, const Forward& w
     }
     few_kernel<T, NQ, VEC, TOP><<<(unsigned)w.parts_cap, 64, smem, static_cast<cudaStream_t>(a.stream)>>>(
         static_cast<const T*>(a.rows), a.ld_rows, (int)a.n, (int)a.dim,
-        static_cast<const T*>(a.queries), a.ld_queries, q0, nq, rf, a.allowed, ld_allowed, w.part,
+        static_cast<const T*>(a.queries), a.ld_queries, (int)a.nq, rf, a.allowed, ld_allowed, w.part,
         w.top, w.groups, w.size, w.err);
     FDB_LAUNCH_CHECK();
 }
 template <typename T, int NQ, bool VEC>
-static void launch_few(const Ctx& c, const fdb_logprob_args& a, const Forward& w, int q0, int nq,
-                       float rf, size_t ld_allowed) {
-    if (w.top) launch_few<T, NQ, VEC, true>(c, a, w, q0, nq, rf, ld_allowed);
-    else launch_few<T, NQ, VEC, false>(c, a, w, q0, nq, rf, ld_allowed);
+static void launch_few(const Ctx& c, const fdb_logprob_args& a, const Forward& w, float rf,
+                       size_t ld_allowed) {
+    if (w.top) launch_few<T, NQ, VEC, true>(c, a, w, rf, ld_allowed);
+    else launch_few<T, NQ, VEC, false>(c, a, w, rf, ld_allowed);
 }
 template <typename T, int NQ>
-static void launch_few(bool vec, const Ctx& c, const fdb_logprob_args& a, const Forward& w, int q0,
-                       int nq, float rf, size_t ld_allowed) {
-    if (vec) launch_few<T, NQ, true>(c, a, w, q0, nq, rf, ld_allowed);
-    else launch_few<T, NQ, false>(c, a, w, q0, nq, rf, ld_allowed);
+static void launch_few(bool vec, const Ctx& c, const fdb_logprob_args& a, const Forward& w,
+                       float rf, size_t ld_allowed) {
+    if (vec) launch_few<T, NQ, true>(c, a, w, rf, ld_allowed);
+    else launch_few<T, NQ, false>(c, a, w, rf, ld_allowed);
 }
 template <typename T>
 static void few_run(const Ctx& c, const fdb_logprob_args& a, const Forward& w, float rf,
@@ -2969,20 +2971,17 @@ static void few_run(const Ctx& c, const fdb_logprob_args& a, const Forward& w, f
     const cudaStream_t s = static_cast<cudaStream_t>(a.stream);
     const bool vec = (reinterpret_cast<uintptr_t>(a.rows) & 15) == 0 &&
                      a.ld_rows * sizeof(T) % 16 == 0 && a.dim * sizeof(T) % 16 == 0;
-    for (size_t q = 0; q < a.nq; q += w.qb) {
-        const int nq = (int)std::min(w.qb, a.nq - q), q0 = (int)q;
-        if (nq == 1) launch_few<T, 1>(vec, c, a, w, q0, nq, rf, ld_allowed);
-        else if (nq == 2) launch_few<T, 2>(vec, c, a, w, q0, nq, rf, ld_allowed);
-        else if constexpr (sizeof(T) == 4) {
-            if (nq <= 4) launch_few<T, 4>(vec, c, a, w, q0, nq, rf, ld_allowed);
-            else launch_few<T, 8>(vec, c, a, w, q0, nq, rf, ld_allowed);
-        } else {  // (more than FEW_16: rows that would be copied, so unaligned ones)
-            launch_few<T, 4, false>(c, a, w, q0, nq, rf, ld_allowed);
-        }
-        FinishArgs f = finish_args(a, w, q, nq);
-        f.parts = f.sizes = (int)w.parts_cap;
-        launch_finish<T>(s, c.device, f);
+    if (a.nq == 1) launch_few<T, 1>(vec, c, a, w, rf, ld_allowed);
+    else if (a.nq == 2) launch_few<T, 2>(vec, c, a, w, rf, ld_allowed);
+    else if constexpr (sizeof(T) == 4) {
+        if (a.nq <= 4) launch_few<T, 4>(vec, c, a, w, rf, ld_allowed);
+        else launch_few<T, 8>(vec, c, a, w, rf, ld_allowed);
+    } else {  // (more than FEW_16: rows that would be copied, so unaligned ones)
+        launch_few<T, 4, false>(c, a, w, rf, ld_allowed);
     }
+    FinishArgs f = finish_args(a, w, 0, a.nq);
+    f.parts = f.sizes = (int)w.parts_cap;
+    launch_finish<T>(s, c.device, f);
 }
 
 void forward_run(Ctx& c, const fdb_logprob_args& a) {
