@@ -67,7 +67,7 @@ __host__ __device__ constexpr int staged_of(bool two, bool grad) {
 }
 constexpr int MAX_STG = 8;
 // K steps of an accumulator, sums in blocks
-__host__ __device__ constexpr int kblock_of(bool two, bool grad) { return grad ? 1 : two ? 2 : 4; }
+__host__ __device__ constexpr int kblock_of(bool two, bool grad) { return !two ? 4 : grad ? 1 : 2; }
 constexpr int MAX_BN = 256;
 constexpr unsigned long long DRAIN_CYCLES = 4000000ull;  // about 2 ms
 constexpr int THREADS = 640;                // 2 issuing warps, 2 idle, 16 epilogue warps
@@ -796,14 +796,14 @@ struct StatsEpilogue {
 // the query's W (see settle_kernel) so that both products read them as they are.
 // One part rounds G by up to 2^-11 of it, as a result in f16 is rounded and an
 // eighth of what a bf16 one is; a second part would cost a second product each.
-template <bool TWO>
+template <bool TWO, bool BLK>
 struct GradEpilogue {
     typedef GradArgs Args;
     const GradArgs& p;
     int q, row;
     bool live;  // (rows up to a multiple of 128 are written)
     Coef k;
-    Columns<true, false, TWO ? 1 : 2> c;
+    Columns<true, false, BLK ? 1 : 2> c;
     const uint32_t* al;
     unsigned char* stage;      // the warp's staged outputs, part 1 STAGED bytes on
     const CUtensorMap* omap;
@@ -987,9 +987,9 @@ template <bool TWO, bool BLK>
 struct EpilogueOf<STATS, TWO, BLK> {
     typedef StatsEpilogue<TWO, BLK> Type;
 };
-template <bool TWO>
-struct EpilogueOf<GRAD, TWO, TWO> {
-    typedef GradEpilogue<TWO> Type;
+template <bool TWO, bool BLK>
+struct EpilogueOf<GRAD, TWO, BLK> {
+    typedef GradEpilogue<TWO, BLK> Type;
 };
 template <bool TWO>
 struct EpilogueOf<PROD_Q, TWO, TWO> {
@@ -1050,8 +1050,8 @@ __device__ __forceinline__ Unit unit_of(const Mma& g, int u) {
 // that matters (f32, and long rows) sums are taken in blocks (BLK): an
 // accumulator holds 128 of K (TWO parts: first the products lo.hi and hi.lo,
 // then hi.hi) or 256, and the epilogue adds them up in registers.  Else an
-// accumulator is a whole tile.  GRAD takes 64 of K, whose sums it has the time
-// for: what a score is off by, its probability is off by of itself (d_rows of
+// accumulator is a whole tile.  GRAD takes 64 of K of two parts, whose sums it has
+// the time for: what a score is off by, its probability is off by of itself (d_rows of
 // 125 x 4405 x 74 f32: 1.3e-6 of its norm with 128, 4.6e-7 with 64 and the half
 // of cut_of; 60 us either way).
 template <int MODE, bool TWO, bool BLK>
@@ -2650,12 +2650,17 @@ __global__ void void_kernel(const int* err, void* dq, size_t ldq, int nq, void* 
 // ---------------------------------------------------------------------------
 constexpr size_t HEAD = 256;                    // error word, GradHead
 constexpr size_t CHUNK_BYTES = (size_t)512 << 20;  // of group maxima, of score gradients
-// dims above which a score's sum is taken in blocks: 2048 x 131072 x 768 bf16
-// takes 284 us with whole sums, so they stay while the loss is below 1e-6.
+// dims above which a score's sum is taken in blocks.  Whole sums are faster (2048 x
+// 131072 x 768 bf16: 284 us) and stay while half of what a sum of one sign loses
+// (see cut_of) is below 6e-7 of it: 768 bf16 (1.1e-6 in all), 256 f16 (0.8e-6).
 // Two parts of 128 are one block: 4096 x 262144 x 96 f32 takes 811 us in tiles
 // of 128 columns, 694 in those of 256, whose waits and loads serve twice as
-// many
+// many.  The gradient's scores of 16-bit rows only have to be as good as G, which
+// is held in 11 bits: at 1024 a score of 200 is off by 3.4e-4, less than the 4.9e-4
+// that G is rounded by; above it would grow to 5e-3 at 16384 (1000 x 50001: 1024
+// whole 328 us, in blocks 389; 2048 662 and 780).
 constexpr size_t BLOCKS_F32 = 128, BLOCKS_F16 = 256, BLOCKS_BF16 = 768;
+constexpr size_t BLOCKS_GRAD = 1024;
 // Queries that few_kernel takes.  f32 rows would have to be split for the tensor
 // cores first: 8 queries take 148 us here and 249 there (100000 x 768), 28 and 27
 // (2000 x 128); 12, in two passes, 239 and 251, but 46 and 27.  16-bit rows are
@@ -2776,12 +2781,10 @@ static int stays(bool two, bool blk, bool grad, int atoms) {
     return atoms * (two ? 2 : 1) * OPER <= stages_of(two, blk, grad) * stage_bytes(two, blk) / 2;
 }
 template <int MODE>
-static void launch_rows(bool two, cudaStream_t s, int device, int sms, const CUtensorMap& a,
-                        const CUtensorMap& b, const Mma& g,
-                        const typename EpilogueOf<MODE, false, false>::Type::Args& p,
-                        const CUtensorMap* out = nullptr) {
-    if (two) launch_rows<MODE, true, true>(s, device, sms, a, b, g, p, out);
-    else launch_rows<MODE, false, false>(s, device, sms, a, b, g, p, out);
+static void launch_product(bool two, cudaStream_t s, int device, int sms, const CUtensorMap& a,
+                           const CUtensorMap& b, const Mma& g, const ProdArgs& p) {
+    if (two) launch_rows<MODE, true, true>(s, device, sms, a, b, g, p);
+    else launch_rows<MODE, false, false>(s, device, sms, a, b, g, p);
 }
 
 // Hands out 256-byte aligned parts of the caller's workspace.
@@ -3073,6 +3076,7 @@ struct Backward {
     bool few;
     int parts, few_blocks;
     size_t kp, nqp, cols, ldg;  // cols: rows of a chunk
+    bool blocks;                // GRAD's sums
     int bn, q_splits, x_splits;
     size_t bytes;
     int* err;
@@ -3099,6 +3103,7 @@ static Backward plan_backward(const Ctx& c, const fdb_logprob_grad_args& a) {
     w.parts = a.dtype == FDB_DTYPE_F32 ? 2 : 1;
     w.kp = up(a.dim, 16);
     w.nqp = up(a.nq, BM);
+    w.blocks = w.parts == 2 || a.dim > BLOCKS_GRAD;
     w.bn = bn_of(w.parts == 2);
     const size_t row_bytes = w.nqp * 2 * w.parts;
     w.cols = std::min<size_t>(std::max<size_t>(MAX_BN, CHUNK_BYTES / row_bytes / MAX_BN * MAX_BN),
@@ -3185,7 +3190,7 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
     const size_t ld_allowed = a.allowed ? a.ld_allowed : 0;
     CoefArgs k{};
     k.nq = nq, k.n = n, k.scale = a.scale;
-    k.whole = 1.0 + cut_of(false, a.dim, w.parts == 2 ? 4 * kblock_of(true, true) : 0);
+    k.whole = 1.0 + cut_of(false, a.dim, w.blocks ? 4 * kblock_of(w.parts == 2, true) : 0);
     k.lse = a.lse, k.entropy = a.entropy;
     k.d_logprob = a.d_logprob, k.d_lse = a.d_lse, k.d_entropy = a.d_entropy;
     k.targets = a.targets, k.allowed = a.allowed, k.ld_allowed = ld_allowed;
@@ -3218,7 +3223,8 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
     const bool two = w.parts == 2;
     const int mtq = (int)((a.nq + PM - 1) / PM), ntd = (d + w.bn - 1) / w.bn;
     const CUtensorMap qk = map2d(FDB_DTYPE_F16, w.qp, width, a.nq, width, BM);
-    const CUtensorMap xk = map2d(FDB_DTYPE_F16, w.xp, width, a.n, width, w.bn / 2);
+    const int grad_bn = bn_of(w.blocks);
+    const CUtensorMap xk = map2d(FDB_DTYPE_F16, w.xp, width, a.n, width, grad_bn / 2);
     const CUtensorMap qm = map2d(FDB_DTYPE_F16, w.qs, width, a.nq, width, 64);
     const CUtensorMap xm = map2d(FDB_DTYPE_F16, w.xp, width, a.n, width, 64);
     const size_t g_rows = w.parts * w.nqp;
@@ -3235,11 +3241,11 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
         {
             Mma g = base;
             g.mt = mtq;
-            g.nt = (cols + w.bn - 1) / w.bn;
+            g.nt = (cols + grad_bn - 1) / grad_bn;
             g.chunks = pick_chunks(g.mt, g.nt, c.sm_count);
             g.atoms = (int)((w.kp + 63) / 64);
             g.klast = (int)((w.kp - 64 * (size_t)(g.atoms - 1)) / 16);
-            g.resident = stays(two, two, true, g.atoms);
+            g.resident = stays(two, w.blocks, true, g.atoms);
             g.a_part = g.b_part = (int)w.kp;
             g.b_row0 = (int)j0;
             g.idesc = idesc_of(FDB_DTYPE_F16, false, false);
@@ -3248,7 +3254,10 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
             p.coef = w.coef, p.xf = w.xf;
             p.allowed = a.allowed, p.ld_allowed = ld_allowed;
             p.ldg = w.ldg, p.nqp = (int)w.nqp, p.rest = w.rest;
-            launch_rows<GRAD>(two, s, c.device, c.sm_count, qk, xk, g, p, &go);
+            if (two) launch_rows<GRAD, true, true>(s, c.device, c.sm_count, qk, xk, g, p, &go);
+            else if (w.blocks)
+                launch_rows<GRAD, false, true>(s, c.device, c.sm_count, qk, xk, g, p, &go);
+            else launch_rows<GRAD, false, false>(s, c.device, c.sm_count, qk, xk, g, p, &go);
         }
         if (a.d_queries) {
             Mma g = base;
@@ -3263,7 +3272,7 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
             ProdArgs p{};
             p.rows = nq, p.cols = d, p.f = w.out_f;
             p.partial = w.dq, p.add = j0 > 0;
-            launch_rows<PROD_Q>(two, s, c.device, c.sm_count, gk, xm, g, p);
+            launch_product<PROD_Q>(two, s, c.device, c.sm_count, gk, xm, g, p);
         }
         if (a.d_rows) {
             Mma g = base;
@@ -3279,7 +3288,7 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
             p.rows = cols, p.cols = d, p.f = w.xf + j0, p.head = w.head;
             p.partial = w.dx;
             p.out = out, p.ldo = a.ld_d_rows, p.dtype = a.dtype;
-            launch_rows<PROD_X>(two, s, c.device, c.sm_count, gm, qm, g, p);
+            launch_product<PROD_X>(two, s, c.device, c.sm_count, gm, qm, g, p);
             if (w.dx) {
                 launch_join(s, c.sm_count, w.dx, w.x_splits, cols, d, w.xf + j0, w.head, out,
                             a.ld_d_rows, a.dtype);

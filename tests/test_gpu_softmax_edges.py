@@ -365,3 +365,32 @@ def test_a_product_out_of_range_that_is_masked(dtype, nq):
         assert all(torch.equal(a, b) for a, b in zip(*got))
     else:  # (d_rows' scale is that of the largest query: its terms are 1e-15 of it)
         assert all(torch.equal(a, b) for a, b in zip(got[0][:2], got[1][:2]))
+
+
+@pytest.mark.parametrize("dtype,size", [("f16", 200.0), ("bf16", 600.0)])
+@pytest.mark.parametrize("nq,n,dim", [(20, 300, 16384), (140, 900, 5000), (33, 700, 2049)])
+def test_long_rows_of_one_sign(dtype, size, nq, n, dim):
+    """Scores of hundreds that are sums of thousands of terms of one sign: the
+    tensor core's additions cut them all the same way, by up to 2^-22 of a sum
+    for each of its 16-wide steps, at most 17 in a block of 256; the blocks are
+    joined in f32.  The gradient's scores are those that the forward pass
+    summed."""
+    import forgegpu as fg
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(dim)
+    q = (torch.rand(nq, dim, device="cuda", generator=gen) + 0.5).to(_type(dtype))
+    x = (torch.rand(n, dim, device="cuda", generator=gen) + 0.5).to(_type(dtype))
+    scale = float(np.float32(size / dim))
+    Q, X = q.double(), x.double()
+    lse = torch.logsumexp(Q @ X.T * scale, 1).float()
+    up = torch.ones(nq, device="cuda")
+    dq, dx = fg.logprobs_backward(q, x, None, lse, d_lse=up, scale=scale)
+    P = torch.exp(Q @ X.T * scale - lse.double()[:, None])
+    es = (Q @ X.T * scale) * (17 * 2.0 ** -22 + (dim / 256 + 2) * 2.0 ** -24)
+    es = es + 2 * size * 2.0 ** -24  # (the score's factor, and t - lse, rounded to f32)
+    e = P * (es + 2.0 ** -19 + _held(dtype)) * scale
+    for got, want, b in ((dq, P @ X * scale, e @ X), (dx, P.T @ Q * scale, e.T @ Q)):
+        k = n if got is dq else nq
+        b = b * (1 + _cut(dtype, k)) + want * _cut(dtype, k) + HALF[dtype] * want + 2.0 ** -25
+        off = (got.double() - want).abs()
+        assert (off <= b).all(), (off / b).max()
