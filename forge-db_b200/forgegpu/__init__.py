@@ -1102,7 +1102,7 @@ def adamw_step(params, grads, m, v, *, lr: float, step: int = 1, betas=(0.9, 0.9
     """One AdamW step in place over lists of tensors, on the current stream
     (fdb_adamw_step in forgegpu.h).  With m_scales and v_scales the moments
     are 8-bit: m int8, v uint8, a float32 scale per 256 elements each.  To
-    autograd it is an in-place change of params and states."""
+    autograd it is an in-place change of params."""
     torch = _torch()
     count = len(params)
     eight = m_scales is not None or v_scales is not None
@@ -1138,8 +1138,8 @@ def adamw_step(params, grads, m, v, *, lr: float, step: int = 1, betas=(0.9, 0.9
                   _scalar(d_grad_scale, torch.float32, p0, "d_grad_scale"),
                   torch._C._cuda_getCurrentRawStream(dev.index))
     _check(lib().fdb_adamw_step(_ctx_of(dev).h, table.buffer_info()[0], count, C.byref(o)))
-    # (written through pointers: a graph that saved one of them has to notice)
-    torch.autograd.graph.increment_version(list(itertools.chain(params, *lists[2:])))
+    # (written through pointers: a graph that saved a param has to notice)
+    torch.autograd.graph.increment_version(params)
 
 
 def adamw_state_values(m, m_scale, v, v_scale):

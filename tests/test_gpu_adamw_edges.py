@@ -57,8 +57,8 @@ def test_a_block_without_v_has_no_m():
 
 @pytest.mark.parametrize("bits", [32, 8])
 def test_a_step_is_an_in_place_change_to_autograd(bits):
-    """A graph that saved a parameter or a state before the step refuses its
-    backward pass; results of logprobs have no history."""
+    """A graph that saved a parameter before the step refuses its backward
+    pass; results of logprobs have no history."""
     import forgegpu as fg
     import torch
     w = torch.nn.Parameter(torch.randn(300, device="cuda"))
@@ -71,10 +71,9 @@ def test_a_step_is_an_in_place_change_to_autograd(bits):
         v = [torch.zeros(300, dtype=torch.uint8, device="cuda")]
         kw = {k: [torch.zeros(2, device="cuda")] for k in ("m_scales", "v_scales")}
     loss = (w * w).sum()
-    written = [w, *m, *v, *(x for xs in kw.values() for x in xs)]
-    before = [x._version for x in written]
+    before = w._version
     fg.adamw_step([w], [g], m, v, lr=1e-2, **kw)
-    assert all(x._version > b for x, b in zip(written, before))
+    assert w._version > before
     with pytest.raises(RuntimeError):
         loss.backward()
     (w * w).sum().backward()
