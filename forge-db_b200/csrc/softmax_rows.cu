@@ -2212,16 +2212,21 @@ struct Upstream {
     float bound;
 };
 __device__ __forceinline__ Upstream upstream_of(const CoefArgs& a, int i) {
-    Upstream u;
-    u.empty = a.lse[i] == -INFINITY;
+    // (all loads but the filter's first: one after the other they take 2 us more)
+    const float lse = a.lse[i];
     const int64_t t = a.targets ? a.targets[i] : -1;
+    const float g = a.d_logprob ? a.d_logprob[i] : 0.0f, dl = a.d_lse ? a.d_lse[i] : 0.0f;
+    const float dh = a.d_entropy ? a.d_entropy[i] : 0.0f;
+    const float H = a.d_entropy ? a.entropy[i] : 0.0f;
+    Upstream u;
+    u.empty = lse == -INFINITY;
     const bool given = !u.empty && t >= 0 && t < a.n &&
                        (!a.allowed ||
                         (a.allowed[(size_t)i * a.ld_allowed + (size_t)(t >> 5)] >> (t & 31) & 1u));
-    u.g = given && a.d_logprob ? a.d_logprob[i] : 0.0;
-    u.dl = !u.empty && a.d_lse ? a.d_lse[i] : 0.0;
-    u.dh = !u.empty && a.d_entropy ? a.d_entropy[i] : 0.0;
-    u.H = u.dh != 0.0 ? (double)a.entropy[i] : 0.0;
+    u.g = given ? g : 0.0;
+    u.dl = u.empty ? 0.0 : dl;
+    u.dh = u.empty ? 0.0 : dh;
+    u.H = u.dh != 0.0 ? (double)H : 0.0;
     u.target = given ? (int)t : -1;
     u.bound = (float)(a.scale * (fabs(u.dl) + 2.0 * fabs(u.g) + fabs(u.dh) * (fabs(u.H) + 1.0)));
     return u;
@@ -3195,7 +3200,7 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
     k.d_logprob = a.d_logprob, k.d_lse = a.d_lse, k.d_entropy = a.d_entropy;
     k.targets = a.targets, k.allowed = a.allowed, k.ld_allowed = ld_allowed;
     k.out = w.coef, k.rest = w.rest;
-    head_kernel<<<(nq + 255) / 256, 256, 0, s>>>(k, w.alive, w.weight,
+    head_kernel<<<(nq + 63) / 64, 64, 0, s>>>(k, w.alive, w.weight,
                                                  reinterpret_cast<uint32_t*>(w.err), HEAD / 4);
     FDB_LAUNCH_CHECK();
     const uint32_t* seen = a.allowed;
