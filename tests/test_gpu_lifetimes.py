@@ -74,3 +74,42 @@ def test_a_failed_call_does_not_fail_the_next():
         got = again()
     assert np.array_equal(ix.batch_search_arrays(x[:3], 2)[0], want[0][0])
     assert torch.equal(got, want[1].lse)
+
+
+_CAPTURED = r"""
+import sys
+sys.path.insert(0, %r)
+import torch
+import forgegpu as fg
+q = torch.randn(20, 64, device="cuda")
+x = torch.randn(3000, 64, device="cuda")
+t = torch.arange(20, device="cuda")
+up = torch.rand(20, device="cuda")
+p, m, v = [x.clone()], [torch.zeros_like(x)], [torch.zeros_like(x)]
+
+def step():
+    r = fg.logprobs(q, x, t, scale=0.2, k=4)
+    d = fg.logprobs_backward(q, x, t, r.lse, d_logprob=up, scale=0.2)
+    fg.adamw_step(p, [d[1]], m, v, lr=1e-2)
+    return list(r) + list(d)
+
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):  # the first call of the process: its context is made here
+    out = step()
+g.replay()
+torch.cuda.synchronize()
+got = [a.clone() for a in out]
+assert all(torch.equal(a, b) for a, b in zip(got, step()))
+print("SAME")
+"""
+
+
+def test_the_first_call_of_a_process_is_captured():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", _CAPTURED % os.path.join(root, "forge-db_b200")],
+                       capture_output=True, text=True, timeout=180)
+    assert r.returncode == 0 and "SAME" in r.stdout, r.stderr[-3000:]
