@@ -18,7 +18,7 @@
 //
 // Bound by memory with f32 moments: f32 p, g, m, v move 28 bytes an element
 // (131072 x 768: 419 us, 6.7 TB/s).  bf16 p, g with 8-bit moments move 10, and
-// 147 instructions an element take longer than that (40 M elements: 198 us).
+// 147 instructions an element take longer than that (40 M elements: 203 us).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

@@ -138,7 +138,10 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
 }
 
 // A running (reference m, sum l = sum 2^(t - m), a = sum 2^(t - m) (t - m)) of
-// one query's columns, t = score * log2(e).  m starts at the first columns'
+// one query's columns, t = score * log2(e), in f32: the sums of 32 columns each are
+// added one after the other, a quarter of a unit's column tiles to a thread (at
+// most some 10^4 of them for a million rows: their roundings, of either sign, come
+// to a few 1e-6 of the sum).  m starts at the first columns'
 // largest t and is raised only when a t exceeds it by more than RAISE: the
 // sums then hold terms of at most 2^8 (f32's relative precision does not
 // care), and a new largest score seldom costs a rescaling.
@@ -796,6 +799,8 @@ struct StatsEpilogue {
 // the query's W (see settle_kernel) so that both products read them as they are.
 // One part rounds G by up to 2^-11 of it, as a result in f16 is rounded and an
 // eighth of what a bf16 one is; a second part would cost a second product each.
+// (d_queries gets back what is cut off the given row's G, d_rows does not: it would
+// take a sum over the queries that share a given row.)
 template <bool TWO, bool BLK>
 struct GradEpilogue {
     typedef GradArgs Args;

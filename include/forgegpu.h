@@ -551,7 +551,9 @@ int fdb_logprobs_status(fdb_ctx* ctx, const void* workspace, void* stream);
  * (host buffers, like fdb_bf_batch_search): p(row | query) with
  * scale = 1 / temperature.  target_ids[nq] (nullable): vector ids; an id that
  * the index does not hold gives a logprob of 0, a repeated id its first row.
- * top_ids / top_logprobs [nq][k], ids UINT64_MAX past the last row.  A
+ * top_ids / top_logprobs [nq][k], ids UINT64_MAX past the last row.  The index
+ * keeps the call's workspace (for more than 8 queries the rows as fp16 pairs, as
+ * large as the rows) until it is freed.  A
  * sharded index is FDB_ERR_UNSUPPORTED, an empty one FDB_ERR_EMPTY_VECTOR_SET. */
 int fdb_bf_logprobs(fdb_bf* h, const float* queries, size_t nq, float temperature,
                     const uint64_t* target_ids, size_t k, float* logprob, float* lse,
