@@ -241,8 +241,8 @@ struct PackSide {
     int rows;            // a warp's: 4 short ones or 1
     int wide;            // rows can be read in 16-byte vectors
 };
-// What the largest is taken of: the scales' bits, or, with weights, the exponents
-// of scale times weight, counted from 1.
+// What the largest is taken of: the scales' bits, or, with weights, WEIGHT_ZERO + the
+// exponent of scale times weight; 0 is none.
 constexpr int NO_WEIGHT = -10000;
 constexpr int WEIGHT_ZERO = 1024;
 __device__ __forceinline__ unsigned most_of(const PackSide& p, int row, float f) {
@@ -1419,8 +1419,8 @@ struct Largest<float> {
 // The loops over the columns are unrolled as measured: aligned rows twice for 1, 4
 // (TOP) and 8 queries (100000 x 768 bf16, 1 query: 70 -> 60 us, f32, 4 queries, TOP:
 // 130 -> 120; not 300000 x 96 f32, 4 queries without TOP: 58 would be 67, nor
-// 100000 x 768 f32, 1 query without TOP: 85 and 99), unaligned ones four times in 16 bits (200000 x 75, 1
-// query: 38 -> 28; f32 with 8 queries would go from 66 to 85).
+// 100000 x 768 f32, 1 query without TOP: 85 and 99), unaligned ones four times in 16
+// bits (200000 x 75, 1 query: 38 -> 28; f32 with 8 queries would go from 66 to 85).
 template <typename T, int NQ, bool VEC, bool TOP>
 __global__ void __launch_bounds__(64)
     few_kernel(const T* __restrict__ x, size_t ld, int n, int d, const T* __restrict__ q,
@@ -1834,7 +1834,10 @@ __global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kern
     float L = 0.0f, A = 0.0f;
     if (p.size) {
         float z = 0.0f;
-        for (int i = tid; i < p.sizes; i += THREADS_) z = fmaxf(z, p.size[i]);
+        for (int i = tid; i < p.sizes; i += THREADS_) {
+            const float v = p.size[i];  // (infinite: of a row that makes its queries NaN)
+            if (v <= FLT_MAX) z = fmaxf(z, v);
+        }
         const int w = __reduce_max_sync(0xffffffffu, __float_as_int(z));
         if (lane == 0) atomicMax(&s_size, w);
     }
@@ -1905,7 +1908,7 @@ __global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kern
                 if (sub == 0 && j < to) cs[j] = ordered64(v[r]);
             }
         }
-        if (p.k > 0 && !p.size) {
+        if (p.k > 0 && !p.xf) {
             const int w = __reduce_max_sync(0xffffffffu, __float_as_int(largest.get()));
             if (lane == 0) atomicMax(&s_size, w);
         }

@@ -394,3 +394,34 @@ def test_long_rows_of_one_sign(dtype, size, nq, n, dim):
         b = b * (1 + _cut(dtype, k)) + want * _cut(dtype, k) + HALF[dtype] * want + 2.0 ** -25
         off = (got.double() - want).abs()
         assert (off <= b).all(), (off / b).max()
+
+
+@pytest.mark.parametrize("dtype,nq", [("f32", 4), ("f32", 300), ("bf16", 2), ("bf16", 300)])
+def test_an_infinity_costs_its_queries_only(dtype, nq):
+    """One query sees a row with an infinity: the others' bits stay, and they are
+    not looked for in all rows (some hundred times the work)."""
+    import forgegpu as fg
+    import torch
+    n = 200000
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    q = torch.randn(nq, 96, device="cuda", generator=gen).to(_type(dtype))
+    x = torch.randn(n, 96, device="cuda", generator=gen).to(_type(dtype))
+    keep = torch.ones(nq, n, dtype=torch.bool)
+    keep[1:, 70000] = False
+    words = torch.from_numpy(so.words(keep.numpy())).cuda()
+    out, times = [], []
+    for value in (0.0, float("inf")):
+        x[70000] = value
+        ev = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+        for _ in range(3):
+            r = fg.logprobs(q, x, scale=0.1, allowed=words, k=10)
+        ev[0].record()
+        for _ in range(5):
+            r = fg.logprobs(q, x, scale=0.1, allowed=words, k=10)
+        ev[1].record()
+        torch.cuda.synchronize()
+        out.append(r)
+        times.append(ev[0].elapsed_time(ev[1]))
+    assert torch.isnan(out[1].lse[0]) and (out[1].top_ids[0] == -1).all()
+    assert all(torch.equal(a[1:], b[1:]) for a, b in zip(*out))
+    assert times[1] < 3 * times[0], times
