@@ -2268,8 +2268,7 @@ __global__ void head_kernel(const CoefArgs a, uint32_t* __restrict__ alive,
     if (q < a.nq) {
         const Upstream u = upstream_of(a, q);
         on = !u.empty;
-        weight[q] = u.bound > 0.0f && u.bound <= FLT_MAX ? max(-100, min(100, ilogbf(u.bound)))
-                                                         : NO_WEIGHT;
+        weight[q] = u.bound > 0.0f && u.bound <= FLT_MAX ? max(-110, ilogbf(u.bound)) : NO_WEIGHT;
     }
     const unsigned b = __ballot_sync(0xffffffffu, on);
     if ((threadIdx.x & 31) == 0 && q < a.nq) alive[q >> 5] = b;

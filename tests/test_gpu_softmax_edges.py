@@ -425,3 +425,22 @@ def test_an_infinity_costs_its_queries_only(dtype, nq):
     assert torch.isnan(out[1].lse[0]) and (out[1].top_ids[0] == -1).all()
     assert all(torch.equal(a[1:], b[1:]) for a, b in zip(*out))
     assert times[1] < 3 * times[0], times
+
+
+@pytest.mark.parametrize("nq", [5, 40])
+@pytest.mark.parametrize("shift", [-90, -60, 60, 115])
+def test_upstream_gradients_far_from_one(nq, shift):
+    """Upstream gradients times a power of two: the gradients times it, bit for
+    bit, up to the ends of f32's range."""
+    import forgegpu as fg
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    q = torch.randn(nq, 64, device="cuda", generator=gen)
+    x = torch.randn(800, 64, device="cuda", generator=gen)
+    t = torch.randint(0, 800, (nq,), device="cuda", generator=gen)
+    r = fg.logprobs(q, x, t, scale=0.2)
+    up = torch.rand(nq, device="cuda", generator=gen) + 0.1
+    dq, dx = fg.logprobs_backward(q, x, t, r.lse, d_logprob=up, scale=0.2)
+    two = 2.0 ** shift
+    eq, ex = fg.logprobs_backward(q, x, t, r.lse, d_logprob=up * two, scale=0.2)
+    assert torch.equal(eq, dq * two) and torch.equal(ex, dx * two)
