@@ -475,12 +475,12 @@ int fdb_bf_remove(fdb_bf* h, uint64_t id, int* removed);
  * probable rows in order, equal scores by row number, -1 and -inf past the
  * allowed rows.  A query that may see no row has lse -inf, entropy 0.  Scores
  * have to lie within +-1e28, as do the products q . x that they are scaled
- * from.  Scores are compared in 64 bits; with rows of 16 bits and more than two
- * queries (four if the rows are not 16-byte aligned) a row whose elements are
- * many times those of the rows near the kth may be left out where its score is
- * above the kth's by less than 2^-18 |q| sqrt(dim) of its largest element.  If a
- * query, or a row it may see, holds an infinity or NaN, the query's outputs
- * are NaN (top_ids -1). */
+ * from.  Scores are compared in 64 bits; with rows of 16 bits, and more than two
+ * queries (four if the rows are not 16-byte aligned) or more than 2048
+ * dimensions, a row whose elements are many times those of the rows near the
+ * kth may be left out where its score is above the kth's by less than
+ * 2^-18 |q| sqrt(dim) of its largest element.  If a query, or a row it may see,
+ * holds an infinity or NaN, the query's outputs are NaN (top_ids -1). */
 typedef struct fdb_logprob_args {
     int dtype; /* FDB_DTYPE_* of queries and rows */
     const void* queries;

@@ -39,6 +39,20 @@ def _lse(q, x, scale, step=128):
                       for i in range(0, q.shape[0], step)]).float()
 
 
+def _least_time(f, runs=8):
+    """The least time of a call on the device, of several."""
+    import torch
+    best = float("inf")
+    for _ in range(runs):
+        ev = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+        ev[0].record()
+        f()
+        ev[1].record()
+        torch.cuda.synchronize()
+        best = min(best, ev[0].elapsed_time(ev[1]))
+    return best
+
+
 @pytest.mark.parametrize("dtype,nq,n,dim", [
     ("bf16", 520, 50000, 64),    # one pass over the units
     ("bf16", 1000, 131072, 32),  # two
@@ -287,16 +301,8 @@ def test_a_row_that_is_not_seen_takes_no_part(dtype, nq, dim, bad, targets, filt
     out, times = [], []
     for value in (0.0, bad):
         x[:2] = value
-        ev = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
-        for _ in range(3):
-            r = fg.logprobs(q, x, t, scale=0.1, allowed=words, k=10)
-        ev[0].record()
-        for _ in range(5):
-            r = fg.logprobs(q, x, t, scale=0.1, allowed=words, k=10)
-        ev[1].record()
-        torch.cuda.synchronize()
-        out.append(r)
-        times.append(ev[0].elapsed_time(ev[1]))
+        out.append(fg.logprobs(q, x, t, scale=0.1, allowed=words, k=10))
+        times.append(_least_time(lambda: fg.logprobs(q, x, t, scale=0.1, allowed=words, k=10)))
     assert all(torch.equal(a, b) for a, b in zip(*out))
     assert times[1] < 3 * times[0], times
 
@@ -412,16 +418,8 @@ def test_an_infinity_costs_its_queries_only(dtype, nq):
     out, times = [], []
     for value in (0.0, float("inf")):
         x[70000] = value
-        ev = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
-        for _ in range(3):
-            r = fg.logprobs(q, x, scale=0.1, allowed=words, k=10)
-        ev[0].record()
-        for _ in range(5):
-            r = fg.logprobs(q, x, scale=0.1, allowed=words, k=10)
-        ev[1].record()
-        torch.cuda.synchronize()
-        out.append(r)
-        times.append(ev[0].elapsed_time(ev[1]))
+        out.append(fg.logprobs(q, x, scale=0.1, allowed=words, k=10))
+        times.append(_least_time(lambda: fg.logprobs(q, x, scale=0.1, allowed=words, k=10)))
     assert torch.isnan(out[1].lse[0]) and (out[1].top_ids[0] == -1).all()
     assert all(torch.equal(a[1:], b[1:]) for a, b in zip(*out))
     assert times[1] < 3 * times[0], times
