@@ -20,6 +20,7 @@
 #include "fdb_device.cuh"
 #include "fdb_internal.h"
 #include "fdb_kernels.h"
+#include "softmax_rows.cuh"
 
 namespace fdb {
 
@@ -156,16 +157,44 @@ static void check_softmax(const A& a) {
                 FDB_ERR_DIM_MISMATCH, "ld_allowed is below (n + 31) / 32 words");
 }
 template <class A>
-static void check_softmax_buffers(const A& a, size_t need) {
+static void check_workspace(const A& a, size_t need) {
+    FDB_REQUIRE(a.workspace && a.workspace_bytes >= need, FDB_ERR_INVALID_ARG,
+                "the workspace is too small: " + std::to_string(need) + " bytes are needed");
+    check_aligned(a.workspace, 256, "the workspace");
+}
+template <class A>
+static void check_operands(const A& a) {
     FDB_REQUIRE(a.queries && a.rows, FDB_ERR_INVALID_ARG, "NULL argument");
     const size_t es = a.dtype == FDB_DTYPE_F32 ? 4 : 2;
     check_aligned(a.queries, es, "queries");
     check_aligned(a.rows, es, "rows");
-    check_aligned(a.targets, 8, "targets");
     check_aligned(a.allowed, 4, "allowed");
-    FDB_REQUIRE(a.workspace && a.workspace_bytes >= need, FDB_ERR_INVALID_ARG,
-                "the workspace is too small: " + std::to_string(need) + " bytes are needed");
-    check_aligned(a.workspace, 256, "the workspace");
+}
+template <class A>
+static void check_softmax_buffers(const A& a, size_t need) {
+    check_operands(a);
+    check_aligned(a.targets, 8, "targets");
+    check_workspace(a, need);
+}
+
+// What a teacher's lists need, forward and backward.
+template <class A>
+static void check_teacher(const A& a) {
+    check_softmax(a);
+    FDB_REQUIRE(a.k >= 1 && a.k <= FDB_MAX_TEACHER, FDB_ERR_INVALID_ARG,
+                "k must be in [1, FDB_MAX_TEACHER]");
+    FDB_REQUIRE(a.ld_ids >= a.k && a.ld_logits >= a.k, FDB_ERR_DIM_MISMATCH,
+                "the teacher's rows overlap: ld is below k");
+    FDB_REQUIRE(a.teacher_scale > 0.0f && a.teacher_scale <= 3.0e38f, FDB_ERR_INVALID_ARG,
+                "teacher_scale must be positive and finite");
+    FDB_REQUIRE(!a.rest || a.teacher_scale == 1.0f, FDB_ERR_INVALID_ARG,
+                "log probabilities (rest) need a teacher_scale of 1");
+}
+template <class A>
+static void check_teacher_buffers(const A& a) {
+    FDB_REQUIRE(a.teacher_ids && a.teacher_logits, FDB_ERR_INVALID_ARG, "NULL teacher");
+    check_aligned(a.teacher_ids, 8, "teacher_ids");
+    check_aligned(a.teacher_logits, 4, "teacher_logits");
 }
 
 // A call without work has not timed out, whatever its workspace holds.
@@ -174,6 +203,24 @@ static void clear_status(int device, const A& a) {
     if (!a.workspace || a.workspace_bytes < 4) return;
     DeviceGuard g(device);
     FDB_CUDA(cudaMemsetAsync(a.workspace, 0, 4, static_cast<cudaStream_t>(a.stream)));
+}
+
+// The gradients' buffers; with no query the rows' gradient is zero and the call done.
+template <class A>
+static bool check_gradients(int device, const A& a) {
+    const size_t es = a.dtype == FDB_DTYPE_F32 ? 4 : 2;
+    FDB_REQUIRE(!a.d_queries || a.ld_d_queries >= a.dim, FDB_ERR_DIM_MISMATCH,
+                "d_queries rows overlap");
+    FDB_REQUIRE(!a.d_rows || a.ld_d_rows >= a.dim, FDB_ERR_DIM_MISMATCH, "d_rows rows overlap");
+    check_aligned(a.d_queries, es, "d_queries");
+    check_aligned(a.d_rows, es, "d_rows");
+    if (a.nq) return false;
+    DeviceGuard g(device);
+    if (a.d_rows)
+        FDB_CUDA(cudaMemset2DAsync(a.d_rows, a.ld_d_rows * es, 0, a.dim * es, a.n,
+                                   static_cast<cudaStream_t>(a.stream)));
+    clear_status(device, a);
+    return true;
 }
 
 // Pinned-or-not host <-> device staging for the host-buffer entry points.
@@ -1244,20 +1291,8 @@ int fdb_logprobs_backward(fdb_ctx* ctx, const fdb_logprob_grad_args* args) {
         FDB_REQUIRE(ctx && args, FDB_ERR_INVALID_ARG, "NULL argument");
         const fdb_logprob_grad_args& a = *args;
         check_softmax(a);
-        const size_t es = a.dtype == FDB_DTYPE_F32 ? 4 : 2;
-        FDB_REQUIRE(!a.d_queries || a.ld_d_queries >= a.dim, FDB_ERR_DIM_MISMATCH,
-                    "d_queries rows overlap");
-        FDB_REQUIRE(!a.d_rows || a.ld_d_rows >= a.dim, FDB_ERR_DIM_MISMATCH,
-                    "d_rows rows overlap");
-        check_aligned(a.d_queries, es, "d_queries");
-        check_aligned(a.d_rows, es, "d_rows");
+        if (check_gradients(ctx->c.device, a)) return;
         DeviceGuard g(ctx->c.device);
-        if (a.nq == 0) {  // no query: the rows' gradient is zero
-            if (a.d_rows)
-                FDB_CUDA(cudaMemset2DAsync(a.d_rows, a.ld_d_rows * es, 0, a.dim * es, a.n,
-                                           static_cast<cudaStream_t>(a.stream)));
-            return clear_status(ctx->c.device, a);
-        }
         FDB_REQUIRE(a.lse, FDB_ERR_INVALID_ARG, "lse is NULL");
         FDB_REQUIRE(!a.d_entropy || a.entropy, FDB_ERR_INVALID_ARG,
                     "d_entropy needs the entropy");
@@ -1278,6 +1313,149 @@ int fdb_logprobs_status(fdb_ctx* ctx, const void* workspace, void* stream) {
         FDB_CUDA(cudaMemcpyAsync(&err, workspace, 4, cudaMemcpyDeviceToHost, s));
         FDB_CUDA(cudaStreamSynchronize(s));
         FDB_REQUIRE(err == 0, FDB_ERR_TIMEOUT, "a wait inside the kernels ran out");
+    });
+}
+
+// ---------------------------------------------------------------------------
+// distillation
+// ---------------------------------------------------------------------------
+int fdb_distill_workspace(fdb_ctx* ctx, const fdb_distill_args* args, size_t* bytes) {
+    return guarded([&] {
+        FDB_REQUIRE(ctx && args && bytes, FDB_ERR_INVALID_ARG, "NULL argument");
+        check_teacher(*args);
+        *bytes = args->nq ? distill::forward_bytes(ctx->c, *args) : 0;
+    });
+}
+
+int fdb_distill(fdb_ctx* ctx, const fdb_distill_args* args) {
+    return guarded([&] {
+        FDB_REQUIRE(ctx && args, FDB_ERR_INVALID_ARG, "NULL argument");
+        const fdb_distill_args& a = *args;
+        check_teacher(a);
+        if (a.nq == 0) return clear_status(ctx->c.device, a);
+        check_operands(a);
+        check_teacher_buffers(a);
+        check_workspace(a, distill::forward_bytes(ctx->c, a));
+        for (const void* p : {(const void*)a.loss, (const void*)a.lse, (const void*)a.logprobs,
+                              (const void*)a.rest_logprob})
+            check_aligned(p, 4, "an output");
+        DeviceGuard g(ctx->c.device);
+        distill::forward_run(ctx->c, a);
+    });
+}
+
+int fdb_distill_backward_workspace(fdb_ctx* ctx, const fdb_distill_grad_args* args,
+                                   size_t* bytes) {
+    return guarded([&] {
+        FDB_REQUIRE(ctx && args && bytes, FDB_ERR_INVALID_ARG, "NULL argument");
+        check_teacher(*args);
+        *bytes = args->nq ? distill::backward_bytes(ctx->c, *args) : 256;
+    });
+}
+
+int fdb_distill_backward(fdb_ctx* ctx, const fdb_distill_grad_args* args) {
+    return guarded([&] {
+        FDB_REQUIRE(ctx && args, FDB_ERR_INVALID_ARG, "NULL argument");
+        const fdb_distill_grad_args& a = *args;
+        check_teacher(a);
+        if (check_gradients(ctx->c.device, a)) return;
+        FDB_REQUIRE(a.lse && a.logprobs && a.d_loss && (!a.rest || a.rest_logprob),
+                    FDB_ERR_INVALID_ARG, "lse, logprobs, rest_logprob or d_loss is NULL");
+        for (const float* p : {a.lse, a.logprobs, a.rest_logprob, a.d_loss})
+            check_aligned(p, 4, "an input");
+        check_operands(a);
+        check_teacher_buffers(a);
+        check_workspace(a, distill::backward_bytes(ctx->c, a));
+        if (!a.d_queries && !a.d_rows) return clear_status(ctx->c.device, a);
+        DeviceGuard g(ctx->c.device);
+        distill::backward_run(ctx->c, a);
+    });
+}
+
+// ---------------------------------------------------------------------------
+// beam search
+// ---------------------------------------------------------------------------
+static void check_beams(const fdb_beam_args& a) {
+    FDB_REQUIRE(a.dtype == FDB_DTYPE_F32 || a.dtype == FDB_DTYPE_F16 || a.dtype == FDB_DTYPE_BF16,
+                FDB_ERR_INVALID_ARG, "unknown dtype");
+    FDB_REQUIRE(a.n > 0, FDB_ERR_EMPTY_VECTOR_SET, "no columns");
+    FDB_REQUIRE(a.n < (1ull << 31) - 512, FDB_ERR_INVALID_ARG, "too many columns");
+    FDB_REQUIRE(a.beams >= 1 && a.beams <= FDB_MAX_BEAMS && a.width >= 1 &&
+                    a.width <= FDB_MAX_BEAMS,
+                FDB_ERR_INVALID_ARG, "beams and width must be in [1, FDB_MAX_BEAMS]");
+    FDB_REQUIRE(a.groups < (1ull << 22), FDB_ERR_INVALID_ARG, "too many groups");
+    FDB_REQUIRE(a.scale > 0.0f && a.scale <= 3.0e38f, FDB_ERR_INVALID_ARG,
+                "scale must be positive and finite");
+    FDB_REQUIRE((a.beams == 1 || a.ld_beam >= a.n) && a.ld_beam < (1ull << 40) &&
+                    a.ld_group < (1ull << 40),
+                FDB_ERR_DIM_MISMATCH, "chains overlap: ld_beam is below n");
+    FDB_REQUIRE(!a.ids || a.ld_ids >= a.n, FDB_ERR_DIM_MISMATCH, "ld_ids is below n");
+    FDB_REQUIRE(!a.allowed || a.ld_allowed == 0 || a.ld_allowed >= (a.n + 31) / 32,
+                FDB_ERR_DIM_MISMATCH, "ld_allowed is below (n + 31) / 32 words");
+}
+
+int fdb_beam_select_workspace(fdb_ctx* ctx, const fdb_beam_args* args, size_t* bytes) {
+    return guarded([&] {
+        FDB_REQUIRE(ctx && args && bytes, FDB_ERR_INVALID_ARG, "NULL argument");
+        check_beams(*args);
+        fdb_beam_args a = *args;
+        a.workspace = nullptr;
+        *bytes = a.groups ? beam::select_bytes(ctx->c, a) : 0;
+    });
+}
+
+int fdb_beam_select(fdb_ctx* ctx, const fdb_beam_args* args) {
+    return guarded([&] {
+        FDB_REQUIRE(ctx && args, FDB_ERR_INVALID_ARG, "NULL argument");
+        const fdb_beam_args& a = *args;
+        check_beams(a);
+        if (a.groups == 0) return;
+        FDB_REQUIRE(a.scores && a.beam_scores, FDB_ERR_INVALID_ARG, "NULL argument");
+        FDB_REQUIRE(a.out_scores && a.out_parents && a.out_ids, FDB_ERR_INVALID_ARG,
+                    "out_scores, out_parents or out_ids is NULL");
+        check_aligned(a.scores, a.dtype == FDB_DTYPE_F32 ? 4 : 2, "scores");
+        check_aligned(a.ids, 8, "ids");
+        check_aligned(a.allowed, 4, "allowed");
+        check_aligned(a.beam_scores, 4, "beam_scores");
+        check_aligned(a.out_scores, 4, "out_scores");
+        check_aligned(a.out_parents, 8, "out_parents");
+        check_aligned(a.out_ids, 8, "out_ids");
+        check_workspace(a, beam::select_bytes(ctx->c, a));
+        DeviceGuard g(ctx->c.device);
+        beam::select_run(ctx->c, a);
+    });
+}
+
+int fdb_beam_reorder(fdb_ctx* ctx, const fdb_beam_state* states, size_t count,
+                     const fdb_reorder_opts* opts) {
+    return guarded([&] {
+        FDB_REQUIRE(ctx && opts && (count == 0 || states), FDB_ERR_INVALID_ARG, "NULL argument");
+        const fdb_reorder_opts& o = *opts;
+        FDB_REQUIRE(o.beams >= 1 && o.beams <= FDB_MAX_BEAMS && o.width >= 1 &&
+                        o.width <= FDB_MAX_BEAMS,
+                    FDB_ERR_INVALID_ARG, "beams and width must be in [1, FDB_MAX_BEAMS]");
+        FDB_REQUIRE(o.groups < (1ull << 22), FDB_ERR_INVALID_ARG, "too many groups");
+        FDB_REQUIRE(o.groups == 0 || count == 0 || o.parents, FDB_ERR_INVALID_ARG,
+                    "parents is NULL");
+        check_aligned(o.parents, 8, "parents");
+        for (size_t i = 0; i < count; ++i) {
+            const fdb_beam_state& t = states[i];
+            if (t.bytes == 0 || t.parts == 0) continue;
+            FDB_REQUIRE(t.src && t.dst, FDB_ERR_INVALID_ARG, "NULL state");
+            FDB_REQUIRE(t.bytes < (1ull << 40) && t.parts < (1ull << 31) &&
+                            t.dst_stride < (1ull << 44) && t.src_stride < (1ull << 44),
+                        FDB_ERR_INVALID_ARG, "a state is too large");
+            FDB_REQUIRE(t.parts == 1 || t.dst_part_stride >= t.bytes, FDB_ERR_DIM_MISMATCH,
+                        "a state's runs overlap");
+            FDB_REQUIRE(t.src != t.dst ||
+                            (o.width == o.beams && t.src_stride == t.dst_stride &&
+                             (t.parts == 1 || t.src_part_stride == t.dst_part_stride)),
+                        FDB_ERR_INVALID_ARG,
+                        "in place needs a width of beams and the same strides");
+        }
+        if (o.groups == 0 || count == 0) return;
+        DeviceGuard g(ctx->c.device);
+        beam::reorder_run(ctx->c, states, count, o);
     });
 }
 

@@ -1,0 +1,449 @@
+// distill.cu -- the loss of a teacher's best rows under a softmax over all rows,
+// and its gradient.
+//
+//   P_e: the teacher's probabilities of the rows that it names, R = 1 - sum P
+//   loss = sum_e P_e (log P_e - log p_e) [+ R (log R - log r)]
+//   p_j = exp(s_j - lse),  r = sum of p over the rows that are not named
+//   dL/ds_j = p_j - P_j at a named row,  p_j (1 - R / r) elsewhere
+//
+// The sums over all rows and the products are fdb_logprobs' (softmax_rows.cu).
+// With `rest` the pass leaves the named rows out (by a filter for each query), as
+// r = 1 - sum p loses all of its bits once the student is sure; their scores, in
+// 64 bits, are joined to it.
+#include <cmath>
+
+#include "softmax_rows.cuh"
+
+namespace fdb {
+namespace distill {
+
+using sr::Carve;
+using sr::Exact;
+using sr::LN2;
+using sr::LOG2E;
+using sr::to_f32;
+using sr::up;
+
+constexpr int MAXK = FDB_MAX_TEACHER;
+constexpr size_t MASK_BYTES = (size_t)256 << 20;  // of one pass's filters
+
+struct Teacher {
+    const int64_t* ids;
+    const float* z;
+    size_t ld_ids, ld;  // ld: of z
+    int k, n;
+    double scale;
+    int rest;
+    const uint32_t* allowed;
+    size_t ld_allowed;
+};
+__device__ __forceinline__ bool sees(const Teacher& t, int q, int64_t id) {
+    return !t.allowed || (t.allowed[(size_t)q * t.ld_allowed + (size_t)(id >> 5)] >> (id & 31) & 1u);
+}
+// The row of an entry that may take part (whether an entry before it has the same
+// id is left), else -1.
+__device__ __forceinline__ int entry_row(const Teacher& t, int q, int e) {
+    const int64_t id = t.ids[(size_t)q * t.ld_ids + e];
+    if (id < 0 || id >= t.n || t.z[(size_t)q * t.ld + e] == -INFINITY || !sees(t, q, id)) return -1;
+    return (int)id;
+}
+
+// ---- sums and maxima over a block, the same bits in every thread ----
+template <int TH>
+__device__ __forceinline__ double block_sum(double v, double* part) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0.0;
+#pragma unroll
+    for (int i = 0; i < TH / 32; ++i) v += part[i];
+    return v;
+}
+// (a NaN is passed over: the sums that follow carry it)
+template <int TH>
+__device__ __forceinline__ double block_max(double v, double* part) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < TH / 32; ++i) v = fmax(v, part[i]);
+    return v;
+}
+
+// A query's entries in shared memory: the rows of those that take part, else -1.
+template <int TH>
+__device__ __forceinline__ void read_entries(const Teacher& t, int q, int* raw, int* row) {
+    for (int e = threadIdx.x; e < t.k; e += TH) raw[e] = entry_row(t, q, e);
+    __syncthreads();
+    for (int e = threadIdx.x; e < t.k; e += TH) {
+        int r = raw[e];
+        for (int i = 0; r >= 0 && i < e; ++i)
+            if (raw[i] == r) r = -1;
+        row[e] = r;
+    }
+    __syncthreads();
+}
+// log P of an entry is scale z - norm; left: R; any: some entry takes part.
+struct Norm {
+    double norm, left;
+    bool any;
+};
+template <int TH>
+__device__ __forceinline__ Norm teacher_norm(const Teacher& t, int q, const int* row, bool others,
+                                             double* part) {
+    const float* z = t.z + (size_t)q * t.ld;
+    double m = -INFINITY;
+    int mine = 0;
+    for (int e = threadIdx.x; e < t.k; e += TH)
+        if (row[e] >= 0) m = fmax(m, t.scale * (double)z[e]), mine = 1;
+    m = block_max<TH>(m, part);
+    const bool any = __syncthreads_or(mine);
+    double s = 0.0;
+    for (int e = threadIdx.x; e < t.k; e += TH)
+        if (row[e] >= 0) s += exp(t.scale * (double)z[e] - m);
+    s = block_sum<TH>(s, part);
+    Norm n{m + log(s), 0.0, any};
+    if (!any) {
+        n.norm = 0.0;
+        n.left = t.rest && others ? 1.0 : 0.0;
+    } else if (t.rest && others && !(n.norm > 0.0)) {
+        n.left = -expm1(n.norm);  // (NaN stays)
+        n.norm = n.norm == n.norm ? 0.0 : NAN;
+    }
+    return n;
+}
+
+// ---------------------------------------------------------------------------
+// forward
+// ---------------------------------------------------------------------------
+// Filters without the named rows, a block per query.  Bound by memory: the words
+// are written once.
+__global__ void __launch_bounds__(128)
+    filter_kernel(const Teacher t, int q0, uint32_t* __restrict__ out, size_t words) {
+    const int q = q0 + (int)blockIdx.x;
+    uint32_t* o = out + (size_t)blockIdx.x * words;
+    const uint32_t* al = t.allowed ? t.allowed + (size_t)q * t.ld_allowed : nullptr;
+    for (size_t w = threadIdx.x; w < words; w += 128) o[w] = al ? al[w] : 0xffffffffu;
+    __syncthreads();
+    for (int e = threadIdx.x; e < t.k; e += 128) {
+        const int r = entry_row(t, q, e);
+        if (r >= 0) atomicAnd(o + (r >> 5), ~(1u << (r & 31)));
+    }
+}
+
+struct LossArgs {
+    Teacher t;
+    sr::Parts parts;
+    const void *q, *x;
+    size_t ldq, ldx;
+    int d;
+    float scale;
+    float *loss, *lse, *logprobs, *rest;
+};
+// One block per query: the pass's sums joined, the named rows scored in 64 bits,
+// the loss.  Gathers k rows a query.
+template <typename T, int TH>
+__global__ void __launch_bounds__(TH) loss_kernel(const LossArgs p) {
+    extern __shared__ double qs_raw[];
+    typename Exact<T>::Q* qs = reinterpret_cast<typename Exact<T>::Q*>(qs_raw);  // [dim]
+    __shared__ int raw[MAXK], row[MAXK], list[MAXK];
+    __shared__ double score[MAXK], part[TH / 32];
+    __shared__ int count;
+    const int tid = threadIdx.x, ql = blockIdx.x, q = p.parts.q0 + ql;
+    const T* qp = static_cast<const T*>(p.q) + (size_t)q * p.ldq;
+    const T* xp = static_cast<const T*>(p.x);
+    if (tid == 0) count = 0;
+    for (int c = tid; c < p.d; c += TH) qs[c] = to_f32<T>(qp[c]);
+    read_entries<TH>(p.t, q, raw, row);
+    for (int e = tid; e < p.t.k; e += TH)
+        if (row[e] >= 0) list[atomicAdd(&count, 1)] = e;
+    __syncthreads();
+
+    // ---- the named rows' scores: 8 or 32 lanes a row, four rows at a time ----
+    constexpr int V = 16 / (int)sizeof(T), ROWS = 4;
+    const bool wide = ((reinterpret_cast<uintptr_t>(xp) | (p.ldx * sizeof(T))) & 15) == 0;
+    const int lanes = p.d * (int)sizeof(T) <= 512 ? 8 : 32, sub = tid & (lanes - 1);
+    const int named = count, per = TH / lanes;
+    for (int i = tid / lanes; i - tid / lanes < named; i += ROWS * per) {
+        const T* x[ROWS];
+        Exact<T> acc[ROWS];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+            x[r] = xp + (size_t)row[list[min(i + r * per, named - 1)]] * p.ldx;
+        int c = sub;
+        if (wide) {
+            for (c = sub * V; c + V <= p.d; c += lanes * V) {
+                uint4 v[ROWS];
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r) v[r] = __ldg(reinterpret_cast<const uint4*>(x[r] + c));
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r) {
+                    const T* e = reinterpret_cast<const T*>(&v[r]);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) acc[r].add(to_f32<T>(e[j]), qs[c + j]);
+                }
+            }
+            // (the row's last, partial vector: one lane's)
+            for (; c < p.d; ++c)
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r) acc[r].add(to_f32<T>(x[r][c]), qs[c]);
+        } else {
+#pragma unroll 4
+            for (; c < p.d; c += lanes)
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r) acc[r].add(to_f32<T>(x[r][c]), qs[c]);
+        }
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            double s = acc[r].sum();
+            for (int o = lanes >> 1; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            if (sub == 0 && i + r * per < named) score[list[i + r * per]] = s * (double)p.scale;
+        }
+    }
+
+    // ---- the pass's sums (see finish_kernel) ----
+    const sr::Parts& ps = p.parts;
+    float m = -INFINITY;
+    for (int i = tid; i < ps.parts; i += TH) m = fmaxf(m, ps.part[(size_t)i * ps.nq + ql].x);
+    const float M = (float)block_max<TH>((double)m, part);
+    double L = 0.0;
+    for (int i = tid; i < ps.parts; i += TH) {
+        const float4 v = ps.part[(size_t)i * ps.nq + ql];
+        if (v.y == 0.0f && v.z == 0.0f) continue;
+        L += v.z == v.z ? (double)(v.y * (v.x == M ? 1.0f : sr::ex2(v.x - M))) : NAN;
+    }
+    L = block_sum<TH>(L, part);
+    const bool bad = !(L == L) || *ps.err != 0;
+    // t was formed with f * rf, rounded to f32, from a sum that was cut
+    float f = 1.0f;
+    if (ps.qf) f = ps.qf[ql] == 0.0f ? 1.0f : ps.qf[ql];
+    const double unit = (double)p.scale * LOG2E;
+    const float rf = f * (float)unit;
+    const bool others = !p.t.rest || L > 0.0;
+    double lse = bad ? NAN : L > 0.0 ? LN2 * (double)M * ((double)f * unit / (double)rf * ps.whole) + log(L)
+                                     : -INFINITY;
+    const double rest_lse = lse;
+    // ---- with the rest, the named rows were left out ----
+    if (p.t.rest && named > 0) {
+        double t = -INFINITY;
+        for (int i = tid; i < named; i += TH) t = fmax(t, score[list[i]]);
+        t = fmax(block_max<TH>(t, part), rest_lse);
+        double s = 0.0;
+        for (int i = tid; i < named; i += TH) {
+            const double v = score[list[i]];
+            s += fabs(v) < INFINITY ? exp(v - t) : NAN;
+        }
+        s = block_sum<TH>(s, part) + exp(rest_lse - t);
+        lse = t + log(s);
+    }
+    const Norm nm = teacher_norm<TH>(p.t, q, row, others, part);
+    const float* z = p.t.z + (size_t)q * p.t.ld;
+    double loss = 0.0;
+    for (int e = tid; e < p.t.k; e += TH) {
+        const double lp = row[e] >= 0 ? score[e] - lse : 0.0;
+        if (row[e] >= 0) {
+            const double lt = p.t.scale * (double)z[e] - nm.norm, w = exp(lt);
+            if (!(w == 0.0)) loss += w * (lt - lp);
+        }
+        if (p.logprobs) p.logprobs[(size_t)q * p.t.k + e] = (float)(lse == lse ? lp : NAN);
+    }
+    loss = block_sum<TH>(loss, part);
+    if (tid != 0) return;
+    const double rest = lse == -INFINITY || rest_lse == -INFINITY ? -INFINITY : rest_lse - lse;
+    if (p.t.rest && nm.any && nm.left > 0.0) loss += nm.left * (log(nm.left) - rest);
+    // (not finite: a query or a row that counts, or a named row with a weight of 0)
+    if (!(lse == lse)) loss = NAN;
+    if (p.loss) p.loss[q] = (float)loss;
+    if (p.lse) p.lse[q] = (float)lse;
+    if (p.rest) p.rest[q] = (float)rest;
+}
+
+// ---------------------------------------------------------------------------
+// backward
+// ---------------------------------------------------------------------------
+struct CoefArgs {
+    Teacher t;
+    double scale;
+    const float *lse, *logprobs, *rest, *d_loss;
+    int* row;                         // [nq][k], see GivenRows
+    float *g, *at_least, *ref, *c;    // G elsewhere = scale c exp(s - ref)
+};
+// One block per query: what the score gradients are formed with.
+__global__ void __launch_bounds__(128) grad_kernel(const CoefArgs p) {
+    __shared__ int raw[MAXK], row[MAXK];
+    __shared__ double part[4];
+    const int tid = threadIdx.x, q = blockIdx.x;
+    read_entries<128>(p.t, q, raw, row);
+    const float lse = p.lse[q], rest = p.t.rest ? p.rest[q] : 0.0f;
+    const bool others = rest > -INFINITY || !(rest == rest);
+    const Norm nm = teacher_norm<128>(p.t, q, row, others, part);
+    const bool live = nm.any && lse != -INFINITY;
+    const double u = live ? (double)p.d_loss[q] : 0.0;
+    const size_t at = (size_t)q * p.t.k;
+    const float* z = p.t.z + (size_t)q * p.t.ld;
+    for (int e = tid; e < p.t.k; e += 128) {
+        p.row[at + e] = live ? row[e] : -1;
+        if (row[e] < 0) continue;
+        const double w = exp(p.t.scale * (double)z[e] - nm.norm);
+        p.g[at + e] = (float)(p.scale * u * (exp((double)p.logprobs[at + e]) - w));
+    }
+    if (tid != 0) return;
+    p.at_least[q] = (float)fabs(u);
+    p.ref[q] = others ? (float)((double)lse + (double)rest) : lse;
+    double c = u * ((p.t.rest ? exp((double)rest) : 1.0) - nm.left);
+    if (live && !(nm.norm == nm.norm)) c = NAN;
+    p.c[q] = live ? (float)c : 0.0f;
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+template <typename A>
+static Teacher teacher_of(const A& a) {
+    Teacher t{};
+    t.ids = a.teacher_ids, t.z = a.teacher_logits;
+    t.ld_ids = a.ld_ids, t.ld = a.ld_logits;
+    t.k = (int)a.k, t.n = (int)a.n;
+    t.scale = a.teacher_scale, t.rest = a.rest != 0;
+    t.allowed = a.allowed, t.ld_allowed = a.allowed ? a.ld_allowed : 0;
+    return t;
+}
+template <typename H, typename A>
+static H head_of(const A& a) {
+    H h{};
+    h.dtype = a.dtype;
+    h.queries = a.queries, h.nq = a.nq, h.ld_queries = a.ld_queries;
+    h.rows = a.rows, h.n = a.n, h.ld_rows = a.ld_rows;
+    h.dim = a.dim, h.scale = a.scale;
+    h.allowed = a.allowed, h.ld_allowed = a.ld_allowed;
+    h.workspace = a.workspace, h.stream = a.stream;
+    return h;
+}
+
+struct Plan {
+    fdb_logprob_args head;
+    size_t words, queries;  // of a filter, of a pass (0: any)
+    uint32_t* filters;
+    size_t bytes;
+};
+static Plan plan_forward(const Ctx& c, const fdb_distill_args& a) {
+    Plan p{};
+    p.head = head_of<fdb_logprob_args>(a);
+    p.words = (a.n + 31) / 32;
+    if (a.rest) {
+        // (the filters are the pass's: the address only has to say that there are some)
+        p.queries = std::min(a.nq, std::max<size_t>(256, MASK_BYTES / (p.words * 4) / 256 * 256));
+        p.head.allowed = reinterpret_cast<const uint32_t*>(256);
+        p.head.ld_allowed = p.words;
+    }
+    p.bytes = up(sr::forward_bytes(c, p.head, p.queries), 256);
+    if (a.rest) {
+        p.filters = reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(a.workspace) + p.bytes);
+        p.bytes += up(p.queries * p.words * 4, 256);
+    }
+    return p;
+}
+size_t forward_bytes(const Ctx& c, const fdb_distill_args& a) { return plan_forward(c, a).bytes; }
+
+template <typename T, int TH>
+static void launch_loss(cudaStream_t s, int device, const LossArgs& p) {
+    const size_t smem = (size_t)p.d * sizeof(typename Exact<T>::Q);
+    if (smem > 32768) {  // (with the static part, over what needs no permission)
+        static std::atomic<uint64_t> done{0};
+        sr::allow_smem(loss_kernel<T, TH>, device,
+                       FDB_MAX_SOFTMAX_DIM * sizeof(typename Exact<T>::Q), done);
+    }
+    loss_kernel<T, TH><<<p.parts.nq, TH, smem, s>>>(p);
+    FDB_LAUNCH_CHECK();
+}
+template <typename T>
+static void launch_loss(cudaStream_t s, int device, const LossArgs& p) {
+    // (few queries: more threads share the rows of one)
+    if (p.parts.nq <= 296) launch_loss<T, 512>(s, device, p);
+    else launch_loss<T, 128>(s, device, p);
+}
+
+struct End : sr::ForwardEnd {
+    const Ctx& c;
+    const fdb_distill_args& a;
+    const Plan& plan;
+    cudaStream_t s;
+    End(const Ctx& c_, const fdb_distill_args& a_, const Plan& p)
+        : c(c_), a(a_), plan(p), s(static_cast<cudaStream_t>(a_.stream)) {
+        queries = p.queries;
+    }
+    const uint32_t* filters(size_t q0, size_t nq) override {
+        const Teacher t = teacher_of(a);
+        if (!a.rest) return a.allowed + q0 * a.ld_allowed;
+        filter_kernel<<<(unsigned)nq, 128, 0, s>>>(t, (int)q0, plan.filters, plan.words);
+        FDB_LAUNCH_CHECK();
+        return plan.filters;
+    }
+    void finish(const sr::Parts& parts) override {
+        LossArgs p{};
+        p.t = teacher_of(a);
+        p.parts = parts;
+        p.q = a.queries, p.ldq = a.ld_queries;
+        p.x = a.rows, p.ldx = a.ld_rows;
+        p.d = (int)a.dim, p.scale = a.scale;
+        p.loss = a.loss, p.lse = a.lse, p.logprobs = a.logprobs;
+        p.rest = a.rest ? a.rest_logprob : nullptr;
+        if (a.dtype == FDB_DTYPE_F32) launch_loss<float>(s, c.device, p);
+        else if (a.dtype == FDB_DTYPE_F16) launch_loss<__half>(s, c.device, p);
+        else launch_loss<__nv_bfloat16>(s, c.device, p);
+    }
+};
+void forward_run(Ctx& c, const fdb_distill_args& a) {
+    const Plan p = plan_forward(c, a);
+    End end(c, a, p);
+    sr::forward_run(c, p.head, &end);
+}
+
+struct BackwardPlan {
+    fdb_logprob_grad_args head;
+    sr::GivenRows given;
+    CoefArgs k;
+    size_t bytes;
+};
+static BackwardPlan plan_backward(const Ctx& c, const fdb_distill_grad_args& a) {
+    BackwardPlan p{};
+    p.head = head_of<fdb_logprob_grad_args>(a);
+    p.head.d_queries = a.d_queries, p.head.ld_d_queries = a.ld_d_queries;
+    p.head.d_rows = a.d_rows, p.head.ld_d_rows = a.ld_d_rows;
+    p.given.k = (int)a.k;
+    const size_t first = up(sr::backward_bytes(c, p.head, &p.given), 256);
+    Carve ws(a.workspace ? static_cast<unsigned char*>(a.workspace) + first : nullptr);
+    CoefArgs& k = p.k;
+    k.row = ws.take<int>(a.nq * a.k);
+    k.g = ws.take<float>(a.nq * a.k);
+    k.at_least = ws.take<float>(a.nq);
+    k.ref = ws.take<float>(a.nq);
+    k.c = ws.take<float>(a.nq);
+    p.given.row = k.row, p.given.g = k.g, p.given.at_least = k.at_least;
+    p.head.lse = k.ref, p.head.d_lse = k.c;
+    p.bytes = first + ws.at;
+    return p;
+}
+size_t backward_bytes(const Ctx& c, const fdb_distill_grad_args& a) {
+    fdb_distill_grad_args b = a;
+    b.workspace = nullptr;
+    return plan_backward(c, b).bytes;
+}
+void backward_run(Ctx& c, const fdb_distill_grad_args& a) {
+    BackwardPlan p = plan_backward(c, a);
+    CoefArgs& k = p.k;
+    k.t = teacher_of(a);
+    k.scale = a.scale;
+    k.lse = a.lse, k.logprobs = a.logprobs, k.rest = a.rest_logprob, k.d_loss = a.d_loss;
+    grad_kernel<<<(unsigned)a.nq, 128, 0, static_cast<cudaStream_t>(a.stream)>>>(k);
+    FDB_LAUNCH_CHECK();
+    sr::backward_run(c, p.head, &p.given);
+}
+
+}  // namespace distill
+}  // namespace fdb

@@ -500,14 +500,24 @@ void ivf_tc_rescan(fdb_ivfpq* h, const ScanParams& base, size_t nq, size_t k, in
 void bf_upload(fdb_bf* h);
 // softmax_rows.cu: log probabilities under a softmax over rows, their gradient
 namespace sr {
-size_t forward_bytes(const Ctx& c, const fdb_logprob_args& a);
-void forward_run(Ctx& c, const fdb_logprob_args& a);
-size_t backward_bytes(const Ctx& c, const fdb_logprob_grad_args& a);
-void backward_run(Ctx& c, const fdb_logprob_grad_args& a);
 // slot[i] (preset to -1): the first row whose id is sorted[i]
 void launch_find_rows(cudaStream_t s, const uint64_t* ids, size_t n, const uint64_t* sorted,
                       size_t count, unsigned long long* slot);
 }  // namespace sr
+// distill.cu
+namespace distill {
+size_t forward_bytes(const Ctx& c, const fdb_distill_args& a);
+void forward_run(Ctx& c, const fdb_distill_args& a);
+size_t backward_bytes(const Ctx& c, const fdb_distill_grad_args& a);
+void backward_run(Ctx& c, const fdb_distill_grad_args& a);
+}  // namespace distill
+// beam.cu
+namespace beam {
+size_t select_bytes(const Ctx& c, const fdb_beam_args& a);
+void select_run(const Ctx& c, const fdb_beam_args& a);
+void reorder_run(const Ctx& c, const fdb_beam_state* states, size_t count,
+                 const fdb_reorder_opts& o);
+}  // namespace beam
 // adamw.cu
 namespace adamw {
 void step(cudaStream_t s, int sms, const fdb_adamw_tensor* ts, size_t count,

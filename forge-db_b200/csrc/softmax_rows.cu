@@ -34,6 +34,7 @@
 #include <cmath>
 
 #include "fdb_internal.h"
+#include "softmax_rows.cuh"
 #include "tc_ptx.cuh"
 
 namespace fdb {
@@ -82,13 +83,7 @@ static_assert(FDB_MAX_ALTERNATIVES + PAD <= 128, "the bound is one of 128 maxima
 constexpr float NONE = -1e30f;              // score of a row that may not be seen
 constexpr float NONE_BELOW = -1e29f;
 constexpr float RAISE = 8.0f;               // see Run
-constexpr double LOG2E = 1.4426950408889634074, LN2 = 0.69314718055994530942;
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ float lo_of(uint64_t v) {
     uint32_t a, b;
     asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
@@ -113,28 +108,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
-}
-
-template <typename T>
-__device__ __forceinline__ float to_f32(T v);
-template <>
-__device__ __forceinline__ float to_f32<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
-template <>
-__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) {
-    return __bfloat162float(v);
-}
-
-template <typename T>
-__device__ __forceinline__ T from_f32(float v);
-template <>
-__device__ __forceinline__ float from_f32<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
-    return __float2bfloat16_rn(v);
 }
 
 // A running (reference m, sum l = sum 2^(t - m), a = sum 2^(t - m) (t - m)) of
@@ -1688,23 +1661,8 @@ __device__ __forceinline__ double unordered64(uint64_t u) {
     return __longlong_as_double((long long)(u >> 63 ? u & 0x7fffffffffffffffull : ~u));
 }
 
-// q . x of ROWS rows in 64 bits over `lanes` lanes (a power of two).  f32:
-// products and sums in 64 bits (of a 64-bit copy of q); 16-bit types: the
-// products are exact in f32, the sums in 64 bits.  z: the largest element.
-template <typename T>
-struct Exact {
-    typedef float Q;
-    double s = 0.0;
-    __device__ __forceinline__ void add(float x, float q) { s += (double)__fmul_rn(x, q); }
-    __device__ __forceinline__ double sum() const { return s; }
-};
-template <>
-struct Exact<float> {
-    typedef double Q;
-    double s = 0.0;
-    __device__ __forceinline__ void add(float x, double q) { s = fma((double)x, q, s); }
-    __device__ __forceinline__ double sum() const { return s; }
-};
+// q . x of ROWS rows in 64 bits (see Exact) over `lanes` lanes (a power of two).
+// z: the largest element.
 template <int ROWS, typename T>
 __device__ __forceinline__ void dot_lanes(const T* const (&x)[ROWS],
                                           const typename Exact<T>::Q* q, int d, int sub, int lanes,
@@ -2211,6 +2169,7 @@ struct CoefArgs {
     size_t ld_allowed;
     Coef* out;
     float* rest;  // nullable
+    const float* at_least;  // nullable, see GivenRows
 };
 // What reaches a query's scores, and a bound B of its G's size (p |lp| <= 1/e).
 struct Upstream {
@@ -2237,6 +2196,7 @@ __device__ __forceinline__ Upstream upstream_of(const CoefArgs& a, int i) {
     u.H = u.dh != 0.0 ? (double)H : 0.0;
     u.target = given ? (int)t : -1;
     u.bound = (float)(a.scale * (fabs(u.dl) + 2.0 * fabs(u.g) + fabs(u.dh) * (fabs(u.H) + 1.0)));
+    if (a.at_least) u.bound = fmaxf(u.bound, (float)(a.scale * (double)a.at_least[i]));
     return u;
 }
 // G_ij = scale [ p_ij (dl - g - h (lp_ij + H)) + g 1{j = t} ] with lp = ln2 x:
@@ -2346,10 +2306,56 @@ __global__ void __launch_bounds__(256)
     }
     if (row < a.n) xf[row] = !(v > 0.0f) ? 1.0f : small ? 0x1p-4f : ldexpf(v, -lx);
 }
+// The score gradients at rows that are given with theirs (see GivenRows), one warp
+// per query, over what GRAD has left there.  One part: the largest of what fp16
+// leaves of a query's is added to its d_queries, as GRAD's given row's is (one of
+// them is most of the sum where it counts).
+struct GivenArgs {
+    GivenRows given;
+    int nq;
+    const int* weight;
+    const float* xf;  // (as settle_kernel left them)
+    __half* gr;
+    size_t ldg;
+    int nqp, parts, j0, cols;  // this chunk
+    float* rest;               // of all chunks, and its row; null: not now
+    int* rest_row;
+};
+__global__ void __launch_bounds__(256) given_kernel(const GivenArgs p) {
+    const int lane = threadIdx.x & 31, q = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (q >= p.nq) return;
+    const int e = p.weight[q];
+    const float w = e == NO_WEIGHT ? 1.0f : ldexpf(1.0f, min(13 - e, 127));
+    const size_t at = (size_t)q * p.given.k;
+    float most = 0.0f;
+    int most_row = -1;
+    for (int i = lane; i < p.given.k; i += 32) {
+        const int row = p.given.row[at + i];
+        if (row < 0) continue;
+        const float v = p.given.g[at + i] * w * p.xf[row];
+        const __half hi = __float2half_rn(v);
+        const float left = v - __half2float(hi);
+        const int col = row - p.j0;
+        if ((unsigned)col < (unsigned)p.cols) {
+            p.gr[(size_t)q * p.ldg + col] = hi;
+            if (p.parts == 2)
+                p.gr[(size_t)(p.nqp + q) * p.ldg + col] = __float2half_rn(left);
+        }
+        if (fabsf(left) > fabsf(most)) most = left, most_row = row;
+    }
+    if (!p.rest) return;
+    const float top = __int_as_float(__reduce_max_sync(0xffffffffu, __float_as_int(fabsf(most))));
+    const unsigned who = __ballot_sync(0xffffffffu, most_row >= 0 && fabsf(most) == top);
+    if (who && lane == __ffs(who) - 1) {
+        p.rest[q] = most;
+        p.rest_row[q] = most_row;
+    }
+}
 // d_queries of 16-bit inputs: rest[r] times the given row is added (see GRAD).
 struct JoinRest {
     const float* rest;  // null: nothing
-    const Coef* coef;
+    const int* row;     // `step` apart
+    int step;
     const __half* x;
     int ldx;
 };
@@ -2403,7 +2409,7 @@ __global__ void __launch_bounds__(256)
             if (rest.rest) {
                 const float g = rest.rest[r];
                 if (g != 0.0f) {
-                    const __half* x = rest.x + (size_t)rest.coef[r].target * rest.ldx + k;
+                    const __half* x = rest.x + (size_t)rest.row[r * rest.step] * rest.ldx + k;
                     v.x = __fmaf_rn(g, __half2float(x[0]), v.x);
                     if (k + 1 < cols) v.y = __fmaf_rn(g, __half2float(x[1]), v.y);
                     if (k + 2 < cols) v.z = __fmaf_rn(g, __half2float(x[2]), v.z);
@@ -2690,7 +2696,6 @@ static size_t smem_of(bool two, bool blk, bool grad) {
            staged_of(two, grad) + 256 + EPI_WARPS * 128 * 4;
 }
 
-static size_t up(size_t v, size_t m) { return (v + m - 1) / m * m; }
 static void launch_align(cudaStream_t s, const void* x, size_t ld, size_t n, size_t d, size_t kp,
                          void* out) {
     // lanes for a row's 16-byte pieces: 8 to 32, so that the fewest are idle at its
@@ -2761,14 +2766,6 @@ static int pick_splits(int tiles, int atoms, int sms, bool two, double out_bytes
     }
     return best;
 }
-// Raises a kernel's shared-memory limit once per device.
-template <typename K>
-static void allow_smem(K* kernel, int device, size_t bytes, std::atomic<uint64_t>& done) {
-    if (device < 64 && done.load(std::memory_order_acquire) >> device & 1u) return;
-    FDB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-    if (device < 64) done.fetch_or(1ull << device, std::memory_order_release);
-}
-
 static unsigned blocks_of(int sms, long long units) {
     return 2 * (unsigned)std::min<long long>(units, sms / 2);
 }
@@ -2798,19 +2795,6 @@ static void launch_product(bool two, cudaStream_t s, int device, int sms, const 
     if (two) launch_rows<MODE, true, true>(s, device, sms, a, b, g, p);
     else launch_rows<MODE, false, false>(s, device, sms, a, b, g, p);
 }
-
-// Hands out 256-byte aligned parts of the caller's workspace.
-struct Carve {
-    unsigned char* base;
-    size_t at = 0;
-    explicit Carve(void* b) : base(static_cast<unsigned char*>(b)) {}
-    template <typename T>
-    T* take(size_t count) {
-        T* p = base ? reinterpret_cast<T*>(base + at) : nullptr;
-        at += up(count * sizeof(T), 256);
-        return p;
-    }
-};
 
 static PackSide pack_side(const void* x, size_t ld, size_t n, size_t dim, int dtype,
                           const uint32_t* seen, __half* out, float* f, unsigned* largest) {
@@ -2849,7 +2833,7 @@ struct Forward {
 static bool mappable(const void* p, size_t ld) {
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * 2 & 15) == 0;
 }
-static Forward plan_forward(const Ctx& c, const fdb_logprob_args& a) {
+static Forward plan_forward(const Ctx& c, const fdb_logprob_args& a, size_t pass_queries) {
     Forward w{};
     Carve ws(a.workspace);
     w.err = ws.take<int>(HEAD / 4);
@@ -2867,6 +2851,7 @@ static Forward plan_forward(const Ctx& c, const fdb_logprob_args& a) {
     const size_t per = a.k ? w.groups * sizeof(float2) : 0;
     w.qb = std::min<size_t>(a.nq, per ? std::max<size_t>(PM, CHUNK_BYTES / per / PM * PM)
                                       : (size_t)1 << 20);
+    if (pass_queries) w.qb = std::min(w.qb, pass_queries);
     if (w.packed) {
         w.qp = ws.take<__half>(a.nq * 2 * w.kp);
         w.xp = ws.take<__half>(a.n * 2 * w.kp);
@@ -2895,10 +2880,10 @@ static Forward plan_forward(const Ctx& c, const fdb_logprob_args& a) {
     w.bytes = ws.at;
     return w;
 }
-size_t forward_bytes(const Ctx& c, const fdb_logprob_args& a) {
+size_t forward_bytes(const Ctx& c, const fdb_logprob_args& a, size_t pass_queries) {
     fdb_logprob_args b = a;
     b.workspace = nullptr;
-    return plan_forward(c, b).bytes;
+    return plan_forward(c, b, pass_queries).bytes;
 }
 
 template <typename T, int THREADS_>
@@ -2952,8 +2937,9 @@ static FinishArgs finish_args(const fdb_logprob_args& a, const Forward& w, size_
     return f;
 }
 
-// A kernel's limit is the process's, not the call's: it is set to the largest
-// size that any call takes, as two threads may launch the same kernel at once.
+static Parts parts_of(const FinishArgs& f) {
+    return Parts{f.part, f.parts, f.q0, f.nq, f.qf, f.whole, f.err};
+}
 template <typename T, int NQ, bool VEC, bool TOP>
 static void launch_few(const Ctx& c, const fdb_logprob_args& a, const Forward& w, float rf,
                        size_t ld_allowed) {
@@ -2982,7 +2968,7 @@ static void launch_few(bool vec, const Ctx& c, const fdb_logprob_args& a, const 
 }
 template <typename T>
 static void few_run(const Ctx& c, const fdb_logprob_args& a, const Forward& w, float rf,
-                    size_t ld_allowed) {
+                    size_t ld_allowed, ForwardEnd* end) {
     const cudaStream_t s = static_cast<cudaStream_t>(a.stream);
     const bool vec = (reinterpret_cast<uintptr_t>(a.rows) & 15) == 0 &&
                      a.ld_rows * sizeof(T) % 16 == 0 && a.dim * sizeof(T) % 16 == 0;
@@ -2996,12 +2982,17 @@ static void few_run(const Ctx& c, const fdb_logprob_args& a, const Forward& w, f
     }
     FinishArgs f = finish_args(a, w, 0, a.nq);
     f.parts = f.sizes = (int)w.parts_cap;
-    launch_finish<T>(s, c.device, f);
+    if (end) end->finish(parts_of(f));
+    else launch_finish<T>(s, c.device, f);
 }
 
-void forward_run(Ctx& c, const fdb_logprob_args& a) {
+void forward_run(Ctx& c, const fdb_logprob_args& given, ForwardEnd* end) {
+    fdb_logprob_args a = given;
     const cudaStream_t s = static_cast<cudaStream_t>(a.stream);
-    const Forward w = plan_forward(c, a);
+    const Forward w = plan_forward(c, a, end ? end->queries : 0);
+    // (few queries are one pass)
+    const bool filters = end && a.allowed && a.ld_allowed;
+    if (filters && w.few) a.allowed = end->filters(0, a.nq);
     const int n = (int)a.n, d = (int)a.dim;
     const float rf = (float)((double)a.scale * LOG2E);
     const size_t ld_allowed = a.allowed ? a.ld_allowed : 0;
@@ -3046,13 +3037,13 @@ void forward_run(Ctx& c, const fdb_logprob_args& a) {
             amap = map2d(a.dtype,
                          static_cast<const unsigned char*>(qb) + q0 * ldq * 2, inner, nq, ldq, BM);
             StatsArgs p{};
-            p.q0 = (int)q0;
+            p.q0 = filters ? 0 : (int)q0;  // (counts for the filters alone)
             p.nq = (int)nq;
             p.n = n;
             p.qf = w.packed ? w.qf + q0 : nullptr;
             p.xf = w.xf;
             p.rf = rf;
-            p.allowed = a.allowed;
+            p.allowed = filters ? end->filters(q0, nq) : a.allowed;
             p.ld_allowed = ld_allowed;
             p.part = w.part;
             p.top = w.top;
@@ -3072,15 +3063,16 @@ void forward_run(Ctx& c, const fdb_logprob_args& a) {
             f.sizes = (int)blocks_of(c.sm_count, (long long)g.mt * g.chunks);
             f.nt = w.nt, f.chunks = g.chunks;
             f.per_tile = w.bn / GROUP, f.per_part = w.bn / GROUP / 4;
-            if (a.dtype == FDB_DTYPE_F32) launch_finish<float>(s, c.device, f);
+            if (end) end->finish(parts_of(f));
+            else if (a.dtype == FDB_DTYPE_F32) launch_finish<float>(s, c.device, f);
             else if (a.dtype == FDB_DTYPE_F16) launch_finish<__half>(s, c.device, f);
             else launch_finish<__nv_bfloat16>(s, c.device, f);
         }
         return;
     }
-    if (a.dtype == FDB_DTYPE_F32) few_run<float>(c, a, w, rf, ld_allowed);
-    else if (a.dtype == FDB_DTYPE_F16) few_run<__half>(c, a, w, rf, ld_allowed);
-    else few_run<__nv_bfloat16>(c, a, w, rf, ld_allowed);
+    if (a.dtype == FDB_DTYPE_F32) few_run<float>(c, a, w, rf, ld_allowed, end);
+    else if (a.dtype == FDB_DTYPE_F16) few_run<__half>(c, a, w, rf, ld_allowed, end);
+    else few_run<__nv_bfloat16>(c, a, w, rf, ld_allowed, end);
 }
 
 // ---- backward ----
@@ -3098,12 +3090,13 @@ struct Backward {
     int* weight;
     Coef* coef;
     float* rest;
+    int* rest_row;
     uint32_t *seen, *alive;
 };
-static Backward plan_backward(const Ctx& c, const fdb_logprob_grad_args& a) {
+static Backward plan_backward(const Ctx& c, const fdb_logprob_grad_args& a, const GivenRows* given) {
     Backward w{};
     Carve ws(a.workspace);
-    w.few = a.nq <= FEW_GRAD && a.dim <= FEW_GRAD_DIM;
+    w.few = !given && a.nq <= FEW_GRAD && a.dim <= FEW_GRAD_DIM;
     if (w.few) {
         w.err = ws.take<int>(HEAD / 4);
         w.few_blocks = (int)std::min<size_t>((a.n + FEW_ROWS - 1) / FEW_ROWS,
@@ -3138,6 +3131,7 @@ static Backward plan_backward(const Ctx& c, const fdb_logprob_grad_args& a) {
     w.weight = ws.take<int>(a.nq);
     w.coef = ws.take<Coef>(a.nq);
     if (w.parts == 1) w.rest = ws.take<float>(a.nq);
+    if (w.parts == 1 && given) w.rest_row = ws.take<int>(a.nq);
     w.gr = ws.take<__half>((size_t)w.parts * w.nqp * w.ldg);
     w.dq = ws.take<float>((size_t)w.q_splits * a.nq * a.dim);
     if (w.x_splits > 1) w.dx = ws.take<float>((size_t)w.x_splits * w.cols * a.dim);
@@ -3146,16 +3140,16 @@ static Backward plan_backward(const Ctx& c, const fdb_logprob_grad_args& a) {
     w.bytes = ws.at;
     return w;
 }
-size_t backward_bytes(const Ctx& c, const fdb_logprob_grad_args& a) {
+size_t backward_bytes(const Ctx& c, const fdb_logprob_grad_args& a, const GivenRows* given) {
     fdb_logprob_grad_args b = a;
     b.workspace = nullptr;
-    return plan_backward(c, b).bytes;
+    return plan_backward(c, b, given).bytes;
 }
 
 template <typename T, int NQ>
 static void launch_few_grad(const Ctx& c, const Backward& w, const FewGrad<T>& p, cudaStream_t s) {
     const size_t smem = few_grad_smem(NQ, p.d, sizeof(T));
-    if (smem > 40960) {  // (see launch_few)
+    if (smem > 40960) {  // (see allow_smem)
         static std::atomic<uint64_t> done{0};
         allow_smem(few_grad_kernel<T, NQ>, c.device, few_grad_smem(NQ, FEW_GRAD_DIM, sizeof(T)),
                    done);
@@ -3184,9 +3178,9 @@ static void few_backward(const Ctx& c, const fdb_logprob_grad_args& a, const Bac
                     a.d_queries, a.ld_d_queries, a.dtype);
 }
 
-void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
+void backward_run(Ctx& c, const fdb_logprob_grad_args& a, const GivenRows* given) {
     const cudaStream_t s = static_cast<cudaStream_t>(a.stream);
-    const Backward w = plan_backward(c, a);
+    const Backward w = plan_backward(c, a, given);
     if (w.few) {
         CoefArgs k{};
         k.nq = (int)a.nq, k.n = (int)a.n, k.scale = a.scale, k.whole = 1.0;
@@ -3207,6 +3201,7 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
     k.d_logprob = a.d_logprob, k.d_lse = a.d_lse, k.d_entropy = a.d_entropy;
     k.targets = a.targets, k.allowed = a.allowed, k.ld_allowed = ld_allowed;
     k.out = w.coef, k.rest = w.rest;
+    if (given) k.at_least = given->at_least;
     head_kernel<<<(nq + 63) / 64, 64, 0, s>>>(k, w.alive, w.weight,
                                                  reinterpret_cast<uint32_t*>(w.err), HEAD / 4);
     FDB_LAUNCH_CHECK();
@@ -3271,6 +3266,12 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
                 launch_rows<GRAD, false, true>(s, c.device, c.sm_count, qk, xk, g, p, &go);
             else launch_rows<GRAD, false, false>(s, c.device, c.sm_count, qk, xk, g, p, &go);
         }
+        if (given) {
+            const GivenArgs p{*given, nq, w.weight, w.xf, w.gr, w.ldg, (int)w.nqp, w.parts,
+                              (int)j0, cols, j0 == 0 ? w.rest : nullptr, w.rest_row};
+            given_kernel<<<(nq + 7) / 8, 256, 0, s>>>(p);
+            FDB_LAUNCH_CHECK();
+        }
         if (a.d_queries) {
             Mma g = base;
             g.mt = mtq, g.nt = ntd;
@@ -3308,8 +3309,10 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a) {
         }
     }
     if (a.d_queries) {
+        JoinRest rest{w.rest, w.rest_row, 1, w.xp, (int)width};
+        if (!given) rest.row = &w.coef->target, rest.step = sizeof(Coef) / sizeof(int);
         launch_join(s, c.sm_count, w.dq, w.q_splits, nq, d, w.out_f, nullptr, a.d_queries,
-                    a.ld_d_queries, a.dtype, JoinRest{w.rest, w.coef, w.xp, (int)width});
+                    a.ld_d_queries, a.dtype, rest);
     }
     void_kernel<<<c.sm_count, 256, 0, s>>>(w.err, a.d_queries, a.ld_d_queries, nq, a.d_rows,
                                            a.ld_d_rows, n, d, a.dtype);

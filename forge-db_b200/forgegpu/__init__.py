@@ -115,6 +115,43 @@ class LogprobGradArgs(C.Structure):
                 ("stream", C.c_void_p)]
 
 
+_TEACHER = [("teacher_ids", C.c_void_p), ("teacher_logits", C.c_void_p), ("k", C.c_size_t),
+            ("ld_ids", C.c_size_t), ("ld_logits", C.c_size_t), ("teacher_scale", C.c_float),
+            ("rest", C.c_int), ("allowed", C.c_void_p), ("ld_allowed", C.c_size_t)]
+
+
+class DistillArgs(C.Structure):
+    _fields_ = LogprobArgs._fields_[:9] + _TEACHER + [
+        ("loss", C.c_void_p), ("lse", C.c_void_p), ("logprobs", C.c_void_p),
+        ("rest_logprob", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("stream", C.c_void_p)]
+
+
+class DistillGradArgs(C.Structure):
+    _fields_ = LogprobArgs._fields_[:9] + _TEACHER + [
+        ("lse", C.c_void_p), ("logprobs", C.c_void_p), ("rest_logprob", C.c_void_p),
+        ("d_loss", C.c_void_p), ("d_queries", C.c_void_p), ("ld_d_queries", C.c_size_t),
+        ("d_rows", C.c_void_p), ("ld_d_rows", C.c_size_t), ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t), ("stream", C.c_void_p)]
+
+
+class BeamArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("scores", C.c_void_p), ("groups", C.c_size_t),
+                ("beams", C.c_size_t), ("n", C.c_size_t), ("ld_group", C.c_size_t),
+                ("ld_beam", C.c_size_t), ("scale", C.c_float), ("normalise", C.c_int),
+                ("ids", C.c_void_p), ("ld_ids", C.c_size_t), ("allowed", C.c_void_p),
+                ("ld_allowed", C.c_size_t), ("beam_scores", C.c_void_p), ("ended", C.c_void_p),
+                ("end_id", C.c_int64), ("width", C.c_size_t), ("out_scores", C.c_void_p),
+                ("out_parents", C.c_void_p), ("out_ids", C.c_void_p), ("out_ended", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+                ("stream", C.c_void_p)]
+
+
+class ReorderOpts(C.Structure):
+    _fields_ = [("parents", C.c_void_p), ("groups", C.c_size_t), ("beams", C.c_size_t),
+                ("width", C.c_size_t), ("clear", C.c_int), ("stream", C.c_void_p)]
+
+
 class AdamwTensor(C.Structure):
     _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("m", C.c_void_p),
                 ("v", C.c_void_p), ("m_scale", C.c_void_p), ("v_scale", C.c_void_p),
@@ -138,6 +175,14 @@ _SIGS = {
                                                   C.POINTER(_sz)]),
     "fdb_logprobs_backward": (C.c_int, [_vp, C.POINTER(LogprobGradArgs)]),
     "fdb_logprobs_status": (C.c_int, [_vp, _vp, _vp]),
+    "fdb_distill_workspace": (C.c_int, [_vp, C.POINTER(DistillArgs), C.POINTER(_sz)]),
+    "fdb_distill": (C.c_int, [_vp, C.POINTER(DistillArgs)]),
+    "fdb_distill_backward_workspace": (C.c_int, [_vp, C.POINTER(DistillGradArgs),
+                                                 C.POINTER(_sz)]),
+    "fdb_distill_backward": (C.c_int, [_vp, C.POINTER(DistillGradArgs)]),
+    "fdb_beam_select_workspace": (C.c_int, [_vp, C.POINTER(BeamArgs), C.POINTER(_sz)]),
+    "fdb_beam_select": (C.c_int, [_vp, C.POINTER(BeamArgs)]),
+    "fdb_beam_reorder": (C.c_int, [_vp, _vp, _sz, C.POINTER(ReorderOpts)]),
     "fdb_bf_logprobs": (C.c_int, [_vp, _vp, _sz, C.c_float, _vp, _sz, _vp, _vp, _vp, _vp, _vp]),
     "fdb_adamw_step": (C.c_int, [_vp, _vp, _sz, C.POINTER(AdamwOpts)]),
     "fdb_adamw_state_values": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp, _vp]),
@@ -913,9 +958,11 @@ class BruteForceIndex:
 
 
 # ---------------------------------------------------------------------------
-# device operators on torch tensors: softmax over rows, AdamW
+# device operators on torch tensors: softmax over rows, beams, AdamW
 # ---------------------------------------------------------------------------
 LogProbs = collections.namedtuple("LogProbs", "logprob lse entropy top_ids top_logprobs")
+Distilled = collections.namedtuple("Distilled", "loss lse logprobs rest")
+Beams = collections.namedtuple("Beams", "scores parents ids ended")
 _device_ctx: dict = {}
 _DTYPE: dict = {}
 
@@ -1085,6 +1132,253 @@ def logprobs_status(workspace):
     _check(lib().fdb_logprobs_status(
         ctx.h, workspace.data_ptr(),
         torch._C._cuda_getCurrentRawStream(workspace.device.index)))
+
+
+def _lists(t, nq: int, k: int, dtype, device, what: str):
+    """(pointer, row distance) of a teacher's [nq, k] lists."""
+    if t.dtype != dtype or t.device != device or t.shape != (nq, k) or \
+            (k > 1 and t.stride(1) != 1) or (nq > 1 and t.stride(0) < k):
+        _refuse(f"{what} must be {dtype} [{nq}, {k}] with contiguous rows on the queries' device")
+    return t.data_ptr(), t.stride(0) if nq > 1 else k
+
+
+def _distill_args(q, x, ids, logits, scale, teacher_scale, rest, allowed):
+    """The fields that both argument structures start with."""
+    torch = _torch()
+    head = _softmax_args(q, x, None, scale, allowed)
+    if ids.dim() != 2:
+        _refuse("teacher_ids must be [nq, k]")
+    nq, k = head[2], ids.shape[1]
+    ip, ldi = _lists(ids, nq, k, torch.int64, q.device, "teacher_ids")
+    zp, ldz = _lists(logits, nq, k, torch.float32, q.device, "teacher_logits")
+    return head[:9] + (ip, zp, k, ldi, ldz, teacher_scale, rest) + head[10:]
+
+
+def distill(queries, rows, teacher_ids, teacher_logits, *, scale: float = 1.0,
+            teacher_scale: float = 1.0, rest: bool = False, allowed=None,
+            workspace=None) -> Distilled:
+    """The loss of a teacher's best rows under softmax(scale * queries @ rows.T),
+    per query, on the current stream (fdb_distill in forgegpu.h).
+
+    teacher_ids: int64 [nq, k], rows (none where negative), teacher_logits:
+    float32 [nq, k].  With rest they are log probabilities, and what they leave
+    is compared with the student's probability of all other rows; else the
+    teacher is softmax(teacher_scale * teacher_logits) over its k rows.
+    allowed, workspace: as for logprobs (logprobs_status reads a timeout).
+    logprobs is the student's log probability of each entry, rest the log of
+    what it leaves to other rows (None without).  The results have no autograd
+    history: the gradient is distill_backward's."""
+    torch = _torch()
+    head = _distill_args(queries, rows, teacher_ids, teacher_logits, scale, teacher_scale,
+                         1 if rest else 0, allowed)
+    dev, nq, k = queries.device, head[2], head[11]
+    ctx = _ctx_of(dev)
+    L = lib()
+    empty, f32 = torch.empty, torch.float32
+    loss, lse = empty(nq, dtype=f32, device=dev), empty(nq, dtype=f32, device=dev)
+    lp = empty((nq, k), dtype=f32, device=dev)
+    other = empty(nq, dtype=f32, device=dev) if rest else None
+    a = DistillArgs(*head, loss.data_ptr(), lse.data_ptr(), lp.data_ptr(),
+                    other.data_ptr() if rest else None)
+    key = (dev.index, "distill", k, a.rest, head[1] & 15, head[4] & 15) + head[0:1] + head[2:4] + \
+        head[5:8]
+    ws, a.workspace_bytes = _workspace(torch, ctx, L.fdb_distill_workspace, a, key, dev, workspace)
+    a.workspace = ws.data_ptr()
+    a.stream = torch._C._cuda_getCurrentRawStream(dev.index)
+    rc = L.fdb_distill(ctx.h, C.byref(a))
+    if rc:
+        _check(rc)
+    return Distilled(loss, lse, lp, other)
+
+
+def distill_backward(queries, rows, teacher_ids, teacher_logits, lse, logprobs, rest=None, *,
+                     d_loss, scale: float = 1.0, teacher_scale: float = 1.0, allowed=None,
+                     need_queries: bool = True, need_rows: bool = True, workspace=None):
+    """(d_queries, d_rows) of sum(d_loss * loss), given what distill returned for
+    the same arguments: lse, logprobs and, if it was called with rest, its rest
+    (fdb_distill_backward in forgegpu.h).  A gradient that is not needed is None."""
+    torch = _torch()
+    head = _distill_args(queries, rows, teacher_ids, teacher_logits, scale, teacher_scale,
+                         0 if rest is None else 1, allowed)
+    dev, f32 = queries.device, torch.float32
+    nq, n, dim, k = head[2], head[5], head[7], head[11]
+    if logprobs.dtype != f32 or logprobs.device != dev or logprobs.shape != (nq, k) or \
+            not logprobs.is_contiguous():
+        _refuse(f"logprobs must be a contiguous {f32} tensor [{nq}, {k}] on the queries' device")
+    ctx = _ctx_of(dev)
+    L = lib()
+    dq = torch.empty((nq, dim), dtype=queries.dtype, device=dev) if need_queries else None
+    dx = torch.empty((n, dim), dtype=queries.dtype, device=dev) if need_rows else None
+    a = DistillGradArgs(*head, _vector(lse, nq, f32, dev, "lse"), logprobs.data_ptr(),
+                        _vector(rest, nq, f32, dev, "rest"),
+                        _vector(d_loss, nq, f32, dev, "d_loss"),
+                        None if dq is None else dq.data_ptr(), dim,
+                        None if dx is None else dx.data_ptr(), dim)
+    key = (dev.index, "distill_backward", k, allowed is not None and head[17]) + head[0:1] + \
+        head[2:4] + head[5:8]
+    ws, a.workspace_bytes = _workspace(torch, ctx, L.fdb_distill_backward_workspace, a, key, dev,
+                                       workspace)
+    a.workspace = ws.data_ptr()
+    a.stream = torch._C._cuda_getCurrentRawStream(dev.index)
+    rc = L.fdb_distill_backward(ctx.h, C.byref(a))
+    if rc:
+        _check(rc)
+    return dq, dx
+
+
+def beam_select(scores, beam_scores, *, width: int | None = None, ids=None, scale: float = 1.0,
+                normalise: bool = True, allowed=None, ended=None, end_id: int = -1,
+                workspace=None) -> Beams:
+    """The `width` best continuations of each search's chains, on the current
+    stream (fdb_beam_select in forgegpu.h): scores [groups, beams, n] are the
+    columns' logits (with normalise) or log probabilities, beam_scores float32
+    [groups, beams] the chains' so far.
+
+    ids: int64 [groups, beams, n], what the columns stand for (none where
+    negative).  allowed: int32 words of a bit per column, one filter or
+    [groups * beams, words].  ended: bool [groups, beams], chains that stay as
+    they are; end_id: the id that ends one.  Results [groups, width]: scores,
+    the chains (int64) and ids (int64) they continue with, ended (bool)."""
+    torch = _torch()
+    dev = scores.device
+    if scores.dim() != 3 or dev.type != "cuda" or scores.dtype not in _DTYPE:
+        _refuse("scores must be a [groups, beams, n] float32, float16 or bfloat16 tensor on a GPU")
+    g, b, n = scores.shape
+    s0, s1, s2 = scores.stride()
+    if (n > 1 and s2 != 1) or (b > 1 and s1 < n):
+        _refuse("scores must have contiguous rows")
+    f32 = torch.float32
+    if beam_scores.dtype != f32 or beam_scores.device != dev or beam_scores.shape != (g, b) or \
+            not beam_scores.is_contiguous():
+        _refuse("beam_scores must be a contiguous float32 [groups, beams] tensor on the scores' "
+                "device")
+    ip = ep = ap = None
+    if ids is not None:
+        if ids.dtype != torch.int64 or ids.device != dev or ids.shape != (g, b, n) or \
+                not ids.is_contiguous():
+            _refuse("ids must be a contiguous int64 tensor of the scores' shape and device")
+        ip = ids.data_ptr()
+    lda = 0
+    if allowed is not None:
+        words = (n + 31) // 32
+        if allowed.dtype != torch.int32 or allowed.device != dev or allowed.dim() not in (1, 2) \
+                or allowed.shape[-1] != words or (words > 1 and allowed.stride(-1) != 1):
+            _refuse(f"allowed must be int32 words [{words}] or [1 or groups * beams, {words}] on "
+                    "the scores' device")
+        filters = 1 if allowed.dim() == 1 else allowed.shape[0]
+        if filters not in (1, g * b):
+            _refuse(f"allowed has {filters} filters for {g * b} chains")
+        ap = allowed.data_ptr()
+        if filters > 1:
+            lda = allowed.stride(0)
+            if lda < words:
+                _refuse("allowed must have contiguous rows")
+    if ended is not None:
+        if ended.dtype not in (torch.bool, torch.uint8) or ended.device != dev or \
+                ended.shape != (g, b) or not ended.is_contiguous():
+            _refuse("ended must be a contiguous bool [groups, beams] tensor on the scores' device")
+        ep = ended.data_ptr()
+    w = b if width is None else width
+    if not 1 <= w <= 128:
+        _refuse("width must be in [1, 128]")
+    ctx = _ctx_of(dev)
+    L = lib()
+    empty = torch.empty
+    top = empty((g, w), dtype=f32, device=dev)
+    parents, out = empty((g, w), dtype=torch.int64, device=dev), empty((g, w), dtype=torch.int64,
+                                                                       device=dev)
+    done = empty((g, w), dtype=torch.bool, device=dev)
+    a = BeamArgs(_DTYPE[scores.dtype], scores.data_ptr(), g, b, n, s0, s1 if b > 1 else n, scale,
+                 1 if normalise else 0, ip, n, ap, lda, beam_scores.data_ptr(), ep, end_id, w,
+                 top.data_ptr(), parents.data_ptr(), out.data_ptr(), done.data_ptr())
+    key = (dev.index, "beam", a.dtype, g, b, n, w, a.normalise, ip is None,
+           scores.data_ptr() & 15, s0, s1)
+    ws, a.workspace_bytes = _workspace(torch, ctx, L.fdb_beam_select_workspace, a, key, dev,
+                                       workspace)
+    a.workspace = ws.data_ptr()
+    a.stream = torch._C._cuda_getCurrentRawStream(dev.index)
+    rc = L.fdb_beam_select(ctx.h, C.byref(a))
+    if rc:
+        _check(rc)
+    return Beams(top, parents, out, done)
+
+
+def _runs(t, what: str):
+    """(row distance, runs of a row, run distance, elements of a run) of a state
+    [groups, beams, ...] whose rows are evenly spaced and whose inner dimensions
+    are contiguous but for one step."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) < 2:
+        _refuse(f"{what} must be [groups, beams, ...]")
+    rows = stride[1] if shape[1] > 1 else stride[0]
+    if shape[0] > 1 and shape[1] > 1 and stride[0] != shape[1] * stride[1]:
+        _refuse(f"{what} must have evenly spaced rows")
+    run, d = 1, len(shape) - 1
+    while d > 1 and (shape[d] == 1 or stride[d] == run):
+        run *= shape[d]
+        d -= 1
+    parts, step = 1, 0
+    while d > 1 and (shape[d] == 1 or parts == 1 or stride[d] == parts * step):
+        if shape[d] > 1:
+            if parts == 1:
+                step = stride[d]
+            parts *= shape[d]
+        d -= 1
+    if d > 1 or (parts > 1 and step < run):
+        _refuse(f"{what} must be contiguous past its second dimension, but for one step")
+    return rows, parts, step, run
+
+
+def beam_reorder(states, parents, out=None):
+    """States that follow their chains, on the current stream (fdb_beam_reorder
+    in forgegpu.h): row [g, w] of each result is row [g, parents[g, w]] of the
+    state [groups, beams, ...].  out: tensors to write to (new ones if None); a
+    state itself, where width is beams, is reordered in place.  States and out
+    may be parts of wider tensors (the positions in use of a cache); what a
+    parent outside [0, beams) would bring is left as it was (zeros in a new
+    one).  Returns the results.  To autograd it is an in-place change of out."""
+    torch = _torch()
+    if parents.dtype != torch.int64 or parents.dim() != 2 or not parents.is_contiguous() or \
+            not parents.is_cuda:
+        _refuse("parents must be a contiguous int64 [groups, width] tensor on a GPU")
+    g, w = parents.shape
+    dev = parents.device
+    if out is not None and len(out) != len(states):
+        _refuse("out must be a list of the states' length")
+    if not states:
+        return []
+    b = states[0].shape[1] if states[0].dim() > 1 else 0
+    new = out is None
+    if new:
+        out = [torch.empty((g, w) + t.shape[2:], dtype=t.dtype, device=dev) for t in states]
+    table = array.array("Q")
+    for t, o in zip(states, out):
+        if t.device != dev or o.device != dev or t.dtype != o.dtype or t.shape[:2] != (g, b) or \
+                o.shape != (g, w) + t.shape[2:]:
+            _refuse("states must be [groups, beams, ...] and out [groups, width, ...] of their "
+                    "types, on the parents' device")
+        es = t.element_size()
+        rows, parts, step, run = _runs(t, "a state")
+        orows, oparts, ostep, orun = _runs(o, "out")
+        if (parts, run) != (oparts, orun):  # (one of them is contiguous: in the other's runs)
+            if oparts == 1 and orun == parts * run:
+                oparts, ostep, orun = parts, run, run
+            elif parts == 1 and run == oparts * orun:
+                parts, step, run = oparts, orun, orun
+            else:
+                _refuse("a state and its out must fall into the same runs")
+        if t.numel() == 0:
+            parts = 0
+        table.extend((t.data_ptr(), o.data_ptr(), rows * es, orows * es, parts, step * es,
+                      ostep * es, run * es))
+    opts = ReorderOpts(parents.data_ptr(), g, b, w, 1 if new else 0,
+                       torch._C._cuda_getCurrentRawStream(dev.index))
+    _check(lib().fdb_beam_reorder(_ctx_of(dev).h, table.buffer_info()[0], len(out),
+                                  C.byref(opts)))
+    if not new:
+        # (written through pointers: a graph that saved one of them has to notice)
+        torch.autograd.graph.increment_version(out)
+    return list(out)
 
 
 def _scalar(t, dtype, like, what: str):

@@ -547,7 +547,162 @@ int fdb_logprobs_backward(fdb_ctx* ctx, const fdb_logprob_grad_args* args);
  * stream, then FDB_OK or FDB_ERR_TIMEOUT.  Such a call's outputs are NaN. */
 int fdb_logprobs_status(fdb_ctx* ctx, const void* workspace, void* stream);
 
-/* The same over the rows of a brute-force index with the dot-product metric
+/* ---- distillation from a teacher's best rows ------------------------------ */
+/* No reference counterpart.  The loss of a teacher's k best rows per query
+ * under the p_ij of fdb_logprobs, whose rules for streams, workspaces, captured
+ * graphs and buffers hold here too (fdb_logprobs_status reads the workspace).
+ *
+ * teacher_ids and teacher_logits [nq][k], rows ld_ids and ld_logits >= k apart.  An entry
+ * takes part if its id is in [0, n), the query may see that row, its logit z is
+ * not -inf and no entry before it that takes part has its id (lists may be
+ * short, unsorted, or empty: the loss is then 0).
+ *   rest = 0:  P = softmax of teacher_scale * z over the entries,
+ *              loss = sum_e P_e (log P_e - log p_e)
+ *   rest = 1:  z are the teacher's log probabilities over all rows: P = exp(z),
+ *              R = 1 - sum P (z that sum to more than 1: P over their sum, R = 0),
+ *              loss = sum_e P_e (log P_e - log p_e) + R (log R - log r),
+ *              r the student's probability of all other rows together, R of none
+ *              if the query sees no other row.  teacher_scale must be 1.
+ * Both are at least 0, and 0 where the student is what the teacher says.
+ *
+ * Outputs, each nullable: loss[nq], lse[nq] (as fdb_logprobs'), logprobs[nq][k]
+ * (log p of each entry, 0 where it takes no part), rest_logprob[nq] (log r, -inf
+ * if the query sees no other row; rest = 1 only).  The named rows' scores are
+ * taken in 64 bits and r is summed over the other rows, so that it holds as a
+ * student becomes sure.  A z that is NaN or +inf makes its query's loss NaN; an
+ * infinity or NaN in a query, or in a row that it may see, all of its outputs. */
+#define FDB_MAX_TEACHER 256 /* largest k */
+typedef struct fdb_distill_args {
+    int dtype; /* FDB_DTYPE_* of queries and rows */
+    const void* queries;
+    size_t nq, ld_queries;
+    const void* rows;
+    size_t n, ld_rows;
+    size_t dim;
+    float scale;
+    const int64_t* teacher_ids;
+    const float* teacher_logits;
+    size_t k, ld_ids, ld_logits;
+    float teacher_scale;
+    int rest;
+    const uint32_t* allowed;
+    size_t ld_allowed;
+    float *loss, *lse, *logprobs, *rest_logprob;
+    void* workspace;
+    size_t workspace_bytes;
+    void* stream;
+} fdb_distill_args;
+int fdb_distill_workspace(fdb_ctx* ctx, const fdb_distill_args* args, size_t* bytes);
+int fdb_distill(fdb_ctx* ctx, const fdb_distill_args* args);
+
+/* Gradient of sum_i d_loss[i] loss[i], given the lse, logprobs and, with
+ * rest = 1, rest_logprob that fdb_distill returned for the same arguments:
+ *     G_ij = scale d_loss_i (p_ij - P_ij)       at the teacher's rows,
+ *            scale d_loss_i p_ij (1 - R / r)    elsewhere
+ *     d_queries = G X,  d_rows = G^T Q
+ * as fdb_logprobs_backward writes them. */
+typedef struct fdb_distill_grad_args {
+    int dtype;
+    const void* queries;
+    size_t nq, ld_queries;
+    const void* rows;
+    size_t n, ld_rows;
+    size_t dim;
+    float scale;
+    const int64_t* teacher_ids;
+    const float* teacher_logits;
+    size_t k, ld_ids, ld_logits;
+    float teacher_scale;
+    int rest;
+    const uint32_t* allowed;
+    size_t ld_allowed;
+    const float *lse, *logprobs, *rest_logprob;
+    const float* d_loss;
+    void* d_queries;
+    size_t ld_d_queries;
+    void* d_rows;
+    size_t ld_d_rows;
+    void* workspace;
+    size_t workspace_bytes;
+    void* stream;
+} fdb_distill_grad_args;
+int fdb_distill_backward_workspace(fdb_ctx* ctx, const fdb_distill_grad_args* args, size_t* bytes);
+int fdb_distill_backward(fdb_ctx* ctx, const fdb_distill_grad_args* args);
+
+/* ---- beam search over rows ------------------------------------------------ */
+/* No reference counterpart.  One step of a beam search: of `groups` searches with
+ * `beams` chains each, the `width` best continuations.  Rules for streams,
+ * workspaces, graphs and buffers as above.
+ *
+ * scores [groups][beams][n] of one type, ld_group and ld_beam elements apart.
+ * With `normalise` they are logits, and a column adds
+ *     l_bj = scale x_bj - log sum_j exp(scale x_bj)
+ * to its chain's score, else l_bj = scale x_bj (log probabilities already, as
+ * fdb_logprobs' top_logprobs).  ids (nullable) [groups][beams][n], ld_ids apart
+ * per chain: what the columns stand for (a column's number if NULL), < 0: no
+ * candidate, as fdb_logprobs' top_ids.  allowed: as fdb_logprobs', a filter for
+ * all chains or one each (chain g * beams + b).  Columns without a candidate,
+ * those not allowed and those whose score is -inf take no part, in the
+ * normaliser either.
+ * beam_scores [groups][beams]: the chains' scores so far, -inf for one that is
+ * not there.  ended (nullable): a chain whose byte is not 0 has one candidate,
+ * itself, with its score and the id end_id; its columns are not read, nor are
+ * those of a chain that is not there.
+ *
+ * Outputs [groups][width]: the best beam_score + l in order, compared in 64 bits,
+ * equal ones by chain, then column (an ended chain stands in column 0); the
+ * chain each continues, the id it adds, and whether it has ended (nullable): its
+ * chain had, or the id is end_id.  Past the last candidate -inf, -1, -1, 0.  A
+ * group with a NaN or +inf in a chain's score or in a score that may count has
+ * NaN, -1, -1, 0. */
+#define FDB_MAX_BEAMS 128 /* largest beams and width */
+typedef struct fdb_beam_args {
+    int dtype; /* FDB_DTYPE_* of scores */
+    const void* scores;
+    size_t groups, beams, n, ld_group, ld_beam;
+    float scale;
+    int normalise;
+    const int64_t* ids;
+    size_t ld_ids;
+    const uint32_t* allowed;
+    size_t ld_allowed;
+    const float* beam_scores;
+    const uint8_t* ended;
+    int64_t end_id;
+    size_t width;
+    float* out_scores;
+    int64_t *out_parents, *out_ids;
+    uint8_t* out_ended;
+    void* workspace;
+    size_t workspace_bytes;
+    void* stream;
+} fdb_beam_args;
+int fdb_beam_select_workspace(fdb_ctx* ctx, const fdb_beam_args* args, size_t* bytes);
+int fdb_beam_select(fdb_ctx* ctx, const fdb_beam_args* args);
+
+/* Moves states after their chains: row g * width + w of dst is row
+ * g * beams + parents[g][w] of src, for each of `count` states.  A row is `parts`
+ * runs of `bytes` bytes, part_stride bytes apart (a cache's heads, of which the
+ * positions in use move); rows are src_stride and dst_stride bytes apart.  What
+ * lies between the runs is left as it was, as is a row whose parent is outside
+ * [0, beams), unless `clear` is not 0: it is then zeroed (not in place).  dst may be src (same strides, width = beams): in place.  No
+ * other overlap.  Needs no workspace. */
+typedef struct fdb_beam_state {
+    const void* src;
+    void* dst;
+    size_t src_stride, dst_stride;
+    size_t parts, src_part_stride, dst_part_stride, bytes;
+} fdb_beam_state;
+typedef struct fdb_reorder_opts {
+    const int64_t* parents;
+    size_t groups, beams, width;
+    int clear;
+    void* stream;
+} fdb_reorder_opts;
+int fdb_beam_reorder(fdb_ctx* ctx, const fdb_beam_state* states, size_t count,
+                     const fdb_reorder_opts* opts);
+
+/* fdb_logprobs over the rows of a brute-force index with the dot-product metric
  * (host buffers, like fdb_bf_batch_search): p(row | query) with
  * scale = 1 / temperature.  target_ids[nq] (nullable): vector ids; an id that
  * the index does not hold gives a logprob of 0, a repeated id its first row.
