@@ -34,7 +34,6 @@ struct Select {
     float* out_scores;
     int64_t *out_parents, *out_ids;
     uint8_t* out_ended;
-    double* lse;  // [chains]
 };
 
 // scale x of a column, -inf if it takes no part
@@ -54,113 +53,691 @@ __device__ __forceinline__ bool absent(const Select& p, int g, int b) {
     return p.beam_scores[(size_t)g * p.beams + b] == -INFINITY;
 }
 
-// One block per chain: its normaliser (0 without), NaN if a column that takes part
-// is NaN or +inf.
-template <typename T>
-__global__ void __launch_bounds__(256) lse_kernel(const Select p) {
-    __shared__ double part[8];
-    const int g = blockIdx.x / p.beams, b = blockIdx.x % p.beams;
-    if (over(p, g, b) || absent(p, g, b)) return;
-    double m = -INFINITY;
-    bool bad = false;
-    for (int j = threadIdx.x; j < p.n; j += 256) {
-        const double v = column<T>(p, g, b, j);
-        bad |= !(v < INFINITY);
-        m = fmax(m, v);
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
-    bad = __syncthreads_or(bad);
-    for (int i = 0; i < 8; ++i) m = fmax(m, part[i]);
-    __syncthreads();
-    double s = 0.0;
-    if (p.normalise && !bad && m > -INFINITY)
-        for (int j = threadIdx.x; j < p.n; j += 256) s += exp(column<T>(p, g, b, j) - m);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
-    __syncthreads();
-    if (threadIdx.x != 0) return;
-    s = 0.0;
-    for (int i = 0; i < 8; ++i) s += part[i];
-    p.lse[blockIdx.x] = bad ? NAN : m == -INFINITY || !p.normalise ? 0.0 : m + log(s);
+// ---------------------------------------------------------------------------
+// order-preserving images of numbers
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t ordered(float f) {
+    const uint32_t u = __float_as_uint(f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(uint32_t u) {
+    return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+__device__ __forceinline__ uint64_t ordered64(double v) {
+    const uint64_t u = (uint64_t)__double_as_longlong(v);
+    return u >> 63 ? ~u : u | 0x8000000000000000ull;
+}
+__device__ __forceinline__ double unordered64(uint64_t u) {
+    return __longlong_as_double((long long)(u >> 63 ? u & 0x7fffffffffffffffull : ~u));
 }
 
-// One block per search: the best candidate after the one before, `width` times.
+
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// ---------------------------------------------------------------------------
+// scanning the chains' columns
+// ---------------------------------------------------------------------------
+// A block takes a part of a chain's columns, TILE at a time, 16 bytes a load, and
+// leaves their sum of exponentials and the `width` best.  Sums are taken relative to a
+// thread's own largest score so far (raised only when it is exceeded by 2^8), 32
+// terms in f32 and those in 64 bits.  A column is looked at again only if it is above
+// the width-th best so far: of the first tile, if it reaches the least of the
+// largest of G >= width groups of threads, which at least G columns do.
+constexpr int TH = 256;               // threads
+constexpr int U = 4;                  // loads of a thread in a tile
+constexpr int MAXW = FDB_MAX_BEAMS;
+constexpr float RAISE = 8.0f;
+
 template <typename T>
-__global__ void __launch_bounds__(1024) pick_kernel(const Select p) {
-    __shared__ double best_s[32];
-    __shared__ unsigned long long best_at[32];
-    const int g = blockIdx.x, tid = threadIdx.x;
-    bool bad = false;
-    for (int b = tid; b < p.beams; b += 1024) {
-        const float s = p.beam_scores[(size_t)g * p.beams + b];
-        bad |= !(s < INFINITY);
-        if (!over(p, g, b) && !absent(p, g, b)) bad |= !(p.lse[(size_t)g * p.beams + b] < INFINITY);
+struct Vec;  // 16 bytes of columns
+template <>
+struct Vec<float> {
+    static constexpr int N = 4;
+    static constexpr uint32_t NONE = 0xff800000u;  // -inf, in every element of a word
+    static __device__ __forceinline__ float max4(const uint4& r, float m) {
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(__uint_as_float(r.x)));
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(__uint_as_float(r.y)));
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(__uint_as_float(r.z)));
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(__uint_as_float(r.w)));
+        return m;
     }
-    bad = __syncthreads_or(bad);
-    double last = INFINITY;
-    unsigned long long last_at = 0;
-    for (int w = 0; w < p.width; ++w) {
-        double s = -INFINITY;
-        unsigned long long at = ~0ull;
-        for (int b = 0; b < p.beams && !bad; ++b) {
-            const double sum = p.beam_scores[(size_t)g * p.beams + b];
-            if (absent(p, g, b)) continue;
-            const bool done = over(p, g, b);
-            const double lse = done ? 0.0 : p.lse[(size_t)g * p.beams + b];
-            for (int j = tid; j < (done ? 1 : p.n); j += 1024) {
-                const double v = done ? sum : sum + (column<T>(p, g, b, j) - lse);
-                const unsigned long long a = (unsigned long long)b << 32 | (unsigned)j;
-                if (v > last || (v == last && a <= last_at && w)) continue;
-                if (v > s || (v == s && a < at)) s = v, at = a;
+    static __device__ __forceinline__ float2 pair(const uint4& r, int i) {
+        return i ? make_float2(__uint_as_float(r.z), __uint_as_float(r.w))
+                 : make_float2(__uint_as_float(r.x), __uint_as_float(r.y));
+    }
+};
+template <>
+struct Vec<__half> {
+    static constexpr int N = 8;
+    static constexpr uint32_t NONE = 0xfc00fc00u;
+    static __device__ __forceinline__ float max4(const uint4& r, float m) {
+        const __half2* h = reinterpret_cast<const __half2*>(&r);
+        const __half2 v = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+        const float2 f = __half22float2(v);
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(f.x));
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(f.y));
+        return m;
+    }
+    static __device__ __forceinline__ float2 pair(const uint4& r, int i) {
+        return __half22float2(reinterpret_cast<const __half2*>(&r)[i]);
+    }
+};
+template <>
+struct Vec<__nv_bfloat16> {
+    static constexpr int N = 8;
+    static constexpr uint32_t NONE = 0xff80ff80u;
+    static __device__ __forceinline__ float max4(const uint4& r, float m) {
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
+        const __nv_bfloat162 v = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+        const float2 f = __bfloat1622float2(v);
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(f.x));
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(f.y));
+        return m;
+    }
+    static __device__ __forceinline__ float2 pair(const uint4& r, int i) {
+        const uint32_t w = reinterpret_cast<const uint32_t*>(&r)[i];
+        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    }
+};
+
+// What a block leaves: sum of 2^((x - m) s), its `count` best columns in order.
+struct Part {
+    double sum;
+    float m;
+    int count;  // -1: a column is NaN or +inf
+};
+struct Scan {
+    Part* part;       // [chains][splits]
+    uint64_t* best;   // [chains][splits][width]: ordered(x) << 32 | ~column
+    int splits;
+    float s;          // scale log2(e)
+    float slack;      // see finish_kernel
+};
+
+// Vector v of a chain whose first column is `skip` columns into vector 0; columns
+// outside of it, or that take no part, as -inf.
+template <typename T, bool GATE>
+__device__ __forceinline__ uint4 load_vec(const Select& p, const T* x, int skip, size_t row, int v,
+                                          int v1) {
+    constexpr int N = Vec<T>::N;
+    uint4 r = make_uint4(Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE);
+    if (v >= v1) return r;
+    const int j0 = v * N - skip;
+    if (j0 >= 0 && j0 <= p.n - N) {
+        r = __ldcs(reinterpret_cast<const uint4*>(x + j0));
+    } else {
+        T* e = reinterpret_cast<T*>(&r);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (j0 + i >= 0 && j0 + i < p.n) e[i] = x[j0 + i];
+    }
+    if (GATE) {
+        uint32_t keep = (1u << N) - 1;
+        if (p.allowed) {
+            const uint32_t* al = p.allowed + row * p.ld_allowed;
+            const int lo = max(j0, 0), w = lo >> 5;
+            uint64_t bits = __ldg(al + w);
+            if (w + 1 < (p.n + 31) >> 5) bits |= (uint64_t)__ldg(al + w + 1) << 32;
+            keep &= (uint32_t)(bits >> (lo & 31)) << (lo - j0);
+        }
+        if (p.ids) {
+            const int64_t* id = p.ids + row * p.ld_ids;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (j0 + i >= 0 && j0 + i < p.n && __ldg(id + j0 + i) < 0) keep &= ~(1u << i);
+        }
+        const uint4 none = make_uint4(Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE);
+        T* e = reinterpret_cast<T*>(&r);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (!(keep >> i & 1u)) e[i] = reinterpret_cast<const T*>(&none)[i];
+    }
+    return r;
+}
+
+
+// ---- the best of what lies in shared memory ----
+constexpr int LIMIT = 256;              // keys that are put in order at once
+constexpr int ASIDE = 512;
+struct Best {
+    uint64_t* buf;                      // [LIMIT + TH * columns of a vector]
+    uint64_t aside[ASIDE], out[MAXW], least;
+    int count, total;
+};
+// Leaves the `width` best of s.count keys, which all differ, in order at buf's front
+// and returns how many they are.  Ranks are counted; of more than TH keys only
+// those that reach the width-th largest of TH maxima are ranked.  Called by all
+// threads, after a barrier.
+__device__ __forceinline__ int keep_best(Best& s, int width) {
+    const int tid = threadIdx.x;
+    const uint64_t* from = s.buf;
+    int n = s.count;
+    if (n > TH) {
+        uint64_t m = 0;
+        for (int i = tid; i < n; i += TH) m = max(m, s.buf[i]);
+        s.aside[tid] = m;
+        if (tid == 0) s.total = 0;
+        __syncthreads();
+        int rank = 0;
+#pragma unroll 8
+        for (int i = 0; i < TH; ++i) rank += s.aside[i] > m;
+        if (rank == width - 1) s.least = m;
+        __syncthreads();
+        const uint64_t least = s.least;
+        for (int i = tid; i < n; i += TH) {
+            const uint64_t v = s.buf[i];
+            if (v < least) continue;
+            const int at = atomicAdd(&s.total, 1);
+            if (at < ASIDE) s.aside[at] = v;
+        }
+        __syncthreads();
+        if (s.total <= ASIDE) n = s.total, from = s.aside;
+    }
+    for (int i = tid; i < n; i += TH) {
+        const uint64_t v = from[i];
+        int rank = 0;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) rank += from[j] > v;
+        if (rank < width) s.out[rank] = v;
+    }
+    __syncthreads();
+    n = min(n, width);
+    for (int i = tid; i < n; i += TH) s.buf[i] = s.out[i];
+    if (tid == 0) s.count = n;
+    __syncthreads();
+    return n;
+}
+
+template <typename T, bool NORM, bool GATE>
+__global__ void __launch_bounds__(TH, 4) scan_kernel(const Select p, const Scan c) {
+    constexpr int N = Vec<T>::N;
+    __shared__ uint64_t buf[LIMIT + TH * N];
+    __shared__ Best s;
+    __shared__ float warp_min[TH / 32];
+    __shared__ double warp_sum[TH / 32];
+    __shared__ float warp_m[TH / 32];
+    const int tid = threadIdx.x;
+    const size_t row = blockIdx.x / c.splits;
+    const int sp = blockIdx.x % c.splits, g = (int)(row / p.beams), b = (int)(row % p.beams);
+    if (over(p, g, b) || absent(p, g, b)) return;
+    const T* x = static_cast<const T*>(p.x) + (size_t)g * p.ld_group + (size_t)b * p.ld_beam;
+    const int skip = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+    const long long nv = ((long long)p.n + skip + N - 1) / N;
+    const int v0 = (int)(nv * sp / c.splits), v1 = (int)(nv * (sp + 1) / c.splits);
+    if (tid == 0) s.count = 0, s.buf = buf;
+
+    float tau = -INFINITY, m = 0.0f;
+    double sum = 0.0;
+    bool started = false, bad = false;
+    uint4 next[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        next[u] = load_vec<T, GATE>(p, x, skip, row, v0 + u * TH + tid, v1);
+    for (int at = v0; at < v1; at += TH * U) {
+        uint4 r[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) r[u] = next[u];
+        if (at + TH * U < v1) {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                next[u] = load_vec<T, GATE>(p, x, skip, row, at + (U + u) * TH + tid, v1);
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < U; ++u) top = Vec<T>::max4(r[u], top);
+        bad |= !(top < INFINITY);
+        if (NORM) {
+            if (top > -INFINITY && (!started || (top - m) * c.s > RAISE)) {
+                if (started) sum *= (double)sr::ex2((m - top) * c.s);
+                m = top;
+                started = true;
+            }
+            const uint64_t m2 = pack2(-m, -m), s2 = pack2(c.s, c.s);
+            uint64_t acc[2] = {0, 0};
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int i = 0; i < N / 2; ++i) {
+                    const float2 f = Vec<T>::pair(r[u], i);
+                    const uint64_t t = mul2(add2(pack2(f.x, f.y), m2), s2);
+                    float t0, t1;
+                    unpack2(t, t0, t1);
+                    acc[i & 1] = add2(acc[i & 1], pack2(sr::ex2(t0), sr::ex2(t1)));
+                }
+            float a0, a1;
+            unpack2(add2(acc[0], acc[1]), a0, a1);
+            sum += (double)(a0 + a1);
+        }
+        const bool first = at == v0;
+        if (first) {
+            // the least of the largest of G >= width groups of threads
+            int groups = 8;
+            while (groups < p.width) groups <<= 1;
+            float t = top;
+            for (int o = 1; o < TH / groups; o <<= 1)
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+#pragma unroll
+            for (int o = 16; o; o >>= 1) t = fminf(t, __shfl_xor_sync(0xffffffffu, t, o));
+            if ((tid & 31) == 0) warp_min[tid >> 5] = t;
+            __syncthreads();
+            tau = warp_min[0];
+#pragma unroll
+            for (int i = 1; i < TH / 32; ++i) tau = fminf(tau, warp_min[i]);
+        }
+        // a column enters if it is above tau (in the first tile, if it reaches it): of
+        // equal ones the lower, which came before, is kept
+        const bool hit = top > -INFINITY && (first ? top >= tau : top > tau);
+        const int hits = __syncthreads_count(hit);
+        if (hits == 0) continue;
+        auto enter = [&](const uint4& v, int u, bool reach) -> bool {
+            bool full = false;
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) {
+                const float2 f = Vec<T>::pair(v, i);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float y = h ? f.y : f.x;
+                    if (!(y > -INFINITY) || !(reach ? y >= tau : y > tau)) continue;
+                    const int col = (at + u * TH + tid) * N - skip + 2 * i + h;
+                    const int to = atomicAdd(&s.count, 1);
+                    buf[to] = (uint64_t)ordered(y) << 32 | (uint32_t)~col;
+                    full |= to >= LIMIT - 1;
+                }
+            }
+            return full;
+        };
+        auto settle = [&](bool full) -> bool {  // whether the width best are known now
+            if (!__syncthreads_or(full) || keep_best(s, p.width) < p.width) return false;
+            tau = unordered((uint32_t)(buf[p.width - 1] >> 32));
+            return true;
+        };
+        if (hits * U <= TH) {  // (there is room for all that they may hold)
+            bool full = false;
+            if (hit) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) full |= enter(r[u], u, first);
+            }
+            settle(full || first);
+        } else {
+            bool reach = first;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                bool full = false;
+                if (hit) full = enter(r[u], u, reach);
+                // (once they are, an equal one further on is not better)
+                if (settle(full || (first && u == U - 1))) reach = false;
             }
         }
+    }
+    __syncthreads();
+    const int have = keep_best(s, p.width);
+    uint64_t* out = c.best + (size_t)blockIdx.x * p.width;
+    for (int i = tid; i < have; i += TH) out[i] = buf[i];
+    // ---- the sums ----
+    bad = __syncthreads_or(bad);
+    if (NORM) {
+        float M = started ? m : -INFINITY;
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            const double os = __shfl_xor_sync(0xffffffffu, s, o);
-            const unsigned long long oa = __shfl_xor_sync(0xffffffffu, at, o);
-            if (os > s || (os == s && oa < at)) s = os, at = oa;
+        for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        if ((tid & 31) == 0) warp_m[tid >> 5] = M;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < TH / 32; ++i) M = fmaxf(M, warp_m[i]);
+        double v = started && M < INFINITY ? sum * (double)sr::ex2((m - M) * c.s) : 0.0;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if ((tid & 31) == 0) warp_sum[tid >> 5] = v;
+        __syncthreads();
+        if (tid == 0) {
+            v = 0.0;
+            for (int i = 0; i < TH / 32; ++i) v += warp_sum[i];
+            c.part[blockIdx.x] = Part{v, M, bad ? -1 : have};
         }
-        __syncthreads();
-        if ((tid & 31) == 0) best_s[tid >> 5] = s, best_at[tid >> 5] = at;
-        __syncthreads();
-        for (int i = 0; i < 32; ++i)
-            if (best_s[i] > s || (best_s[i] == s && best_at[i] < at)) s = best_s[i], at = best_at[i];
-        last = s, last_at = at;
-        if (tid != 0) continue;
-        const size_t o = (size_t)g * p.width + w;
-        const bool none = bad || s == -INFINITY;
-        const int b = (int)(at >> 32), j = (int)(at & 0x7fffffffu);
-        const bool done = !none && over(p, g, b);
-        int64_t id = -1;
-        if (!none)
-            id = done ? p.end_id : p.ids ? p.ids[((size_t)g * p.beams + b) * p.ld_ids + j] : j;
-        p.out_scores[o] = bad ? NAN : (float)s;
-        p.out_parents[o] = none ? -1 : b;
-        p.out_ids[o] = id;
-        if (p.out_ended) p.out_ended[o] = !none && (done || id == p.end_id);
+    } else if (tid == 0) {
+        c.part[blockIdx.x] = Part{0.0, 0.0f, bad ? -1 : have};
     }
 }
 
-static size_t plan(const fdb_beam_args& a, Select* p) {
-    Carve ws(a.workspace);
-    double* lse = ws.take<double>(a.groups * a.beams);
-    if (p) p->lse = lse;
-    return ws.at;
+// ---------------------------------------------------------------------------
+// the best of all chains
+// ---------------------------------------------------------------------------
+constexpr int CAP = 2048, ROUND = 1024;
+enum { LIVE = 0, OVER = 1, ABSENT = 2 };
+struct Choice {
+    uint64_t score[CAP], at[CAP];       // ordered64; chain << 32 | column
+    uint64_t near_score[ASIDE], near_at[ASIDE];
+    uint64_t set[TH], least;
+    double out_score[MAXW];
+    uint64_t out_at[MAXW];
+    int count, total, have;
+};
+__device__ __forceinline__ void add(Choice& s, double v, int b, int j) {
+    const int to = atomicAdd(&s.count, 1);
+    s.score[to] = ordered64(v);
+    s.at[to] = (uint64_t)b << 32 | (uint32_t)j;
 }
-size_t select_bytes(const Ctx&, const fdb_beam_args& a) { return plan(a, nullptr); }
+// The width-th largest of TH values, 0 if there are fewer that are not 0.
+__device__ __forceinline__ uint64_t set_bound(Choice& s, uint64_t v, int width) {
+    s.set[threadIdx.x] = v;
+    __syncthreads();
+    int rank = 0;
+#pragma unroll 8
+    for (int i = 0; i < TH; ++i) rank += s.set[i] > v || (s.set[i] == v && i < (int)threadIdx.x);
+    if (rank == width - 1) s.least = v;
+    __syncthreads();
+    return s.least;
+}
+// The candidates whose scores are not `slack` below the width-th, those in front
+// ranked into out_*.  Returns them: [0, n) of `score` and `at`.  Called by all
+// threads, after a barrier.
+struct Ranked {
+    const uint64_t *score, *at;
+    int n;
+};
+__device__ __forceinline__ Ranked rank_all(Choice& s, int width, double slack) {
+    const int tid = threadIdx.x;
+    Ranked r{s.score, s.at, s.count};
+    if (r.n > TH) {
+        uint64_t m = 0;
+        for (int i = tid; i < r.n; i += TH) m = max(m, s.score[i]);
+        if (tid == 0) s.total = 0;
+        const uint64_t bound = set_bound(s, m, width);
+        const uint64_t least = bound ? ordered64(unordered64(bound) - slack) : 0;
+        for (int i = tid; i < r.n; i += TH) {
+            if (s.score[i] < least) continue;
+            const int to = atomicAdd(&s.total, 1);
+            if (to < ASIDE) s.near_score[to] = s.score[i], s.near_at[to] = s.at[i];
+        }
+        __syncthreads();
+        if (s.total <= ASIDE) r = Ranked{s.near_score, s.near_at, s.total};
+    }
+    for (int i = tid; i < r.n; i += TH) {
+        const uint64_t v = r.score[i], a = r.at[i];
+        int rank = 0;
+#pragma unroll 4
+        for (int j = 0; j < r.n; ++j) {
+            const uint64_t o = r.score[j];
+            rank += o > v || (o == v && r.at[j] < a);
+        }
+        if (rank < width) s.out_score[rank] = unordered64(v), s.out_at[rank] = a;
+    }
+    if (tid == 0) s.have = min(r.n, width);
+    __syncthreads();
+    return r;
+}
+__device__ __forceinline__ void write_out(const Select& p, int g, const Choice& s, bool bad) {
+    for (int w = threadIdx.x; w < p.width; w += TH) {
+        const size_t o = (size_t)g * p.width + w;
+        const bool some = !bad && w < s.have;
+        const int b = some ? (int)(s.out_at[w] >> 32) : -1;
+        const int j = some ? (int)(s.out_at[w] & 0x7fffffffu) : 0;
+        const bool done = some && over(p, g, b);
+        int64_t id = -1;
+        if (some)
+            id = done ? p.end_id : p.ids ? p.ids[((size_t)g * p.beams + b) * p.ld_ids + j] : j;
+        p.out_scores[o] = bad ? NAN : some ? (float)s.out_score[w] : -INFINITY;
+        p.out_parents[o] = b;
+        p.out_ids[o] = id;
+        if (p.out_ended) p.out_ended[o] = some && (done || id == p.end_id);
+    }
+}
 
+// One block per search.  The chains' normalisers are sums of f32 exponentials, off by
+// up to `slack` / 2: where that leaves open which of two chains' columns is the better,
+// among the chosen or at their end, the chains' sums are taken again in 64 bits.
+template <typename T, bool NORM>
+__global__ void __launch_bounds__(TH) finish_kernel(const Select p, const Scan c) {
+    __shared__ Choice s;
+    __shared__ double sum[MAXW], lse[MAXW];
+    __shared__ float top[MAXW];
+    __shared__ unsigned char kind[MAXW], close[MAXW], sure[MAXW];
+    __shared__ double part[TH / 32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = blockIdx.x, S = c.splits;
+    const size_t row0 = (size_t)g * p.beams;
+    // ---- the chains: a warp each ----
+    bool bad = false;
+    for (int b = warp; b < p.beams; b += TH / 32) {
+        const float given = p.beam_scores[row0 + b];
+        const int k = over(p, g, b) ? OVER : LIVE;
+        bad |= !(given < INFINITY);
+        double L = 0.0;
+        float M = -INFINITY;
+        const bool live = k == LIVE && given > -INFINITY;
+        if (live) {
+            for (int i = lane; i < S; i += 32) {
+                const Part q = c.part[(row0 + b) * S + i];
+                bad |= q.count < 0;
+                if (NORM && q.sum > 0.0) M = fmaxf(M, q.m);
+            }
+            if (NORM) {
+#pragma unroll
+                for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+                for (int i = lane; i < S; i += 32) {
+                    const Part q = c.part[(row0 + b) * S + i];
+                    if (q.sum > 0.0) L += q.sum * exp(((double)q.m - (double)M) * p.scale);
+                }
+#pragma unroll
+                for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+            }
+        }
+        if (lane == 0) {
+            sum[b] = given;
+            kind[b] = given == -INFINITY ? ABSENT : k;
+            lse[b] = L > 0.0 ? (double)M * p.scale + log(L) : 0.0;
+            top[b] = M;
+            close[b] = sure[b] = 0;
+        }
+    }
+    if (__syncthreads_or(bad)) return write_out(p, g, s, true);
+
+    // candidate `rank` of list i = chain * splits + part; whether there is one
+    const int lists = p.beams * S;
+    auto candidate = [&](int i, int rank, double& v, int& b, int& j) -> bool {
+        b = i / S;
+        j = 0;
+        v = sum[b];
+        if (kind[b] != LIVE) return kind[b] == OVER && rank == 0 && i == b * S;
+        if (rank >= c.part[row0 * S + i].count) return false;
+        const uint64_t key = c.best[(row0 * S + i) * p.width + rank];
+        j = (int)~(uint32_t)key;
+        v += (double)unordered((uint32_t)(key >> 32)) * p.scale - lse[b];
+        return true;
+    };
+    const double slack = NORM && p.beams > 1 ? (double)c.slack : 0.0;
+    for (;;) {
+        // ---- what the width-th is not below: of the lists' first ones, in TH sets ----
+        uint64_t m = 0;
+        for (int i = tid; i < lists; i += TH) {
+            double v;
+            int b, j;
+            if (candidate(i, 0, v, b, j)) m = max(m, ordered64(v));
+        }
+        if (tid == 0) s.count = 0;
+        uint64_t bound = set_bound(s, m, p.width);
+        double least = bound ? unordered64(bound) - slack : -INFINITY;
+        bool dropped = false;
+        // ---- the lists, so many ranks at a time, until none reaches it ----
+        const int some = min(lists, ROUND), ranks = max(1, ROUND / some);
+        for (int r0 = 0; r0 < p.width; r0 += ranks) {
+            bool any = false;
+            for (int l0 = 0; l0 < lists; l0 += some) {
+#pragma unroll 4
+                for (int k = tid; k < some * ranks; k += TH) {
+                    const int i = l0 + k / ranks, rank = r0 + k % ranks;
+                    double v;
+                    int b, j;
+                    if (i < lists && rank < p.width && candidate(i, rank, v, b, j) && v >= least)
+                        add(s, v, b, j), any = true;
+                }
+                __syncthreads();
+                if (s.count > CAP - ROUND) {
+                    rank_all(s, p.width, 0.0);
+                    for (int w = tid; w < s.have; w += TH)
+                        s.score[w] = ordered64(s.out_score[w]), s.at[w] = s.out_at[w];
+                    if (tid == 0) s.count = s.have;
+                    if (s.have == p.width) least = s.out_score[p.width - 1] - slack;
+                    dropped = true;
+                }
+                __syncthreads();
+            }
+            if (!__syncthreads_or(any)) break;
+        }
+        const Ranked r = rank_all(s, p.width, slack);
+        if (slack == 0.0) break;
+        // ---- is their order sure? ----
+        const int have = s.have;
+        for (int w = tid; w + 1 < have; w += TH) {
+            const int a = (int)(s.out_at[w] >> 32), b = (int)(s.out_at[w + 1] >> 32);
+            if (a != b && s.out_score[w] - s.out_score[w + 1] <= slack) close[a] = close[b] = 1;
+        }
+        if (have == p.width) {
+            const double last = s.out_score[have - 1];
+            const uint64_t last_at = s.out_at[have - 1];
+            const int a = (int)(last_at >> 32);
+            for (int i = tid; i < r.n; i += TH) {
+                const double v = unordered64(r.score[i]);
+                const int b = (int)(r.at[i] >> 32);
+                const bool behind = v < last || (v == last && r.at[i] > last_at);
+                if (behind && b != a && last - v <= slack) close[a] = close[b] = 1;
+            }
+        }
+        if (dropped)
+            for (int b = tid; b < p.beams; b += TH) close[b] = 1;
+        __syncthreads();
+        bool more = false;
+        for (int b = 0; b < p.beams; ++b) {
+            if (!close[b] || sure[b] || kind[b] != LIVE) continue;
+            more = true;
+            if (!(top[b] > -INFINITY)) continue;  // (no columns)
+            double t = 0.0;
+            for (int j = tid; j < p.n; j += TH)
+                t += exp(column<T>(p, g, b, j) - (double)top[b] * p.scale);
+#pragma unroll
+            for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+            if (lane == 0) part[warp] = t;
+            __syncthreads();
+            if (tid == 0) {
+                t = 0.0;
+                for (int i = 0; i < TH / 32; ++i) t += part[i];
+                lse[b] = (double)top[b] * p.scale + log(t);
+            }
+            __syncthreads();
+        }
+        if (!more) break;
+        for (int b = tid; b < p.beams; b += TH) sure[b] |= close[b];
+        __syncthreads();
+    }
+    write_out(p, g, s, false);
+}
+
+// One block per search whose columns are CAP at most in all: their normalisers in 64
+// bits, a warp per chain, and the best.
 template <typename T>
-static void run(const fdb_beam_args& a, const Select& p) {
+__global__ void __launch_bounds__(TH) small_kernel(const Select p) {
+    __shared__ Choice s;
+    const int tid = threadIdx.x, lane = tid & 31, g = blockIdx.x;
+    if (tid == 0) s.count = 0;
+    __syncthreads();
+    bool bad = false;
+    for (int b = tid >> 5; b < p.beams; b += TH / 32) {
+        const double sum = p.beam_scores[(size_t)g * p.beams + b];
+        bad |= !(sum < INFINITY);
+        if (absent(p, g, b)) continue;
+        if (over(p, g, b)) {
+            if (lane == 0) add(s, sum, b, 0);
+            continue;
+        }
+        double lse = 0.0;
+        if (p.normalise) {
+            double m = -INFINITY, t = 0.0;
+            for (int j = lane; j < p.n; j += 32) m = fmax(m, column<T>(p, g, b, j));
+#pragma unroll
+            for (int o = 16; o; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
+            if (m > -INFINITY)
+                for (int j = lane; j < p.n; j += 32) t += exp(column<T>(p, g, b, j) - m);
+#pragma unroll
+            for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+            if (m > -INFINITY) lse = m + log(t);
+        }
+        for (int j = lane; j < p.n; j += 32) {
+            const double v = column<T>(p, g, b, j);
+            bad |= !(v < INFINITY);
+            if (v > -INFINITY) add(s, sum + (v - lse), b, j);
+        }
+    }
+    bad = __syncthreads_or(bad);
+    if (!bad) rank_all(s, p.width, 0.0);
+    write_out(p, g, s, bad);
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+struct Plan {
+    bool small;
+    Scan c;
+    size_t bytes;
+};
+static Plan plan(const Ctx& c, const fdb_beam_args& a) {
+    Plan p{};
+    p.small = a.beams * a.n <= CAP;
+    if (p.small) return p;
+    const size_t rows = a.groups * a.beams, per = a.dtype == FDB_DTYPE_F32 ? 4 : 8;
+    const size_t most = (a.n / per + TH) / TH;  // (a load for every thread)
+    p.c.splits = (int)std::max<size_t>(1, std::min(most, ((size_t)c.sm_count * 8 + rows - 1) / rows));
+    Carve ws(a.workspace);
+    p.c.part = ws.take<Part>(rows * p.c.splits);
+    p.c.best = ws.take<uint64_t>(rows * p.c.splits * a.width);
+    p.bytes = ws.at;
+    return p;
+}
+size_t select_bytes(const Ctx& c, const fdb_beam_args& a) { return plan(c, a).bytes; }
+
+template <typename T, bool NORM>
+static void run(const fdb_beam_args& a, const Select& p, const Scan& c) {
     const cudaStream_t s = static_cast<cudaStream_t>(a.stream);
-    lse_kernel<T><<<(unsigned)(a.groups * a.beams), 256, 0, s>>>(p);
+    const unsigned blocks = (unsigned)(a.groups * a.beams * c.splits);
+    if (a.ids || a.allowed) scan_kernel<T, NORM, true><<<blocks, TH, 0, s>>>(p, c);
+    else scan_kernel<T, NORM, false><<<blocks, TH, 0, s>>>(p, c);
     FDB_LAUNCH_CHECK();
-    pick_kernel<T><<<(unsigned)a.groups, 1024, 0, s>>>(p);
+    finish_kernel<T, NORM><<<(unsigned)a.groups, TH, 0, s>>>(p, c);
     FDB_LAUNCH_CHECK();
 }
-void select_run(const Ctx&, const fdb_beam_args& a) {
+template <typename T>
+static void run(const Ctx& ctx, const fdb_beam_args& a, const Select& p) {
+    Plan l = plan(ctx, a);
+    if (l.small) {
+        small_kernel<T><<<(unsigned)a.groups, TH, 0, static_cast<cudaStream_t>(a.stream)>>>(p);
+        FDB_LAUNCH_CHECK();
+        return;
+    }
+    l.c.s = (float)std::min((double)a.scale * sr::LOG2E, 3e38);
+    // What two normalisers may be off by: the exponentials (2^-22 of themselves, and
+    // once more where a reference is raised), f32 sums of 32 of them in four chains
+    // (8 x 2^-24), and in the exponents, whose mean size under the softmax is at most
+    // log2 n, a subtraction, a product and the factor s (2.5 x 2^-24 ln 2 of them).
+    l.c.slack = (float)(2.0 * (0x1p-21 + 0x1p-21 + 1.75 * 0x1p-24 * (std::log2((double)a.n) + 1.0)));
+    if (a.normalise) run<T, true>(a, p, l.c);
+    else run<T, false>(a, p, l.c);
+}
+void select_run(const Ctx& ctx, const fdb_beam_args& a) {
     Select p{};
     p.x = a.scores;
     p.beams = (int)a.beams, p.n = (int)a.n, p.width = (int)a.width;
@@ -171,69 +748,191 @@ void select_run(const Ctx&, const fdb_beam_args& a) {
     p.beam_scores = a.beam_scores, p.ended = a.ended, p.end_id = a.end_id;
     p.out_scores = a.out_scores, p.out_parents = a.out_parents, p.out_ids = a.out_ids;
     p.out_ended = a.out_ended;
-    plan(a, &p);
-    if (a.dtype == FDB_DTYPE_F32) run<float>(a, p);
-    else if (a.dtype == FDB_DTYPE_F16) run<__half>(a, p);
-    else run<__nv_bfloat16>(a, p);
+    if (a.dtype == FDB_DTYPE_F32) run<float>(ctx, a, p);
+    else if (a.dtype == FDB_DTYPE_F16) run<__half>(ctx, a, p);
+    else run<__nv_bfloat16>(ctx, a, p);
 }
 
 // ---------------------------------------------------------------------------
 // states
 // ---------------------------------------------------------------------------
-// Out of place: a block per run of a row.  In place: a block per 16 bytes x
-// threads of all of a search's rows; a thread reads its bytes of every row before
-// it writes any.
+// All states of a call in one launch (STATES of them).  Out of place a warp moves 4 KB
+// of a run, eight loads a lane in flight, or, of runs that are shorter, several.  In
+// place a thread takes 16 bytes of every row of a search, all of them before it writes
+// any; rows that stay where they are are not touched.  Bound by memory.
+constexpr int STATES = 64;
+constexpr int PIECE = 8;                 // vectors of a lane
 struct State {
     const unsigned char* src;
     unsigned char* dst;
-    size_t src_stride, dst_stride, parts, src_part, dst_part, bytes;
+    size_t src_stride, dst_stride, src_part, dst_part;
+    size_t vecs;                         // of a run
+    unsigned parts, runs, pieces, first; // first: unit of the launch
+    int vec, lanes;                      // log2 of a vector's bytes, of a run's lanes
 };
-__global__ void __launch_bounds__(256)
-    move_kernel(const State t, const int64_t* __restrict__ parents, int beams, int width,
-                int clear) {
-    const size_t row = blockIdx.x / t.parts, part = blockIdx.x % t.parts;
-    const size_t g = row / width;
-    const int64_t from = parents[row];
-    const bool none = from < 0 || from >= beams;
-    if (none && !clear) return;
-    const unsigned char* s = none ? nullptr : t.src + (g * beams + (size_t)from) * t.src_stride + part * t.src_part;
-    unsigned char* d = t.dst + row * t.dst_stride + part * t.dst_part;
-    for (size_t i = threadIdx.x; i < t.bytes; i += 256) d[i] = none ? 0 : s[i];
-}
-__global__ void __launch_bounds__(128)
-    turn_kernel(const State t, const int64_t* __restrict__ parents, int beams) {
-    extern __shared__ unsigned char held[];  // [beams][128]
-    const size_t g = blockIdx.x / t.parts, part = blockIdx.x % t.parts;
-    const size_t row0 = g * beams;
-    for (size_t i = threadIdx.x; i < t.bytes; i += 128) {
-        unsigned char* c = t.dst + row0 * t.dst_stride + part * t.dst_part + i;
-        for (int b = 0; b < beams; ++b) {
-            const int64_t from = parents[row0 + b];
-            if (from >= 0 && from < beams) held[b * 128 + threadIdx.x] = c[from * t.dst_stride];
-        }
-        for (int b = 0; b < beams; ++b) {
-            const int64_t from = parents[row0 + b];
-            if (from >= 0 && from < beams) c[b * t.dst_stride] = held[b * 128 + threadIdx.x];
-        }
+struct States {
+    State e[STATES];
+    int count;
+};
+__device__ __forceinline__ const State& state_of(const States& t, unsigned unit) {
+    int lo = 0, hi = t.count;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (t.e[mid].first <= unit) lo = mid;
+        else hi = mid;
     }
+    return t.e[lo];
 }
-void reorder_run(const Ctx&, const fdb_beam_state* states, size_t count,
+template <typename V>
+__device__ __forceinline__ void move_run(const State& t, unsigned unit, int lane,
+                                         const int64_t* __restrict__ parents, unsigned beams,
+                                         unsigned width, int clear) {
+    const unsigned piece = unit % t.pieces;
+    const unsigned run = (unit / t.pieces << (5 - t.lanes)) + (lane >> t.lanes);
+    if (run >= t.runs) return;
+    const unsigned row = run / t.parts, part = run % t.parts;
+    const int64_t from = parents[row];
+    const bool none = (uint64_t)from >= beams;
+    if (none && !clear) return;
+    const size_t at = (size_t)(row / width) * beams + (none ? 0 : (size_t)from);
+    const V* s = reinterpret_cast<const V*>(t.src + at * t.src_stride + part * t.src_part);
+    V* d = reinterpret_cast<V*>(t.dst + row * t.dst_stride + part * t.dst_part);
+    const size_t v0 = (size_t)piece * (32 * PIECE) + (lane & ((1 << t.lanes) - 1));
+    V r[PIECE];
+#pragma unroll
+    for (int k = 0; k < PIECE; ++k) {
+        r[k] = V();
+        if (v0 + 32 * k < t.vecs && !none) r[k] = __ldg(s + v0 + 32 * k);
+    }
+#pragma unroll
+    for (int k = 0; k < PIECE; ++k)
+        if (v0 + 32 * k < t.vecs) d[v0 + 32 * k] = r[k];
+}
+__global__ void __launch_bounds__(256)
+    move_kernel(const __grid_constant__ States t, const int64_t* __restrict__ parents,
+                unsigned beams, unsigned width, int clear, unsigned units) {
+    const unsigned u = blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (u >= units) return;
+    const State& e = state_of(t, u);
+    const unsigned unit = u - e.first;
+    if (e.vec == 4) move_run<uint4>(e, unit, lane, parents, beams, width, clear);
+    else if (e.vec == 3) move_run<uint2>(e, unit, lane, parents, beams, width, clear);
+    else if (e.vec == 2) move_run<unsigned>(e, unit, lane, parents, beams, width, clear);
+    else if (e.vec == 1) move_run<unsigned short>(e, unit, lane, parents, beams, width, clear);
+    else move_run<unsigned char>(e, unit, lane, parents, beams, width, clear);
+}
+template <typename V>
+__device__ __forceinline__ void turn_run(const State& t, unsigned unit, const int* from, int beams,
+                                         unsigned char* held_raw) {
+    V* held = reinterpret_cast<V*>(held_raw) + threadIdx.x;  // [beams][threads]
+    const unsigned piece = unit % t.pieces, run = unit / t.pieces;
+    const size_t g = run / t.parts, part = run % t.parts;
+    const size_t v = (size_t)piece * blockDim.x + threadIdx.x;
+    if (v >= t.vecs) return;
+    unsigned char* c = t.dst + g * beams * t.dst_stride + part * t.dst_part + v * sizeof(V);
+#pragma unroll 4
+    for (int b = 0; b < beams; ++b)
+        if (from[b] >= 0)
+            held[b * blockDim.x] = *reinterpret_cast<const V*>(c + (size_t)from[b] * t.dst_stride);
+#pragma unroll 4
+    for (int b = 0; b < beams; ++b)
+        if (from[b] >= 0) *reinterpret_cast<V*>(c + (size_t)b * t.dst_stride) = held[b * blockDim.x];
+}
+__global__ void turn_kernel(const __grid_constant__ States t, const int64_t* __restrict__ parents,
+                            int beams) {
+    extern __shared__ uint4 held[];
+    __shared__ int from[MAXW];  // the row that comes, -1: it stays as it is
+    const State& e = state_of(t, blockIdx.x);
+    const unsigned unit = blockIdx.x - e.first;
+    const size_t g = unit / e.pieces / e.parts;
+    for (int b = threadIdx.x; b < beams; b += blockDim.x) {
+        const int64_t f = parents[g * beams + b];
+        from[b] = (uint64_t)f < (uint64_t)beams && f != b ? (int)f : -1;
+    }
+    __syncthreads();
+    unsigned char* h = reinterpret_cast<unsigned char*>(held);
+    if (e.vec == 4) turn_run<uint4>(e, unit, from, beams, h);
+    else if (e.vec == 3) turn_run<uint2>(e, unit, from, beams, h);
+    else if (e.vec == 2) turn_run<unsigned>(e, unit, from, beams, h);
+    else if (e.vec == 1) turn_run<unsigned short>(e, unit, from, beams, h);
+    else turn_run<unsigned char>(e, unit, from, beams, h);
+}
+
+void reorder_run(const Ctx& c, const fdb_beam_state* states, size_t count,
                  const fdb_reorder_opts& o) {
     const cudaStream_t s = static_cast<cudaStream_t>(o.stream);
+    // threads that fit with 16 bytes of every row each
+    const int turn_threads = (int)std::max<size_t>(32, std::min<size_t>(256, 3072 / o.beams / 32 * 32));
+    States move{}, turn{};
+    unsigned long long move_units = 0, turn_units = 0;
+    auto flush_move = [&] {
+        if (move.count)
+            move_kernel<<<(unsigned)((move_units + 7) / 8), 256, 0, s>>>(
+                move, o.parents, (unsigned)o.beams, (unsigned)o.width, o.clear, (unsigned)move_units);
+        FDB_LAUNCH_CHECK();
+        move.count = 0, move_units = 0;
+    };
+    auto flush_turn = [&] {
+        if (turn.count) {
+            const size_t smem = (size_t)turn_threads * o.beams * 16;
+            if (smem > 40960) {  // (with the static part, over what needs no permission)
+                static std::atomic<uint64_t> done{0};
+                sr::allow_smem(turn_kernel, c.device, 65536, done);
+            }
+            turn_kernel<<<(unsigned)turn_units, turn_threads, smem, s>>>(turn, o.parents,
+                                                                         (int)o.beams);
+        }
+        FDB_LAUNCH_CHECK();
+        turn.count = 0, turn_units = 0;
+    };
+    // (all of them looked at before the first is moved)
+    std::vector<State> all;
+    all.reserve(count);
     for (size_t i = 0; i < count; ++i) {
         const fdb_beam_state& a = states[i];
         if (a.bytes == 0 || a.parts == 0) continue;
-        const State t{static_cast<const unsigned char*>(a.src), static_cast<unsigned char*>(a.dst),
-                      a.src_stride, a.dst_stride, a.parts, a.src_part_stride, a.dst_part_stride,
-                      a.bytes};
-        if (a.src == a.dst)
-            turn_kernel<<<(unsigned)(o.groups * a.parts), 128, o.beams * 128, s>>>(
-                t, o.parents, (int)o.beams);
-        else
-            move_kernel<<<(unsigned)(o.groups * o.width * a.parts), 256, 0, s>>>(
-                t, o.parents, (int)o.beams, (int)o.width, o.clear);
-        FDB_LAUNCH_CHECK();
+        const bool here = a.src == a.dst;
+        State t{};
+        t.src = static_cast<const unsigned char*>(a.src), t.dst = static_cast<unsigned char*>(a.dst);
+        t.src_stride = a.src_stride, t.dst_stride = a.dst_stride;
+        t.src_part = a.src_part_stride, t.dst_part = a.dst_part_stride;
+        size_t bytes = a.bytes, parts = a.parts;
+        if (parts > 1 && t.dst_part == bytes && (here || t.src_part == bytes))
+            bytes *= parts, parts = 1;  // (runs without gaps are one)
+        uintptr_t bits = reinterpret_cast<uintptr_t>(a.src) | reinterpret_cast<uintptr_t>(a.dst) |
+                         t.src_stride | t.dst_stride | bytes;
+        if (parts > 1) bits |= t.src_part | t.dst_part;
+        while (t.vec < 4 && !(bits >> t.vec & 1)) ++t.vec;
+        t.vecs = bytes >> t.vec;
+        t.parts = (unsigned)parts;
+        const size_t runs = (here ? o.groups : o.groups * o.width) * parts;
+        t.lanes = 5;
+        while (!here && t.lanes > 0 && t.vecs <= (size_t)1 << (t.lanes - 1)) --t.lanes;
+        const size_t piece = here ? (size_t)turn_threads : t.lanes < 5 ? t.vecs : 32 * PIECE;
+        const size_t pieces = (t.vecs + piece - 1) / piece;
+        const unsigned long long groups = here ? runs : (runs + (32u >> t.lanes) - 1) >> (5 - t.lanes);
+        FDB_REQUIRE(runs < (1ull << 31) && pieces < (1ull << 31) && groups * pieces < (1ull << 31),
+                    FDB_ERR_INVALID_ARG, "a state is too large");
+        t.runs = (unsigned)runs, t.pieces = (unsigned)pieces;
+        t.first = (unsigned)(groups * pieces);  // (its units, until it has a place)
+        all.push_back(t);
     }
+    for (State& t : all) {
+        const bool here = t.src == t.dst;
+        States& table = here ? turn : move;
+        unsigned long long& units = here ? turn_units : move_units;
+        if (table.count == STATES || units + t.first >= (1ull << 31)) {
+            if (here) flush_turn();
+            else flush_move();
+        }
+        const unsigned mine = t.first;
+        t.first = (unsigned)units;
+        table.e[table.count++] = t;
+        units += mine;
+    }
+    flush_move();
+    flush_turn();
 }
 
 }  // namespace beam

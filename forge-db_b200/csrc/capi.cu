@@ -158,6 +158,7 @@ static void check_softmax(const A& a) {
 }
 template <class A>
 static void check_workspace(const A& a, size_t need) {
+    if (need == 0) return;
     FDB_REQUIRE(a.workspace && a.workspace_bytes >= need, FDB_ERR_INVALID_ARG,
                 "the workspace is too small: " + std::to_string(need) + " bytes are needed");
     check_aligned(a.workspace, 256, "the workspace");

@@ -1293,9 +1293,10 @@ def beam_select(scores, beam_scores, *, width: int | None = None, ids=None, scal
                  top.data_ptr(), parents.data_ptr(), out.data_ptr(), done.data_ptr())
     key = (dev.index, "beam", a.dtype, g, b, n, w, a.normalise, ip is None,
            scores.data_ptr() & 15, s0, s1)
-    ws, a.workspace_bytes = _workspace(torch, ctx, L.fdb_beam_select_workspace, a, key, dev,
-                                       workspace)
-    a.workspace = ws.data_ptr()
+    if _ws_bytes.get(key) != 0 or workspace is not None:  # (small searches need none)
+        ws, a.workspace_bytes = _workspace(torch, ctx, L.fdb_beam_select_workspace, a, key, dev,
+                                           workspace)
+        a.workspace = ws.data_ptr()
     a.stream = torch._C._cuda_getCurrentRawStream(dev.index)
     rc = L.fdb_beam_select(ctx.h, C.byref(a))
     if rc:

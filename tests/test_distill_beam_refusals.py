@@ -19,7 +19,7 @@ BASE = dict(dtype=0, queries=256, nq=4, ld_queries=8, rows=512, n=100, ld_rows=8
             teacher_ids=1024, teacher_logits=2048, k=3, ld_ids=3, ld_logits=3, teacher_scale=1.0)
 GRAD = dict(lse=256, logprobs=512, rest_logprob=768, d_loss=1024, d_queries=4096, ld_d_queries=8,
             d_rows=8192, ld_d_rows=8)
-BEAM = dict(dtype=0, scores=256, groups=2, beams=3, n=50, ld_group=150, ld_beam=50, scale=1.0,
+BEAM = dict(dtype=0, scores=256, groups=2, beams=3, n=1000, ld_group=3000, ld_beam=1000, scale=1.0,
             normalise=1, beam_scores=512, width=3, out_scores=1024, out_parents=2048, out_ids=4096)
 
 
@@ -92,8 +92,8 @@ def test_gradient_buffers(call, change, code, text):
     (dict(beams=0), -1, b"FDB_MAX_BEAMS"), (dict(beams=129), -1, b"FDB_MAX_BEAMS"),
     (dict(width=0), -1, b"FDB_MAX_BEAMS"), (dict(width=129), -1, b"FDB_MAX_BEAMS"),
     (dict(groups=1 << 22), -1, b"groups"), (dict(scale=0.0), -1, b"scale"),
-    (dict(scale=float("inf")), -1, b"scale"), (dict(ld_beam=49), -2, b"ld_beam"),
-    (dict(ids=64, ld_ids=49), -2, b"ld_ids"), (dict(allowed=64, ld_allowed=1), -2, b"ld_allowed"),
+    (dict(scale=float("inf")), -1, b"scale"), (dict(ld_beam=999), -2, b"ld_beam"),
+    (dict(ids=64, ld_ids=999), -2, b"ld_ids"), (dict(allowed=64, ld_allowed=31), -2, b"ld_allowed"),
 ])
 def test_select_refuses(call, change, code, text):
     fg, L, ctx = call
@@ -107,7 +107,7 @@ def test_select_refuses(call, change, code, text):
 @pytest.mark.parametrize("change,text", [
     (dict(scores=None), b"NULL"), (dict(beam_scores=None), b"NULL"), (dict(out_scores=None), b"NULL"),
     (dict(out_parents=None), b"NULL"), (dict(out_ids=None), b"NULL"), (dict(scores=258), b"scores"),
-    (dict(ids=260, ld_ids=50), b"ids"), (dict(beam_scores=514), b"beam_scores"),
+    (dict(ids=260, ld_ids=1000), b"ids"), (dict(beam_scores=514), b"beam_scores"),
     (dict(out_parents=2052), b"out_parents"), (dict(out_ids=4100), b"out_ids"),
     (dict(workspace=None), b"workspace"), (dict(workspace=1024 + 128), b"workspace"),
     (dict(workspace_bytes=1), b"workspace"),
