@@ -94,14 +94,20 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 // ---------------------------------------------------------------------------
 // scanning the chains' columns
 // ---------------------------------------------------------------------------
-// A block takes a part of a chain's columns, TILE at a time, 16 bytes a load, and
-// leaves their sum of exponentials and the `width` best.  Sums are taken relative to a
-// thread's own largest score so far (raised only when it is exceeded by 2^8), 32
-// terms in f32 and those in 64 bits.  A column is looked at again only if it is above
-// the width-th best so far: of the first tile, if it reaches the least of the
-// largest of G >= width groups of threads, which at least G columns do.
+// A block takes a part of a chain's columns, a tile of TH * U loads of 16 bytes at a
+// time, and leaves their sum of exponentials and the `width` best.  The pass over the
+// columns only adds up and keeps each thread's largest of a tile: 130 instructions and
+// 32 exponentials for 32 columns of 16 bits, no barrier.  The best are found from those
+// maxima afterwards: of the threads' largest the width-th (or, for few, the least of
+// the largest of G >= width groups of threads) is reached by at least `width` columns
+// and by hardly more; only the maxima that reach it are looked behind, by reading
+// their columns again.
+// Sums are taken relative to a thread's own largest score so far (raised only when it
+// is exceeded by 2^8), 32 terms in f32 and those in 64 bits.
 constexpr int TH = 256;               // threads
 constexpr int U = 4;                  // loads of a thread in a tile
+constexpr int TILES = 16;             // of a block
+constexpr int GROUPS = 1024;          // maxima looked behind at once
 constexpr int MAXW = FDB_MAX_BEAMS;
 constexpr float RAISE = 8.0f;
 
@@ -218,7 +224,8 @@ constexpr int LIMIT = 256;              // keys that are put in order at once
 constexpr int ASIDE = 512;
 struct Best {
     uint64_t* buf;                      // [LIMIT + TH * columns of a vector]
-    uint64_t aside[ASIDE], out[MAXW], least;
+    alignas(16) uint64_t aside[ASIDE];  // (read four floats at a time, too)
+    uint64_t out[MAXW], least;
     int count, total;
 };
 // Leaves the `width` best of s.count keys, which all differ, in order at buf's front
@@ -265,14 +272,22 @@ __device__ __forceinline__ int keep_best(Best& s, int width) {
     return n;
 }
 
+template <typename T>
+struct ScanShared {
+    float top[TILES][TH];
+    uint64_t buf[LIMIT + TH * Vec<T>::N];
+    Best s;
+    int list[GROUPS], groups;
+    float warp_min[TH / 32], warp_m[TH / 32];
+    double warp_sum[TH / 32];
+};
 template <typename T, bool NORM, bool GATE>
 __global__ void __launch_bounds__(TH, 4) scan_kernel(const Select p, const Scan c) {
-    constexpr int N = Vec<T>::N;
-    __shared__ uint64_t buf[LIMIT + TH * N];
-    __shared__ Best s;
-    __shared__ float warp_min[TH / 32];
-    __shared__ double warp_sum[TH / 32];
-    __shared__ float warp_m[TH / 32];
+    constexpr int N = Vec<T>::N, STEP = TH * U;
+    extern __shared__ uint4 scan_raw[];
+    ScanShared<T>& sh = *reinterpret_cast<ScanShared<T>*>(scan_raw);
+    Best& s = sh.s;
+    uint64_t* buf = sh.buf;
     const int tid = threadIdx.x;
     const size_t row = blockIdx.x / c.splits;
     const int sp = blockIdx.x % c.splits, g = (int)(row / p.beams), b = (int)(row % p.beams);
@@ -281,28 +296,31 @@ __global__ void __launch_bounds__(TH, 4) scan_kernel(const Select p, const Scan 
     const int skip = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
     const long long nv = ((long long)p.n + skip + N - 1) / N;
     const int v0 = (int)(nv * sp / c.splits), v1 = (int)(nv * (sp + 1) / c.splits);
-    if (tid == 0) s.count = 0, s.buf = buf;
 
-    float tau = -INFINITY, m = 0.0f;
+    // ---- sums, and the largest of each thread's columns of a tile ----
+    float m = 0.0f, most = -INFINITY;
     double sum = 0.0;
-    bool started = false, bad = false;
+    bool started = false;
     uint4 next[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
         next[u] = load_vec<T, GATE>(p, x, skip, row, v0 + u * TH + tid, v1);
-    for (int at = v0; at < v1; at += TH * U) {
+    int tiles = 0;
+#pragma unroll 1
+    for (int at = v0; at < v1; at += STEP, ++tiles) {
         uint4 r[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) r[u] = next[u];
-        if (at + TH * U < v1) {
+        if (at + STEP < v1) {
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                next[u] = load_vec<T, GATE>(p, x, skip, row, at + (U + u) * TH + tid, v1);
+                next[u] = load_vec<T, GATE>(p, x, skip, row, at + STEP + u * TH + tid, v1);
         }
         float top = -INFINITY;
 #pragma unroll
         for (int u = 0; u < U; ++u) top = Vec<T>::max4(r[u], top);
-        bad |= !(top < INFINITY);
+        sh.top[tiles][tid] = top;
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(top));
         if (NORM) {
             if (top > -INFINITY && (!started || (top - m) * c.s > RAISE)) {
                 if (started) sum *= (double)sr::ex2((m - top) * c.s);
@@ -325,64 +343,96 @@ __global__ void __launch_bounds__(TH, 4) scan_kernel(const Select p, const Scan 
             unpack2(add2(acc[0], acc[1]), a0, a1);
             sum += (double)(a0 + a1);
         }
-        const bool first = at == v0;
-        if (first) {
-            // the least of the largest of G >= width groups of threads
-            int groups = 8;
-            while (groups < p.width) groups <<= 1;
-            float t = top;
-            for (int o = 1; o < TH / groups; o <<= 1)
-                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+    }
+    if (tid == 0) s.count = 0, s.buf = buf, sh.groups = 0;
+    const bool bad = __syncthreads_or(!(most < INFINITY));
+
+    // ---- a bound that at least `width` columns reach ----
+    float tau = -INFINITY;
+    if (p.width <= 16) {
+        const int group = p.width <= 8 ? 32 : 16;
+        float t = most;
 #pragma unroll
-            for (int o = 16; o; o >>= 1) t = fminf(t, __shfl_xor_sync(0xffffffffu, t, o));
-            if ((tid & 31) == 0) warp_min[tid >> 5] = t;
-            __syncthreads();
-            tau = warp_min[0];
-#pragma unroll
-            for (int i = 1; i < TH / 32; ++i) tau = fminf(tau, warp_min[i]);
+        for (int o = 1; o < 32; o <<= 1) {
+            const float v = __shfl_xor_sync(0xffffffffu, t, o);
+            t = o < group ? fmaxf(t, v) : fminf(t, v);
         }
-        // a column enters if it is above tau (in the first tile, if it reaches it): of
-        // equal ones the lower, which came before, is kept
-        const bool hit = top > -INFINITY && (first ? top >= tau : top > tau);
-        const int hits = __syncthreads_count(hit);
-        if (hits == 0) continue;
-        auto enter = [&](const uint4& v, int u, bool reach) -> bool {
-            bool full = false;
+        if ((tid & 31) == 0) sh.warp_min[tid >> 5] = t;
+        __syncthreads();
+        tau = sh.warp_min[0];
 #pragma unroll
-            for (int i = 0; i < N / 2; ++i) {
-                const float2 f = Vec<T>::pair(v, i);
+        for (int i = 1; i < TH / 32; ++i) tau = fminf(tau, sh.warp_min[i]);
+    } else {
+        float* all = reinterpret_cast<float*>(s.aside);
+        all[tid] = most;
+        __syncthreads();
+        int above = 0, from = 0;
+        const float4* four = reinterpret_cast<const float4*>(all);
+#pragma unroll 8
+        for (int i = 0; i < TH / 4; ++i) {
+            const float4 v = four[i];
+            above += (v.x > most) + (v.y > most) + (v.z > most) + (v.w > most);
+            from += (v.x >= most) + (v.y >= most) + (v.z >= most) + (v.w >= most);
+        }
+        if (above < p.width && p.width <= from) sh.warp_min[0] = most;  // (equal ones all write the same)
+        __syncthreads();
+        tau = bad ? -INFINITY : sh.warp_min[0];
+    }
+    // ---- the maxima that reach it, and the columns behind them ----
+    for (int t = 0; t < tiles; ++t) {
+        const float top = sh.top[t][tid];
+        if (top > -INFINITY && top >= tau && !bad) {
+            const int to = atomicAdd(&sh.groups, 1);
+            if (to < GROUPS) sh.list[to] = t * TH + tid;
+        }
+    }
+    __syncthreads();
+    const int groups = sh.groups;
+    auto enter = [&](const uint4& v, int first, bool reach, int room) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float y = h ? f.y : f.x;
-                    if (!(y > -INFINITY) || !(reach ? y >= tau : y > tau)) continue;
-                    const int col = (at + u * TH + tid) * N - skip + 2 * i + h;
-                    const int to = atomicAdd(&s.count, 1);
-                    buf[to] = (uint64_t)ordered(y) << 32 | (uint32_t)~col;
-                    full |= to >= LIMIT - 1;
-                }
+        for (int i = 0; i < N / 2; ++i) {
+            const float2 f = Vec<T>::pair(v, i);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float y = h ? f.y : f.x;
+                if (!(y > -INFINITY) || !(reach ? y >= tau : y > tau)) continue;
+                const int to = atomicAdd(&s.count, 1);
+                if (to < room) buf[to] = (uint64_t)ordered(y) << 32 | (uint32_t)~(first + 2 * i + h);
             }
-            return full;
-        };
-        auto settle = [&](bool full) -> bool {  // whether the width best are known now
-            if (!__syncthreads_or(full) || keep_best(s, p.width) < p.width) return false;
-            tau = unordered((uint32_t)(buf[p.width - 1] >> 32));
-            return true;
-        };
-        if (hits * U <= TH) {  // (there is room for all that they may hold)
-            bool full = false;
-            if (hit) {
-#pragma unroll
-                for (int u = 0; u < U; ++u) full |= enter(r[u], u, first);
-            }
-            settle(full || first);
-        } else {
-            bool reach = first;
-#pragma unroll
+        }
+    };
+    constexpr int ROOM = LIMIT + TH * N;
+    bool all = groups > GROUPS;
+    if (!all) {
+        for (int k = tid; k < groups * U; k += TH) {
+            const int e = sh.list[k / U], at = v0 + e / TH * STEP + k % U * TH + e % TH;
+            enter(load_vec<T, GATE>(p, x, skip, row, at, v1), at * N - skip, true, ROOM);
+        }
+        __syncthreads();
+        all = s.count > ROOM;
+    }
+    if (all) {
+        // too many columns are as good: tile by tile, the best kept at any time.  (A
+        // column that equals the width-th and lies further on is not better.)
+        __syncthreads();
+        if (tid == 0) s.count = 0;
+        __syncthreads();
+        bool reach = true;
+        for (int t = 0; t < tiles; ++t) {
+            const float top = sh.top[t][tid];
+            const bool hit = top > -INFINITY && (reach ? top >= tau : top > tau);
+            if (!__syncthreads_or(hit)) continue;
+#pragma unroll 1
             for (int u = 0; u < U; ++u) {
-                bool full = false;
-                if (hit) full = enter(r[u], u, reach);
-                // (once they are, an equal one further on is not better)
-                if (settle(full || (first && u == U - 1))) reach = false;
+                const int at = v0 + t * STEP + u * TH + tid;
+                if (hit) enter(load_vec<T, GATE>(p, x, skip, row, at, v1), at * N - skip, reach, ROOM);
+                __syncthreads();
+                const bool full = s.count >= LIMIT;
+                __syncthreads();
+                if (full && keep_best(s, p.width) == p.width) {
+                    tau = unordered((uint32_t)(buf[p.width - 1] >> 32));
+                    reach = false;
+                }
             }
         }
     }
@@ -391,23 +441,22 @@ __global__ void __launch_bounds__(TH, 4) scan_kernel(const Select p, const Scan 
     uint64_t* out = c.best + (size_t)blockIdx.x * p.width;
     for (int i = tid; i < have; i += TH) out[i] = buf[i];
     // ---- the sums ----
-    bad = __syncthreads_or(bad);
     if (NORM) {
         float M = started ? m : -INFINITY;
 #pragma unroll
         for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-        if ((tid & 31) == 0) warp_m[tid >> 5] = M;
+        if ((tid & 31) == 0) sh.warp_m[tid >> 5] = M;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < TH / 32; ++i) M = fmaxf(M, warp_m[i]);
+        for (int i = 0; i < TH / 32; ++i) M = fmaxf(M, sh.warp_m[i]);
         double v = started && M < INFINITY ? sum * (double)sr::ex2((m - M) * c.s) : 0.0;
 #pragma unroll
         for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if ((tid & 31) == 0) warp_sum[tid >> 5] = v;
+        if ((tid & 31) == 0) sh.warp_sum[tid >> 5] = v;
         __syncthreads();
         if (tid == 0) {
             v = 0.0;
-            for (int i = 0; i < TH / 32; ++i) v += warp_sum[i];
+            for (int i = 0; i < TH / 32; ++i) v += sh.warp_sum[i];
             c.part[blockIdx.x] = Part{v, M, bad ? -1 : have};
         }
     } else if (tid == 0) {
@@ -701,7 +750,8 @@ static Plan plan(const Ctx& c, const fdb_beam_args& a) {
     if (p.small) return p;
     const size_t rows = a.groups * a.beams, per = a.dtype == FDB_DTYPE_F32 ? 4 : 8;
     const size_t most = (a.n / per + TH) / TH;  // (a load for every thread)
-    p.c.splits = (int)std::max<size_t>(1, std::min(most, ((size_t)c.sm_count * 8 + rows - 1) / rows));
+    const size_t least = (a.n / per + 2 + TILES * TH * U - 1) / (TILES * TH * U);
+    p.c.splits = (int)std::max(least, std::min(most, ((size_t)c.sm_count * 4 + rows - 1) / rows));
     Carve ws(a.workspace);
     p.c.part = ws.take<Part>(rows * p.c.splits);
     p.c.best = ws.take<uint64_t>(rows * p.c.splits * a.width);
@@ -710,13 +760,22 @@ static Plan plan(const Ctx& c, const fdb_beam_args& a) {
 }
 size_t select_bytes(const Ctx& c, const fdb_beam_args& a) { return plan(c, a).bytes; }
 
+template <typename T, bool NORM, bool GATE>
+static void launch_scan(cudaStream_t s, int device, unsigned blocks, const Select& p, const Scan& c) {
+    constexpr size_t smem = sizeof(ScanShared<T>);
+    if (smem > 48 * 1024) {
+        static std::atomic<uint64_t> done{0};
+        sr::allow_smem(scan_kernel<T, NORM, GATE>, device, smem, done);
+    }
+    scan_kernel<T, NORM, GATE><<<blocks, TH, smem, s>>>(p, c);
+    FDB_LAUNCH_CHECK();
+}
 template <typename T, bool NORM>
-static void run(const fdb_beam_args& a, const Select& p, const Scan& c) {
+static void run(int device, const fdb_beam_args& a, const Select& p, const Scan& c) {
     const cudaStream_t s = static_cast<cudaStream_t>(a.stream);
     const unsigned blocks = (unsigned)(a.groups * a.beams * c.splits);
-    if (a.ids || a.allowed) scan_kernel<T, NORM, true><<<blocks, TH, 0, s>>>(p, c);
-    else scan_kernel<T, NORM, false><<<blocks, TH, 0, s>>>(p, c);
-    FDB_LAUNCH_CHECK();
+    if (a.ids || a.allowed) launch_scan<T, NORM, true>(s, device, blocks, p, c);
+    else launch_scan<T, NORM, false>(s, device, blocks, p, c);
     finish_kernel<T, NORM><<<(unsigned)a.groups, TH, 0, s>>>(p, c);
     FDB_LAUNCH_CHECK();
 }
@@ -734,8 +793,8 @@ static void run(const Ctx& ctx, const fdb_beam_args& a, const Select& p) {
     // (8 x 2^-24), and in the exponents, whose mean size under the softmax is at most
     // log2 n, a subtraction, a product and the factor s (2.5 x 2^-24 ln 2 of them).
     l.c.slack = (float)(2.0 * (0x1p-21 + 0x1p-21 + 1.75 * 0x1p-24 * (std::log2((double)a.n) + 1.0)));
-    if (a.normalise) run<T, true>(a, p, l.c);
-    else run<T, false>(a, p, l.c);
+    if (a.normalise) run<T, true>(ctx.device, a, p, l.c);
+    else run<T, false>(ctx.device, a, p, l.c);
 }
 void select_run(const Ctx& ctx, const fdb_beam_args& a) {
     Select p{};
@@ -798,15 +857,24 @@ __device__ __forceinline__ void move_run(const State& t, unsigned unit, int lane
     const V* s = reinterpret_cast<const V*>(t.src + at * t.src_stride + part * t.src_part);
     V* d = reinterpret_cast<V*>(t.dst + row * t.dst_stride + part * t.dst_part);
     const size_t v0 = (size_t)piece * (32 * PIECE) + (lane & ((1 << t.lanes) - 1));
+    s += v0, d += v0;
+    const int left = (int)min(t.vecs - min(v0, t.vecs), (size_t)32 * PIECE);
     V r[PIECE];
+    if (left > 32 * (PIECE - 1) && !none) {
+#pragma unroll
+        for (int k = 0; k < PIECE; ++k) r[k] = __ldcs(s + 32 * k);
+#pragma unroll
+        for (int k = 0; k < PIECE; ++k) __stcs(d + 32 * k, r[k]);
+        return;
+    }
 #pragma unroll
     for (int k = 0; k < PIECE; ++k) {
         r[k] = V();
-        if (v0 + 32 * k < t.vecs && !none) r[k] = __ldg(s + v0 + 32 * k);
+        if (32 * k < left && !none) r[k] = __ldcs(s + 32 * k);
     }
 #pragma unroll
     for (int k = 0; k < PIECE; ++k)
-        if (v0 + 32 * k < t.vecs) d[v0 + 32 * k] = r[k];
+        if (32 * k < left) d[32 * k] = r[k];
 }
 __global__ void __launch_bounds__(256)
     move_kernel(const __grid_constant__ States t, const int64_t* __restrict__ parents,
