@@ -6,6 +6,7 @@
 //
 // Scores are compared in 64 bits, as a 32-bit sum of two of them would make equal
 // what is not.
+#include <climits>
 #include <cmath>
 
 #include "softmax_rows.cuh"
@@ -278,7 +279,7 @@ struct ScanShared {
     uint64_t buf[LIMIT + TH * Vec<T>::N];
     Best s;
     int list[GROUPS], groups;
-    float warp_min[TH / 32], warp_m[TH / 32];
+    float warp_min[TH / 32], warp_m[TH / 32], bound;
     double warp_sum[TH / 32];
 };
 template <typename T, bool NORM, bool GATE>
@@ -297,25 +298,34 @@ __global__ void __launch_bounds__(TH, 4) scan_kernel(const Select p, const Scan 
     const long long nv = ((long long)p.n + skip + N - 1) / N;
     const int v0 = (int)(nv * sp / c.splits), v1 = (int)(nv * (sp + 1) / c.splits);
 
+    if (tid == 0) s.count = 0, s.buf = buf, sh.groups = 0;
+
     // ---- sums, and the largest of each thread's columns of a tile ----
     float m = 0.0f, most = -INFINITY;
     double sum = 0.0;
     bool started = false;
     uint4 next[U];
+    const uint4* vecs = reinterpret_cast<const uint4*>(x - skip);
+    // (whole vectors of columns that all take part are loaded without further ado)
+    const int whole0 = GATE ? INT_MAX : skip ? 1 : 0, whole1 = min(v1, (int)((p.n + (long long)skip) / N));
+    auto load = [&](int at) {
+        if (at >= whole0 && at + STEP <= whole1) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-        next[u] = load_vec<T, GATE>(p, x, skip, row, v0 + u * TH + tid, v1);
+            for (int u = 0; u < U; ++u) next[u] = __ldcs(vecs + (at + u * TH + tid));
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                next[u] = load_vec<T, GATE>(p, x, skip, row, at + u * TH + tid, v1);
+        }
+    };
+    load(v0);
     int tiles = 0;
 #pragma unroll 1
     for (int at = v0; at < v1; at += STEP, ++tiles) {
         uint4 r[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) r[u] = next[u];
-        if (at + STEP < v1) {
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                next[u] = load_vec<T, GATE>(p, x, skip, row, at + STEP + u * TH + tid, v1);
-        }
+        if (at + STEP < v1) load(at + STEP);
         float top = -INFINITY;
 #pragma unroll
         for (int u = 0; u < U; ++u) top = Vec<T>::max4(r[u], top);
@@ -344,46 +354,55 @@ __global__ void __launch_bounds__(TH, 4) scan_kernel(const Select p, const Scan 
             sum += (double)(a0 + a1);
         }
     }
-    if (tid == 0) s.count = 0, s.buf = buf, sh.groups = 0;
+    // ---- a bound that at least `width` columns reach; the sums ----
+    float bound = most, M = started ? m : -INFINITY;
+    const int group = p.width <= 8 ? 32 : 16;  // (of threads, for 8 or 16 groups)
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const float v = __shfl_xor_sync(0xffffffffu, bound, o);
+        bound = o < group ? fmaxf(bound, v) : fminf(bound, v);
+        if (NORM) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    }
+    float* all_most = reinterpret_cast<float*>(s.aside);
+    if ((tid & 31) == 0) sh.warp_min[tid >> 5] = bound, sh.warp_m[tid >> 5] = M;
+    if (p.width > 16) all_most[tid] = most;
     const bool bad = __syncthreads_or(!(most < INFINITY));
-
-    // ---- a bound that at least `width` columns reach ----
-    float tau = -INFINITY;
-    if (p.width <= 16) {
-        const int group = p.width <= 8 ? 32 : 16;
-        float t = most;
+    float tau = sh.warp_min[0];
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const float v = __shfl_xor_sync(0xffffffffu, t, o);
-            t = o < group ? fmaxf(t, v) : fminf(t, v);
-        }
-        if ((tid & 31) == 0) sh.warp_min[tid >> 5] = t;
-        __syncthreads();
-        tau = sh.warp_min[0];
-#pragma unroll
-        for (int i = 1; i < TH / 32; ++i) tau = fminf(tau, sh.warp_min[i]);
-    } else {
-        float* all = reinterpret_cast<float*>(s.aside);
-        all[tid] = most;
-        __syncthreads();
+    for (int i = 1; i < TH / 32; ++i) tau = fminf(tau, sh.warp_min[i]);
+    if (p.width > 16) {
         int above = 0, from = 0;
-        const float4* four = reinterpret_cast<const float4*>(all);
+        const float4* four = reinterpret_cast<const float4*>(all_most);
 #pragma unroll 8
         for (int i = 0; i < TH / 4; ++i) {
             const float4 v = four[i];
             above += (v.x > most) + (v.y > most) + (v.z > most) + (v.w > most);
             from += (v.x >= most) + (v.y >= most) + (v.z >= most) + (v.w >= most);
         }
-        if (above < p.width && p.width <= from) sh.warp_min[0] = most;  // (equal ones all write the same)
+        if (above < p.width && p.width <= from) sh.bound = most;  // (equal ones all write the same)
         __syncthreads();
-        tau = bad ? -INFINITY : sh.warp_min[0];
+        tau = sh.bound;
+    }
+    if (NORM) {
+#pragma unroll
+        for (int i = 0; i < TH / 32; ++i) M = fmaxf(M, sh.warp_m[i]);
+        sum = started && M < INFINITY ? sum * (double)sr::ex2((m - M) * c.s) : 0.0;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if ((tid & 31) == 0) sh.warp_sum[tid >> 5] = sum;
     }
     // ---- the maxima that reach it, and the columns behind them ----
-    for (int t = 0; t < tiles; ++t) {
-        const float top = sh.top[t][tid];
-        if (top > -INFINITY && top >= tau && !bad) {
-            const int to = atomicAdd(&sh.groups, 1);
-            if (to < GROUPS) sh.list[to] = t * TH + tid;
+    if (bad) {
+        if (tid == 0) c.part[blockIdx.x] = Part{0.0, 0.0f, -1};
+        return;
+    }
+    if (most > -INFINITY && most >= tau) {
+        for (int t = 0; t < tiles; ++t) {
+            const float top = sh.top[t][tid];
+            if (top > -INFINITY && top >= tau) {
+                const int to = atomicAdd(&sh.groups, 1);
+                if (to < GROUPS) sh.list[to] = t * TH + tid;
+            }
         }
     }
     __syncthreads();
@@ -437,30 +456,25 @@ __global__ void __launch_bounds__(TH, 4) scan_kernel(const Select p, const Scan 
         }
     }
     __syncthreads();
-    const int have = keep_best(s, p.width);
     uint64_t* out = c.best + (size_t)blockIdx.x * p.width;
-    for (int i = tid; i < have; i += TH) out[i] = buf[i];
-    // ---- the sums ----
-    if (NORM) {
-        float M = started ? m : -INFINITY;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-        if ((tid & 31) == 0) sh.warp_m[tid >> 5] = M;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < TH / 32; ++i) M = fmaxf(M, sh.warp_m[i]);
-        double v = started && M < INFINITY ? sum * (double)sr::ex2((m - M) * c.s) : 0.0;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if ((tid & 31) == 0) sh.warp_sum[tid >> 5] = v;
-        __syncthreads();
-        if (tid == 0) {
-            v = 0.0;
-            for (int i = 0; i < TH / 32; ++i) v += sh.warp_sum[i];
-            c.part[blockIdx.x] = Part{v, M, bad ? -1 : have};
+    const int count = s.count, have = min(count, p.width);
+    if (count <= TH) {
+        if (tid < count) {
+            const uint64_t v = buf[tid];
+            int rank = 0;
+#pragma unroll 4
+            for (int i = 0; i < count; ++i) rank += buf[i] > v;
+            if (rank < p.width) out[rank] = v;
         }
-    } else if (tid == 0) {
-        c.part[blockIdx.x] = Part{0.0, 0.0f, bad ? -1 : have};
+    } else {
+        keep_best(s, p.width);
+        for (int i = tid; i < have; i += TH) out[i] = buf[i];
+    }
+    if (tid == 0) {
+        double v = 0.0;
+        if (NORM)
+            for (int i = 0; i < TH / 32; ++i) v += sh.warp_sum[i];
+        c.part[blockIdx.x] = Part{v, M, have};
     }
 }
 
@@ -472,7 +486,8 @@ enum { LIVE = 0, OVER = 1, ABSENT = 2 };
 struct Choice {
     uint64_t score[CAP], at[CAP];       // ordered64; chain << 32 | column
     uint64_t near_score[ASIDE], near_at[ASIDE];
-    uint64_t set[TH], least;
+    alignas(16) float set[TH];
+    float bound;
     double out_score[MAXW];
     uint64_t out_at[MAXW];
     int count, total, have;
@@ -482,16 +497,25 @@ __device__ __forceinline__ void add(Choice& s, double v, int b, int j) {
     s.score[to] = ordered64(v);
     s.at[to] = (uint64_t)b << 32 | (uint32_t)j;
 }
-// The width-th largest of TH values, 0 if there are fewer that are not 0.
-__device__ __forceinline__ uint64_t set_bound(Choice& s, uint64_t v, int width) {
-    s.set[threadIdx.x] = v;
+// The width-th largest of n values, -inf if there are fewer.
+__device__ __forceinline__ float set_bound(Choice& s, float v, int n, int width) {
+    const int tid = threadIdx.x;
+    s.set[tid] = v;
+    if (tid == 0) s.bound = -INFINITY;
     __syncthreads();
-    int rank = 0;
-#pragma unroll 8
-    for (int i = 0; i < TH; ++i) rank += s.set[i] > v || (s.set[i] == v && i < (int)threadIdx.x);
-    if (rank == width - 1) s.least = v;
+    int above = 0, from = 0;
+    const float4* four = reinterpret_cast<const float4*>(s.set);
+    if (tid < n) {
+#pragma unroll 4
+        for (int i = 0; i < (n + 3) / 4; ++i) {  // (past n: -inf)
+            const float4 o = four[i];
+            above += (o.x > v) + (o.y > v) + (o.z > v) + (o.w > v);
+            from += (o.x >= v) + (o.y >= v) + (o.z >= v) + (o.w >= v);
+        }
+        if (above < width && width <= from) s.bound = v;  // (equal ones all write the same)
+    }
     __syncthreads();
-    return s.least;
+    return s.bound;
 }
 // The candidates whose scores are not `slack` below the width-th, those in front
 // ranked into out_*.  Returns them: [0, n) of `score` and `at`.  Called by all
@@ -504,11 +528,10 @@ __device__ __forceinline__ Ranked rank_all(Choice& s, int width, double slack) {
     const int tid = threadIdx.x;
     Ranked r{s.score, s.at, s.count};
     if (r.n > TH) {
-        uint64_t m = 0;
-        for (int i = tid; i < r.n; i += TH) m = max(m, s.score[i]);
+        float m = -INFINITY;
+        for (int i = tid; i < r.n; i += TH) m = fmaxf(m, __double2float_rd(unordered64(s.score[i])));
         if (tid == 0) s.total = 0;
-        const uint64_t bound = set_bound(s, m, width);
-        const uint64_t least = bound ? ordered64(unordered64(bound) - slack) : 0;
+        const uint64_t least = ordered64((double)set_bound(s, m, TH, width) - slack);
         for (int i = tid; i < r.n; i += TH) {
             if (s.score[i] < least) continue;
             const int to = atomicAdd(&s.total, 1);
@@ -611,16 +634,17 @@ __global__ void __launch_bounds__(TH) finish_kernel(const Select p, const Scan c
     };
     const double slack = NORM && p.beams > 1 ? (double)c.slack : 0.0;
     for (;;) {
-        // ---- what the width-th is not below: of the lists' first ones, in TH sets ----
-        uint64_t m = 0;
-        for (int i = tid; i < lists; i += TH) {
+        // ---- what the width-th is not below: the width-th of TH candidates, as many of
+        // each list in front as there is room for (or of the maxima of TH sets of lists) ----
+        float m = -INFINITY;
+        const int each = max(1, min(TH / lists, p.width));
+        for (int k = tid; k < lists * each; k += TH) {
             double v;
             int b, j;
-            if (candidate(i, 0, v, b, j)) m = max(m, ordered64(v));
+            if (candidate(k / each, k % each, v, b, j)) m = fmaxf(m, __double2float_rd(v));
         }
         if (tid == 0) s.count = 0;
-        uint64_t bound = set_bound(s, m, p.width);
-        double least = bound ? unordered64(bound) - slack : -INFINITY;
+        double least = (double)set_bound(s, m, min(lists * each, TH), p.width) - slack;
         bool dropped = false;
         // ---- the lists, so many ranks at a time, until none reaches it ----
         const int some = min(lists, ROUND), ranks = max(1, ROUND / some);
@@ -636,7 +660,7 @@ __global__ void __launch_bounds__(TH) finish_kernel(const Select p, const Scan c
                         add(s, v, b, j), any = true;
                 }
                 __syncthreads();
-                if (s.count > CAP - ROUND) {
+                if (s.count > CAP - ROUND) {  // (what is just behind the width-th is dropped)
                     rank_all(s, p.width, 0.0);
                     for (int w = tid; w < s.have; w += TH)
                         s.score[w] = ordered64(s.out_score[w]), s.at[w] = s.out_at[w];
@@ -676,8 +700,18 @@ __global__ void __launch_bounds__(TH) finish_kernel(const Select p, const Scan c
             more = true;
             if (!(top[b] > -INFINITY)) continue;  // (no columns)
             double t = 0.0;
-            for (int j = tid; j < p.n; j += TH)
-                t += exp(column<T>(p, g, b, j) - (double)top[b] * p.scale);
+            const T* x = static_cast<const T*>(p.x) + (size_t)g * p.ld_group + (size_t)b * p.ld_beam;
+            const int skip = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+            const int nv = (int)(((long long)p.n + skip + Vec<T>::N - 1) / Vec<T>::N);
+            for (int v = tid; v < nv; v += TH) {
+                const uint4 q = load_vec<T, true>(p, x, skip, row0 + b, v, nv);
+#pragma unroll
+                for (int i = 0; i < Vec<T>::N / 2; ++i) {
+                    const float2 f = Vec<T>::pair(q, i);
+                    t += exp(((double)f.x - (double)top[b]) * p.scale) +
+                         exp(((double)f.y - (double)top[b]) * p.scale);
+                }
+            }
 #pragma unroll
             for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
             if (lane == 0) part[warp] = t;
