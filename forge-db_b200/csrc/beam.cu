@@ -108,6 +108,7 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 constexpr int TH = 256;               // threads
 constexpr int U = 4;                  // loads of a thread in a tile
 constexpr int TILES = 16;             // of a block
+constexpr int RING = 2;               // tiles on their way
 constexpr int GROUPS = 1024;          // maxima looked behind at once
 constexpr int MAXW = FDB_MAX_BEAMS;
 constexpr float RAISE = 8.0f;
@@ -273,22 +274,36 @@ __device__ __forceinline__ int keep_best(Best& s, int width) {
     return n;
 }
 
+// (the copies in flight are done with when the best are looked for)
 template <typename T>
 struct ScanShared {
+    union {
+        uint4 ring[RING][U][TH];
+        struct {
+            uint64_t buf[LIMIT + TH * Vec<T>::N];
+            Best s;
+            int list[GROUPS];
+        } e;
+    };
     float top[TILES][TH];
-    uint64_t buf[LIMIT + TH * Vec<T>::N];
-    Best s;
-    int list[GROUPS], groups;
     float warp_min[TH / 32], warp_m[TH / 32], bound;
+    int groups;
     double warp_sum[TH / 32];
 };
+// 16 bytes of which `bytes` are read, the others zero.
+__device__ __forceinline__ void copy_async(void* dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                     (uint32_t)__cvta_generic_to_shared(dst)),
+                 "l"(src), "r"(bytes)
+                 : "memory");
+}
 template <typename T, bool NORM, bool GATE>
 __global__ void __launch_bounds__(TH, 4) scan_kernel(const Select p, const Scan c) {
     constexpr int N = Vec<T>::N, STEP = TH * U;
     extern __shared__ uint4 scan_raw[];
     ScanShared<T>& sh = *reinterpret_cast<ScanShared<T>*>(scan_raw);
-    Best& s = sh.s;
-    uint64_t* buf = sh.buf;
+    Best& s = sh.e.s;
+    uint64_t* buf = sh.e.buf;
     const int tid = threadIdx.x;
     const size_t row = blockIdx.x / c.splits;
     const int sp = blockIdx.x % c.splits, g = (int)(row / p.beams), b = (int)(row % p.beams);
@@ -297,39 +312,65 @@ __global__ void __launch_bounds__(TH, 4) scan_kernel(const Select p, const Scan 
     const int skip = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
     const long long nv = ((long long)p.n + skip + N - 1) / N;
     const int v0 = (int)(nv * sp / c.splits), v1 = (int)(nv * (sp + 1) / c.splits);
-
-    if (tid == 0) s.count = 0, s.buf = buf, sh.groups = 0;
+    const int tiles = (v1 - v0 + STEP - 1) / STEP;
+    if (tid == 0) sh.groups = 0;
 
     // ---- sums, and the largest of each thread's columns of a tile ----
+    // Without gates a thread's loads go through its own places of a ring in shared
+    // memory, RING tiles ahead; else through registers, one ahead.
     float m = 0.0f, most = -INFINITY;
     double sum = 0.0;
     bool started = false;
-    uint4 next[U];
+    uint4 next[GATE ? U : 1];
     const uint4* vecs = reinterpret_cast<const uint4*>(x - skip);
-    // (whole vectors of columns that all take part are loaded without further ado)
-    const int whole0 = GATE ? INT_MAX : skip ? 1 : 0, whole1 = min(v1, (int)((p.n + (long long)skip) / N));
-    auto load = [&](int at) {
-        if (at >= whole0 && at + STEP <= whole1) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) next[u] = __ldcs(vecs + (at + u * TH + tid));
-        } else {
+    auto fetch = [&](int t) {
+        if (GATE) {
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                next[u] = load_vec<T, GATE>(p, x, skip, row, at + u * TH + tid, v1);
-        }
-    };
-    load(v0);
-    int tiles = 0;
-#pragma unroll 1
-    for (int at = v0; at < v1; at += STEP, ++tiles) {
-        uint4 r[U];
+                next[u * GATE] = load_vec<T, GATE>(p, x, skip, row, v0 + t * STEP + u * TH + tid, v1);
+        } else {
 #pragma unroll
-        for (int u = 0; u < U; ++u) r[u] = next[u];
-        if (at + STEP < v1) load(at + STEP);
+            for (int u = 0; u < U; ++u) {
+                const int v = v0 + t * STEP + u * TH + tid;
+                // (a first vector that starts in front of the row is read by itself)
+                int left = v < v1 && (v > 0 || skip == 0) ? p.n - (v * N - skip) : 0;
+                left = min(left, N) * (int)sizeof(T);
+                copy_async(&sh.ring[t % RING][u][tid], vecs + (left ? v : 0), left);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int t = 0; t < (GATE ? 1 : RING); ++t)
+        if (t < tiles) fetch(t);
+        else asm volatile("cp.async.commit_group;" ::: "memory");
+#pragma unroll 1
+    for (int t = 0; t < tiles; ++t) {
+        uint4 r[U];
+        if (GATE) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) r[u] = next[u * GATE];
+            if (t + 1 < tiles) fetch(t + 1);
+        } else {
+            asm volatile("cp.async.wait_group %0;" ::"n"(RING - 1) : "memory");
+#pragma unroll
+            for (int u = 0; u < U; ++u) r[u] = sh.ring[t % RING][u][tid];
+            if (t + RING < tiles) fetch(t + RING);
+            else asm volatile("cp.async.commit_group;" ::: "memory");
+            const int at = v0 + t * STEP;
+            if ((at == 0 && skip) || (long long)(at + STEP) * N - skip > p.n || at + STEP > v1) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int v = at + u * TH + tid, j0 = v * N - skip;
+                    if (v >= v1 || j0 < 0 || j0 > p.n - N)
+                        r[u] = load_vec<T, false>(p, x, skip, row, v, v1);
+                }
+            }
+        }
         float top = -INFINITY;
 #pragma unroll
         for (int u = 0; u < U; ++u) top = Vec<T>::max4(r[u], top);
-        sh.top[tiles][tid] = top;
+        sh.top[t][tid] = top;
         asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(top));
         if (NORM) {
             if (top > -INFINITY && (!started || (top - m) * c.s > RAISE)) {
@@ -344,9 +385,9 @@ __global__ void __launch_bounds__(TH, 4) scan_kernel(const Select p, const Scan 
 #pragma unroll
                 for (int i = 0; i < N / 2; ++i) {
                     const float2 f = Vec<T>::pair(r[u], i);
-                    const uint64_t t = mul2(add2(pack2(f.x, f.y), m2), s2);
+                    const uint64_t t2 = mul2(add2(pack2(f.x, f.y), m2), s2);
                     float t0, t1;
-                    unpack2(t, t0, t1);
+                    unpack2(t2, t0, t1);
                     acc[i & 1] = add2(acc[i & 1], pack2(sr::ex2(t0), sr::ex2(t1)));
                 }
             float a0, a1;
@@ -354,6 +395,7 @@ __global__ void __launch_bounds__(TH, 4) scan_kernel(const Select p, const Scan 
             sum += (double)(a0 + a1);
         }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     // ---- a bound that at least `width` columns reach; the sums ----
     float bound = most, M = started ? m : -INFINITY;
     const int group = p.width <= 8 ? 32 : 16;  // (of threads, for 8 or 16 groups)
@@ -365,12 +407,14 @@ __global__ void __launch_bounds__(TH, 4) scan_kernel(const Select p, const Scan 
     }
     float* all_most = reinterpret_cast<float*>(s.aside);
     if ((tid & 31) == 0) sh.warp_min[tid >> 5] = bound, sh.warp_m[tid >> 5] = M;
-    if (p.width > 16) all_most[tid] = most;
     const bool bad = __syncthreads_or(!(most < INFINITY));
+    if (tid == 0) s.count = 0, s.buf = buf;
     float tau = sh.warp_min[0];
 #pragma unroll
     for (int i = 1; i < TH / 32; ++i) tau = fminf(tau, sh.warp_min[i]);
     if (p.width > 16) {
+        all_most[tid] = most;
+        __syncthreads();
         int above = 0, from = 0;
         const float4* four = reinterpret_cast<const float4*>(all_most);
 #pragma unroll 8
@@ -401,7 +445,7 @@ __global__ void __launch_bounds__(TH, 4) scan_kernel(const Select p, const Scan 
             const float top = sh.top[t][tid];
             if (top > -INFINITY && top >= tau) {
                 const int to = atomicAdd(&sh.groups, 1);
-                if (to < GROUPS) sh.list[to] = t * TH + tid;
+                if (to < GROUPS) sh.e.list[to] = t * TH + tid;
             }
         }
     }
@@ -424,7 +468,7 @@ __global__ void __launch_bounds__(TH, 4) scan_kernel(const Select p, const Scan 
     bool all = groups > GROUPS;
     if (!all) {
         for (int k = tid; k < groups * U; k += TH) {
-            const int e = sh.list[k / U], at = v0 + e / TH * STEP + k % U * TH + e % TH;
+            const int e = sh.e.list[k / U], at = v0 + e / TH * STEP + k % U * TH + e % TH;
             enter(load_vec<T, GATE>(p, x, skip, row, at, v1), at * N - skip, true, ROOM);
         }
         __syncthreads();
