@@ -18,7 +18,6 @@ namespace fdb {
 namespace distill {
 
 using sr::Carve;
-using sr::Exact;
 using sr::LN2;
 using sr::LOG2E;
 using sr::to_f32;
@@ -48,31 +47,33 @@ __device__ __forceinline__ int entry_row(const Teacher& t, int q, int e) {
     return (int)id;
 }
 
-// ---- sums and maxima over a block, the same bits in every thread ----
-template <int TH>
-__device__ __forceinline__ double block_sum(double v, double* part) {
+// ---- sums and maxima of C values over a block, the same bits in every thread ----
+// (`part` [TH / 32][C] is the call's own: no barrier guards it from another use.)
+template <int TH, int C, typename V, typename F>
+__device__ __forceinline__ void block_all(V (&v)[C], V* part, F&& both) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.0;
+    for (int o = 16; o; o >>= 1)
 #pragma unroll
-    for (int i = 0; i < TH / 32; ++i) v += part[i];
-    return v;
+        for (int c = 0; c < C; ++c) v[c] = both(v[c], __shfl_xor_sync(0xffffffffu, v[c], o));
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+        for (int c = 0; c < C; ++c) part[(threadIdx.x >> 5) * C + c] = v[c];
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < C; ++c) v[c] = part[c];
+#pragma unroll
+    for (int i = 1; i < TH / 32; ++i)
+#pragma unroll
+        for (int c = 0; c < C; ++c) v[c] = both(v[c], part[i * C + c]);
+}
+template <int TH, int C>
+__device__ __forceinline__ void block_sums(double (&v)[C], double* part) {
+    block_all<TH>(v, part, [](double a, double b) { return a + b; });
 }
 // (a NaN is passed over: the sums that follow carry it)
-template <int TH>
-__device__ __forceinline__ double block_max(double v, double* part) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < TH / 32; ++i) v = fmax(v, part[i]);
-    return v;
+template <int TH, int C>
+__device__ __forceinline__ void block_maxima(float (&v)[C], float* part) {
+    block_all<TH>(v, part, [](float a, float b) { return fmaxf(a, b); });
 }
 
 // A query's entries in shared memory: the rows of those that take part, else -1.
@@ -88,34 +89,26 @@ __device__ __forceinline__ void read_entries(const Teacher& t, int q, int* raw, 
     }
     __syncthreads();
 }
-// log P of an entry is scale z - norm; left: R; any: some entry takes part.
+// The teacher's part, from the largest logit zm of the entries that take part (-inf:
+// there is none) and the sum of exp(scale (z - zm)): log P of an entry is
+// scale z - norm, `left` is R.
 struct Norm {
     double norm, left;
     bool any;
 };
-template <int TH>
-__device__ __forceinline__ Norm teacher_norm(const Teacher& t, int q, const int* row, bool others,
-                                             double* part) {
-    const float* z = t.z + (size_t)q * t.ld;
-    double m = -INFINITY;
-    int mine = 0;
-    for (int e = threadIdx.x; e < t.k; e += TH)
-        if (row[e] >= 0) m = fmax(m, t.scale * (double)z[e]), mine = 1;
-    m = block_max<TH>(m, part);
-    const bool any = __syncthreads_or(mine);
-    double s = 0.0;
-    for (int e = threadIdx.x; e < t.k; e += TH)
-        if (row[e] >= 0) s += exp(t.scale * (double)z[e] - m);
-    s = block_sum<TH>(s, part);
-    Norm n{m + log(s), 0.0, any};
-    if (!any) {
-        n.norm = 0.0;
-        n.left = t.rest && others ? 1.0 : 0.0;
-    } else if (t.rest && others && !(n.norm > 0.0)) {
+__device__ __forceinline__ Norm teacher_norm(const Teacher& t, float zm, double sum, bool any,
+                                             bool others) {
+    if (!any) return Norm{0.0, t.rest && others ? 1.0 : 0.0, false};
+    Norm n{t.scale * (double)zm + log(sum), 0.0, true};
+    if (t.rest && others && !(n.norm > 0.0)) {
         n.left = -expm1(n.norm);  // (NaN stays)
         n.norm = n.norm == n.norm ? 0.0 : NAN;
     }
     return n;
+}
+// exp(scale (z - zm)); of an infinite zm NaN, as it should be.
+__device__ __forceinline__ double above(const Teacher& t, float z, float zm) {
+    return exp(t.scale * ((double)z - (double)zm));
 }
 
 // ---------------------------------------------------------------------------
@@ -145,20 +138,49 @@ struct LossArgs {
     float scale;
     float *loss, *lse, *logprobs, *rest;
 };
-// One block per query: the pass's sums joined, the named rows scored in 64 bits,
-// the loss.  Gathers k rows a query.
+// A vector's products with a query, added up in pairs.
+template <typename T>
+__device__ __forceinline__ float dot_vec(const uint4& v, const float* q) {
+    constexpr int V = 16 / (int)sizeof(T);
+    const T* e = reinterpret_cast<const T*>(&v);
+    float y[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) y[i] = to_f32<T>(e[i]) * q[i];
+#pragma unroll
+    for (int w = V / 2; w; w >>= 1)
+#pragma unroll
+        for (int i = 0; i < w; ++i) y[i] += y[i + w];
+    return y[0];
+}
+// One block per query: the pass's sums joined, the named rows scored (16 bytes'
+// products in f32, their sums in 64 bits), the loss.  Gathers k rows a query.
 template <typename T, int TH>
 __global__ void __launch_bounds__(TH) loss_kernel(const LossArgs p) {
-    extern __shared__ double qs_raw[];
-    typename Exact<T>::Q* qs = reinterpret_cast<typename Exact<T>::Q*>(qs_raw);  // [dim]
+    extern __shared__ float4 q_raw[];
+    float* qs = reinterpret_cast<float*>(q_raw);  // [dim]
     __shared__ int raw[MAXK], row[MAXK], list[MAXK];
-    __shared__ double score[MAXK], part[TH / 32];
+    __shared__ double score[MAXK], sums[TH / 32][3], sums2[TH / 32];
+    __shared__ float maxima[TH / 32][3];
     __shared__ int count;
     const int tid = threadIdx.x, ql = blockIdx.x, q = p.parts.q0 + ql;
     const T* qp = static_cast<const T*>(p.q) + (size_t)q * p.ldq;
     const T* xp = static_cast<const T*>(p.x);
+    const float* z = p.t.z + (size_t)q * p.t.ld;
     if (tid == 0) count = 0;
     for (int c = tid; c < p.d; c += TH) qs[c] = to_f32<T>(qp[c]);
+    // ---- the pass's sums (see finish_kernel): a thread's share ----
+    const sr::Parts& ps = p.parts;
+    float M = -INFINITY;
+    double L = 0.0;
+    for (int i = tid; i < ps.parts; i += TH) {
+        const float4 v = ps.part[(size_t)i * ps.nq + ql];
+        if (v.y == 0.0f && v.z == 0.0f) continue;
+        if (v.x > M) {
+            if (L != 0.0) L *= (double)sr::ex2(M - v.x);
+            M = v.x;
+        }
+        L += v.z == v.z ? (double)(v.y * (v.x == M ? 1.0f : sr::ex2(v.x - M))) : NAN;
+    }
     read_entries<TH>(p.t, q, raw, row);
     for (int e = tid; e < p.t.k; e += TH)
         if (row[e] >= 0) list[atomicAdd(&count, 1)] = e;
@@ -171,53 +193,63 @@ __global__ void __launch_bounds__(TH) loss_kernel(const LossArgs p) {
     const int named = count, per = TH / lanes;
     for (int i = tid / lanes; i - tid / lanes < named; i += ROWS * per) {
         const T* x[ROWS];
-        Exact<T> acc[ROWS];
+        double acc[ROWS];
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r)
+        for (int r = 0; r < ROWS; ++r) {
             x[r] = xp + (size_t)row[list[min(i + r * per, named - 1)]] * p.ldx;
+            acc[r] = 0.0;
+        }
         int c = sub;
         if (wide) {
+#pragma unroll 2
             for (c = sub * V; c + V <= p.d; c += lanes * V) {
                 uint4 v[ROWS];
 #pragma unroll
                 for (int r = 0; r < ROWS; ++r) v[r] = __ldg(reinterpret_cast<const uint4*>(x[r] + c));
+                float y[V];
 #pragma unroll
-                for (int r = 0; r < ROWS; ++r) {
-                    const T* e = reinterpret_cast<const T*>(&v[r]);
+                for (int j = 0; j < V; j += 4)
+                    *reinterpret_cast<float4*>(y + j) = *reinterpret_cast<const float4*>(qs + c + j);
 #pragma unroll
-                    for (int j = 0; j < V; ++j) acc[r].add(to_f32<T>(e[j]), qs[c + j]);
-                }
+                for (int r = 0; r < ROWS; ++r) acc[r] += (double)dot_vec<T>(v[r], y);
             }
             // (the row's last, partial vector: one lane's)
             for (; c < p.d; ++c)
 #pragma unroll
-                for (int r = 0; r < ROWS; ++r) acc[r].add(to_f32<T>(x[r][c]), qs[c]);
+                for (int r = 0; r < ROWS; ++r) acc[r] += (double)(to_f32<T>(x[r][c]) * qs[c]);
         } else {
 #pragma unroll 4
             for (; c < p.d; c += lanes)
 #pragma unroll
-                for (int r = 0; r < ROWS; ++r) acc[r].add(to_f32<T>(x[r][c]), qs[c]);
+                for (int r = 0; r < ROWS; ++r) acc[r] += (double)(to_f32<T>(x[r][c]) * qs[c]);
         }
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) {
-            double s = acc[r].sum();
-            for (int o = lanes >> 1; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            if (sub == 0 && i + r * per < named) score[list[i + r * per]] = s * (double)p.scale;
-        }
+        for (int o = 16; o; o >>= 1)
+            if (o < lanes)
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], o);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+            if (sub == 0 && i + r * per < named) score[list[i + r * per]] = acc[r] * (double)p.scale;
     }
+    __syncthreads();
 
-    // ---- the pass's sums (see finish_kernel) ----
-    const sr::Parts& ps = p.parts;
-    float m = -INFINITY;
-    for (int i = tid; i < ps.parts; i += TH) m = fmaxf(m, ps.part[(size_t)i * ps.nq + ql].x);
-    const float M = (float)block_max<TH>((double)m, part);
-    double L = 0.0;
-    for (int i = tid; i < ps.parts; i += TH) {
-        const float4 v = ps.part[(size_t)i * ps.nq + ql];
-        if (v.y == 0.0f && v.z == 0.0f) continue;
-        L += v.z == v.z ? (double)(v.y * (v.x == M ? 1.0f : sr::ex2(v.x - M))) : NAN;
-    }
-    L = block_sum<TH>(L, part);
+    // ---- maxima: of the pass's references, of the logits, of the named scores ----
+    float mx[3] = {M, -INFINITY, -INFINITY};
+    for (int e = tid; e < p.t.k; e += TH)
+        if (row[e] >= 0) mx[1] = fmaxf(mx[1], z[e]), mx[2] = fmaxf(mx[2], (float)score[e]);
+    block_maxima<TH>(mx, &maxima[0][0]);
+    const float zm = mx[1];
+    const double tm = mx[2];
+    // ---- sums relative to them ----
+    double sum[3] = {L == 0.0 ? 0.0 : L * (double)(M == mx[0] ? 1.0f : sr::ex2(M - mx[0])), 0.0, 0.0};
+    for (int e = tid; e < p.t.k; e += TH)
+        if (row[e] >= 0) {
+            sum[1] += above(p.t, z[e], zm);
+            sum[2] += fabs(score[e]) < INFINITY ? exp(score[e] - tm) : NAN;
+        }
+    block_sums<TH>(sum, &sums[0][0]);
+    L = sum[0];
     const bool bad = !(L == L) || *ps.err != 0;
     // t was formed with f * rf, rounded to f32, from a sum that was cut
     float f = 1.0f;
@@ -225,40 +257,31 @@ __global__ void __launch_bounds__(TH) loss_kernel(const LossArgs p) {
     const double unit = (double)p.scale * LOG2E;
     const float rf = f * (float)unit;
     const bool others = !p.t.rest || L > 0.0;
-    double lse = bad ? NAN : L > 0.0 ? LN2 * (double)M * ((double)f * unit / (double)rf * ps.whole) + log(L)
-                                     : -INFINITY;
-    const double rest_lse = lse;
-    // ---- with the rest, the named rows were left out ----
-    if (p.t.rest && named > 0) {
-        double t = -INFINITY;
-        for (int i = tid; i < named; i += TH) t = fmax(t, score[list[i]]);
-        t = fmax(block_max<TH>(t, part), rest_lse);
-        double s = 0.0;
-        for (int i = tid; i < named; i += TH) {
-            const double v = score[list[i]];
-            s += fabs(v) < INFINITY ? exp(v - t) : NAN;
-        }
-        s = block_sum<TH>(s, part) + exp(rest_lse - t);
-        lse = t + log(s);
+    const double rest_lse =
+        bad ? NAN : L > 0.0 ? LN2 * (double)mx[0] * ((double)f * unit / (double)rf * ps.whole) + log(L)
+                            : -INFINITY;
+    double lse = rest_lse;
+    if (p.t.rest && named > 0) {  // (the named rows were left out)
+        const double t = fmax(tm, rest_lse);
+        lse = t + log(sum[2] * exp(tm - t) + exp(rest_lse - t));
     }
-    const Norm nm = teacher_norm<TH>(p.t, q, row, others, part);
-    const float* z = p.t.z + (size_t)q * p.t.ld;
-    double loss = 0.0;
+    const Norm nm = teacher_norm(p.t, zm, sum[1], named > 0, others);
+    double loss[1] = {0.0};
     for (int e = tid; e < p.t.k; e += TH) {
         const double lp = row[e] >= 0 ? score[e] - lse : 0.0;
         if (row[e] >= 0) {
             const double lt = p.t.scale * (double)z[e] - nm.norm, w = exp(lt);
-            if (!(w == 0.0)) loss += w * (lt - lp);
+            if (!(w == 0.0)) loss[0] += w * (lt - lp);
         }
         if (p.logprobs) p.logprobs[(size_t)q * p.t.k + e] = (float)(lse == lse ? lp : NAN);
     }
-    loss = block_sum<TH>(loss, part);
+    block_sums<TH>(loss, sums2);
     if (tid != 0) return;
     const double rest = lse == -INFINITY || rest_lse == -INFINITY ? -INFINITY : rest_lse - lse;
-    if (p.t.rest && nm.any && nm.left > 0.0) loss += nm.left * (log(nm.left) - rest);
+    if (p.t.rest && nm.any && nm.left > 0.0) loss[0] += nm.left * (log(nm.left) - rest);
     // (not finite: a query or a row that counts, or a named row with a weight of 0)
-    if (!(lse == lse)) loss = NAN;
-    if (p.loss) p.loss[q] = (float)loss;
+    if (!(lse == lse)) loss[0] = NAN;
+    if (p.loss) p.loss[q] = (float)loss[0];
     if (p.lse) p.lse[q] = (float)lse;
     if (p.rest) p.rest[q] = (float)rest;
 }
@@ -276,16 +299,27 @@ struct CoefArgs {
 // One block per query: what the score gradients are formed with.
 __global__ void __launch_bounds__(128) grad_kernel(const CoefArgs p) {
     __shared__ int raw[MAXK], row[MAXK];
-    __shared__ double part[4];
+    __shared__ double sums[4];
+    __shared__ float maxima[4];
     const int tid = threadIdx.x, q = blockIdx.x;
+    const float lse = p.lse[q], rest = p.t.rest ? p.rest[q] : 0.0f, up = p.d_loss[q];
     read_entries<128>(p.t, q, raw, row);
-    const float lse = p.lse[q], rest = p.t.rest ? p.rest[q] : 0.0f;
     const bool others = rest > -INFINITY || !(rest == rest);
-    const Norm nm = teacher_norm<128>(p.t, q, row, others, part);
-    const bool live = nm.any && lse != -INFINITY;
-    const double u = live ? (double)p.d_loss[q] : 0.0;
-    const size_t at = (size_t)q * p.t.k;
     const float* z = p.t.z + (size_t)q * p.t.ld;
+    float zm[1] = {-INFINITY};
+    bool mine = false;
+    for (int e = tid; e < p.t.k; e += 128)
+        if (row[e] >= 0) zm[0] = fmaxf(zm[0], z[e]), mine = true;
+    const bool any = __syncthreads_or(mine);
+    block_maxima<128>(zm, maxima);
+    double sum[1] = {0.0};
+    for (int e = tid; e < p.t.k; e += 128)
+        if (row[e] >= 0) sum[0] += above(p.t, z[e], zm[0]);
+    block_sums<128>(sum, sums);
+    const Norm nm = teacher_norm(p.t, zm[0], sum[0], any, others);
+    const bool live = nm.any && lse != -INFINITY;
+    const double u = live ? (double)up : 0.0;
+    const size_t at = (size_t)q * p.t.k;
     for (int e = tid; e < p.t.k; e += 128) {
         p.row[at + e] = live ? row[e] : -1;
         if (row[e] < 0) continue;
@@ -352,11 +386,10 @@ size_t forward_bytes(const Ctx& c, const fdb_distill_args& a) { return plan_forw
 
 template <typename T, int TH>
 static void launch_loss(cudaStream_t s, int device, const LossArgs& p) {
-    const size_t smem = (size_t)p.d * sizeof(typename Exact<T>::Q);
+    const size_t smem = up((size_t)p.d, 4) * 4;
     if (smem > 32768) {  // (with the static part, over what needs no permission)
         static std::atomic<uint64_t> done{0};
-        sr::allow_smem(loss_kernel<T, TH>, device,
-                       FDB_MAX_SOFTMAX_DIM * sizeof(typename Exact<T>::Q), done);
+        sr::allow_smem(loss_kernel<T, TH>, device, FDB_MAX_SOFTMAX_DIM * 4, done);
     }
     loss_kernel<T, TH><<<p.parts.nq, TH, smem, s>>>(p);
     FDB_LAUNCH_CHECK();

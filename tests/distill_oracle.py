@@ -66,14 +66,17 @@ def forward(q, x, ids, z, scale, tscale, rest, allowed):
 
 
 def forward_bounds(o, es):
-    """lse: as the log-softmax's (es the scores' bound).  An entry's score is taken
-    in 64 bits, so its log probability is off as the lse is; log r is the
-    difference of two such sums, the loss lse - R lse_rest and what is exact;
-    each rounded once."""
+    """lse: as the log-softmax's (es the scores' bound).  An entry's score is a sum in
+    64 bits of sums in f32 of up to 8 products, each off by half a step and added in
+    three levels: 4 * 2^-24 of the products' sizes, less than es, which counts 2^-22
+    and more of them.  Its log probability is off by that and as the lse is; log r
+    is the difference of two such sums, the loss lse - R lse_rest and the mean of the
+    named scores; each rounded once."""
     e = so.forward_bounds(o["f"], es)[0]
+    named = np.where(o["keep"], es, 0.0).max(1)
     fin = lambda v: np.where(np.isfinite(v), np.abs(v), 0.0)  # noqa: E731
-    return dict(lse=e, logprobs=e[:, None] + H32 * fin(o["logprobs"]),
-                rest=2 * e + H32 * fin(o["rest"]), loss=2 * e + H32 * fin(o["loss"]))
+    return dict(lse=e, logprobs=(e + named)[:, None] + H32 * fin(o["logprobs"]),
+                rest=2 * e + H32 * fin(o["rest"]), loss=2 * e + named + H32 * fin(o["loss"]))
 
 
 def backward(q, x, o, ids, lse, logprobs, rest, d_loss, scale):
