@@ -1443,11 +1443,20 @@ int fdb_beam_reorder(fdb_ctx* ctx, const fdb_beam_state* states, size_t count,
             const fdb_beam_state& t = states[i];
             if (t.bytes == 0 || t.parts == 0) continue;
             FDB_REQUIRE(t.src && t.dst, FDB_ERR_INVALID_ARG, "NULL state");
-            FDB_REQUIRE(t.bytes < (1ull << 40) && t.parts < (1ull << 31) &&
-                            t.dst_stride < (1ull << 44) && t.src_stride < (1ull << 44),
+            FDB_REQUIRE(t.bytes < (1ull << 40) && t.parts < (1ull << 24) &&
+                            t.dst_stride < (1ull << 40) && t.src_stride < (1ull << 40) &&
+                            t.dst_part_stride < (1ull << 40) && t.src_part_stride < (1ull << 40) &&
+                            t.parts * t.dst_part_stride < (1ull << 44),
                         FDB_ERR_INVALID_ARG, "a state is too large");
-            FDB_REQUIRE(t.parts == 1 || t.dst_part_stride >= t.bytes, FDB_ERR_DIM_MISMATCH,
-                        "a state's runs overlap");
+            // rows beside each other, or (all rows' first runs, then all rows' second ones)
+            // runs of all rows beside each other
+            const size_t rows = o.groups * o.width;
+            const bool apart =
+                (t.parts == 1 || t.dst_part_stride >= t.bytes) &&
+                (rows <= 1 || t.dst_stride >= (t.parts - 1) * t.dst_part_stride + t.bytes ||
+                 (t.dst_stride >= t.bytes &&
+                  t.dst_part_stride >= (rows - 1) * t.dst_stride + t.bytes));
+            FDB_REQUIRE(apart, FDB_ERR_DIM_MISMATCH, "a state's runs overlap");
             FDB_REQUIRE(t.src != t.dst ||
                             (o.width == o.beams && t.src_stride == t.dst_stride &&
                              (t.parts == 1 || t.src_part_stride == t.dst_part_stride)),

@@ -2478,6 +2478,7 @@ struct FewGrad {
     size_t ld_dx;
     float* partial;  // [blocks][nq][d], nullable
     int* err;
+    GivenRows given;
 };
 constexpr int FEW_ROWS = 16;
 constexpr int few_per_sm(int NQ) { return NQ <= 2 ? 3 : 2; }  // (blocks; registers)
@@ -2491,7 +2492,9 @@ static size_t few_grad_smem(int NQ, size_t d, size_t elem) {
 __device__ __forceinline__ int few_at(int c) {
     return (c & ~63) + 2 * (c & 31) + (c >> 5 & 1);
 }
-template <typename T, int NQ>
+// GIVEN: with score gradients at given rows.  Each thread looks after up to NQ of
+// them (at most 256 a query) and lays those of the block's rows over the others.
+template <typename T, int NQ, bool GIVEN>
 __global__ void __launch_bounds__(256, few_per_sm(NQ)) few_grad_kernel(const FewGrad<T> p) {
     extern __shared__ float4 few_raw[];
     const int d = p.d, ct_n = (d + 3) / 4, dp = (d + 63) & ~63;
@@ -2533,6 +2536,12 @@ __global__ void __launch_bounds__(256, few_per_sm(NQ)) few_grad_kernel(const Few
                              c + ct_n < d ? o[few_at(c + ct_n)] : 0.0f);
             acc[j][h] = 0ull;
         }
+    int given[GIVEN ? NQ : 1];
+#pragma unroll
+    for (int e = 0; e < (GIVEN ? NQ : 0); ++e) {
+        const int i = e * 256 + tid;
+        given[e] = i < p.nq * p.given.k ? p.given.row[i] : -1;
+    }
     // (unsigned: the last step may pass 2^31)
     for (unsigned u0 = blockIdx.x * FEW_ROWS; u0 < (unsigned)p.n; u0 += gridDim.x * FEW_ROWS) {
         const int r0 = (int)u0;
@@ -2609,7 +2618,23 @@ __global__ void __launch_bounds__(256, few_per_sm(NQ)) few_grad_kernel(const Few
             }
             gs[r * NQ + j] = make_float2(g, g);
         }
-        __syncthreads();
+        if (GIVEN) {
+            bool here = false;
+#pragma unroll
+            for (int e = 0; e < NQ; ++e) here |= (unsigned)(given[e] - r0) < (unsigned)FEW_ROWS;
+            if (__syncthreads_or(here)) {
+#pragma unroll
+                for (int e = 0; e < NQ; ++e)
+                    if ((unsigned)(given[e] - r0) < (unsigned)FEW_ROWS) {
+                        const int i = e * 256 + tid;
+                        const float g = p.given.g[i];
+                        gs[(given[e] - r0) * NQ + i / p.given.k] = make_float2(g, g);
+                    }
+                __syncthreads();
+            }
+        } else {
+            __syncthreads();
+        }
         if (rg < groups) {
 #pragma unroll (NQ > 4 ? 1 : 2)
             for (int r = rg; r < FEW_ROWS; r += groups) {
@@ -3113,7 +3138,7 @@ struct Backward {
 static Backward plan_backward(const Ctx& c, const fdb_logprob_grad_args& a, const GivenRows* given) {
     Backward w{};
     Carve ws(a.workspace);
-    w.few = !given && a.nq <= FEW_GRAD && a.dim <= FEW_GRAD_DIM;
+    w.few = a.nq <= FEW_GRAD && a.dim <= FEW_GRAD_DIM;
     if (w.few) {
         w.err = ws.take<int>(HEAD / 4);
         w.few_blocks = (int)std::min<size_t>((a.n + FEW_ROWS - 1) / FEW_ROWS,
@@ -3163,20 +3188,27 @@ size_t backward_bytes(const Ctx& c, const fdb_logprob_grad_args& a, const GivenR
     return plan_backward(c, b, given).bytes;
 }
 
-template <typename T, int NQ>
+template <typename T, int NQ, bool GIVEN>
 static void launch_few_grad(const Ctx& c, const Backward& w, const FewGrad<T>& p, cudaStream_t s) {
     const size_t smem = few_grad_smem(NQ, p.d, sizeof(T));
     if (smem > 40960) {  // (see allow_smem)
         static std::atomic<uint64_t> done{0};
-        allow_smem(few_grad_kernel<T, NQ>, c.device, few_grad_smem(NQ, FEW_GRAD_DIM, sizeof(T)),
-                   done);
+        allow_smem(few_grad_kernel<T, NQ, GIVEN>, c.device,
+                   few_grad_smem(NQ, FEW_GRAD_DIM, sizeof(T)), done);
     }
-    few_grad_kernel<T, NQ><<<w.few_blocks, 256, smem, s>>>(p);
+    few_grad_kernel<T, NQ, GIVEN><<<w.few_blocks, 256, smem, s>>>(p);
     FDB_LAUNCH_CHECK();
+}
+template <typename T, bool GIVEN>
+static void launch_few_grad(const Ctx& c, const Backward& w, const FewGrad<T>& p, cudaStream_t s) {
+    if (p.nq == 1) launch_few_grad<T, 1, GIVEN>(c, w, p, s);
+    else if (p.nq == 2) launch_few_grad<T, 2, GIVEN>(c, w, p, s);
+    else if (p.nq <= 4) launch_few_grad<T, 4, GIVEN>(c, w, p, s);
+    else launch_few_grad<T, 8, GIVEN>(c, w, p, s);
 }
 template <typename T>
 static void few_backward(const Ctx& c, const fdb_logprob_grad_args& a, const Backward& w,
-                         const CoefArgs& k) {
+                         const CoefArgs& k, const GivenRows* given) {
     const cudaStream_t s = static_cast<cudaStream_t>(a.stream);
     FewGrad<T> p{};
     p.x = static_cast<const T*>(a.rows), p.ldx = a.ld_rows;
@@ -3186,10 +3218,12 @@ static void few_backward(const Ctx& c, const fdb_logprob_grad_args& a, const Bac
     p.dx = static_cast<T*>(a.d_rows), p.ld_dx = a.ld_d_rows;
     p.partial = a.d_queries ? w.dq : nullptr;
     p.err = w.err;
-    if (a.nq == 1) launch_few_grad<T, 1>(c, w, p, s);
-    else if (a.nq == 2) launch_few_grad<T, 2>(c, w, p, s);
-    else if (a.nq <= 4) launch_few_grad<T, 4>(c, w, p, s);
-    else launch_few_grad<T, 8>(c, w, p, s);
+    if (given) {
+        p.given = *given;
+        launch_few_grad<T, true>(c, w, p, s);
+    } else {
+        launch_few_grad<T, false>(c, w, p, s);
+    }
     if (a.d_queries)
         launch_join(s, c.sm_count, w.dq, w.few_blocks, (int)a.nq, (int)a.dim, nullptr, nullptr,
                     a.d_queries, a.ld_d_queries, a.dtype);
@@ -3204,9 +3238,9 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a, const GivenRows* given
         k.lse = a.lse, k.entropy = a.entropy;
         k.d_logprob = a.d_logprob, k.d_lse = a.d_lse, k.d_entropy = a.d_entropy;
         k.targets = a.targets, k.allowed = a.allowed, k.ld_allowed = a.allowed ? a.ld_allowed : 0;
-        if (a.dtype == FDB_DTYPE_F32) few_backward<float>(c, a, w, k);
-        else if (a.dtype == FDB_DTYPE_F16) few_backward<__half>(c, a, w, k);
-        else few_backward<__nv_bfloat16>(c, a, w, k);
+        if (a.dtype == FDB_DTYPE_F32) few_backward<float>(c, a, w, k, given);
+        else if (a.dtype == FDB_DTYPE_F16) few_backward<__half>(c, a, w, k, given);
+        else few_backward<__nv_bfloat16>(c, a, w, k, given);
         return;
     }
     const int n = (int)a.n, d = (int)a.dim, nq = (int)a.nq;

@@ -63,7 +63,7 @@ struct ForwardEnd {
 // Score gradients at given rows, in the place of what backward_run's formula
 // gives there.
 struct GivenRows {
-    int k;
+    int k;                 // at most 256
     const int* row;        // [nq][k], each of a query once, < 0: none
     const float* g;        // [nq][k] dL / ds * scale
     const float* at_least; // [nq] a bound of their sizes over scale, >= 0

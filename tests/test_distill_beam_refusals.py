@@ -133,6 +133,9 @@ def test_reorder_refuses(call):
         assert run(good, **kw) == -1
     assert run((0,) + good[1:]) == -1 and run(good[:1] + (0,) + good[2:]) == -1
     assert run((256, 4096, 64, 64, 2, 16, 16, 64)) == -2          # runs that overlap
+    assert run((256, 4096, 64, 0, 1, 0, 0, 64)) == -2             # rows on top of each other
+    assert run((256, 4096, 64, 48, 1, 0, 0, 64)) == -2
+    assert run((256, 4096, 64, 80, 2, 100, 100, 64)) == -2        # runs between the rows
     assert run((256, 256, 64, 64, 1, 0, 0, 64), width=2) == -1    # in place, another width
     assert run((256, 256, 64, 128, 1, 0, 0, 64)) == -1            # in place, other strides
 

@@ -284,6 +284,26 @@ def test_the_used_part_of_a_cache_moves(dtype, heads, room, used, dim, off, inpl
     assert torch.equal(out, want)
 
 
+def test_states_with_their_heads_outside():
+    """[heads][groups * beams][positions] seen as [groups, beams, heads, positions]: rows lie
+    between each other's heads."""
+    import forgegpu as fg
+    import torch
+    t = torch.randn(5, 6, 40, device="cuda")
+    view = lambda a: a.view(5, 2, 3, 40).permute(1, 2, 0, 3)  # noqa: E731
+    o = torch.empty_like(t)
+    parents = torch.tensor([[2, 2, 0], [1, 0, 2]], device="cuda")
+    want = turned(view(t), parents)
+    fg.beam_reorder([view(t)], parents, out=[view(o)])
+    assert torch.equal(view(o), want)
+    before = t.clone()
+    fg.beam_reorder([view(t)[:, :, :, :7]], parents, out=[view(t)[:, :, :, :7]])
+    assert torch.equal(view(t)[:, :, :, :7], want[:, :, :, :7])
+    assert torch.equal(t[:, :, 7:], before[:, :, 7:])
+    with pytest.raises(fg.ForgeGpuError):
+        fg.beam_reorder([view(t)], parents, out=[o[0, 0].expand(2, 3, 5, 40)])
+
+
 def test_reorder_many_states_on_a_stream_and_captured():
     import forgegpu as fg
     import torch
