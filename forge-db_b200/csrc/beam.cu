@@ -41,10 +41,11 @@ struct Select {
 template <typename T>
 __device__ __forceinline__ double column(const Select& p, int g, int b, int j) {
     const size_t row = (size_t)g * p.beams + b;
-    if (p.ids && p.ids[row * p.ld_ids + j] < 0) return -INFINITY;
-    if (p.allowed && !(p.allowed[row * p.ld_allowed + (j >> 5)] >> (j & 31) & 1u)) return -INFINITY;
-    const T* x = static_cast<const T*>(p.x) + (size_t)g * p.ld_group + (size_t)b * p.ld_beam;
-    return p.scale * (double)to_f32<T>(x[j]);
+    // (all loads first)
+    const float x = to_f32<T>(static_cast<const T*>(p.x)[(size_t)g * p.ld_group + (size_t)b * p.ld_beam + j]);
+    const int64_t id = p.ids ? p.ids[row * p.ld_ids + j] : 0;
+    const uint32_t w = p.allowed ? p.allowed[row * p.ld_allowed + (j >> 5)] : 0xffffffffu;
+    return id < 0 || !(w >> (j & 31) & 1u) ? -INFINITY : p.scale * (double)x;
 }
 __device__ __forceinline__ bool over(const Select& p, int g, int b) {
     return p.ended && p.ended[(size_t)g * p.beams + b];
@@ -86,9 +87,9 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     uint64_t d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
     return d;
 }
 
@@ -107,7 +108,8 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 // is exceeded by 2^8), 32 terms in f32 and those in 64 bits.
 constexpr int TH = 256;               // threads
 constexpr int U = 4;                  // loads of a thread in a tile
-constexpr int TILES = 16;             // of a block
+constexpr int SPAN = 2;               // tiles whose largest is kept together
+constexpr int SPANS = 16;             // of a block
 constexpr int RING = 2;               // tiles on their way
 constexpr int GROUPS = 1024;          // maxima looked behind at once
 constexpr int MAXW = FDB_MAX_BEAMS;
@@ -119,11 +121,16 @@ template <>
 struct Vec<float> {
     static constexpr int N = 4;
     static constexpr uint32_t NONE = 0xff800000u;  // -inf, in every element of a word
-    static __device__ __forceinline__ float max4(const uint4& r, float m) {
-        asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(__uint_as_float(r.x)));
-        asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(__uint_as_float(r.y)));
-        asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(__uint_as_float(r.z)));
-        asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(__uint_as_float(r.w)));
+    // the largest (NaN if one is) of U vectors
+    static __device__ __forceinline__ float most(const uint4 (&r)[U]) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(__uint_as_float(r[u].x)));
+            asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(__uint_as_float(r[u].y)));
+            asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(__uint_as_float(r[u].z)));
+            asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(__uint_as_float(r[u].w)));
+        }
         return m;
     }
     static __device__ __forceinline__ float2 pair(const uint4& r, int i) {
@@ -135,13 +142,15 @@ template <>
 struct Vec<__half> {
     static constexpr int N = 8;
     static constexpr uint32_t NONE = 0xfc00fc00u;
-    static __device__ __forceinline__ float max4(const uint4& r, float m) {
-        const __half2* h = reinterpret_cast<const __half2*>(&r);
-        const __half2 v = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
-        const float2 f = __half22float2(v);
-        asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(f.x));
-        asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(f.y));
-        return m;
+    static __device__ __forceinline__ float most(const uint4 (&r)[U]) {
+        const __half2* h = reinterpret_cast<const __half2*>(r);
+        __half2 m = h[0];
+#pragma unroll
+        for (int i = 1; i < 4 * U; ++i) m = __hmax2_nan(m, h[i]);
+        const float2 f = __half22float2(m);
+        float v;
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(f.x), "f"(f.y));
+        return v;
     }
     static __device__ __forceinline__ float2 pair(const uint4& r, int i) {
         return __half22float2(reinterpret_cast<const __half2*>(&r)[i]);
@@ -151,13 +160,15 @@ template <>
 struct Vec<__nv_bfloat16> {
     static constexpr int N = 8;
     static constexpr uint32_t NONE = 0xff80ff80u;
-    static __device__ __forceinline__ float max4(const uint4& r, float m) {
-        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
-        const __nv_bfloat162 v = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
-        const float2 f = __bfloat1622float2(v);
-        asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(f.x));
-        asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(f.y));
-        return m;
+    static __device__ __forceinline__ float most(const uint4 (&r)[U]) {
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(r);
+        __nv_bfloat162 m = h[0];
+#pragma unroll
+        for (int i = 1; i < 4 * U; ++i) m = __hmax2_nan(m, h[i]);
+        const float2 f = __bfloat1622float2(m);
+        float v;
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(f.x), "f"(f.y));
+        return v;
     }
     static __device__ __forceinline__ float2 pair(const uint4& r, int i) {
         const uint32_t w = reinterpret_cast<const uint32_t*>(&r)[i];
@@ -285,59 +296,55 @@ struct ScanShared {
             int list[GROUPS];
         } e;
     };
-    float top[TILES][TH];
+    float top[SPANS][TH];  // a thread's largest of each span
     float warp_min[TH / 32], warp_m[TH / 32], bound;
     int groups;
     double warp_sum[TH / 32];
 };
-// 16 bytes of which `bytes` are read, the others zero.
-__device__ __forceinline__ void copy_async(void* dst, const void* src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                     (uint32_t)__cvta_generic_to_shared(dst)),
-                 "l"(src), "r"(bytes)
-                 : "memory");
-}
+// What a thread's exponents are relative to: 2^(x s - reference).  Below the range
+// where x s stays finite its terms are 0 (finish_kernel takes such sums again).
+__device__ __forceinline__ float reference(float m, float s) { return fmaxf(m * s, -1e30f); }
 template <typename T, bool NORM, bool GATE>
-__global__ void __launch_bounds__(TH, 4) scan_kernel(const Select p, const Scan c) {
+__device__ __forceinline__ void scan_part(const Select& p, const Scan& c, ScanShared<T>& sh,
+                                          size_t row, int sp, int g, int b) {
     constexpr int N = Vec<T>::N, STEP = TH * U;
-    extern __shared__ uint4 scan_raw[];
-    ScanShared<T>& sh = *reinterpret_cast<ScanShared<T>*>(scan_raw);
     Best& s = sh.e.s;
     uint64_t* buf = sh.e.buf;
     const int tid = threadIdx.x;
-    const size_t row = blockIdx.x / c.splits;
-    const int sp = blockIdx.x % c.splits, g = (int)(row / p.beams), b = (int)(row % p.beams);
-    if (over(p, g, b) || absent(p, g, b)) return;
     const T* x = static_cast<const T*>(p.x) + (size_t)g * p.ld_group + (size_t)b * p.ld_beam;
     const int skip = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
     const long long nv = ((long long)p.n + skip + N - 1) / N;
     const int v0 = (int)(nv * sp / c.splits), v1 = (int)(nv * (sp + 1) / c.splits);
-    const int tiles = (v1 - v0 + STEP - 1) / STEP;
+    const int tiles = (v1 - v0 + STEP - 1) / STEP, spans = (tiles + SPAN - 1) / SPAN;
     if (tid == 0) sh.groups = 0;
 
     // ---- sums, and the largest of each thread's columns of a tile ----
     // Without gates a thread's loads go through its own places of a ring in shared
     // memory, RING tiles ahead; else through registers, one ahead.
-    float m = 0.0f, most = -INFINITY;
+    float m = 0.0f, ref = 0.0f, most = -INFINITY, span = -INFINITY;
     double sum = 0.0;
     bool started = false;
     uint4 next[GATE ? U : 1];
     const uint4* vecs = reinterpret_cast<const uint4*>(x - skip);
+    // (tiles of whole vectors, in the row from end to end)
+    const int whole0 = skip ? 1 : 0, whole1 = min(v1, (int)(((long long)p.n + skip) / N));
+    auto whole = [&](int t) { return v0 + t * STEP >= whole0 && v0 + (t + 1) * STEP <= whole1; };
+    const uint4* mine = vecs + v0 + tid;
+    const uint32_t places = (uint32_t)__cvta_generic_to_shared(&sh.ring[0][0][tid]);
     auto fetch = [&](int t) {
         if (GATE) {
 #pragma unroll
             for (int u = 0; u < U; ++u)
                 next[u * GATE] = load_vec<T, GATE>(p, x, skip, row, v0 + t * STEP + u * TH + tid, v1);
-        } else {
+        } else if (whole(t)) {
+            const uint4* src = mine + t * STEP;
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int v = v0 + t * STEP + u * TH + tid;
-                // (a first vector that starts in front of the row is read by itself)
-                int left = v < v1 && (v > 0 || skip == 0) ? p.n - (v * N - skip) : 0;
-                left = min(left, N) * (int)sizeof(T);
-                copy_async(&sh.ring[t % RING][u][tid], vecs + (left ? v : 0), left);
-            }
-        }
+            for (int u = 0; u < U; ++u)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                                 places + (uint32_t)((t % RING * U + u) * TH * 16)),
+                             "l"(src + u * TH)
+                             : "memory");
+        }  // (others are read when it is their turn)
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
@@ -353,39 +360,40 @@ __global__ void __launch_bounds__(TH, 4) scan_kernel(const Select p, const Scan 
             if (t + 1 < tiles) fetch(t + 1);
         } else {
             asm volatile("cp.async.wait_group %0;" ::"n"(RING - 1) : "memory");
+            if (whole(t)) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) r[u] = sh.ring[t % RING][u][tid];
+                for (int u = 0; u < U; ++u) r[u] = sh.ring[t % RING][u][tid];
+            } else {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    r[u] = load_vec<T, false>(p, x, skip, row, v0 + t * STEP + u * TH + tid, v1);
+            }
             if (t + RING < tiles) fetch(t + RING);
             else asm volatile("cp.async.commit_group;" ::: "memory");
-            const int at = v0 + t * STEP;
-            if ((at == 0 && skip) || (long long)(at + STEP) * N - skip > p.n || at + STEP > v1) {
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int v = at + u * TH + tid, j0 = v * N - skip;
-                    if (v >= v1 || j0 < 0 || j0 > p.n - N)
-                        r[u] = load_vec<T, false>(p, x, skip, row, v, v1);
-                }
-            }
         }
-        float top = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < U; ++u) top = Vec<T>::max4(r[u], top);
-        sh.top[t][tid] = top;
-        asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(top));
+        const float top = Vec<T>::most(r);
+        if (t % SPAN) asm("max.NaN.f32 %0, %0, %1;" : "+f"(span) : "f"(top));
+        else span = top;
+        if (t % SPAN == SPAN - 1 || t + 1 == tiles) {
+            sh.top[t / SPAN][tid] = span;
+            asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(span));
+        }
         if (NORM) {
             if (top > -INFINITY && (!started || (top - m) * c.s > RAISE)) {
-                if (started) sum *= (double)sr::ex2((m - top) * c.s);
+                const float to = reference(top, c.s);
+                if (started) sum *= (double)sr::ex2(ref - to);
                 m = top;
+                ref = to;
                 started = true;
             }
-            const uint64_t m2 = pack2(-m, -m), s2 = pack2(c.s, c.s);
+            const uint64_t c2 = pack2(-ref, -ref), s2 = pack2(c.s, c.s);
             uint64_t acc[2] = {0, 0};
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int i = 0; i < N / 2; ++i) {
                     const float2 f = Vec<T>::pair(r[u], i);
-                    const uint64_t t2 = mul2(add2(pack2(f.x, f.y), m2), s2);
+                    const uint64_t t2 = fma2(pack2(f.x, f.y), s2, c2);
                     float t0, t1;
                     unpack2(t2, t0, t1);
                     acc[i & 1] = add2(acc[i & 1], pack2(sr::ex2(t0), sr::ex2(t1)));
@@ -430,7 +438,10 @@ __global__ void __launch_bounds__(TH, 4) scan_kernel(const Select p, const Scan 
     if (NORM) {
 #pragma unroll
         for (int i = 0; i < TH / 32; ++i) M = fmaxf(M, sh.warp_m[i]);
-        sum = started && M < INFINITY ? sum * (double)sr::ex2((m - M) * c.s) : 0.0;
+        // (what rounding the reference moved, and the distance of the block's)
+        if (sum > 0.0)
+            sum *= (double)sr::ex2((float)((double)ref - (double)m * c.s)) *
+                   (double)sr::ex2((m - M) * c.s);
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if ((tid & 31) == 0) sh.warp_sum[tid >> 5] = sum;
@@ -441,7 +452,7 @@ __global__ void __launch_bounds__(TH, 4) scan_kernel(const Select p, const Scan 
         return;
     }
     if (most > -INFINITY && most >= tau) {
-        for (int t = 0; t < tiles; ++t) {
+        for (int t = 0; t < spans; ++t) {
             const float top = sh.top[t][tid];
             if (top > -INFINITY && top >= tau) {
                 const int to = atomicAdd(&sh.groups, 1);
@@ -467,27 +478,28 @@ __global__ void __launch_bounds__(TH, 4) scan_kernel(const Select p, const Scan 
     constexpr int ROOM = LIMIT + TH * N;
     bool all = groups > GROUPS;
     if (!all) {
-        for (int k = tid; k < groups * U; k += TH) {
-            const int e = sh.e.list[k / U], at = v0 + e / TH * STEP + k % U * TH + e % TH;
+        for (int k = tid; k < groups * (SPAN * U); k += TH) {
+            const int e = sh.e.list[k / (SPAN * U)];
+            const int at = v0 + (e / TH * (SPAN * U) + k % (SPAN * U)) * TH + e % TH;
             enter(load_vec<T, GATE>(p, x, skip, row, at, v1), at * N - skip, true, ROOM);
         }
         __syncthreads();
         all = s.count > ROOM;
     }
     if (all) {
-        // too many columns are as good: tile by tile, the best kept at any time.  (A
+        // too many columns are as good: span by span, the best kept at any time.  (A
         // column that equals the width-th and lies further on is not better.)
         __syncthreads();
         if (tid == 0) s.count = 0;
         __syncthreads();
         bool reach = true;
-        for (int t = 0; t < tiles; ++t) {
+        for (int t = 0; t < spans; ++t) {
             const float top = sh.top[t][tid];
             const bool hit = top > -INFINITY && (reach ? top >= tau : top > tau);
             if (!__syncthreads_or(hit)) continue;
 #pragma unroll 1
-            for (int u = 0; u < U; ++u) {
-                const int at = v0 + t * STEP + u * TH + tid;
+            for (int u = 0; u < SPAN * U; ++u) {
+                const int at = v0 + (t * (SPAN * U) + u) * TH + tid;
                 if (hit) enter(load_vec<T, GATE>(p, x, skip, row, at, v1), at * N - skip, reach, ROOM);
                 __syncthreads();
                 const bool full = s.count >= LIMIT;
@@ -561,6 +573,21 @@ __device__ __forceinline__ float set_bound(Choice& s, float v, int n, int width)
     __syncthreads();
     return s.bound;
 }
+// Of the candidates that the threads hold (-inf: none; the first threads all of `held`)
+// those not `slack` below the width-th are added.
+constexpr int HELD = 4;
+template <int H>
+__device__ __forceinline__ void pick(Choice& s, const double (&v)[H], const int (&b)[H],
+                                     const int (&j)[H], int held, int width, double slack) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int h = 0; h < H; ++h) m = fmaxf(m, __double2float_rd(v[h]));
+    const double least = (double)set_bound(s, m, min(held, TH), width) - slack;
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+        if (v[h] > -INFINITY && v[h] >= least) add(s, v[h], b[h], j[h]);
+    __syncthreads();
+}
 // The candidates whose scores are not `slack` below the width-th, those in front
 // ranked into out_*.  Returns them: [0, n) of `score` and `at`.  Called by all
 // threads, after a barrier.
@@ -615,42 +642,74 @@ __device__ __forceinline__ void write_out(const Select& p, int g, const Choice& 
     }
 }
 
-// One block per search.  The chains' normalisers are sums of f32 exponentials, off by
-// up to `slack` / 2: where that leaves open which of two chains' columns is the better,
-// among the chosen or at their end, the chains' sums are taken again in 64 bits.
+// One block per search.  The chains' normalisers are sums of f32 exponentials, off by up to `slack` / 2: where that leaves open which of two chains'
+// columns is the better, among the chosen or at their end, the chains' sums are taken
+// again in 64 bits.
+struct FinishShared {
+    Choice s;
+    double sum[MAXW], lse[MAXW], part[TH / 32];
+    float top[MAXW];
+    unsigned char kind[MAXW], close[MAXW], sure[MAXW];
+};
 template <typename T, bool NORM>
-__global__ void __launch_bounds__(TH) finish_kernel(const Select p, const Scan c) {
-    __shared__ Choice s;
-    __shared__ double sum[MAXW], lse[MAXW];
-    __shared__ float top[MAXW];
-    __shared__ unsigned char kind[MAXW], close[MAXW], sure[MAXW];
-    __shared__ double part[TH / 32];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = blockIdx.x, S = c.splits;
+__device__ __forceinline__ void finish_search(const Select& p, const Scan& c, FinishShared& f, int g) {
+    Choice& s = f.s;
+    double *sum = f.sum, *lse = f.lse, *part = f.part;
+    float* top = f.top;
+    unsigned char *kind = f.kind, *close = f.close, *sure = f.sure;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, S = c.splits;
     const size_t row0 = (size_t)g * p.beams;
+    // ---- the lists, if a thread can hold its share of them: on their way while the
+    // chains are looked at (what a chain without columns left is not used) ----
+    const int lists = p.beams * S;
+    const bool held = lists * p.width <= TH * HELD;
+    uint64_t key[HELD];
+    int count[HELD];
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+        const int k = h * TH + tid;
+        key[h] = 0, count[h] = 0;
+        if (held && k < lists * p.width) {
+            key[h] = c.best[row0 * S * p.width + k];
+            count[h] = c.part[row0 * S + k / p.width].count;
+        }
+    }
     // ---- the chains: a warp each ----
-    bool bad = false;
+    bool bad = false, again = false;
     for (int b = warp; b < p.beams; b += TH / 32) {
         const float given = p.beam_scores[row0 + b];
+        const Part mine = c.part[(row0 + b) * S + min(lane, S - 1)];
         const int k = over(p, g, b) ? OVER : LIVE;
         bad |= !(given < INFINITY);
         double L = 0.0;
         float M = -INFINITY;
         const bool live = k == LIVE && given > -INFINITY;
+        bool lost = false;  // (columns, but a sum of 0)
         if (live) {
             for (int i = lane; i < S; i += 32) {
-                const Part q = c.part[(row0 + b) * S + i];
+                const Part q = i < 32 ? mine : c.part[(row0 + b) * S + i];
                 bad |= q.count < 0;
                 if (NORM && q.sum > 0.0) M = fmaxf(M, q.m);
+                lost |= q.count > 0;
             }
             if (NORM) {
 #pragma unroll
                 for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
                 for (int i = lane; i < S; i += 32) {
-                    const Part q = c.part[(row0 + b) * S + i];
+                    const Part q = i < 32 ? mine : c.part[(row0 + b) * S + i];
                     if (q.sum > 0.0) L += q.sum * exp(((double)q.m - (double)M) * p.scale);
                 }
 #pragma unroll
                 for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+                lost = __any_sync(0xffffffffu, lost) && !(L > 0.0);
+                if (lost) {  // (scores out of f32's range: relative to their largest, in 64 bits)
+                    for (int i = lane; i < S; i += 32)
+                        if (c.part[(row0 + b) * S + i].count > 0)
+                            M = fmaxf(M, unordered((uint32_t)(c.best[((row0 + b) * S + i) * p.width] >> 32)));
+#pragma unroll
+                    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+                    again = true;
+                }
             }
         }
         if (lane == 0) {
@@ -658,86 +717,30 @@ __global__ void __launch_bounds__(TH) finish_kernel(const Select p, const Scan c
             kind[b] = given == -INFINITY ? ABSENT : k;
             lse[b] = L > 0.0 ? (double)M * p.scale + log(L) : 0.0;
             top[b] = M;
-            close[b] = sure[b] = 0;
+            close[b] = NORM && lost;
+            sure[b] = 0;
         }
     }
     if (__syncthreads_or(bad)) return write_out(p, g, s, true);
 
     // candidate `rank` of list i = chain * splits + part; whether there is one
-    const int lists = p.beams * S;
-    auto candidate = [&](int i, int rank, double& v, int& b, int& j) -> bool {
+    // (`key` and `count`: as loaded)
+    auto worth = [&](int i, int rank, uint64_t key, int count, double& v, int& b, int& j) -> bool {
         b = i / S;
         j = 0;
         v = sum[b];
         if (kind[b] != LIVE) return kind[b] == OVER && rank == 0 && i == b * S;
-        if (rank >= c.part[row0 * S + i].count) return false;
-        const uint64_t key = c.best[(row0 * S + i) * p.width + rank];
+        if (rank >= count) return false;
         j = (int)~(uint32_t)key;
         v += (double)unordered((uint32_t)(key >> 32)) * p.scale - lse[b];
         return true;
     };
-    const double slack = NORM && p.beams > 1 ? (double)c.slack : 0.0;
-    for (;;) {
-        // ---- what the width-th is not below: the width-th of TH candidates, as many of
-        // each list in front as there is room for (or of the maxima of TH sets of lists) ----
-        float m = -INFINITY;
-        const int each = max(1, min(TH / lists, p.width));
-        for (int k = tid; k < lists * each; k += TH) {
-            double v;
-            int b, j;
-            if (candidate(k / each, k % each, v, b, j)) m = fmaxf(m, __double2float_rd(v));
-        }
-        if (tid == 0) s.count = 0;
-        double least = (double)set_bound(s, m, min(lists * each, TH), p.width) - slack;
-        bool dropped = false;
-        // ---- the lists, so many ranks at a time, until none reaches it ----
-        const int some = min(lists, ROUND), ranks = max(1, ROUND / some);
-        for (int r0 = 0; r0 < p.width; r0 += ranks) {
-            bool any = false;
-            for (int l0 = 0; l0 < lists; l0 += some) {
-#pragma unroll 4
-                for (int k = tid; k < some * ranks; k += TH) {
-                    const int i = l0 + k / ranks, rank = r0 + k % ranks;
-                    double v;
-                    int b, j;
-                    if (i < lists && rank < p.width && candidate(i, rank, v, b, j) && v >= least)
-                        add(s, v, b, j), any = true;
-                }
-                __syncthreads();
-                if (s.count > CAP - ROUND) {  // (what is just behind the width-th is dropped)
-                    rank_all(s, p.width, 0.0);
-                    for (int w = tid; w < s.have; w += TH)
-                        s.score[w] = ordered64(s.out_score[w]), s.at[w] = s.out_at[w];
-                    if (tid == 0) s.count = s.have;
-                    if (s.have == p.width) least = s.out_score[p.width - 1] - slack;
-                    dropped = true;
-                }
-                __syncthreads();
-            }
-            if (!__syncthreads_or(any)) break;
-        }
-        const Ranked r = rank_all(s, p.width, slack);
-        if (slack == 0.0) break;
-        // ---- is their order sure? ----
-        const int have = s.have;
-        for (int w = tid; w + 1 < have; w += TH) {
-            const int a = (int)(s.out_at[w] >> 32), b = (int)(s.out_at[w + 1] >> 32);
-            if (a != b && s.out_score[w] - s.out_score[w + 1] <= slack) close[a] = close[b] = 1;
-        }
-        if (have == p.width) {
-            const double last = s.out_score[have - 1];
-            const uint64_t last_at = s.out_at[have - 1];
-            const int a = (int)(last_at >> 32);
-            for (int i = tid; i < r.n; i += TH) {
-                const double v = unordered64(r.score[i]);
-                const int b = (int)(r.at[i] >> 32);
-                const bool behind = v < last || (v == last && r.at[i] > last_at);
-                if (behind && b != a && last - v <= slack) close[a] = close[b] = 1;
-            }
-        }
-        if (dropped)
-            for (int b = tid; b < p.beams; b += TH) close[b] = 1;
-        __syncthreads();
+    auto candidate = [&](int i, int rank, double& v, int& b, int& j) -> bool {
+        return worth(i, rank, c.best[(row0 * S + i) * p.width + rank], c.part[row0 * S + i].count, v,
+                     b, j);
+    };
+    // the sums of the chains marked, unless they have been taken already; whether one was
+    auto sums_again = [&]() -> bool {
         bool more = false;
         for (int b = 0; b < p.beams; ++b) {
             if (!close[b] || sure[b] || kind[b] != LIVE) continue;
@@ -767,32 +770,118 @@ __global__ void __launch_bounds__(TH) finish_kernel(const Select p, const Scan c
             }
             __syncthreads();
         }
-        if (!more) break;
         for (int b = tid; b < p.beams; b += TH) sure[b] |= close[b];
         __syncthreads();
+        return more;
+    };
+    if (__syncthreads_or(again)) sums_again();
+    const double slack = NORM && p.beams > 1 ? (double)c.slack : 0.0;
+    for (;;) {
+        if (tid == 0) s.count = 0;
+        bool dropped = false;
+        if (held) {
+            double v[HELD];
+            int b[HELD], col[HELD];
+#pragma unroll
+            for (int h = 0; h < HELD; ++h) {
+                const int k = h * TH + tid, i = k / p.width;
+                if (i >= lists || !worth(i, k - i * p.width, key[h], count[h], v[h], b[h], col[h]))
+                    v[h] = -INFINITY;
+            }
+            pick(s, v, b, col, lists * p.width, p.width, slack);
+        } else {
+            // ---- what the width-th is not below: the width-th of TH candidates, as many
+            // of each list in front as there is room for (or of the maxima of TH sets) ----
+            float m = -INFINITY;
+            const int each = max(1, min(TH / lists, p.width));
+            for (int k = tid; k < lists * each; k += TH) {
+                double v;
+                int b, j;
+                if (candidate(k / each, k % each, v, b, j)) m = fmaxf(m, __double2float_rd(v));
+            }
+            double least = (double)set_bound(s, m, min(lists * each, TH), p.width) - slack;
+            // ---- the lists, so many ranks at a time, until none reaches it ----
+            const int some = min(lists, ROUND), ranks = max(1, ROUND / some);
+            for (int r0 = 0; r0 < p.width; r0 += ranks) {
+                bool any = false;
+                for (int l0 = 0; l0 < lists; l0 += some) {
+    #pragma unroll 4
+                    for (int k = tid; k < some * ranks; k += TH) {
+                        const int i = l0 + k / ranks, rank = r0 + k % ranks;
+                        double v;
+                        int b, j;
+                        if (i < lists && rank < p.width && candidate(i, rank, v, b, j) && v >= least)
+                            add(s, v, b, j), any = true;
+                    }
+                    __syncthreads();
+                    if (s.count > CAP - ROUND) {  // (what is just behind the width-th is dropped)
+                        rank_all(s, p.width, 0.0);
+                        for (int w = tid; w < s.have; w += TH)
+                            s.score[w] = ordered64(s.out_score[w]), s.at[w] = s.out_at[w];
+                        if (tid == 0) s.count = s.have;
+                        if (s.have == p.width) least = s.out_score[p.width - 1] - slack;
+                        dropped = true;
+                    }
+                    __syncthreads();
+                }
+                if (!__syncthreads_or(any)) break;
+            }
+        }
+        const Ranked r = rank_all(s, p.width, slack);
+        if (slack == 0.0) break;
+        // ---- is their order sure? ----
+        const int have = s.have;
+        for (int w = tid; w + 1 < have; w += TH) {
+            const int a = (int)(s.out_at[w] >> 32), b = (int)(s.out_at[w + 1] >> 32);
+            if (a != b && s.out_score[w] - s.out_score[w + 1] <= slack) close[a] = close[b] = 1;
+        }
+        if (have == p.width) {
+            const double last = s.out_score[have - 1];
+            const uint64_t last_at = s.out_at[have - 1];
+            const int a = (int)(last_at >> 32);
+            for (int i = tid; i < r.n; i += TH) {
+                const double v = unordered64(r.score[i]);
+                const int b = (int)(r.at[i] >> 32);
+                const bool behind = v < last || (v == last && r.at[i] > last_at);
+                if (behind && b != a && last - v <= slack) close[a] = close[b] = 1;
+            }
+        }
+        if (dropped)
+            for (int b = tid; b < p.beams; b += TH) close[b] = 1;
+        __syncthreads();
+        if (!sums_again()) break;
     }
     write_out(p, g, s, false);
 }
 
+template <typename T, bool NORM, bool GATE>
+__global__ void __launch_bounds__(TH, 4) scan_kernel(const Select p, const Scan c) {
+    extern __shared__ uint4 scan_raw[];
+    const size_t row = blockIdx.x / c.splits;
+    const int g = (int)(row / p.beams), b = (int)(row % p.beams);
+    if (over(p, g, b) || absent(p, g, b)) return;
+    scan_part<T, NORM, GATE>(p, c, *reinterpret_cast<ScanShared<T>*>(scan_raw), row,
+                             blockIdx.x % c.splits, g, b);
+}
+template <typename T, bool NORM>
+__global__ void __launch_bounds__(TH, 4) finish_kernel(const Select p, const Scan c) {
+    __shared__ FinishShared f;
+    finish_search<T, NORM>(p, c, f, blockIdx.x);
+}
+
 // One block per search whose columns are CAP at most in all: their normalisers in 64
-// bits, a warp per chain, and the best.
+// bits, a warp per chain, and the best, a thread's share of the columns in registers.
 template <typename T>
-__global__ void __launch_bounds__(TH) small_kernel(const Select p) {
+__global__ void __launch_bounds__(TH, 4) small_kernel(const Select p) {
+    constexpr int H = CAP / TH;
     __shared__ Choice s;
+    __shared__ double lse[MAXW];
     const int tid = threadIdx.x, lane = tid & 31, g = blockIdx.x;
+    const size_t row0 = (size_t)g * p.beams;
     if (tid == 0) s.count = 0;
-    __syncthreads();
-    bool bad = false;
-    for (int b = tid >> 5; b < p.beams; b += TH / 32) {
-        const double sum = p.beam_scores[(size_t)g * p.beams + b];
-        bad |= !(sum < INFINITY);
-        if (absent(p, g, b)) continue;
-        if (over(p, g, b)) {
-            if (lane == 0) add(s, sum, b, 0);
-            continue;
-        }
-        double lse = 0.0;
-        if (p.normalise) {
+    if (p.normalise) {
+        for (int b = tid >> 5; b < p.beams; b += TH / 32) {
+            if (absent(p, g, b) || over(p, g, b)) continue;
             double m = -INFINITY, t = 0.0;
             for (int j = lane; j < p.n; j += 32) m = fmax(m, column<T>(p, g, b, j));
 #pragma unroll
@@ -801,16 +890,36 @@ __global__ void __launch_bounds__(TH) small_kernel(const Select p) {
                 for (int j = lane; j < p.n; j += 32) t += exp(column<T>(p, g, b, j) - m);
 #pragma unroll
             for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-            if (m > -INFINITY) lse = m + log(t);
+            if (lane == 0) lse[b] = m > -INFINITY ? m + log(t) : 0.0;
         }
-        for (int j = lane; j < p.n; j += 32) {
-            const double v = column<T>(p, g, b, j);
-            bad |= !(v < INFINITY);
-            if (v > -INFINITY) add(s, sum + (v - lse), b, j);
+        __syncthreads();
+    }
+    bool bad = false;
+    double v[H];
+    int b[H], j[H];
+    const int all = p.beams * p.n;
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+        const int k = h * TH + tid;
+        v[h] = -INFINITY;
+        if (k >= all) continue;
+        b[h] = k / p.n, j[h] = k - b[h] * p.n;
+        const float given = p.beam_scores[row0 + b[h]];
+        const double x = column<T>(p, g, b[h], j[h]);
+        bad |= !(given < INFINITY);
+        if (given == -INFINITY) continue;
+        if (over(p, g, b[h])) {
+            if (j[h] == 0) v[h] = given;
+        } else {
+            bad |= !(x < INFINITY);
+            if (x > -INFINITY) v[h] = (double)given + (p.normalise ? x - lse[b[h]] : x);
         }
     }
     bad = __syncthreads_or(bad);
-    if (!bad) rank_all(s, p.width, 0.0);
+    if (!bad) {
+        pick(s, v, b, j, all, p.width, 0.0);
+        rank_all(s, p.width, 0.0);
+    }
     write_out(p, g, s, bad);
 }
 
@@ -827,9 +936,13 @@ static Plan plan(const Ctx& c, const fdb_beam_args& a) {
     p.small = a.beams * a.n <= CAP;
     if (p.small) return p;
     const size_t rows = a.groups * a.beams, per = a.dtype == FDB_DTYPE_F32 ? 4 : 8;
-    const size_t most = (a.n / per + TH) / TH;  // (a load for every thread)
-    const size_t least = (a.n / per + 2 + TILES * TH * U - 1) / (TILES * TH * U);
-    p.c.splits = (int)std::max(least, std::min(most, ((size_t)c.sm_count * 4 + rows - 1) / rows));
+    // Blocks that are all resident at once (four a multiprocessor), of a tile or more: a
+    // block starts and ends with some 4 us in which it loads nothing (512 chains of 131072
+    // bf16: 29.9 us with a block each, 31.8 with two, 36 with three).
+    const size_t vecs = a.n / per + 2;  // (at most)
+    const size_t most = (vecs + TH * U - 1) / (TH * U);
+    const size_t least = (most + SPANS * SPAN - 1) / (SPANS * SPAN);
+    p.c.splits = (int)std::max(least, std::min(most, std::max<size_t>(1, (size_t)c.sm_count * 4 / rows)));
     Carve ws(a.workspace);
     p.c.part = ws.take<Part>(rows * p.c.splits);
     p.c.best = ws.take<uint64_t>(rows * p.c.splits * a.width);
@@ -841,10 +954,8 @@ size_t select_bytes(const Ctx& c, const fdb_beam_args& a) { return plan(c, a).by
 template <typename T, bool NORM, bool GATE>
 static void launch_scan(cudaStream_t s, int device, unsigned blocks, const Select& p, const Scan& c) {
     constexpr size_t smem = sizeof(ScanShared<T>);
-    if (smem > 48 * 1024) {
-        static std::atomic<uint64_t> done{0};
-        sr::allow_smem(scan_kernel<T, NORM, GATE>, device, smem, done);
-    }
+    static std::atomic<uint64_t> done{0};
+    sr::allow_smem(scan_kernel<T, NORM, GATE>, device, smem, done);
     scan_kernel<T, NORM, GATE><<<blocks, TH, smem, s>>>(p, c);
     FDB_LAUNCH_CHECK();
 }
