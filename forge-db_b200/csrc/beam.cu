@@ -404,6 +404,8 @@ __device__ __forceinline__ void scan_part(const Select& p, const Scan& c, ScanSh
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+    // (finish_kernel's blocks may take their places: they wait for this grid's results)
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // ---- a bound that at least `width` columns reach; the sums ----
     float bound = most, M = started ? m : -INFINITY;
     const int group = p.width <= 8 ? 32 : 16;  // (of threads, for 8 or 16 groups)
@@ -542,8 +544,8 @@ enum { LIVE = 0, OVER = 1, ABSENT = 2 };
 struct Choice {
     uint64_t score[CAP], at[CAP];       // ordered64; chain << 32 | column
     uint64_t near_score[ASIDE], near_at[ASIDE];
-    alignas(16) float set[TH];
-    float bound;
+    float set[TH];
+    uint32_t bound;
     double out_score[MAXW];
     uint64_t out_at[MAXW];
     int count, total, have;
@@ -553,36 +555,30 @@ __device__ __forceinline__ void add(Choice& s, double v, int b, int j) {
     s.score[to] = ordered64(v);
     s.at[to] = (uint64_t)b << 32 | (uint32_t)j;
 }
-// The width-th largest of n values, -inf if there are fewer.
-__device__ __forceinline__ float set_bound(Choice& s, float v, int n, int width) {
+// The width-th largest of s.set[0, n), n <= TH (-inf if there are fewer): the least of
+// those that fewer than `width` are above.  Called by all threads, after a barrier;
+// s.bound is all ones.
+__device__ __forceinline__ float bound_of(Choice& s, int n, int width) {
     const int tid = threadIdx.x;
-    s.set[tid] = v;
-    if (tid == 0) s.bound = -INFINITY;
-    __syncthreads();
-    int above = 0, from = 0;
-    const float4* four = reinterpret_cast<const float4*>(s.set);
+    if (n < width) return -INFINITY;
     if (tid < n) {
-#pragma unroll 4
-        for (int i = 0; i < (n + 3) / 4; ++i) {  // (past n: -inf)
-            const float4 o = four[i];
-            above += (o.x > v) + (o.y > v) + (o.z > v) + (o.w > v);
-            from += (o.x >= v) + (o.y >= v) + (o.z >= v) + (o.w >= v);
-        }
-        if (above < width && width <= from) s.bound = v;  // (equal ones all write the same)
+        const float v = s.set[tid];
+        int above = 0;
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) above += s.set[i] > v;
+        if (above < width) atomicMin(&s.bound, ordered(v));
     }
     __syncthreads();
-    return s.bound;
+    return unordered(s.bound);
 }
-// Of the candidates that the threads hold (-inf: none; the first threads all of `held`)
-// those not `slack` below the width-th are added.
+// Of the candidates that the threads hold (-inf: none) those not `slack` below the
+// width-th of s.set[0, n) are added.
 constexpr int HELD = 4;
 template <int H>
 __device__ __forceinline__ void pick(Choice& s, const double (&v)[H], const int (&b)[H],
-                                     const int (&j)[H], int held, int width, double slack) {
-    float m = -INFINITY;
-#pragma unroll
-    for (int h = 0; h < H; ++h) m = fmaxf(m, __double2float_rd(v[h]));
-    const double least = (double)set_bound(s, m, min(held, TH), width) - slack;
+                                     const int (&j)[H], int n, int width, double slack) {
+    __syncthreads();
+    const double least = (double)bound_of(s, n, width) - slack;
 #pragma unroll
     for (int h = 0; h < H; ++h)
         if (v[h] > -INFINITY && v[h] >= least) add(s, v[h], b[h], j[h]);
@@ -601,8 +597,10 @@ __device__ __forceinline__ Ranked rank_all(Choice& s, int width, double slack) {
     if (r.n > TH) {
         float m = -INFINITY;
         for (int i = tid; i < r.n; i += TH) m = fmaxf(m, __double2float_rd(unordered64(s.score[i])));
-        if (tid == 0) s.total = 0;
-        const uint64_t least = ordered64((double)set_bound(s, m, TH, width) - slack);
+        s.set[tid] = m;
+        if (tid == 0) s.total = 0, s.bound = ~0u;
+        __syncthreads();
+        const uint64_t least = ordered64((double)bound_of(s, TH, width) - slack);
         for (int i = tid; i < r.n; i += TH) {
             if (s.score[i] < least) continue;
             const int to = atomicAdd(&s.total, 1);
@@ -642,7 +640,78 @@ __device__ __forceinline__ void write_out(const Select& p, int g, const Choice& 
     }
 }
 
-// One block per search.  The chains' normalisers are sums of f32 exponentials, off by up to `slack` / 2: where that leaves open which of two chains'
+// 2^t within 2^-46 of itself, t < 1000: the Taylor series of e^(f ln 2), |f| <= 1/2, to
+// f^11 (what is left out: 0.347^12 / 12! = 6e-15).  A third of exp()'s operations, which
+// sums of a whole chain by one block wait for (131072 columns: 50 us).
+__device__ __forceinline__ double exp2_series(double t) {
+    constexpr double L = sr::LN2;
+    constexpr double c2 = L * L / 2, c3 = c2 * L / 3, c4 = c3 * L / 4, c5 = c4 * L / 5, c6 = c5 * L / 6,
+                     c7 = c6 * L / 7, c8 = c7 * L / 8, c9 = c8 * L / 9, c10 = c9 * L / 10,
+                     c11 = c10 * L / 11;
+    if (!(t > -1000.0)) return 0.0;
+    const double n = rint(t), f = t - n;
+    double y = fma(c11, f, c10);
+    y = fma(y, f, c9);
+    y = fma(y, f, c8);
+    y = fma(y, f, c7);
+    y = fma(y, f, c6);
+    y = fma(y, f, c5);
+    y = fma(y, f, c4);
+    y = fma(y, f, c3);
+    y = fma(y, f, c2);
+    y = fma(y, f, L);
+    y = fma(y, f, 1.0);
+    return __hiloint2double(__double2hiint(y) + ((int)n << 20), __double2loint(y));
+}
+// ---- clusters of blocks ----
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address, in the cluster's window, of block `rank`'s copy of `p`.
+__device__ __forceinline__ uint32_t address_in(const void* p, int rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;"
+        : "=r"(r)
+        : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    return r;
+}
+// A block's share of the sum of 2^((x - top) unit) over chain b's columns, in 64 bits;
+// the whole block's, in every thread.
+template <typename T>
+__device__ __forceinline__ double sum_share(const Select& p, int g, int b, float top, int rank,
+                                            int blocks, double* part) {
+    const double unit = p.scale * sr::LOG2E;
+    const T* x = static_cast<const T*>(p.x) + (size_t)g * p.ld_group + (size_t)b * p.ld_beam;
+    const int skip = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+    const int nv = (int)(((long long)p.n + skip + Vec<T>::N - 1) / Vec<T>::N);
+    constexpr int AHEAD = 4;  // (loads in flight: one at a time they are what it waits for)
+    double t = 0.0;
+    for (int v = rank * TH + (int)threadIdx.x; v < nv; v += AHEAD * blocks * TH) {
+        uint4 q[AHEAD];
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a)
+            q[a] = load_vec<T, true>(p, x, skip, (size_t)g * p.beams + b, v + a * blocks * TH, nv);
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a)
+#pragma unroll
+            for (int i = 0; i < Vec<T>::N / 2; ++i) {
+                const float2 f = Vec<T>::pair(q[a], i);
+                t += exp2_series(((double)f.x - (double)top) * unit) +
+                     exp2_series(((double)f.y - (double)top) * unit);
+            }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = t;
+    __syncthreads();
+    t = 0.0;
+    for (int i = 0; i < TH / 32; ++i) t += part[i];
+    return t;
+}
+// One block per search, with others of its cluster to help where sums are taken again.
+// The chains' normalisers are sums of f32 exponentials, off by up to `slack` / 2: where that leaves open which of two chains'
 // columns is the better, among the chosen or at their end, the chains' sums are taken
 // again in 64 bits.
 struct FinishShared {
@@ -650,11 +719,36 @@ struct FinishShared {
     double sum[MAXW], lse[MAXW], part[TH / 32];
     float top[MAXW];
     unsigned char kind[MAXW], close[MAXW], sure[MAXW];
+    double shares[8];  // of the cluster's blocks
+    int task;          // the chain whose sum is taken, -1: no more
+    float task_top;
 };
+// The other blocks of a cluster: shares of sums, as long as the first asks for them.
+template <typename T>
+__device__ __forceinline__ void help_search(const Select& p, FinishShared& f, int g, int rank,
+                                            int blocks) {
+    const uint32_t task_at = address_in(&f.task, 0), top_at = address_in(&f.task_top, 0);
+    const uint32_t share_at = address_in(&f.shares[rank], 0);
+    for (;;) {
+        cluster_sync();
+        int b;
+        float top;
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(b) : "r"(task_at) : "memory");
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(top) : "r"(top_at) : "memory");
+        if (b >= 0) {
+            const double t = sum_share<T>(p, g, b, top, rank, blocks, f.part);
+            if (threadIdx.x == 0)
+                asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(share_at), "d"(t) : "memory");
+        }
+        cluster_sync();
+        if (b < 0) return;
+    }
+}
 template <typename T, bool NORM>
-__device__ __forceinline__ void finish_search(const Select& p, const Scan& c, FinishShared& f, int g) {
+__device__ __forceinline__ void finish_search(const Select& p, const Scan& c, FinishShared& f, int g,
+                                              int blocks) {
     Choice& s = f.s;
-    double *sum = f.sum, *lse = f.lse, *part = f.part;
+    double *sum = f.sum, *lse = f.lse;
     float* top = f.top;
     unsigned char *kind = f.kind, *close = f.close, *sure = f.sure;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, S = c.splits;
@@ -746,26 +840,13 @@ __device__ __forceinline__ void finish_search(const Select& p, const Scan& c, Fi
             if (!close[b] || sure[b] || kind[b] != LIVE) continue;
             more = true;
             if (!(top[b] > -INFINITY)) continue;  // (no columns)
-            double t = 0.0;
-            const T* x = static_cast<const T*>(p.x) + (size_t)g * p.ld_group + (size_t)b * p.ld_beam;
-            const int skip = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-            const int nv = (int)(((long long)p.n + skip + Vec<T>::N - 1) / Vec<T>::N);
-            for (int v = tid; v < nv; v += TH) {
-                const uint4 q = load_vec<T, true>(p, x, skip, row0 + b, v, nv);
-#pragma unroll
-                for (int i = 0; i < Vec<T>::N / 2; ++i) {
-                    const float2 f = Vec<T>::pair(q, i);
-                    t += exp(((double)f.x - (double)top[b]) * p.scale) +
-                         exp(((double)f.y - (double)top[b]) * p.scale);
-                }
-            }
-#pragma unroll
-            for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-            if (lane == 0) part[warp] = t;
-            __syncthreads();
+            if (tid == 0) f.task = b, f.task_top = top[b];
+            if (blocks > 1) cluster_sync();
+            const double mine = sum_share<T>(p, g, b, top[b], 0, blocks, f.part);
+            if (blocks > 1) cluster_sync();
             if (tid == 0) {
-                t = 0.0;
-                for (int i = 0; i < TH / 32; ++i) t += part[i];
+                double t = mine;
+                for (int i = 1; i < blocks; ++i) t += f.shares[i];
                 lse[b] = (double)top[b] * p.scale + log(t);
             }
             __syncthreads();
@@ -777,29 +858,32 @@ __device__ __forceinline__ void finish_search(const Select& p, const Scan& c, Fi
     if (__syncthreads_or(again)) sums_again();
     const double slack = NORM && p.beams > 1 ? (double)c.slack : 0.0;
     for (;;) {
-        if (tid == 0) s.count = 0;
+        // What the width-th is not below: of the first q of each list, which are at least
+        // twice the width, the width-th (of more than TH lists, of the largest of TH sets).
+        const int q = lists > TH ? 1 : max(1, min((2 * p.width + lists - 1) / lists, min(TH / lists, p.width)));
+        if (tid == 0) s.count = 0, s.bound = ~0u;
         bool dropped = false;
         if (held) {
             double v[HELD];
             int b[HELD], col[HELD];
 #pragma unroll
             for (int h = 0; h < HELD; ++h) {
-                const int k = h * TH + tid, i = k / p.width;
-                if (i >= lists || !worth(i, k - i * p.width, key[h], count[h], v[h], b[h], col[h]))
+                const int k = h * TH + tid, i = k / p.width, rank = k - i * p.width;
+                if (i >= lists || !worth(i, rank, key[h], count[h], v[h], b[h], col[h]))
                     v[h] = -INFINITY;
+                if (i < lists && rank < q) s.set[i * q + rank] = __double2float_rd(v[h]);
             }
-            pick(s, v, b, col, lists * p.width, p.width, slack);
+            pick(s, v, b, col, lists * q, p.width, slack);
         } else {
-            // ---- what the width-th is not below: the width-th of TH candidates, as many
-            // of each list in front as there is room for (or of the maxima of TH sets) ----
             float m = -INFINITY;
-            const int each = max(1, min(TH / lists, p.width));
-            for (int k = tid; k < lists * each; k += TH) {
+            for (int k = tid; k < lists * q; k += TH) {
                 double v;
                 int b, j;
-                if (candidate(k / each, k % each, v, b, j)) m = fmaxf(m, __double2float_rd(v));
+                if (candidate(k / q, k % q, v, b, j)) m = fmaxf(m, __double2float_rd(v));
             }
-            double least = (double)set_bound(s, m, min(lists * each, TH), p.width) - slack;
+            s.set[tid] = m;
+            __syncthreads();
+            double least = (double)bound_of(s, min(lists * q, TH), p.width) - slack;
             // ---- the lists, so many ranks at a time, until none reaches it ----
             const int some = min(lists, ROUND), ranks = max(1, ROUND / some);
             for (int r0 = 0; r0 < p.width; r0 += ranks) {
@@ -864,9 +948,18 @@ __global__ void __launch_bounds__(TH, 4) scan_kernel(const Select p, const Scan 
                              blockIdx.x % c.splits, g, b);
 }
 template <typename T, bool NORM>
-__global__ void __launch_bounds__(TH, 4) finish_kernel(const Select p, const Scan c) {
+__global__ void __launch_bounds__(TH, 4) finish_kernel(const Select p, const Scan c, int blocks) {
     __shared__ FinishShared f;
-    finish_search<T, NORM>(p, c, f, blockIdx.x);
+    const int g = blockIdx.x / blocks, rank = blockIdx.x % blocks;  // (a cluster's blocks lie side by side)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (rank > 0) return help_search<T>(p, f, g, rank, blocks);
+    finish_search<T, NORM>(p, c, f, g, blocks);
+    if (blocks > 1) {
+        __syncthreads();
+        if (threadIdx.x == 0) f.task = -1;
+        cluster_sync();
+        cluster_sync();  // (the others have read it)
+    }
 }
 
 // One block per search whose columns are CAP at most in all: their normalisers in 64
@@ -878,7 +971,7 @@ __global__ void __launch_bounds__(TH, 4) small_kernel(const Select p) {
     __shared__ double lse[MAXW];
     const int tid = threadIdx.x, lane = tid & 31, g = blockIdx.x;
     const size_t row0 = (size_t)g * p.beams;
-    if (tid == 0) s.count = 0;
+    if (tid == 0) s.count = 0, s.bound = ~0u;
     if (p.normalise) {
         for (int b = tid >> 5; b < p.beams; b += TH / 32) {
             if (absent(p, g, b) || over(p, g, b)) continue;
@@ -917,7 +1010,11 @@ __global__ void __launch_bounds__(TH, 4) small_kernel(const Select p) {
     }
     bad = __syncthreads_or(bad);
     if (!bad) {
-        pick(s, v, b, j, all, p.width, 0.0);
+        float m = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < H; ++h) m = fmaxf(m, __double2float_rd(v[h]));
+        s.set[tid] = m;
+        pick(s, v, b, j, min(all, TH), p.width, 0.0);
         rank_all(s, p.width, 0.0);
     }
     write_out(p, g, s, bad);
@@ -942,7 +1039,9 @@ static Plan plan(const Ctx& c, const fdb_beam_args& a) {
     const size_t vecs = a.n / per + 2;  // (at most)
     const size_t most = (vecs + TH * U - 1) / (TH * U);
     const size_t least = (most + SPANS * SPAN - 1) / (SPANS * SPAN);
-    p.c.splits = (int)std::max(least, std::min(most, std::max<size_t>(1, (size_t)c.sm_count * 4 / rows)));
+    // (and no more lists than a block of the finish holds in registers, if they would do)
+    const size_t lists = std::max<size_t>(1, TH * HELD / (a.beams * a.width));
+    p.c.splits = (int)std::max(least, std::min({most, lists, std::max<size_t>(1, (size_t)c.sm_count * 4 / rows)}));
     Carve ws(a.workspace);
     p.c.part = ws.take<Part>(rows * p.c.splits);
     p.c.best = ws.take<uint64_t>(rows * p.c.splits * a.width);
@@ -960,13 +1059,24 @@ static void launch_scan(cudaStream_t s, int device, unsigned blocks, const Selec
     FDB_LAUNCH_CHECK();
 }
 template <typename T, bool NORM>
-static void run(int device, const fdb_beam_args& a, const Select& p, const Scan& c) {
+static void run(const Ctx& ctx, const fdb_beam_args& a, const Select& p, const Scan& c) {
     const cudaStream_t s = static_cast<cudaStream_t>(a.stream);
-    const unsigned blocks = (unsigned)(a.groups * a.beams * c.splits);
-    if (a.ids || a.allowed) launch_scan<T, NORM, true>(s, device, blocks, p, c);
-    else launch_scan<T, NORM, false>(s, device, blocks, p, c);
-    finish_kernel<T, NORM><<<(unsigned)a.groups, TH, 0, s>>>(p, c);
-    FDB_LAUNCH_CHECK();
+    const unsigned parts = (unsigned)(a.groups * a.beams * c.splits);
+    if (a.ids || a.allowed) launch_scan<T, NORM, true>(s, ctx.device, parts, p, c);
+    else launch_scan<T, NORM, false>(s, ctx.device, parts, p, c);
+    // Launched while the scan ends; blocks that help, where there is room for them (64 x 8
+    // x 131072, 64 places: a chain's sum again takes 48 us by one block).
+    unsigned blocks = 1;
+    while (NORM && a.beams > 1 && blocks < 8 && a.groups * blocks * 2 <= (size_t)ctx.sm_count * 4) blocks *= 2;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = blocks, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t how{};
+    how.gridDim = dim3((unsigned)a.groups * blocks), how.blockDim = dim3(TH), how.stream = s;
+    how.attrs = attr, how.numAttrs = 2;
+    FDB_CUDA(cudaLaunchKernelEx(&how, finish_kernel<T, NORM>, p, c, (int)blocks));
 }
 template <typename T>
 static void run(const Ctx& ctx, const fdb_beam_args& a, const Select& p) {
@@ -982,8 +1092,8 @@ static void run(const Ctx& ctx, const fdb_beam_args& a, const Select& p) {
     // (8 x 2^-24), and in the exponents, whose mean size under the softmax is at most
     // log2 n, a subtraction, a product and the factor s (2.5 x 2^-24 ln 2 of them).
     l.c.slack = (float)(2.0 * (0x1p-21 + 0x1p-21 + 1.75 * 0x1p-24 * (std::log2((double)a.n) + 1.0)));
-    if (a.normalise) run<T, true>(ctx.device, a, p, l.c);
-    else run<T, false>(ctx.device, a, p, l.c);
+    if (a.normalise) run<T, true>(ctx, a, p, l.c);
+    else run<T, false>(ctx, a, p, l.c);
 }
 void select_run(const Ctx& ctx, const fdb_beam_args& a) {
     Select p{};
