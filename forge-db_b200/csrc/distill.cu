@@ -295,32 +295,38 @@ struct CoefArgs {
     const float *lse, *logprobs, *rest, *d_loss;
     int* row;                         // [nq][k], see GivenRows
     float *g, *at_least, *ref, *c;    // G elsewhere = scale c exp(s - ref)
+    sr::BackwardHead head;
 };
-// One block per query: what the score gradients are formed with.
-__global__ void __launch_bounds__(128) grad_kernel(const CoefArgs p) {
+// One block per query: what the score gradients are formed with.  A chain of short steps;
+// a warp where a list is short enough, as a barrier of one warp costs nothing (2048 lists
+// of 32: 12.0 us with 128 threads).
+template <int TH>
+__global__ void __launch_bounds__(TH) grad_kernel(const CoefArgs p) {
     __shared__ int raw[MAXK], row[MAXK];
-    __shared__ double sums[4];
-    __shared__ float maxima[4];
+    __shared__ double sums[TH / 32];
+    __shared__ float maxima[TH / 32];
     const int tid = threadIdx.x, q = blockIdx.x;
+    if (q == 0)
+        for (int i = tid; i < p.head.words; i += TH) p.head.clear[i] = 0u;
     const float lse = p.lse[q], rest = p.t.rest ? p.rest[q] : 0.0f, up = p.d_loss[q];
-    read_entries<128>(p.t, q, raw, row);
+    read_entries<TH>(p.t, q, raw, row);
     const bool others = rest > -INFINITY || !(rest == rest);
     const float* z = p.t.z + (size_t)q * p.t.ld;
     float zm[1] = {-INFINITY};
     bool mine = false;
-    for (int e = tid; e < p.t.k; e += 128)
+    for (int e = tid; e < p.t.k; e += TH)
         if (row[e] >= 0) zm[0] = fmaxf(zm[0], z[e]), mine = true;
     const bool any = __syncthreads_or(mine);
-    block_maxima<128>(zm, maxima);
+    block_maxima<TH>(zm, maxima);
     double sum[1] = {0.0};
-    for (int e = tid; e < p.t.k; e += 128)
+    for (int e = tid; e < p.t.k; e += TH)
         if (row[e] >= 0) sum[0] += above(p.t, z[e], zm[0]);
-    block_sums<128>(sum, sums);
+    block_sums<TH>(sum, sums);
     const Norm nm = teacher_norm(p.t, zm[0], sum[0], any, others);
     const bool live = nm.any && lse != -INFINITY;
     const double u = live ? (double)up : 0.0;
     const size_t at = (size_t)q * p.t.k;
-    for (int e = tid; e < p.t.k; e += 128) {
+    for (int e = tid; e < p.t.k; e += TH) {
         p.row[at + e] = live ? row[e] : -1;
         if (row[e] < 0) continue;
         const double w = exp(p.t.scale * (double)z[e] - nm.norm);
@@ -328,6 +334,7 @@ __global__ void __launch_bounds__(128) grad_kernel(const CoefArgs p) {
     }
     if (tid != 0) return;
     p.at_least[q] = (float)fabs(u);
+    if (p.head.weight) p.head.weight[q] = sr::weight_of((float)(p.scale * fabs(u)));
     p.ref[q] = others ? (float)((double)lse + (double)rest) : lse;
     double c = u * ((p.t.rest ? exp((double)rest) : 1.0) - nm.left);
     if (live && !(nm.norm == nm.norm)) c = NAN;
@@ -395,10 +402,13 @@ static void launch_loss(cudaStream_t s, int device, const LossArgs& p) {
     FDB_LAUNCH_CHECK();
 }
 template <typename T>
-static void launch_loss(cudaStream_t s, int device, const LossArgs& p) {
-    // (few queries: more threads share the rows of one)
-    if (p.parts.nq <= 296) launch_loss<T, 512>(s, device, p);
-    else launch_loss<T, 128>(s, device, p);
+static void launch_loss(cudaStream_t s, int device, int sms, const LossArgs& p) {
+    // Few queries: more threads share the rows of one.  Many: as few as leave all blocks
+    // resident at once, where a chain of short steps is what a block waits for (2048 lists
+    // of 32 rows of 768 bf16: 37 us with 128 threads, 29 with 64).
+    if (p.parts.nq <= 2 * sms) launch_loss<T, 512>(s, device, p);
+    else if (p.parts.nq <= 8 * sms) launch_loss<T, 128>(s, device, p);
+    else launch_loss<T, 64>(s, device, p);
 }
 
 struct End : sr::ForwardEnd {
@@ -426,9 +436,9 @@ struct End : sr::ForwardEnd {
         p.d = (int)a.dim, p.scale = a.scale;
         p.loss = a.loss, p.lse = a.lse, p.logprobs = a.logprobs;
         p.rest = a.rest ? a.rest_logprob : nullptr;
-        if (a.dtype == FDB_DTYPE_F32) launch_loss<float>(s, c.device, p);
-        else if (a.dtype == FDB_DTYPE_F16) launch_loss<__half>(s, c.device, p);
-        else launch_loss<__nv_bfloat16>(s, c.device, p);
+        if (a.dtype == FDB_DTYPE_F32) launch_loss<float>(s, c.device, c.sm_count, p);
+        else if (a.dtype == FDB_DTYPE_F16) launch_loss<__half>(s, c.device, c.sm_count, p);
+        else launch_loss<__nv_bfloat16>(s, c.device, c.sm_count, p);
     }
 };
 void forward_run(Ctx& c, const fdb_distill_args& a) {
@@ -473,7 +483,10 @@ void backward_run(Ctx& c, const fdb_distill_grad_args& a) {
     k.t = teacher_of(a);
     k.scale = a.scale;
     k.lse = a.lse, k.logprobs = a.logprobs, k.rest = a.rest_logprob, k.d_loss = a.d_loss;
-    grad_kernel<<<(unsigned)a.nq, 128, 0, static_cast<cudaStream_t>(a.stream)>>>(k);
+    k.head = sr::backward_head(c, p.head, p.given);
+    const cudaStream_t s = static_cast<cudaStream_t>(a.stream);
+    if (a.k <= 64) grad_kernel<32><<<(unsigned)a.nq, 32, 0, s>>>(k);
+    else grad_kernel<128><<<(unsigned)a.nq, 128, 0, s>>>(k);
     FDB_LAUNCH_CHECK();
     sr::backward_run(c, p.head, &p.given);
 }

@@ -206,6 +206,7 @@ struct PackSide {
     size_t ld;
     int n;
     const uint32_t* seen;
+    const float* lse;    // nullable: a row whose lse is -inf counts as zeros, too
     __half* out;
     float* f;
     unsigned* largest;   // see most_of, nullable
@@ -216,7 +217,6 @@ struct PackSide {
 };
 // What the largest is taken of: the scales' bits, or, with weights, WEIGHT_ZERO + the
 // exponent of scale times weight; 0 is none.
-constexpr int NO_WEIGHT = -10000;
 constexpr int WEIGHT_ZERO = 1024;
 __device__ __forceinline__ unsigned most_of(const PackSide& p, int row, float f) {
     if (!p.largest || !(f > 0.0f)) return 0u;
@@ -230,7 +230,8 @@ __device__ __forceinline__ unsigned pack_row(const PackSide& p, int row, int d, 
     const int lane = threadIdx.x & 31;
     const T* src = static_cast<const T*>(p.x) + (size_t)row * p.ld;
     __half* dst = p.out + (size_t)row * (size_t)(PARTS * kp);
-    const bool use = !p.seen || (p.seen[row >> 5] >> (row & 31) & 1u);
+    const bool use = (!p.seen || (p.seen[row >> 5] >> (row & 31) & 1u)) &&
+                     (!p.lse || p.lse[row] != -INFINITY);
     const bool held = p.wide && d <= 32 * V * NV;
     const bool pairs = !held && d <= 64 * NP;  // two columns a lane and step
     uint4 raw[NV];
@@ -341,7 +342,8 @@ __device__ __forceinline__ unsigned pack_short(const PackSide& p, int row0, int 
     for (int r = 0; r < R; ++r) {
         const int row = row0 + r;
         raw[r] = make_uint4(0, 0, 0, 0);
-        const bool use = row < p.n && (!p.seen || (p.seen[row >> 5] >> (row & 31) & 1u));
+        const bool use = row < p.n && (!p.seen || (p.seen[row >> 5] >> (row & 31) & 1u)) &&
+                         (!p.lse || p.lse[row] != -INFINITY);
         if (use && c < d)
             raw[r] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) +
                                                           (size_t)row * p.ld + c));
@@ -2245,7 +2247,7 @@ __global__ void head_kernel(const CoefArgs a, uint32_t* __restrict__ alive,
     if (q < a.nq) {
         const Upstream u = upstream_of(a, q);
         on = !u.empty;
-        weight[q] = u.bound > 0.0f && u.bound <= FLT_MAX ? max(-110, ilogbf(u.bound)) : NO_WEIGHT;
+        weight[q] = weight_of(u.bound);
     }
     const unsigned b = __ballot_sync(0xffffffffu, on);
     if ((threadIdx.x & 31) == 0 && q < a.nq) alive[q >> 5] = b;
@@ -3188,6 +3190,12 @@ size_t backward_bytes(const Ctx& c, const fdb_logprob_grad_args& a, const GivenR
     return plan_backward(c, b, given).bytes;
 }
 
+BackwardHead backward_head(const Ctx& c, const fdb_logprob_grad_args& a, const GivenRows& given) {
+    const Backward w = plan_backward(c, a, &given);
+    if (w.few) return BackwardHead{};
+    return BackwardHead{w.weight, reinterpret_cast<uint32_t*>(w.err), (int)(HEAD / 4)};
+}
+
 template <typename T, int NQ, bool GIVEN>
 static void launch_few_grad(const Ctx& c, const Backward& w, const FewGrad<T>& p, cudaStream_t s) {
     const size_t smem = few_grad_smem(NQ, p.d, sizeof(T));
@@ -3253,9 +3261,11 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a, const GivenRows* given
     k.targets = a.targets, k.allowed = a.allowed, k.ld_allowed = ld_allowed;
     k.out = w.coef, k.rest = w.rest;
     if (given) k.at_least = given->at_least;
-    head_kernel<<<(nq + 63) / 64, 64, 0, s>>>(k, w.alive, w.weight,
-                                                 reinterpret_cast<uint32_t*>(w.err), HEAD / 4);
-    FDB_LAUNCH_CHECK();
+    if (!given) {
+        head_kernel<<<(nq + 63) / 64, 64, 0, s>>>(k, w.alive, w.weight,
+                                                     reinterpret_cast<uint32_t*>(w.err), HEAD / 4);
+        FDB_LAUNCH_CHECK();
+    }
     const uint32_t* seen = a.allowed;
     if (w.seen) {
         const size_t words = (a.n + 31) / 32;
@@ -3267,6 +3277,7 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a, const GivenRows* given
     PackSide qside = pack_side(a.queries, a.ld_queries, a.nq, a.dim, a.dtype, w.alive, w.qp, w.qf,
                                &w.head->q_most);
     qside.weight = w.weight;
+    if (given) qside.seen = nullptr, qside.lse = a.lse;
     launch_pack(s, a.dtype, qside,
                 pack_side(a.rows, a.ld_rows, a.n, a.dim, a.dtype, seen, w.xp, w.xf,
                           reinterpret_cast<unsigned*>(&w.head->x_most)),

@@ -69,9 +69,22 @@ struct GivenRows {
     const float* at_least; // [nq] a bound of their sizes over scale, >= 0
 };
 
+// What the caller of backward_run with given rows does before it: the exponents of the
+// queries' bounds, and a cleared head of the workspace (weight null: neither).
+struct BackwardHead {
+    int* weight;      // [nq], weight_of(scale * at_least)
+    uint32_t* clear;  // [words]
+    int words;
+};
+constexpr int NO_WEIGHT = -10000;
+__device__ __forceinline__ int weight_of(float bound) {
+    return bound > 0.0f && bound <= 3.402823466e38f ? max(-110, ilogbf(bound)) : NO_WEIGHT;
+}
+
 size_t forward_bytes(const Ctx& c, const fdb_logprob_args& a, size_t pass_queries = 0);
 void forward_run(Ctx& c, const fdb_logprob_args& a, ForwardEnd* end = nullptr);
 size_t backward_bytes(const Ctx& c, const fdb_logprob_grad_args& a, const GivenRows* given = nullptr);
+BackwardHead backward_head(const Ctx& c, const fdb_logprob_grad_args& a, const GivenRows& given);
 void backward_run(Ctx& c, const fdb_logprob_grad_args& a, const GivenRows* given = nullptr);
 
 // Raises a kernel's shared-memory limit once per device.  A kernel's limit is the
