@@ -778,13 +778,14 @@ __device__ __forceinline__ void finish_search(const Select& p, const Scan& c, Fi
         double L = 0.0;
         float M = -INFINITY;
         const bool live = k == LIVE && given > -INFINITY;
-        bool lost = false;  // (columns, but a sum of 0)
+        bool lost = false, odd = false;  // (columns, but a sum of 0, or none in f32)
         if (live) {
             for (int i = lane; i < S; i += 32) {
                 const Part q = i < 32 ? mine : c.part[(row0 + b) * S + i];
                 bad |= q.count < 0;
                 if (NORM && q.sum > 0.0) M = fmaxf(M, q.m);
                 lost |= q.count > 0;
+                odd |= !(q.sum == q.sum);
             }
             if (NORM) {
 #pragma unroll
@@ -795,7 +796,9 @@ __device__ __forceinline__ void finish_search(const Select& p, const Scan& c, Fi
                 }
 #pragma unroll
                 for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-                lost = __any_sync(0xffffffffu, lost) && !(L > 0.0);
+                odd = __any_sync(0xffffffffu, odd);
+                lost = __any_sync(0xffffffffu, lost) && (odd || !(L > 0.0));
+                if (lost) M = -INFINITY;
                 if (lost) {  // (scores out of f32's range: relative to their largest, in 64 bits)
                     for (int i = lane; i < S; i += 32)
                         if (c.part[(row0 + b) * S + i].count > 0)
@@ -1061,6 +1064,7 @@ static void launch_scan(cudaStream_t s, int device, unsigned blocks, const Selec
 template <typename T, bool NORM>
 static void run(const Ctx& ctx, const fdb_beam_args& a, const Select& p, const Scan& c) {
     const cudaStream_t s = static_cast<cudaStream_t>(a.stream);
+    FDB_REQUIRE(a.groups * a.beams * c.splits < (1ull << 31), FDB_ERR_INVALID_ARG, "too many chains");
     const unsigned parts = (unsigned)(a.groups * a.beams * c.splits);
     if (a.ids || a.allowed) launch_scan<T, NORM, true>(s, ctx.device, parts, p, c);
     else launch_scan<T, NORM, false>(s, ctx.device, parts, p, c);

@@ -1439,6 +1439,7 @@ int fdb_beam_reorder(fdb_ctx* ctx, const fdb_beam_state* states, size_t count,
         FDB_REQUIRE(o.groups == 0 || count == 0 || o.parents, FDB_ERR_INVALID_ARG,
                     "parents is NULL");
         check_aligned(o.parents, 8, "parents");
+        std::vector<std::pair<uintptr_t, size_t>> read, written;
         for (size_t i = 0; i < count; ++i) {
             const fdb_beam_state& t = states[i];
             if (t.bytes == 0 || t.parts == 0) continue;
@@ -1462,6 +1463,20 @@ int fdb_beam_reorder(fdb_ctx* ctx, const fdb_beam_state* states, size_t count,
                              (t.parts == 1 || t.src_part_stride == t.dst_part_stride)),
                         FDB_ERR_INVALID_ARG,
                         "in place needs a width of beams and the same strides");
+            read.emplace_back(reinterpret_cast<uintptr_t>(t.src), i);
+            written.emplace_back(reinterpret_cast<uintptr_t>(t.dst), i);
+        }
+        // a state that is written twice, or read by one and written by another
+        std::sort(read.begin(), read.end());
+        std::sort(written.begin(), written.end());
+        for (size_t i = 0; i < written.size(); ++i) {
+            FDB_REQUIRE(i == 0 || written[i - 1].first != written[i].first, FDB_ERR_INVALID_ARG,
+                        "a state is written twice");
+            for (auto r = std::lower_bound(read.begin(), read.end(),
+                                           std::make_pair(written[i].first, (size_t)0));
+                 r != read.end() && r->first == written[i].first; ++r)
+                FDB_REQUIRE(r->second == written[i].second, FDB_ERR_INVALID_ARG,
+                            "a state that one reads is written by another");
         }
         if (o.groups == 0 || count == 0) return;
         DeviceGuard g(ctx->c.device);

@@ -569,7 +569,8 @@ int fdb_logprobs_status(fdb_ctx* ctx, const void* workspace, void* stream);
  * (log p of each entry, 0 where it takes no part), rest_logprob[nq] (log r, -inf
  * if the query sees no other row; rest = 1 only).  The named rows' scores are
  * taken in 64 bits and r is summed over the other rows, so that it holds as a
- * student becomes sure.  A z that is NaN or +inf makes its query's loss NaN; an
+ * student becomes sure (the workspace holds a filter for each query of a pass for
+ * that: 256 MiB at most, or those of 256 queries).  A z that is NaN or +inf makes its query's loss NaN; an
  * infinity or NaN in a query, or in a row that it may see, all of its outputs. */
 #define FDB_MAX_TEACHER 256 /* largest k */
 typedef struct fdb_distill_args {
@@ -646,15 +647,17 @@ int fdb_distill_backward(fdb_ctx* ctx, const fdb_distill_grad_args* args);
  * normaliser either.
  * beam_scores [groups][beams]: the chains' scores so far, -inf for one that is
  * not there.  ended (nullable): a chain whose byte is not 0 has one candidate,
- * itself, with its score and the id end_id; its columns are not read, nor are
- * those of a chain that is not there.
+ * itself, with its score and the id end_id; its columns do not count, nor do
+ * those of a chain that is not there, whatever they hold.
  *
  * Outputs [groups][width]: the best beam_score + l in order, compared in 64 bits,
- * equal ones by chain, then column (an ended chain stands in column 0); the
- * chain each continues, the id it adds, and whether it has ended (nullable): its
- * chain had, or the id is end_id.  Past the last candidate -inf, -1, -1, 0.  A
- * group with a NaN or +inf in a chain's score or in a score that may count has
- * NaN, -1, -1, 0. */
+ * equal ones by chain, then column (an ended chain stands in column 0; of columns
+ * that only the sum with the chain's score makes equal, those of larger x are
+ * taken); the chain each continues, the id it adds, and whether it has ended
+ * (nullable): its chain had, or the id is end_id.  Past the last candidate -inf,
+ * -1, -1, 0.  A group with a NaN or +inf in a chain's score or in a score that may
+ * count has NaN, -1, -1, 0.  Searches of 2048 columns in all at most need no
+ * workspace (0 bytes). */
 #define FDB_MAX_BEAMS 128 /* largest beams and width */
 typedef struct fdb_beam_args {
     int dtype; /* FDB_DTYPE_* of scores */
@@ -685,8 +688,9 @@ int fdb_beam_select(fdb_ctx* ctx, const fdb_beam_args* args);
  * runs of `bytes` bytes, part_stride bytes apart (a cache's heads, of which the
  * positions in use move); rows are src_stride and dst_stride bytes apart.  What
  * lies between the runs is left as it was, as is a row whose parent is outside
- * [0, beams), unless `clear` is not 0: it is then zeroed (not in place).  dst may be src (same strides, width = beams): in place.  No
- * other overlap.  Needs no workspace. */
+ * [0, beams), unless `clear` is not 0: it is then zeroed (not in place).  dst may
+ * be src (same strides, width = beams): in place.  No other overlap.  Needs no
+ * workspace. */
 typedef struct fdb_beam_state {
     const void* src;
     void* dst;

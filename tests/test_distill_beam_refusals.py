@@ -140,6 +140,22 @@ def test_reorder_refuses(call):
     assert run((256, 256, 64, 128, 1, 0, 0, 64)) == -1            # in place, other strides
 
 
+def test_reorder_refuses_states_that_meet(call):
+    fg, L, ctx = call
+    opts = fg.ReorderOpts(parents=64, groups=2, beams=3, width=3)
+
+    def run(*pairs):
+        flat = [v for s, d in pairs for v in (s, d, 64, 64, 1, 0, 0, 64)]
+        table = (C.c_uint64 * len(flat))(*flat)
+        return L.fdb_beam_reorder(ctx, C.addressof(table), len(pairs), C.byref(opts))
+
+    assert run((4096, 8192), (12288, 8192)) == -1                 # one place for two
+    assert run((4096, 4096), (4096, 4096)) == -1
+    assert run((4096, 8192), (8192, 4096)) == -1                  # each other's places
+    assert run((4096, 4096), (4096, 8192)) == -1                  # turned and read
+    assert b"written" in L.fdb_last_error()
+
+
 def test_oracle_gradient_against_differences():
     """The 64-bit gradient of the 64-bit loss: central differences with h = 1e-5 are off by
     h^2 times third derivatives of size 1, and by 2^-52 / h."""

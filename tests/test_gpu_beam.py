@@ -207,6 +207,36 @@ def test_ended_chains():
     assert r.ended.tolist() == [[False, True, True]] and r.scores[0, 1] == -1.5
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("scale", [3e37, 1e20, 1e-6])
+def test_scales_at_the_ends_of_f32(dtype, scale):
+    """scale * x out of f32's range either way: scores are those of 64 bits."""
+    import forgegpu as fg
+    import torch
+    rng = np.random.default_rng(5)
+    X, x = put(rng.standard_normal((2, 3, 40000)) * 100, dtype)
+    bs = -np.arange(6, dtype=np.float32).reshape(2, 3)
+    r = fg.beam_select(X, torch.from_numpy(bs).cuda(), width=6, scale=scale)
+    s, p, i, e = do.select(x, bs, 6, scale=scale)
+    assert np.array_equal(r.ids.cpu().numpy(), i) and np.array_equal(r.parents.cpu().numpy(), p)
+    with np.errstate(over="ignore", invalid="ignore"):
+        s = np.where(np.abs(s) > 3.4e38, np.sign(s) * np.inf, s)
+    got = r.scores.double().cpu().numpy()
+    assert np.array_equal(np.isinf(got), np.isinf(s))
+    fin = np.isfinite(s)
+    assert (np.abs(got[fin] - s[fin]) <= 2.0 ** -23 * np.abs(s[fin]) + 2.0 ** -17).all()
+
+
+def test_without_searches():
+    import forgegpu as fg
+    import torch
+    x = torch.zeros((0, 3, 5000), device="cuda")
+    r = fg.beam_select(x, x[:, :, 0].contiguous(), width=4)
+    assert r.ids.shape == (0, 4)
+    o, = fg.beam_reorder([x], r.parents[:, :3].contiguous())
+    assert o.shape == (0, 3, 5000)
+
+
 def test_large_offsets():
     """Chains more than 2^31 elements apart."""
     import forgegpu as fg

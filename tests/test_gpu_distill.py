@@ -402,6 +402,43 @@ def test_passes_of_a_large_call():
             assert (a[at] - b).abs().max() <= 2.0 ** -17
 
 
+def test_offsets_beyond_32_bits():
+    """2.2e9 elements of rows: rows past 2^32 bytes and 2^31 elements are named, score and
+    get their gradient like copies of them in a small table."""
+    import forgegpu as fg
+    import torch
+    n, d = 2_150_000, 1024
+    g = torch.Generator(device="cuda").manual_seed(0)
+    X = torch.empty(n, d, dtype=torch.bfloat16, device="cuda")
+    for i in range(0, n, 50_000):
+        X[i:i + 50_000] = torch.randn(min(50_000, n - i), d, generator=g, device="cuda")
+    pick = torch.tensor([0, 1_048_576, 2_097_151, 2_097_152, 2_149_999], device="cuda")
+    near = (pick[:, None] + torch.arange(-40, 41, device="cuda")).flatten()
+    near = near[(near >= 0) & (near < n)].unique()
+    bits = np.zeros((1, n), bool)
+    bits[0, near.cpu().numpy()] = True
+    keep, = cuda(so.words(bits)[0])
+    small = X[near].contiguous()
+    I = torch.stack([pick, pick.roll(1), pick.roll(2)], 1).repeat(4, 1)
+    where = torch.searchsorted(near, I)
+    Q = (X[pick].float() * 1.2).bfloat16().repeat(4, 1)
+    Z = torch.log(torch.tensor([[0.5, 0.2, 0.1]], device="cuda")).repeat(20, 1)
+    up = torch.full((20,), 0.05, device="cuda")
+    for nq in (5, 20):
+        a = fg.distill(Q[:nq], X, I[:nq], Z[:nq], scale=0.02, rest=True, allowed=keep)
+        b = fg.distill(Q[:nq], small, where[:nq], Z[:nq], scale=0.02, rest=True)
+        for u, v in zip(a, b):  # (the same scores in other groups: each lse within 2^-19)
+            assert (u - v).abs().max() <= 2.0 ** -17
+        ga = fg.distill_backward(Q[:nq], X, I[:nq], Z[:nq], a.lse, a.logprobs, a.rest,
+                                 d_loss=up[:nq], scale=0.02, allowed=keep)
+        gb = fg.distill_backward(Q[:nq], small, where[:nq], Z[:nq], a.lse, a.logprobs, a.rest,
+                                 d_loss=up[:nq], scale=0.02)
+        # two roundings to bf16 of sums that differ far below them
+        assert ((ga[0] - gb[0]).abs().float() <= 2.0 ** -7 * gb[0].abs().float() + 1e-6).all()
+        assert ((ga[1][near] - gb[1]).abs().float() <= 2.0 ** -7 * gb[1].abs().float() + 1e-6).all()
+        assert not ga[1][1000:1_048_000].any()
+
+
 def test_same_call_same_bits_in_graphs_and_on_streams():
     import forgegpu as fg
     import torch
