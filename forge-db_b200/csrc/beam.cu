@@ -15,6 +15,9 @@ namespace fdb {
 namespace beam {
 
 using sr::Carve;
+using sr::hi_of;
+using sr::lo_of;
+using sr::packf;
 using sr::to_f32;
 using sr::up;
 
@@ -73,25 +76,6 @@ __device__ __forceinline__ double unordered64(uint64_t u) {
     return __longlong_as_double((long long)(u >> 63 ? u & 0x7fffffffffffffffull : ~u));
 }
 
-
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-    uint64_t d;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
-    return d;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
 
 // ---------------------------------------------------------------------------
 // scanning the chains' columns
@@ -386,21 +370,18 @@ __device__ __forceinline__ void scan_part(const Select& p, const Scan& c, ScanSh
                 ref = to;
                 started = true;
             }
-            const uint64_t c2 = pack2(-ref, -ref), s2 = pack2(c.s, c.s);
+            const uint64_t c2 = packf(-ref, -ref), s2 = packf(c.s, c.s);
             uint64_t acc[2] = {0, 0};
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int i = 0; i < N / 2; ++i) {
                     const float2 f = Vec<T>::pair(r[u], i);
-                    const uint64_t t2 = fma2(pack2(f.x, f.y), s2, c2);
-                    float t0, t1;
-                    unpack2(t2, t0, t1);
-                    acc[i & 1] = add2(acc[i & 1], pack2(sr::ex2(t0), sr::ex2(t1)));
+                    const uint64_t t2 = tc::fma2(packf(f.x, f.y), s2, c2);
+                    acc[i & 1] = tc::add2(acc[i & 1], packf(sr::ex2(lo_of(t2)), sr::ex2(hi_of(t2))));
                 }
-            float a0, a1;
-            unpack2(add2(acc[0], acc[1]), a0, a1);
-            sum += (double)(a0 + a1);
+            const uint64_t both = tc::add2(acc[0], acc[1]);
+            sum += (double)(lo_of(both) + hi_of(both));
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");

@@ -138,22 +138,21 @@ struct LossArgs {
     float scale;
     float *loss, *lse, *logprobs, *rest;
 };
-// A vector's products with a query, added up in pairs.
+// Two sums of a vector's products with a query's: of the even and of the odd columns.
 template <typename T>
-__device__ __forceinline__ float dot_vec(const uint4& v, const float* q) {
-    constexpr int V = 16 / (int)sizeof(T);
+__device__ __forceinline__ uint64_t dot_vec(const uint4& v, const float* q, uint64_t sums) {
     const T* e = reinterpret_cast<const T*>(&v);
-    float y[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) y[i] = to_f32<T>(e[i]) * q[i];
-#pragma unroll
-    for (int w = V / 2; w; w >>= 1)
-#pragma unroll
-        for (int i = 0; i < w; ++i) y[i] += y[i + w];
-    return y[0];
+    for (int i = 0; i < 16 / (int)sizeof(T); i += 4) {
+        const float4 y = *reinterpret_cast<const float4*>(q + i);
+        sums = tc::fma2(sr::packf(to_f32<T>(e[i]), to_f32<T>(e[i + 1])), sr::packf(y.x, y.y), sums);
+        sums = tc::fma2(sr::packf(to_f32<T>(e[i + 2]), to_f32<T>(e[i + 3])), sr::packf(y.z, y.w), sums);
+    }
+    return sums;
 }
-// One block per query: the pass's sums joined, the named rows scored (16 bytes'
-// products in f32, their sums in 64 bits), the loss.  Gathers k rows a query.
+// One block per query: the pass's sums joined, the named rows scored (sums of up to
+// four 16-byte vectors' products in f32, theirs in 64 bits), the loss.  Gathers k rows
+// a query.
 template <typename T, int TH>
 __global__ void __launch_bounds__(TH) loss_kernel(const LossArgs p) {
     extern __shared__ float4 q_raw[];
@@ -201,17 +200,20 @@ __global__ void __launch_bounds__(TH) loss_kernel(const LossArgs p) {
         }
         int c = sub;
         if (wide) {
+            constexpr int STEPS = 4;
+            for (c = sub * V; c + V <= p.d;) {
+                uint64_t two[ROWS] = {};
 #pragma unroll 2
-            for (c = sub * V; c + V <= p.d; c += lanes * V) {
-                uint4 v[ROWS];
+                for (int n = 0; n < STEPS && c + V <= p.d; ++n, c += lanes * V) {
+                    uint4 v[ROWS];
 #pragma unroll
-                for (int r = 0; r < ROWS; ++r) v[r] = __ldg(reinterpret_cast<const uint4*>(x[r] + c));
-                float y[V];
+                    for (int r = 0; r < ROWS; ++r)
+                        v[r] = __ldg(reinterpret_cast<const uint4*>(x[r] + c));
 #pragma unroll
-                for (int j = 0; j < V; j += 4)
-                    *reinterpret_cast<float4*>(y + j) = *reinterpret_cast<const float4*>(qs + c + j);
+                    for (int r = 0; r < ROWS; ++r) two[r] = dot_vec<T>(v[r], qs + c, two[r]);
+                }
 #pragma unroll
-                for (int r = 0; r < ROWS; ++r) acc[r] += (double)dot_vec<T>(v[r], y);
+                for (int r = 0; r < ROWS; ++r) acc[r] += (double)(sr::lo_of(two[r]) + sr::hi_of(two[r]));
             }
             // (the row's last, partial vector: one lane's)
             for (; c < p.d; ++c)

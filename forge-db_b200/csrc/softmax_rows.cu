@@ -84,21 +84,6 @@ constexpr float NONE = -1e30f;              // score of a row that may not be se
 constexpr float NONE_BELOW = -1e29f;
 constexpr float RAISE = 8.0f;               // see Run
 
-__device__ __forceinline__ float lo_of(uint64_t v) {
-    uint32_t a, b;
-    asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
-    return __uint_as_float(a);
-}
-__device__ __forceinline__ float hi_of(uint64_t v) {
-    uint32_t a, b;
-    asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
-    return __uint_as_float(b);
-}
-__device__ __forceinline__ uint64_t packf(float a, float b) {
-    uint64_t d;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(__float_as_uint(a)), "r"(__float_as_uint(b)));
-    return d;
-}
 __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));

@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 
 #include "fdb_internal.h"
+#include "tc_ptx.cuh"
 
 namespace fdb {
 namespace sr {
@@ -16,6 +17,23 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// ---- pairs of f32 ----
+__device__ __forceinline__ float lo_of(uint64_t v) {
+    uint32_t a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
+    return __uint_as_float(a);
+}
+__device__ __forceinline__ float hi_of(uint64_t v) {
+    uint32_t a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
+    return __uint_as_float(b);
+}
+__device__ __forceinline__ uint64_t packf(float a, float b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(__float_as_uint(a)), "r"(__float_as_uint(b)));
+    return d;
 }
 
 template <typename T>

@@ -552,9 +552,9 @@ int fdb_logprobs_status(fdb_ctx* ctx, const void* workspace, void* stream);
  * under the p_ij of fdb_logprobs, whose rules for streams, workspaces, captured
  * graphs and buffers hold here too (fdb_logprobs_status reads the workspace).
  *
- * teacher_ids and teacher_logits [nq][k], rows ld_ids and ld_logits >= k apart.  An entry
- * takes part if its id is in [0, n), the query may see that row, its logit z is
- * not -inf and no entry before it that takes part has its id (lists may be
+ * teacher_ids and teacher_logits [nq][k], rows ld_ids and ld_logits >= k apart.  An
+ * entry takes part if its id is in [0, n), the query may see that row, its logit z
+ * is not -inf and no entry before it that takes part has its id (lists may be
  * short, unsorted, or empty: the loss is then 0).
  *   rest = 0:  P = softmax of teacher_scale * z over the entries,
  *              loss = sum_e P_e (log P_e - log p_e)
@@ -567,11 +567,11 @@ int fdb_logprobs_status(fdb_ctx* ctx, const void* workspace, void* stream);
  *
  * Outputs, each nullable: loss[nq], lse[nq] (as fdb_logprobs'), logprobs[nq][k]
  * (log p of each entry, 0 where it takes no part), rest_logprob[nq] (log r, -inf
- * if the query sees no other row; rest = 1 only).  The named rows' scores are
- * taken in 64 bits and r is summed over the other rows, so that it holds as a
- * student becomes sure (the workspace holds a filter for each query of a pass for
- * that: 256 MiB at most, or those of 256 queries).  A z that is NaN or +inf makes its query's loss NaN; an
- * infinity or NaN in a query, or in a row that it may see, all of its outputs. */
+ * if the query sees no other row; rest = 1 only).  r is summed over the other
+ * rows, so that it holds its precision as a student becomes sure (the workspace has
+ * a filter for each query of a pass for that: 256 MiB at most, or those of 256
+ * queries).  A z that is NaN or +inf makes its query's loss NaN; an infinity or NaN
+ * in a query, or in a row that it may see, all of its outputs. */
 #define FDB_MAX_TEACHER 256 /* largest k */
 typedef struct fdb_distill_args {
     int dtype; /* FDB_DTYPE_* of queries and rows */

@@ -67,11 +67,13 @@ def forward(q, x, ids, z, scale, tscale, rest, allowed):
 
 def forward_bounds(o, es):
     """lse: as the log-softmax's (es the scores' bound).  An entry's score is a sum in
-    64 bits of sums in f32 of up to 8 products, each off by half a step and added in
-    three levels: 4 * 2^-24 of the products' sizes, less than es, which counts 2^-22
-    and more of them.  Its log probability is off by that and as the lse is; log r
-    is the difference of two such sums, the loss lse - R lse_rest and the mean of the
-    named scores; each rounded once."""
+    64 bits of f32 sums over a lane's columns, four vectors at most: chains of 4 fused
+    products a vector of 16 bits (2 of f32), the first product of which is exact (of f32
+    rounded), and one addition, (d / 64 + 4 + 1) 2^-24 of the products' sizes or less for
+    lanes that share d columns 256 a step, and 17 * 2^-24 at most: less than es, which
+    counts (d / 16 + 1) 2^-22 of them (f32: 15 * 2^-22).  Its log probability is off by
+    that and as the lse is; log r is the difference of two such sums, the loss
+    lse - R lse_rest and the mean of the named scores; each rounded once."""
     e = so.forward_bounds(o["f"], es)[0]
     named = np.where(o["keep"], es, 0.0).max(1)
     fin = lambda v: np.where(np.isfinite(v), np.abs(v), 0.0)  # noqa: E731
