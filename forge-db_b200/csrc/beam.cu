@@ -40,15 +40,15 @@ struct Select {
     uint8_t* out_ended;
 };
 
-// scale x of a column, -inf if it takes no part
+// A column's x, -inf if it takes no part.
 template <typename T>
-__device__ __forceinline__ double column(const Select& p, int g, int b, int j) {
+__device__ __forceinline__ float column(const Select& p, int g, int b, int j) {
     const size_t row = (size_t)g * p.beams + b;
     // (all loads first)
     const float x = to_f32<T>(static_cast<const T*>(p.x)[(size_t)g * p.ld_group + (size_t)b * p.ld_beam + j]);
     const int64_t id = p.ids ? p.ids[row * p.ld_ids + j] : 0;
     const uint32_t w = p.allowed ? p.allowed[row * p.ld_allowed + (j >> 5)] : 0xffffffffu;
-    return id < 0 || !(w >> (j & 31) & 1u) ? -INFINITY : p.scale * (double)x;
+    return id < 0 || !(w >> (j & 31) & 1u) ? -INFINITY : x;
 }
 __device__ __forceinline__ bool over(const Select& p, int g, int b) {
     return p.ended && p.ended[(size_t)g * p.beams + b];
@@ -59,37 +59,39 @@ __device__ __forceinline__ bool absent(const Select& p, int g, int b) {
 }
 
 // ---------------------------------------------------------------------------
-// order-preserving images of numbers
+// order-preserving images of numbers (of -0 and 0 the same)
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t ordered(float f) {
-    const uint32_t u = __float_as_uint(f);
+    const uint32_t u = __float_as_uint(f + 0.0f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float unordered(uint32_t u) {
     return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
 __device__ __forceinline__ uint64_t ordered64(double v) {
-    const uint64_t u = (uint64_t)__double_as_longlong(v);
+    const uint64_t u = (uint64_t)__double_as_longlong(v + 0.0);
     return u >> 63 ? ~u : u | 0x8000000000000000ull;
 }
 __device__ __forceinline__ double unordered64(uint64_t u) {
     return __longlong_as_double((long long)(u >> 63 ? u & 0x7fffffffffffffffull : ~u));
 }
 
-
 // ---------------------------------------------------------------------------
 // scanning the chains' columns
 // ---------------------------------------------------------------------------
 // A block takes a part of a chain's columns, a tile of TH * U loads of 16 bytes at a
 // time, and leaves their sum of exponentials and the `width` best.  The pass over the
-// columns only adds up and keeps each thread's largest of a tile: 130 instructions and
-// 32 exponentials for 32 columns of 16 bits, no barrier.  The best are found from those
-// maxima afterwards: of the threads' largest the width-th (or, for few, the least of
-// the largest of G >= width groups of threads) is reached by at least `width` columns
-// and by hardly more; only the maxima that reach it are looked behind, by reading
-// their columns again.
+// columns only adds up and keeps each thread's largest of a span of tiles, without a
+// barrier.  The best are found from those maxima afterwards: of the threads' largest the
+// width-th (or, for few, the least of the largest of G >= width groups of threads) is
+// reached by at least `width` columns and by hardly more; only the maxima that reach it
+// are looked behind, by reading their columns again.
 // Sums are taken relative to a thread's own largest score so far (raised only when it
-// is exceeded by 2^8), 32 terms in f32 and those in 64 bits.
+// is exceeded by 2^8), a tile's terms in f32 and those in 64 bits.
+// 64 x 8 x 131072 columns, width 8: f32 48 us (5.5 TB/s, where a copy has 6.4), bf16 30
+// (4.5 TB/s): a block's start and end, some 4 us without loads, and one exponential a
+// column (40 % of their unit's rate).  Looking for the best column by column, as they
+// come, took 74 us; a block for each search's last to end, with the finish, 46.
 constexpr int TH = 256;               // threads
 constexpr int U = 4;                  // loads of a thread in a tile
 constexpr int SPAN = 2;               // tiles whose largest is kept together
@@ -214,7 +216,6 @@ __device__ __forceinline__ uint4 load_vec(const Select& p, const T* x, int skip,
     }
     return r;
 }
-
 
 // ---- the best of what lies in shared memory ----
 constexpr int LIMIT = 256;              // keys that are put in order at once
@@ -658,29 +659,23 @@ __device__ __forceinline__ uint32_t address_in(const void* p, int rank) {
     return r;
 }
 // A block's share of the sum of 2^((x - top) unit) over chain b's columns, in 64 bits;
-// the whole block's, in every thread.
+// the whole block's, in every thread.  By column, whatever the chain's alignment: equal
+// chains have equal sums.
 template <typename T>
 __device__ __forceinline__ double sum_share(const Select& p, int g, int b, float top, int rank,
                                             int blocks, double* part) {
     const double unit = p.scale * sr::LOG2E;
-    const T* x = static_cast<const T*>(p.x) + (size_t)g * p.ld_group + (size_t)b * p.ld_beam;
-    const int skip = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-    const int nv = (int)(((long long)p.n + skip + Vec<T>::N - 1) / Vec<T>::N);
-    constexpr int AHEAD = 4;  // (loads in flight: one at a time they are what it waits for)
+    constexpr int AHEAD = 8;  // (loads in flight: one at a time they are what it waits for)
     double t = 0.0;
-    for (int v = rank * TH + (int)threadIdx.x; v < nv; v += AHEAD * blocks * TH) {
-        uint4 q[AHEAD];
+    for (long long j = rank * TH + (int)threadIdx.x; j < p.n; j += AHEAD * blocks * TH) {
+        float x[AHEAD];
 #pragma unroll
-        for (int a = 0; a < AHEAD; ++a)
-            q[a] = load_vec<T, true>(p, x, skip, (size_t)g * p.beams + b, v + a * blocks * TH, nv);
+        for (int a = 0; a < AHEAD; ++a) {
+            const long long at = j + a * blocks * TH;
+            x[a] = at < p.n ? column<T>(p, g, b, (int)at) : -INFINITY;
+        }
 #pragma unroll
-        for (int a = 0; a < AHEAD; ++a)
-#pragma unroll
-            for (int i = 0; i < Vec<T>::N / 2; ++i) {
-                const float2 f = Vec<T>::pair(q[a], i);
-                t += exp2_series(((double)f.x - (double)top) * unit) +
-                     exp2_series(((double)f.y - (double)top) * unit);
-            }
+        for (int a = 0; a < AHEAD; ++a) t += exp2_series(((double)x[a] - (double)top) * unit);
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
@@ -692,9 +687,11 @@ __device__ __forceinline__ double sum_share(const Select& p, int g, int b, float
     return t;
 }
 // One block per search, with others of its cluster to help where sums are taken again.
-// The chains' normalisers are sums of f32 exponentials, off by up to `slack` / 2: where that leaves open which of two chains'
-// columns is the better, among the chosen or at their end, the chains' sums are taken
-// again in 64 bits.
+// The chains' normalisers are sums of f32 exponentials, off by up to `slack` / 2: where
+// that leaves open which of two chains' columns is the better, among the chosen or at
+// their end, the chains' sums are taken again in 64 bits.  Bound by a chain of short
+// steps: 6 us for 4 chains of 10000 columns, 8 for 64 x 8 of 131072 (width 64: 13), a
+// chain's sum again 10 us by eight blocks, 48 by one.
 struct FinishShared {
     Choice s;
     double sum[MAXW], lse[MAXW], part[TH / 32];
@@ -873,7 +870,7 @@ __device__ __forceinline__ void finish_search(const Select& p, const Scan& c, Fi
             for (int r0 = 0; r0 < p.width; r0 += ranks) {
                 bool any = false;
                 for (int l0 = 0; l0 < lists; l0 += some) {
-    #pragma unroll 4
+#pragma unroll 4
                     for (int k = tid; k < some * ranks; k += TH) {
                         const int i = l0 + k / ranks, rank = r0 + k % ranks;
                         double v;
@@ -960,11 +957,11 @@ __global__ void __launch_bounds__(TH, 4) small_kernel(const Select p) {
         for (int b = tid >> 5; b < p.beams; b += TH / 32) {
             if (absent(p, g, b) || over(p, g, b)) continue;
             double m = -INFINITY, t = 0.0;
-            for (int j = lane; j < p.n; j += 32) m = fmax(m, column<T>(p, g, b, j));
+            for (int j = lane; j < p.n; j += 32) m = fmax(m, p.scale * column<T>(p, g, b, j));
 #pragma unroll
             for (int o = 16; o; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
             if (m > -INFINITY)
-                for (int j = lane; j < p.n; j += 32) t += exp(column<T>(p, g, b, j) - m);
+                for (int j = lane; j < p.n; j += 32) t += exp(p.scale * column<T>(p, g, b, j) - m);
 #pragma unroll
             for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
             if (lane == 0) lse[b] = m > -INFINITY ? m + log(t) : 0.0;
@@ -982,7 +979,7 @@ __global__ void __launch_bounds__(TH, 4) small_kernel(const Select p) {
         if (k >= all) continue;
         b[h] = k / p.n, j[h] = k - b[h] * p.n;
         const float given = p.beam_scores[row0 + b[h]];
-        const double x = column<T>(p, g, b[h], j[h]);
+        const double x = p.scale * column<T>(p, g, b[h], j[h]);
         bad |= !(given < INFINITY);
         if (given == -INFINITY) continue;
         if (over(p, g, b[h])) {
@@ -1049,8 +1046,7 @@ static void run(const Ctx& ctx, const fdb_beam_args& a, const Select& p, const S
     const unsigned parts = (unsigned)(a.groups * a.beams * c.splits);
     if (a.ids || a.allowed) launch_scan<T, NORM, true>(s, ctx.device, parts, p, c);
     else launch_scan<T, NORM, false>(s, ctx.device, parts, p, c);
-    // Launched while the scan ends; blocks that help, where there is room for them (64 x 8
-    // x 131072, 64 places: a chain's sum again takes 48 us by one block).
+    // Launched while the scan ends; blocks that help, where there is room for them.
     unsigned blocks = 1;
     while (NORM && a.beams > 1 && blocks < 8 && a.groups * blocks * 2 <= (size_t)ctx.sm_count * 4) blocks *= 2;
     cudaLaunchAttribute attr[2] = {};
@@ -1072,11 +1068,13 @@ static void run(const Ctx& ctx, const fdb_beam_args& a, const Select& p) {
         return;
     }
     l.c.s = (float)std::min((double)a.scale * sr::LOG2E, 3e38);
-    // What two normalisers may be off by: the exponentials (2^-22 of themselves, and
-    // once more where a reference is raised), f32 sums of 32 of them in four chains
-    // (8 x 2^-24), and in the exponents, whose mean size under the softmax is at most
-    // log2 n, a subtraction, a product and the factor s (2.5 x 2^-24 ln 2 of them).
-    l.c.slack = (float)(2.0 * (0x1p-21 + 0x1p-21 + 1.75 * 0x1p-24 * (std::log2((double)a.n) + 1.0)));
+    // What two normalisers may be off by.  Each term: its exponential and up to three
+    // factors that are exponentials (2^-22 each), ten additions (2^-24), and in the
+    // exponent the product's rounding and that of s (2 x 2^-24 of it, times ln 2); the
+    // sum sees the exponents' mean under the softmax, at most their entropy, log2 n, and
+    // the 8 that a reference may lie below the largest.
+    l.c.slack = (float)(2.0 * (0x1p-20 + 10 * 0x1p-24 +
+                               1.4 * 0x1p-24 * (std::log2((double)a.n) + 8.0)));
     if (a.normalise) run<T, true>(ctx, a, p, l.c);
     else run<T, false>(ctx, a, p, l.c);
 }

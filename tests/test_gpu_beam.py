@@ -27,11 +27,12 @@ def put(a, dtype, pad=0, shift=0):
 
 
 def check(r, want, n=2 ** 17):
-    """Scores, where a chain's normaliser is a sum of n f32 exponentials e = 2^t of
-    t <= 8, within 2^-22 of each (twice, where a reference is raised), 8 additions of
-    2^-24 in a row, and an error of 2.5 roundings of t in its exponent: ln 2 * 2.5 *
-    2^-24 |t|, of which the sum sees the mean under the softmax, at most log2 n (the
-    entropy) + 1.  Their sum, and half a step of f32 for the score itself."""
+    """Scores.  A chain's normaliser is a sum of n f32 exponentials 2^t relative to a
+    reference at most 8 below the largest: each is within 2^-22 of itself, as are up to
+    three factors (a raised reference, the thread's and its block's), ten additions are off
+    by 2^-24, and the exponent by the roundings of its product and of scale * log2 e: ln 2 *
+    2 * 2^-24 |t|, of which the sum sees the mean under the softmax, at most log2 n (the
+    entropy) + 8.  Their sum, and half a step of f32 for the score itself."""
     s, p, i, e = want
     assert np.array_equal(r.parents.cpu().numpy(), p)
     assert np.array_equal(r.ids.cpu().numpy(), i)
@@ -40,7 +41,7 @@ def check(r, want, n=2 ** 17):
     fin = np.isfinite(s)
     assert np.array_equal(got[~fin], s[~fin], equal_nan=True)
     off = np.abs(got[fin] - s[fin])
-    lse = 2.0 ** -21 + 2.0 ** -21 + 1.75 * 2.0 ** -24 * (np.log2(n) + 1)
+    lse = 2.0 ** -20 + 10 * 2.0 ** -24 + 1.4 * 2.0 ** -24 * (np.log2(n) + 8)
     assert (off <= so.H32 * np.abs(s[fin]) * (1 + 2.0 ** -10) + lse).all(), off.max()
 
 
@@ -110,6 +111,21 @@ def test_equal_and_sorted_scores(dtype, g, b, n, w, kind):
     check(r, do.select(x, bs, w))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [50, 9000])
+@pytest.mark.parametrize("normalise", [True, False])
+def test_zeros_of_either_sign_are_equal(dtype, n, normalise):
+    import forgegpu as fg
+    import torch
+    x = np.full((1, 3, n), -1.0)
+    x[0, :, 3::5] = -0.0
+    x[0, :, 4::5] = 0.0
+    X, x = put(x, dtype)
+    bs = np.array([[0.0, -0.0, -0.5]], np.float32)
+    r = fg.beam_select(X, torch.from_numpy(bs).cuda(), width=12, normalise=normalise)
+    check(r, do.select(x, bs, 12, normalise=normalise))
+
+
 @pytest.mark.parametrize("dtype,g,b,n,w", [("f32", 3, 4, 5000, 8), ("bf16", 2, 8, 3000, 16)])
 def test_chains_whose_normalisers_nearly_agree(dtype, g, b, n, w):
     """The chains' best columns are the same, their normalisers differ by 1e-6 to 1e-10:
@@ -127,6 +143,20 @@ def test_chains_whose_normalisers_nearly_agree(dtype, g, b, n, w):
     gaps = -np.diff(want[0][:, :4])
     assert (gaps > 1e-12).all() and gaps.min() < 1e-5  # (what 64 bits hold apart, 32 do not)
     check(fg.beam_select(X, torch.from_numpy(bs).cuda(), width=w), want)
+
+
+@pytest.mark.parametrize("dtype,g,b,n,w", [("f32", 2, 4, 5003, 9), ("bf16", 1, 8, 30001, 16),
+                                           ("f16", 3, 5, 2049, 20)])
+def test_equal_chains_of_any_alignment(dtype, g, b, n, w):
+    """The chains hold the same columns and start at different places of 16 bytes: their
+    columns are equal and go by chain."""
+    import forgegpu as fg
+    import torch
+    x = np.repeat(np.random.default_rng(6).standard_normal((g, 1, n)) * 3, b, 1)
+    X, x = put(x, dtype)
+    bs = np.zeros((g, b), np.float32)
+    r = fg.beam_select(X, torch.from_numpy(bs).cuda(), width=w)
+    check(r, do.select(x, bs, w))
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
