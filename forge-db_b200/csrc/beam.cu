@@ -622,15 +622,15 @@ __device__ __forceinline__ void write_out(const Select& p, int g, const Choice& 
     }
 }
 
-// 2^t within 2^-46 of itself, t < 1000: the Taylor series of e^(f ln 2), |f| <= 1/2, to
-// f^11 (what is left out: 0.347^12 / 12! = 6e-15).  A third of exp()'s operations, which
-// sums of a whole chain by one block wait for (131072 columns: 50 us).
+// 2^t within 2^-46 of itself, -1000 <= t < 1000: the Taylor series of e^(f ln 2), |f| <= 1/2, to
+// f^11 (what is left out: 0.347^12 / 12! = 6e-15).  Less than half of exp()'s operations,
+// on a pipe that such a sum keeps a few multiprocessors busy with.
 __device__ __forceinline__ double exp2_series(double t) {
     constexpr double L = sr::LN2;
     constexpr double c2 = L * L / 2, c3 = c2 * L / 3, c4 = c3 * L / 4, c5 = c4 * L / 5, c6 = c5 * L / 6,
                      c7 = c6 * L / 7, c8 = c7 * L / 8, c9 = c8 * L / 9, c10 = c9 * L / 10,
                      c11 = c10 * L / 11;
-    if (!(t > -1000.0)) return 0.0;
+    t = fmax(t, -1000.0);  // (as good as 0; no branch, so that several run at once)
     const double n = rint(t), f = t - n;
     double y = fma(c11, f, c10);
     y = fma(y, f, c9);
@@ -665,17 +665,36 @@ template <typename T>
 __device__ __forceinline__ double sum_share(const Select& p, int g, int b, float top, int rank,
                                             int blocks, double* part) {
     const double unit = p.scale * sr::LOG2E;
+    const size_t row = (size_t)g * p.beams + b;
+    const T* xs = static_cast<const T*>(p.x) + (size_t)g * p.ld_group + (size_t)b * p.ld_beam;
+    const int64_t* ids = p.ids ? p.ids + row * p.ld_ids : nullptr;
+    const uint32_t* al = p.allowed ? p.allowed + row * p.ld_allowed : nullptr;
     constexpr int AHEAD = 8;  // (loads in flight: one at a time they are what it waits for)
+    const int step = blocks * TH;
     double t = 0.0;
-    for (long long j = rank * TH + (int)threadIdx.x; j < p.n; j += AHEAD * blocks * TH) {
-        float x[AHEAD];
+    for (long long j0 = rank * TH + (int)threadIdx.x; j0 < p.n; j0 += AHEAD * step) {
+        const int j = (int)j0, last = p.n - 1;
+        T raw[AHEAD];
+        bool in[AHEAD];
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a) {
-            const long long at = j + a * blocks * TH;
-            x[a] = at < p.n ? column<T>(p, g, b, (int)at) : -INFINITY;
+            in[a] = j0 + a * step <= last;
+            raw[a] = xs[in[a] ? j + a * step : last];
+        }
+        if (ids) {
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) in[a] &= ids[in[a] ? j + a * step : last] >= 0;
+        }
+        if (al) {
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) {
+                const int at = in[a] ? j + a * step : last;
+                in[a] &= (bool)(al[at >> 5] >> (at & 31) & 1u);
+            }
         }
 #pragma unroll
-        for (int a = 0; a < AHEAD; ++a) t += exp2_series(((double)x[a] - (double)top) * unit);
+        for (int a = 0; a < AHEAD; ++a)
+            t += in[a] ? exp2_series(((double)to_f32<T>(raw[a]) - (double)top) * unit) : 0.0;
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
@@ -691,7 +710,7 @@ __device__ __forceinline__ double sum_share(const Select& p, int g, int b, float
 // that leaves open which of two chains' columns is the better, among the chosen or at
 // their end, the chains' sums are taken again in 64 bits.  Bound by a chain of short
 // steps: 6 us for 4 chains of 10000 columns, 8 for 64 x 8 of 131072 (width 64: 13), a
-// chain's sum again 10 us by eight blocks, 48 by one.
+// chain's sum again 14 us by eight blocks, some 50 by one.
 struct FinishShared {
     Choice s;
     double sum[MAXW], lse[MAXW], part[TH / 32];
