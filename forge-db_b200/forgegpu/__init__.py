@@ -1197,7 +1197,8 @@ def distill_backward(queries, rows, teacher_ids, teacher_logits, lse, logprobs, 
                      need_queries: bool = True, need_rows: bool = True, workspace=None):
     """(d_queries, d_rows) of sum(d_loss * loss), given what distill returned for
     the same arguments: lse, logprobs and, if it was called with rest, its rest
-    (fdb_distill_backward in forgegpu.h).  A gradient that is not needed is None."""
+    (fdb_distill_backward in forgegpu.h).  A gradient that is not needed is None;
+    the teacher's lists have none."""
     torch = _torch()
     head = _distill_args(queries, rows, teacher_ids, teacher_logits, scale, teacher_scale,
                          0 if rest is None else 1, allowed)

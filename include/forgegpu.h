@@ -156,8 +156,8 @@ int fdb_ctx_init_comm_timeout(fdb_ctx* ctx, int rank, int world, const void* ncc
  * search_with_timeout (ivf_pq.rs:1369-1455). */
 int fdb_ctx_set_wait_limit(fdb_ctx* ctx, double seconds);
 /* Test hook for the timeout path: the next `count` list-scan launches of the
- * tensor path (or fdb_logprobs / fdb_logprobs_backward calls that use it) on
- * this context issue no work, so the waits inside them find a flag that
+ * tensor path (or fdb_logprobs and fdb_distill calls that use it, and their
+ * gradients') on this context issue no work, so the waits inside them find a flag that
  * nothing sets and run out after the wait limit (no fault, no hang: nothing
  * is in flight).  The call that contains them returns FDB_ERR_TIMEOUT
  * (fdb_logprobs_status does). */
