@@ -871,9 +871,15 @@ __device__ __forceinline__ void finish_search(const Select& p, const Scan& c, Fi
                 const int k = h * TH + tid, i = k / p.width, rank = k - i * p.width;
                 if (i >= lists || !worth(i, rank, key[h], count[h], v[h], b[h], col[h]))
                     v[h] = -INFINITY;
-                if (i < lists && rank < q) s.set[i * q + rank] = __double2float_rd(v[h]);
+                if (lists <= TH && i < lists && rank < q) s.set[i * q + rank] = __double2float_rd(v[h]);
             }
-            pick(s, v, b, col, lists * q, p.width, slack);
+            if (lists > TH) {
+                float m = -INFINITY;
+#pragma unroll
+                for (int h = 0; h < HELD; ++h) m = fmaxf(m, __double2float_rd(v[h]));
+                s.set[tid] = m;
+            }
+            pick(s, v, b, col, min(lists * q, TH), p.width, slack);
         } else {
             float m = -INFINITY;
             for (int k = tid; k < lists * q; k += TH) {
@@ -1231,8 +1237,8 @@ __global__ void turn_kernel(const __grid_constant__ States t, const int64_t* __r
 void reorder_run(const Ctx& c, const fdb_beam_state* states, size_t count,
                  const fdb_reorder_opts& o) {
     const cudaStream_t s = static_cast<cudaStream_t>(o.stream);
-    // threads that fit with 16 bytes of every row each
-    const int turn_threads = (int)std::max<size_t>(32, std::min<size_t>(256, 3072 / o.beams / 32 * 32));
+    // threads that fit into 48 KB with 16 bytes of every row each
+    const int turn_threads = (int)std::max<size_t>(32, std::min<size_t>(256, 49152 / (16 * o.beams) / 32 * 32));
     States move{}, turn{};
     unsigned long long move_units = 0, turn_units = 0;
     auto flush_move = [&] {

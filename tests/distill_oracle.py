@@ -159,6 +159,9 @@ def select(x, beam_scores, width, *, ids=None, scale=1.0, normalise=True, allowe
         p = np.concatenate([np.full(len(r[0]), r[1]) for r in rows])
         c = np.concatenate([r[2] for r in rows])
         d = np.concatenate([np.full(len(r[0]), r[3]) for r in rows])
+        if len(v) > width:  # (all that equal the width-th stay)
+            near = v >= np.partition(v, len(v) - width)[len(v) - width]
+            v, p, c, d = v[near], p[near], c[near], d[near]
         order = np.lexsort((c, p, -v))[:width]
         m = len(order)
         name = c[order] if ids is None else ids[i, p[order], c[order]]

@@ -91,6 +91,37 @@ def test_select(dtype, g, b, n, w, mask, ended, ids, pad, shift, normalise):
                        end_id=end))
 
 
+@pytest.mark.parametrize("normalise", [True, False])
+@pytest.mark.parametrize("dtype,b,n,w", [("f32", 32, 131072, 2), ("f32", 16, 140000, 3),
+                                         ("bf16", 1, 4900000, 1), ("bf16", 1, 2500000, 3),
+                                         ("f16", 64, 80000, 1), ("f32", 128, 270001, 10)])
+def test_more_lists_than_threads(dtype, b, n, w, normalise):
+    """One search's chains in so many parts that a block of 256 threads joins more lists
+    than that, of few columns each."""
+    import forgegpu as fg
+    import torch
+    x, bs, _, _, _ = problem(1, b, n, "none", False, False, b + n)
+    X, x = put(x, dtype, 0, 0)
+    r = fg.beam_select(X, torch.from_numpy(bs).cuda(), width=w, normalise=normalise)
+    check(r, do.select(x, bs, w, normalise=normalise), n)
+
+
+def test_more_lists_than_a_round():
+    """128 chains of nine parts: 1152 lists.  Without normalisers and with equal scores of
+    the chains the best are the largest columns, in order."""
+    import forgegpu as fg
+    import torch
+    b, n, w = 128, 1060000, 40
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn((1, b, n), device="cuda", generator=gen)
+    r = fg.beam_select(x, torch.zeros((1, b), device="cuda"), width=w, normalise=False)
+    flat = x.view(-1)
+    at = (flat >= flat.topk(w).values[-1]).nonzero().view(-1)
+    at = at[flat[at].sort(descending=True, stable=True).indices][:w]
+    assert torch.equal(r.scores[0], flat[at])
+    assert torch.equal(r.parents[0], at // n) and torch.equal(r.ids[0], at % n)
+
+
 @pytest.mark.parametrize("dtype,g,b,n,w", [("f32", 2, 4, 10000, 4), ("bf16", 3, 8, 30000, 8),
                                            ("f16", 1, 16, 5000, 16), ("f32", 1, 64, 3000, 64)])
 @pytest.mark.parametrize("kind", ["same", "rising", "falling", "steps", "few values"])
