@@ -167,19 +167,6 @@ __global__ void __launch_bounds__(TH) loss_kernel(const LossArgs p) {
     const float* z = p.t.z + (size_t)q * p.t.ld;
     if (tid == 0) count = 0;
     for (int c = tid; c < p.d; c += TH) qs[c] = to_f32<T>(qp[c]);
-    // ---- the pass's sums (see finish_kernel): a thread's share ----
-    const sr::Parts& ps = p.parts;
-    float M = -INFINITY;
-    double L = 0.0;
-    for (int i = tid; i < ps.parts; i += TH) {
-        const float4 v = ps.part[(size_t)i * ps.nq + ql];
-        if (v.y == 0.0f && v.z == 0.0f) continue;
-        if (v.x > M) {
-            if (L != 0.0) L *= (double)sr::ex2(M - v.x);
-            M = v.x;
-        }
-        L += v.z == v.z ? (double)(v.y * (v.x == M ? 1.0f : sr::ex2(v.x - M))) : NAN;
-    }
     read_entries<TH>(p.t, q, raw, row);
     for (int e = tid; e < p.t.k; e += TH)
         if (row[e] >= 0) list[atomicAdd(&count, 1)] = e;
@@ -233,6 +220,21 @@ __global__ void __launch_bounds__(TH) loss_kernel(const LossArgs p) {
 #pragma unroll
         for (int r = 0; r < ROWS; ++r)
             if (sub == 0 && i + r * per < named) score[list[i + r * per]] = acc[r] * (double)p.scale;
+    }
+    // ---- the pass's sums (see finish_kernel): a thread's share ----
+    // (until here nothing of the pass was read: blocks that found room were ahead of it)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const sr::Parts& ps = p.parts;
+    float M = -INFINITY;
+    double L = 0.0;
+    for (int i = tid; i < ps.parts; i += TH) {
+        const float4 v = ps.part[(size_t)i * ps.nq + ql];
+        if (v.y == 0.0f && v.z == 0.0f) continue;
+        if (v.x > M) {
+            if (L != 0.0) L *= (double)sr::ex2(M - v.x);
+            M = v.x;
+        }
+        L += v.z == v.z ? (double)(v.y * (v.x == M ? 1.0f : sr::ex2(v.x - M))) : NAN;
     }
     __syncthreads();
 
@@ -400,8 +402,15 @@ static void launch_loss(cudaStream_t s, int device, const LossArgs& p) {
         static std::atomic<uint64_t> done{0};
         sr::allow_smem(loss_kernel<T, TH>, device, FDB_MAX_SOFTMAX_DIM * 4, done);
     }
-    loss_kernel<T, TH><<<p.parts.nq, TH, smem, s>>>(p);
-    FDB_LAUNCH_CHECK();
+    // (launched while the pass runs)
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t how{};
+    how.gridDim = dim3((unsigned)p.parts.nq), how.blockDim = dim3(TH);
+    how.dynamicSmemBytes = smem, how.stream = s;
+    how.attrs = &attr, how.numAttrs = 1;
+    FDB_CUDA(cudaLaunchKernelEx(&how, loss_kernel<T, TH>, p));
 }
 template <typename T>
 static void launch_loss(cudaStream_t s, int device, int sms, const LossArgs& p) {

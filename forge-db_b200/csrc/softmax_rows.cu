@@ -1080,6 +1080,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     cluster_sync();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    // (see few_kernel)
+    if (MODE == STATS) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int units = PROD ? g.mt * g.nt * g.chunks : g.mt * g.chunks;
     int last_stage = -1;  // MMA issuer: last stage committed, and its phase
     uint32_t last_phase = 0;
@@ -1387,6 +1389,8 @@ __global__ void __launch_bounds__(64)
                size_t ldq, int nq, float rf, const uint32_t* __restrict__ allowed,
                size_t ld_allowed, float4* __restrict__ part, float2* __restrict__ top,
                size_t groups, float* __restrict__ size, int* __restrict__ err) {
+    // (a kernel launched to overlap waits for this grid's results itself)
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (blockIdx.x == 0 && threadIdx.x == 0) *err = 0;  // (this path has no waits)
     constexpr int V = 16 / (int)sizeof(T);
     constexpr int RB = 8;
