@@ -309,6 +309,7 @@ __global__ void __launch_bounds__(TH) grad_kernel(const CoefArgs p) {
     __shared__ int raw[MAXK], row[MAXK];
     __shared__ double sums[TH / 32];
     __shared__ float maxima[TH / 32];
+    sr::wait_for_last();
     const int tid = threadIdx.x, q = blockIdx.x;
     if (q == 0)
         for (int i = tid; i < p.head.words; i += TH) p.head.clear[i] = 0u;
@@ -402,15 +403,7 @@ static void launch_loss(cudaStream_t s, int device, const LossArgs& p) {
         static std::atomic<uint64_t> done{0};
         sr::allow_smem(loss_kernel<T, TH>, device, FDB_MAX_SOFTMAX_DIM * 4, done);
     }
-    // (launched while the pass runs)
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t how{};
-    how.gridDim = dim3((unsigned)p.parts.nq), how.blockDim = dim3(TH);
-    how.dynamicSmemBytes = smem, how.stream = s;
-    how.attrs = &attr, how.numAttrs = 1;
-    FDB_CUDA(cudaLaunchKernelEx(&how, loss_kernel<T, TH>, p));
+    sr::launch(true, s, loss_kernel<T, TH>, p.parts.nq, TH, smem, p);
 }
 template <typename T>
 static void launch_loss(cudaStream_t s, int device, int sms, const LossArgs& p) {

@@ -388,6 +388,7 @@ __device__ __forceinline__ unsigned pack_short(const PackSide& p, int row0, int 
 template <typename T, int PARTS>
 __global__ void __launch_bounds__(256)
     pack_kernel(const PackSide a, const PackSide b, int d, int kp, int* err) {
+    wait_for_last();
     if (err && blockIdx.x == 0 && threadIdx.x == 0) *err = 0;
     const bool first = (int)blockIdx.x < a.blocks;
     const PackSide& p = first ? a : b;
@@ -1080,8 +1081,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     cluster_sync();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    // (see few_kernel)
-    if (MODE == STATS) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    wait_for_last();
     const int units = PROD ? g.mt * g.nt * g.chunks : g.mt * g.chunks;
     int last_stage = -1;  // MMA issuer: last stage committed, and its phase
     uint32_t last_phase = 0;
@@ -1389,8 +1389,7 @@ __global__ void __launch_bounds__(64)
                size_t ldq, int nq, float rf, const uint32_t* __restrict__ allowed,
                size_t ld_allowed, float4* __restrict__ part, float2* __restrict__ top,
                size_t groups, float* __restrict__ size, int* __restrict__ err) {
-    // (a kernel launched to overlap waits for this grid's results itself)
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    wait_for_last();
     if (blockIdx.x == 0 && threadIdx.x == 0) *err = 0;  // (this path has no waits)
     constexpr int V = 16 / (int)sizeof(T);
     constexpr int RB = 8;
@@ -2154,6 +2153,7 @@ __global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kern
 __global__ void __launch_bounds__(1024)
     any_kernel(const uint32_t* __restrict__ allowed, size_t ld, int nq, size_t words,
                uint32_t* __restrict__ out) {
+    wait_for_last();
     __shared__ uint32_t part[32][33];
     const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
     const size_t w = (size_t)blockIdx.x * 32 + lane;
@@ -2230,6 +2230,7 @@ __device__ __forceinline__ Coef coef_of(const CoefArgs& a, int i, double f, doub
 __global__ void head_kernel(const CoefArgs a, uint32_t* __restrict__ alive,
                             int* __restrict__ weight, uint32_t* __restrict__ head,
                             int head_words) {
+    wait_for_last();
     const int q = blockIdx.x * blockDim.x + threadIdx.x;
     if (q < head_words) head[q] = 0u;
     bool on = false;
@@ -2263,6 +2264,9 @@ __global__ void __launch_bounds__(256)
                   const int* __restrict__ weight, __half* __restrict__ qs,
                   float* __restrict__ out_f, __half* __restrict__ xp, float* __restrict__ xf,
                   int kp, int parts, int qblocks, const GradHead* __restrict__ head) {
+    wait_for_last();
+    qp = here(qp), qf = here(qf), weight = here(weight), xp = here(xp), xf = here(xf);
+    head = here(head);
     const int lane = threadIdx.x & 31;
     const float mx = head->x_most;
     const int lx = mx > 0.0f ? ilogbf(mx) : 0;
@@ -2330,6 +2334,7 @@ struct GivenArgs {
     int* rest_row;
 };
 __global__ void __launch_bounds__(256) given_kernel(const GivenArgs p) {
+    wait_for_last();
     const int lane = threadIdx.x & 31, q = blockIdx.x * 8 + (threadIdx.x >> 5);
     if (q >= p.nq) return;
     const int e = p.weight[q];
@@ -2376,6 +2381,8 @@ __global__ void __launch_bounds__(256)
     join_kernel(const float* __restrict__ partial, int splits, int rows, int cols,
                 const float* __restrict__ f, const GradHead* __restrict__ head, void* out,
                 size_t ldo, int dtype, const JoinRest rest) {
+    wait_for_last();
+    partial = here(partial), f = here(f), head = here(head);
     constexpr int LANES = 256 / TURNS;
     __shared__ float4 part[TURNS][LANES];
     const unsigned per4 = (unsigned)(cols + 3) / 4;
@@ -2437,12 +2444,11 @@ static void launch_join(cudaStream_t s, int sms, const float* partial, int split
                         int cols, const float* f, const GradHead* head, void* out, size_t ldo,
                         int dtype, const JoinRest& rest = JoinRest{}) {
     if (splits >= 16)
-        join_kernel<8><<<sms * 8, 256, 0, s>>>(partial, splits, rows, cols, f, head, out, ldo,
-                                               dtype, rest);
+        launch(true, s, join_kernel<8>, sms * 8, 256, 0, partial, splits, rows, cols, f, head, out,
+               ldo, dtype, rest);
     else
-        join_kernel<1><<<sms * 8, 256, 0, s>>>(partial, splits, rows, cols, f, head, out, ldo,
-                                               dtype, rest);
-    FDB_LAUNCH_CHECK();
+        launch(true, s, join_kernel<1>, sms * 8, 256, 0, partial, splits, rows, cols, f, head, out,
+               ldo, dtype, rest);
 }
 // ---------------------------------------------------------------------------
 // the gradient for a few queries: one pass over the rows on the FMA pipes
@@ -2487,6 +2493,7 @@ __device__ __forceinline__ int few_at(int c) {
 // them (at most 256 a query) and lays those of the block's rows over the others.
 template <typename T, int NQ, bool GIVEN>
 __global__ void __launch_bounds__(256, few_per_sm(NQ)) few_grad_kernel(const FewGrad<T> p) {
+    wait_for_last();
     extern __shared__ float4 few_raw[];
     const int d = p.d, ct_n = (d + 3) / 4, dp = (d + 63) & ~63;
     float* qs = reinterpret_cast<float*>(few_raw);                  // [NQ][dp], see few_at
@@ -2686,6 +2693,7 @@ __global__ void __launch_bounds__(256, few_per_sm(NQ)) few_grad_kernel(const Few
 // A call whose waits ran out has no gradient: NaN.
 __global__ void void_kernel(const int* err, void* dq, size_t ldq, int nq, void* dx, size_t ldx,
                             int n, int cols, int dtype) {
+    wait_for_last();
     if (*err == 0) return;
     const size_t step = (size_t)gridDim.x * 256, i0 = (size_t)blockIdx.x * 256 + threadIdx.x;
     if (dq)
@@ -2803,7 +2811,7 @@ static unsigned blocks_of(int sms, long long units) {
     return 2 * (unsigned)std::min<long long>(units, sms / 2);
 }
 template <int MODE, bool TWO, bool BLK>
-static void launch_rows(cudaStream_t s, int device, int sms, const CUtensorMap& a,
+static void launch_rows(bool over, cudaStream_t s, int device, int sms, const CUtensorMap& a,
                         const CUtensorMap& b, const Mma& g,
                         const typename EpilogueOf<MODE, TWO, BLK>::Type::Args& p,
                         const CUtensorMap* out = nullptr) {
@@ -2813,9 +2821,8 @@ static void launch_rows(cudaStream_t s, int device, int sms, const CUtensorMap& 
     const size_t smem = smem_of(TWO, BLK, MODE == GRAD);
     static std::atomic<uint64_t> done{0};
     allow_smem(rows_kernel<MODE, TWO, BLK>, device, smem, done);
-    rows_kernel<MODE, TWO, BLK><<<blocks_of(sms, units), THREADS, smem, s>>>(a, b, out ? *out : a,
-                                                                             g, p);
-    FDB_LAUNCH_CHECK();
+    launch(over, s, rows_kernel<MODE, TWO, BLK>, blocks_of(sms, units), THREADS, smem, a, b,
+           out ? *out : a, g, p);
 }
 // A's K steps stay in shared memory where they fill at most half of the ring
 // (4096 x 262144 x 96 f32: a tile's copies shrink to a third).
@@ -2825,8 +2832,8 @@ static int stays(bool two, bool blk, bool grad, int atoms) {
 template <int MODE>
 static void launch_product(bool two, cudaStream_t s, int device, int sms, const CUtensorMap& a,
                            const CUtensorMap& b, const Mma& g, const ProdArgs& p) {
-    if (two) launch_rows<MODE, true, true>(s, device, sms, a, b, g, p);
-    else launch_rows<MODE, false, false>(s, device, sms, a, b, g, p);
+    if (two) launch_rows<MODE, true, true>(true, s, device, sms, a, b, g, p);
+    else launch_rows<MODE, false, false>(true, s, device, sms, a, b, g, p);
 }
 
 static PackSide pack_side(const void* x, size_t ld, size_t n, size_t dim, int dtype,
@@ -2840,14 +2847,12 @@ static PackSide pack_side(const void* x, size_t ld, size_t n, size_t dim, int dt
     p.blocks = (int)((n + 8 * p.rows - 1) / (8 * p.rows));
     return p;
 }
-static void launch_pack(cudaStream_t s, int dtype, const PackSide& a, const PackSide& b, size_t d,
+static void launch_pack(bool over, cudaStream_t s, int dtype, const PackSide& a, const PackSide& b, size_t d,
                         size_t kp, int* err) {
-    const unsigned blocks = (unsigned)(a.blocks + b.blocks);
-    const int D = (int)d, K = (int)kp;
-    if (dtype == FDB_DTYPE_F32) pack_kernel<float, 2><<<blocks, 256, 0, s>>>(a, b, D, K, err);
-    else if (dtype == FDB_DTYPE_F16) pack_kernel<__half, 1><<<blocks, 256, 0, s>>>(a, b, D, K, err);
-    else pack_kernel<__nv_bfloat16, 1><<<blocks, 256, 0, s>>>(a, b, D, K, err);
-    FDB_LAUNCH_CHECK();
+    const auto kernel = dtype == FDB_DTYPE_F32   ? pack_kernel<float, 2>
+                        : dtype == FDB_DTYPE_F16 ? pack_kernel<__half, 1>
+                                                 : pack_kernel<__nv_bfloat16, 1>;
+    launch(over, s, kernel, a.blocks + b.blocks, 256, 0, a, b, (int)d, (int)kp, err);
 }
 
 // The forward pass's workspace and launch shape.
@@ -3036,7 +3041,7 @@ void forward_run(Ctx& c, const fdb_logprob_args& given, ForwardEnd* end) {
         const void *qb = a.queries, *xb = a.rows;
         size_t ldq = a.ld_queries, ldx = a.ld_rows, inner = a.dim;
         if (w.packed) {
-            launch_pack(s, a.dtype,
+            launch_pack(false, s, a.dtype,
                         pack_side(a.queries, a.ld_queries, a.nq, a.dim, a.dtype, nullptr,
                                   static_cast<__half*>(w.qp), w.qf, nullptr),
                         pack_side(a.rows, a.ld_rows, a.n, a.dim, a.dtype, nullptr,
@@ -3082,14 +3087,16 @@ void forward_run(Ctx& c, const fdb_logprob_args& given, ForwardEnd* end) {
             p.top = w.top;
             p.groups = w.groups;
             p.size = w.size;
+            // (before the first of a call may lie another one's kernel)
+            const bool over = q0 > 0 || filters || w.packed || w.copy_q || w.copy_x;
             if (w.packed && !w.blocks)
-                launch_rows<STATS, true, false>(s, c.device, c.sm_count, amap, bmap, g, p);
+                launch_rows<STATS, true, false>(over, s, c.device, c.sm_count, amap, bmap, g, p);
             else if (w.packed)
-                launch_rows<STATS, true, true>(s, c.device, c.sm_count, amap, bmap, g, p);
+                launch_rows<STATS, true, true>(over, s, c.device, c.sm_count, amap, bmap, g, p);
             else if (w.blocks)
-                launch_rows<STATS, false, true>(s, c.device, c.sm_count, amap, bmap, g, p);
+                launch_rows<STATS, false, true>(over, s, c.device, c.sm_count, amap, bmap, g, p);
             else
-                launch_rows<STATS, false, false>(s, c.device, c.sm_count, amap, bmap, g, p);
+                launch_rows<STATS, false, false>(over, s, c.device, c.sm_count, amap, bmap, g, p);
             FinishArgs f = finish_args(a, w, q0, nq);
             f.parts = g.chunks * 4;
             f.qf = p.qf;
@@ -3193,8 +3200,7 @@ static void launch_few_grad(const Ctx& c, const Backward& w, const FewGrad<T>& p
         allow_smem(few_grad_kernel<T, NQ, GIVEN>, c.device,
                    few_grad_smem(NQ, FEW_GRAD_DIM, sizeof(T)), done);
     }
-    few_grad_kernel<T, NQ, GIVEN><<<w.few_blocks, 256, smem, s>>>(p);
-    FDB_LAUNCH_CHECK();
+    launch(GIVEN, s, few_grad_kernel<T, NQ, GIVEN>, w.few_blocks, 256, smem, p);
 }
 template <typename T, bool GIVEN>
 static void launch_few_grad(const Ctx& c, const Backward& w, const FewGrad<T>& p, cudaStream_t s) {
@@ -3258,24 +3264,21 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a, const GivenRows* given
     const uint32_t* seen = a.allowed;
     if (w.seen) {
         const size_t words = (a.n + 31) / 32;
-        any_kernel<<<(unsigned)((words + 31) / 32), 1024, 0, s>>>(a.allowed, a.ld_allowed, nq,
-                                                                  words, w.seen);
-        FDB_LAUNCH_CHECK();
+        launch(true, s, any_kernel, (words + 31) / 32, 1024, 0, a.allowed, a.ld_allowed, nq, words,
+               w.seen);
         seen = w.seen;
     }
     PackSide qside = pack_side(a.queries, a.ld_queries, a.nq, a.dim, a.dtype, w.alive, w.qp, w.qf,
                                &w.head->q_most);
     qside.weight = w.weight;
     if (given) qside.seen = nullptr, qside.lse = a.lse;
-    launch_pack(s, a.dtype, qside,
+    launch_pack(true, s, a.dtype, qside,
                 pack_side(a.rows, a.ld_rows, a.n, a.dim, a.dtype, seen, w.xp, w.xf,
                           reinterpret_cast<unsigned*>(&w.head->x_most)),
                 a.dim, w.kp, nullptr);
     const int qblocks = (nq + 7) / 8;
-    settle_kernel<<<qblocks + (n + 255) / 256, 256, 0, s>>>(k, w.qp, w.qf, w.weight, w.qs, w.out_f,
-                                                            w.xp, w.xf, (int)w.kp, w.parts, qblocks,
-                                                            w.head);
-    FDB_LAUNCH_CHECK();
+    launch(true, s, settle_kernel, qblocks + (n + 255) / 256, 256, 0, k, w.qp, w.qf, w.weight, w.qs,
+           w.out_f, w.xp, w.xf, (int)w.kp, w.parts, qblocks, w.head);
 
     const size_t width = w.parts * w.kp;
     const bool two = w.parts == 2;
@@ -3312,16 +3315,15 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a, const GivenRows* given
             p.coef = w.coef, p.xf = w.xf;
             p.allowed = a.allowed, p.ld_allowed = ld_allowed;
             p.ldg = w.ldg, p.nqp = (int)w.nqp, p.rest = w.rest;
-            if (two) launch_rows<GRAD, true, true>(s, c.device, c.sm_count, qk, xk, g, p, &go);
+            if (two) launch_rows<GRAD, true, true>(true, s, c.device, c.sm_count, qk, xk, g, p, &go);
             else if (w.blocks)
-                launch_rows<GRAD, false, true>(s, c.device, c.sm_count, qk, xk, g, p, &go);
-            else launch_rows<GRAD, false, false>(s, c.device, c.sm_count, qk, xk, g, p, &go);
+                launch_rows<GRAD, false, true>(true, s, c.device, c.sm_count, qk, xk, g, p, &go);
+            else launch_rows<GRAD, false, false>(true, s, c.device, c.sm_count, qk, xk, g, p, &go);
         }
         if (given) {
             const GivenArgs p{*given, nq, w.weight, w.xf, w.gr, w.ldg, (int)w.nqp, w.parts,
                               (int)j0, cols, j0 == 0 ? w.rest : nullptr, w.rest_row};
-            given_kernel<<<(nq + 7) / 8, 256, 0, s>>>(p);
-            FDB_LAUNCH_CHECK();
+            launch(true, s, given_kernel, (nq + 7) / 8, 256, 0, p);
         }
         if (a.d_queries) {
             Mma g = base;
@@ -3365,9 +3367,8 @@ void backward_run(Ctx& c, const fdb_logprob_grad_args& a, const GivenRows* given
         launch_join(s, c.sm_count, w.dq, w.q_splits, nq, d, w.out_f, nullptr, a.d_queries,
                     a.ld_d_queries, a.dtype, rest);
     }
-    void_kernel<<<c.sm_count, 256, 0, s>>>(w.err, a.d_queries, a.ld_d_queries, nq, a.d_rows,
-                                           a.ld_d_rows, n, d, a.dtype);
-    FDB_LAUNCH_CHECK();
+    launch(true, s, void_kernel, c.sm_count, 256, 0, w.err, a.d_queries, a.ld_d_queries, nq, a.d_rows,
+           a.ld_d_rows, n, d, a.dtype);
 }
 
 // One thread per row: its id among the sorted wanted ones, the lowest row kept.

@@ -115,6 +115,35 @@ static void allow_smem(K* kernel, int device, size_t bytes, std::atomic<uint64_t
     if (device < 64) done.fetch_or(1ull << device, std::memory_order_release);
 }
 
+// Kernels that follow one another in a call overlap: the next one's blocks take their
+// places while the last one's end (some 2 us a launch).  Each of them waits, before it
+// reads or writes anything that another one does, for all before it to be done: with
+// one that did not, those after it would not know of those before.  What one of them
+// left must not be read through a pointer that the compiler knows as the kernel's own
+// (`const __restrict__`), as such a load may move ahead of the wait: see here().
+__device__ __forceinline__ void wait_for_last() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+template <typename T>
+__device__ __forceinline__ T* here(T* p) {
+    asm volatile("" : "+l"(p)::"memory");
+    return p;
+}
+// `over`: overlapping with the kernel before it, which is the same call's.
+template <typename... P, typename... A>
+static void launch(bool over, cudaStream_t s, void (*kernel)(P...), size_t blocks, int threads,
+                   size_t smem, const A&... args) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t how{};
+    how.gridDim = dim3((unsigned)blocks), how.blockDim = dim3((unsigned)threads);
+    how.dynamicSmemBytes = smem, how.stream = s;
+    how.attrs = &attr, how.numAttrs = over ? 1 : 0;
+    FDB_CUDA(cudaLaunchKernelEx(&how, kernel, static_cast<P>(args)...));
+}
+
 inline size_t up(size_t v, size_t m) { return (v + m - 1) / m * m; }
 // Hands out 256-byte aligned parts of the caller's workspace.
 struct Carve {
