@@ -127,6 +127,7 @@ __global__ void __launch_bounds__(128)
         const int r = entry_row(t, q, e);
         if (r >= 0) atomicAnd(o + (r >> 5), ~(1u << (r & 31)));
     }
+    sr::wait_for_last();  // (beside the packing of the rows)
 }
 
 struct LossArgs {
@@ -424,11 +425,10 @@ struct End : sr::ForwardEnd {
         : c(c_), a(a_), plan(p), s(static_cast<cudaStream_t>(a_.stream)) {
         queries = p.queries;
     }
-    const uint32_t* filters(size_t q0, size_t nq) override {
+    const uint32_t* filters(size_t q0, size_t nq, bool over) override {
         const Teacher t = teacher_of(a);
         if (!a.rest) return a.allowed + q0 * a.ld_allowed;
-        filter_kernel<<<(unsigned)nq, 128, 0, s>>>(t, (int)q0, plan.filters, plan.words);
-        FDB_LAUNCH_CHECK();
+        sr::launch(over, s, filter_kernel, nq, 128, 0, t, (int)q0, plan.filters, plan.words);
         return plan.filters;
     }
     void finish(const sr::Parts& parts) override {

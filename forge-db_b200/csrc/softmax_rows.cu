@@ -388,14 +388,15 @@ __device__ __forceinline__ unsigned pack_short(const PackSide& p, int row0, int 
 template <typename T, int PARTS>
 __global__ void __launch_bounds__(256)
     pack_kernel(const PackSide a, const PackSide b, int d, int kp, int* err) {
-    wait_for_last();
     if (err && blockIdx.x == 0 && threadIdx.x == 0) *err = 0;
     const bool first = (int)blockIdx.x < a.blocks;
     const PackSide& p = first ? a : b;
+    if (p.seen || p.lse || p.weight) wait_for_last();  // (others: beside the kernel before it)
     const int row = (((int)blockIdx.x - (first ? 0 : a.blocks)) * 8 + (threadIdx.x >> 5)) * p.rows;
     const unsigned mine = row >= p.n      ? 0u
                           : p.rows == 4 ? pack_short<T, PARTS>(p, row, d, kp)
                                         : pack_row<T, PARTS>(p, row, d, kp);
+    wait_for_last();
     if (!p.largest) return;
     // the block's largest, unless it is there already
     __shared__ unsigned most[8];
@@ -2153,7 +2154,6 @@ __global__ void __launch_bounds__(THREADS_, THREADS_ == 128 ? 7 : 1) finish_kern
 __global__ void __launch_bounds__(1024)
     any_kernel(const uint32_t* __restrict__ allowed, size_t ld, int nq, size_t words,
                uint32_t* __restrict__ out) {
-    wait_for_last();
     __shared__ uint32_t part[32][33];
     const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
     const size_t w = (size_t)blockIdx.x * 32 + lane;
@@ -2167,6 +2167,7 @@ __global__ void __launch_bounds__(1024)
     r = __reduce_or_sync(0xffffffffu, part[lane][row]);
     const size_t o = (size_t)blockIdx.x * 32 + row;
     if (lane == 0 && o < words) out[o] = r;
+    wait_for_last();  // (beside the kernel before it)
 }
 struct CoefArgs {
     int nq, n;
@@ -3030,7 +3031,7 @@ void forward_run(Ctx& c, const fdb_logprob_args& given, ForwardEnd* end) {
     const Forward w = plan_forward(c, a, end ? end->queries : 0);
     // (few queries are one pass)
     const bool filters = end && a.allowed && a.ld_allowed;
-    if (filters && w.few) a.allowed = end->filters(0, a.nq);
+    if (filters && w.few) a.allowed = end->filters(0, a.nq, false);
     const int n = (int)a.n, d = (int)a.dim;
     const float rf = (float)((double)a.scale * LOG2E);
     const size_t ld_allowed = a.allowed ? a.ld_allowed : 0;
@@ -3081,14 +3082,14 @@ void forward_run(Ctx& c, const fdb_logprob_args& given, ForwardEnd* end) {
             p.qf = w.packed ? w.qf + q0 : nullptr;
             p.xf = w.xf;
             p.rf = rf;
-            p.allowed = filters ? end->filters(q0, nq) : a.allowed;
+            bool over = q0 > 0 || w.packed || w.copy_q || w.copy_x;
+            p.allowed = filters ? end->filters(q0, nq, over) : a.allowed;
+            over |= filters;
             p.ld_allowed = ld_allowed;
             p.part = w.part;
             p.top = w.top;
             p.groups = w.groups;
             p.size = w.size;
-            // (before the first of a call may lie another one's kernel)
-            const bool over = q0 > 0 || filters || w.packed || w.copy_q || w.copy_x;
             if (w.packed && !w.blocks)
                 launch_rows<STATS, true, false>(over, s, c.device, c.sm_count, amap, bmap, g, p);
             else if (w.packed)

@@ -74,8 +74,8 @@ struct Parts {
 struct ForwardEnd {
     size_t queries;  // of one pass at most
     // Before a pass, if the call has filters of a query each (ld_allowed > 0):
-    // those of its queries, the first one's first.
-    virtual const uint32_t* filters(size_t q0, size_t nq) = 0;
+    // those of its queries, the first one's first (`over`: see launch()).
+    virtual const uint32_t* filters(size_t q0, size_t nq, bool over) = 0;
     virtual void finish(const Parts& p) = 0;
 };
 // Score gradients at given rows, in the place of what backward_run's formula
@@ -116,7 +116,7 @@ static void allow_smem(K* kernel, int device, size_t bytes, std::atomic<uint64_t
 }
 
 // Kernels that follow one another in a call overlap: the next one's blocks take their
-// places while the last one's end (some 2 us a launch).  Each of them waits, before it
+// places while the last one's end (some 1.5 us a launch).  Each of them waits, before it
 // reads or writes anything that another one does, for all before it to be done: with
 // one that did not, those after it would not know of those before.  What one of them
 // left must not be read through a pointer that the compiler knows as the kernel's own
