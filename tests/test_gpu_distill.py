@@ -493,6 +493,63 @@ def test_same_call_same_bits_in_graphs_and_on_streams():
     assert same(graphs[0][1], one()) and same(graphs[1][1], two())
 
 
+@pytest.mark.parametrize("dtype,nq,n,dim,mask,rest", [
+    ("f32", 1, 10000, 128, "none", False), ("f32", 8, 20000, 64, "each", True),
+    ("f32", 300, 9000, 130, "each", True), ("bf16", 40, 5000, 96, "each", True),
+    ("bf16", 200, 3000, 65, "none", False), ("f16", 700, 400, 256, "one", True)])
+def test_inputs_written_just_before(dtype, nq, n, dim, mask, rest):
+    """Kernels of a call overlap, a call and what wrote its inputs do not: calls behind
+    writes to their inputs leave what they leave when all is waited for, eager and
+    captured with the writes."""
+    import forgegpu as fg
+    import torch
+    sets = []
+    for i in range(4):
+        Q, X, _, A, *_ = make(dtype, nq, n, dim, mask, seed=50 + i)
+        sets.append([Q, X, *cuda(*lists(nq, n, 12, rest, seed=i)), torch.rand(nq, device="cuda")] +
+                    ([] if A is None else [A]))
+    now = [v.clone() for v in sets[0]]
+
+    def call():
+        q, x, ids, z, u = now[:5]
+        A = now[5] if len(now) > 5 else None
+        r = fg.distill(q, x, ids, z, scale=0.1, rest=rest, allowed=A)
+        g = fg.distill_backward(q, x, ids, z, r.lse, r.logprobs, r.rest, d_loss=u, scale=0.1,
+                                allowed=A)
+        return [v for v in (*r, *g) if v is not None]
+
+    def write(i):
+        for v, w in zip(now, sets[i]):
+            v.copy_(w)
+
+    want = []
+    for i in range(4):
+        write(i)
+        torch.cuda.synchronize()
+        want.append(call())
+        torch.cuda.synchronize()
+
+    def run():
+        got = []
+        for i in (1, 3, 0, 2, 3, 1):
+            write(i)
+            got.append((i, call()))
+        return got
+
+    def check_all(got):
+        torch.cuda.synchronize()
+        for i, out in got:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[i])), i
+
+    check_all(run())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = run()
+    for _ in range(3):
+        g.replay()
+        check_all(got)
+
+
 def test_a_wait_that_runs_out(ctx):
     import forgegpu as fg
     import torch
