@@ -1414,6 +1414,10 @@ int fdb_beam_select(fdb_ctx* ctx, const fdb_beam_args* args) {
         FDB_REQUIRE(a.scores && a.beam_scores, FDB_ERR_INVALID_ARG, "NULL argument");
         FDB_REQUIRE(a.out_scores && a.out_parents && a.out_ids, FDB_ERR_INVALID_ARG,
                     "out_scores, out_parents or out_ids is NULL");
+        // (a search's chains are read while others' results are written)
+        FDB_REQUIRE(a.out_scores != a.beam_scores && (!a.ended || a.out_ended != a.ended) &&
+                        (!a.ids || a.out_ids != a.ids) && a.out_ids != a.out_parents,
+                    FDB_ERR_INVALID_ARG, "an output is an input or another output");
         check_aligned(a.scores, a.dtype == FDB_DTYPE_F32 ? 4 : 2, "scores");
         check_aligned(a.ids, 8, "ids");
         check_aligned(a.allowed, 4, "allowed");

@@ -110,7 +110,9 @@ def test_select_refuses(call, change, code, text):
     (dict(ids=260, ld_ids=1000), b"ids"), (dict(beam_scores=514), b"beam_scores"),
     (dict(out_parents=2052), b"out_parents"), (dict(out_ids=4100), b"out_ids"),
     (dict(workspace=None), b"workspace"), (dict(workspace=1024 + 128), b"workspace"),
-    (dict(workspace_bytes=1), b"workspace"),
+    (dict(workspace_bytes=1), b"workspace"), (dict(out_scores=512), b"an output is an input"),
+    (dict(ended=600, out_ended=600), b"an output is an input"),
+    (dict(ids=4096, ld_ids=1000), b"an output is an input"), (dict(out_ids=2048), b"another output"),
 ])
 def test_select_buffers(call, change, text):
     fg, L, ctx = call
