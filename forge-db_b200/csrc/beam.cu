@@ -83,7 +83,7 @@ __device__ __forceinline__ double unordered64(uint64_t u) {
 // time, and leaves their sum of exponentials and the `width` best.  The pass over the
 // columns only adds up and keeps each thread's largest of a span of tiles, without a
 // barrier.  The best are found from those maxima afterwards: of the threads' largest the
-// width-th (or, for few, the least of the largest of G >= width groups of threads) is
+// width-th (or, for 16 at most, the least of the largest of G >= width groups of threads) is
 // reached by at least `width` columns and by hardly more; only the maxima that reach it
 // are looked behind, by reading their columns again.
 // Sums are taken relative to a thread's own largest score so far (raised only when it
@@ -282,13 +282,47 @@ struct ScanShared {
         } e;
     };
     float top[SPANS][TH];  // a thread's largest of each span
-    float warp_min[TH / 32], warp_m[TH / 32], bound;
+    float warp_min[TH / 32], warp_m[TH / 32];
+    uint32_t bound;
     int groups;
     double warp_sum[TH / 32];
 };
 // What a thread's exponents are relative to: 2^(x s - reference).  Below the range
 // where x s stays finite its terms are 0 (finish_kernel takes such sums again).
 __device__ __forceinline__ float reference(float m, float s) { return fmaxf(m * s, -1e30f); }
+// The width-th largest of the threads' values: each warp sorts its own, and a thread looks
+// for its place among the eight (comparing with all took 6 us of a block's end).  Called
+// by all threads, after a barrier.
+template <typename T>
+__device__ __forceinline__ float bound_of_maxima(ScanShared<T>& sh, float most, int width) {
+    uint32_t* sorted = reinterpret_cast<uint32_t*>(sh.e.s.aside);  // [warps][32], falling
+    const int tid = threadIdx.x, lane = tid & 31;
+    uint32_t v = ordered(most);
+#pragma unroll
+    for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+        for (int j = k >> 1; j; j >>= 1) {
+            const uint32_t o = __shfl_xor_sync(0xffffffffu, v, j);
+            v = ((lane & k) == 0) == ((lane & j) == 0) ? max(v, o) : min(v, o);
+        }
+    sorted[tid] = v;
+    if (tid == 0) sh.bound = ~0u;
+    __syncthreads();
+    int above = 0;
+#pragma unroll
+    for (int w = 0; w < TH / 32; ++w) {
+        int at = 0;  // (how many of the warp's are larger)
+#pragma unroll
+        for (int step = 16; step; step >>= 1)
+            if (sorted[w * 32 + at + step - 1] > v) at += step;
+        if (sorted[w * 32 + at] > v) ++at;
+        above += at;
+    }
+    const uint32_t least = __reduce_min_sync(0xffffffffu, above < width ? v : ~0u);
+    if (lane == 0) atomicMin(&sh.bound, least);
+    __syncthreads();
+    return unordered(sh.bound);
+}
 template <typename T, bool NORM, bool GATE>
 __device__ __forceinline__ void scan_part(const Select& p, const Scan& c, ScanShared<T>& sh,
                                           size_t row, int sp, int g, int b) {
@@ -397,28 +431,14 @@ __device__ __forceinline__ void scan_part(const Select& p, const Scan& c, ScanSh
         bound = o < group ? fmaxf(bound, v) : fminf(bound, v);
         if (NORM) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     }
-    float* all_most = reinterpret_cast<float*>(s.aside);
     if ((tid & 31) == 0) sh.warp_min[tid >> 5] = bound, sh.warp_m[tid >> 5] = M;
     const bool bad = __syncthreads_or(!(most < INFINITY));
     if (tid == 0) s.count = 0, s.buf = buf;
     float tau = sh.warp_min[0];
 #pragma unroll
     for (int i = 1; i < TH / 32; ++i) tau = fminf(tau, sh.warp_min[i]);
-    if (p.width > 16) {
-        all_most[tid] = most;
-        __syncthreads();
-        int above = 0, from = 0;
-        const float4* four = reinterpret_cast<const float4*>(all_most);
-#pragma unroll 8
-        for (int i = 0; i < TH / 4; ++i) {
-            const float4 v = four[i];
-            above += (v.x > most) + (v.y > most) + (v.z > most) + (v.w > most);
-            from += (v.x >= most) + (v.y >= most) + (v.z >= most) + (v.w >= most);
-        }
-        if (above < p.width && p.width <= from) sh.bound = most;  // (equal ones all write the same)
-        __syncthreads();
-        tau = sh.bound;
-    }
+    // (or a group has no column, and all columns would reach it)
+    if (p.width > 16 || tau == -INFINITY) tau = bound_of_maxima(sh, most, p.width);
     if (NORM) {
 #pragma unroll
         for (int i = 0; i < TH / 32; ++i) M = fmaxf(M, sh.warp_m[i]);
