@@ -140,20 +140,53 @@ struct LossArgs {
     float *loss, *lse, *logprobs, *rest;
 };
 // Two sums of a vector's products with a query's: of the even and of the odd columns.
-template <typename T>
-__device__ __forceinline__ uint64_t dot_vec(const uint4& v, const float* q, uint64_t sums) {
+template <typename T, typename VT>
+__device__ __forceinline__ uint64_t dot_vec(const VT& v, const float* q, uint64_t sums) {
+    constexpr int V = sizeof(VT) / sizeof(T);
     const T* e = reinterpret_cast<const T*>(&v);
+    if constexpr (V == 1) {
+        sums = sr::packf(__fmaf_rn(to_f32<T>(e[0]), *q, sr::lo_of(sums)), 0.0f);
+    } else if constexpr (V == 2) {
+        const float2 y = *reinterpret_cast<const float2*>(q);
+        sums = tc::fma2(sr::packf(to_f32<T>(e[0]), to_f32<T>(e[1])), sr::packf(y.x, y.y), sums);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 16 / (int)sizeof(T); i += 4) {
-        const float4 y = *reinterpret_cast<const float4*>(q + i);
-        sums = tc::fma2(sr::packf(to_f32<T>(e[i]), to_f32<T>(e[i + 1])), sr::packf(y.x, y.y), sums);
-        sums = tc::fma2(sr::packf(to_f32<T>(e[i + 2]), to_f32<T>(e[i + 3])), sr::packf(y.z, y.w), sums);
+        for (int i = 0; i < V; i += 4) {
+            const float4 y = *reinterpret_cast<const float4*>(q + i);
+            sums = tc::fma2(sr::packf(to_f32<T>(e[i]), to_f32<T>(e[i + 1])), sr::packf(y.x, y.y), sums);
+            sums = tc::fma2(sr::packf(to_f32<T>(e[i + 2]), to_f32<T>(e[i + 3])), sr::packf(y.z, y.w), sums);
+        }
     }
     return sums;
 }
-// One block per query: the pass's sums joined, the named rows scored (sums of up to
-// four 16-byte vectors' products in f32, theirs in 64 bits), the loss.  Gathers k rows
-// a query.
+// Adds a lane's share of the products of ROWS rows with a query, by vectors of VT: f32
+// sums of up to four of them, theirs in 64 bits.
+template <typename T, typename VT, int ROWS>
+__device__ __forceinline__ void dot_rows(const T* const (&x)[ROWS], const float* q, int d, int sub,
+                                         int lanes, double (&acc)[ROWS]) {
+    constexpr int V = sizeof(VT) / sizeof(T), STEPS = 4, AHEAD = sizeof(VT) == 16 ? 2 : 4;
+    int c = sub * V;
+    while (c + V <= d) {
+        uint64_t two[ROWS] = {};
+#pragma unroll AHEAD
+        for (int n = 0; n < STEPS && c + V <= d; ++n, c += lanes * V) {
+            VT v[ROWS];
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) v[r] = __ldg(reinterpret_cast<const VT*>(x[r] + c));
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) two[r] = dot_vec<T, VT>(v[r], q + c, two[r]);
+        }
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) acc[r] += (double)(sr::lo_of(two[r]) + sr::hi_of(two[r]));
+    }
+    // (the row's last, partial vector: one lane's)
+    for (; c < d; ++c)
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) acc[r] += (double)(to_f32<T>(x[r][c]) * q[c]);
+}
+// One block per query: the pass's sums joined, the named rows scored, the loss.  Gathers k
+// rows a query, by vectors of what all rows are aligned to (a call of 2878 lists of 16 rows
+// of 518 f16, aligned to 4 bytes: 62.1 us an element at a time, 59.7 by pairs).
 template <typename T, int TH>
 __global__ void __launch_bounds__(TH) loss_kernel(const LossArgs p) {
     extern __shared__ float4 q_raw[];
@@ -174,8 +207,8 @@ __global__ void __launch_bounds__(TH) loss_kernel(const LossArgs p) {
     __syncthreads();
 
     // ---- the named rows' scores: 8 or 32 lanes a row, four rows at a time ----
-    constexpr int V = 16 / (int)sizeof(T), ROWS = 4;
-    const bool wide = ((reinterpret_cast<uintptr_t>(xp) | (p.ldx * sizeof(T))) & 15) == 0;
+    constexpr int ROWS = 4;
+    const uintptr_t odd = reinterpret_cast<uintptr_t>(xp) | (p.ldx * sizeof(T));
     const int lanes = p.d * (int)sizeof(T) <= 512 ? 8 : 32, sub = tid & (lanes - 1);
     const int named = count, per = TH / lanes;
     for (int i = tid / lanes; i - tid / lanes < named; i += ROWS * per) {
@@ -186,33 +219,10 @@ __global__ void __launch_bounds__(TH) loss_kernel(const LossArgs p) {
             x[r] = xp + (size_t)row[list[min(i + r * per, named - 1)]] * p.ldx;
             acc[r] = 0.0;
         }
-        int c = sub;
-        if (wide) {
-            constexpr int STEPS = 4;
-            for (c = sub * V; c + V <= p.d;) {
-                uint64_t two[ROWS] = {};
-#pragma unroll 2
-                for (int n = 0; n < STEPS && c + V <= p.d; ++n, c += lanes * V) {
-                    uint4 v[ROWS];
-#pragma unroll
-                    for (int r = 0; r < ROWS; ++r)
-                        v[r] = __ldg(reinterpret_cast<const uint4*>(x[r] + c));
-#pragma unroll
-                    for (int r = 0; r < ROWS; ++r) two[r] = dot_vec<T>(v[r], qs + c, two[r]);
-                }
-#pragma unroll
-                for (int r = 0; r < ROWS; ++r) acc[r] += (double)(sr::lo_of(two[r]) + sr::hi_of(two[r]));
-            }
-            // (the row's last, partial vector: one lane's)
-            for (; c < p.d; ++c)
-#pragma unroll
-                for (int r = 0; r < ROWS; ++r) acc[r] += (double)(to_f32<T>(x[r][c]) * qs[c]);
-        } else {
-#pragma unroll 4
-            for (; c < p.d; c += lanes)
-#pragma unroll
-                for (int r = 0; r < ROWS; ++r) acc[r] += (double)(to_f32<T>(x[r][c]) * qs[c]);
-        }
+        if ((odd & 15) == 0) dot_rows<T, uint4>(x, qs, p.d, sub, lanes, acc);
+        else if ((odd & 7) == 0) dot_rows<T, uint2>(x, qs, p.d, sub, lanes, acc);
+        else if (sizeof(T) == 4 || (odd & 3) == 0) dot_rows<T, unsigned>(x, qs, p.d, sub, lanes, acc);
+        else if constexpr (sizeof(T) == 2) dot_rows<T, unsigned short>(x, qs, p.d, sub, lanes, acc);
 #pragma unroll
         for (int o = 16; o; o >>= 1)
             if (o < lanes)
