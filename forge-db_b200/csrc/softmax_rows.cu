@@ -197,7 +197,7 @@ struct PackSide {
     unsigned* largest;   // see most_of, nullable
     const int* weight;   // nullable
     int blocks;          // of 8 warps
-    int rows;            // a warp's: 4 short ones or 1
+    int rows;            // a warp's: 4 short ones (512 bytes at most) or 1
     int wide;            // rows can be read in 16-byte vectors
 };
 // What the largest is taken of: the scales' bits, or, with weights, WEIGHT_ZERO + the
@@ -317,7 +317,8 @@ __device__ __forceinline__ unsigned pack_row(const PackSide& p, int row, int d, 
 }
 // Rows of one vector a lane at most, four at a time: a warp that waits for one
 // such row after the other has too little in flight (262144 x 96 f32: 85 us,
-// four at a time 43).
+// four at a time 43).  Rows that are not aligned are read an element at a time
+// (198627 x 25 f32: 81 us one row at a time, 37 so).
 template <typename T, int PARTS>
 __device__ __forceinline__ unsigned pack_short(const PackSide& p, int row0, int d, int kp) {
     constexpr int V = 16 / (int)sizeof(T), R = 4;
@@ -329,9 +330,15 @@ __device__ __forceinline__ unsigned pack_short(const PackSide& p, int row0, int 
         raw[r] = make_uint4(0, 0, 0, 0);
         const bool use = row < p.n && (!p.seen || (p.seen[row >> 5] >> (row & 31) & 1u)) &&
                          (!p.lse || p.lse[row] != -INFINITY);
-        if (use && c < d)
-            raw[r] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) +
-                                                          (size_t)row * p.ld + c));
+        const T* src = static_cast<const T*>(p.x) + (size_t)row * p.ld + c;
+        if (use && p.wide) {
+            if (c < d) raw[r] = __ldg(reinterpret_cast<const uint4*>(src));
+        } else if (use) {
+            T* e = reinterpret_cast<T*>(&raw[r]);
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (c + j < d) e[j] = __ldg(src + j);
+        }
     }
     float mx[R];
     unsigned most = 0u;
@@ -2844,7 +2851,7 @@ static PackSide pack_side(const void* x, size_t ld, size_t n, size_t dim, int dt
     const size_t es = elem(dtype);
     p.wide = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ld * es & 15) == 0 &&
              (dim * es & 15) == 0;
-    p.rows = p.wide && dim * es <= 512 ? 4 : 1;
+    p.rows = dim * es <= 512 ? 4 : 1;
     p.blocks = (int)((n + 8 * p.rows - 1) / (8 * p.rows));
     return p;
 }
