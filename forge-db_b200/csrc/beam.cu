@@ -217,6 +217,37 @@ __device__ __forceinline__ uint4 load_vec(const Select& p, const T* x, int skip,
     return r;
 }
 
+// The width-th largest of the threads' values (images of `ordered`): each warp sorts its
+// own into `sorted` [TH], a thread looks for its place among the eight.  (Comparing each
+// with all took 6 us of a scan's end.)  *bound is all ones, behind a barrier.
+__device__ __forceinline__ uint32_t width_th(uint32_t v, int width, uint32_t* sorted,
+                                             uint32_t* bound) {
+    const int tid = threadIdx.x, lane = tid & 31;
+#pragma unroll
+    for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+        for (int j = k >> 1; j; j >>= 1) {
+            const uint32_t o = __shfl_xor_sync(0xffffffffu, v, j);
+            v = ((lane & k) == 0) == ((lane & j) == 0) ? max(v, o) : min(v, o);
+        }
+    sorted[tid] = v;  // (falling)
+    __syncthreads();
+    int above = 0;
+#pragma unroll
+    for (int w = 0; w < TH / 32; ++w) {
+        int at = 0;  // (how many of the warp's are larger)
+#pragma unroll
+        for (int step = 16; step; step >>= 1)
+            if (sorted[w * 32 + at + step - 1] > v) at += step;
+        if (sorted[w * 32 + at] > v) ++at;
+        above += at;
+    }
+    const uint32_t least = __reduce_min_sync(0xffffffffu, above < width ? v : ~0u);
+    if (lane == 0) atomicMin(bound, least);
+    __syncthreads();
+    return *bound;
+}
+
 // ---- the best of what lies in shared memory ----
 constexpr int LIMIT = 256;              // keys that are put in order at once
 constexpr int ASIDE = 512;
@@ -290,39 +321,6 @@ struct ScanShared {
 // What a thread's exponents are relative to: 2^(x s - reference).  Below the range
 // where x s stays finite its terms are 0 (finish_kernel takes such sums again).
 __device__ __forceinline__ float reference(float m, float s) { return fmaxf(m * s, -1e30f); }
-// The width-th largest of the threads' values: each warp sorts its own, and a thread looks
-// for its place among the eight (comparing with all took 6 us of a block's end).  Called
-// by all threads, after a barrier.
-template <typename T>
-__device__ __forceinline__ float bound_of_maxima(ScanShared<T>& sh, float most, int width) {
-    uint32_t* sorted = reinterpret_cast<uint32_t*>(sh.e.s.aside);  // [warps][32], falling
-    const int tid = threadIdx.x, lane = tid & 31;
-    uint32_t v = ordered(most);
-#pragma unroll
-    for (int k = 2; k <= 32; k <<= 1)
-#pragma unroll
-        for (int j = k >> 1; j; j >>= 1) {
-            const uint32_t o = __shfl_xor_sync(0xffffffffu, v, j);
-            v = ((lane & k) == 0) == ((lane & j) == 0) ? max(v, o) : min(v, o);
-        }
-    sorted[tid] = v;
-    if (tid == 0) sh.bound = ~0u;
-    __syncthreads();
-    int above = 0;
-#pragma unroll
-    for (int w = 0; w < TH / 32; ++w) {
-        int at = 0;  // (how many of the warp's are larger)
-#pragma unroll
-        for (int step = 16; step; step >>= 1)
-            if (sorted[w * 32 + at + step - 1] > v) at += step;
-        if (sorted[w * 32 + at] > v) ++at;
-        above += at;
-    }
-    const uint32_t least = __reduce_min_sync(0xffffffffu, above < width ? v : ~0u);
-    if (lane == 0) atomicMin(&sh.bound, least);
-    __syncthreads();
-    return unordered(sh.bound);
-}
 template <typename T, bool NORM, bool GATE>
 __device__ __forceinline__ void scan_part(const Select& p, const Scan& c, ScanShared<T>& sh,
                                           size_t row, int sp, int g, int b) {
@@ -335,7 +333,7 @@ __device__ __forceinline__ void scan_part(const Select& p, const Scan& c, ScanSh
     const long long nv = ((long long)p.n + skip + N - 1) / N;
     const int v0 = (int)(nv * sp / c.splits), v1 = (int)(nv * (sp + 1) / c.splits);
     const int tiles = (v1 - v0 + STEP - 1) / STEP, spans = (tiles + SPAN - 1) / SPAN;
-    if (tid == 0) sh.groups = 0;
+    if (tid == 0) sh.groups = 0, sh.bound = ~0u;
 
     // ---- sums, and the largest of each thread's columns of a tile ----
     // Without gates a thread's loads go through its own places of a ring in shared
@@ -438,7 +436,9 @@ __device__ __forceinline__ void scan_part(const Select& p, const Scan& c, ScanSh
 #pragma unroll
     for (int i = 1; i < TH / 32; ++i) tau = fminf(tau, sh.warp_min[i]);
     // (or a group has no column, and all columns would reach it)
-    if (p.width > 16 || tau == -INFINITY) tau = bound_of_maxima(sh, most, p.width);
+    if (p.width > 16 || tau == -INFINITY)
+        tau = unordered(width_th(ordered(most), p.width, reinterpret_cast<uint32_t*>(s.aside),
+                                 &sh.bound));
     if (NORM) {
 #pragma unroll
         for (int i = 0; i < TH / 32; ++i) M = fmaxf(M, sh.warp_m[i]);
@@ -557,21 +557,25 @@ __device__ __forceinline__ void add(Choice& s, double v, int b, int j) {
     s.score[to] = ordered64(v);
     s.at[to] = (uint64_t)b << 32 | (uint32_t)j;
 }
-// The width-th largest of s.set[0, n), n <= TH (-inf if there are fewer): the least of
-// those that fewer than `width` are above.  Called by all threads, after a barrier;
-// s.bound is all ones.
+// The width-th largest of s.set[0, n), n <= TH (-inf if there are fewer).  Called by all
+// threads, after a barrier; s.bound is all ones.
 __device__ __forceinline__ float bound_of(Choice& s, int n, int width) {
-    const int tid = threadIdx.x;
     if (n < width) return -INFINITY;
-    if (tid < n) {
-        const float v = s.set[tid];
-        int above = 0;
+    const int tid = threadIdx.x;
+    if (n <= 32) {  // (a few comparisons are done sooner)
+        if (tid < n) {
+            const float v = s.set[tid];
+            int above = 0;
 #pragma unroll 8
-        for (int i = 0; i < n; ++i) above += s.set[i] > v;
-        if (above < width) atomicMin(&s.bound, ordered(v));
+            for (int i = 0; i < n; ++i) above += s.set[i] > v;
+            if (above < width) atomicMin(&s.bound, ordered(v));
+        }
+        __syncthreads();
+        return unordered(s.bound);
     }
-    __syncthreads();
-    return unordered(s.bound);
+    // (what is sorted takes its places)
+    return unordered(width_th(tid < n ? ordered(s.set[tid]) : 0u, width,
+                              reinterpret_cast<uint32_t*>(s.set), &s.bound));
 }
 // Of the candidates that the threads hold (-inf: none) those not `slack` below the
 // width-th of s.set[0, n) are added.
@@ -768,7 +772,7 @@ __device__ __forceinline__ void finish_search(const Select& p, const Scan& c, Fi
     double *sum = f.sum, *lse = f.lse;
     float* top = f.top;
     unsigned char *kind = f.kind, *close = f.close, *sure = f.sure;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, S = c.splits;
+    const int tid = threadIdx.x, S = c.splits;
     const size_t row0 = (size_t)g * p.beams;
     // ---- the lists, if a thread can hold its share of them: on their way while the
     // chains are looked at (what a chain without columns left is not used) ----
@@ -785,48 +789,56 @@ __device__ __forceinline__ void finish_search(const Select& p, const Scan& c, Fi
             count[h] = c.part[row0 * S + k / p.width].count;
         }
     }
-    // ---- the chains: a warp each ----
+    // ---- the chains: as many lanes each as they have parts ----
     bool bad = false, again = false;
-    for (int b = warp; b < p.beams; b += TH / 32) {
-        const float given = p.beam_scores[row0 + b];
-        const Part mine = c.part[(row0 + b) * S + min(lane, S - 1)];
-        const int k = over(p, g, b) ? OVER : LIVE;
+    int lanes = 1;
+    while (lanes < 32 && lanes < S) lanes *= 2;
+    for (int b0 = 0; b0 < p.beams; b0 += TH / lanes) {
+        const int b = b0 + tid / lanes, lane = tid & (lanes - 1);
+        const bool here = b < p.beams;
+        const float given = here ? p.beam_scores[row0 + b] : -INFINITY;
+        Part mine{0.0, -INFINITY, 0};
+        if (here && lane < S) mine = c.part[(row0 + b) * S + lane];
+        const int k = here && over(p, g, b) ? OVER : LIVE;
         bad |= !(given < INFINITY);
         double L = 0.0;
         float M = -INFINITY;
         const bool live = k == LIVE && given > -INFINITY;
-        bool lost = false, odd = false;  // (columns, but a sum of 0, or none in f32)
-        if (live) {
-            for (int i = lane; i < S; i += 32) {
-                const Part q = i < 32 ? mine : c.part[(row0 + b) * S + i];
+        int some = 0;  // 1: columns, 2: a sum that is none in f32
+        if (live)
+            for (int i = lane; i < S; i += lanes) {
+                const Part q = i < lanes ? mine : c.part[(row0 + b) * S + i];
                 bad |= q.count < 0;
                 if (NORM && q.sum > 0.0) M = fmaxf(M, q.m);
-                lost |= q.count > 0;
-                odd |= !(q.sum == q.sum);
+                some |= (q.count > 0 ? 1 : 0) | (q.sum == q.sum ? 0 : 2);
             }
-            if (NORM) {
-#pragma unroll
-                for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-                for (int i = lane; i < S; i += 32) {
-                    const Part q = i < 32 ? mine : c.part[(row0 + b) * S + i];
-                    if (q.sum > 0.0) L += q.sum * exp(((double)q.m - (double)M) * p.scale);
+        bool lost = false;  // (columns, but a sum of 0 or none)
+        if (NORM) {
+            for (int o = lanes / 2; o; o >>= 1) {
+                M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+                some |= __shfl_xor_sync(0xffffffffu, some, o);
+            }
+            if (live)
+                for (int i = lane; i < S; i += lanes) {
+                    const Part q = i < lanes ? mine : c.part[(row0 + b) * S + i];
+                    if (q.sum > 0.0)
+                        L += q.m == M ? q.sum : q.sum * exp(((double)q.m - (double)M) * p.scale);
                 }
-#pragma unroll
-                for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-                odd = __any_sync(0xffffffffu, odd);
-                lost = __any_sync(0xffffffffu, lost) && (odd || !(L > 0.0));
-                if (lost) M = -INFINITY;
-                if (lost) {  // (scores out of f32's range: relative to their largest, in 64 bits)
-                    for (int i = lane; i < S; i += 32)
+            for (int o = lanes / 2; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+            lost = (some & 1) && ((some & 2) || !(L > 0.0));
+            if (__any_sync(0xffffffffu, lost)) {
+                // (scores out of f32's range: relative to their largest, in 64 bits)
+                if (lost) {
+                    M = -INFINITY;
+                    for (int i = lane; i < S; i += lanes)
                         if (c.part[(row0 + b) * S + i].count > 0)
                             M = fmaxf(M, unordered((uint32_t)(c.best[((row0 + b) * S + i) * p.width] >> 32)));
-#pragma unroll
-                    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
                     again = true;
                 }
+                for (int o = lanes / 2; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
             }
         }
-        if (lane == 0) {
+        if (lane == 0 && here) {
             sum[b] = given;
             kind[b] = given == -INFINITY ? ABSENT : k;
             lse[b] = L > 0.0 ? (double)M * p.scale + log(L) : 0.0;
@@ -878,9 +890,12 @@ __device__ __forceinline__ void finish_search(const Select& p, const Scan& c, Fi
     if (__syncthreads_or(again)) sums_again();
     const double slack = NORM && p.beams > 1 ? (double)c.slack : 0.0;
     for (;;) {
-        // What the width-th is not below: of the first q of each list, which are at least
-        // twice the width, the width-th (of more than TH lists, of the largest of TH sets).
-        const int q = lists > TH ? 1 : max(1, min((2 * p.width + lists - 1) / lists, min(TH / lists, p.width)));
+        // What the width-th is not below: of the first q of each list, the width-th (of more
+        // than TH lists, of the largest of TH sets).  Few of them, four times the width, if
+        // that saves sorting them (see bound_of), else TH: one chain may hold all the best
+        // (12 x 32 x 14365, width 32: with twice the width 38 us, 24 so).
+        const int few = p.width <= 8 ? (4 * p.width + lists - 1) / lists : TH;
+        const int q = max(1, min(few, min(TH / lists, p.width)));
         if (tid == 0) s.count = 0, s.bound = ~0u;
         bool dropped = false;
         if (held) {
