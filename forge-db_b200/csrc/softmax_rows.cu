@@ -319,7 +319,7 @@ __device__ __forceinline__ unsigned pack_row(const PackSide& p, int row, int d, 
 // such row after the other has too little in flight (262144 x 96 f32: 85 us,
 // four at a time 43).  Rows that are not aligned are read an element at a time
 // (198627 x 25 f32: 81 us one row at a time, 37 so).
-template <typename T, int PARTS>
+template <typename T, int PARTS, bool WIDE>
 __device__ __forceinline__ unsigned pack_short(const PackSide& p, int row0, int d, int kp) {
     constexpr int V = 16 / (int)sizeof(T), R = 4;
     const int lane = threadIdx.x & 31, c = lane * V;
@@ -331,7 +331,7 @@ __device__ __forceinline__ unsigned pack_short(const PackSide& p, int row0, int 
         const bool use = row < p.n && (!p.seen || (p.seen[row >> 5] >> (row & 31) & 1u)) &&
                          (!p.lse || p.lse[row] != -INFINITY);
         const T* src = static_cast<const T*>(p.x) + (size_t)row * p.ld + c;
-        if (use && p.wide) {
+        if (use && WIDE) {
             if (c < d) raw[r] = __ldg(reinterpret_cast<const uint4*>(src));
         } else if (use) {
             T* e = reinterpret_cast<T*>(&raw[r]);
@@ -401,8 +401,9 @@ __global__ void __launch_bounds__(256)
     if (p.seen || p.lse || p.weight) wait_for_last();  // (others: beside the kernel before it)
     const int row = (((int)blockIdx.x - (first ? 0 : a.blocks)) * 8 + (threadIdx.x >> 5)) * p.rows;
     const unsigned mine = row >= p.n      ? 0u
-                          : p.rows == 4 ? pack_short<T, PARTS>(p, row, d, kp)
-                                        : pack_row<T, PARTS>(p, row, d, kp);
+                          : p.rows != 4 ? pack_row<T, PARTS>(p, row, d, kp)
+                          : p.wide      ? pack_short<T, PARTS, true>(p, row, d, kp)
+                                        : pack_short<T, PARTS, false>(p, row, d, kp);
     wait_for_last();
     if (!p.largest) return;
     // the block's largest, unless it is there already
