@@ -198,6 +198,114 @@ static void check_teacher_buffers(const A& a) {
     check_aligned(a.teacher_logits, 4, "teacher_logits");
 }
 
+// rows x parts runs of `bytes` bytes of a call's memory, `stride` and `part_stride` bytes
+// apart.
+struct Runs {
+    uintptr_t at;
+    size_t rows, stride, parts, part_stride, bytes;
+    Runs(const void* p, size_t rows_, size_t stride_, size_t parts_, size_t part_stride_,
+         size_t bytes_)
+        : at(reinterpret_cast<uintptr_t>(p)), rows(rows_), stride(rows_ > 1 ? stride_ : 0),
+          parts(parts_), part_stride(parts_ > 1 ? part_stride_ : 0), bytes(bytes_) {
+        // (no memory is as wide, and sums of such distances stay within 64 bits)
+        constexpr unsigned long long most = 1ull << 56;
+        FDB_REQUIRE(bytes < most && (rows <= 1 || stride <= most / (rows - 1)) &&
+                        (parts <= 1 || part_stride <= most / (parts - 1)) && at < most,
+                    FDB_ERR_INVALID_ARG, "a buffer is too large");
+    }
+    static Runs flat(const void* p, size_t bytes) { return Runs(p, 1, 0, 1, 0, bytes); }
+    size_t row_bytes() const { return (parts - 1) * part_stride + bytes; }
+    uintptr_t end() const { return at + (rows - 1) * stride + row_bytes(); }
+};
+// Whether sum t_k step_k is in [lo, hi] for some t_k in [0 or -count_k, count_k], steps
+// falling.  Few t_k are left at each step where the runs of one buffer lie apart; a pair that
+// needs more than `tries` of them is taken to meet.
+struct Walk {
+    long long step, least, most;  // of t
+};
+static bool reaches(const Walk* w, int n, long long lo, long long hi, int& tries) {
+    if (n == 0) return lo <= 0 && hi >= 0;
+    long long least = 0, most = 0;  // what the steps after this one can add
+    for (int k = 1; k < n; ++k) least += w[k].least * w[k].step, most += w[k].most * w[k].step;
+    auto floor_of = [&](long long v) { return v / w->step - (v % w->step < 0); };
+    const long long first = std::max(w->least, -floor_of(most - lo));
+    const long long last = std::min(w->most, floor_of(hi - least));
+    if (n == 1) return first <= last;
+    for (long long t = first; t <= last; ++t)
+        if (tries-- <= 0 || reaches(w + 1, n - 1, lo - t * w->step, hi - t * w->step, tries))
+            return true;
+    return false;
+}
+// Whether a byte is in both.
+static bool meet(const Runs& a, const Runs& b) {
+    if (a.end() <= b.at || b.end() <= a.at) return false;
+    // the distances from runs of b to runs of a, by their steps
+    Walk w[4];
+    int n = 0;
+    auto walk = [&](size_t step, size_t count, bool back) {
+        if (step == 0 || count <= 1) return;
+        int k = 0;
+        while (k < n && w[k].step != (long long)step) ++k;
+        if (k == n) w[n++] = Walk{(long long)step, 0, 0};
+        (back ? w[k].least : w[k].most) += back ? -(long long)(count - 1) : (long long)(count - 1);
+    };
+    walk(a.stride, a.rows, false);
+    walk(a.part_stride, a.parts, false);
+    walk(b.stride, b.rows, true);
+    walk(b.part_stride, b.parts, true);
+    std::sort(w, w + n, [](const Walk& x, const Walk& y) { return x.step > y.step; });
+    const long long from = (long long)a.at - (long long)b.at;
+    int tries = 1 << 16;
+    // (a run of a, `from` + the walk behind one of b, meets it in (-a.bytes, b.bytes))
+    return reaches(w, n, 1 - (long long)a.bytes - from, (long long)b.bytes - 1 - from, tries);
+}
+// What a call reads and writes.
+struct Buffers {
+    struct Buffer {
+        Runs runs;
+        bool written;
+    };
+    std::vector<Buffer> of;
+    void add(const Runs& r, bool written) {
+        if (r.at && r.bytes && r.rows && r.parts) of.push_back(Buffer{r, written});
+    }
+    // Whether one that is written meets another one.
+    bool meet() {
+        std::sort(of.begin(), of.end(),
+                  [](const Buffer& x, const Buffer& y) { return x.runs.at < y.runs.at; });
+        for (size_t i = 0, n; i < of.size(); i = n) {
+            uintptr_t end = of[i].runs.end();
+            for (n = i + 1; n < of.size() && of[n].runs.at < end; ++n)
+                end = std::max(end, of[n].runs.end());
+            if (n > i + 1 && !beside(i, n) && pairs_meet(i, n)) return true;
+        }
+        return false;
+    }
+
+private:
+    // Whether buffers [i, n) lie beside each other in rows of one distance: parts of one
+    // tensor's rows, of which there may be many.
+    bool beside(size_t i, size_t n) const {
+        const size_t stride = of[i].runs.stride;
+        std::vector<std::pair<size_t, size_t>> place;  // in a row, and its end
+        for (size_t k = i; k < n; ++k) {
+            const Runs& r = of[k].runs;
+            if (r.stride != stride || r.row_bytes() > stride) return false;
+            place.emplace_back(r.at % stride, r.at % stride + r.row_bytes());
+        }
+        std::sort(place.begin(), place.end());
+        for (size_t k = 1; k < place.size(); ++k)
+            if (place[k - 1].second > place[k].first) return false;
+        return place.back().second <= place[0].first + stride;
+    }
+    bool pairs_meet(size_t i, size_t n) const {
+        for (; i < n; ++i)
+            for (size_t j = i + 1; j < n && of[j].runs.at < of[i].runs.end(); ++j)
+                if ((of[i].written || of[j].written) && ::meet(of[i].runs, of[j].runs)) return true;
+        return false;
+    }
+};
+
 // A call without work has not timed out, whatever its workspace holds.
 template <class A>
 static void clear_status(int device, const A& a) {
@@ -1443,7 +1551,9 @@ int fdb_beam_reorder(fdb_ctx* ctx, const fdb_beam_state* states, size_t count,
         FDB_REQUIRE(o.groups == 0 || count == 0 || o.parents, FDB_ERR_INVALID_ARG,
                     "parents is NULL");
         check_aligned(o.parents, 8, "parents");
-        std::vector<std::pair<uintptr_t, size_t>> read, written;
+        Buffers all;
+        all.of.reserve(2 * count + 1);
+        all.add(Runs::flat(o.parents, o.groups * o.width * 8), false);
         for (size_t i = 0; i < count; ++i) {
             const fdb_beam_state& t = states[i];
             if (t.bytes == 0 || t.parts == 0) continue;
@@ -1467,21 +1577,15 @@ int fdb_beam_reorder(fdb_ctx* ctx, const fdb_beam_state* states, size_t count,
                              (t.parts == 1 || t.src_part_stride == t.dst_part_stride)),
                         FDB_ERR_INVALID_ARG,
                         "in place needs a width of beams and the same strides");
-            read.emplace_back(reinterpret_cast<uintptr_t>(t.src), i);
-            written.emplace_back(reinterpret_cast<uintptr_t>(t.dst), i);
+            if (t.src != t.dst)
+                all.add(Runs(t.src, o.groups * o.beams, t.src_stride, t.parts, t.src_part_stride,
+                             t.bytes),
+                        false);
+            all.add(Runs(t.dst, rows, t.dst_stride, t.parts, t.dst_part_stride, t.bytes), true);
         }
-        // a state that is written twice, or read by one and written by another
-        std::sort(read.begin(), read.end());
-        std::sort(written.begin(), written.end());
-        for (size_t i = 0; i < written.size(); ++i) {
-            FDB_REQUIRE(i == 0 || written[i - 1].first != written[i].first, FDB_ERR_INVALID_ARG,
-                        "a state is written twice");
-            for (auto r = std::lower_bound(read.begin(), read.end(),
-                                           std::make_pair(written[i].first, (size_t)0));
-                 r != read.end() && r->first == written[i].first; ++r)
-                FDB_REQUIRE(r->second == written[i].second, FDB_ERR_INVALID_ARG,
-                            "a state that one reads is written by another");
-        }
+        // (a state that is written twice, or read and written, but for one in place)
+        FDB_REQUIRE(!all.meet(), FDB_ERR_INVALID_ARG,
+                    "a state that is written is a part of another one or of parents");
         if (o.groups == 0 || count == 0) return;
         DeviceGuard g(ctx->c.device);
         beam::reorder_run(ctx->c, states, count, o);

@@ -689,8 +689,9 @@ int fdb_beam_select(fdb_ctx* ctx, const fdb_beam_args* args);
  * positions in use move); rows are src_stride and dst_stride bytes apart.  What
  * lies between the runs is left as it was, as is a row whose parent is outside
  * [0, beams), unless `clear` is not 0: it is then zeroed (not in place).  dst may
- * be src (same strides, width = beams): in place.  No other overlap.  Needs no
- * workspace. */
+ * be src (same strides, width = beams): in place.  A written state that shares a byte
+ * with another one, with one that is read or with parents is refused; states that
+ * only lie within one another's gaps are not.  Needs no workspace. */
 typedef struct fdb_beam_state {
     const void* src;
     void* dst;
