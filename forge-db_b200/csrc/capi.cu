@@ -1522,10 +1522,6 @@ int fdb_beam_select(fdb_ctx* ctx, const fdb_beam_args* args) {
         FDB_REQUIRE(a.scores && a.beam_scores, FDB_ERR_INVALID_ARG, "NULL argument");
         FDB_REQUIRE(a.out_scores && a.out_parents && a.out_ids, FDB_ERR_INVALID_ARG,
                     "out_scores, out_parents or out_ids is NULL");
-        // (a search's chains are read while others' results are written)
-        FDB_REQUIRE(a.out_scores != a.beam_scores && (!a.ended || a.out_ended != a.ended) &&
-                        (!a.ids || a.out_ids != a.ids) && a.out_ids != a.out_parents,
-                    FDB_ERR_INVALID_ARG, "an output is an input or another output");
         check_aligned(a.scores, a.dtype == FDB_DTYPE_F32 ? 4 : 2, "scores");
         check_aligned(a.ids, 8, "ids");
         check_aligned(a.allowed, 4, "allowed");
@@ -1533,7 +1529,34 @@ int fdb_beam_select(fdb_ctx* ctx, const fdb_beam_args* args) {
         check_aligned(a.out_scores, 4, "out_scores");
         check_aligned(a.out_parents, 8, "out_parents");
         check_aligned(a.out_ids, 8, "out_ids");
-        check_workspace(a, beam::select_bytes(ctx->c, a));
+        const size_t need = beam::select_bytes(ctx->c, a);
+        check_workspace(a, need);
+        // (a search's chains are read while others' results are written)
+        const size_t es = a.dtype == FDB_DTYPE_F32 ? 4 : 2, chains = a.groups * a.beams;
+        const size_t outs = a.groups * a.width;
+        Buffers all;
+        all.of.reserve(10);
+        all.add(Runs(a.scores, a.groups, a.ld_group * es, a.beams, a.ld_beam * es, a.n * es), false);
+        all.add(Runs::flat(a.beam_scores, chains * 4), false);
+        all.add(Runs::flat(a.ended, chains), false);
+        all.add(Runs::flat(a.out_scores, outs * 4), true);
+        all.add(Runs::flat(a.out_parents, outs * 8), true);
+        all.add(Runs::flat(a.out_ids, outs * 8), true);
+        all.add(Runs::flat(a.out_ended, outs), true);
+        if (need) all.add(Runs::flat(a.workspace, need), true);
+        if (a.ids) {
+            FDB_REQUIRE(a.ld_ids < (1ull << 40), FDB_ERR_INVALID_ARG, "ld_ids is too large");
+            all.add(Runs(a.ids, chains, a.ld_ids * 8, 1, 0, a.n * 8), false);
+        }
+        if (a.allowed) {
+            FDB_REQUIRE(a.ld_allowed < (1ull << 40), FDB_ERR_INVALID_ARG, "ld_allowed is too large");
+            all.add(Runs(a.allowed, a.ld_allowed ? chains : 1, a.ld_allowed * 4, 1, 0,
+                         (a.n + 31) / 32 * 4),
+                    false);
+        }
+        FDB_REQUIRE(!all.meet(), FDB_ERR_INVALID_ARG,
+                    "an output is an input or another output, or shares a byte with one (or the "
+                    "workspace does)");
         DeviceGuard g(ctx->c.device);
         beam::select_run(ctx->c, a);
     });

@@ -656,8 +656,9 @@ int fdb_distill_backward(fdb_ctx* ctx, const fdb_distill_grad_args* args);
  * taken); the chain each continues, the id it adds, and whether it has ended
  * (nullable): its chain had, or the id is end_id.  Past the last candidate -inf,
  * -1, -1, 0.  A group with a NaN or +inf in a chain's score or in a score that may
- * count has NaN, -1, -1, 0.  Searches of 2048 columns in all at most need no
- * workspace (0 bytes). */
+ * count has NaN, -1, -1, 0.  An output, or the workspace, that shares a byte with
+ * another buffer of the call is refused.  Searches of 2048 columns in all at most
+ * need no workspace (0 bytes). */
 #define FDB_MAX_BEAMS 128 /* largest beams and width */
 typedef struct fdb_beam_args {
     int dtype; /* FDB_DTYPE_* of scores */
