@@ -294,6 +294,9 @@ __global__ void __launch_bounds__(TH) loss_kernel(const LossArgs p) {
     if (tid != 0) return;
     const double rest = lse == -INFINITY || rest_lse == -INFINITY ? -INFINITY : rest_lse - lse;
     if (p.t.rest && nm.any && nm.left > 0.0) loss[0] += nm.left * (log(nm.left) - rest);
+    // (a divergence: what lies below 0 is the scores' and the lse's rounding, which come
+    // from different sums; a NaN stays)
+    if (loss[0] < 0.0) loss[0] = 0.0;
     // (not finite: a query or a row that counts, or a named row with a weight of 0)
     if (!(lse == lse)) loss[0] = NAN;
     if (p.loss) p.loss[q] = (float)loss[0];

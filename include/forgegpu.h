@@ -563,7 +563,8 @@ int fdb_logprobs_status(fdb_ctx* ctx, const void* workspace, void* stream);
  *              loss = sum_e P_e (log P_e - log p_e) + R (log R - log r),
  *              r the student's probability of all other rows together, R of none
  *              if the query sees no other row.  teacher_scale must be 1.
- * Both are at least 0, and 0 where the student is what the teacher says.
+ * Both are at least 0, and within rounding of 0 where the student is what the
+ * teacher says (a log p may lie a rounding above 0).
  *
  * Outputs, each nullable: loss[nq], lse[nq] (as fdb_logprobs'), logprobs[nq][k]
  * (log p of each entry, 0 where it takes no part), rest_logprob[nq] (log r, -inf
