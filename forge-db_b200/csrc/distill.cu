@@ -18,6 +18,7 @@ namespace fdb {
 namespace distill {
 
 using sr::Carve;
+using sr::Exact;
 using sr::LN2;
 using sr::LOG2E;
 using sr::to_f32;
@@ -139,58 +140,60 @@ struct LossArgs {
     float scale;
     float *loss, *lse, *logprobs, *rest;
 };
-// Two sums of a vector's products with a query's: of the even and of the odd columns.
+// Adds a vector's products with a query's to two sums, of the even and of the odd columns.
 template <typename T, typename VT>
-__device__ __forceinline__ uint64_t dot_vec(const VT& v, const float* q, uint64_t sums) {
+__device__ __forceinline__ void dot_vec(const VT& v, const typename Exact<T>::Q* q,
+                                        Exact<T> (&sums)[2]) {
     constexpr int V = sizeof(VT) / sizeof(T);
+    typedef typename Exact<T>::Q Q;
     const T* e = reinterpret_cast<const T*>(&v);
-    if constexpr (V == 1) {
-        sums = sr::packf(__fmaf_rn(to_f32<T>(e[0]), *q, sr::lo_of(sums)), 0.0f);
-    } else if constexpr (V == 2) {
-        const float2 y = *reinterpret_cast<const float2*>(q);
-        sums = tc::fma2(sr::packf(to_f32<T>(e[0]), to_f32<T>(e[1])), sr::packf(y.x, y.y), sums);
-    } else {
+    Q y[V];
+    // (16 bytes of the query at a time)
+    constexpr int AT_ONCE = 16 / sizeof(Q) < V ? 16 / sizeof(Q) : V;
 #pragma unroll
-        for (int i = 0; i < V; i += 4) {
-            const float4 y = *reinterpret_cast<const float4*>(q + i);
-            sums = tc::fma2(sr::packf(to_f32<T>(e[i]), to_f32<T>(e[i + 1])), sr::packf(y.x, y.y), sums);
-            sums = tc::fma2(sr::packf(to_f32<T>(e[i + 2]), to_f32<T>(e[i + 3])), sr::packf(y.z, y.w), sums);
-        }
+    for (int i = 0; i < V; i += AT_ONCE) {
+        struct alignas(AT_ONCE * sizeof(Q)) Piece {
+            Q y[AT_ONCE];
+        };
+        *reinterpret_cast<Piece*>(y + i) = *reinterpret_cast<const Piece*>(q + i);
     }
-    return sums;
+#pragma unroll
+    for (int i = 0; i < V; ++i) sums[i & 1].add(to_f32<T>(e[i]), y[i]);
 }
-// Adds a lane's share of the products of ROWS rows with a query, by vectors of VT: f32
-// sums of up to four of them, theirs in 64 bits.
+// A lane's share of the products of ROWS rows with a query, by vectors of VT, in 64 bits: a
+// sum in f32 is off by 2^-24 of its terms, which is much of a score that large terms leave of
+// one another, and of the differences between named rows.  (f32 sums of four vectors: a call
+// of 1000 lists of 64 rows of 768 bf16 86 us, so 90; 500 of 128 rows of 768 f32 51, so 61.)
+// Two steps at a time for 16-byte vectors of 16-bit types (the first of those calls: 92 us
+// with one), one for f32 (the second one: 74 us with two).
 template <typename T, typename VT, int ROWS>
-__device__ __forceinline__ void dot_rows(const T* const (&x)[ROWS], const float* q, int d, int sub,
-                                         int lanes, double (&acc)[ROWS]) {
-    constexpr int V = sizeof(VT) / sizeof(T), STEPS = 4, AHEAD = sizeof(VT) == 16 ? 2 : 4;
+__device__ __forceinline__ void dot_rows(const T* const (&x)[ROWS], const typename Exact<T>::Q* q,
+                                         int d, int sub, int lanes, double (&acc)[ROWS]) {
+    constexpr int V = sizeof(VT) / sizeof(T), AHEAD = sizeof(T) == 4 ? 1 : V == 8 ? 2 : 4;
+    Exact<T> sums[ROWS][2];
     int c = sub * V;
-    while (c + V <= d) {
-        uint64_t two[ROWS] = {};
 #pragma unroll AHEAD
-        for (int n = 0; n < STEPS && c + V <= d; ++n, c += lanes * V) {
-            VT v[ROWS];
+    for (; c + V <= d; c += lanes * V) {
+        VT v[ROWS];
 #pragma unroll
-            for (int r = 0; r < ROWS; ++r) v[r] = __ldg(reinterpret_cast<const VT*>(x[r] + c));
+        for (int r = 0; r < ROWS; ++r) v[r] = __ldg(reinterpret_cast<const VT*>(x[r] + c));
 #pragma unroll
-            for (int r = 0; r < ROWS; ++r) two[r] = dot_vec<T, VT>(v[r], q + c, two[r]);
-        }
-#pragma unroll
-        for (int r = 0; r < ROWS; ++r) acc[r] += (double)(sr::lo_of(two[r]) + sr::hi_of(two[r]));
+        for (int r = 0; r < ROWS; ++r) dot_vec<T, VT>(v[r], q + c, sums[r]);
     }
     // (the row's last, partial vector: one lane's)
     for (; c < d; ++c)
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) acc[r] += (double)(to_f32<T>(x[r][c]) * q[c]);
+        for (int r = 0; r < ROWS; ++r) sums[r][0].add(to_f32<T>(x[r][c]), q[c]);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) acc[r] = sums[r][0].sum() + sums[r][1].sum();
 }
 // One block per query: the pass's sums joined, the named rows scored, the loss.  Gathers k
 // rows a query, by vectors of what all rows are aligned to (a call of 2878 lists of 16 rows
-// of 518 f16, aligned to 4 bytes: 62.1 us an element at a time, 59.7 by pairs).
+// of 518 f16, aligned to 4 bytes: 65.5 us an element at a time, 64.9 by pairs).
 template <typename T, int TH>
 __global__ void __launch_bounds__(TH) loss_kernel(const LossArgs p) {
     extern __shared__ float4 q_raw[];
-    float* qs = reinterpret_cast<float*>(q_raw);  // [dim]
+    typename Exact<T>::Q* qs = reinterpret_cast<typename Exact<T>::Q*>(q_raw);  // [dim]
     __shared__ int raw[MAXK], row[MAXK], list[MAXK];
     __shared__ double score[MAXK], sums[TH / 32][3], sums2[TH / 32];
     __shared__ float maxima[TH / 32][3];
@@ -215,10 +218,8 @@ __global__ void __launch_bounds__(TH) loss_kernel(const LossArgs p) {
         const T* x[ROWS];
         double acc[ROWS];
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) {
+        for (int r = 0; r < ROWS; ++r)
             x[r] = xp + (size_t)row[list[min(i + r * per, named - 1)]] * p.ldx;
-            acc[r] = 0.0;
-        }
         if ((odd & 15) == 0) dot_rows<T, uint4>(x, qs, p.d, sub, lanes, acc);
         else if ((odd & 7) == 0) dot_rows<T, uint2>(x, qs, p.d, sub, lanes, acc);
         else if (sizeof(T) == 4 || (odd & 3) == 0) dot_rows<T, unsigned>(x, qs, p.d, sub, lanes, acc);
@@ -412,10 +413,11 @@ size_t forward_bytes(const Ctx& c, const fdb_distill_args& a) { return plan_forw
 
 template <typename T, int TH>
 static void launch_loss(cudaStream_t s, int device, const LossArgs& p) {
-    const size_t smem = up((size_t)p.d, 4) * 4;
+    typedef typename Exact<T>::Q Q;
+    const size_t smem = up((size_t)p.d * sizeof(Q), 16);
     if (smem > 32768) {  // (with the static part, over what needs no permission)
         static std::atomic<uint64_t> done{0};
-        sr::allow_smem(loss_kernel<T, TH>, device, FDB_MAX_SOFTMAX_DIM * 4, done);
+        sr::allow_smem(loss_kernel<T, TH>, device, FDB_MAX_SOFTMAX_DIM * sizeof(Q), done);
     }
     sr::launch(true, s, loss_kernel<T, TH>, p.parts.nq, TH, smem, p);
 }

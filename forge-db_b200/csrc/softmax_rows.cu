@@ -1660,23 +1660,6 @@ __device__ __forceinline__ double unordered64(uint64_t u) {
     return __longlong_as_double((long long)(u >> 63 ? u & 0x7fffffffffffffffull : ~u));
 }
 
-// Sums of q . x in 64 bits.  f32: products and sums in 64 bits (of a 64-bit copy
-// of q); 16-bit types: the products are exact in f32, the sums in 64 bits.
-template <typename T>
-struct Exact {
-    typedef float Q;
-    double s = 0.0;
-    __device__ __forceinline__ void add(float x, float q) { s += (double)__fmul_rn(x, q); }
-    __device__ __forceinline__ double sum() const { return s; }
-};
-template <>
-struct Exact<float> {
-    typedef double Q;
-    double s = 0.0;
-    __device__ __forceinline__ void add(float x, double q) { s = fma((double)x, q, s); }
-    __device__ __forceinline__ double sum() const { return s; }
-};
-
 // q . x of ROWS rows in 64 bits (see Exact) over `lanes` lanes (a power of two).
 // z: the largest element.
 template <int ROWS, typename T>

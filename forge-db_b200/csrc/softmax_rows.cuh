@@ -58,6 +58,23 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
     return __float2bfloat16_rn(v);
 }
 
+// Sums of q . x in 64 bits.  f32: products and sums in 64 bits (of a 64-bit copy
+// of q); 16-bit types: the products are exact in f32, the sums in 64 bits.
+template <typename T>
+struct Exact {
+    typedef float Q;
+    double s = 0.0;
+    __device__ __forceinline__ void add(float x, float q) { s += (double)__fmul_rn(x, q); }
+    __device__ __forceinline__ double sum() const { return s; }
+};
+template <>
+struct Exact<float> {
+    typedef double Q;
+    double s = 0.0;
+    __device__ __forceinline__ void add(float x, double q) { s = fma((double)x, q, s); }
+    __device__ __forceinline__ double sum() const { return s; }
+};
+
 // What a pass over the scores of queries [q0, q0 + nq) leaves: for part i and
 // query q the triple part[i * nq + q] of fdb_logprobs' sums, in units of
 // t = score * log2(e) as they were formed: f * rf for a score, with f = qf[q] (1 if
