@@ -94,3 +94,29 @@ def test_named_scores_are_sums_in_64_bits(dtype, nq, n, half, pad, shift, rest):
     lse = (p.lse - r.lse).double().abs().cpu().numpy()
     far = np.abs(lp[:, 3]) + 2 * np.abs(r.lse.double().cpu().numpy())
     assert (off <= lse + 2 * do.H32 * far).all()
+
+
+@pytest.mark.parametrize("dtype,nq,n,d", [("f16", 20, 262144, 1024), ("f16", 300, 100003, 512),
+                                          ("bf16", 20, 262144, 1024), ("f32", 20, 262144, 256)])
+def test_what_sums_lose_is_added_where_the_mass_lies(dtype, nq, n, d):
+    """One row scores 10, all others 0, by sums of integers that lose nothing.  What a tensor
+    core's sum of terms of one sign loses, 5.2e-8 a step of 16 columns (bf16 2.3e-8), is half
+    added to every score, so that each is off by at most that share of itself here, and the
+    lse by that share of their mean under the softmax, 0.8 or 1.8, however large the largest
+    is.  Exponentials and f32 sums have 2^-20 and the output its rounding, as everywhere."""
+    import forgegpu as fg
+    import torch
+    dt = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[dtype]
+    Q = torch.ones(nq, d, dtype=dt, device="cuda")
+    X = torch.ones(n, d, dtype=dt, device="cuda")
+    X[:, 1::2] = -1
+    X[n // 3] = 1
+    scale = float(np.float32(10 / d))
+    I = torch.full((nq, 1), 5, dtype=torch.int64, device="cuda")
+    r = fg.distill(Q, X, I, torch.zeros(nq, 1, device="cuda"), scale=scale)
+    top = scale * d
+    want = np.log(np.exp(top) + (n - 1))
+    mean = top * np.exp(top - want)
+    share = (2.3e-8 if dtype == "bf16" else 5.2e-8) / 2 * (d / 16)
+    off = (r.lse.double() - want).abs().max().item()
+    assert off <= share * mean + 2.0 ** -20 + do.H32 * want, off
