@@ -91,7 +91,9 @@ __device__ __forceinline__ double unordered64(uint64_t u) {
 // 64 x 8 x 131072 columns, width 8: f32 48 us (5.5 TB/s, where a copy has 6.4), bf16 30
 // (4.5 TB/s): a block's start and end, some 4 us without loads, and one exponential a
 // column (40 % of their unit's rate).  Looking for the best column by column, as they
-// come, took 74 us; a block for each search's last to end, with the finish, 46.
+// come, took 74 us; a block for each search's last to end, with the finish, 46.  With
+// filters or ids the columns pass through registers, one tile ahead, and each is tested:
+// the same chains with a filter each take 94 and 57 us.
 constexpr int TH = 256;               // threads
 constexpr int U = 4;                  // loads of a thread in a tile
 constexpr int SPAN = 2;               // tiles whose largest is kept together
@@ -1080,7 +1082,11 @@ static Plan plan(const Ctx& c, const fdb_beam_args& a) {
     const size_t vecs = a.n / per + 2;  // (at most)
     const size_t most = (vecs + TH * U - 1) / (TH * U);
     const size_t least = (most + SPANS * SPAN - 1) / (SPANS * SPAN);
-    // (and no more lists than a block of the finish holds in registers, if they would do)
+    // And no more lists than a block of the finish holds in registers, even where that leaves
+    // multiprocessors idle: of 1 to 4 searches of 4 to 64 chains of 131072 columns, widths 8 to
+    // 64, all but a few are slower with more parts, read by the finish's second form (1 x 32,
+    // width 32, f32: 26.5 us, 30.7 with parts for all; 1 x 8, width 8: 16.2, 21.6, and 20.1 with
+    // a block a multiprocessor), and those few within 2 us.
     const size_t lists = std::max<size_t>(1, TH * HELD / (a.beams * a.width));
     p.c.splits = (int)std::max(least, std::min({most, lists, std::max<size_t>(1, (size_t)c.sm_count * 4 / rows)}));
     Carve ws(a.workspace);
@@ -1160,7 +1166,9 @@ void select_run(const Ctx& ctx, const fdb_beam_args& a) {
 // All states of a call in one launch (STATES of them).  Out of place a warp moves 4 KB
 // of a run, eight loads a lane in flight, or, of runs that are shorter, several.  In
 // place a thread takes 16 bytes of every row of a search, all of them before it writes
-// any; rows that stay where they are are not touched.  Bound by memory.
+// any; rows that stay where they are are not touched.  Out of place bound by memory (6.6
+// TB/s).  In place by the loads in flight, fewer as a thread holds more rows: 512 rows of 512
+// KB in all moved at 5.5 TB/s by searches of 8 beams, 4.1 of 16, 2.5 of 32, 0.8 of 128.
 constexpr int STATES = 64;
 constexpr int PIECE = 8;                 // vectors of a lane
 struct State {

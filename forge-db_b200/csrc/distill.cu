@@ -115,8 +115,10 @@ __device__ __forceinline__ double above(const Teacher& t, float z, float zm) {
 // ---------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------
-// Filters without the named rows, a block per query.  Bound by memory: the words
-// are written once.
+// Filters without the named rows, a block per query.  Bound by the latency of the words
+// that a thread takes one after the other: 5 us for 1000 filters of 50001 rows, but of few
+// queries over many rows with filters of their own more than the pass itself (one query of
+// 1e7 rows: 1044 us where the pass takes 720; 22 without a filter).
 __global__ void __launch_bounds__(128)
     filter_kernel(const Teacher t, int q0, uint32_t* __restrict__ out, size_t words) {
     const int q = q0 + (int)blockIdx.x;
